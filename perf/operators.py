@@ -338,21 +338,25 @@ def run(state):
 
     s = state
     if op == "plan":
-        plan = lq.kv8_plan(s["context"], s["new"], s["table"], s["free"], s["taken"], page=s["case"]["page"],
-                           tokens=s["tokens"], max_tokens=s["most"])
+        # The plan's buffers are kept from step to step.
+        plan = s["plan"] = lq.kv8_plan(s["context"], s["new"], s["table"], s["free"], s["taken"], page=s["case"]["page"],
+                                       tokens=s["tokens"], max_tokens=s["most"], out=s.get("plan"))
         return {name: getattr(plan, name) for name in ("table", "lengths", "token_offsets", "page_offsets", "positions",
                                                        "slots", "taken")}
-    cache = lq.Kv8Cache(s["k_codes"], s["v_codes"], s["k_scale"], s["v_scale"])
+    if "cache" not in s:  # a layer's cache lives as long as the program
+        s["cache"] = lq.Kv8Cache(s["k_codes"], s["v_codes"], s["k_scale"], s["v_scale"])
+    cache = s["cache"]
     if op == "append":
         lq.kv8_append(s["k"], s["v"], cache, s["slots"], s["positions"], rope=s["rope"])
         # The cache as its readers see it.
         return {"k": cache.k * cache.k_scale[:, :, None, None], "k_scale": cache.k_scale,
                 "v": cache.v * cache.v_scale[:, :, None, None], "v_scale": cache.v_scale}
-    plan = lq.Kv8Plan(context=s["context"], lengths=s["lengths"], token_offsets=s["token_offsets"],
-                      page_offsets=s["page_offsets"], table=s["table"], tokens=s["tokens"], max_tokens=s["most"])
-    if "workspace" not in s:  # kept from step to step, as a serving loop keeps it
+    if "step" not in s:  # the step's plan, which all layers share, and the workspace, which all steps share
+        s["step"] = lq.Kv8Plan(context=s["context"], lengths=s["lengths"], token_offsets=s["token_offsets"],
+                               page_offsets=s["page_offsets"], table=s["table"], tokens=s["tokens"], max_tokens=s["most"])
         s["workspace"] = lq.Kv8Workspace(s["q"].device)
-    return lq.kv8_attention(s["q"], cache, plan, scale=s["case"]["dim"] ** -0.5, rope=s["rope"], workspace=s["workspace"])
+    return lq.kv8_attention(s["q"], cache, s["step"], scale=s["case"]["dim"] ** -0.5, rope=s["rope"],
+                            workspace=s["workspace"])
 
 
 # ------------------------------------------------- the definitions, 64 bits
