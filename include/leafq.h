@@ -412,6 +412,103 @@ int leafq_advance_position(void* stream, int32_t* position, int32_t count);
 /* positions[s] += count for every s < sequences, on the stream. */
 int leafq_advance_positions(void* stream, int32_t* positions, int sequences, int32_t count);
 
+/* ------------------------------------------------------------------------
+ * Paged INT8 KV cache: requests of different lengths share one pool of
+ * pages, keys and values are held as INT8 codes with one fp32 scale per
+ * page and kv head, and attention reads the codes.  A page holds `page`
+ * tokens (16, 32, 64 or 128) of every kv head; the head size `dim` is 32,
+ * 64, 96 or 128.  Pools and request lengths may be large: code offsets are
+ * 64-bit, a slot (page index * page + row) fits int32.
+ *
+ * One step of a batch: leafq_kv8_plan gives every request the pages its new
+ * tokens need and every new token its slot, then per layer leafq_kv8_append
+ * writes the new keys and values and leafq_kv8_attention attends.  All three
+ * read the lengths on the device, so one CUDA graph serves every step whose
+ * bounds (requests, tokens, max_tokens) are the same.  The reference keeps
+ * an fp32 cache per sequence instead (kv_cache.cpp); these results are not
+ * bit-identical to it. */
+typedef struct leafq_kv8_cache {
+    int8_t* k_codes;      /* [pages][kv_heads][page][dim], 16-byte aligned */
+    int8_t* v_codes;
+    float* k_scales;      /* [pages][kv_heads]; a value is code * scale */
+    float* v_scales;
+    int64_t pages;
+    int32_t page, kv_heads, dim;
+} leafq_kv8_cache;
+
+/* The arrays of one step; every pointer is device memory.  context is the
+ * step's input, the rest is written by leafq_kv8_plan. */
+typedef struct leafq_kv8_step {
+    const int32_t* context;       /* [requests] cached tokens before the step */
+    const int32_t* lengths;       /* [requests] cached tokens after it */
+    const int32_t* token_offsets; /* [requests + 1] first new token of each request */
+    const int32_t* page_offsets;  /* [requests + 1] prefix of the pages each request holds after it */
+    const int32_t* table;         /* [requests][max_pages] page of each run of `page` tokens */
+    int64_t max_pages;
+    int64_t tokens;               /* rows of q (at least token_offsets[requests]) */
+    int64_t max_tokens;           /* bound on any request's new tokens */
+    int32_t requests;
+} leafq_kv8_step;
+
+/* Block tables and slot map from request lengths.  Request s holds
+ * context[s] tokens and brings new_tokens[s] (0 or more).  It needs
+ * ceil((context + new) / page) - ceil(context / page) more pages, taken in
+ * request order from free_pages[*taken ...]; they are written to its row of
+ * table behind the pages it has.  Outputs: lengths, token_offsets,
+ * page_offsets (see leafq_kv8_step); positions and slots [tokens], the
+ * position and slot of each new token (requests in order, a request's tokens
+ * in order); *taken_after, the pages taken in all.  A request that does not
+ * fit its table row, or whose pages would reach past free_count (counting
+ * those of every earlier request that fits its row), is refused: it gets no
+ * pages, its tokens get slot -1 and lengths[s] = context[s].  Rows of
+ * positions / slots past the last new token get 0 / -1; more new tokens than
+ * `tokens`, or a negative length, is reported by leafq_device_status.
+ * Outputs other than table must not overlap the inputs. */
+int leafq_kv8_plan(void* stream, const int32_t* context, const int32_t* new_tokens, int requests, int32_t* table,
+                   int64_t max_pages, const int32_t* free_pages, int64_t free_count, const int32_t* taken, int page,
+                   int64_t tokens, int32_t* lengths, int32_t* token_offsets, int32_t* page_offsets,
+                   int32_t* positions, int32_t* slots, int32_t* taken_after, uint32_t flags);
+
+/* Writes the rows of k and v [tokens][kv_heads * dim] (rows k_stride /
+ * v_stride floats apart, so they may be columns of a q|k|v matrix) to their
+ * slots; slot -1 skips the row.  With cos_table / sin_table (leafq_rope_tables,
+ * [table_rows][rotary_dim / 2]; rotary_dim a multiple of 8) the keys are
+ * rotated by their positions first, as leafq_rotary_append rotates them.
+ * Per page and kv head, with the new rows behind `first` older ones:
+ *   need  = max(absmax(new rows) / 127, 1e-12)
+ *   scale = first > 0 ? max(old scale, need) : need
+ *   older codes become rint(code * (old scale / scale)) when the scale grew
+ *   new codes = rint(x * (1 / scale))
+ * (a NaN row makes the scale NaN).  The tokens of one page must be
+ * consecutive rows with consecutive slots, as leafq_kv8_plan lays them out.
+ * A slot outside the pool or a position outside the tables is skipped and
+ * reported by leafq_device_status.  positions may be NULL without tables. */
+int leafq_kv8_append(void* stream, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                     int64_t tokens, const int32_t* positions, const int32_t* slots, int rotary_dim,
+                     const float* cos_table, const float* sin_table, int64_t table_rows,
+                     const leafq_kv8_cache* cache, uint32_t flags);
+
+/* Bytes of workspace leafq_kv8_attention needs for this geometry, 0 when it
+ * needs none.  The workspace must be zeroed once before its first use; every
+ * call leaves the words that need it zero again.  Calls that overlap on the
+ * GPU need workspaces of their own. */
+size_t leafq_kv8_attention_workspace_bytes(int64_t max_tokens, int heads, int kv_heads, int dim);
+
+/* Causal grouped-query attention of the step's new tokens over the cache.
+ * q [tokens][heads * dim] (rows q_stride floats apart) is rotated by position
+ * when tables are given; the query of new token t of request s is at position
+ * context[s] + t and sees the keys j < min(position + 1, lengths[s]):
+ *   out = sum_j softmax_j(scale * q . key_j) value_j,
+ * fp32 throughout (sums, softmax statistics, output), a row that sees no key
+ * gives zeros.  heads is a multiple of the cache's kv_heads; out [tokens]
+ * [heads * dim]; rows past the last new token are not written.  A table entry
+ * outside the pool or a position outside the tables hides the key or empties
+ * the row, and leafq_device_status reports it. */
+int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int heads, int rotary_dim,
+                        const float* cos_table, const float* sin_table, int64_t table_rows,
+                        const leafq_kv8_cache* cache, const leafq_kv8_step* step, float scale, float* out,
+                        void* workspace, size_t workspace_bytes, uint32_t flags);
+
 #ifdef __cplusplus
 }
 #endif

@@ -85,6 +85,12 @@ _SIGNATURES = {
     "leafq_expf": ([_vp, _vp, _i64, _vp], _int),
     "leafq_advance_position": ([_vp, _vp, ctypes.c_int32], _int),
     "leafq_advance_positions": ([_vp, _vp, _int, ctypes.c_int32], _int),
+    "leafq_kv8_plan": ([_vp, _vp, _vp, _int, _vp, _i64, _vp, _i64, _vp, _int, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                        _u32], _int),
+    "leafq_kv8_append": ([_vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _int, _vp, _vp, _i64, _vp, _u32], _int),
+    "leafq_kv8_attention_workspace_bytes": ([_i64, _int, _int, _int], _size),
+    "leafq_kv8_attention": ([_vp, _vp, _i64, _int, _int, _vp, _vp, _i64, _vp, _vp, _f32, _vp, _vp, _size, _u32],
+                            _int),
 }
 
 
@@ -116,6 +122,20 @@ class ModelDesc(ctypes.Structure):
         (name, _vp) for name in ("embed", "embed_scales", "final_norm", "lm_head", "lm_head_scales",
                                  "cos_table", "sin_table", "layer", "ids", "position", "history",
                                  "logits")]
+
+
+class Kv8CacheDesc(ctypes.Structure):
+    """leafq_kv8_cache (include/leafq.h)."""
+
+    _fields_ = [(name, _vp) for name in ("k_codes", "v_codes", "k_scales", "v_scales")] + [
+        ("pages", _i64), ("page", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("dim", ctypes.c_int32)]
+
+
+class Kv8StepDesc(ctypes.Structure):
+    """leafq_kv8_step (include/leafq.h)."""
+
+    _fields_ = [(name, _vp) for name in ("context", "lengths", "token_offsets", "page_offsets", "table")] + [
+        ("max_pages", _i64), ("tokens", _i64), ("max_tokens", _i64), ("requests", ctypes.c_int32)]
 
 
 _lib = None

@@ -157,6 +157,11 @@ int leafq_device_status(void) {
                   "); the kernel skipped it");
         return LEAFQ_ERR_INVALID;
     }
+    if ((word >> 16) == kSiteKv8Range) {
+        set_error("a paged-cache length, slot, page or position was out of range (block " +
+                  std::to_string(word & 0xffffu) + "); the kernel skipped it");
+        return LEAFQ_ERR_INVALID;
+    }
     set_error("a device wait timed out (site " + std::to_string(word >> 16) + ", block " +
               std::to_string(word & 0xffffu) + ")");
     return LEAFQ_ERR_TIMEOUT;

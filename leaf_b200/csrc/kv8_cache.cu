@@ -1,0 +1,463 @@
+// Paged INT8 KV cache: the step plan and the append (include/leafq.h).
+//
+//   kv8_plan_kernel    block tables and slot map from request lengths
+//   kv8_append_kernel  RoPE on the keys, quantisation of keys and values into
+//                      their pages, the pages' scales grown where they must
+#include <climits>
+
+#include "leafq_device.cuh"
+#include "leafq_internal.h"
+
+namespace leafq {
+namespace {
+
+// ------------------------------------------------------------------- plan
+// Two prefix sums over the requests (new tokens, new pages) decide everything:
+// a request's first row, the free pages it takes, whether the pool reaches.
+// Every block scans all requests itself, a chunk of blockDim.x at a time with
+// a running carry (8 bytes per request from L2), so that no block waits for
+// another; block 0 writes the per-request outputs and the blocks share the
+// chunk's tokens.  Four consecutive tokens per thread: one search of the
+// chunk's prefix, one page lookup per page, 16-byte stores.  A new page's
+// table entry is written by the thread that has the page's first token.
+struct PlanArgs {
+    const int32_t* context;
+    const int32_t* fresh;
+    int32_t* table;
+    const int32_t* free_pages;
+    const int32_t* taken;
+    int32_t* lengths;
+    int32_t* token_offsets;
+    int32_t* page_offsets;
+    int32_t* positions;
+    int32_t* slots;
+    int32_t* taken_after;
+    int64_t max_pages, free_count, tokens;
+    int requests, shift;  // page = 1 << shift
+};
+
+constexpr int kPlanMaxThreads = 1024;
+
+// Inclusive scan over the block of two values at once; total of the block in
+// the last argument pair.  Every thread calls it.
+__device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t& total_a, int64_t& total_b,
+                                            int64_t (*part)[2]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int64_t oa = __shfl_up_sync(~0u, a, d), ob = __shfl_up_sync(~0u, b, d);
+        if (lane >= d) {
+            a += oa;
+            b += ob;
+        }
+    }
+    __syncthreads();  // the previous scan's parts have been read
+    if (lane == 31) {
+        part[warp][0] = a;
+        part[warp][1] = b;
+    }
+    __syncthreads();
+    int64_t before_a = 0, before_b = 0;
+    total_a = total_b = 0;
+    for (int w = 0; w < warps; ++w) {
+        const int64_t pa = part[w][0], pb = part[w][1];
+        if (w < warp) {
+            before_a += pa;
+            before_b += pb;
+        }
+        total_a += pa;
+        total_b += pb;
+    }
+    a += before_a;
+    b += before_b;
+}
+
+__global__ void __launch_bounds__(kPlanMaxThreads) kv8_plan_kernel(const PlanArgs g) {
+    __shared__ int64_t part[32][2];
+    __shared__ int64_t first_s[kPlanMaxThreads + 1];  // first token of each request of the chunk
+    __shared__ int64_t source_s[kPlanMaxThreads];     // free_pages index of table column 0 (if it were new); LLONG_MIN: refused
+    __shared__ int32_t context_s[kPlanMaxThreads];
+    __shared__ long long reached_s;                   // pages granted so far
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int tid = threadIdx.x, threads = blockDim.x;
+    const int64_t page = int64_t{1} << g.shift;
+    const int64_t taken = *g.taken;
+    const bool writer = blockIdx.x == 0;
+    if (tid == 0) reached_s = 0;
+    int64_t token_base = 0, need_base = 0, page_base = 0;
+    for (int base = 0; base < g.requests; base += threads) {
+        const int r = base + tid;
+        const bool live = r < g.requests;
+        int64_t c = live ? g.context[r] : 0, n = live ? g.fresh[r] : 0;
+        if (c < 0 || n < 0) {
+            if (writer) record_device_error(kSiteKv8Range);
+            c = max64(c, 0);
+            n = 0;
+        }
+        const int64_t before = (c + page - 1) >> g.shift, after = (c + n + page - 1) >> g.shift;
+        const bool fits = after <= g.max_pages;
+        const int64_t need = fits ? after - before : 0;
+        int64_t tn = n, tp = need, chunk_tokens, chunk_pages;
+        block_scan2(tn, tp, chunk_tokens, chunk_pages, part);
+        const int64_t upto = need_base + tp;  // pages wanted by requests 0 .. r
+        const bool granted = fits && (need == 0 || (taken >= 0 && taken + upto <= g.free_count));
+        const int64_t length = granted ? c + n : c;
+        first_s[tid] = token_base + tn - n;
+        if (tid == threads - 1) first_s[threads] = token_base + tn;
+        source_s[tid] = granted ? taken + upto - need - before : LLONG_MIN;
+        context_s[tid] = static_cast<int32_t>(c);
+        if (writer) {
+            // Pages held are bounded by the table's row (a context past it is the caller's error).
+            int64_t held = live ? min64((length + page - 1) >> g.shift, g.max_pages) : 0, none = 0, chunk_held, unused;
+            block_scan2(held, none, chunk_held, unused, part);
+            if (live) {
+                g.lengths[r] = static_cast<int32_t>(length);
+                g.token_offsets[r + 1] = static_cast<int32_t>(min64(token_base + tn, g.tokens));
+                g.page_offsets[r + 1] = static_cast<int32_t>(min64(page_base + held, INT_MAX));
+                if (granted && need > 0) atomicMax(&reached_s, static_cast<long long>(upto));
+            }
+            page_base += chunk_held;
+        }
+        __syncthreads();
+        // Tokens [t0, t1) of the chunk, in aligned groups of four.
+        const int64_t t0 = token_base, t1 = min64(token_base + chunk_tokens, g.tokens);
+        const int count = min(threads, g.requests - base);
+        for (int64_t u = t0 / 4 + (int64_t)blockIdx.x * threads + tid; u * 4 < t1; u += (int64_t)gridDim.x * threads) {
+            const int64_t begin = max64(u * 4, t0), end = min64(u * 4 + 4, t1);
+            int lo = 0, hi = count - 1;  // the last request whose first token is at most begin
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (first_s[mid] <= begin) lo = mid;
+                else hi = mid - 1;
+            }
+            int32_t pos4[4], slot4[4];
+            int64_t known = -1, id = -1;  // the last page looked up
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t t = u * 4 + i;
+                pos4[i] = 0;
+                slot4[i] = -1;
+                if (t < begin || t >= end) continue;
+                while (lo + 1 < count && first_s[lo + 1] <= t) {
+                    ++lo;
+                    known = -1;
+                }
+                const int64_t c_r = context_s[lo], p = c_r + (t - first_s[lo]), column = p >> g.shift;
+                pos4[i] = static_cast<int32_t>(p);
+                if (source_s[lo] == LLONG_MIN) continue;
+                if (column != known) {
+                    known = column;
+                    int32_t* entry = g.table + (int64_t)(base + lo) * g.max_pages + column;
+                    if (column >= (c_r + page - 1) >> g.shift) {
+                        id = g.free_pages[source_s[lo] + column];
+                        if ((p & (page - 1)) == 0) *entry = static_cast<int32_t>(id);
+                    } else {
+                        id = *entry;
+                    }
+                }
+                slot4[i] = static_cast<int32_t>(id * page + (p & (page - 1)));
+            }
+            if (begin == u * 4 && end == u * 4 + 4) {
+                *reinterpret_cast<int4*>(g.positions + u * 4) = make_int4(pos4[0], pos4[1], pos4[2], pos4[3]);
+                *reinterpret_cast<int4*>(g.slots + u * 4) = make_int4(slot4[0], slot4[1], slot4[2], slot4[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (u * 4 + i >= begin && u * 4 + i < end) {
+                        g.positions[u * 4 + i] = pos4[i];
+                        g.slots[u * 4 + i] = slot4[i];
+                    }
+            }
+        }
+        token_base += chunk_tokens;
+        need_base += chunk_pages;
+        __syncthreads();  // the chunk's arrays are free
+    }
+    for (int64_t t = token_base + (int64_t)blockIdx.x * threads + tid; t < g.tokens; t += (int64_t)gridDim.x * threads) {
+        g.positions[t] = 0;
+        g.slots[t] = -1;
+    }
+    if (writer && tid == 0) {
+        g.token_offsets[0] = 0;
+        g.page_offsets[0] = 0;
+        *g.taken_after = static_cast<int32_t>(taken + reached_s);
+        if (token_base > g.tokens) record_device_error(kSiteKv8Range);
+    }
+}
+
+// ----------------------------------------------------------------- append
+// A run is the new rows of one page: consecutive rows with consecutive slots
+// inside the page.  A block owns the runs that start among its `span` rows,
+// for one kv head, of the keys (blockIdx.z 0) or the values (1).  One pass:
+// the run's rows (rotated) stay in registers between the absmax and the
+// codes, kAppendItems items of 8 values per thread, blockDim.x * kAppendItems
+// items = page * dim / 8.  An item is the two quarters of a rotation pair:
+// values a .. a+3 and b .. b+3 with b = a + rotary / 2 (behind the rotated
+// part, pairs of the remaining half).  The absmax is a maximum over bit
+// patterns, which is exact, order-free and lets a NaN through.
+constexpr int kAppendItems = 4;
+
+struct AppendArgs {
+    const float* rows[2];
+    int64_t stride[2];
+    int8_t* codes[2];
+    float* scales[2];
+    const int32_t* positions;
+    const int32_t* slots;
+    const float* cos_table;
+    const float* sin_table;
+    int64_t table_rows, tokens, pages;
+    int shift, kv_heads, dim, rotary, span;
+};
+
+__device__ __forceinline__ uint32_t pack_codes(float4 x, float multiplier) {
+    const float v[4] = {x.x, x.y, x.z, x.w};
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        int c = __float2int_rn(__fmul_rn(v[i], multiplier));
+        c = c > 127 ? 127 : (c < -127 ? -127 : c);
+        word |= (static_cast<uint32_t>(c) & 0xffu) << (8 * i);
+    }
+    return word;
+}
+
+__device__ __forceinline__ uint32_t largest_bits(uint32_t m, float4 x) {
+    m = max(m, __float_as_uint(x.x) & 0x7fffffffu);
+    m = max(m, __float_as_uint(x.y) & 0x7fffffffu);
+    m = max(m, __float_as_uint(x.z) & 0x7fffffffu);
+    return max(m, __float_as_uint(x.w) & 0x7fffffffu);
+}
+
+__global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs g) {
+    __shared__ uint32_t starts_s[4];   // rows of the span that start a run
+    __shared__ uint32_t follow_s[16];  // rows behind a start that belong to its run
+    __shared__ uint32_t largest_s[16];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    const int head = blockIdx.y, which = blockIdx.z;
+    const int page = 1 << g.shift;
+    const int64_t row0 = (int64_t)blockIdx.x * g.span;
+    const int64_t pool = g.pages << g.shift;
+    // span <= page <= blockDim.x: one row per thread.
+    bool start = false;
+    if (tid < g.span && row0 + tid < g.tokens) {
+        const int64_t slot = g.slots[row0 + tid];
+        if (slot >= 0 && slot < pool) {
+            start = (slot & (page - 1)) == 0 || row0 + tid == 0 || g.slots[row0 + tid - 1] != slot - 1;
+        } else if (slot != -1 && head == 0 && which == 0) {
+            record_device_error(kSiteKv8Range);
+        }
+    }
+    const uint32_t ballot = __ballot_sync(~0u, start);
+    if (lane == 0 && warp < 4) starts_s[warp] = ballot;
+    __syncthreads();
+    const int per_row = g.dim >> 3;
+    const bool rotate = which == 0 && g.rotary > 0;
+    const int half = rotate ? g.rotary >> 1 : 0;
+    for (int word = 0; word < 4 && word * 32 < g.span; ++word) {
+        for (uint32_t left = starts_s[word]; left != 0; left &= left - 1) {
+            const int64_t row = row0 + word * 32 + __ffs(left) - 1;
+            const int64_t slot = g.slots[row];
+            const int first = static_cast<int>(slot & (page - 1));
+            // Rows of the run: until the page ends or the slots stop following.
+            const bool follows = tid < page - first && row + tid < g.tokens && g.slots[row + tid] == slot + tid;
+            const uint32_t mask = __ballot_sync(~0u, follows);
+            if (lane == 0) follow_s[warp] = mask;
+            __syncthreads();
+            int n = 0;
+            for (int w = 0; w * 32 < page; ++w) {
+                const uint32_t gap = ~follow_s[w];
+                if (gap != 0) {
+                    n += __ffs(gap) - 1;
+                    break;
+                }
+                n += 32;
+            }
+            const int64_t tile = (slot >> g.shift) * g.kv_heads + head;
+            float* scale_at = g.scales[which] + tile;
+            const float before = *scale_at;
+            float4 a[kAppendItems], b[kAppendItems];
+            uint32_t largest = 0;
+#pragma unroll
+            for (int i = 0; i < kAppendItems; ++i) {
+                const int item = tid + i * blockDim.x, r = item / per_row, j = item - r * per_row;
+                a[i] = b[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (r >= n) continue;
+                const float* src = g.rows[which] + (row + r) * g.stride[which] + (int64_t)head * g.dim;
+                const bool turned = 4 * j < half;
+                const int at = turned ? 4 * j : 2 * half + 4 * (j - half / 4);
+                const int to = turned ? at + half : at + ((g.dim - 2 * half) >> 1);
+                a[i] = *reinterpret_cast<const float4*>(src + at);
+                b[i] = *reinterpret_cast<const float4*>(src + to);
+                if (turned) {
+                    int64_t pos = g.positions[row + r];
+                    if (pos < 0 || pos >= g.table_rows) {
+                        if (j == 0 && head == 0) record_device_error(kSiteKv8Range);
+                        pos = 0;
+                    }
+                    const float4 c = *reinterpret_cast<const float4*>(g.cos_table + pos * half + at);
+                    const float4 s = *reinterpret_cast<const float4*>(g.sin_table + pos * half + at);
+                    const float4 x = a[i], y = b[i];
+                    a[i].x = __fsub_rn(__fmul_rn(x.x, c.x), __fmul_rn(y.x, s.x));
+                    a[i].y = __fsub_rn(__fmul_rn(x.y, c.y), __fmul_rn(y.y, s.y));
+                    a[i].z = __fsub_rn(__fmul_rn(x.z, c.z), __fmul_rn(y.z, s.z));
+                    a[i].w = __fsub_rn(__fmul_rn(x.w, c.w), __fmul_rn(y.w, s.w));
+                    b[i].x = __fadd_rn(__fmul_rn(y.x, c.x), __fmul_rn(x.x, s.x));
+                    b[i].y = __fadd_rn(__fmul_rn(y.y, c.y), __fmul_rn(x.y, s.y));
+                    b[i].z = __fadd_rn(__fmul_rn(y.z, c.z), __fmul_rn(x.z, s.z));
+                    b[i].w = __fadd_rn(__fmul_rn(y.w, c.w), __fmul_rn(x.w, s.w));
+                }
+                largest = largest_bits(largest_bits(largest, a[i]), b[i]);
+            }
+            largest = __reduce_max_sync(~0u, largest);
+            if (lane == 0) largest_s[warp] = largest;
+            __syncthreads();  // also: every thread has read the old scale
+            for (int w = 0; w < warps; ++w) largest = max(largest, largest_s[w]);
+            float need = __fdiv_rn(__uint_as_float(largest), 127.0f);
+            if (need < 1e-12f) need = 1e-12f;  // keeps a NaN
+            const float scale = first > 0 && !(need > before) && !isnan(need) ? before : need;
+            int8_t* codes = g.codes[which] + ((tile << g.shift) * g.dim);
+            if (first > 0 && scale != before) {
+                // The page's older codes, rounded to the grown scale.
+                const float ratio = __fdiv_rn(before, scale);
+                for (int i = tid; i < first * g.dim / 4; i += blockDim.x) {
+                    uint32_t* at = reinterpret_cast<uint32_t*>(codes) + i;
+                    const uint32_t old = *at;
+                    *at = pack_codes(make_float4(static_cast<int8_t>(old), static_cast<int8_t>(old >> 8),
+                                                 static_cast<int8_t>(old >> 16), static_cast<int8_t>(old >> 24)),
+                                     ratio);
+                }
+            }
+            const float multiplier = __fdiv_rn(1.0f, scale);
+#pragma unroll
+            for (int i = 0; i < kAppendItems; ++i) {
+                const int item = tid + i * blockDim.x, r = item / per_row, j = item - r * per_row;
+                if (r >= n) continue;
+                const bool turned = 4 * j < half;
+                const int at = turned ? 4 * j : 2 * half + 4 * (j - half / 4);
+                const int to = turned ? at + half : at + ((g.dim - 2 * half) >> 1);
+                int8_t* dst = codes + (int64_t)(first + r) * g.dim;
+                *reinterpret_cast<uint32_t*>(dst + at) = pack_codes(a[i], multiplier);
+                *reinterpret_cast<uint32_t*>(dst + to) = pack_codes(b[i], multiplier);
+            }
+            if (tid == 0) *scale_at = scale;
+            __syncthreads();  // follow_s and largest_s are free
+        }
+    }
+}
+
+int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1; }
+
+}  // namespace
+
+bool kv8_cache_valid(const leafq_kv8_cache* c, const char* what) {
+    if (!c || !c->k_codes || !c->v_codes || !c->k_scales || !c->v_scales || c->pages <= 0 || c->kv_heads <= 0 ||
+        c->kv_heads > 65535 || page_shift(c->page) < 0 || c->pages > INT_MAX / c->page) {
+        set_error(std::string(what) + ": invalid cache (pages of 16, 32, 64 or 128 tokens, slots within int32)");
+        return false;
+    }
+    if (!aligned16(c->k_codes) || !aligned16(c->v_codes)) {
+        set_error(std::string(what) + ": cache codes must be 16-byte aligned");
+        return false;
+    }
+    return true;
+}
+
+bool kv8_rope_valid(int dim, int rotary_dim, const float* cos_table, const float* sin_table, int64_t table_rows,
+                    const char* what) {
+    if (!cos_table && !sin_table && rotary_dim == 0) return true;
+    if (!cos_table || !sin_table || rotary_dim <= 0 || rotary_dim > dim || rotary_dim % 8 != 0 || table_rows <= 0 ||
+        !aligned16(cos_table) || !aligned16(sin_table)) {
+        set_error(std::string(what) +
+                  ": rotation needs two 16-byte aligned tables and rotary_dim a multiple of 8 within the head");
+        return false;
+    }
+    return true;
+}
+
+}  // namespace leafq
+
+using namespace leafq;
+
+extern "C" {
+
+int leafq_kv8_plan(void* stream, const int32_t* context, const int32_t* new_tokens, int requests, int32_t* table,
+                   int64_t max_pages, const int32_t* free_pages, int64_t free_count, const int32_t* taken, int page,
+                   int64_t tokens, int32_t* lengths, int32_t* token_offsets, int32_t* page_offsets,
+                   int32_t* positions, int32_t* slots, int32_t* taken_after, uint32_t flags) {
+    clear_error();
+    const int shift = page_shift(page);
+    if (requests < 0 || max_pages < 0 || free_count < 0 || tokens < 0 || shift < 0) {
+        set_error("leafq_kv8_plan: negative size, or a page that is not 16, 32, 64 or 128 tokens");
+        return LEAFQ_ERR_INVALID;
+    }
+    if (max_pages > INT_MAX / page || tokens > INT_MAX || free_count > INT_MAX) {
+        set_error("leafq_kv8_plan: lengths, tokens and pages must fit int32");
+        return LEAFQ_ERR_INVALID;
+    }
+    if (!token_offsets || !page_offsets || !taken || !taken_after ||
+        (requests > 0 && (!context || !new_tokens || !lengths || (max_pages > 0 && !table))) ||
+        (tokens > 0 && (!positions || !slots)) || (free_count > 0 && !free_pages)) {
+        set_error("leafq_kv8_plan: null pointer");
+        return LEAFQ_ERR_INVALID;
+    }
+    if (!aligned16(positions) || !aligned16(slots)) {
+        set_error("leafq_kv8_plan: positions and slots must be 16-byte aligned");
+        return LEAFQ_ERR_INVALID;
+    }
+    PlanArgs g{context, new_tokens, table, free_pages, taken, lengths, token_offsets, page_offsets, positions, slots,
+               taken_after, max_pages, free_count, tokens, requests, shift};
+    // One block for a decode step; with many tokens one block per 4096 of them.
+    const int threads = requests <= 256 && tokens <= 1024 ? 256 : kPlanMaxThreads;
+    int64_t blocks = (tokens + 4 * threads - 1) / (4 * threads);
+    blocks = blocks < 1 ? 1 : blocks > sm_count() ? sm_count() : blocks;
+    return launch(kv8_plan_kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads), 0,
+                  static_cast<cudaStream_t>(stream), (flags & LEAFQ_FLAG_PDL) != 0, "leafq_kv8_plan", g);
+}
+
+int leafq_kv8_append(void* stream, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                     int64_t tokens, const int32_t* positions, const int32_t* slots, int rotary_dim,
+                     const float* cos_table, const float* sin_table, int64_t table_rows,
+                     const leafq_kv8_cache* cache, uint32_t flags) {
+    clear_error();
+    if (!kv8_cache_valid(cache, "leafq_kv8_append")) return LEAFQ_ERR_INVALID;
+    if (!kv8_dim_supported(cache->dim)) {
+        set_error("leafq_kv8_append: head sizes are 32, 64, 96 and 128");
+        return LEAFQ_ERR_UNSUPPORTED;
+    }
+    if (!kv8_rope_valid(cache->dim, rotary_dim, cos_table, sin_table, table_rows, "leafq_kv8_append"))
+        return LEAFQ_ERR_INVALID;
+    const int64_t width = (int64_t)cache->kv_heads * cache->dim;
+    if (tokens < 0 || tokens > INT_MAX) {
+        set_error("leafq_kv8_append: tokens must be between 0 and 2^31 - 1");
+        return LEAFQ_ERR_INVALID;
+    }
+    if (tokens == 0) return LEAFQ_OK;
+    if (!k || !v || !slots || (rotary_dim > 0 && !positions)) {
+        set_error("leafq_kv8_append: null pointer");
+        return LEAFQ_ERR_INVALID;
+    }
+    if ((tokens > 1 && (k_stride < width || v_stride < width)) || k_stride % 4 != 0 || v_stride % 4 != 0 ||
+        !aligned16(k) || !aligned16(v)) {
+        set_error("leafq_kv8_append: rows must be 16-byte aligned and must not overlap");
+        return LEAFQ_ERR_INVALID;
+    }
+    AppendArgs g{{k, v}, {k_stride, v_stride}, {cache->k_codes, cache->v_codes}, {cache->k_scales, cache->v_scales},
+                 positions, slots, cos_table, sin_table, table_rows, tokens, cache->pages, page_shift(cache->page),
+                 cache->kv_heads, cache->dim, rotary_dim, 1};
+    // 32 .. 512 threads in whole warps, at least the page.
+    const int threads = (cache->page * cache->dim / 8 / kAppendItems + 31) / 32 * 32;
+    // Few rows: one per block, so that a decode step's rows run side by side;
+    // many: a page's worth, so that most blocks have one whole run.
+    int span = 1;
+    while (span < cache->page && tokens / (2 * span) * cache->kv_heads * 2 >= 4 * (int64_t)sm_count()) span *= 2;
+    g.span = span;
+    return launch(kv8_append_kernel, dim3(static_cast<unsigned>((tokens + span - 1) / span), cache->kv_heads, 2),
+                  dim3(threads), 0, static_cast<cudaStream_t>(stream),
+                  (flags & LEAFQ_FLAG_PDL) != 0, "leafq_kv8_append", g);
+}
+
+}  // extern "C"

@@ -51,6 +51,7 @@ enum WaitSite : unsigned {
     kSiteDecodeCodes = 12,
     kSiteAllGather = 13,
     kSiteCacheRange = 14,  // not a wait: a position outside the KV cache
+    kSiteKv8Range = 15,    // not a wait: a paged-cache index or length out of range
 };
 
 __device__ __forceinline__ unsigned long long global_timer_ns() {

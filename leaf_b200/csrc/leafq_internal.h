@@ -138,4 +138,11 @@ int launch_gemm_i8_per_channel(cudaStream_t s, const int8_t* a, const int8_t* b,
                                const float* bias, float input_scale, const float* wscales,
                                float* out, int64_t m, int64_t k, int64_t n, int activation);
 
+// Paged INT8 KV cache: checks shared by its entry points (error text set on
+// failure) and the head sizes it is built for.
+bool kv8_cache_valid(const leafq_kv8_cache* cache, const char* what);
+bool kv8_rope_valid(int dim, int rotary_dim, const float* cos_table, const float* sin_table, int64_t table_rows,
+                    const char* what);
+inline bool kv8_dim_supported(int dim) { return dim == 32 || dim == 64 || dim == 96 || dim == 128; }
+
 }  // namespace leafq

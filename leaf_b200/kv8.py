@@ -1,0 +1,220 @@
+"""Paged INT8 KV cache: the operators of include/leafq.h's ``leafq_kv8_*``.
+
+A pool of pages holds the keys and values of many requests as INT8 codes with
+one scale per page and kv head.  One step of a batch is ``kv8_plan`` (pages and
+slots from the request lengths, on the device), then per layer ``kv8_append``
+(rotate, quantise, write) and ``kv8_attention``.  The reference keeps an fp32
+cache per sequence (kv_cache.cpp:21-59); this one holds a quarter of its bytes
+and lets requests of different lengths share memory, at the rounding of 8 bits.
+
+``Kv8Cache``, ``Kv8Plan`` and ``Kv8Workspace`` are handles a serving loop makes
+once and keeps; the calls only enqueue work on the current stream.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import LeafError, check, load
+
+PAGE_SIZES = (16, 32, 64, 128)
+HEAD_SIZES = (32, 64, 96, 128)
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _need(ok: bool, message: str) -> None:
+    if not ok:
+        raise LeafError(_lib.LEAFQ_ERR_INVALID, message)
+
+
+def _check_i32(t: torch.Tensor, name: str, numel: Optional[int] = None, device=None) -> None:
+    _need(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous(), f"{name} must be a contiguous int32 CUDA tensor")
+    _need(numel is None or t.numel() == numel, f"{name} must hold {numel} values")
+    _need(device is None or t.device == device, f"{name} is on another device")
+
+
+def _check_rows(t: torch.Tensor, name: str, width: int, device) -> None:
+    """fp32 [tokens, width] rows, contiguous in themselves (columns of a wider matrix are)."""
+    _need(t.is_cuda and t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == width,
+          f"{name} must be float32 [tokens, {width}] on a CUDA device")
+    _need(t.device == device, f"{name} is on another device")
+    _need(t.shape[0] == 0 or (t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= width)),
+          f"the rows of {name} must be contiguous and must not overlap")
+
+
+def _rope_args(rope, dim: int, device):
+    """(rotary_dim, cos, sin, rows) for the C call."""
+    if rope is None:
+        return 0, None, None, 0
+    cos, sin = rope
+    _need(cos.is_cuda and cos.dtype == torch.float32 and cos.dim() == 2 and cos.is_contiguous() and
+          sin.dtype == torch.float32 and sin.shape == cos.shape and sin.is_contiguous() and
+          cos.device == device and sin.device == device,
+          "rope tables must be two contiguous float32 [positions, rotary_dim / 2] CUDA tensors")
+    _need(2 * cos.shape[1] <= dim, "rope tables are wider than the head")
+    return 2 * cos.shape[1], cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+
+
+class Kv8Cache:
+    """One layer's pool: int8 ``k`` and ``v`` [pages, kv_heads, page, dim] and
+    float32 ``k_scale`` and ``v_scale`` [pages, kv_heads]."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        _need(k.dim() == 4 and k.shape == v.shape, "codes must be two [pages, kv_heads, page, dim] tensors")
+        self.pages, self.kv_heads, self.page, self.dim = k.shape
+        for t, name in ((k, "key codes"), (v, "value codes")):
+            _need(t.is_cuda and t.dtype == torch.int8 and t.is_contiguous(), f"{name} must be contiguous int8 CUDA tensors")
+        for t, name in ((k_scale, "key scales"), (v_scale, "value scales")):
+            _need(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and
+                  tuple(t.shape) == (self.pages, self.kv_heads), f"{name} must be contiguous float32 [pages, kv_heads]")
+        _need(all(t.device == k.device for t in (v, k_scale, v_scale)), "codes and scales must be on one device")
+        _need(self.page in PAGE_SIZES, f"pages hold {PAGE_SIZES} tokens")
+        _need(self.dim in HEAD_SIZES, f"head sizes are {HEAD_SIZES}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device = k.device
+        self.desc = _lib.Kv8CacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.pages,
+                                      self.page, self.kv_heads, self.dim)
+        self.ref = ctypes.byref(self.desc)
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page: int, dim: int, device="cuda") -> "Kv8Cache":
+        """An uninitialised pool (a page's contents count only once written)."""
+        codes = [torch.empty((pages, kv_heads, page, dim), dtype=torch.int8, device=device) for _ in range(2)]
+        scales = [torch.empty((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(*codes, *scales)
+
+
+class Kv8Plan:
+    """The arrays of one step: ``context`` and ``lengths`` [requests] (cached
+    tokens before and after), ``token_offsets`` and ``page_offsets``
+    [requests + 1], ``table`` [requests, max_pages], and, from ``kv8_plan``,
+    ``positions`` and ``slots`` [tokens] and ``taken``.  ``tokens`` and
+    ``max_tokens`` are the host's bounds: the rows of the step, and any one
+    request's new tokens."""
+
+    def __init__(self, context, lengths, token_offsets, page_offsets, table, tokens: int, max_tokens: int,
+                 positions=None, slots=None, taken=None):
+        _need(table.dim() == 2, "the block table must be [requests, max_pages]")
+        requests, device = table.shape[0], table.device
+        _check_i32(table, "the block table")
+        _check_i32(context, "context", requests, device)
+        _check_i32(lengths, "lengths", requests, device)
+        _check_i32(token_offsets, "token_offsets", requests + 1, device)
+        _check_i32(page_offsets, "page_offsets", requests + 1, device)
+        _need(tokens >= 0 and max_tokens >= 0, "token counts must not be negative")
+        self.context, self.lengths, self.table = context, lengths, table
+        self.token_offsets, self.page_offsets = token_offsets, page_offsets
+        self.positions, self.slots, self.taken = positions, slots, taken
+        self.requests, self.tokens, self.max_tokens, self.device = requests, int(tokens), int(max_tokens), device
+        self.desc = _lib.Kv8StepDesc(context.data_ptr(), lengths.data_ptr(), token_offsets.data_ptr(),
+                                     page_offsets.data_ptr(), table.data_ptr(), table.shape[1], self.tokens,
+                                     self.max_tokens, requests)
+        self.ref = ctypes.byref(self.desc)
+
+
+class Kv8Workspace:
+    """Device scratch of ``kv8_attention``, zeroed when it grows.  Reuse it
+    across calls on one stream."""
+
+    def __init__(self, device="cuda"):
+        self.device = torch.device(device)
+        self.buffer = torch.empty(0, dtype=torch.uint8, device=self.device)
+
+    def get(self, nbytes: int) -> torch.Tensor:
+        if nbytes > self.buffer.numel():
+            self.buffer = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
+        return self.buffer
+
+
+def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
+             taken: torch.Tensor, page: int, tokens: int, max_tokens: Optional[int] = None,
+             out: Optional[Kv8Plan] = None, flags: int = 0) -> Kv8Plan:
+    """Pages and slots of a step.  Request s holds context[s] tokens and brings
+    new_tokens[s]; the pages they need are taken from free_pages[taken:] in
+    request order and written into its row of ``table`` (in place).  A request
+    that does not fit its row or the free pages is refused: slots -1 and
+    lengths[s] == context[s].  tokens: the step's rows, at least the sum of
+    new_tokens (the rest get slot -1); max_tokens: a bound on any request's new
+    tokens (default: tokens).  ``taken`` is only read, the new count is the
+    plan's ``taken``.  ``out``: a plan of the same sizes whose buffers are
+    reused."""
+    requests = context.numel()
+    if out is not None and out.context is context and out.table is table and out.tokens == tokens and out.slots is not None:
+        plan = out
+    else:
+        device = context.device
+        _need(out is None, "the plan to reuse is of other buffers or sizes")
+        _check_i32(context, "context")
+        _need(table.dim() == 2 and table.shape[0] == requests, "the block table must be [requests, max_pages]")
+        sizes = (requests, requests + 1, requests + 1, 1, tokens, tokens)
+        room = [-(-n // 4) * 4 for n in sizes]  # 16-byte aligned pieces
+        pieces = torch.empty(sum(room), dtype=torch.int32, device=device).split(room)
+        lengths, token_offsets, page_offsets, after, positions, slots = (p[:n] for p, n in zip(pieces, sizes))
+        plan = Kv8Plan(context, lengths, token_offsets, page_offsets, table, tokens,
+                       tokens if max_tokens is None else max_tokens, positions, slots, after)
+    _check_i32(new_tokens, "new_tokens", requests, plan.device)
+    _check_i32(free_pages, "free_pages", None, plan.device)
+    _check_i32(taken, "taken", 1, plan.device)
+    check(load().leafq_kv8_plan(_stream(plan.device), context.data_ptr(), new_tokens.data_ptr(), requests,
+                                table.data_ptr(), table.shape[1], free_pages.data_ptr(), free_pages.numel(),
+                                taken.data_ptr(), page, tokens, plan.lengths.data_ptr(), plan.token_offsets.data_ptr(),
+                                plan.page_offsets.data_ptr(), plan.positions.data_ptr(), plan.slots.data_ptr(),
+                                plan.taken.data_ptr(), flags))
+    return plan
+
+
+def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: Kv8Cache, slots: torch.Tensor,
+               positions: Optional[torch.Tensor] = None, rope=None, flags: int = 0) -> None:
+    """Writes the rows of k and v (fp32 [tokens, kv_heads * dim]; columns of a
+    wider matrix will do) into the cache at their slots, -1 skipping a row.
+    With rope = (cos, sin) tables [positions, rotary_dim / 2] the keys are
+    rotated by ``positions`` first.  A page's scale grows when a new row needs
+    it, and its older codes are rounded to the new scale."""
+    width = cache.kv_heads * cache.dim
+    _check_rows(k, "k", width, cache.device)
+    _check_rows(v, "v", width, cache.device)
+    tokens = k.shape[0]
+    _need(v.shape[0] == tokens, "k and v must have the same rows")
+    _check_i32(slots, "slots", tokens, cache.device)
+    rotary, cos, sin, rows = _rope_args(rope, cache.dim, cache.device)
+    if rope is not None:
+        _need(positions is not None, "rotation needs positions")
+        _check_i32(positions, "positions", tokens, cache.device)
+    check(load().leafq_kv8_append(_stream(cache.device), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), tokens,
+                                  None if positions is None else positions.data_ptr(), slots.data_ptr(), rotary, cos,
+                                  sin, rows, cache.ref, flags))
+
+
+def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float, rope=None,
+                  out: Optional[torch.Tensor] = None, workspace: Optional[Kv8Workspace] = None,
+                  flags: int = 0) -> torch.Tensor:
+    """Causal grouped-query attention of the step's rows q (fp32
+    [tokens, heads * dim]; columns of a wider matrix will do) over the cache,
+    rotated by position when rope tables are given.  Returns fp32
+    [tokens, heads * dim]; a row that sees no key is zero, rows past the step's
+    last new token are not written."""
+    _need(q.dim() == 2 and q.shape[1] % cache.dim == 0, "q must be [tokens, heads * dim]")
+    _check_rows(q, "q", q.shape[1], cache.device)
+    tokens, heads = q.shape[0], q.shape[1] // cache.dim
+    _need(tokens == plan.tokens, "q has other rows than the plan")
+    _need(plan.device == cache.device, "the plan is on another device")
+    if out is None:
+        out = torch.empty((tokens, q.shape[1]), dtype=torch.float32, device=cache.device)
+    else:
+        _need(out.is_cuda and out.dtype == torch.float32 and out.is_contiguous() and out.shape == q.shape and
+              out.device == cache.device, "out must be contiguous float32 of q's shape")
+    rotary, cos, sin, rows = _rope_args(rope, cache.dim, cache.device)
+    lib = load()
+    need = lib.leafq_kv8_attention_workspace_bytes(plan.max_tokens, heads, cache.kv_heads, cache.dim)
+    pointer = None
+    if need:
+        pointer = (workspace or Kv8Workspace(cache.device)).get(need).data_ptr()
+    check(lib.leafq_kv8_attention(_stream(cache.device), q.data_ptr(), q.stride(0), heads, rotary, cos, sin, rows,
+                                  cache.ref, plan.ref, scale, out.data_ptr(), pointer, need, flags))
+    return out

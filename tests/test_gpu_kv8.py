@@ -1,0 +1,521 @@
+"""The paged INT8 cache's operators on the GPU against their definitions in
+64-bit floats (oracle/kv8.py).
+
+Tolerances, with u = 2^-24:
+* plan: whole numbers, equal.
+* append: a scale is a quotient of a rotated value (two products and a sum:
+  3 u of the pair's magnitude) by 127, so within 8 u of the exact one; a code
+  may differ by one where the exact quotient lies within 127 * 16 u of a half.
+* attention: rounding a score of reach R (scale * sum |q||k|) costs at most
+  (dim + 16) u R -- each product and each partial sum of the dot, the rotation,
+  the scale factors -- and enters the weights of numerator and denominator;
+  the exponentials, their sums and the value products add 64 u.  With values
+  up to V: |error| <= V * (2 (dim + 16) R + 64) u.  Errors are random, so the
+  2-norm of the whole output is held to 1e-5 of its own as well.
+"""
+import numpy as np
+import pytest
+import torch
+
+import leaf_b200 as lq
+from leaf_b200 import _lib
+from oracle import kv8 as ok
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _i32(a):
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
+
+
+def _status_ok():
+    return _lib.load().leafq_device_status() == 0
+
+
+def _rope(rows, rotary):
+    rate = 10000.0 ** (-np.arange(0, rotary, 2) / rotary)
+    angle = np.arange(rows)[:, None] * rate
+    return np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+
+
+def _rope_cuda(rope):
+    return None if rope is None else tuple(torch.from_numpy(t).cuda() for t in rope)
+
+
+# ------------------------------------------------------------------- plan
+def _check_plan(context, new, table, free, taken, page, tokens):
+    expect = ok.plan(context, new, table, free, taken, page, tokens)
+    t = _i32(table)
+    got = lq.kv8_plan(_i32(context), _i32(new), t, _i32(free), _i32([taken]), page, tokens)
+    torch.cuda.synchronize()
+    for name in ("lengths", "token_offsets", "page_offsets", "positions", "slots", "table"):
+        assert np.array_equal(getattr(got, name).cpu().numpy(), expect[name]), name
+    assert int(got.taken.item()) == expect["taken"]
+    return got
+
+
+def _plan_case(rng, requests, page, longest, most_new):
+    context = rng.integers(0, longest + 1, requests)
+    new = rng.integers(0, most_new + 1, requests)
+    new[rng.random(requests) < 0.2] = 0
+    context[rng.random(requests) < 0.2] = 0
+    held = [ok.pages_of(int(c), page) for c in context]
+    max_pages = max(ok.pages_of(int(c + n), page) for c, n in zip(context, new)) + 1
+    order = rng.permutation(sum(held) + int(sum(ok.pages_of(int(n), page) + 1 for n in new)))
+    table, at = np.full((requests, max_pages), -1), 0
+    for s, b in enumerate(held):
+        table[s, :b] = order[at:at + b]
+        at += b
+    return context, new, table, order, at
+
+
+@pytest.mark.parametrize("requests", [1, 3, 64, 255, 257, 1025, 2500])
+@pytest.mark.parametrize("page,longest,most_new", [(16, 40, 1), (16, 300, 70), (64, 500, 200), (128, 1000, 3)])
+def test_plan(cuda_device, requests, page, longest, most_new):
+    rng = np.random.default_rng(requests * 1000 + page + most_new)
+    context, new, table, order, taken = _plan_case(rng, requests, page, longest, most_new)
+    _check_plan(context, new, table, order, taken, page, int(new.sum()))
+    _check_plan(context, new, table, order, taken, page, int(new.sum()) + 13)  # rows beyond the last token
+    assert _status_ok()
+
+
+@pytest.mark.parametrize("requests", [5, 300, 1500])
+def test_plan_refuses_what_does_not_fit(cuda_device, requests):
+    rng = np.random.default_rng(requests)
+    context, new, table, order, taken = _plan_case(rng, requests, 16, 200, 90)
+    for cut in (0, 1, 7, order.size // 2):  # a pool that ends too early
+        _check_plan(context, new, table, order[:taken + cut], taken, 16, int(new.sum()))
+    narrow = table[:, :table.shape[1] * 2 // 3].copy()  # rows that end too early
+    fits = np.array([ok.pages_of(int(c), 16) <= narrow.shape[1] for c in context])
+    _check_plan(context * fits, new, narrow, order, taken, 16, int(new.sum()))
+    assert _status_ok()
+
+
+def test_plan_without_requests_or_tokens(cuda_device):
+    table = np.zeros((0, 4), dtype=np.int64)
+    _check_plan([], [], table, [3, 1], 0, 32, 0)
+    _check_plan([], [], table, [3, 1], 1, 32, 6)
+    _check_plan([0, 5, 32], [0, 0, 0], np.array([[-1, -1], [2, -1], [0, -1]]), [], 0, 32, 0)
+    assert _status_ok()
+
+
+def test_plan_reports_negative_lengths_and_too_few_rows(cuda_device):
+    got = lq.kv8_plan(_i32([4, -3]), _i32([2, 5]), _i32([[0, 1], [2, 3]]), _i32([4, 5]), _i32([0]), 16, 2)
+    torch.cuda.synchronize()
+    assert got.slots.tolist() == [4, 5] and got.lengths.tolist() == [6, 0]
+    assert _lib.load().leafq_device_status() == _lib.LEAFQ_ERR_INVALID
+    lq.kv8_plan(_i32([4, 3]), _i32([2, 5]), _i32([[0, 1], [2, 3]]), _i32([4, 5]), _i32([0]), 16, 3)
+    assert _lib.load().leafq_device_status() == _lib.LEAFQ_ERR_INVALID
+    assert _status_ok()
+
+
+def test_plan_steps_follow_one_another(cuda_device):
+    # Ten steps of unlike growth: every step's pages come from where the last stopped.
+    rng = np.random.default_rng(5)
+    requests, page = 40, 16
+    context = np.zeros(requests, dtype=np.int64)
+    table, taken = np.full((requests, 40), -1), 0
+    free = rng.permutation(requests * 40)
+    t, plan = _i32(table), None
+    length, count = _i32(context), _i32([0])
+    for step in range(10):
+        new = rng.integers(0, 40, requests)
+        expect = ok.plan(context, new, table, free, taken, page, 2000)
+        plan = lq.kv8_plan(length, _i32(new), t, _i32(free), count, page, 2000, out=plan)
+        torch.cuda.synchronize()
+        assert np.array_equal(t.cpu().numpy(), expect["table"]) and np.array_equal(plan.slots.cpu().numpy(), expect["slots"])
+        length.copy_(plan.lengths)
+        count.copy_(plan.taken)
+        context, table, taken = expect["lengths"], expect["table"], expect["taken"]
+        live = expect["slots"][expect["slots"] >= 0]
+        assert len(set(live.tolist())) == live.size
+
+
+# ----------------------------------------------------------------- append
+def _runs(rng, page, pool, counts, firsts):
+    """Slots of runs of rows: request i writes counts[i] rows from row firsts[i] of a page of its own on."""
+    order, slots, at = rng.permutation(pool), [], 0
+    for n, f in zip(counts, firsts):
+        slots += [int(order[at + p // page]) * page + p % page for p in range(f, f + n)]
+        at += ok.pages_of(f + n, page)
+    assert at <= pool
+    return np.array(slots)
+
+
+def _check_append(rng, slots, page, kv, dim, pool, rotary, positions=None, spread=1.0):
+    tokens = len(slots)
+    heads = 3 * kv  # k and v are columns of a q | k | v matrix
+    qkv = (rng.standard_normal((tokens, (heads + 2 * kv) * dim)) * spread).astype(np.float32)
+    positions = rng.integers(0, 500, tokens) if positions is None else positions
+    rope = _rope(500, rotary) if rotary else None
+    codes = rng.integers(-127, 128, (2, pool, kv, page, dim)).astype(np.int8)
+    scales = (rng.uniform(0.5, 1.5, (2, pool, kv)) * 0.025 * spread).astype(np.float32)
+    g = torch.from_numpy(qkv).cuda()
+    cache = lq.Kv8Cache(*(torch.from_numpy(c).cuda() for c in codes), *(torch.from_numpy(s).cuda() for s in scales))
+    k, v = g[:, heads * dim:(heads + kv) * dim], g[:, (heads + kv) * dim:]
+    lq.kv8_append(k, v, cache, _i32(slots), _i32(positions), rope=_rope_cuda(rope))
+    torch.cuda.synchronize()
+    live = np.asarray(slots) >= 0
+    rows = qkv[:, heads * dim:].reshape(tokens, 2, kv, dim)
+    for side, x, got, got_scale in ((0, ok.rotate(rows[:, 0], positions, rope), cache.k, cache.k_scale),
+                                    (1, rows[:, 1], cache.v, cache.v_scale)):
+        expect, expect_scale, unrounded = ok.append(x, np.where(live, slots, -1), codes[side], scales[side])
+        got, got_scale = got.cpu().numpy(), got_scale.cpu().numpy()
+        assert np.all(np.abs(got_scale - expect_scale) <= 8 * U * expect_scale)
+        differ = got != expect
+        tie = np.abs(np.abs(unrounded - np.floor(unrounded)) - 0.5) < 127 * 16 * U
+        assert not np.any(differ & ~tie), f"{int((differ & ~tie).sum())} codes differ"
+        assert np.all(np.abs(got.astype(int) - expect) <= 1)
+    return cache
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("rotate", ["none", "part", "all"])
+def test_append_pages_and_heads(cuda_device, dim, page, rotate):
+    rng = np.random.default_rng(dim * 1000 + page)
+    rotary = {"none": 0, "part": dim // 4 // 8 * 8 or 8, "all": dim}[rotate]
+    counts = [1, page, 2 * page + 3, page - 1, 5, 1, 1]
+    firsts = [0, 0, page // 2, 1, page - 2, page - 1, 3]
+    slots = _runs(rng, page, 16, counts, firsts)
+    _check_append(rng, slots, page, 2, dim, 16, rotary)
+    assert _status_ok()
+
+
+@pytest.mark.parametrize("tokens,kv", [(1, 1), (1, 5), (700, 1), (3001, 8)])
+def test_append_row_counts(cuda_device, tokens, kv):
+    rng = np.random.default_rng(tokens)
+    page = 64
+    slots = _runs(rng, page, ok.pages_of(tokens + 7, page), [tokens], [7])
+    _check_append(rng, slots, page, kv, 64, ok.pages_of(tokens + 7, page), 64)
+
+
+def test_append_many_single_rows(cuda_device):
+    # A decode step: every row in a page of its own, somewhere inside it.
+    rng = np.random.default_rng(9)
+    for tokens in (64, 700):
+        slots = rng.permutation(tokens) * 32 + rng.integers(0, 32, tokens)
+        _check_append(rng, slots, 32, 4, 64, tokens, 64)
+
+
+def test_append_skips_rows_without_a_slot(cuda_device):
+    rng = np.random.default_rng(11)
+    slots = _runs(rng, 32, 8, [20, 40, 1], [4, 0, 31])
+    slots = np.concatenate([[-1, -1], slots[:20], [-1], slots[20:], [-1] * 5])
+    _check_append(rng, slots, 32, 2, 64, 8, 64)
+    # What a skipped row holds does not matter, nor does its position.
+    k = torch.full((3, 64), float("nan"), device="cuda")
+    k[1] = 2.0
+    cache = lq.Kv8Cache.empty(2, 1, 16, 64)
+    cache.k_scale.fill_(float("nan"))  # a fresh page's old scale is not read
+    rope = _rope_cuda(_rope(4, 64))
+    lq.kv8_append(k, k, cache, _i32([-1, 16, -1]), _i32([-7, 0, 900]), rope=rope)
+    assert torch.all(cache.v[1, 0, 0] == 127) and float(cache.v_scale[1, 0]) == np.float32(2.0) / np.float32(127)
+    assert torch.all(cache.k[1, 0, 0] == 127)
+    assert _status_ok()
+
+
+def test_append_reports_slots_outside_the_pool(cuda_device):
+    cache = lq.Kv8Cache.empty(2, 1, 16, 32)
+    for t in (cache.k, cache.v):
+        t.fill_(3)
+    before = cache.k.clone()
+    k = torch.ones((3, 32), device="cuda")
+    lq.kv8_append(k, k, cache, _i32([32, -5, 2**31 - 1]))
+    assert _lib.load().leafq_device_status() == _lib.LEAFQ_ERR_INVALID
+    assert torch.equal(cache.k, before) and torch.equal(cache.v, before)
+    lq.kv8_append(k[:1], k[:1], cache, _i32([0]), _i32([9]), rope=_rope_cuda(_rope(9, 32)))  # a position past the tables
+    assert _lib.load().leafq_device_status() == _lib.LEAFQ_ERR_INVALID
+
+
+def test_append_zero_and_not_a_number(cuda_device):
+    cache = lq.Kv8Cache.empty(3, 1, 16, 32)
+    k = torch.zeros((3, 32), device="cuda")
+    k[1, 5] = float("nan")
+    k[2, 7] = float("inf")
+    lq.kv8_append(k, k, cache, _i32([0, 16, 32]))
+    s = cache.k_scale[:, 0].tolist()
+    assert s[0] == np.float32(1e-12) and torch.all(cache.k[0, 0, 0] == 0)
+    assert np.isnan(s[1]) and np.isinf(s[2])  # the page shows what went in
+
+
+def test_append_twice_is_append_once(cuda_device):
+    rng = np.random.default_rng(3)
+    cache = _check_append(rng, _runs(rng, 16, 6, [30, 9], [5, 11]), 16, 2, 64, 6, 0)
+    k = torch.randn((9, 128), device="cuda")
+    slots = _i32(np.arange(20, 29))
+    lq.kv8_append(k, k, cache, slots)
+    once = [t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    lq.kv8_append(k, k, cache, slots)
+    assert all(torch.equal(a, b) for a, b in zip(once, (cache.k, cache.v, cache.k_scale, cache.v_scale)))
+
+
+# -------------------------------------------------------------- attention
+class _Batch:
+    """A step over random caches: lists of cached and new tokens per request."""
+
+    def __init__(self, rng, context, new, page, kv, group, dim, rotary=0, lengths=None, spread=1.0, pad=0, spare=2):
+        self.rng, self.page, self.kv, self.group, self.dim = rng, page, kv, group, dim
+        self.context, self.new = list(context), list(new)
+        self.lengths = [c + n for c, n in zip(context, new)] if lengths is None else list(lengths)
+        held = [ok.pages_of(n, page) for n in self.lengths]
+        self.pool = sum(held) + spare
+        order = rng.permutation(self.pool)
+        self.table = np.full((len(held), max(held, default=0) + 1), -1)
+        at = 0
+        for s, b in enumerate(held):
+            self.table[s, :b] = order[at:at + b]
+            at += b
+        self.unused = order[at:]
+        self.codes = np.clip(np.rint(rng.standard_normal((2, self.pool, kv, page, dim)) * 38), -127, 127).astype(np.int8)
+        self.scales = (rng.uniform(0.5, 1.5, (2, self.pool, kv)) * 0.025).astype(np.float32)
+        self.scales[:, self.unused] = np.nan  # pages nobody holds are not read
+        self.tokens = sum(new) + pad
+        self.q = (rng.standard_normal((self.tokens, kv * group * dim)) * spread).astype(np.float32)
+        self.rope = _rope(max([c + n for c, n in zip(context, new)] + [1]), rotary) if rotary else None
+        self.scale = dim ** -0.5
+        self.cache = lq.Kv8Cache(*(torch.from_numpy(c).cuda() for c in self.codes),
+                                 *(torch.from_numpy(s).cuda() for s in self.scales))
+        prefix = lambda x: _i32(np.concatenate([[0], np.cumsum(np.asarray(x, dtype=np.int64))]))  # noqa: E731
+        self.plan = lq.Kv8Plan(_i32(self.context), _i32(self.lengths), prefix(new), prefix(held), _i32(self.table),
+                               self.tokens, max(new, default=0))
+
+    def run(self, q=None, **more):
+        q = torch.from_numpy(self.q).cuda() if q is None else q
+        return lq.kv8_attention(q, self.cache, self.plan, self.scale, rope=_rope_cuda(self.rope), **more)
+
+    def check(self, got=None):
+        got = (self.run() if got is None else got).cpu().numpy().astype(np.float64)
+        expect, bound = np.zeros_like(got), np.zeros_like(got)
+        heads = self.kv * self.group
+        at = 0
+        for s, (c, n) in enumerate(zip(self.context, self.new)):
+            positions = np.arange(c, c + n)
+            q = ok.rotate(self.q[at:at + n].reshape(n, heads, self.dim), positions, self.rope)
+            held = self.table[s, :ok.pages_of(self.lengths[s], self.page)]
+            for h in range(self.kv):
+                k, v = (self.codes[i][held, h].reshape(-1, self.dim).astype(np.float64) *
+                        np.repeat(self.scales[i][held, h].astype(np.float64), self.page)[:, None] for i in range(2))
+                out, reach = ok.attention(q[:, h * self.group:(h + 1) * self.group],
+                                          np.minimum(positions + 1, self.lengths[s]), k, v, self.scale)
+                cols = slice(h * self.group * self.dim, (h + 1) * self.group * self.dim)
+                expect[at:at + n, cols] = out.reshape(n, self.group * self.dim)
+                largest = np.abs(v[:self.lengths[s]]).max(initial=0.0)
+                err = largest * (2 * (self.dim + 16) * reach + 64) * U
+                bound[at:at + n, cols] = np.repeat(err, self.dim, axis=1)
+            at += n
+        got, expect, bound = got[:at], expect[:at], bound[:at]
+        off = np.abs(got - expect)
+        assert np.all(off <= bound), f"largest error {off.max()}, {int((off > bound).sum())} of {off.size} too far"
+        assert np.linalg.norm(off) <= 1e-5 * np.linalg.norm(expect)
+        assert _status_ok()
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("group", [1, 2, 3, 7, 8, 12, 16, 40])
+def test_attention_decode_heads(cuda_device, dim, group):
+    rng = np.random.default_rng(dim + group)
+    _Batch(rng, [0, 1, 15, 63, 64, 300], [1] * 6, 64, 2, group, dim, rotary=dim).check()
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("new", [1, 2, 5, 9])
+def test_attention_decode_pages(cuda_device, page, new):
+    rng = np.random.default_rng(page + new)
+    context = [0, 1, page - 1, page, page + 1, 3 * page - new, 1000, 17]
+    _Batch(rng, context, [new] * 8, page, 3, 4, 64, rotary=32).check()
+    _Batch(rng, context, [new, 0, 1, new, 0, new, 1, 0], page, 1, 8, 128).check()
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("group,page", [(1, 64), (3, 16), (8, 64), (8, 128), (5, 32)])
+def test_attention_prompts(cuda_device, dim, group, page):
+    rng = np.random.default_rng(dim + group + page)
+    _Batch(rng, [0, 0, 100, 37, 513], [130, 1, 65, 200, 33], page, 2, group, dim, rotary=dim).check()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [16, 127, 128, 129, 255, 257, 600])
+def test_attention_prompt_lengths(cuda_device, dim, new):
+    rng = np.random.default_rng(new)
+    _Batch(rng, [0], [new], 64, 1, 2, dim, rotary=dim).check()
+    _Batch(rng, [new], [new], 16, 2, 1, dim).check()
+
+
+def test_attention_long_caches(cuda_device):
+    rng = np.random.default_rng(21)
+    _Batch(rng, [40000, 3, 9001], [1, 1, 1], 128, 2, 8, 64, rotary=64).check()
+    _Batch(rng, [20000, 500], [2, 3], 16, 1, 4, 128).check()
+    _Batch(rng, [12000], [40], 32, 1, 8, 64).check()
+
+
+def test_attention_many_requests(cuda_device):
+    rng = np.random.default_rng(22)
+    n = 700
+    _Batch(rng, rng.integers(0, 90, n), rng.integers(0, 3, n), 16, 2, 2, 64, rotary=64).check()
+
+
+@pytest.mark.parametrize("spread", [0.0, 1e-6, 12.0, 1e4])
+def test_attention_score_ranges(cuda_device, spread):
+    # Flat rows, tiny queries, near one-hot rows, and scores in the tens of thousands.
+    rng = np.random.default_rng(23)
+    for new in (1, 70):
+        b = _Batch(rng, [0, 333], [new, new], 64, 2, 8, 64, spread=spread)
+        got = b.run()
+        assert torch.isfinite(got).all()
+        if spread <= 12:
+            b.check(got)
+        else:  # the weights are one-hot up to ties: each output is (nearly) some visible value, within the pages' largest
+            assert float(got.abs().max()) <= 127 * float(np.nanmax(b.scales)) * (1 + 64 * U)
+
+
+def test_attention_unlike_scales(cuda_device):
+    # Pages whose scales differ by twelve orders of magnitude, one of them all zeros.
+    rng = np.random.default_rng(24)
+    for new in (1, 40):
+        b = _Batch(rng, [200, 90], [new, new], 16, 2, 4, 64, spread=0.5)
+        held = b.table[0, :3]
+        b.scales[1, held] = [[1e-12] * 2, [40.0] * 2, [1e-6] * 2]
+        b.codes[1, held[0]] = 0
+        b.cache.v_scale.copy_(torch.from_numpy(b.scales[1]))
+        b.cache.v.copy_(torch.from_numpy(b.codes[1]))
+        b.check()
+
+
+def test_attention_rows_that_see_nothing(cuda_device):
+    # Refused requests keep their old length: their queries see the cached keys only, or none at all.
+    rng = np.random.default_rng(25)
+    for new in (1, 3, 90):
+        b = _Batch(rng, [0, 20, 64, 0], [new] * 4, 16, 2, 4, 64, lengths=[0, 20, 64 + new, 0], spare=12)
+        out = b.run(out=torch.full(b.q.shape, float("nan"), device="cuda"))
+        assert torch.all(out[:new] == 0) and torch.all(out[3 * new:] == 0)
+        b.check(out)
+
+
+def test_attention_leaves_rows_past_the_last_token(cuda_device):
+    rng = np.random.default_rng(26)
+    for new in (1, 60):
+        b = _Batch(rng, [5, 70], [new, new], 32, 2, 4, 64, pad=3)
+        b.q[-3:] = np.nan
+        out = b.run(out=torch.full(b.q.shape, 7.0, device="cuda"))
+        assert torch.all(out[-3:] == 7.0)
+        b.check(out)
+
+
+def test_attention_reports_pages_outside_the_pool(cuda_device):
+    rng = np.random.default_rng(27)
+    for new in (1, 50):
+        b = _Batch(rng, [100, 30], [new, new], 16, 1, 4, 64)
+        b.plan.table[0, 2] = b.pool
+        b.plan.table[1, 0] = -1
+        out = b.run()
+        assert _lib.load().leafq_device_status() == _lib.LEAFQ_ERR_INVALID
+        assert torch.isfinite(out).all()
+        b.rope = _rope(40, 64)  # positions past the tables
+        b.run()
+        assert _lib.load().leafq_device_status() == _lib.LEAFQ_ERR_INVALID
+        assert _status_ok()
+
+
+def test_attention_not_a_number_stays_in_its_request(cuda_device):
+    rng = np.random.default_rng(28)
+    for new in (1, 50):
+        b = _Batch(rng, [100, 30], [new, new], 16, 2, 4, 64)
+        b.cache.k_scale[int(b.table[0, 1]), 0] = float("nan")
+        out = b.run().reshape(2, new, 2, -1)
+        assert torch.isnan(out[0, :, 0]).all()
+        assert torch.isfinite(out[0, :, 1]).all() and torch.isfinite(out[1]).all()
+
+
+def test_attention_columns_streams_and_repeats(cuda_device):
+    rng = np.random.default_rng(29)
+    for context, new in (([700, 3000, 12], [1, 1, 1]), ([100, 0, 7], [90, 140, 1])):
+        b = _Batch(rng, context, new, 64, 4, 8, 64, rotary=64)
+        width = b.q.shape[1]
+        wide = torch.randn((b.tokens, width + 512), device="cuda")
+        wide[:, :width] = torch.from_numpy(b.q).cuda()
+        ws = lq.Kv8Workspace()
+        first = b.run(wide[:, :width], workspace=ws)
+        b.check(first)
+        other = torch.cuda.Stream()
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            again = [b.run(wide[:, :width], workspace=ws) for _ in range(3)]
+        other.synchronize()
+        assert all(torch.equal(first, x) for x in again)  # the same bits every time
+
+
+def test_attention_code_offsets_past_32_bits(cuda_device):
+    # A pool of 2.4 GB of keys: the held pages lie at both of its ends.
+    page, kv, dim = 128, 4, 128
+    pages = 2_400_000_000 // (page * kv * dim) + 1
+    cache = lq.Kv8Cache.empty(pages, kv, page, dim)
+    rng = np.random.default_rng(30)
+    for context, new in (([300], [1]), ([200], [40])):
+        b = _Batch(rng, context, new, page, kv, 2, dim, spare=0)
+        place = [pages - 1 - i if i % 2 else i for i in range(b.pool)]
+        for big, small in ((cache.k, b.cache.k), (cache.v, b.cache.v), (cache.k_scale, b.cache.k_scale),
+                           (cache.v_scale, b.cache.v_scale)):
+            big[place] = small
+        b.plan.table.copy_(torch.where(b.plan.table >= 0, _i32(place)[b.plan.table.clamp(min=0).long()], -1))
+        b.check(lq.kv8_attention(torch.from_numpy(b.q).cuda(), cache, b.plan, b.scale))
+        k = torch.randn((2, kv * dim), device="cuda")
+        lq.kv8_append(k, k, cache, _i32([(pages - 3) * page, (pages - 3) * page + 1]))
+        back = cache.k[pages - 3, :, :2].float() * cache.k_scale[pages - 3][:, None, None]
+        assert float((back.permute(1, 0, 2).reshape(2, -1) - k).abs().max()) <= 0.51 * float(cache.k_scale[pages - 3].max())
+
+
+def test_step_in_a_graph(cuda_device):
+    # Plan, append and attention captured once and replayed while the requests grow.
+    rng = np.random.default_rng(31)
+    requests, page, kv, group, dim = 5, 16, 2, 4, 64
+    table = torch.full((requests, 20), -1, dtype=torch.int32, device="cuda")
+    free = _i32(rng.permutation(100))
+    length, new, taken = _i32([0] * requests), _i32([1] * requests), _i32([0])
+    cache = lq.Kv8Cache.empty(100, kv, page, dim)
+    rope = _rope_cuda(_rope(320, dim))
+    qkv = torch.zeros((requests, (kv * group + 2 * kv) * dim), device="cuda")
+    q, k, v = qkv.split([kv * group * dim, kv * dim, kv * dim], dim=1)
+    out, ws, plan = torch.zeros(q.shape, device="cuda"), lq.Kv8Workspace(), None
+
+    def step():
+        nonlocal plan
+        for flags in (_lib.LEAFQ_FLAG_PDL,):
+            plan = lq.kv8_plan(length, new, table, free, taken, page, requests, max_tokens=1, out=plan, flags=flags)
+            lq.kv8_append(k, v, cache, plan.slots, plan.positions, rope=rope, flags=flags)
+            lq.kv8_attention(q, cache, plan, dim ** -0.5, rope=rope, out=out, workspace=ws, flags=flags)
+            length.copy_(plan.lengths)
+            taken.copy_(plan.taken)
+
+    step()
+    torch.cuda.synchronize()
+    length.zero_()
+    taken.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    seen = []
+    for t in range(40):
+        row = torch.randn(qkv.shape, generator=torch.Generator().manual_seed(t))
+        qkv.copy_(row)
+        seen.append(row.numpy())
+        graph.replay()
+    torch.cuda.synchronize()
+    assert length.tolist() == [40] * requests and int(taken.item()) == 3 * requests
+    rows = np.stack(seen)  # [steps, requests, width]
+    rope = _rope(320, dim)
+    for s in range(requests):
+        x = rows[:, s].reshape(40, -1, dim)
+        turned = ok.rotate(x[:, :kv * group + kv], np.arange(40), rope)
+        held = table[s, :3].tolist()
+        for h in range(kv):
+            keys = (cache.k[held, h].float() * cache.k_scale[held, h][:, None, None]).reshape(-1, dim)[:40].cpu().numpy()
+            values = (cache.v[held, h].float() * cache.v_scale[held, h][:, None, None]).reshape(-1, dim)[:40].cpu().numpy()
+            # What the cache holds is what went in, to its own rounding: half a code each time a scale grew.
+            assert np.abs(keys - turned[:, kv * group + h]).max() <= 8 * float(cache.k_scale[held, h].max())
+            expect, _ = ok.attention(turned[-1:, h * group:(h + 1) * group], [40], keys.astype(np.float64),
+                                     values.astype(np.float64), dim ** -0.5)
+            got = out[s].reshape(kv, group, dim)[h].cpu().numpy()
+            assert np.linalg.norm(got - expect[0]) <= 1e-5 * np.linalg.norm(expect[0])
+    assert _status_ok()

@@ -1,0 +1,104 @@
+"""The paged INT8 cache's entry points reject invalid arguments on the host,
+before touching a device."""
+import ctypes
+
+import pytest
+import torch
+
+import leaf_b200 as lq
+from leaf_b200 import _lib
+
+P = ctypes.c_void_p(256)
+ODD = ctypes.c_void_p(264)
+
+
+def _cache(**change):
+    fields = dict(k_codes=256, v_codes=256, k_scales=256, v_scales=256, pages=8, page=64, kv_heads=2, dim=64)
+    fields.update(change)
+    return _lib.Kv8CacheDesc(**fields)
+
+
+def _step(**change):
+    fields = dict(context=256, lengths=256, token_offsets=256, page_offsets=256, table=256, max_pages=4, tokens=3,
+                  max_tokens=1, requests=3)
+    fields.update(change)
+    return _lib.Kv8StepDesc(**fields)
+
+
+def _plan(context=P, new=P, requests=3, table=P, max_pages=4, free=P, free_count=8, taken=P, page=64, tokens=3, lengths=P,
+          token_offsets=P, page_offsets=P, positions=P, slots=P, after=P):
+    return _lib.load().leafq_kv8_plan(None, context, new, requests, table, max_pages, free, free_count, taken, page, tokens,
+                                      lengths, token_offsets, page_offsets, positions, slots, after, 0)
+
+
+@pytest.mark.parametrize("change", [dict(requests=-1), dict(max_pages=-1), dict(free_count=-1), dict(tokens=-1),
+                                    dict(page=0), dict(page=48), dict(page=256), dict(max_pages=2**31 // 64),
+                                    dict(tokens=2**31), dict(context=None), dict(new=None), dict(table=None),
+                                    dict(free=None), dict(taken=None), dict(lengths=None), dict(token_offsets=None),
+                                    dict(page_offsets=None), dict(positions=None), dict(slots=None), dict(after=None),
+                                    dict(positions=ODD), dict(slots=ODD)])
+def test_plan_rejects(change):
+    assert _plan(**change) == _lib.LEAFQ_ERR_INVALID
+    assert _lib.load().leafq_last_error()
+
+
+def _append(cache=None, k=P, k_stride=128, v=P, v_stride=128, tokens=2, positions=P, slots=P, rotary=64, cos=P, sin=P,
+            rows=100):
+    cache = _cache() if cache is None else cache
+    return _lib.load().leafq_kv8_append(None, k, k_stride, v, v_stride, tokens, positions, slots, rotary, cos, sin, rows,
+                                        ctypes.byref(cache), 0)
+
+
+@pytest.mark.parametrize("change", [dict(cache=_cache(k_codes=None)), dict(cache=_cache(v_scales=None)),
+                                    dict(cache=_cache(pages=0)), dict(cache=_cache(page=24)),
+                                    dict(cache=_cache(kv_heads=0)), dict(cache=_cache(pages=2**26)),
+                                    dict(cache=_cache(k_codes=264)), dict(k=None), dict(v=None), dict(slots=None),
+                                    dict(positions=None), dict(tokens=-1), dict(tokens=2**31), dict(k_stride=127),
+                                    dict(v_stride=130), dict(k_stride=64), dict(k=ODD), dict(v=ODD), dict(rotary=0),
+                                    dict(rotary=60), dict(rotary=72), dict(cos=None), dict(sin=ODD), dict(rows=0)])
+def test_append_rejects(change):
+    assert _append(**change) == _lib.LEAFQ_ERR_INVALID
+    assert _lib.load().leafq_last_error()
+
+
+def _attend(cache=None, step=None, q=P, stride=256, heads=4, rotary=0, cos=None, sin=None, rows=0, scale=0.125, out=P,
+            workspace=P, nbytes=1 << 40):
+    cache, step = _cache() if cache is None else cache, _step() if step is None else step
+    return _lib.load().leafq_kv8_attention(None, q, stride, heads, rotary, cos, sin, rows, ctypes.byref(cache),
+                                           ctypes.byref(step), scale, out, workspace, nbytes, 0)
+
+
+@pytest.mark.parametrize("change", [dict(cache=_cache(page=8)), dict(step=_step(tokens=-1)), dict(step=_step(requests=-1)),
+                                    dict(step=_step(max_tokens=-1)), dict(step=_step(max_pages=-1)),
+                                    dict(step=_step(max_pages=2**31 // 64)), dict(step=_step(context=None)),
+                                    dict(step=_step(lengths=None)), dict(step=_step(token_offsets=None)),
+                                    dict(step=_step(page_offsets=None)), dict(step=_step(table=None)), dict(heads=0),
+                                    dict(heads=5), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+                                    dict(scale=float("inf")), dict(q=None), dict(out=None), dict(q=ODD), dict(out=ODD),
+                                    dict(stride=255), dict(stride=258), dict(rotary=64), dict(rotary=72, cos=P, sin=P, rows=9)])
+def test_attention_rejects(change):
+    assert _attend(**change) == _lib.LEAFQ_ERR_INVALID
+    assert _lib.load().leafq_last_error()
+
+
+def test_unsupported_head_sizes():
+    for dim in (16, 48, 80, 160, 256):
+        assert _append(cache=_cache(dim=dim), k_stride=1024, v_stride=1024) == _lib.LEAFQ_ERR_UNSUPPORTED
+        assert _attend(cache=_cache(dim=dim), stride=4096) == _lib.LEAFQ_ERR_UNSUPPORTED
+
+
+def test_empty_calls_are_no_ops():
+    assert _append(tokens=0, k=None, v=None, slots=None) == 0
+    assert _attend(step=_step(tokens=0), q=None, out=None) == 0
+    assert _attend(step=_step(requests=0), q=None, out=None) == 0
+
+
+def test_python_refuses_what_it_cannot_pass_on():
+    f = lambda *s: torch.zeros(s)  # noqa: E731
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(lq.LeafError, match="CUDA"):
+        lq.Kv8Cache(f(2, 1, 16, 32).to(torch.int8), f(2, 1, 16, 32).to(torch.int8), f(2, 1), f(2, 1))
+    with pytest.raises(lq.LeafError, match="block table"):
+        lq.Kv8Plan(i(2), i(2), i(3), i(3), i(2), 2, 1)
+    with pytest.raises(lq.LeafError, match="int32 CUDA"):
+        lq.kv8_plan(i(2), i(2), i(2, 3), i(4), i(1), 16, 2)
