@@ -7,7 +7,10 @@
 //   out = sum_j exp(x_j - m) vs cv_j / sum_j exp(x_j - m),  m = max x
 // in one pass over the keys: when the maximum grows from m to m', the sums so
 // far are multiplied by exp(m - m').
+#include <cuda_fp16.h>
+
 #include <climits>
+#include <type_traits>
 
 #include "leafq_device.cuh"
 #include "leafq_internal.h"
@@ -28,86 +31,594 @@ struct AttendArgs {
     int heads, group, rotary, shift;
 };
 
-// Element d of a query row, rotated by position p.
-__device__ __forceinline__ float rotated(const AttendArgs& g, const float* q, int d, int64_t p) {
+constexpr float kLog2e = 1.4426950408889634f;
+// Weights are held as 2^kLift times their value relative to the largest, so
+// that the second half of a weight's fp16 split stays a normal number down to
+// 2^-28 of the largest; 2^14 times 127 codes is far from fp32's range.
+constexpr float kLift = 14.0f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Bytes s of {a, b} (two 16-bit halves of a prmt selector) as two fp16 codes.
+// The codes come biased to 0 .. 255 (sign bit flipped): 0x6400 + u is the
+// fp16 number 1024 + u, exact, and subtracting 1152 leaves the code.
+__device__ __forceinline__ uint32_t codes_half2(uint32_t biased, uint32_t selector) {
+    uint32_t r;
+    asm("{\n\t.reg .b32 x;\n\t"
+        "prmt.b32 x, %1, 0x64646464, %2;\n\t"
+        "sub.rn.f16x2 %0, x, %3;\n\t}"
+        : "=r"(r)
+        : "r"(biased), "r"(selector), "r"(0x64806480u));
+    return r;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void async_copy4(void* smem_dst, const void* gmem_src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem_dst)), "l"(gmem_src) : "memory");
+}
+template <int kPending>
+__device__ __forceinline__ void wait_async_copies_but() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// Eight values of a query row, its item j of D / 8 (a rotation pair's quarters
+// as in the append): a at `at`, b at `to`.
+template <int D>
+__device__ __forceinline__ void query_item(const AttendArgs& g, const float* row, int j, int64_t pos, int& at, int& to,
+                                           float4& a, float4& b) {
     const int half = g.rotary >> 1;
-    const float x = q[d];
-    if (d >= g.rotary) return x;
-    const int j = d < half ? d : d - half;
-    const float c = g.cos_table[p * half + j], s = g.sin_table[p * half + j];
-    return d < half ? __fsub_rn(__fmul_rn(x, c), __fmul_rn(q[d + half], s))
-                    : __fadd_rn(__fmul_rn(x, c), __fmul_rn(q[d - half], s));
+    const bool turned = 4 * j < half;
+    at = turned ? 4 * j : 2 * half + 4 * (j - half / 4);
+    to = turned ? at + half : at + ((D - 2 * half) >> 1);
+    a = *reinterpret_cast<const float4*>(row + at);
+    b = *reinterpret_cast<const float4*>(row + to);
+    if (turned) {
+        const float4 c = *reinterpret_cast<const float4*>(g.cos_table + pos * half + at);
+        const float4 s = *reinterpret_cast<const float4*>(g.sin_table + pos * half + at);
+        const float4 x = a, y = b;
+        a = make_float4(__fsub_rn(__fmul_rn(x.x, c.x), __fmul_rn(y.x, s.x)), __fsub_rn(__fmul_rn(x.y, c.y), __fmul_rn(y.y, s.y)),
+                        __fsub_rn(__fmul_rn(x.z, c.z), __fmul_rn(y.z, s.z)), __fsub_rn(__fmul_rn(x.w, c.w), __fmul_rn(y.w, s.w)));
+        b = make_float4(__fadd_rn(__fmul_rn(y.x, c.x), __fmul_rn(x.x, s.x)), __fadd_rn(__fmul_rn(y.y, c.y), __fmul_rn(x.y, s.y)),
+                        __fadd_rn(__fmul_rn(y.z, c.z), __fmul_rn(x.z, s.z)), __fadd_rn(__fmul_rn(y.w, c.w), __fmul_rn(x.w, s.w)));
+    }
 }
 
-// One warp per query row, lanes over the head's elements.
+// The power of two that brings a row's largest magnitude into [256, 512), as
+// a float and its inverse (1 for a row of zeros): exact, and fp16's range
+// then holds the row whatever its own.
+__device__ __forceinline__ void row_power(uint32_t largest_bits, float& up, float& down) {
+    const int e = static_cast<int>(largest_bits >> 23);
+    int k = 262 - e;
+    k = k > 253 ? 253 : (k < 1 ? 1 : k);
+    if (largest_bits == 0) k = 127;
+    up = __uint_as_float(static_cast<uint32_t>(k) << 23);
+    down = __uint_as_float(static_cast<uint32_t>(254 - k) << 23);
+}
+
+// ---------------------------------------------------------- split form
+// Few query rows, many keys (decode).  A block owns 8 query rows of one kv
+// head (rows r = token * group + head-in-group of a request) and a range of the keys; its warps take chunks of 32 keys in
+// turn, each warp with its own running maximum, sum and output.
+//
+// Tensor cores: m16n8k16, fp16 in, fp32 sums.  The codes are exact in fp16.
+// An fp32 operand is split into hi + lo, 11 significand bits each, so a
+// product loses no more than 2^-22 of it; the eight rows' hi parts are rows
+// 0-7 of the 16-row operand and their lo parts rows 8-15, so one MMA does
+// both and the two accumulator halves are added in the same thread.
+//   S = Q K^T: B is K as stored (a lane's bytes are consecutive elements of
+//   one key); the contraction's order over the head is whatever falls out.
+//   O = P V: the accumulator layout of S is the operand layout of P; B pairs
+//   the bytes of two keys by byte permutes.  A step's columns 2t, 2t+1, 2t+8,
+//   2t+9 are keys t, 4+t, 8+t, 12+t, which makes the V reads conflict-free.
+// The V scale is folded into the exponent: w_j = 2^(x_j + log2 vs - M) with M
+// the running maximum of x_j + log2 vs; O sums w_j cv_j and L sums w_j / vs,
+// so O / L is the softmax average whatever the scales' range.
+//
+// Bound: HBM (the codes are read once: cp.async into a ring per warp, 16-byte
+// pieces, rows swizzled so that both fragment reads touch every bank once);
+// behind it the conversions, 5 and 7 issue slots per four codes of K and V.
 template <int D>
-__global__ void __launch_bounds__(256) kv8_attend_warp_kernel(const AttendArgs g) {
-    constexpr int E = D / 32;
+struct Split {
+    static constexpr int kWarps = D <= 64 ? 8 : 4;
+    static constexpr int kBlocksPerSm = D <= 64 ? 2 : 3;
+    static constexpr int kStages = D <= 64 ? 3 : 2;
+    static constexpr int kThreads = kWarps * 32;
+    static constexpr int kBlocks = 148 * kBlocksPerSm;   // key ranges of one row block
+    static constexpr int kChunk = 32;                    // keys per warp and turn
+    static constexpr int kTile = kChunk * D;             // bytes of K (or V) per chunk
+    static constexpr int kStage = 2 * kTile + 32;        // + {ks, vs} of its two 16-key groups
+    static constexpr int kRing = kStages * kStage;
+    static constexpr int kPart = 8 * (D + 2);            // floats of one partial result: m, l, O
+    static constexpr size_t kSmem = (size_t)kWarps * kRing + 8 * D * sizeof(float);
+    static_assert(kRing >= kPart * 4, "a warp's partial result goes through its ring");
+};
+
+// Where 16-byte piece c of row r of a chunk lies within the row.
+template <int D>
+__device__ __forceinline__ int k_piece(int r, int c) {
+    return D == 128 ? c ^ ((r & 1) << 2) : c;
+}
+template <int D>
+__device__ __forceinline__ int v_piece(int r, int c) {
+    return D == 128 ? c ^ ((r & 3) << 1) : D == 64 ? c ^ (r & 2) : c;
+}
+
+// The last request whose units start at or before u (a search by the warp,
+// 32 probes a step).
+__device__ __forceinline__ int find_request(const int32_t* page_offsets, int requests, int64_t factor, int64_t u, int lane) {
+    int lo = 0, n = requests;
+    while (n > 1) {
+        const int step = (n + 31) / 32, at = lo + lane * step;
+        const bool below = lane * step < n && factor * page_offsets[at] <= u;
+        const int hit = __popc(__ballot_sync(~0u, below)) - 1;
+        lo += hit * step;
+        n = min(step, n - hit * step);
+    }
+    return lo;
+}
+
+template <int D>
+__global__ void __launch_bounds__(Split<D>::kThreads, Split<D>::kBlocksPerSm)
+kv8_attend_split_kernel(const AttendArgs g, float* parts, uint32_t* arrivals, int ranges, int row_blocks) {
+    using C = Split<D>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int last_s;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int gq = lane >> 2, tq = lane & 3;
+    uint8_t* ring = smem + warp * C::kRing;
+    float* q_s = reinterpret_cast<float*>(smem + C::kWarps * C::kRing);
     grid_dependency_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t row = id / g.heads;
-    const int head = static_cast<int>(id - row * g.heads);
-    if (row >= g.step.tokens || row >= g.step.token_offsets[g.step.requests]) return;
-    int lo = 0, hi = g.step.requests - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (g.step.token_offsets[mid] <= row) lo = mid;
-        else hi = mid - 1;
+    grid_launch_dependents();
+
+    // Row blocks of one key range are neighbours, so that they share its codes in L2.
+    const int range = blockIdx.x / row_blocks, row_block = blockIdx.x - range * row_blocks;
+    const int page = 1 << g.shift;
+    const int requests = g.step.requests, kv_heads = g.cache.kv_heads;
+    const int64_t units = (int64_t)kv_heads * g.step.page_offsets[requests];
+    // Work: units (page, head, request) in a row, an even share per block --
+    // a request's head may then be split over blocks, which costs a partial
+    // result each -- or one block for each request's head where that is no
+    // longer than an even share and the joining (about 12 chunks' time).
+    int64_t shares = min64(ranges, (units << g.shift) / (C::kWarps * C::kChunk));
+    if (shares < 1) shares = 1;
+    const int64_t segments = (int64_t)requests * kv_heads;
+    bool whole = false;
+    if (segments <= ranges) {
+        int longest = 0;
+        for (int s = lane; s < requests; s += 32) longest = max(longest, g.step.page_offsets[s + 1] - g.step.page_offsets[s]);
+        longest = __reduce_max_sync(~0u, longest);
+        whole = (int64_t)longest << g.shift <= (units << g.shift) / shares + 12 * C::kChunk;
     }
-    const int64_t pos = (int64_t)g.step.context[lo] + row - g.step.token_offsets[lo];
-    const int64_t held = min64(g.step.page_offsets[lo + 1] - g.step.page_offsets[lo], g.step.max_pages) << g.shift;
-    int64_t keys = min64(min64(pos + 1, g.step.lengths[lo]), held);
-    if (pos < 0 || (g.rotary > 0 && pos >= g.table_rows)) {
-        if (lane == 0) record_device_error(kSiteKv8Range);
-        keys = 0;
-    }
-    float q[E], o[E], m = -INFINITY, l = 0.0f;
-    const float* src = g.q + row * g.q_stride + (int64_t)head * D;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        q[e] = keys > 0 ? rotated(g, src, lane * E + e, pos) : 0.0f;
-        o[e] = 0.0f;
-    }
-    const int kvh = head / g.group;
-    const int64_t page = int64_t{1} << g.shift;
-    const int32_t* table = g.step.table + lo * g.step.max_pages;
-    for (int64_t j0 = 0; j0 < keys; j0 += page) {
-        const int64_t id_page = table[j0 >> g.shift];
-        if (id_page < 0 || id_page >= g.cache.pages) {
-            if (lane == 0) record_device_error(kSiteKv8Range);
-            continue;
+    int64_t begin = 0, end = 0;
+    int s = 0;
+    if (whole) {
+        if (range < segments) {
+            s = range / kv_heads;
+            const int64_t first = g.step.page_offsets[s], held = g.step.page_offsets[s + 1] - first;
+            begin = first * kv_heads + (range - (int64_t)s * kv_heads) * held;
+            end = begin + held;
         }
-        const int64_t tile = id_page * g.cache.kv_heads + kvh;
-        const float ks = g.cache.k_scales[tile] * g.scale, vs = g.cache.v_scales[tile];
-        const int8_t* kc = g.cache.k_codes + (tile << g.shift) * D + lane * E;
-        const int8_t* vc = g.cache.v_codes + (tile << g.shift) * D + lane * E;
-        const int n = static_cast<int>(min64(page, keys - j0));
-        for (int j = 0; j < n; ++j) {
-            float x = 0.0f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) x = fmaf(q[e], static_cast<float>(kc[j * D + e]), x);
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(~0u, x, d);
-            x *= ks;
-            const float grown = fmaxf(m, x), old = m == -INFINITY ? 0.0f : expf(m - grown);
-            const float p = expf(x - grown);
-            m = grown;
-            l = l * old + p;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = o[e] * old + p * vs * static_cast<float>(vc[j * D + e]);
-        }
+    } else if (range < shares) {
+        begin = units * range / shares;
+        end = units * (range + 1) / shares;
+        s = find_request(g.step.page_offsets, requests, kv_heads, begin, lane);
     }
-    float* dst = g.out + row * (int64_t)g.heads * D + (int64_t)head * D + lane * E;
+
+    for (int64_t u = begin; u < end;) {
+        // Segment: pages [p0, p1) of head h of request s.
+        int64_t base = (int64_t)kv_heads * g.step.page_offsets[s];
+        int held = g.step.page_offsets[s + 1] - g.step.page_offsets[s];
+        while (u >= base + (int64_t)kv_heads * held && s + 1 < requests) {
+            ++s;
+            base = (int64_t)kv_heads * g.step.page_offsets[s];
+            held = g.step.page_offsets[s + 1] - g.step.page_offsets[s];
+        }
+        if (held <= 0 || u < base || u >= base + (int64_t)kv_heads * held) break;  // offsets that are no prefix sum
+        const int h = static_cast<int>((u - base) / held);
+        const int64_t start = base + (int64_t)h * held;  // the segment's first unit
+        const int p0 = static_cast<int>(u - start), p1 = static_cast<int>(min64(held, end - start));
+        u = start + p1;
+        const int64_t context = g.step.context[s];
+        const int64_t row0 = max64(0, g.step.token_offsets[s]);
+        const int new_rows = static_cast<int>(
+            max64(0, min64(min64(g.step.token_offsets[s + 1], g.step.tokens) - row0, INT_MAX / g.group)) * g.group);
+        const int first_row = row_block * 8;
+        if (first_row >= new_rows) continue;
+        const int rows = min(8, new_rows - first_row);
+        const int64_t length = g.step.lengths[s];
+        // Keys [ka, kb) for the block; the last row sees the most.
+        const int64_t last_pos = context + (first_row + rows - 1) / g.group;
+        const int64_t ka = (int64_t)p0 << g.shift;
+        const int64_t kb = min64(min64((int64_t)p1 << g.shift, length), last_pos + 1);
+
+        // The rows, rotated, in shared memory.
+        for (int item = tid; item < 8 * (D / 8); item += C::kThreads) {
+            const int r = item / (D / 8), j = item - r * (D / 8);
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
+            int at = 4 * j, to = at + D / 2;
+            if (r < rows) {
+                const int t = (first_row + r) / g.group, hq = (first_row + r) - t * g.group;
+                int64_t pos = context + t;
+                if (g.rotary > 0 && (pos < 0 || pos >= g.table_rows)) {
+                    if (j == 0) record_device_error(kSiteKv8Range);
+                    pos = 0;
+                }
+                query_item<D>(g, g.q + (row0 + t) * g.q_stride + (int64_t)(h * g.group + hq) * D, j, pos, at, to, a, b);
+            }
+            *reinterpret_cast<float4*>(q_s + r * D + at) = a;
+            *reinterpret_cast<float4*>(q_s + r * D + to) = b;
+        }
+
+        // This warp's chunks: ka + 32 (warp + kWarps i).  Loads run kStages - 1
+        // turns ahead, the page numbers they need one turn further.
+        const int32_t* table = g.step.table + (int64_t)s * g.step.max_pages;
+        const int chunks = kb > ka ? static_cast<int>((kb - ka + C::kChunk - 1) / C::kChunk) : 0;
+        const int mine = chunks > warp ? (chunks - warp + C::kWarps - 1) / C::kWarps : 0;
+        const auto key_of = [&](int i) { return ka + (int64_t)C::kChunk * (warp + C::kWarps * i); };
+        const auto page_of = [&](int i) {  // lanes 0-15: the page of the chunk's first 16 keys; 16-31: of the others
+            const int64_t key = key_of(i) + (lane & 16);
+            int32_t id = -1;
+            if (i < mine && key < kb && (key >> g.shift) < g.step.max_pages) {
+                id = table[key >> g.shift];
+                if (id < 0 || id >= g.cache.pages) {
+                    record_device_error(kSiteKv8Range);
+                    id = -1;
+                }
+            }
+            return id;
+        };
+        // Copies chunk i; returns which of its two groups are there (bits 0, 1).
+        const auto load = [&](int i, int id) {
+            uint8_t* stage = ring + (i % C::kStages) * C::kStage;
+            const int id0 = __shfl_sync(~0u, id, 0), id1 = __shfl_sync(~0u, id, 16);
+            if (i < mine) {
+                const int64_t key = key_of(i);
+                constexpr int kPieces = D / 16;  // of a row
 #pragma unroll
-    for (int e = 0; e < E; ++e) dst[e] = m == -INFINITY && l == 0.0f ? 0.0f : o[e] / l;
+                for (int n = 0; n < 2 * kPieces * 16 / 32; ++n) {
+                    const int c = n * 32 + lane, r = c / kPieces, cc = c - r * kPieces;
+                    const int64_t tile = ((int64_t)(r < 16 ? id0 : id1) * kv_heads + h) << g.shift;
+                    if (tile >= 0) {
+                        const int64_t src = (tile + ((key + r) & (page - 1))) * D + cc * 16;
+                        async_copy16(stage + r * D + 16 * k_piece<D>(r, cc), g.cache.k_codes + src);
+                        async_copy16(stage + C::kTile + r * D + 16 * v_piece<D>(r, cc), g.cache.v_codes + src);
+                    }
+                }
+                if (lane < 4) {
+                    const int64_t tile = (int64_t)(lane < 2 ? id0 : id1) * kv_heads + h;
+                    if (tile >= 0)
+                        async_copy4(stage + 2 * C::kTile + 4 * lane, (lane & 1 ? g.cache.v_scales : g.cache.k_scales) + tile);
+                }
+            }
+            commit_async_copies();
+            return (id0 >= 0 ? 1 : 0) | (id1 >= 0 ? 2 : 0);
+        };
+        int there[C::kStages];  // by stage
+        int next_id = page_of(0);
+#pragma unroll
+        for (int i = 0; i < C::kStages - 1; ++i) {
+            const int id = next_id;
+            next_id = page_of(i + 1);
+            there[i] = load(i, id);
+        }
+
+        __syncthreads();
+        // Query fragments: lane (gq, tq) holds row gq's elements that meet its
+        // bytes of a key: 16 of each 64 (D = 64, 128), else D / 4 in a row.
+        uint32_t q[D / 16][4];
+        float factor;  // from an MMA sum to x_j / ks
+        {
+            const float* row = q_s + gq * D;
+            uint32_t largest = 0;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+                const int at = D % 64 == 0 ? (j / 4) * 64 + tq * 16 + (j % 4) * 4 : tq * (D / 4) + j * 4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) largest = max(largest, __float_as_uint(row[at + e]) & 0x7fffffffu);
+            }
+            largest = max(largest, __shfl_xor_sync(~0u, largest, 1));
+            largest = max(largest, __shfl_xor_sync(~0u, largest, 2));
+            float up, down;
+            row_power(largest, up, down);
+            factor = down * g.scale * kLog2e;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+                const int at = D % 64 == 0 ? (j / 4) * 64 + tq * 16 + (j % 4) * 4 : tq * (D / 4) + j * 4;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float x = row[at + 2 * e] * up, y = row[at + 2 * e + 1] * up;
+                    const uint32_t hi = half2_bits(x, y);
+                    const __half2 h2 = *reinterpret_cast<const __half2*>(&hi);
+                    q[j][2 * e] = hi;
+                    q[j][2 * e + 1] = half2_bits(x - __low2float(h2), y - __high2float(h2));
+                }
+            }
+        }
+        // Keys that row gq sees; none for a row past the request's.
+        const int64_t row_pos = context + (first_row + gq) / g.group;
+        const bool seen = gq < rows && row_pos >= 0 && (g.rotary == 0 || row_pos < g.table_rows);
+        const int64_t limit = seen ? min64(kb, row_pos + 1) : 0;
+
+        float o[D / 8][4], m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+
+        for (int i = 0; i < mine; ++i) {
+            {
+                const int id = next_id;
+                next_id = page_of(i + C::kStages);
+                const int t = load(i + C::kStages - 1, id);
+#pragma unroll
+                for (int n = 0; n < C::kStages; ++n)
+                    if (n == (i + C::kStages - 1) % C::kStages) there[n] = t;
+            }
+            wait_async_copies_but<C::kStages - 1>();
+            __syncwarp();
+            const uint8_t* stage = ring + (i % C::kStages) * C::kStage;
+            const int64_t key = key_of(i);
+            int groups = 0;
+#pragma unroll
+            for (int n = 0; n < C::kStages; ++n)
+                if (n == i % C::kStages) groups = there[n];
+            const float4 scales = *reinterpret_cast<const float4*>(stage + 2 * C::kTile);
+            const float ks[2] = {groups & 1 ? scales.x * factor : 0.0f, groups & 2 ? scales.z * factor : 0.0f};
+            const float vs[2] = {groups & 1 ? scales.y : 1.0f, groups & 2 ? scales.w : 1.0f};
+            const float lvs[2] = {log2f(vs[0]), log2f(vs[1])};
+
+            // Scores of keys key + 8 n + {tq, 4 + tq} (n-tile n), in x + log2 vs.
+            float x[4][2], top = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                // Column c of the tile is key (c >> 1) + 4 (c & 1): lane gq's key.
+                const int r = 8 * n + (gq >> 1) + 4 * (gq & 1);
+                uint32_t w[D / 16];
+                if constexpr (D % 64 == 0) {
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c)
+                        *reinterpret_cast<uint4*>(w + 4 * c) =
+                            *reinterpret_cast<const uint4*>(stage + r * D + 16 * k_piece<D>(r, 4 * c + tq));
+                } else {
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c)
+                        *reinterpret_cast<uint2*>(w + 2 * c) = *reinterpret_cast<const uint2*>(stage + r * D + tq * (D / 4) + 8 * c);
+                }
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) {
+                    const uint32_t biased = w[j] ^ 0x80808080u;
+                    mma_f16(acc, q[j], codes_half2(biased, 0x4140u), codes_half2(biased, 0x4342u));
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) x[n][e] = fmaf(acc[e] + acc[e + 2], ks[n >> 1], lvs[n >> 1]);
+            }
+            const bool partial = groups != 3 || key + C::kChunk > limit;
+            if (__any_sync(~0u, partial)) {
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (!(groups & (1 << (n >> 1))) || key + 8 * n + tq + 4 * e >= limit) x[n][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) top = fmaxf(top, fmaxf(x[n][0], x[n][1]));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+            if (__any_sync(~0u, top > m)) {
+                const float grown = fmaxf(m, top);
+                const float old = m == -INFINITY ? 0.0f : ex2(m - grown);
+                m = grown;
+                l *= old;
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][e] *= old;
+            }
+            const float shift = m == -INFINITY ? 0.0f : m - kLift;
+            const float inverse[2] = {__frcp_rn(vs[0]), __frcp_rn(vs[1])};
+            uint32_t p[2][4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                float hi[2], lo[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float w = ex2(x[n][e] - shift);
+                    l = fmaf(w, inverse[n >> 1], l);
+                    hi[e] = __uint_as_float(__float_as_uint(w) & 0xffffe000u);  // 11 bits: exact in fp16
+                    lo[e] = w - hi[e];
+                }
+                p[n >> 1][2 * (n & 1)] = half2_bits(hi[0], hi[1]);
+                p[n >> 1][2 * (n & 1) + 1] = half2_bits(lo[0], lo[1]);
+            }
+#pragma unroll
+            for (int step = 0; step < 2; ++step) {
+                // Keys 16 step + 4 k + tq, elements gq (D / 8) ..: byte n of them is n-tile n's column gq.
+                constexpr int kWords = D / 32;
+                uint32_t w[4][kWords];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int r = 16 * step + 4 * k + tq;
+                    const uint8_t* row = stage + C::kTile + r * D;
+                    if constexpr (D == 128) {
+                        *reinterpret_cast<uint4*>(w[k]) = *reinterpret_cast<const uint4*>(row + 16 * v_piece<D>(r, gq));
+                    } else if constexpr (D == 64) {
+                        *reinterpret_cast<uint2*>(w[k]) =
+                            *reinterpret_cast<const uint2*>(row + 16 * v_piece<D>(r, gq >> 1) + 8 * (gq & 1));
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < kWords; ++c) w[k][c] = *reinterpret_cast<const uint32_t*>(row + gq * (D / 8) + 4 * c);
+                    }
+#pragma unroll
+                    for (int c = 0; c < kWords; ++c) w[k][c] ^= 0x80808080u;
+                }
+#pragma unroll
+                for (int c = 0; c < kWords; ++c) {
+                    // Bytes of keys (2t, 2t+1) and (2t+8, 2t+9) side by side.
+                    const uint32_t a01 = __byte_perm(w[0][c], w[1][c], 0x5140), a23 = __byte_perm(w[0][c], w[1][c], 0x7362);
+                    const uint32_t b01 = __byte_perm(w[2][c], w[3][c], 0x5140), b23 = __byte_perm(w[2][c], w[3][c], 0x7362);
+                    mma_f16(o[4 * c], p[step], codes_half2(a01, 0x4140u), codes_half2(b01, 0x4140u));
+                    mma_f16(o[4 * c + 1], p[step], codes_half2(a01, 0x4342u), codes_half2(b01, 0x4342u));
+                    mma_f16(o[4 * c + 2], p[step], codes_half2(a23, 0x4140u), codes_half2(b23, 0x4140u));
+                    mma_f16(o[4 * c + 3], p[step], codes_half2(a23, 0x4342u), codes_half2(b23, 0x4342u));
+                }
+            }
+            __syncwarp();  // the stage is read before it is copied into again
+        }
+        wait_async_copies_but<0>();
+        __syncwarp();
+
+        // Join the warps: each leaves m, l and O in its ring.
+        float* part = reinterpret_cast<float*>(ring);
+        l += __shfl_xor_sync(~0u, l, 1);
+        l += __shfl_xor_sync(~0u, l, 2);
+        if (tq == 0) {
+            part[gq] = m;
+            part[8 + gq] = l;
+        }
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+            // n-tile j's columns 2t, 2t+1 are elements (2t) (D/8) + j and (2t+1) (D/8) + j.
+            part[16 + gq * D + 2 * tq * (D / 8) + j] = o[j][0] + o[j][2];
+            part[16 + gq * D + (2 * tq + 1) * (D / 8) + j] = o[j][1] + o[j][3];
+        }
+        __syncthreads();
+        const bool split = p0 > 0 || p1 < held;
+        const int64_t mine_part = ((2 * (int64_t)range + (p0 > 0 ? 0 : 1)) * row_blocks + row_block) * C::kPart;
+        for (int item = tid; item < 8 * D; item += C::kThreads) {
+            const int r = item / D, d = item - r * D;
+            float top = -INFINITY, sum = 0.0f, total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < C::kWarps; ++w) top = fmaxf(top, reinterpret_cast<const float*>(smem + w * C::kRing)[r]);
+#pragma unroll
+            for (int w = 0; w < C::kWarps; ++w) {
+                const float* other = reinterpret_cast<const float*>(smem + w * C::kRing);
+                const float weight = other[r] == -INFINITY ? (other[8 + r] == 0.0f ? 0.0f : 1.0f) : ex2(other[r] - top);
+                total = fmaf(weight, other[8 + r], total);
+                sum = fmaf(weight, other[16 + item], sum);
+            }
+            if (split) {
+                float* to = parts + mine_part;
+                if (d == 0) {
+                    to[r] = top;
+                    to[8 + r] = total;
+                }
+                to[16 + item] = sum;
+            } else if (r < rows) {
+                const int t = (first_row + r) / g.group, hq = (first_row + r) - t * g.group;
+                g.out[(row0 + t) * (int64_t)g.heads * D + (int64_t)(h * g.group + hq) * D + d] = total == 0.0f ? 0.0f : sum / total;
+            }
+        }
+        if (split) {
+            // The last block to arrive joins the segment's parts, in block order.
+            const int64_t i0 = ((start + 1) * shares - 1) / units, i1 = ((start + held) * shares - 1) / units;
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                uint32_t* arrived = arrivals + i0 * row_blocks + row_block;
+                last_s = atomicAdd(arrived, 1u) == static_cast<uint32_t>(i1 - i0);
+                if (last_s) *arrived = 0;
+            }
+            __syncthreads();
+            if (last_s) {
+                __threadfence();
+                const auto other = [&](int64_t i) {
+                    return parts + ((2 * i + (i == i0 ? 1 : 0)) * row_blocks + row_block) * C::kPart;
+                };
+                for (int item = tid; item < rows * D; item += C::kThreads) {
+                    const int r = item / D, d = item - r * D;
+                    float top = -INFINITY, sum = 0.0f, total = 0.0f;
+                    for (int64_t i = i0; i <= i1; ++i) top = fmaxf(top, __ldcg(other(i) + r));
+                    for (int64_t i = i0; i <= i1; ++i) {
+                        const float* from = other(i);
+                        const float their = __ldcg(from + r), part_l = __ldcg(from + 8 + r);
+                        const float weight = their == -INFINITY ? (part_l == 0.0f ? 0.0f : 1.0f) : ex2(their - top);
+                        total = fmaf(weight, part_l, total);
+                        sum = fmaf(weight, __ldcg(from + 16 + item), sum);
+                    }
+                    const int t = (first_row + r) / g.group, hq = (first_row + r) - t * g.group;
+                    g.out[(row0 + t) * (int64_t)g.heads * D + (int64_t)(h * g.group + hq) * D + d] =
+                        total == 0.0f ? 0.0f : sum / total;
+                }
+            }
+        }
+        __syncthreads();  // the rings and q_s are free for the next segment
+    }
+
+    // Requests that hold no page: their rows see no key.
+    for (int r = range; r < requests; r += ranges) {
+        if (g.step.page_offsets[r + 1] != g.step.page_offsets[r]) continue;
+        const int64_t row0 = max64(0, g.step.token_offsets[r]);
+        const int64_t count = max64(0, min64(g.step.token_offsets[r + 1], g.step.tokens) - row0) * g.group;
+        for (int64_t row = row_block * 8; row < min64(count, row_block * 8 + 8); ++row)
+            for (int d = tid; d < kv_heads * D; d += C::kThreads)
+                g.out[(row0 + row / g.group) * (int64_t)g.heads * D + ((int64_t)(d / D) * g.group + row % g.group) * D + d % D] =
+                    0.0f;
+    }
+}
+
+// Row blocks of 8, key ranges per row block, and the workspace: the arrival
+// counters of every (range, row block), then two partial results for each.
+struct SplitShape {
+    int64_t row_blocks, ranges;
+    size_t counter_bytes, part_bytes;
+};
+
+template <int D>
+SplitShape split_shape(int64_t max_tokens, int group) {
+    SplitShape f;
+    f.row_blocks = (max_tokens * group + 7) / 8;
+    if (f.row_blocks < 1) f.row_blocks = 1;
+    // About one wave of blocks in all; from there on one block per row block,
+    // whose requests it walks alone.
+    f.ranges = (Split<D>::kBlocks + f.row_blocks - 1) / f.row_blocks;
+    f.counter_bytes = (static_cast<size_t>(f.ranges * f.row_blocks) * sizeof(uint32_t) + 255) / 256 * 256;
+    f.part_bytes = f.ranges > 1 ? 2 * static_cast<size_t>(f.ranges * f.row_blocks) * Split<D>::kPart * sizeof(float) : 0;
+    return f;
 }
 
 template <int D>
-int run_warp(cudaStream_t s, const AttendArgs& g, bool pdl) {
-    const int64_t rows = g.step.tokens * g.heads;
-    return launch(kv8_attend_warp_kernel<D>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, s, pdl,
-                  "leafq_kv8_attention", g);
+int run_split(cudaStream_t s, const AttendArgs& g, void* workspace, bool pdl) {
+    const SplitShape f = split_shape<D>(g.step.max_tokens, g.group);
+    if (f.ranges * f.row_blocks > INT_MAX / 8) {
+        set_error("leafq_kv8_attention: max_tokens * group is too large");
+        return LEAFQ_ERR_INVALID;
+    }
+    const int st = allow_smem(reinterpret_cast<const void*>(kv8_attend_split_kernel<D>), Split<D>::kSmem, "leafq_kv8_attention");
+    if (st) return st;
+    uint32_t* arrivals = static_cast<uint32_t*>(workspace);
+    float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + f.counter_bytes);
+    return launch(kv8_attend_split_kernel<D>, dim3(static_cast<unsigned>(f.ranges * f.row_blocks)), dim3(Split<D>::kThreads),
+                  Split<D>::kSmem, s, pdl, "leafq_kv8_attention", g, parts, arrivals, static_cast<int>(f.ranges),
+                  static_cast<int>(f.row_blocks));
+}
+
+// Calls f(integral constant D) for a supported head size.
+template <typename F>
+auto with_dim(int dim, F&& f) {
+    switch (dim) {
+        case 32: return f(std::integral_constant<int, 32>{});
+        case 64: return f(std::integral_constant<int, 64>{});
+        case 96: return f(std::integral_constant<int, 96>{});
+        default: return f(std::integral_constant<int, 128>{});
+    }
 }
 
 }  // namespace
@@ -118,8 +629,13 @@ using namespace leafq;
 extern "C" {
 
 size_t leafq_kv8_attention_workspace_bytes(int64_t max_tokens, int heads, int kv_heads, int dim) {
-    (void)max_tokens, (void)heads, (void)kv_heads, (void)dim;
-    return 0;
+    if (max_tokens <= 0 || max_tokens > INT_MAX || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
+        !kv8_dim_supported(dim))
+        return 0;
+    return with_dim(dim, [&](auto d) {
+        const SplitShape f = split_shape<d()>(max_tokens, heads / kv_heads);
+        return f.counter_bytes + f.part_bytes;
+    });
 }
 
 int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int heads, int rotary_dim,
@@ -151,18 +667,19 @@ int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int head
         set_error("leafq_kv8_attention: q and out rows must be 16-byte aligned and must not overlap");
         return LEAFQ_ERR_INVALID;
     }
-    (void)workspace, (void)workspace_bytes;
+    if (step->max_tokens == 0) return LEAFQ_OK;
+    const size_t need = leafq_kv8_attention_workspace_bytes(step->max_tokens, heads, cache->kv_heads, cache->dim);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
+        set_error("leafq_kv8_attention: this shape needs " + std::to_string(need) +
+                  " bytes of 16-byte aligned workspace");
+        return LEAFQ_ERR_INVALID;
+    }
     AttendArgs g{q, q_stride, cos_table, sin_table, table_rows, *cache, *step, out, scale, heads,
                  heads / cache->kv_heads, rotary_dim, 0};
     while ((1 << g.shift) < cache->page) ++g.shift;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool pdl = (flags & LEAFQ_FLAG_PDL) != 0;
-    switch (cache->dim) {
-        case 32: return run_warp<32>(s, g, pdl);
-        case 64: return run_warp<64>(s, g, pdl);
-        case 96: return run_warp<96>(s, g, pdl);
-        default: return run_warp<128>(s, g, pdl);
-    }
+    return with_dim(cache->dim, [&](auto d) { return run_split<d()>(s, g, workspace, pdl); });
 }
 
 }  // extern "C"
