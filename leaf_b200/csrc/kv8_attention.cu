@@ -127,9 +127,10 @@ __device__ __forceinline__ void row_power(uint32_t largest_bits, float& up, floa
 //   O = P V: the accumulator layout of S is the operand layout of P; B pairs
 //   the bytes of two keys by byte permutes.  A step's columns 2t, 2t+1, 2t+8,
 //   2t+9 are keys t, 4+t, 8+t, 12+t, which makes the V reads conflict-free.
-// The V scale is folded into the exponent: w_j = 2^(x_j + log2 vs - M) with M
-// the running maximum of x_j + log2 vs; O sums w_j cv_j and L sums w_j / vs,
-// so O / L is the softmax average whatever the scales' range.
+// A V scale vs = f 2^e goes half into the exponent, half into the weight:
+// u_j = 2^(x_j + e - M) with M the running maximum of x_j + e; O sums f u_j cv_j
+// and L sums u_j 2^-e, so O / L is the softmax average whatever the scales'
+// range, and neither half rounds.
 //
 // Bound: HBM (the codes are read once: cp.async into a ring per warp, 16-byte
 // pieces, rows swizzled so that both fragment reads touch every bank once);
@@ -145,9 +146,10 @@ struct Split {
     static constexpr int kTile = kChunk * D;             // bytes of K (or V) per chunk
     static constexpr int kStage = 2 * kTile + 32;        // + {ks, vs} of its two 16-key groups
     static constexpr int kRing = kStages * kStage;
-    static constexpr int kPart = 8 * (D + 2);            // floats of one partial result: m, l, O
+    static constexpr int kPart = 8 * (D + 2);            // floats of one partial result: m [8], l [8], O [8][D]
     static constexpr size_t kSmem = (size_t)kWarps * kRing + 8 * D * sizeof(float);
     static_assert(kRing >= kPart * 4, "a warp's partial result goes through its ring");
+    static_assert(kWarps * kRing >= (kBlocks + 1) * 8 * 4 + (kThreads * 4 + 8 * D) * 4, "joining goes through the rings");
 };
 
 // Where 16-byte piece c of row r of a chunk lies within the row.
@@ -235,18 +237,17 @@ kv8_attend_split_kernel(const AttendArgs g, float* parts, uint32_t* arrivals, in
         const int64_t start = base + (int64_t)h * held;  // the segment's first unit
         const int p0 = static_cast<int>(u - start), p1 = static_cast<int>(min64(held, end - start));
         u = start + p1;
-        const int64_t context = g.step.context[s];
+        const int context = g.step.context[s];
         const int64_t row0 = max64(0, g.step.token_offsets[s]);
         const int new_rows = static_cast<int>(
             max64(0, min64(min64(g.step.token_offsets[s + 1], g.step.tokens) - row0, INT_MAX / g.group)) * g.group);
         const int first_row = row_block * 8;
         if (first_row >= new_rows) continue;
         const int rows = min(8, new_rows - first_row);
-        const int64_t length = g.step.lengths[s];
         // Keys [ka, kb) for the block; the last row sees the most.
-        const int64_t last_pos = context + (first_row + rows - 1) / g.group;
-        const int64_t ka = (int64_t)p0 << g.shift;
-        const int64_t kb = min64(min64((int64_t)p1 << g.shift, length), last_pos + 1);
+        const int ka = p0 << g.shift;
+        const int kb = static_cast<int>(min64(min64((int64_t)p1 << g.shift, g.step.lengths[s]),
+                                              (int64_t)context + (first_row + rows - 1) / g.group + 1));
 
         // The rows, rotated, in shared memory.
         for (int item = tid; item < 8 * (D / 8); item += C::kThreads) {
@@ -255,7 +256,7 @@ kv8_attend_split_kernel(const AttendArgs g, float* parts, uint32_t* arrivals, in
             int at = 4 * j, to = at + D / 2;
             if (r < rows) {
                 const int t = (first_row + r) / g.group, hq = (first_row + r) - t * g.group;
-                int64_t pos = context + t;
+                int64_t pos = (int64_t)context + t;
                 if (g.rotary > 0 && (pos < 0 || pos >= g.table_rows)) {
                     if (j == 0) record_device_error(kSiteKv8Range);
                     pos = 0;
@@ -266,57 +267,51 @@ kv8_attend_split_kernel(const AttendArgs g, float* parts, uint32_t* arrivals, in
             *reinterpret_cast<float4*>(q_s + r * D + to) = b;
         }
 
-        // This warp's chunks: ka + 32 (warp + kWarps i).  Loads run kStages - 1
-        // turns ahead, the page numbers they need one turn further.
+        // This warp's chunks: keys ka + 32 (warp + kWarps i) and on.  Loads run
+        // kStages - 1 turns ahead, the page numbers they need one turn further.
+        // A chunk is two groups of 16 keys, each 16 D consecutive bytes of a page.
         const int32_t* table = g.step.table + (int64_t)s * g.step.max_pages;
-        const int chunks = kb > ka ? static_cast<int>((kb - ka + C::kChunk - 1) / C::kChunk) : 0;
+        const int chunks = kb > ka ? (kb - ka + C::kChunk - 1) / C::kChunk : 0;
         const int mine = chunks > warp ? (chunks - warp + C::kWarps - 1) / C::kWarps : 0;
-        const auto key_of = [&](int i) { return ka + (int64_t)C::kChunk * (warp + C::kWarps * i); };
-        const auto page_of = [&](int i) {  // lanes 0-15: the page of the chunk's first 16 keys; 16-31: of the others
-            const int64_t key = key_of(i) + (lane & 16);
-            int32_t id = -1;
-            if (i < mine && key < kb && (key >> g.shift) < g.step.max_pages) {
-                id = table[key >> g.shift];
-                if (id < 0 || id >= g.cache.pages) {
-                    record_device_error(kSiteKv8Range);
-                    id = -1;
-                }
-            }
-            return id;
+        const auto page_of = [&](int i) {  // lanes 0-15: the page of the chunk's first group; 16-31: of the second
+            const int key = ka + C::kChunk * (warp + C::kWarps * i) + (lane & 16);
+            return i < mine && key < kb && (key >> g.shift) < g.step.max_pages ? table[key >> g.shift] : INT_MIN;
         };
-        // Copies chunk i; returns which of its two groups are there (bits 0, 1).
-        const auto load = [&](int i, int id) {
-            uint8_t* stage = ring + (i % C::kStages) * C::kStage;
-            const int id0 = __shfl_sync(~0u, id, 0), id1 = __shfl_sync(~0u, id, 16);
+        constexpr int kPieces = D / 16;  // 16-byte pieces of a row
+        const auto load = [&](int i, int slot, int id) {
+            uint8_t* stage = ring + slot * C::kStage;
             if (i < mine) {
-                const int64_t key = key_of(i);
-                constexpr int kPieces = D / 16;  // of a row
+                const int key = ka + C::kChunk * (warp + C::kWarps * i);
 #pragma unroll
-                for (int n = 0; n < 2 * kPieces * 16 / 32; ++n) {
-                    const int c = n * 32 + lane, r = c / kPieces, cc = c - r * kPieces;
-                    const int64_t tile = ((int64_t)(r < 16 ? id0 : id1) * kv_heads + h) << g.shift;
-                    if (tile >= 0) {
-                        const int64_t src = (tile + ((key + r) & (page - 1))) * D + cc * 16;
-                        async_copy16(stage + r * D + 16 * k_piece<D>(r, cc), g.cache.k_codes + src);
-                        async_copy16(stage + C::kTile + r * D + 16 * v_piece<D>(r, cc), g.cache.v_codes + src);
+                for (int half = 0; half < 2; ++half) {
+                    const int page_id = __shfl_sync(~0u, id, 16 * half);
+                    const int64_t tile = (int64_t)page_id * kv_heads + h;
+                    float* scales = reinterpret_cast<float*>(stage + 2 * C::kTile) + 2 * half;
+                    if (page_id >= 0 && page_id < g.cache.pages) {
+                        const int64_t src = ((tile << g.shift) + ((key + 16 * half) & (page - 1))) * D + lane * 16;
+#pragma unroll
+                        for (int n = 0; n < kPieces / 2; ++n) {
+                            const int c = n * 32 + lane, r = 16 * half + c / kPieces, cc = c % kPieces;
+                            async_copy16(stage + r * D + 16 * k_piece<D>(r, cc), g.cache.k_codes + src + n * 512);
+                            async_copy16(stage + C::kTile + r * D + 16 * v_piece<D>(r, cc), g.cache.v_codes + src + n * 512);
+                        }
+                        if (lane == 0) async_copy4(scales, g.cache.k_scales + tile);
+                        if (lane == 1) async_copy4(scales + 1, g.cache.v_scales + tile);
+                    } else if (lane == 0) {
+                        scales[0] = 0.0f;
+                        scales[1] = -1.0f;  // the group is not there
+                        if (page_id != INT_MIN) record_device_error(kSiteKv8Range);
                     }
-                }
-                if (lane < 4) {
-                    const int64_t tile = (int64_t)(lane < 2 ? id0 : id1) * kv_heads + h;
-                    if (tile >= 0)
-                        async_copy4(stage + 2 * C::kTile + 4 * lane, (lane & 1 ? g.cache.v_scales : g.cache.k_scales) + tile);
                 }
             }
             commit_async_copies();
-            return (id0 >= 0 ? 1 : 0) | (id1 >= 0 ? 2 : 0);
         };
-        int there[C::kStages];  // by stage
         int next_id = page_of(0);
 #pragma unroll
         for (int i = 0; i < C::kStages - 1; ++i) {
             const int id = next_id;
             next_id = page_of(i + 1);
-            there[i] = load(i, id);
+            load(i, i, id);
         }
 
         __syncthreads();
@@ -352,9 +347,9 @@ kv8_attend_split_kernel(const AttendArgs g, float* parts, uint32_t* arrivals, in
             }
         }
         // Keys that row gq sees; none for a row past the request's.
-        const int64_t row_pos = context + (first_row + gq) / g.group;
+        const int64_t row_pos = (int64_t)context + (first_row + gq) / g.group;
         const bool seen = gq < rows && row_pos >= 0 && (g.rotary == 0 || row_pos < g.table_rows);
-        const int64_t limit = seen ? min64(kb, row_pos + 1) : 0;
+        const int limit = seen ? static_cast<int>(min64(kb, row_pos + 1)) : 0;
 
         float o[D / 8][4], m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -362,29 +357,31 @@ kv8_attend_split_kernel(const AttendArgs g, float* parts, uint32_t* arrivals, in
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
 
+        int slot = 0;
         for (int i = 0; i < mine; ++i) {
             {
-                const int id = next_id;
+                const int id = next_id, into = slot == 0 ? C::kStages - 1 : slot - 1;
                 next_id = page_of(i + C::kStages);
-                const int t = load(i + C::kStages - 1, id);
-#pragma unroll
-                for (int n = 0; n < C::kStages; ++n)
-                    if (n == (i + C::kStages - 1) % C::kStages) there[n] = t;
+                load(i + C::kStages - 1, into, id);
             }
             wait_async_copies_but<C::kStages - 1>();
             __syncwarp();
-            const uint8_t* stage = ring + (i % C::kStages) * C::kStage;
-            const int64_t key = key_of(i);
-            int groups = 0;
-#pragma unroll
-            for (int n = 0; n < C::kStages; ++n)
-                if (n == i % C::kStages) groups = there[n];
+            const uint8_t* stage = ring + slot * C::kStage;
+            slot = slot + 1 == C::kStages ? 0 : slot + 1;
+            const int key = ka + C::kChunk * (warp + C::kWarps * i);
             const float4 scales = *reinterpret_cast<const float4*>(stage + 2 * C::kTile);
-            const float ks[2] = {groups & 1 ? scales.x * factor : 0.0f, groups & 2 ? scales.z * factor : 0.0f};
-            const float vs[2] = {groups & 1 ? scales.y : 1.0f, groups & 2 ? scales.w : 1.0f};
-            const float lvs[2] = {log2f(vs[0]), log2f(vs[1])};
+            float ks[2], bias[2], frac[2], back[2];  // per group: x / sum, e, f, 2^-e
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const float vs = n == 0 ? scales.y : scales.w;
+                const int e = (__float_as_int(vs) >> 23) & 255;
+                ks[n] = (n == 0 ? scales.x : scales.z) * factor;
+                bias[n] = vs < 0.0f ? -INFINITY : static_cast<float>(e - 127);
+                back[n] = __int_as_float(max(0, 254 - e) << 23);
+                frac[n] = vs * back[n];
+            }
 
-            // Scores of keys key + 8 n + {tq, 4 + tq} (n-tile n), in x + log2 vs.
+            // Scores of keys key + 8 n + {tq, 4 + tq} (n-tile n), in x + e.
             float x[4][2], top = -INFINITY;
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
@@ -408,77 +405,71 @@ kv8_attend_split_kernel(const AttendArgs g, float* parts, uint32_t* arrivals, in
                     mma_f16(acc, q[j], codes_half2(biased, 0x4140u), codes_half2(biased, 0x4342u));
                 }
 #pragma unroll
-                for (int e = 0; e < 2; ++e) x[n][e] = fmaf(acc[e] + acc[e + 2], ks[n >> 1], lvs[n >> 1]);
+                for (int e = 0; e < 2; ++e) x[n][e] = fmaf(acc[e] + acc[e + 2], ks[n >> 1], bias[n >> 1]);
             }
-            const bool partial = groups != 3 || key + C::kChunk > limit;
-            if (__any_sync(~0u, partial)) {
+            if (__any_sync(~0u, key + C::kChunk > limit)) {
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        if (!(groups & (1 << (n >> 1))) || key + 8 * n + tq + 4 * e >= limit) x[n][e] = -INFINITY;
+                        if (key + 8 * n + tq + 4 * e >= limit) x[n][e] = -INFINITY;
             }
 #pragma unroll
             for (int n = 0; n < 4; ++n) top = fmaxf(top, fmaxf(x[n][0], x[n][1]));
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-            if (__any_sync(~0u, top > m)) {
-                const float grown = fmaxf(m, top);
-                const float old = m == -INFINITY ? 0.0f : ex2(m - grown);
-                m = grown;
-                l *= old;
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][e] *= old;
-            }
+            // O and L so far count relative to the maximum so far.
+            const float grown = fmaxf(m, top);
+            const float old = m == -INFINITY ? 0.0f : ex2(m - grown);
+            m = grown;
+            l *= old;
             const float shift = m == -INFINITY ? 0.0f : m - kLift;
-            const float inverse[2] = {__frcp_rn(vs[0]), __frcp_rn(vs[1])};
             uint32_t p[2][4];
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 float hi[2], lo[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float w = ex2(x[n][e] - shift);
-                    l = fmaf(w, inverse[n >> 1], l);
+                    const float u = ex2(x[n][e] - shift), w = u * frac[n >> 1];
+                    l = fmaf(u, back[n >> 1], l);
                     hi[e] = __uint_as_float(__float_as_uint(w) & 0xffffe000u);  // 11 bits: exact in fp16
                     lo[e] = w - hi[e];
                 }
                 p[n >> 1][2 * (n & 1)] = half2_bits(hi[0], hi[1]);
                 p[n >> 1][2 * (n & 1) + 1] = half2_bits(lo[0], lo[1]);
             }
+            // A chunk's products sum up in the MMA, whose additions truncate; the
+            // chunks are added (and rescaled) in rounded fp32.
+            constexpr int kWords = D / 32;
 #pragma unroll
-            for (int step = 0; step < 2; ++step) {
-                // Keys 16 step + 4 k + tq, elements gq (D / 8) ..: byte n of them is n-tile n's column gq.
-                constexpr int kWords = D / 32;
-                uint32_t w[4][kWords];
+            for (int c = 0; c < kWords; ++c) {
+                float part[4][4] = {};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int r = 16 * step + 4 * k + tq;
-                    const uint8_t* row = stage + C::kTile + r * D;
-                    if constexpr (D == 128) {
-                        *reinterpret_cast<uint4*>(w[k]) = *reinterpret_cast<const uint4*>(row + 16 * v_piece<D>(r, gq));
-                    } else if constexpr (D == 64) {
-                        *reinterpret_cast<uint2*>(w[k]) =
-                            *reinterpret_cast<const uint2*>(row + 16 * v_piece<D>(r, gq >> 1) + 8 * (gq & 1));
-                    } else {
+                for (int step = 0; step < 2; ++step) {
+                    // Keys 16 step + 4 k + tq, elements gq (D / 8) ..: byte n of them is n-tile n's column gq.
+                    uint32_t w[4];
 #pragma unroll
-                        for (int c = 0; c < kWords; ++c) w[k][c] = *reinterpret_cast<const uint32_t*>(row + gq * (D / 8) + 4 * c);
+                    for (int k = 0; k < 4; ++k) {
+                        const int r = 16 * step + 4 * k + tq;
+                        const uint8_t* row = stage + C::kTile + r * D;
+                        w[k] = *reinterpret_cast<const uint32_t*>(
+                                   D == 128 ? row + 16 * v_piece<D>(r, gq) + 4 * c
+                                            : (D == 64 ? row + 16 * v_piece<D>(r, gq >> 1) + 8 * (gq & 1) + 4 * c
+                                                       : row + gq * (D / 8) + 4 * c)) ^
+                               0x80808080u;
                     }
-#pragma unroll
-                    for (int c = 0; c < kWords; ++c) w[k][c] ^= 0x80808080u;
-                }
-#pragma unroll
-                for (int c = 0; c < kWords; ++c) {
                     // Bytes of keys (2t, 2t+1) and (2t+8, 2t+9) side by side.
-                    const uint32_t a01 = __byte_perm(w[0][c], w[1][c], 0x5140), a23 = __byte_perm(w[0][c], w[1][c], 0x7362);
-                    const uint32_t b01 = __byte_perm(w[2][c], w[3][c], 0x5140), b23 = __byte_perm(w[2][c], w[3][c], 0x7362);
-                    mma_f16(o[4 * c], p[step], codes_half2(a01, 0x4140u), codes_half2(b01, 0x4140u));
-                    mma_f16(o[4 * c + 1], p[step], codes_half2(a01, 0x4342u), codes_half2(b01, 0x4342u));
-                    mma_f16(o[4 * c + 2], p[step], codes_half2(a23, 0x4140u), codes_half2(b23, 0x4140u));
-                    mma_f16(o[4 * c + 3], p[step], codes_half2(a23, 0x4342u), codes_half2(b23, 0x4342u));
+                    const uint32_t a01 = __byte_perm(w[0], w[1], 0x5140), a23 = __byte_perm(w[0], w[1], 0x7362);
+                    const uint32_t b01 = __byte_perm(w[2], w[3], 0x5140), b23 = __byte_perm(w[2], w[3], 0x7362);
+                    mma_f16(part[0], p[step], codes_half2(a01, 0x4140u), codes_half2(b01, 0x4140u));
+                    mma_f16(part[1], p[step], codes_half2(a01, 0x4342u), codes_half2(b01, 0x4342u));
+                    mma_f16(part[2], p[step], codes_half2(a23, 0x4140u), codes_half2(b23, 0x4140u));
+                    mma_f16(part[3], p[step], codes_half2(a23, 0x4342u), codes_half2(b23, 0x4342u));
                 }
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[4 * c + n][e] = fmaf(o[4 * c + n][e], old, part[n][e]);
             }
             __syncwarp();  // the stage is read before it is copied into again
         }
@@ -539,23 +530,58 @@ kv8_attend_split_kernel(const AttendArgs g, float* parts, uint32_t* arrivals, in
             __syncthreads();
             if (last_s) {
                 __threadfence();
-                const auto other = [&](int64_t i) {
-                    return parts + ((2 * i + (i == i0 ? 1 : 0)) * row_blocks + row_block) * C::kPart;
+                // Weights of the parts' rows, then their weighted sums, four elements and
+                // every kSets-th part per thread.
+                const int n = static_cast<int>(i1 - i0) + 1;
+                const auto other = [&](int i) {
+                    return parts + ((2 * (i0 + i) + (i == 0 ? 1 : 0)) * row_blocks + row_block) * C::kPart;
                 };
-                for (int item = tid; item < rows * D; item += C::kThreads) {
-                    const int r = item / D, d = item - r * D;
-                    float top = -INFINITY, sum = 0.0f, total = 0.0f;
-                    for (int64_t i = i0; i <= i1; ++i) top = fmaxf(top, __ldcg(other(i) + r));
-                    for (int64_t i = i0; i <= i1; ++i) {
-                        const float* from = other(i);
-                        const float their = __ldcg(from + r), part_l = __ldcg(from + 8 + r);
+                float* weight_s = reinterpret_cast<float*>(smem);  // [n][8], then the rows' sums [8]
+                for (int r = warp; r < 8; r += C::kWarps) {
+                    float top = -INFINITY, total = 0.0f;
+                    for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(other(i) + r));
+                    top = warp_max_f32(top);
+                    for (int i = lane; i < n; i += 32) {
+                        const float their = __ldcg(other(i) + r), part_l = __ldcg(other(i) + 8 + r);
                         const float weight = their == -INFINITY ? (part_l == 0.0f ? 0.0f : 1.0f) : ex2(their - top);
+                        weight_s[i * 8 + r] = weight;
                         total = fmaf(weight, part_l, total);
-                        sum = fmaf(weight, __ldcg(from + 16 + item), sum);
                     }
+#pragma unroll
+                    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
+                    if (lane == 0) weight_s[n * 8 + r] = total;
+                }
+                __syncthreads();
+                constexpr int kItems = 8 * D / 4, kSets = C::kThreads > kItems ? C::kThreads / kItems : 1;
+                float4* set_s = reinterpret_cast<float4*>(weight_s + (n * 8 + 8));
+                for (int item = tid % kItems, set = tid / kItems; item < kItems && set < kSets; item += C::kThreads) {
+                    const int r = item / (D / 4);
+                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+                    for (int i = set; i < n; i += kSets) {
+                        const float weight = weight_s[i * 8 + r];
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(other(i) + 16) + item);
+                        sum.x = fmaf(weight, v.x, sum.x);
+                        sum.y = fmaf(weight, v.y, sum.y);
+                        sum.z = fmaf(weight, v.z, sum.z);
+                        sum.w = fmaf(weight, v.w, sum.w);
+                    }
+                    set_s[set * kItems + item] = sum;
+                }
+                __syncthreads();
+                for (int item = tid; item < rows * (D / 4); item += C::kThreads) {
+                    const int r = item / (D / 4), d = 4 * (item - r * (D / 4));
+                    float4 sum = set_s[item];
+#pragma unroll
+                    for (int set = 1; set < kSets; ++set) {
+                        const float4 v = set_s[set * kItems + item];
+                        sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+                    }
+                    const float total = weight_s[n * 8 + r];
+                    const float4 y = total == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                                   : make_float4(sum.x / total, sum.y / total, sum.z / total, sum.w / total);
                     const int t = (first_row + r) / g.group, hq = (first_row + r) - t * g.group;
-                    g.out[(row0 + t) * (int64_t)g.heads * D + (int64_t)(h * g.group + hq) * D + d] =
-                        total == 0.0f ? 0.0f : sum / total;
+                    *reinterpret_cast<float4*>(g.out + (row0 + t) * (int64_t)g.heads * D + (int64_t)(h * g.group + hq) * D + d) = y;
                 }
             }
         }
