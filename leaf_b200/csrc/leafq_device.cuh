@@ -52,6 +52,7 @@ enum WaitSite : unsigned {
     kSiteAllGather = 13,
     kSiteCacheRange = 14,  // not a wait: a position outside the KV cache
     kSiteKv8Range = 15,    // not a wait: a paged-cache index or length out of range
+    kSiteKv8Tile = 16,
 };
 
 __device__ __forceinline__ unsigned long long global_timer_ns() {
