@@ -111,6 +111,25 @@ int cuda_status(cudaError_t err, const char* what) {
 int sm_count() { return device_info().sms; }
 int max_smem_per_block() { return device_info().smem; }
 
+int device_watch(DeviceWatch* watch) {
+    static std::mutex mutex;
+    static std::unordered_map<int, DeviceWatch> cache;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(mutex);
+    DeviceWatch& found = cache[dev];
+    if (!found.error) {
+        void *error = nullptr, *limit = nullptr;
+        cudaError_t err = cudaGetSymbolAddress(&error, g_device_error);
+        if (err == cudaSuccess) err = cudaGetSymbolAddress(&limit, g_wait_limit_ns);
+        if (err != cudaSuccess) return cuda_status(err, "device_watch");
+        found.error = static_cast<unsigned int*>(error);
+        found.limit_ns = static_cast<const unsigned long long*>(limit);
+    }
+    *watch = found;
+    return LEAFQ_OK;
+}
+
 int allow_smem(const void* kernel, size_t bytes, const char* what) {
     static std::mutex mutex;
     static std::unordered_map<const void*, size_t> done;

@@ -1,0 +1,96 @@
+// Shared by the two forms of the paged INT8 cache's attention (kv8_attention.cu
+// for few query rows, kv8_tile.cu for many).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <climits>
+#include <cmath>
+
+#include "leafq_device.cuh"
+#include "leafq_internal.h"
+
+namespace leafq {
+
+struct Kv8AttendArgs {
+    const float* q;
+    int64_t q_stride;
+    const float* cos_table;
+    const float* sin_table;
+    int64_t table_rows;
+    leafq_kv8_cache cache;
+    leafq_kv8_step step;
+    float* out;
+    float scale;
+    int heads, group, rotary, shift;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+// Weights are held as 2^kLift times their value relative to the largest, so
+// that the second half of a weight's fp16 split stays a normal number down to
+// 2^-28 of the largest; 2^14 times 127 codes is far from fp32's range.
+constexpr float kLift = 14.0f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Bytes s of {a, b} (two 16-bit halves of a prmt selector) as two fp16 codes.
+// The codes come biased to 0 .. 255 (sign bit flipped): 0x6400 + u is the
+// fp16 number 1024 + u, exact, and subtracting 1152 leaves the code.
+__device__ __forceinline__ uint32_t codes_half2(uint32_t biased, uint32_t selector) {
+    uint32_t r;
+    asm("{\n\t.reg .b32 x;\n\t"
+        "prmt.b32 x, %1, 0x64646464, %2;\n\t"
+        "sub.rn.f16x2 %0, x, %3;\n\t}"
+        : "=r"(r)
+        : "r"(biased), "r"(selector), "r"(0x64806480u));
+    return r;
+}
+
+// Eight values of a query row, its item j of D / 8 (a rotation pair's quarters
+// as in the append): a at `at`, b at `to`.
+template <int D>
+__device__ __forceinline__ void query_item(const Kv8AttendArgs& g, const float* row, int j, int64_t pos, int& at, int& to,
+                                           float4& a, float4& b) {
+    const int half = g.rotary >> 1;
+    const bool turned = 4 * j < half;
+    at = turned ? 4 * j : 2 * half + 4 * (j - half / 4);
+    to = turned ? at + half : at + ((D - 2 * half) >> 1);
+    a = *reinterpret_cast<const float4*>(row + at);
+    b = *reinterpret_cast<const float4*>(row + to);
+    if (turned) {
+        const float4 c = *reinterpret_cast<const float4*>(g.cos_table + pos * half + at);
+        const float4 s = *reinterpret_cast<const float4*>(g.sin_table + pos * half + at);
+        const float4 x = a, y = b;
+        a = make_float4(__fsub_rn(__fmul_rn(x.x, c.x), __fmul_rn(y.x, s.x)), __fsub_rn(__fmul_rn(x.y, c.y), __fmul_rn(y.y, s.y)),
+                        __fsub_rn(__fmul_rn(x.z, c.z), __fmul_rn(y.z, s.z)), __fsub_rn(__fmul_rn(x.w, c.w), __fmul_rn(y.w, s.w)));
+        b = make_float4(__fadd_rn(__fmul_rn(y.x, c.x), __fmul_rn(x.x, s.x)), __fadd_rn(__fmul_rn(y.y, c.y), __fmul_rn(x.y, s.y)),
+                        __fadd_rn(__fmul_rn(y.z, c.z), __fmul_rn(x.z, s.z)), __fadd_rn(__fmul_rn(y.w, c.w), __fmul_rn(x.w, s.w)));
+    }
+}
+
+// The power of two that brings a row's largest magnitude into [256, 512), as
+// a float and its inverse (1 for a row of zeros): exact, and fp16's range
+// then holds the row whatever its own.
+__device__ __forceinline__ void row_power(uint32_t largest_bits, float& up, float& down) {
+    const int e = static_cast<int>(largest_bits >> 23);
+    int k = 262 - e;
+    k = k > 253 ? 253 : (k < 1 ? 1 : k);
+    if (largest_bits == 0) k = 127;
+    up = __uint_as_float(static_cast<uint32_t>(k) << 23);
+    down = __uint_as_float(static_cast<uint32_t>(254 - k) << 23);
+}
+
+// Many query rows of a request (kv8_tile.cu).
+int launch_kv8_tiles(cudaStream_t s, const Kv8AttendArgs& g, bool pdl);
+
+}  // namespace leafq

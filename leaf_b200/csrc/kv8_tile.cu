@@ -1,0 +1,584 @@
+// Attention over the paged INT8 cache, many query rows (prompts, long chunks).
+//
+// Compiled as a whole program (build.py): setmaxnreg is ignored in relocatable
+// device code.
+#define LEAFQ_WHOLE_PROGRAM
+#include "kv8_attention.cuh"
+
+namespace leafq {
+namespace {
+
+// A block owns 128 query
+// rows of one kv head of a request (rows r = token * group + head-in-group),
+// walks the keys in tiles, and two blocks share an SM, so that one's MMAs run
+// under the other's softmax.  Roles:
+//   warps 0-3  softmax: one row per thread (its TMEM lane), a tile's scores in
+//              registers; thread 0 issues the MMAs (kind::f16, fp32
+//              accumulators in TMEM)
+//   warps 4-7  codes to fp16: 16-byte global loads one tile ahead, byte
+//              permutes, 128-byte-swizzled shared memory
+// The softmax warps take registers that the converting ones leave (setmaxnreg).
+// The arithmetic is the split form's: codes exact in fp16, fp32 operands as
+// hi + lo halves, the V scale in the exponent.
+//   S [128][keys] = Qhi K^T + Qlo K^T   Q and K K-major in shared memory
+//   O [128][D]   += Phi V + Plo V       P from TMEM, V as stored (MN-major)
+// Each 32 columns of S are replaced in place by 16 columns of P's hi pairs and
+// 16 of its lo pairs.  O is rescaled only when a row's maximum grows by more
+// than 2^kSlack since its reference was taken: weights then stay below
+// 2^(kTileLift + kSlack) < 65504, fp16's largest.  The MMA's additions truncate,
+// which adds up over long sums (8192 keys: 5.5e-6 of the result), so every
+// kSpan keys O is added to a rounded sum (in local memory) and starts anew
+// -- and the lo halves of Q go first, while S is small.
+constexpr float kTileLift = 6.0f, kSlack = 8.0f;
+
+template <int D>
+struct TileShape {
+    static constexpr int kRows = 128;
+    static constexpr int kKeys = D <= 64 ? 128 : 64;
+    static constexpr int kBlocks = (D + 63) / 64;        // 64-element (128-byte) column blocks
+    static constexpr int kStages = D <= 64 ? 2 : 1;      // of K and of V
+    static constexpr int kGroups = kKeys / 16;           // of keys that share a page for certain
+    static constexpr int kInfo = 4;                      // ring of the groups' scales
+    static constexpr int kQBytes = kBlocks * kRows * 128;
+    static constexpr int kKvBytes = kBlocks * kKeys * 128;
+    static constexpr int kSpan = 512 / kKeys;            // tiles between O's additions to the rounded sum
+    static constexpr int kThreads = 256;
+    static constexpr int kSoftmaxRegs = 184, kConvertRegs = 72;
+    static constexpr int kPieces = kKeys * D / 16 / 128; // 16-byte pieces of a K (or V) tile per converting thread
+    static constexpr int kOutCols = kBlocks * 64;        // O columns (those past D are not read)
+    static constexpr uint32_t kTmemCols = 256;
+    static constexpr size_t kSmem = 1024 + 2 * kQBytes + 2 * kStages * kKvBytes + kInfo * kGroups * 16 + kRows * 4 + 256;
+    static_assert(kKeys + kOutCols <= 256, "two blocks share the SM's 512 TMEM columns");
+    static_assert(2 * kQBytes >= kRows * D * 4, "the output leaves through Q's shared memory");
+    static_assert(128 * (kSoftmaxRegs + kConvertRegs) == kThreads * 128, "the split of what the launch gives (128 a thread)");
+};
+
+// The library's device error word and wait limit (leafq_device.cuh), which this
+// file, compiled as a whole program, cannot name.
+__device__ __forceinline__ void report(const DeviceWatch& w, unsigned site) {
+    atomicCAS(w.error, 0u, (site << 16) | (blockIdx.x & 0xffffu));
+}
+
+// Bounded wait that other requests' range errors do not end.
+__device__ __forceinline__ bool tile_wait(const DeviceWatch& w, uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long start = global_timer_ns();
+    for (uint32_t spins = 1;; ++spins) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((spins & 255u) == 0u && global_timer_ns() - start > *static_cast<volatile const unsigned long long*>(w.limit_ns)) {
+            report(w, kSiteKv8Tile);
+            return false;
+        }
+    }
+}
+
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// The A operand from tensor memory: two fp16 per 32-bit column.
+__device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Instruction descriptor for kind::f16: fp32 accumulator (1) in [4,6), fp16 A
+// and B (0), B MN-major (bit 16) or K-major, N >> 3 in [17,23), M >> 4 in [24,29).
+__host__ __device__ constexpr uint32_t umma_idesc_f16(uint32_t m, uint32_t n, bool b_mn) {
+    return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+template <int D>
+__global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_tiles) {
+    using C = TileShape<D>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* q_hi = smem;
+    uint8_t* q_lo = q_hi + C::kQBytes;
+    uint8_t* k_tiles = q_lo + C::kQBytes;
+    uint8_t* v_tiles = k_tiles + C::kStages * C::kKvBytes;
+    float4* info = reinterpret_cast<float4*>(v_tiles + C::kStages * C::kKvBytes);  // [kInfo][kGroups]: ks, log2 vs, 1 / vs
+    float* factor_s = reinterpret_cast<float*>(info + C::kInfo * C::kGroups);
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(factor_s + C::kRows);
+    uint64_t* k_empty = k_full + C::kStages;
+    uint64_t* v_full = k_empty + C::kStages;
+    uint64_t* v_empty = v_full + C::kStages;
+    uint64_t* s_full = v_empty + C::kStages;
+    uint64_t* p_full = s_full + 1;
+    uint64_t* o_full = p_full + 1;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_full + 1);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    grid_dependency_wait();
+    grid_launch_dependents();
+
+    // Work item, the rows that see most keys first.  Request s may have row
+    // tiles floor(token_offsets[s] * group / 128) + s and on: enough of them.
+    const int item = row_tiles - 1 - blockIdx.x / g.cache.kv_heads;
+    const int h = blockIdx.x % g.cache.kv_heads;
+    const int requests = g.step.requests;
+    int s = 0;
+    for (int n = requests; n > 1;) {
+        const int step = (n + 31) / 32, at = s + lane * step;
+        const bool below = lane * step < n && ((int64_t)g.step.token_offsets[at] * g.group >> 7) + at <= item;
+        const int hit = max(__popc(__ballot_sync(~0u, below)) - 1, 0);
+        s += hit * step;
+        n = min(step, n - hit * step);
+    }
+    const int64_t row0 = max64(0, g.step.token_offsets[s]);
+    const int new_rows = static_cast<int>(
+        max64(0, min64(min64(g.step.token_offsets[s + 1], g.step.tokens) - row0, INT_MAX / g.group)) * g.group);
+    const int64_t tile_index = item - ((row0 * g.group >> 7) + s);
+    if (tile_index < 0 || tile_index * C::kRows >= new_rows) return;
+    const int first_row = static_cast<int>(tile_index) * C::kRows;
+    const int rows = min(C::kRows, new_rows - first_row);
+    const int context = g.step.context[s];
+    const int64_t held = min64(g.step.page_offsets[s + 1] - g.step.page_offsets[s], g.step.max_pages);
+    const int keys = static_cast<int>(max64(0, min64(min64(held << g.shift, g.step.lengths[s]),
+                                                     (int64_t)context + (first_row + rows - 1) / g.group + 1)));
+    const int tiles = (keys + C::kKeys - 1) / C::kKeys;
+
+    if (tid == 0) {
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(&k_full[i], 4);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 4);
+            mbar_init(&v_empty[i], 1);
+        }
+        mbar_init(s_full, 1);
+        mbar_init(p_full, 4);
+        mbar_init(o_full, 1);
+        fence_barrier_init();
+    }
+    if (warp == 7) {
+        tmem_alloc(tmem_holder, C::kTmemCols);
+        tmem_relinquish();
+    }
+    {
+        // The rows: D / 8 lanes per row, eight values each, rotated, scaled by
+        // the row's power of two, split, stored swizzled (warps 0-7).
+        constexpr int kLanes = D / 8;  // 4, 8, 12, 16: a row's lanes are in one warp
+        constexpr int kRowsAtOnce = 32 / kLanes;
+        const int sub = lane / kLanes, j = lane - sub * kLanes;
+        for (int base = warp * kRowsAtOnce; base < C::kRows; base += 8 * kRowsAtOnce) {
+            const int r = base + sub;
+            const bool live = sub < kRowsAtOnce && r < C::kRows;
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
+            int at = 4 * j, to = at + D / 2;
+            if (live && r < rows) {
+                const int t = (first_row + r) / g.group, hq = (first_row + r) - t * g.group;
+                int64_t pos = (int64_t)context + t;
+                if (g.rotary > 0 && (pos < 0 || pos >= g.table_rows)) {
+                    if (j == 0) report(watch, kSiteKv8Range);
+                    pos = 0;
+                }
+                query_item<D>(g, g.q + (row0 + t) * g.q_stride + (int64_t)(h * g.group + hq) * D, j, pos, at, to, a, b);
+            }
+            uint32_t largest = 0;
+            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) largest = max(largest, __float_as_uint(v[e]) & 0x7fffffffu);
+            if constexpr (kLanes == 12) {
+                uint32_t all = 0;
+#pragma unroll
+                for (int e = 0; e < kLanes; ++e) all = max(all, __shfl_sync(~0u, largest, min(sub * kLanes + e, 31)));
+                largest = all;
+            } else {
+#pragma unroll
+                for (int d = kLanes / 2; d > 0; d >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, d));
+            }
+            float up, down;
+            row_power(largest, up, down);
+            if (live) {
+                if (j == 0) factor_s[r] = down * g.scale * kLog2e;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int d = half == 0 ? at : to;
+                    const float x0 = v[4 * half] * up, x1 = v[4 * half + 1] * up, x2 = v[4 * half + 2] * up, x3 = v[4 * half + 3] * up;
+                    uint2 hi, lo;
+                    hi.x = half2_bits(x0, x1);
+                    hi.y = half2_bits(x2, x3);
+                    const __half2 h01 = *reinterpret_cast<const __half2*>(&hi.x), h23 = *reinterpret_cast<const __half2*>(&hi.y);
+                    lo.x = half2_bits(x0 - __low2float(h01), x1 - __high2float(h01));
+                    lo.y = half2_bits(x2 - __low2float(h23), x3 - __high2float(h23));
+                    const int offset = (d >> 6) * (C::kRows * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2;
+                    *reinterpret_cast<uint2*>(q_hi + offset) = hi;
+                    *reinterpret_cast<uint2*>(q_lo + offset) = lo;
+                }
+            }
+        }
+        fence_proxy_async_smem();
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    const uint32_t s_tmem = tmem, o_tmem = tmem + C::kKeys;
+
+    if (warp < 4) {
+        // ------------------------------------------- softmax and MMA issue
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
+        constexpr uint32_t s_desc = umma_idesc_f16(C::kRows, C::kKeys, false), o_desc = umma_idesc_f16(C::kRows, C::kOutCols, true);
+        const uint32_t qh = smem_u32(q_hi), ql = smem_u32(q_lo), kt = smem_u32(k_tiles), vt = smem_u32(v_tiles);
+        const auto scores = [&](int j) {  // S of tile j (thread 0)
+            const int stage = j % C::kStages;
+            if (!tile_wait(watch, &k_full[stage], (j / C::kStages) & 1)) return;
+            tcgen05_fence_after();
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                    umma_f16(s_tmem,
+                             umma_desc_k_sw128((part == 0 ? ql : qh) + (i >> 2) * (C::kRows * 128)) + 2 * (i & 3),
+                             umma_desc_k_sw128(kt + stage * C::kKvBytes + (i >> 2) * (C::kKeys * 128)) + 2 * (i & 3), s_desc,
+                             part > 0 || i > 0);
+            umma_commit(&k_empty[stage]);
+            umma_commit(s_full);
+        };
+        const auto values = [&](int j) {  // O += P V of tile j (thread 0)
+            const int stage = j % C::kStages;
+            if (!tile_wait(watch, &v_full[stage], (j / C::kStages) & 1)) return;
+            tcgen05_fence_after();
+#pragma unroll
+            for (int i = 0; i < C::kKeys / 16; ++i)
+#pragma unroll
+                for (int part = 0; part < 2; ++part)
+                    umma_f16_ta(o_tmem, s_tmem + (i >> 1) * 32 + part * 16 + (i & 1) * 8,
+                                umma_desc_mn_sw128(vt + stage * C::kKvBytes + i * 2048, C::kKeys * 128), o_desc,
+                                j % C::kSpan > 0 || i > 0 || part > 0);
+            umma_commit(&v_empty[stage]);
+        };
+        if (tid == 0 && tiles > 0) scores(0);
+        __syncwarp();
+
+        const int r = tid;
+        const int64_t pos = (int64_t)context + (first_row + r) / g.group;
+        const bool seen = r < rows && pos >= 0 && (g.rotary == 0 || pos < g.table_rows);
+        const int limit = seen ? static_cast<int>(min64(keys, pos + 1)) : 0;
+        const float factor = factor_s[r];
+        const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+        float m = -INFINITY, l = 0.0f, m_sum = -INFINITY;
+        float o_sum[C::kOutCols];  // the rounded sum, relative to m_sum; indexed at run time: local memory
+        // Adds O, complete up to the tile before, to it.
+        const auto add_o = [&](bool first) {
+            const float old = first || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m);
+            m_sum = m;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t y[32];
+                tmem_ld_32x32b_x32(o_tmem + lanes + 32 * c, y);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    o_sum[32 * c + e] = first ? __uint_as_float(y[e]) : fmaf(o_sum[32 * c + e], old, __uint_as_float(y[e]));
+            }
+        };
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            ok = __all_sync(~0u, tile_wait(watch, s_full, j & 1));
+            if (!ok) break;
+            tcgen05_fence_after();
+            const bool anew = j % C::kSpan == 0;
+            if (anew && j > 0) add_o(j == C::kSpan);
+            uint32_t x[C::kKeys];
+#pragma unroll
+            for (int c = 0; c < C::kKeys / 32; ++c)
+                tmem_ld_32x32b_x32(s_tmem + lanes + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
+            const float4* scales = info + (j % C::kInfo) * C::kGroups;
+            const int visible = limit - j * C::kKeys;  // columns of this tile that the row sees
+            const bool whole = __all_sync(~0u, visible >= C::kKeys);
+            tmem_wait_ld();
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < C::kKeys; ++e)
+                    if (e >= visible) x[e] = 0xff800000u;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < C::kGroups; ++n) {
+                const float* at = reinterpret_cast<const float*>(x) + 16 * n;
+                float most = fmaxf(at[0], at[1]);
+#pragma unroll
+                for (int e = 2; e < 16; e += 2) most = max3(most, at[e], at[e + 1]);
+                const float4 scale = scales[n];
+                // A column that is not seen stays -inf whatever the scale.
+                const float value = fmaf(most, scale.x * factor, scale.y);
+                top = fmaxf(top, most == -INFINITY ? most : value);
+            }
+            if (anew) {
+                // O starts anew with this tile: only L has a reference to keep.
+                const float grown = fmaxf(m, top);
+                l *= m == -INFINITY ? 0.0f : ex2(m - grown);
+                m = grown;
+            } else if (__any_sync(~0u, top > m + kSlack)) {
+                // PV of the tile before has completed with this tile's S.
+                const float grown = top > m + kSlack ? top : m;
+                const float old = m == -INFINITY ? 0.0f : ex2(m - grown);
+                m = grown;
+                l *= old;
+#pragma unroll 1
+                for (int c = 0; c < C::kOutCols / 32; ++c) {
+                    uint32_t y[32];
+                    tmem_ld_32x32b_x32(o_tmem + lanes + 32 * c, y);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * old);
+                    tmem_st_32x32b_x32(o_tmem + lanes + 32 * c, y);
+                }
+            }
+            const float shift = m == -INFINITY ? 0.0f : m - kTileLift;
+#pragma unroll
+            for (int c = 0; c < C::kKeys / 32; ++c) {
+                uint32_t p[32];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float4 scale = scales[2 * c + half];
+                    const unsigned long long a = pack2(scale.x * factor, scale.x * factor);
+                    const unsigned long long b = pack2(scale.y - shift, scale.y - shift);
+                    unsigned long long sum = 0;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const int at = 32 * c + 16 * half + e;
+                        const float2 y = unpack2(fma2(pack2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), a, b));
+                        float w0 = ex2(y.x), w1 = ex2(y.y);
+                        if (!whole) {  // -inf times a scale of zero is no number
+                            w0 = at >= visible ? 0.0f : w0;
+                            w1 = at + 1 >= visible ? 0.0f : w1;
+                        }
+                        const unsigned long long w = pack2(w0, w1);
+                        sum = add2(sum, w);
+                        const float h0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u);
+                        const float h1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
+                        const float2 low = unpack2(sub2(w, pack2(h0, h1)));
+                        p[8 * half + e / 2] = half2_bits(h0, h1);
+                        p[16 + 8 * half + e / 2] = half2_bits(low.x, low.y);
+                    }
+                    const float2 both = unpack2(sum);
+                    l = fmaf(both.x + both.y, scale.z, l);
+                }
+                tmem_st_32x32b_x32(s_tmem + lanes + 32 * c, p);
+            }
+            tmem_wait_st();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full);
+            if (tid == 0 && tile_wait(watch, p_full, j & 1)) {
+                tcgen05_fence_after();
+                values(j);
+                if (j + 1 < tiles) scores(j + 1);
+            }
+            __syncwarp();
+        }
+        if (tid == 0 && tiles > 0) umma_commit(o_full);  // whatever was issued has completed before the block ends
+        __syncwarp();
+        if (tiles > 0) tile_wait(watch, o_full, 0);
+        __syncwarp();
+        tcgen05_fence_after();
+        const bool summed = tiles > C::kSpan;
+        const float old = !summed || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m);
+        // Out through shared memory (Q's, no longer read): whole rows per store.
+        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+        uint8_t* stage = smem + warp * (32 * D * 4);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+            uint32_t x[32];
+            if (tiles > 0) {
+                tmem_ld_32x32b_x32(o_tmem + lanes + 32 * c, x);
+                tmem_wait_ld();
+                if (summed) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(fmaf(o_sum[32 * c + e], old, __uint_as_float(x[e])));
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (tiles > 0 && l != 0.0f)
+                    y = make_float4(__uint_as_float(x[e]) * inverse, __uint_as_float(x[e + 1]) * inverse,
+                                    __uint_as_float(x[e + 2]) * inverse, __uint_as_float(x[e + 3]) * inverse);
+                const int piece = 8 * c + e / 4;  // of the row's D / 4
+                *reinterpret_cast<float4*>(stage + lane * (D * 4) + ((piece ^ (lane & 7)) << 4)) = y;
+            }
+        }
+        __syncwarp();
+        for (int i = lane; i < 32 * (D / 4); i += 32) {
+            const int rr = i / (D / 4), piece = i - rr * (D / 4);
+            const int row = warp * 32 + rr;
+            if (row >= rows) break;
+            const float4 y = *reinterpret_cast<const float4*>(stage + rr * (D * 4) + ((piece ^ (rr & 7)) << 4));
+            const int t = (first_row + row) / g.group, hq = (first_row + row) - t * g.group;
+            *reinterpret_cast<float4*>(g.out + (row0 + t) * (int64_t)g.heads * D + (int64_t)(h * g.group + hq) * D + 4 * piece) = y;
+        }
+    } else {
+        // ---------------------------------------------- codes to fp16
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kConvertRegs));
+        const int ct = tid - 128;
+        constexpr int kRowPieces = D / 16;
+        const int32_t* table = g.step.table + (int64_t)s * g.step.max_pages;
+        const int page = 1 << g.shift;
+        // The page of this thread's piece n of tile j, -1 where there is no key.
+        const auto page_of = [&](int j, int n) {
+            const int key = j * C::kKeys + (n * 128 + ct) / kRowPieces;
+            return key < keys ? table[key >> g.shift] : INT_MIN;
+        };
+        const auto fetch = [&](int j, const int32_t (&ids)[C::kPieces], const int8_t* codes, uint4 (&w)[C::kPieces]) {
+#pragma unroll
+            for (int n = 0; n < C::kPieces; ++n) {
+                const int row = (n * 128 + ct) / kRowPieces, cc = (n * 128 + ct) % kRowPieces;
+                const int key = j * C::kKeys + row;
+                w[n] = make_uint4(0u, 0u, 0u, 0u);
+                if (ids[n] >= 0 && ids[n] < g.cache.pages)
+                    w[n] = __ldg(reinterpret_cast<const uint4*>(
+                        codes + ((((int64_t)ids[n] * g.cache.kv_heads + h) << g.shift) + (key & (page - 1))) * D + cc * 16));
+            }
+        };
+        const auto convert = [&](const uint4 (&w)[C::kPieces], uint8_t* tile) {
+#pragma unroll
+            for (int n = 0; n < C::kPieces; ++n) {
+                const int row = (n * 128 + ct) / kRowPieces, cc = (n * 128 + ct) % kRowPieces;
+                const uint32_t b[4] = {w[n].x ^ 0x80808080u, w[n].y ^ 0x80808080u, w[n].z ^ 0x80808080u, w[n].w ^ 0x80808080u};
+                uint8_t* line = tile + (cc >> 2) * (C::kKeys * 128) + row * 128;
+                const int chunk = (cc & 3) * 2;
+                *reinterpret_cast<uint4*>(line + ((chunk ^ (row & 7)) << 4)) =
+                    make_uint4(codes_half2(b[0], 0x4140u), codes_half2(b[0], 0x4342u), codes_half2(b[1], 0x4140u), codes_half2(b[1], 0x4342u));
+                *reinterpret_cast<uint4*>(line + (((chunk + 1) ^ (row & 7)) << 4)) =
+                    make_uint4(codes_half2(b[2], 0x4140u), codes_half2(b[2], 0x4342u), codes_half2(b[3], 0x4140u), codes_half2(b[3], 0x4342u));
+            }
+        };
+        // Loads run a tile ahead (page numbers two): K of tile j + 1 is asked for
+        // once K of tile j is converted, V likewise.
+        int32_t ids[C::kPieces];
+        uint4 k[C::kPieces], v[C::kPieces];
+        int32_t group_id = INT_MIN;  // page of 16-key group ct, in the first lanes
+        float ks = 0.0f, vs = 0.0f;
+        const auto group_page = [&](int j) {
+            const int key = j * C::kKeys + 16 * ct;
+            return ct < C::kGroups && key < keys ? table[key >> g.shift] : INT_MIN;
+        };
+        const auto fetch_scales = [&](int32_t id) {
+            ks = vs = 0.0f;
+            if (id >= 0 && id < g.cache.pages) {
+                const int64_t at = (int64_t)id * g.cache.kv_heads + h;
+                ks = __ldg(g.cache.k_scales + at);
+                vs = __ldg(g.cache.v_scales + at);
+            } else if (id != INT_MIN) {
+                report(watch, kSiteKv8Range);
+            }
+        };
+#pragma unroll
+        for (int n = 0; n < C::kPieces; ++n) ids[n] = page_of(0, n);
+        group_id = group_page(0);
+        fetch(0, ids, g.cache.k_codes, k);
+        fetch(0, ids, g.cache.v_codes, v);
+        fetch_scales(group_id);
+        bool there = group_id >= 0 && group_id < g.cache.pages;
+#pragma unroll
+        for (int n = 0; n < C::kPieces; ++n) ids[n] = page_of(1, n);
+        group_id = group_page(1);
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            const int stage = j % C::kStages;
+            const uint32_t reuse = ((j / C::kStages) - 1) & 1;
+            if (j >= C::kStages) ok = __all_sync(~0u, tile_wait(watch, &k_empty[stage], reuse));
+            if (!ok) break;
+            convert(k, k_tiles + stage * C::kKvBytes);
+            if (ct < C::kGroups) {
+                float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);  // hides the group
+                // A page of zeros counts in the sum as any other.
+                if (there) f = vs == 0.0f ? make_float4(ks, -126.0f, 0x1p126f, 0.0f) : make_float4(ks, log2f(vs), 1.0f / vs, 0.0f);
+                info[(j % C::kInfo) * C::kGroups + ct] = f;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&k_full[stage]);
+            if (j + 1 < tiles) {
+                fetch(j + 1, ids, g.cache.k_codes, k);
+                fetch_scales(group_id);
+                there = group_id >= 0 && group_id < g.cache.pages;
+            }
+            if (j >= C::kStages) ok = __all_sync(~0u, tile_wait(watch, &v_empty[stage], reuse));
+            if (!ok) break;
+            convert(v, v_tiles + stage * C::kKvBytes);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_full[stage]);
+            if (j + 1 < tiles) {
+                fetch(j + 1, ids, g.cache.v_codes, v);
+#pragma unroll
+                for (int n = 0; n < C::kPieces; ++n) ids[n] = page_of(j + 2, n);
+                group_id = group_page(j + 2);
+            }
+        }
+    }
+    __syncwarp();
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == 7) {
+        tcgen05_fence_after();
+        tmem_dealloc(tmem, C::kTmemCols);
+    }
+}
+
+template <int D>
+int run_tile(cudaStream_t s, const Kv8AttendArgs& g, bool pdl) {
+    DeviceWatch watch;
+    int st = device_watch(&watch);
+    if (st) return st;
+    const int64_t row_tiles = (g.step.tokens * g.group >> 7) + g.step.requests;
+    if (row_tiles * g.cache.kv_heads > INT_MAX) {
+        set_error("leafq_kv8_attention: too many rows");
+        return LEAFQ_ERR_INVALID;
+    }
+    const void* kernel = reinterpret_cast<const void*>(kv8_attend_tile_kernel<D>);
+    static const int registers = [kernel] {
+        cudaFuncAttributes a;
+        return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (registers != 128) {  // setmaxnreg would wait for registers that the launch does not have
+        set_error("leafq_kv8_attention: the tile kernel was built with " + std::to_string(registers) + " registers a thread, not 128");
+        return LEAFQ_ERR_CUDA;
+    }
+    st = allow_smem(kernel, TileShape<D>::kSmem, "leafq_kv8_attention");
+    if (st) return st;
+    return launch(kv8_attend_tile_kernel<D>, dim3(static_cast<unsigned>(row_tiles * g.cache.kv_heads)),
+                  dim3(TileShape<D>::kThreads), TileShape<D>::kSmem, s, pdl, "leafq_kv8_attention", g, watch,
+                  static_cast<int>(row_tiles));
+}
+
+}  // namespace
+
+int launch_kv8_tiles(cudaStream_t s, const Kv8AttendArgs& g, bool pdl) {
+    switch (g.cache.dim) {
+        case 32: return run_tile<32>(s, g, pdl);
+        case 64: return run_tile<64>(s, g, pdl);
+        case 96: return run_tile<96>(s, g, pdl);
+        default: return run_tile<128>(s, g, pdl);
+    }
+}
+
+}  // namespace leafq

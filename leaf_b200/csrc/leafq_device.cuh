@@ -22,6 +22,9 @@
 
 namespace leafq {
 
+// A file compiled as a whole program (LEAFQ_WHOLE_PROGRAM) cannot see the
+// library's device variables; its kernels get their addresses (device_watch).
+#ifndef LEAFQ_WHOLE_PROGRAM
 // Error word written by kernels whose waits time out (first writer wins).
 // Codes: 0 = fine; otherwise (site << 16) | (blockIdx.x & 0xffff).
 extern __device__ unsigned int g_device_error;
@@ -35,6 +38,7 @@ constexpr unsigned long long kDefaultWaitLimitNs = 2000000000ull;
 extern __device__ unsigned long long g_wait_limit_ns;
 
 __device__ __forceinline__ unsigned long long wait_limit_ns() { return g_wait_limit_ns; }
+#endif
 
 enum WaitSite : unsigned {
     kSiteGemvFull = 1,
@@ -61,6 +65,7 @@ __device__ __forceinline__ unsigned long long global_timer_ns() {
     return t;
 }
 
+#ifndef LEAFQ_WHOLE_PROGRAM
 __device__ __forceinline__ void record_device_error(unsigned site) {
     atomicCAS(&g_device_error, 0u, (site << 16) | (blockIdx.x & 0xffffu));
 }
@@ -68,6 +73,7 @@ __device__ __forceinline__ void record_device_error(unsigned site) {
 __device__ __forceinline__ bool device_error_raised() {
     return *((volatile unsigned int*)&g_device_error) != 0u;
 }
+#endif
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -116,6 +122,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
     return done != 0;
 }
 
+#ifndef LEAFQ_WHOLE_PROGRAM
 // Bounded wait for the phase with the given parity to complete.  Returns
 // false (after recording `site`) when the limit passes or another block has
 // already reported an error.
@@ -133,6 +140,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
         }
     }
 }
+#endif
 
 // ------------------------------------------------------ bulk (TMA) copies
 __device__ __forceinline__ uint64_t l2_policy_evict_first() {

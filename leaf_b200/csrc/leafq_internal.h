@@ -22,6 +22,14 @@ int sm_count();
 // Opt-in dynamic shared memory per block of the current device (cached).
 int max_smem_per_block();
 
+// The current device's error word and wait limit, for kernels of files that
+// are compiled as whole programs (addresses cached per device).
+struct DeviceWatch {
+    unsigned int* error;
+    const unsigned long long* limit_ns;
+};
+int device_watch(DeviceWatch* watch);
+
 // Launch `kernel` with grid/block/smem on `stream`, with the programmatic
 // stream serialisation attribute when `pdl`.  Returns LEAFQ_OK or
 // LEAFQ_ERR_CUDA.
