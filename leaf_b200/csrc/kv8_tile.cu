@@ -3,6 +3,8 @@
 // Compiled as a whole program (build.py): setmaxnreg is ignored in relocatable
 // device code.
 #define LEAFQ_WHOLE_PROGRAM
+#include <type_traits>
+
 #include "kv8_attention.cuh"
 
 namespace leafq {
@@ -352,37 +354,41 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
                 }
             }
             const float shift = m == -INFINITY ? 0.0f : m - kTileLift;
+            const auto weigh = [&](auto masked) {
 #pragma unroll
-            for (int c = 0; c < C::kKeys / 32; ++c) {
-                uint32_t p[32];
+                for (int c = 0; c < C::kKeys / 32; ++c) {
+                    uint32_t p[32];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const float4 scale = scales[2 * c + half];
-                    const unsigned long long a = pack2(scale.x * factor, scale.x * factor);
-                    const unsigned long long b = pack2(scale.y - shift, scale.y - shift);
-                    unsigned long long sum = 0;
+                    for (int half = 0; half < 2; ++half) {
+                        const float4 scale = scales[2 * c + half];
+                        const unsigned long long a = pack2(scale.x * factor, scale.x * factor);
+                        const unsigned long long b = pack2(scale.y - shift, scale.y - shift);
+                        unsigned long long sum = 0;
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const int at = 32 * c + 16 * half + e;
-                        const float2 y = unpack2(fma2(pack2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), a, b));
-                        float w0 = ex2(y.x), w1 = ex2(y.y);
-                        if (!whole) {  // -inf times a scale of zero is no number
-                            w0 = at >= visible ? 0.0f : w0;
-                            w1 = at + 1 >= visible ? 0.0f : w1;
+                        for (int e = 0; e < 16; e += 2) {
+                            const int at = 32 * c + 16 * half + e;
+                            const float2 y = unpack2(fma2(pack2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), a, b));
+                            float w0 = ex2(y.x), w1 = ex2(y.y);
+                            if constexpr (decltype(masked)::value) {  // -inf times a scale of zero is no number
+                                w0 = at >= visible ? 0.0f : w0;
+                                w1 = at + 1 >= visible ? 0.0f : w1;
+                            }
+                            const unsigned long long w = pack2(w0, w1);
+                            sum = add2(sum, w);
+                            const float h0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u);
+                            const float h1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
+                            const float2 low = unpack2(sub2(w, pack2(h0, h1)));
+                            p[8 * half + e / 2] = half2_bits(h0, h1);
+                            p[16 + 8 * half + e / 2] = half2_bits(low.x, low.y);
                         }
-                        const unsigned long long w = pack2(w0, w1);
-                        sum = add2(sum, w);
-                        const float h0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u);
-                        const float h1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
-                        const float2 low = unpack2(sub2(w, pack2(h0, h1)));
-                        p[8 * half + e / 2] = half2_bits(h0, h1);
-                        p[16 + 8 * half + e / 2] = half2_bits(low.x, low.y);
+                        const float2 both = unpack2(sum);
+                        l = fmaf(both.x + both.y, scale.z, l);
                     }
-                    const float2 both = unpack2(sum);
-                    l = fmaf(both.x + both.y, scale.z, l);
+                    tmem_st_32x32b_x32(s_tmem + lanes + 32 * c, p);
                 }
-                tmem_st_32x32b_x32(s_tmem + lanes + 32 * c, p);
-            }
+            };
+            if (whole) weigh(std::false_type{});
+            else weigh(std::true_type{});
             tmem_wait_st();
             tcgen05_fence_before();
             __syncwarp();
@@ -441,20 +447,24 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
         constexpr int kRowPieces = D / 16;
         const int32_t* table = g.step.table + (int64_t)s * g.step.max_pages;
         const int page = 1 << g.shift;
+        const int64_t page_bytes = ((int64_t)g.cache.kv_heads << g.shift) * D, head_bytes = ((int64_t)h << g.shift) * D;
         // The page of this thread's piece n of tile j, -1 where there is no key.
         const auto page_of = [&](int j, int n) {
             const int key = j * C::kKeys + (n * 128 + ct) / kRowPieces;
             return key < keys ? table[key >> g.shift] : INT_MIN;
         };
-        const auto fetch = [&](int j, const int32_t (&ids)[C::kPieces], const int8_t* codes, uint4 (&w)[C::kPieces]) {
+        const auto fetch = [&](const int8_t* codes, const int64_t (&from)[C::kPieces], uint4 (&w)[C::kPieces]) {
+#pragma unroll
+            for (int n = 0; n < C::kPieces; ++n)
+                w[n] = from[n] >= 0 ? __ldg(reinterpret_cast<const uint4*>(codes + from[n])) : make_uint4(0u, 0u, 0u, 0u);
+        };
+        // Byte offsets of the pieces of tile j, whose pages are ids.
+        const auto locate = [&](int j, const int32_t (&ids)[C::kPieces], int64_t (&from)[C::kPieces]) {
 #pragma unroll
             for (int n = 0; n < C::kPieces; ++n) {
                 const int row = (n * 128 + ct) / kRowPieces, cc = (n * 128 + ct) % kRowPieces;
-                const int key = j * C::kKeys + row;
-                w[n] = make_uint4(0u, 0u, 0u, 0u);
-                if (ids[n] >= 0 && ids[n] < g.cache.pages)
-                    w[n] = __ldg(reinterpret_cast<const uint4*>(
-                        codes + ((((int64_t)ids[n] * g.cache.kv_heads + h) << g.shift) + (key & (page - 1))) * D + cc * 16));
+                const int inside = ((j * C::kKeys + row) & (page - 1)) * D + cc * 16;
+                from[n] = static_cast<uint32_t>(ids[n]) < static_cast<uint32_t>(g.cache.pages) ? ids[n] * page_bytes + (head_bytes + inside) : -1;
             }
         };
         const auto convert = [&](const uint4 (&w)[C::kPieces], uint8_t* tile) {
@@ -473,6 +483,7 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
         // Loads run a tile ahead (page numbers two): K of tile j + 1 is asked for
         // once K of tile j is converted, V likewise.
         int32_t ids[C::kPieces];
+        int64_t from[C::kPieces];
         uint4 k[C::kPieces], v[C::kPieces];
         int32_t group_id = INT_MIN;  // page of 16-key group ct, in the first lanes
         float ks = 0.0f, vs = 0.0f;
@@ -493,8 +504,9 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
 #pragma unroll
         for (int n = 0; n < C::kPieces; ++n) ids[n] = page_of(0, n);
         group_id = group_page(0);
-        fetch(0, ids, g.cache.k_codes, k);
-        fetch(0, ids, g.cache.v_codes, v);
+        locate(0, ids, from);
+        fetch(g.cache.k_codes, from, k);
+        fetch(g.cache.v_codes, from, v);
         fetch_scales(group_id);
         bool there = group_id >= 0 && group_id < g.cache.pages;
 #pragma unroll
@@ -517,7 +529,8 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
             __syncwarp();
             if (lane == 0) mbar_arrive(&k_full[stage]);
             if (j + 1 < tiles) {
-                fetch(j + 1, ids, g.cache.k_codes, k);
+                locate(j + 1, ids, from);
+                fetch(g.cache.k_codes, from, k);
                 fetch_scales(group_id);
                 there = group_id >= 0 && group_id < g.cache.pages;
             }
@@ -528,7 +541,7 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[stage]);
             if (j + 1 < tiles) {
-                fetch(j + 1, ids, g.cache.v_codes, v);
+                fetch(g.cache.v_codes, from, v);
 #pragma unroll
                 for (int n = 0; n < C::kPieces; ++n) ids[n] = page_of(j + 2, n);
                 group_id = group_page(j + 2);
