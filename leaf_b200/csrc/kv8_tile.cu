@@ -15,11 +15,12 @@ namespace {
 // walks the keys in tiles, and two blocks share an SM, so that one's MMAs run
 // under the other's softmax.  Roles:
 //   warps 0-3  softmax: one row per thread (its TMEM lane), a tile's scores in
-//              registers; thread 0 issues the MMAs (kind::f16, fp32
-//              accumulators in TMEM)
-//   warps 4-7  codes to fp16: 16-byte global loads one tile ahead, byte
+//              registers
+//   warps 4-6  codes to fp16: 16-byte global loads a tile ahead, byte
 //              permutes, 128-byte-swizzled shared memory
-// The softmax warps take registers that the converting ones leave (setmaxnreg).
+//   warp 7     MMA issue (kind::f16, fp32 accumulators in TMEM)
+// The softmax warps take registers that the others leave (setmaxnreg).  S has
+// two buffers: the next tile's scores are computed under this tile's softmax.
 // The arithmetic is the split form's: codes exact in fp16, fp32 operands as
 // hi + lo halves, the V scale in the exponent.
 //   S [128][keys] = Qhi K^T + Qlo K^T   Q and K K-major in shared memory
@@ -36,23 +37,26 @@ constexpr float kTileLift = 6.0f, kSlack = 8.0f;
 template <int D>
 struct TileShape {
     static constexpr int kRows = 128;
-    static constexpr int kKeys = D <= 64 ? 128 : 64;
+    static constexpr int kKeys = D <= 64 ? 96 : 64;
     static constexpr int kBlocks = (D + 63) / 64;        // 64-element (128-byte) column blocks
     static constexpr int kStages = D <= 64 ? 2 : 1;      // of K and of V
     static constexpr int kGroups = kKeys / 16;           // of keys that share a page for certain
-    static constexpr int kInfo = 4;                      // ring of the groups' scales
+    static constexpr int kInfo = 4;                      // ring of the groups' scales: a tile's are read while those of
+                                                         // up to kStages + 1 later tiles are written
     static constexpr int kQBytes = kBlocks * kRows * 128;
     static constexpr int kKvBytes = kBlocks * kKeys * 128;
     static constexpr int kSpan = 512 / kKeys;            // tiles between O's additions to the rounded sum
     static constexpr int kThreads = 256;
-    static constexpr int kSoftmaxRegs = 184, kConvertRegs = 72;
-    static constexpr int kPieces = kKeys * D / 16 / 128; // 16-byte pieces of a K (or V) tile per converting thread
+    static constexpr int kSoftmaxRegs = 168, kOtherRegs = 88;
+    static constexpr int kConverters = 96;
+    static constexpr int kAllPieces = kKeys * D / 16;    // 16-byte pieces of a K (or V) tile
+    static constexpr int kPieces = (kAllPieces + kConverters - 1) / kConverters;
     static constexpr int kOutCols = kBlocks * 64;        // O columns (those past D are not read)
     static constexpr uint32_t kTmemCols = 256;
     static constexpr size_t kSmem = 1024 + 2 * kQBytes + 2 * kStages * kKvBytes + kInfo * kGroups * 16 + kRows * 4 + 256;
-    static_assert(kKeys + kOutCols <= 256, "two blocks share the SM's 512 TMEM columns");
+    static_assert(2 * kKeys + kOutCols <= 256, "two blocks share the SM's 512 TMEM columns");
     static_assert(2 * kQBytes >= kRows * D * 4, "the output leaves through Q's shared memory");
-    static_assert(128 * (kSoftmaxRegs + kConvertRegs) == kThreads * 128, "the split of what the launch gives (128 a thread)");
+    static_assert(128 * (kSoftmaxRegs + kOtherRegs) == kThreads * 128, "the split of what the launch gives (128 a thread)");
 };
 
 // The library's device error word and wait limit (leafq_device.cuh), which this
@@ -110,6 +114,23 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Loads of read-only data that stay where they are written, ahead of their use.
+__device__ __forceinline__ uint4 load_now(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ int32_t load_now(const int32_t* p) {
+    int32_t v;
+    asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float load_now(const float* p) {
+    float v;
+    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -131,10 +152,11 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
     uint64_t* k_empty = k_full + C::kStages;
     uint64_t* v_full = k_empty + C::kStages;
     uint64_t* v_empty = v_full + C::kStages;
-    uint64_t* s_full = v_empty + C::kStages;
-    uint64_t* p_full = s_full + 1;
-    uint64_t* o_full = p_full + 1;
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_full + 1);
+    uint64_t* s_full = v_empty + C::kStages;  // by S buffer, as p_full
+    uint64_t* p_full = s_full + 2;
+    uint64_t* o_done = p_full + 2;            // PV of a tile has completed
+    uint64_t* drained = o_done + 1;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     grid_dependency_wait();
     grid_launch_dependents();
@@ -167,14 +189,17 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
 
     if (tid == 0) {
         for (int i = 0; i < C::kStages; ++i) {
-            mbar_init(&k_full[i], 4);
+            mbar_init(&k_full[i], 3);
             mbar_init(&k_empty[i], 1);
-            mbar_init(&v_full[i], 4);
+            mbar_init(&v_full[i], 3);
             mbar_init(&v_empty[i], 1);
         }
-        mbar_init(s_full, 1);
-        mbar_init(p_full, 4);
-        mbar_init(o_full, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+        }
+        mbar_init(o_done, 1);
+        mbar_init(drained, 1);
         fence_barrier_init();
     }
     if (warp == 7) {
@@ -240,44 +265,11 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem = *tmem_holder;
-    const uint32_t s_tmem = tmem, o_tmem = tmem + C::kKeys;
+    const uint32_t o_tmem = tmem + 2 * C::kKeys;
 
     if (warp < 4) {
-        // ------------------------------------------- softmax and MMA issue
+        // ------------------------------------------------------- softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
-        constexpr uint32_t s_desc = umma_idesc_f16(C::kRows, C::kKeys, false), o_desc = umma_idesc_f16(C::kRows, C::kOutCols, true);
-        const uint32_t qh = smem_u32(q_hi), ql = smem_u32(q_lo), kt = smem_u32(k_tiles), vt = smem_u32(v_tiles);
-        const auto scores = [&](int j) {  // S of tile j (thread 0)
-            const int stage = j % C::kStages;
-            if (!tile_wait(watch, &k_full[stage], (j / C::kStages) & 1)) return;
-            tcgen05_fence_after();
-#pragma unroll
-            for (int part = 0; part < 2; ++part)
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    umma_f16(s_tmem,
-                             umma_desc_k_sw128((part == 0 ? ql : qh) + (i >> 2) * (C::kRows * 128)) + 2 * (i & 3),
-                             umma_desc_k_sw128(kt + stage * C::kKvBytes + (i >> 2) * (C::kKeys * 128)) + 2 * (i & 3), s_desc,
-                             part > 0 || i > 0);
-            umma_commit(&k_empty[stage]);
-            umma_commit(s_full);
-        };
-        const auto values = [&](int j) {  // O += P V of tile j (thread 0)
-            const int stage = j % C::kStages;
-            if (!tile_wait(watch, &v_full[stage], (j / C::kStages) & 1)) return;
-            tcgen05_fence_after();
-#pragma unroll
-            for (int i = 0; i < C::kKeys / 16; ++i)
-#pragma unroll
-                for (int part = 0; part < 2; ++part)
-                    umma_f16_ta(o_tmem, s_tmem + (i >> 1) * 32 + part * 16 + (i & 1) * 8,
-                                umma_desc_mn_sw128(vt + stage * C::kKvBytes + i * 2048, C::kKeys * 128), o_desc,
-                                j % C::kSpan > 0 || i > 0 || part > 0);
-            umma_commit(&v_empty[stage]);
-        };
-        if (tid == 0 && tiles > 0) scores(0);
-        __syncwarp();
-
         const int r = tid;
         const int64_t pos = (int64_t)context + (first_row + r) / g.group;
         const bool seen = r < rows && pos >= 0 && (g.rotary == 0 || pos < g.table_rows);
@@ -292,21 +284,31 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
             m_sum = m;
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
+                float z[32];
                 uint32_t y[32];
                 tmem_ld_32x32b_x32(o_tmem + lanes + 32 * c, y);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) z[e] = first ? 0.0f : o_sum[32 * c + e];
                 tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    o_sum[32 * c + e] = first ? __uint_as_float(y[e]) : fmaf(o_sum[32 * c + e], old, __uint_as_float(y[e]));
+                for (int e = 0; e < 32; ++e) o_sum[32 * c + e] = fmaf(z[e], old, __uint_as_float(y[e]));
             }
         };
         bool ok = true;
         for (int j = 0; j < tiles; ++j) {
-            ok = __all_sync(~0u, tile_wait(watch, s_full, j & 1));
+            const uint32_t s_tmem = tmem + (j & 1) * C::kKeys;
+            ok = __all_sync(~0u, tile_wait(watch, &s_full[j & 1], (j >> 1) & 1));
             if (!ok) break;
             tcgen05_fence_after();
             const bool anew = j % C::kSpan == 0;
-            if (anew && j > 0) add_o(j == C::kSpan);
+            // This tile's S means that PV of tile j - 2 is done: o_done is waited for
+            // one phase on at most, here and below.
+            if (anew && j > 0) {
+                ok = __all_sync(~0u, tile_wait(watch, o_done, (j - 1) & 1));
+                if (!ok) break;
+                tcgen05_fence_after();
+                add_o(j == C::kSpan);
+            }
             uint32_t x[C::kKeys];
 #pragma unroll
             for (int c = 0; c < C::kKeys / 32; ++c)
@@ -338,7 +340,9 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
                 l *= m == -INFINITY ? 0.0f : ex2(m - grown);
                 m = grown;
             } else if (__any_sync(~0u, top > m + kSlack)) {
-                // PV of the tile before has completed with this tile's S.
+                ok = __all_sync(~0u, tile_wait(watch, o_done, (j - 1) & 1));
+                if (!ok) break;
+                tcgen05_fence_after();
                 const float grown = top > m + kSlack ? top : m;
                 const float old = m == -INFINITY ? 0.0f : ex2(m - grown);
                 m = grown;
@@ -392,17 +396,10 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
             tmem_wait_st();
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
-            if (tid == 0 && tile_wait(watch, p_full, j & 1)) {
-                tcgen05_fence_after();
-                values(j);
-                if (j + 1 < tiles) scores(j + 1);
-            }
-            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[j & 1]);
         }
-        if (tid == 0 && tiles > 0) umma_commit(o_full);  // whatever was issued has completed before the block ends
-        __syncwarp();
-        if (tiles > 0) tile_wait(watch, o_full, 0);
+        // Not o_done, which may be two phases back here.
+        if (ok && tiles > 0) tile_wait(watch, drained, 0);
         __syncwarp();
         tcgen05_fence_after();
         const bool summed = tiles > C::kSpan;
@@ -440,37 +437,45 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
             const int t = (first_row + row) / g.group, hq = (first_row + row) - t * g.group;
             *reinterpret_cast<float4*>(g.out + (row0 + t) * (int64_t)g.heads * D + (int64_t)(h * g.group + hq) * D + 4 * piece) = y;
         }
-    } else {
+    } else if (warp < 7) {
         // ---------------------------------------------- codes to fp16
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kConvertRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
         const int ct = tid - 128;
         constexpr int kRowPieces = D / 16;
         const int32_t* table = g.step.table + (int64_t)s * g.step.max_pages;
         const int page = 1 << g.shift;
         const int64_t page_bytes = ((int64_t)g.cache.kv_heads << g.shift) * D, head_bytes = ((int64_t)h << g.shift) * D;
-        // The page of this thread's piece n of tile j, -1 where there is no key.
-        const auto page_of = [&](int j, int n) {
-            const int key = j * C::kKeys + (n * 128 + ct) / kRowPieces;
-            return key < keys ? table[key >> g.shift] : INT_MIN;
+        // Loads are asked for where they stand: the page numbers of a tile two
+        // tiles ahead, its codes and scales one.
+        const auto page_of = [&](int j, int row) {  // of key row `row` of tile j; past the keys: some page
+            const int key = min(j * C::kKeys + row, keys - 1);
+            return load_now(table + (key >> g.shift));
         };
+        const auto row_of = [&](int n) { return (n * C::kConverters + ct) / kRowPieces; };
+        const auto piece_of = [&](int n) { return (n * C::kConverters + ct) % kRowPieces; };
+        const auto mine = [&](int n) { return C::kAllPieces % C::kConverters == 0 || n * C::kConverters + ct < C::kAllPieces; };
         const auto fetch = [&](const int8_t* codes, const int64_t (&from)[C::kPieces], uint4 (&w)[C::kPieces]) {
 #pragma unroll
-            for (int n = 0; n < C::kPieces; ++n)
-                w[n] = from[n] >= 0 ? __ldg(reinterpret_cast<const uint4*>(codes + from[n])) : make_uint4(0u, 0u, 0u, 0u);
+            for (int n = 0; n < C::kPieces; ++n) {
+                w[n] = make_uint4(0u, 0u, 0u, 0u);
+                if (from[n] >= 0) w[n] = load_now(reinterpret_cast<const uint4*>(codes + from[n]));
+            }
         };
-        // Byte offsets of the pieces of tile j, whose pages are ids.
+        // Byte offsets of the pieces of tile j, whose pages are ids; -1: no key there.
         const auto locate = [&](int j, const int32_t (&ids)[C::kPieces], int64_t (&from)[C::kPieces]) {
 #pragma unroll
             for (int n = 0; n < C::kPieces; ++n) {
-                const int row = (n * 128 + ct) / kRowPieces, cc = (n * 128 + ct) % kRowPieces;
-                const int inside = ((j * C::kKeys + row) & (page - 1)) * D + cc * 16;
-                from[n] = static_cast<uint32_t>(ids[n]) < static_cast<uint32_t>(g.cache.pages) ? ids[n] * page_bytes + (head_bytes + inside) : -1;
+                const int key = j * C::kKeys + row_of(n);
+                const int inside = (key & (page - 1)) * D + piece_of(n) * 16;
+                const bool there = mine(n) && key < keys && static_cast<uint32_t>(ids[n]) < static_cast<uint32_t>(g.cache.pages);
+                from[n] = there ? ids[n] * page_bytes + (head_bytes + inside) : -1;
             }
         };
         const auto convert = [&](const uint4 (&w)[C::kPieces], uint8_t* tile) {
 #pragma unroll
             for (int n = 0; n < C::kPieces; ++n) {
-                const int row = (n * 128 + ct) / kRowPieces, cc = (n * 128 + ct) % kRowPieces;
+                if (!mine(n)) continue;
+                const int row = row_of(n), cc = piece_of(n);
                 const uint32_t b[4] = {w[n].x ^ 0x80808080u, w[n].y ^ 0x80808080u, w[n].z ^ 0x80808080u, w[n].w ^ 0x80808080u};
                 uint8_t* line = tile + (cc >> 2) * (C::kKeys * 128) + row * 128;
                 const int chunk = (cc & 3) * 2;
@@ -480,38 +485,36 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
                     make_uint4(codes_half2(b[2], 0x4140u), codes_half2(b[2], 0x4342u), codes_half2(b[3], 0x4140u), codes_half2(b[3], 0x4342u));
             }
         };
-        // Loads run a tile ahead (page numbers two): K of tile j + 1 is asked for
-        // once K of tile j is converted, V likewise.
-        int32_t ids[C::kPieces];
+        int32_t ids[C::kPieces], group_id = 0;  // pages of the pieces, and of 16-key group ct in the first lanes
         int64_t from[C::kPieces];
         uint4 k[C::kPieces], v[C::kPieces];
-        int32_t group_id = INT_MIN;  // page of 16-key group ct, in the first lanes
-        float ks = 0.0f, vs = 0.0f;
-        const auto group_page = [&](int j) {
-            const int key = j * C::kKeys + 16 * ct;
-            return ct < C::kGroups && key < keys ? table[key >> g.shift] : INT_MIN;
+        float ks = 0.0f, vs = -1.0f;  // the group's scales; -1: not there
+        const auto ask_pages = [&](int j) {
+#pragma unroll
+            for (int n = 0; n < C::kPieces; ++n) ids[n] = page_of(j, min(row_of(n), C::kKeys - 1));
+            if (ct < C::kGroups) group_id = page_of(j, 16 * ct);
         };
-        const auto fetch_scales = [&](int32_t id) {
-            ks = vs = 0.0f;
-            if (id >= 0 && id < g.cache.pages) {
-                const int64_t at = (int64_t)id * g.cache.kv_heads + h;
-                ks = __ldg(g.cache.k_scales + at);
-                vs = __ldg(g.cache.v_scales + at);
-            } else if (id != INT_MIN) {
-                report(watch, kSiteKv8Range);
+        const auto ask_scales = [&](int j) {
+            ks = 0.0f;
+            vs = -1.0f;
+            if (ct < C::kGroups && j * C::kKeys + 16 * ct < keys) {
+                if (static_cast<uint32_t>(group_id) < static_cast<uint32_t>(g.cache.pages)) {
+                    const int64_t at = (int64_t)group_id * g.cache.kv_heads + h;
+                    ks = load_now(g.cache.k_scales + at);
+                    vs = load_now(g.cache.v_scales + at);
+                } else {
+                    report(watch, kSiteKv8Range);
+                }
             }
         };
-#pragma unroll
-        for (int n = 0; n < C::kPieces; ++n) ids[n] = page_of(0, n);
-        group_id = group_page(0);
-        locate(0, ids, from);
-        fetch(g.cache.k_codes, from, k);
-        fetch(g.cache.v_codes, from, v);
-        fetch_scales(group_id);
-        bool there = group_id >= 0 && group_id < g.cache.pages;
-#pragma unroll
-        for (int n = 0; n < C::kPieces; ++n) ids[n] = page_of(1, n);
-        group_id = group_page(1);
+        if (tiles > 0) {
+            ask_pages(0);
+            locate(0, ids, from);
+            fetch(g.cache.k_codes, from, k);
+            ask_scales(0);
+            fetch(g.cache.v_codes, from, v);
+            ask_pages(1);
+        }
         bool ok = true;
         for (int j = 0; j < tiles; ++j) {
             const int stage = j % C::kStages;
@@ -522,30 +525,69 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
             if (ct < C::kGroups) {
                 float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);  // hides the group
                 // A page of zeros counts in the sum as any other.
-                if (there) f = vs == 0.0f ? make_float4(ks, -126.0f, 0x1p126f, 0.0f) : make_float4(ks, log2f(vs), 1.0f / vs, 0.0f);
+                if (!(vs < 0.0f)) f = vs == 0.0f ? make_float4(ks, -126.0f, 0x1p126f, 0.0f) : make_float4(ks, log2f(vs), 1.0f / vs, 0.0f);
                 info[(j % C::kInfo) * C::kGroups + ct] = f;
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&k_full[stage]);
-            if (j + 1 < tiles) {
-                locate(j + 1, ids, from);
-                fetch(g.cache.k_codes, from, k);
-                fetch_scales(group_id);
-                there = group_id >= 0 && group_id < g.cache.pages;
-            }
+            locate(j + 1, ids, from);  // no key there past the last tile
+            fetch(g.cache.k_codes, from, k);
+            ask_scales(j + 1);
             if (j >= C::kStages) ok = __all_sync(~0u, tile_wait(watch, &v_empty[stage], reuse));
             if (!ok) break;
             convert(v, v_tiles + stage * C::kKvBytes);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[stage]);
-            if (j + 1 < tiles) {
-                fetch(g.cache.v_codes, from, v);
+            fetch(g.cache.v_codes, from, v);
+            ask_pages(j + 2);
+        }
+    } else {
+        // ------------------------------------------------------ MMA issue
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+        if (tiles > 0 && lane == 0) {
+            constexpr uint32_t s_desc = umma_idesc_f16(C::kRows, C::kKeys, false), o_desc = umma_idesc_f16(C::kRows, C::kOutCols, true);
+            const uint32_t qh = smem_u32(q_hi), ql = smem_u32(q_lo), kt = smem_u32(k_tiles), vt = smem_u32(v_tiles);
+            // S of tile j, into the buffer that PV of tile j - 2 reads: MMAs of
+            // unlike accumulators keep no order, so that one is waited for.
+            const auto scores = [&](int j) {
+                const int stage = j % C::kStages;
+                if (!tile_wait(watch, &k_full[stage], (j / C::kStages) & 1)) return false;
+                if (j >= 2 && !tile_wait(watch, o_done, j & 1)) return false;
+                tcgen05_fence_after();
 #pragma unroll
-                for (int n = 0; n < C::kPieces; ++n) ids[n] = page_of(j + 2, n);
-                group_id = group_page(j + 2);
+                for (int part = 0; part < 2; ++part)
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i)
+                        umma_f16(tmem + (j & 1) * C::kKeys,
+                                 umma_desc_k_sw128((part == 0 ? ql : qh) + (i >> 2) * (C::kRows * 128)) + 2 * (i & 3),
+                                 umma_desc_k_sw128(kt + stage * C::kKvBytes + (i >> 2) * (C::kKeys * 128)) + 2 * (i & 3), s_desc,
+                                 part > 0 || i > 0);
+                umma_commit(&k_empty[stage]);
+                umma_commit(&s_full[j & 1]);
+                return true;
+            };
+            bool ok = scores(0);
+            for (int j = 0; j < tiles && ok; ++j) {
+                if (j + 1 < tiles) ok = scores(j + 1);
+                const int stage = j % C::kStages;
+                if (!ok || !tile_wait(watch, &v_full[stage], (j / C::kStages) & 1) ||
+                    !tile_wait(watch, &p_full[j & 1], (j >> 1) & 1))
+                    break;
+                tcgen05_fence_after();
+#pragma unroll
+                for (int i = 0; i < C::kKeys / 16; ++i)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+                        umma_f16_ta(o_tmem, tmem + (j & 1) * C::kKeys + (i >> 1) * 32 + part * 16 + (i & 1) * 8,
+                                    umma_desc_mn_sw128(vt + stage * C::kKvBytes + i * 2048, C::kKeys * 128), o_desc,
+                                    j % C::kSpan > 0 || i > 0 || part > 0);
+                umma_commit(&v_empty[stage]);
+                umma_commit(o_done);
             }
+            umma_commit(drained);  // all that was issued has completed: the output may be read, the block may end
+            tile_wait(watch, drained, 0);
         }
     }
     __syncwarp();

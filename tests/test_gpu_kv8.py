@@ -446,6 +446,20 @@ def test_attention_columns_streams_and_repeats(cuda_device):
         assert all(torch.equal(first, x) for x in again)  # the same bits every time
 
 
+@pytest.mark.parametrize("dim,group,page", [(32, 8, 64), (64, 8, 16), (96, 2, 32), (128, 3, 16), (128, 8, 128)])
+def test_attention_repeats_bit_for_bit(cuda_device, dim, group, page):
+    # Enough blocks and tiles for an unordered read or write to show.
+    rng = np.random.default_rng(dim + group)
+    for context, new in (([3000, 10, 1500, 4000], [700, 1300, 300, 900]), ([9000, 20000, 300, 7000], [1, 1, 1, 1])):
+        b = _Batch(rng, context, new, page, 4, group, dim, rotary=dim)
+        q = torch.from_numpy(b.q).cuda()
+        first = b.run(q)
+        assert torch.isfinite(first).all()
+        for _ in range(12):
+            assert torch.equal(first, b.run(q))
+    assert _status_ok()
+
+
 def test_attention_code_offsets_past_32_bits(cuda_device):
     # A pool of 2.4 GB of keys: the held pages lie at both of its ends.
     page, kv, dim = 128, 4, 128
