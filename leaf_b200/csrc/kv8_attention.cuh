@@ -56,6 +56,15 @@ __device__ __forceinline__ uint32_t codes_half2(uint32_t biased, uint32_t select
     return r;
 }
 
+// Rotates the pairs of a and b, in the rounding steps of leafq_rotary_append.
+__device__ __forceinline__ void turn(float4& a, float4& b, float4 c, float4 s) {
+    const float4 x = a, y = b;
+    a = make_float4(__fsub_rn(__fmul_rn(x.x, c.x), __fmul_rn(y.x, s.x)), __fsub_rn(__fmul_rn(x.y, c.y), __fmul_rn(y.y, s.y)),
+                    __fsub_rn(__fmul_rn(x.z, c.z), __fmul_rn(y.z, s.z)), __fsub_rn(__fmul_rn(x.w, c.w), __fmul_rn(y.w, s.w)));
+    b = make_float4(__fadd_rn(__fmul_rn(y.x, c.x), __fmul_rn(x.x, s.x)), __fadd_rn(__fmul_rn(y.y, c.y), __fmul_rn(x.y, s.y)),
+                    __fadd_rn(__fmul_rn(y.z, c.z), __fmul_rn(x.z, s.z)), __fadd_rn(__fmul_rn(y.w, c.w), __fmul_rn(x.w, s.w)));
+}
+
 // Eight values of a query row, its item j of D / 8 (a rotation pair's quarters
 // as in the append): a at `at`, b at `to`.
 template <int D>
@@ -67,15 +76,9 @@ __device__ __forceinline__ void query_item(const Kv8AttendArgs& g, const float* 
     to = turned ? at + half : at + ((D - 2 * half) >> 1);
     a = *reinterpret_cast<const float4*>(row + at);
     b = *reinterpret_cast<const float4*>(row + to);
-    if (turned) {
-        const float4 c = *reinterpret_cast<const float4*>(g.cos_table + pos * half + at);
-        const float4 s = *reinterpret_cast<const float4*>(g.sin_table + pos * half + at);
-        const float4 x = a, y = b;
-        a = make_float4(__fsub_rn(__fmul_rn(x.x, c.x), __fmul_rn(y.x, s.x)), __fsub_rn(__fmul_rn(x.y, c.y), __fmul_rn(y.y, s.y)),
-                        __fsub_rn(__fmul_rn(x.z, c.z), __fmul_rn(y.z, s.z)), __fsub_rn(__fmul_rn(x.w, c.w), __fmul_rn(y.w, s.w)));
-        b = make_float4(__fadd_rn(__fmul_rn(y.x, c.x), __fmul_rn(x.x, s.x)), __fadd_rn(__fmul_rn(y.y, c.y), __fmul_rn(x.y, s.y)),
-                        __fadd_rn(__fmul_rn(y.z, c.z), __fmul_rn(x.z, s.z)), __fadd_rn(__fmul_rn(y.w, c.w), __fmul_rn(x.w, s.w)));
-    }
+    if (turned)
+        turn(a, b, *reinterpret_cast<const float4*>(g.cos_table + pos * half + at),
+             *reinterpret_cast<const float4*>(g.sin_table + pos * half + at));
 }
 
 // The power of two that brings a row's largest magnitude into [256, 512), as

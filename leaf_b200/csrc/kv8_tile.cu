@@ -39,10 +39,11 @@ struct TileShape {
     static constexpr int kRows = 128;
     static constexpr int kKeys = D <= 64 ? 96 : 64;
     static constexpr int kBlocks = (D + 63) / 64;        // 64-element (128-byte) column blocks
-    static constexpr int kStages = D <= 64 ? 2 : 1;      // of K and of V
+    static constexpr int kKStages = 2;
+    static constexpr int kVStages = D <= 64 ? 2 : 1;
     static constexpr int kGroups = kKeys / 16;           // of keys that share a page for certain
     static constexpr int kInfo = 4;                      // ring of the groups' scales: a tile's are read while those of
-                                                         // up to kStages + 1 later tiles are written
+                                                         // up to kKStages + 1 later tiles are written
     static constexpr int kQBytes = kBlocks * kRows * 128;
     static constexpr int kKvBytes = kBlocks * kKeys * 128;
     static constexpr int kSpan = 512 / kKeys;            // tiles between O's additions to the rounded sum
@@ -53,7 +54,11 @@ struct TileShape {
     static constexpr int kPieces = (kAllPieces + kConverters - 1) / kConverters;
     static constexpr int kOutCols = kBlocks * 64;        // O columns (those past D are not read)
     static constexpr uint32_t kTmemCols = 256;
-    static constexpr size_t kSmem = 1024 + 2 * kQBytes + 2 * kStages * kKvBytes + kInfo * kGroups * 16 + kRows * 4 + 256;
+    static constexpr bool kSumInSmem = D <= 64;          // else in local memory
+    static constexpr int kSumBytes = kSumInSmem ? kRows * D * 4 : kRows * 4;  // (it also takes the rows' factors first)
+    static constexpr size_t kSmem = 2 * kQBytes + (kKStages + kVStages) * kKvBytes + kSumBytes + kInfo * kGroups * 16 +
+                                    (2 * kKStages + 2 * kVStages + 7) * 8 + 8;
+    static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two blocks share the SM's shared memory");
     static_assert(2 * kKeys + kOutCols <= 256, "two blocks share the SM's 512 TMEM columns");
     static_assert(2 * kQBytes >= kRows * D * 4, "the output leaves through Q's shared memory");
     static_assert(128 * (kSoftmaxRegs + kOtherRegs) == kThreads * 128, "the split of what the launch gives (128 a thread)");
@@ -120,6 +125,11 @@ __device__ __forceinline__ uint4 load_now(const uint4* p) {
     asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
+__device__ __forceinline__ float4 load_now(const float4* p) {
+    float4 v;
+    asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+    return v;
+}
 __device__ __forceinline__ int32_t load_now(const int32_t* p) {
     int32_t v;
     asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
@@ -131,6 +141,17 @@ __device__ __forceinline__ float load_now(const float* p) {
     return v;
 }
 
+// An array that stays in local memory: its address, and 16 bytes of it.
+__device__ __forceinline__ uint32_t local_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_local(p)); }
+__device__ __forceinline__ float4 load_local(uint32_t at) {
+    float4 v;
+    asm volatile("ld.local.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_local(uint32_t at, float4 v) {
+    asm volatile("st.local.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -140,23 +161,24 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 template <int D>
 __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_tiles) {
     using C = TileShape<D>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* q_hi = smem;
     uint8_t* q_lo = q_hi + C::kQBytes;
     uint8_t* k_tiles = q_lo + C::kQBytes;
-    uint8_t* v_tiles = k_tiles + C::kStages * C::kKvBytes;
-    float4* info = reinterpret_cast<float4*>(v_tiles + C::kStages * C::kKvBytes);  // [kInfo][kGroups]: ks, log2 vs, 1 / vs
-    float* factor_s = reinterpret_cast<float*>(info + C::kInfo * C::kGroups);
-    uint64_t* k_full = reinterpret_cast<uint64_t*>(factor_s + C::kRows);
-    uint64_t* k_empty = k_full + C::kStages;
-    uint64_t* v_full = k_empty + C::kStages;
-    uint64_t* v_empty = v_full + C::kStages;
-    uint64_t* s_full = v_empty + C::kStages;  // by S buffer, as p_full
+    uint8_t* v_tiles = k_tiles + C::kKStages * C::kKvBytes;
+    float4* sum_s = reinterpret_cast<float4*>(v_tiles + C::kVStages * C::kKvBytes);  // [D / 4][128]
+    float* factor_s = reinterpret_cast<float*>(sum_s);                              // [128], before the first sum
+    float4* info = reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(sum_s) + C::kSumBytes);  // [kInfo][kGroups]: ks, log2 vs, 1 / vs
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(info + C::kInfo * C::kGroups);
+    uint64_t* k_empty = k_full + C::kKStages;
+    uint64_t* v_full = k_empty + C::kKStages;
+    uint64_t* v_empty = v_full + C::kVStages;
+    uint64_t* s_full = v_empty + C::kVStages;  // by S buffer, as p_full
     uint64_t* p_full = s_full + 2;
-    uint64_t* o_done = p_full + 2;            // PV of a tile has completed
+    uint64_t* o_done = p_full + 2;             // PV of a tile has completed
     uint64_t* drained = o_done + 1;
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
+    uint64_t* q_full = drained + 1;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(q_full + 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     grid_dependency_wait();
     grid_launch_dependents();
@@ -187,79 +209,32 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
                                                      (int64_t)context + (first_row + rows - 1) / g.group + 1)));
     const int tiles = (keys + C::kKeys - 1) / C::kKeys;
 
-    if (tid == 0) {
-        for (int i = 0; i < C::kStages; ++i) {
-            mbar_init(&k_full[i], 3);
-            mbar_init(&k_empty[i], 1);
-            mbar_init(&v_full[i], 3);
-            mbar_init(&v_empty[i], 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
-        }
-        mbar_init(o_done, 1);
-        mbar_init(drained, 1);
-        fence_barrier_init();
+    if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled tiles need it; dynamic shared memory starts there
+        if (tid == 0) report(watch, kSiteKv8Tile);
+        return;
     }
     if (warp == 7) {
+        if (lane == 0) {
+            for (int i = 0; i < C::kKStages; ++i) {
+                mbar_init(&k_full[i], 3);
+                mbar_init(&k_empty[i], 1);
+            }
+            for (int i = 0; i < C::kVStages; ++i) {
+                mbar_init(&v_full[i], 3);
+                mbar_init(&v_empty[i], 1);
+            }
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&s_full[i], 1);
+                mbar_init(&p_full[i], 4);
+            }
+            mbar_init(o_done, 1);
+            mbar_init(drained, 1);
+            mbar_init(q_full, 4);
+            fence_barrier_init();
+        }
+        __syncwarp();
         tmem_alloc(tmem_holder, C::kTmemCols);
         tmem_relinquish();
-    }
-    {
-        // The rows: D / 8 lanes per row, eight values each, rotated, scaled by
-        // the row's power of two, split, stored swizzled (warps 0-7).
-        constexpr int kLanes = D / 8;  // 4, 8, 12, 16: a row's lanes are in one warp
-        constexpr int kRowsAtOnce = 32 / kLanes;
-        const int sub = lane / kLanes, j = lane - sub * kLanes;
-        for (int base = warp * kRowsAtOnce; base < C::kRows; base += 8 * kRowsAtOnce) {
-            const int r = base + sub;
-            const bool live = sub < kRowsAtOnce && r < C::kRows;
-            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
-            int at = 4 * j, to = at + D / 2;
-            if (live && r < rows) {
-                const int t = (first_row + r) / g.group, hq = (first_row + r) - t * g.group;
-                int64_t pos = (int64_t)context + t;
-                if (g.rotary > 0 && (pos < 0 || pos >= g.table_rows)) {
-                    if (j == 0) report(watch, kSiteKv8Range);
-                    pos = 0;
-                }
-                query_item<D>(g, g.q + (row0 + t) * g.q_stride + (int64_t)(h * g.group + hq) * D, j, pos, at, to, a, b);
-            }
-            uint32_t largest = 0;
-            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) largest = max(largest, __float_as_uint(v[e]) & 0x7fffffffu);
-            if constexpr (kLanes == 12) {
-                uint32_t all = 0;
-#pragma unroll
-                for (int e = 0; e < kLanes; ++e) all = max(all, __shfl_sync(~0u, largest, min(sub * kLanes + e, 31)));
-                largest = all;
-            } else {
-#pragma unroll
-                for (int d = kLanes / 2; d > 0; d >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, d));
-            }
-            float up, down;
-            row_power(largest, up, down);
-            if (live) {
-                if (j == 0) factor_s[r] = down * g.scale * kLog2e;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int d = half == 0 ? at : to;
-                    const float x0 = v[4 * half] * up, x1 = v[4 * half + 1] * up, x2 = v[4 * half + 2] * up, x3 = v[4 * half + 3] * up;
-                    uint2 hi, lo;
-                    hi.x = half2_bits(x0, x1);
-                    hi.y = half2_bits(x2, x3);
-                    const __half2 h01 = *reinterpret_cast<const __half2*>(&hi.x), h23 = *reinterpret_cast<const __half2*>(&hi.y);
-                    lo.x = half2_bits(x0 - __low2float(h01), x1 - __high2float(h01));
-                    lo.y = half2_bits(x2 - __low2float(h23), x3 - __high2float(h23));
-                    const int offset = (d >> 6) * (C::kRows * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2;
-                    *reinterpret_cast<uint2*>(q_hi + offset) = hi;
-                    *reinterpret_cast<uint2*>(q_lo + offset) = lo;
-                }
-            }
-        }
-        fence_proxy_async_smem();
     }
     tcgen05_fence_before();
     __syncthreads();
@@ -270,28 +245,122 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
     if (warp < 4) {
         // ------------------------------------------------------- softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
+        {
+            // The warp's 32 rows: D / 8 lanes per row, eight values each, all asked
+            // for before the first is used, rotated, scaled by the row's power of
+            // two, split, stored swizzled.
+            constexpr int kLanes = D / 8;  // 4, 8, 12, 16
+            constexpr int kAtOnce = 32 / kLanes, kTurns = 32 / kAtOnce, kBatch = kTurns < 4 ? kTurns : 4;
+            const int sub = lane / kLanes, i = lane - sub * kLanes;
+            const int half = g.rotary >> 1;
+            const bool turned = 4 * i < half;
+            const int at = turned ? 4 * i : 2 * half + 4 * (i - half / 4);
+            const int to = turned ? at + half : at + ((D - 2 * half) >> 1);
+#pragma unroll 1
+            for (int first = 0; first < kTurns; first += kBatch) {
+                float4 a[kBatch], b[kBatch], cs[kBatch], sn[kBatch];
+#pragma unroll
+                for (int n = 0; n < kBatch; ++n) {
+                    const int r = warp * 32 + (first + n) * kAtOnce + sub;
+                    a[n] = b[n] = sn[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    cs[n] = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+                    if (sub < kAtOnce && r < rows) {
+                        const int t = (first_row + r) / g.group, hq = (first_row + r) - t * g.group;
+                        const float* src = g.q + (row0 + t) * g.q_stride + (int64_t)(h * g.group + hq) * D;
+                        a[n] = load_now(reinterpret_cast<const float4*>(src + at));
+                        b[n] = load_now(reinterpret_cast<const float4*>(src + to));
+                        if (turned) {
+                            int64_t pos = (int64_t)context + t;
+                            if (pos < 0 || pos >= g.table_rows) {
+                                if (i == 0) report(watch, kSiteKv8Range);
+                                pos = 0;
+                            }
+                            cs[n] = load_now(reinterpret_cast<const float4*>(g.cos_table + pos * half + at));
+                            sn[n] = load_now(reinterpret_cast<const float4*>(g.sin_table + pos * half + at));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < kBatch; ++n) {
+                    const int r = warp * 32 + (first + n) * kAtOnce + sub;
+                    if (turned) turn(a[n], b[n], cs[n], sn[n]);
+                    const float v[8] = {a[n].x, a[n].y, a[n].z, a[n].w, b[n].x, b[n].y, b[n].z, b[n].w};
+                    uint32_t largest = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) largest = max(largest, __float_as_uint(v[e]) & 0x7fffffffu);
+                    if constexpr (kLanes == 12) {
+                        uint32_t all = 0;
+#pragma unroll
+                        for (int e = 0; e < kLanes; ++e) all = max(all, __shfl_sync(~0u, largest, min(sub * kLanes + e, 31)));
+                        largest = all;
+                    } else {
+#pragma unroll
+                        for (int d = kLanes / 2; d > 0; d >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, d));
+                    }
+                    float up, down;
+                    row_power(largest, up, down);
+                    if (sub < kAtOnce && r < warp * 32 + 32) {
+                        if (i == 0) factor_s[r] = down * g.scale * kLog2e;
+#pragma unroll
+                        for (int part = 0; part < 2; ++part) {
+                            const int d = part == 0 ? at : to;
+                            const float x0 = v[4 * part] * up, x1 = v[4 * part + 1] * up, x2 = v[4 * part + 2] * up, x3 = v[4 * part + 3] * up;
+                            uint2 hi, lo;
+                            hi.x = half2_bits(x0, x1);
+                            hi.y = half2_bits(x2, x3);
+                            const __half2 h01 = *reinterpret_cast<const __half2*>(&hi.x), h23 = *reinterpret_cast<const __half2*>(&hi.y);
+                            lo.x = half2_bits(x0 - __low2float(h01), x1 - __high2float(h01));
+                            lo.y = half2_bits(x2 - __low2float(h23), x3 - __high2float(h23));
+                            const int offset = (d >> 6) * (C::kRows * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2;
+                            *reinterpret_cast<uint2*>(q_hi + offset) = hi;
+                            *reinterpret_cast<uint2*>(q_lo + offset) = lo;
+                        }
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
         const int r = tid;
         const int64_t pos = (int64_t)context + (first_row + r) / g.group;
         const bool seen = r < rows && pos >= 0 && (g.rotary == 0 || pos < g.table_rows);
         const int limit = seen ? static_cast<int>(min64(keys, pos + 1)) : 0;
         const float factor = factor_s[r];
+        __syncwarp();  // its place is free
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
         float m = -INFINITY, l = 0.0f, m_sum = -INFINITY;
-        float o_sum[C::kOutCols];  // the rounded sum, relative to m_sum; indexed at run time: local memory
+        __align__(16) float o_sum[C::kSumInSmem ? 4 : D];  // the rounded sum, relative to m_sum
+        const uint32_t o_local = local_address(o_sum);
+        const auto get_sum = [&](int c) { return C::kSumInSmem ? sum_s[c * C::kRows + r] : load_local(o_local + 16 * c); };
+        const auto put_sum = [&](int c, float4 v) {
+            if (C::kSumInSmem) sum_s[c * C::kRows + r] = v;
+            else store_local(o_local + 16 * c, v);
+        };
         // Adds O, complete up to the tile before, to it.
         const auto add_o = [&](bool first) {
             const float old = first || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m);
             m_sum = m;
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                float z[32];
-                uint32_t y[32];
-                tmem_ld_32x32b_x32(o_tmem + lanes + 32 * c, y);
+            constexpr int kBatch = 64;  // elements asked for at a time
 #pragma unroll
-                for (int e = 0; e < 32; ++e) z[e] = first ? 0.0f : o_sum[32 * c + e];
-                tmem_wait_ld();
+            for (int base = 0; base < D; base += kBatch) {
+                float4 z[kBatch / 4];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o_sum[32 * c + e] = fmaf(z[e], old, __uint_as_float(y[e]));
+                for (int c = 0; c < kBatch / 4; ++c)
+                    z[c] = first || base + 4 * c >= D ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : get_sum(base / 4 + c);
+#pragma unroll
+                for (int part = 0; part < kBatch && base + part < D; part += 32) {
+                    uint32_t y[32];
+                    tmem_ld_32x32b_x32(o_tmem + lanes + base + part, y);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const float4 s4 = z[part / 4 + c];
+                        put_sum((base + part) / 4 + c,
+                                make_float4(fmaf(s4.x, old, __uint_as_float(y[4 * c])), fmaf(s4.y, old, __uint_as_float(y[4 * c + 1])),
+                                            fmaf(s4.z, old, __uint_as_float(y[4 * c + 2])), fmaf(s4.w, old, __uint_as_float(y[4 * c + 3]))));
+                    }
+                }
             }
         };
         bool ok = true;
@@ -415,7 +484,13 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
                 tmem_wait_ld();
                 if (summed) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(fmaf(o_sum[32 * c + e], old, __uint_as_float(x[e])));
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 z = get_sum(8 * c + e / 4);
+                        x[e] = __float_as_uint(fmaf(z.x, old, __uint_as_float(x[e])));
+                        x[e + 1] = __float_as_uint(fmaf(z.y, old, __uint_as_float(x[e + 1])));
+                        x[e + 2] = __float_as_uint(fmaf(z.z, old, __uint_as_float(x[e + 2])));
+                        x[e + 3] = __float_as_uint(fmaf(z.w, old, __uint_as_float(x[e + 3])));
+                    }
                 }
             }
 #pragma unroll
@@ -451,24 +526,26 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
             const int key = min(j * C::kKeys + row, keys - 1);
             return load_now(table + (key >> g.shift));
         };
-        const auto row_of = [&](int n) { return (n * C::kConverters + ct) / kRowPieces; };
-        const auto piece_of = [&](int n) { return (n * C::kConverters + ct) % kRowPieces; };
-        const auto mine = [&](int n) { return C::kAllPieces % C::kConverters == 0 || n * C::kConverters + ct < C::kAllPieces; };
-        const auto fetch = [&](const int8_t* codes, const int64_t (&from)[C::kPieces], uint4 (&w)[C::kPieces]) {
-#pragma unroll
-            for (int n = 0; n < C::kPieces; ++n) {
-                w[n] = make_uint4(0u, 0u, 0u, 0u);
-                if (from[n] >= 0) w[n] = load_now(reinterpret_cast<const uint4*>(codes + from[n]));
-            }
+        // Four pieces a row and 64-element block at a time: eight lanes then store
+        // to eight different bank groups.
+        const auto row_of = [&](int n) {
+            const int q = n * C::kConverters + ct;
+            return kRowPieces % 4 == 0 ? (q >> 2) % C::kKeys : q / kRowPieces;
         };
-        // Byte offsets of the pieces of tile j, whose pages are ids; -1: no key there.
-        const auto locate = [&](int j, const int32_t (&ids)[C::kPieces], int64_t (&from)[C::kPieces]) {
+        const auto piece_of = [&](int n) {
+            const int q = n * C::kConverters + ct;
+            return kRowPieces % 4 == 0 ? (q & 3) + 4 * (q / (4 * C::kKeys)) : q % kRowPieces;
+        };
+        const auto mine = [&](int n) { return C::kAllPieces % C::kConverters == 0 || n * C::kConverters + ct < C::kAllPieces; };
+        // The pieces of tile j, whose pages are ids; zeros where there is no key.
+        const auto fetch = [&](const int8_t* codes, int j, const int32_t (&ids)[C::kPieces], uint4 (&w)[C::kPieces]) {
 #pragma unroll
             for (int n = 0; n < C::kPieces; ++n) {
                 const int key = j * C::kKeys + row_of(n);
                 const int inside = (key & (page - 1)) * D + piece_of(n) * 16;
-                const bool there = mine(n) && key < keys && static_cast<uint32_t>(ids[n]) < static_cast<uint32_t>(g.cache.pages);
-                from[n] = there ? ids[n] * page_bytes + (head_bytes + inside) : -1;
+                w[n] = make_uint4(0u, 0u, 0u, 0u);
+                if (mine(n) && key < keys && static_cast<uint32_t>(ids[n]) < static_cast<uint32_t>(g.cache.pages))
+                    w[n] = load_now(reinterpret_cast<const uint4*>(codes + (ids[n] * page_bytes + (head_bytes + inside))));
             }
         };
         const auto convert = [&](const uint4 (&w)[C::kPieces], uint8_t* tile) {
@@ -485,13 +562,12 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
                     make_uint4(codes_half2(b[2], 0x4140u), codes_half2(b[2], 0x4342u), codes_half2(b[3], 0x4140u), codes_half2(b[3], 0x4342u));
             }
         };
-        int32_t ids[C::kPieces], group_id = 0;  // pages of the pieces, and of 16-key group ct in the first lanes
-        int64_t from[C::kPieces];
+        int32_t ids[C::kPieces], later[C::kPieces], group_id = 0;  // pages of the pieces of two tiles; of 16-key group ct in the first lanes
         uint4 k[C::kPieces], v[C::kPieces];
         float ks = 0.0f, vs = -1.0f;  // the group's scales; -1: not there
-        const auto ask_pages = [&](int j) {
+        const auto ask_pages = [&](int j, int32_t (&into)[C::kPieces]) {
 #pragma unroll
-            for (int n = 0; n < C::kPieces; ++n) ids[n] = page_of(j, min(row_of(n), C::kKeys - 1));
+            for (int n = 0; n < C::kPieces; ++n) into[n] = page_of(j, min(row_of(n), C::kKeys - 1));
             if (ct < C::kGroups) group_id = page_of(j, 16 * ct);
         };
         const auto ask_scales = [&](int j) {
@@ -507,21 +583,8 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
                 }
             }
         };
-        if (tiles > 0) {
-            ask_pages(0);
-            locate(0, ids, from);
-            fetch(g.cache.k_codes, from, k);
-            ask_scales(0);
-            fetch(g.cache.v_codes, from, v);
-            ask_pages(1);
-        }
-        bool ok = true;
-        for (int j = 0; j < tiles; ++j) {
-            const int stage = j % C::kStages;
-            const uint32_t reuse = ((j / C::kStages) - 1) & 1;
-            if (j >= C::kStages) ok = __all_sync(~0u, tile_wait(watch, &k_empty[stage], reuse));
-            if (!ok) break;
-            convert(k, k_tiles + stage * C::kKvBytes);
+        const auto put_k = [&](int j) {  // k and the scales, into K of tile j
+            convert(k, k_tiles + (j % C::kKStages) * C::kKvBytes);
             if (ct < C::kGroups) {
                 float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);  // hides the group
                 // A page of zeros counts in the sum as any other.
@@ -530,18 +593,40 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
             }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&k_full[stage]);
-            locate(j + 1, ids, from);  // no key there past the last tile
-            fetch(g.cache.k_codes, from, k);
-            ask_scales(j + 1);
-            if (j >= C::kStages) ok = __all_sync(~0u, tile_wait(watch, &v_empty[stage], reuse));
+            if (lane == 0) mbar_arrive(&k_full[j % C::kKStages]);
+        };
+        if (tiles > 0) {
+            ask_pages(0, ids);
+            fetch(g.cache.k_codes, 0, ids, k);
+            ask_scales(0);
+            fetch(g.cache.v_codes, 0, ids, v);
+            ask_pages(1, ids);
+            put_k(0);
+            fetch(g.cache.k_codes, 1, ids, k);
+            ask_scales(1);
+            ask_pages(2, later);
+        }
+        bool ok = true;
+        // K of tile j + 1 before V of tile j: its scores are computed first.
+        for (int j = 0; j < tiles; ++j) {
+            if (j + 1 < tiles) {
+                if (j + 1 >= C::kKStages) ok = __all_sync(~0u, tile_wait(watch, &k_empty[(j + 1) % C::kKStages], ((j + 1) / C::kKStages - 1) & 1));
+                if (!ok) break;
+                put_k(j + 1);
+                fetch(g.cache.k_codes, j + 2, later, k);
+                ask_scales(j + 2);
+            }
+            const int stage = j % C::kVStages;
+            if (j >= C::kVStages) ok = __all_sync(~0u, tile_wait(watch, &v_empty[stage], (j / C::kVStages - 1) & 1));
             if (!ok) break;
             convert(v, v_tiles + stage * C::kKvBytes);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[stage]);
-            fetch(g.cache.v_codes, from, v);
-            ask_pages(j + 2);
+            fetch(g.cache.v_codes, j + 1, ids, v);
+#pragma unroll
+            for (int n = 0; n < C::kPieces; ++n) ids[n] = later[n];
+            ask_pages(j + 3, later);
         }
     } else {
         // ------------------------------------------------------ MMA issue
@@ -552,8 +637,8 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
             // S of tile j, into the buffer that PV of tile j - 2 reads: MMAs of
             // unlike accumulators keep no order, so that one is waited for.
             const auto scores = [&](int j) {
-                const int stage = j % C::kStages;
-                if (!tile_wait(watch, &k_full[stage], (j / C::kStages) & 1)) return false;
+                const int stage = j % C::kKStages;
+                if (!tile_wait(watch, &k_full[stage], (j / C::kKStages) & 1)) return false;
                 if (j >= 2 && !tile_wait(watch, o_done, j & 1)) return false;
                 tcgen05_fence_after();
 #pragma unroll
@@ -568,11 +653,11 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
                 umma_commit(&s_full[j & 1]);
                 return true;
             };
-            bool ok = scores(0);
+            bool ok = tile_wait(watch, q_full, 0) && scores(0);
             for (int j = 0; j < tiles && ok; ++j) {
                 if (j + 1 < tiles) ok = scores(j + 1);
-                const int stage = j % C::kStages;
-                if (!ok || !tile_wait(watch, &v_full[stage], (j / C::kStages) & 1) ||
+                const int stage = j % C::kVStages;
+                if (!ok || !tile_wait(watch, &v_full[stage], (j / C::kVStages) & 1) ||
                     !tile_wait(watch, &p_full[j & 1], (j >> 1) & 1))
                     break;
                 tcgen05_fence_after();
