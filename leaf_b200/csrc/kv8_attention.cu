@@ -158,7 +158,7 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
         const int context = g.step.context[s];
         const int64_t row0 = max64(0, g.step.token_offsets[s]);
         const int new_rows = static_cast<int>(
-            max64(0, min64(min64(g.step.token_offsets[s + 1], g.step.tokens) - row0, INT_MAX / g.group)) * g.group);
+            max64(0, min64(min64(g.step.token_offsets[s + 1], g.step.tokens) - row0, g.most_tokens)) * g.group);
         const int first_row = row_block * 8;
         if (first_row >= new_rows) continue;
         const int rows = min(8, new_rows - first_row);
@@ -623,7 +623,7 @@ int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int head
         return LEAFQ_ERR_INVALID;
     }
     Kv8AttendArgs g{q, q_stride, cos_table, sin_table, table_rows, *cache, *step, out, scale, heads,
-                 heads / cache->kv_heads, rotary_dim, 0};
+                 heads / cache->kv_heads, rotary_dim, 0, INT_MAX / (heads / cache->kv_heads)};
     while ((1 << g.shift) < cache->page) ++g.shift;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool pdl = (flags & LEAFQ_FLAG_PDL) != 0;

@@ -23,6 +23,7 @@ struct Kv8AttendArgs {
     float* out;
     float scale;
     int heads, group, rotary, shift;
+    int most_tokens;  // of a request: its rows (tokens * group) fit int32
 };
 
 constexpr float kLog2e = 1.4426950408889634f;

@@ -3,6 +3,7 @@
 // Compiled as a whole program (build.py): setmaxnreg is ignored in relocatable
 // device code.
 #define LEAFQ_WHOLE_PROGRAM
+#include <algorithm>
 #include <type_traits>
 
 #include "kv8_attention.cuh"
@@ -34,6 +35,13 @@ namespace {
 // -- and the lo halves of Q go first, while S is small.
 constexpr float kTileLift = 6.0f, kSlack = 8.0f;
 
+// What the roles of a block need to know of an item: 128 query rows of one kv
+// head of a request.  tiles < 0: there are no more.
+struct TileItem {
+    int row0, first_row, rows, context, keys, tiles, head, unused;
+    uint8_t power[128];  // of two, that each row was scaled down by (its exponent bits)
+};
+
 template <int D>
 struct TileShape {
     static constexpr int kRows = 128;
@@ -47,21 +55,28 @@ struct TileShape {
     static constexpr int kQBytes = kBlocks * kRows * 128;
     static constexpr int kKvBytes = kBlocks * kKeys * 128;
     static constexpr int kSpan = 512 / kKeys;            // tiles between O's additions to the rounded sum
-    static constexpr int kThreads = 256;
-    static constexpr int kSoftmaxRegs = 168, kOtherRegs = 88;
-    static constexpr int kConverters = 96;
+    // Converting warps and the registers of the launch, of the softmax warps, of the
+    // others.  (Nine warps put five on one of the SM's four schedulers, so the
+    // launch gives 96 registers a thread; eight give 128.)  Registers belong to a
+    // scheduler: a softmax warp can take only what the converting warp beside it,
+    // four warps on, has left.
+    static constexpr int kConvWarps = D <= 64 ? 3 : 4;
+    static constexpr int kThreads = (4 + kConvWarps + 1) * 32;
+    static constexpr int kLaunchRegs = D <= 64 ? 128 : 96;
+    static constexpr int kSoftmaxRegs = D <= 64 ? 128 : 112, kOtherRegs = D <= 64 ? 128 : 80;
+    static constexpr int kConverters = kConvWarps * 32;
     static constexpr int kAllPieces = kKeys * D / 16;    // 16-byte pieces of a K (or V) tile
     static constexpr int kPieces = (kAllPieces + kConverters - 1) / kConverters;
     static constexpr int kOutCols = kBlocks * 64;        // O columns (those past D are not read)
     static constexpr uint32_t kTmemCols = 256;
     static constexpr bool kSumInSmem = D <= 64;          // else in local memory
-    static constexpr int kSumBytes = kSumInSmem ? kRows * D * 4 : kRows * 4;  // (it also takes the rows' factors first)
+    static constexpr int kSumBytes = kSumInSmem ? kRows * D * 4 : 0;
     static constexpr size_t kSmem = 2 * kQBytes + (kKStages + kVStages) * kKvBytes + kSumBytes + kInfo * kGroups * 16 +
-                                    (2 * kKStages + 2 * kVStages + 7) * 8 + 8;
+                                    sizeof(TileItem) + (2 * kKStages + 2 * kVStages + 9) * 8 + 8;
     static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two blocks share the SM's shared memory");
     static_assert(2 * kKeys + kOutCols <= 256, "two blocks share the SM's 512 TMEM columns");
-    static_assert(2 * kQBytes >= kRows * D * 4, "the output leaves through Q's shared memory");
-    static_assert(128 * (kSoftmaxRegs + kOtherRegs) == kThreads * 128, "the split of what the launch gives (128 a thread)");
+    static_assert(kSoftmaxRegs + kOtherRegs <= 2 * kLaunchRegs && kOtherRegs <= kLaunchRegs && kConvWarps >= 3,
+                  "the split of what the launch gives each scheduler");
 };
 
 // The library's device error word and wait limit (leafq_device.cuh), which this
@@ -74,13 +89,11 @@ __device__ __forceinline__ void report(const DeviceWatch& w, unsigned site) {
 __device__ __forceinline__ bool tile_wait(const DeviceWatch& w, uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
     const unsigned long long start = global_timer_ns();
-    for (uint32_t spins = 1;; ++spins) {
+    do {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((spins & 255u) == 0u && global_timer_ns() - start > *static_cast<volatile const unsigned long long*>(w.limit_ns)) {
-            report(w, kSiteKv8Tile);
-            return false;
-        }
-    }
+    } while (global_timer_ns() - start <= *static_cast<volatile const unsigned long long*>(w.limit_ns));
+    report(w, kSiteKv8Tile);
+    return false;
 }
 
 __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -159,68 +172,45 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_tiles) {
+__global__ void __launch_bounds__(TileShape<D>::kThreads, 2)
+kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_tiles) {
     using C = TileShape<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* q_hi = smem;
     uint8_t* q_lo = q_hi + C::kQBytes;
     uint8_t* k_tiles = q_lo + C::kQBytes;
     uint8_t* v_tiles = k_tiles + C::kKStages * C::kKvBytes;
-    float4* sum_s = reinterpret_cast<float4*>(v_tiles + C::kVStages * C::kKvBytes);  // [D / 4][128]
-    float* factor_s = reinterpret_cast<float*>(sum_s);                              // [128], before the first sum
-    float4* info = reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(sum_s) + C::kSumBytes);  // [kInfo][kGroups]: ks, log2 vs, 1 / vs
-    uint64_t* k_full = reinterpret_cast<uint64_t*>(info + C::kInfo * C::kGroups);
+    float4* sum_s = reinterpret_cast<float4*>(v_tiles + C::kVStages * C::kKvBytes);  // kSumInSmem: [4 warps][D / 4][32]
+    float4* info = sum_s + C::kSumBytes / 16;                                        // [kInfo][kGroups]: ks, log2 vs, 1 / vs
+    TileItem* item = reinterpret_cast<TileItem*>(info + C::kInfo * C::kGroups);
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(item + 1);
     uint64_t* k_empty = k_full + C::kKStages;
     uint64_t* v_full = k_empty + C::kKStages;
     uint64_t* v_empty = v_full + C::kVStages;
     uint64_t* s_full = v_empty + C::kVStages;  // by S buffer, as p_full
     uint64_t* p_full = s_full + 2;
     uint64_t* o_done = p_full + 2;             // PV of a tile has completed
-    uint64_t* drained = o_done + 1;
-    uint64_t* q_full = drained + 1;
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(q_full + 1);
+    uint64_t* q_full = o_done + 1;             // an item's rows and description are there
+    uint64_t* q_empty = q_full + 1;            // its last scores are computed, its description is read
+    uint64_t* item_done = q_empty + 1;         // all its MMAs have completed
+    uint64_t* drained = item_done + 1;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    grid_dependency_wait();
-    grid_launch_dependents();
-
-    // Work item, the rows that see most keys first.  Request s may have row
-    // tiles floor(token_offsets[s] * group / 128) + s and on: enough of them.
-    const int item = row_tiles - 1 - blockIdx.x / g.cache.kv_heads;
-    const int h = blockIdx.x % g.cache.kv_heads;
-    const int requests = g.step.requests;
-    int s = 0;
-    for (int n = requests; n > 1;) {
-        const int step = (n + 31) / 32, at = s + lane * step;
-        const bool below = lane * step < n && ((int64_t)g.step.token_offsets[at] * g.group >> 7) + at <= item;
-        const int hit = max(__popc(__ballot_sync(~0u, below)) - 1, 0);
-        s += hit * step;
-        n = min(step, n - hit * step);
-    }
-    const int64_t row0 = max64(0, g.step.token_offsets[s]);
-    const int new_rows = static_cast<int>(
-        max64(0, min64(min64(g.step.token_offsets[s + 1], g.step.tokens) - row0, INT_MAX / g.group)) * g.group);
-    const int64_t tile_index = item - ((row0 * g.group >> 7) + s);
-    if (tile_index < 0 || tile_index * C::kRows >= new_rows) return;
-    const int first_row = static_cast<int>(tile_index) * C::kRows;
-    const int rows = min(C::kRows, new_rows - first_row);
-    const int context = g.step.context[s];
-    const int64_t held = min64(g.step.page_offsets[s + 1] - g.step.page_offsets[s], g.step.max_pages);
-    const int keys = static_cast<int>(max64(0, min64(min64(held << g.shift, g.step.lengths[s]),
-                                                     (int64_t)context + (first_row + rows - 1) / g.group + 1)));
-    const int tiles = (keys + C::kKeys - 1) / C::kKeys;
+    constexpr int kMmaWarp = 4 + C::kConvWarps;
+    const auto token_of = [&](int row) { return static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(g.group)); };
 
     if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled tiles need it; dynamic shared memory starts there
         if (tid == 0) report(watch, kSiteKv8Tile);
         return;
     }
-    if (warp == 7) {
+    if (warp == kMmaWarp) {
         if (lane == 0) {
             for (int i = 0; i < C::kKStages; ++i) {
-                mbar_init(&k_full[i], 3);
+                mbar_init(&k_full[i], C::kConvWarps);
                 mbar_init(&k_empty[i], 1);
             }
             for (int i = 0; i < C::kVStages; ++i) {
-                mbar_init(&v_full[i], 3);
+                mbar_init(&v_full[i], C::kConvWarps);
                 mbar_init(&v_empty[i], 1);
             }
             for (int i = 0; i < 2; ++i) {
@@ -228,8 +218,10 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
                 mbar_init(&p_full[i], 4);
             }
             mbar_init(o_done, 1);
+            mbar_init(q_full, C::kConvWarps);
+            mbar_init(q_empty, 1 + 4);
+            mbar_init(item_done, 1);
             mbar_init(drained, 1);
-            mbar_init(q_full, 4);
             fence_barrier_init();
         }
         __syncwarp();
@@ -241,319 +233,345 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
     tcgen05_fence_after();
     const uint32_t tmem = *tmem_holder;
     const uint32_t o_tmem = tmem + 2 * C::kKeys;
+    grid_dependency_wait();
+    grid_launch_dependents();
 
+    // Tiles are counted on over the items (n); barriers of per-tile and per-item
+    // phases are waited for in order by every role.
     if (warp < 4) {
         // ------------------------------------------------------- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
-        {
-            // The warp's 32 rows: D / 8 lanes per row, eight values each, all asked
-            // for before the first is used, rotated, scaled by the row's power of
-            // two, split, stored swizzled.
-            constexpr int kLanes = D / 8;  // 4, 8, 12, 16
-            constexpr int kAtOnce = 32 / kLanes, kTurns = 32 / kAtOnce, kBatch = kTurns < 4 ? kTurns : 4;
-            const int sub = lane / kLanes, i = lane - sub * kLanes;
-            const int half = g.rotary >> 1;
-            const bool turned = 4 * i < half;
-            const int at = turned ? 4 * i : 2 * half + 4 * (i - half / 4);
-            const int to = turned ? at + half : at + ((D - 2 * half) >> 1);
-#pragma unroll 1
-            for (int first = 0; first < kTurns; first += kBatch) {
-                float4 a[kBatch], b[kBatch], cs[kBatch], sn[kBatch];
-#pragma unroll
-                for (int n = 0; n < kBatch; ++n) {
-                    const int r = warp * 32 + (first + n) * kAtOnce + sub;
-                    a[n] = b[n] = sn[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    cs[n] = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-                    if (sub < kAtOnce && r < rows) {
-                        const int t = (first_row + r) / g.group, hq = (first_row + r) - t * g.group;
-                        const float* src = g.q + (row0 + t) * g.q_stride + (int64_t)(h * g.group + hq) * D;
-                        a[n] = load_now(reinterpret_cast<const float4*>(src + at));
-                        b[n] = load_now(reinterpret_cast<const float4*>(src + to));
-                        if (turned) {
-                            int64_t pos = (int64_t)context + t;
-                            if (pos < 0 || pos >= g.table_rows) {
-                                if (i == 0) report(watch, kSiteKv8Range);
-                                pos = 0;
-                            }
-                            cs[n] = load_now(reinterpret_cast<const float4*>(g.cos_table + pos * half + at));
-                            sn[n] = load_now(reinterpret_cast<const float4*>(g.sin_table + pos * half + at));
-                        }
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < kBatch; ++n) {
-                    const int r = warp * 32 + (first + n) * kAtOnce + sub;
-                    if (turned) turn(a[n], b[n], cs[n], sn[n]);
-                    const float v[8] = {a[n].x, a[n].y, a[n].z, a[n].w, b[n].x, b[n].y, b[n].z, b[n].w};
-                    uint32_t largest = 0;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) largest = max(largest, __float_as_uint(v[e]) & 0x7fffffffu);
-                    if constexpr (kLanes == 12) {
-                        uint32_t all = 0;
-#pragma unroll
-                        for (int e = 0; e < kLanes; ++e) all = max(all, __shfl_sync(~0u, largest, min(sub * kLanes + e, 31)));
-                        largest = all;
-                    } else {
-#pragma unroll
-                        for (int d = kLanes / 2; d > 0; d >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, d));
-                    }
-                    float up, down;
-                    row_power(largest, up, down);
-                    if (sub < kAtOnce && r < warp * 32 + 32) {
-                        if (i == 0) factor_s[r] = down * g.scale * kLog2e;
-#pragma unroll
-                        for (int part = 0; part < 2; ++part) {
-                            const int d = part == 0 ? at : to;
-                            const float x0 = v[4 * part] * up, x1 = v[4 * part + 1] * up, x2 = v[4 * part + 2] * up, x3 = v[4 * part + 3] * up;
-                            uint2 hi, lo;
-                            hi.x = half2_bits(x0, x1);
-                            hi.y = half2_bits(x2, x3);
-                            const __half2 h01 = *reinterpret_cast<const __half2*>(&hi.x), h23 = *reinterpret_cast<const __half2*>(&hi.y);
-                            lo.x = half2_bits(x0 - __low2float(h01), x1 - __high2float(h01));
-                            lo.y = half2_bits(x2 - __low2float(h23), x3 - __high2float(h23));
-                            const int offset = (d >> 6) * (C::kRows * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2;
-                            *reinterpret_cast<uint2*>(q_hi + offset) = hi;
-                            *reinterpret_cast<uint2*>(q_lo + offset) = lo;
-                        }
-                    }
-                }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
-        }
-        const int r = tid;
-        const int64_t pos = (int64_t)context + (first_row + r) / g.group;
-        const bool seen = r < rows && pos >= 0 && (g.rotary == 0 || pos < g.table_rows);
-        const int limit = seen ? static_cast<int>(min64(keys, pos + 1)) : 0;
-        const float factor = factor_s[r];
-        __syncwarp();  // its place is free
+        if constexpr (C::kSoftmaxRegs > C::kLaunchRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-        float m = -INFINITY, l = 0.0f, m_sum = -INFINITY;
-        __align__(16) float o_sum[C::kSumInSmem ? 4 : D];  // the rounded sum, relative to m_sum
+        float4* my_sum = sum_s + warp * (D / 4) * 32;
+        __align__(16) float o_sum[C::kSumInSmem ? 4 : D];  // the rounded sum
         const uint32_t o_local = local_address(o_sum);
-        const auto get_sum = [&](int c) { return C::kSumInSmem ? sum_s[c * C::kRows + r] : load_local(o_local + 16 * c); };
+        // Elements 4 c .. 4 c + 3 of a row; in shared memory the rows are permuted so
+        // that a row's pieces lie in different banks, as a column's do.
+        const auto get_sum = [&](int c) { return C::kSumInSmem ? my_sum[c * 32 + (lane ^ (c & 7))] : load_local(o_local + 16 * c); };
         const auto put_sum = [&](int c, float4 v) {
-            if (C::kSumInSmem) sum_s[c * C::kRows + r] = v;
+            if (C::kSumInSmem) my_sum[c * 32 + (lane ^ (c & 7))] = v;
             else store_local(o_local + 16 * c, v);
         };
-        // Adds O, complete up to the tile before, to it.
-        const auto add_o = [&](bool first) {
-            const float old = first || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m);
-            m_sum = m;
-            constexpr int kBatch = 64;  // elements asked for at a time
-#pragma unroll
-            for (int base = 0; base < D; base += kBatch) {
-                float4 z[kBatch / 4];
-#pragma unroll
-                for (int c = 0; c < kBatch / 4; ++c)
-                    z[c] = first || base + 4 * c >= D ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : get_sum(base / 4 + c);
-#pragma unroll
-                for (int part = 0; part < kBatch && base + part < D; part += 32) {
-                    uint32_t y[32];
-                    tmem_ld_32x32b_x32(o_tmem + lanes + base + part, y);
+        int n = 0;
+        bool ok = true;
+        for (int it = 0;; ++it) {
+            ok = ok && __all_sync(~0u, tile_wait(watch, q_full, it & 1));
+            if (!ok) break;
+            const int tiles = item->tiles, first_row = item->first_row, rows = item->rows, row0 = item->row0, context = item->context,
+                      keys = item->keys, head = item->head;
+            const float factor = __uint_as_float(static_cast<uint32_t>(item->power[tid]) << 23) * g.scale * kLog2e;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_empty);
+            if (tiles < 0) break;
+            const int r = tid;
+            const int t = token_of(first_row + r), hq = (first_row + r) - t * g.group;
+            const int64_t pos = (int64_t)context + t;
+            const bool seen = r < rows && pos >= 0 && (g.rotary == 0 || pos < g.table_rows);
+            const int limit = seen ? static_cast<int>(min64(keys, pos + 1)) : 0;
+            float* out = g.out + ((int64_t)row0 + t) * g.heads * D + (int64_t)(head * g.group + hq) * D;
+            float m = -INFINITY, l = 0.0f, m_sum = -INFINITY;
+            for (int j = 0; j < tiles; ++j, ++n) {
+                const uint32_t s_tmem = tmem + (n & 1) * C::kKeys;
+                ok = __all_sync(~0u, tile_wait(watch, &s_full[n & 1], (n >> 1) & 1));
+                if (!ok) break;
+                tcgen05_fence_after();
+                const float4* scales = info + (n % C::kInfo) * C::kGroups;
+                const int visible = limit - j * C::kKeys;  // columns of this tile that the row sees
+                const bool whole = __all_sync(~0u, visible >= C::kKeys);
+                // 32 scores at a time, read twice: the loops' code has to stay in the
+                // instruction cache beside the other roles'.  What is not seen is -inf.
+                const auto read = [&](int c, uint32_t (&x)[32]) {
+                    tmem_ld_32x32b_x32(s_tmem + lanes + 32 * c, x);
                     tmem_wait_ld();
+                    if (!whole) {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        const float4 s4 = z[part / 4 + c];
-                        put_sum((base + part) / 4 + c,
-                                make_float4(fmaf(s4.x, old, __uint_as_float(y[4 * c])), fmaf(s4.y, old, __uint_as_float(y[4 * c + 1])),
-                                            fmaf(s4.z, old, __uint_as_float(y[4 * c + 2])), fmaf(s4.w, old, __uint_as_float(y[4 * c + 3]))));
+                        for (int e = 0; e < 32; ++e) x[e] = 32 * c + e >= visible ? 0xff800000u : x[e];
+                    }
+                };
+                // From an MMA sum to x_j: above zero, so that -inf stays.
+                const auto slope = [&](float ks) { return ks * factor == 0.0f ? 1e-37f : ks * factor; };
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < C::kKeys / 32; ++c) {
+                    uint32_t x[32];
+                    read(c, x);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const float* at = reinterpret_cast<const float*>(x) + 16 * half;
+                        float most = fmaxf(at[0], at[1]);
+#pragma unroll
+                        for (int e = 2; e < 16; e += 2) most = max3(most, at[e], at[e + 1]);
+                        const float4 scale = scales[2 * c + half];
+                        top = fmaxf(top, fmaf(most, slope(scale.x), scale.y));
                     }
                 }
-            }
-        };
-        bool ok = true;
-        for (int j = 0; j < tiles; ++j) {
-            const uint32_t s_tmem = tmem + (j & 1) * C::kKeys;
-            ok = __all_sync(~0u, tile_wait(watch, &s_full[j & 1], (j >> 1) & 1));
-            if (!ok) break;
-            tcgen05_fence_after();
-            const bool anew = j % C::kSpan == 0;
-            // This tile's S means that PV of tile j - 2 is done: o_done is waited for
-            // one phase on at most, here and below.
-            if (anew && j > 0) {
-                ok = __all_sync(~0u, tile_wait(watch, o_done, (j - 1) & 1));
-                if (!ok) break;
-                tcgen05_fence_after();
-                add_o(j == C::kSpan);
-            }
-            uint32_t x[C::kKeys];
-#pragma unroll
-            for (int c = 0; c < C::kKeys / 32; ++c)
-                tmem_ld_32x32b_x32(s_tmem + lanes + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
-            const float4* scales = info + (j % C::kInfo) * C::kGroups;
-            const int visible = limit - j * C::kKeys;  // columns of this tile that the row sees
-            const bool whole = __all_sync(~0u, visible >= C::kKeys);
-            tmem_wait_ld();
-            if (!whole) {
-#pragma unroll
-                for (int e = 0; e < C::kKeys; ++e)
-                    if (e >= visible) x[e] = 0xff800000u;
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < C::kGroups; ++n) {
-                const float* at = reinterpret_cast<const float*>(x) + 16 * n;
-                float most = fmaxf(at[0], at[1]);
-#pragma unroll
-                for (int e = 2; e < 16; e += 2) most = max3(most, at[e], at[e + 1]);
-                const float4 scale = scales[n];
-                // A column that is not seen stays -inf whatever the scale.
-                const float value = fmaf(most, scale.x * factor, scale.y);
-                top = fmaxf(top, most == -INFINITY ? most : value);
-            }
-            if (anew) {
-                // O starts anew with this tile: only L has a reference to keep.
-                const float grown = fmaxf(m, top);
-                l *= m == -INFINITY ? 0.0f : ex2(m - grown);
-                m = grown;
-            } else if (__any_sync(~0u, top > m + kSlack)) {
-                ok = __all_sync(~0u, tile_wait(watch, o_done, (j - 1) & 1));
-                if (!ok) break;
-                tcgen05_fence_after();
-                const float grown = top > m + kSlack ? top : m;
-                const float old = m == -INFINITY ? 0.0f : ex2(m - grown);
-                m = grown;
-                l *= old;
+                // This tile's S means that PV of tile n - 2 is done: o_done is waited
+                // for one phase on at most, here and below.
+                const bool anew = j % C::kSpan == 0;
+                const float m_before = m;
+                if (anew) {
+                    // O starts anew with this tile: only L has a reference to keep.
+                    const float grown = fmaxf(m, top);
+                    l *= m == -INFINITY ? 0.0f : ex2(m - grown);
+                    m = grown;
+                } else if (__any_sync(~0u, top > m + kSlack)) {
+                    ok = __all_sync(~0u, tile_wait(watch, o_done, (n - 1) & 1));
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    const float grown = top > m + kSlack ? top : m;
+                    const float old = m == -INFINITY ? 0.0f : ex2(m - grown);
+                    m = grown;
+                    l *= old;
 #pragma unroll 1
-                for (int c = 0; c < C::kOutCols / 32; ++c) {
-                    uint32_t y[32];
-                    tmem_ld_32x32b_x32(o_tmem + lanes + 32 * c, y);
-                    tmem_wait_ld();
+                    for (int c = 0; c < C::kOutCols / 32; ++c) {
+                        uint32_t y[32];
+                        tmem_ld_32x32b_x32(o_tmem + lanes + 32 * c, y);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * old);
-                    tmem_st_32x32b_x32(o_tmem + lanes + 32 * c, y);
+                        for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * old);
+                        tmem_st_32x32b_x32(o_tmem + lanes + 32 * c, y);
+                    }
                 }
-            }
-            const float shift = m == -INFINITY ? 0.0f : m - kTileLift;
-            const auto weigh = [&](auto masked) {
-#pragma unroll
+                const float shift = m == -INFINITY ? 0.0f : m - kTileLift;
+#pragma unroll 1
                 for (int c = 0; c < C::kKeys / 32; ++c) {
-                    uint32_t p[32];
+                    uint32_t x[32], p[32];
+                    read(c, x);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const float4 scale = scales[2 * c + half];
-                        const unsigned long long a = pack2(scale.x * factor, scale.x * factor);
-                        const unsigned long long b = pack2(scale.y - shift, scale.y - shift);
+                        const float a1 = slope(scale.x), b1 = scale.y - shift;
+                        const unsigned long long a = pack2(a1, a1), b = pack2(b1, b1);
                         unsigned long long sum = 0;
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            const int at = 32 * c + 16 * half + e;
-                            const float2 y = unpack2(fma2(pack2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), a, b));
-                            float w0 = ex2(y.x), w1 = ex2(y.y);
-                            if constexpr (decltype(masked)::value) {  // -inf times a scale of zero is no number
-                                w0 = at >= visible ? 0.0f : w0;
-                                w1 = at + 1 >= visible ? 0.0f : w1;
-                            }
+                        for (int e = 16 * half; e < 16 * half + 16; e += 2) {
+                            const float2 y = unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), a, b));
+                            const float w0 = ex2(y.x), w1 = ex2(y.y);
                             const unsigned long long w = pack2(w0, w1);
                             sum = add2(sum, w);
                             const float h0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u);
                             const float h1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
                             const float2 low = unpack2(sub2(w, pack2(h0, h1)));
-                            p[8 * half + e / 2] = half2_bits(h0, h1);
-                            p[16 + 8 * half + e / 2] = half2_bits(low.x, low.y);
+                            p[e / 2] = half2_bits(h0, h1);
+                            p[16 + e / 2] = half2_bits(low.x, low.y);
                         }
                         const float2 both = unpack2(sum);
                         l = fmaf(both.x + both.y, scale.z, l);
                     }
                     tmem_st_32x32b_x32(s_tmem + lanes + 32 * c, p);
                 }
-            };
-            if (whole) weigh(std::false_type{});
-            else weigh(std::true_type{});
-            tmem_wait_st();
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[j & 1]);
-        }
-        // Not o_done, which may be two phases back here.
-        if (ok && tiles > 0) tile_wait(watch, drained, 0);
-        __syncwarp();
-        tcgen05_fence_after();
-        const bool summed = tiles > C::kSpan;
-        const float old = !summed || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m);
-        // Out through shared memory (Q's, no longer read): whole rows per store.
-        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-        uint8_t* stage = smem + warp * (32 * D * 4);
+                if (anew && j > 0) {
+                    // Adds O, complete up to the tile before, to the rounded sum.
+                    ok = __all_sync(~0u, tile_wait(watch, o_done, (n - 1) & 1));
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    const bool first = j == C::kSpan;
+                    const float old = first || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m_before);
+                    m_sum = m_before;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-            uint32_t x[32];
-            if (tiles > 0) {
-                tmem_ld_32x32b_x32(o_tmem + lanes + 32 * c, x);
-                tmem_wait_ld();
-                if (summed) {
+                    for (int c = 0; c < D / 4; c += 8) {
+                        float4 z[8];
+                        uint32_t y[32];
+                        tmem_ld_32x32b_x32(o_tmem + lanes + 4 * c, y);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 z = get_sum(8 * c + e / 4);
-                        x[e] = __float_as_uint(fmaf(z.x, old, __uint_as_float(x[e])));
-                        x[e + 1] = __float_as_uint(fmaf(z.y, old, __uint_as_float(x[e + 1])));
-                        x[e + 2] = __float_as_uint(fmaf(z.z, old, __uint_as_float(x[e + 2])));
-                        x[e + 3] = __float_as_uint(fmaf(z.w, old, __uint_as_float(x[e + 3])));
+                        for (int e = 0; e < 8; ++e) z[e] = first ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : get_sum(c + e);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            put_sum(c + e, make_float4(fmaf(z[e].x, old, __uint_as_float(y[4 * e])), fmaf(z[e].y, old, __uint_as_float(y[4 * e + 1])),
+                                                       fmaf(z[e].z, old, __uint_as_float(y[4 * e + 2])),
+                                                       fmaf(z[e].w, old, __uint_as_float(y[4 * e + 3]))));
+                    }
+                }
+                tmem_wait_st();
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[n & 1]);
+            }
+            ok = ok && __all_sync(~0u, tile_wait(watch, item_done, it & 1));
+            if (!ok) break;
+            tcgen05_fence_after();
+            // The rows' output: O (and the rounded sum) over L, zeros for a row that
+            // sees no key.
+            const bool summed = tiles > C::kSpan;
+            const float old = !summed || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m);
+            const float inverse = l == 0.0f ? 0.0f : __frcp_rn(l);
+#pragma unroll 1
+            for (int c = 0; c < D / 4; c += 8) {
+                uint32_t x[32];
+                tmem_ld_32x32b_x32(o_tmem + lanes + 4 * c, x);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float4 y = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]), __uint_as_float(x[4 * e + 2]),
+                                           __uint_as_float(x[4 * e + 3]));
+                    if (summed) {
+                        const float4 z = get_sum(c + e);
+                        y = make_float4(fmaf(z.x, old, y.x), fmaf(z.y, old, y.y), fmaf(z.z, old, y.z), fmaf(z.w, old, y.w));
+                    }
+                    y = l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                  : make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
+                    if (C::kSumInSmem) put_sum(c + e, y);
+                    else if (r < rows) *reinterpret_cast<float4*>(out + 4 * (c + e)) = y;
+                }
+            }
+            if constexpr (C::kSumInSmem) {
+                // Through the warp's sums: whole rows per store.
+                __syncwarp();
+                constexpr int kRowLanes = D / 4;  // 8 or 16 lanes a row
+#pragma unroll 4
+                for (int i = 0; i < 32; i += 32 / kRowLanes) {
+                    const int row = i + lane / kRowLanes, c = lane % kRowLanes;
+                    float* to = reinterpret_cast<float*>(__shfl_sync(~0u, reinterpret_cast<uintptr_t>(out), row));
+                    const float4 v = my_sum[c * 32 + (row ^ (c & 7))];
+                    if (warp * 32 + row < rows) *reinterpret_cast<float4*>(to + 4 * c) = v;
+                }
+                __syncwarp();
+            }
+            tcgen05_fence_before();
+        }
+    } else if (warp < kMmaWarp) {
+        // ------------------------------- the items, their rows, codes to fp16
+        if constexpr (C::kOtherRegs < C::kLaunchRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+        const int ct = tid - 128, cw = warp - 4;
+        constexpr int kRowPieces = D / 16;
+        const int page = 1 << g.shift;
+        const int64_t page_bytes = ((int64_t)g.cache.kv_heads << g.shift) * D;
+
+        // Items: row tiles x kv heads, those that see most keys first, dealt to the
+        // blocks back and forth.  Request s may have row tiles
+        // floor(token_offsets[s] * group / 128) + s and on: enough of them.
+        const uint32_t total = static_cast<uint32_t>(row_tiles) * g.cache.kv_heads;
+        struct Next {
+            int row0, first_row, rows, context, keys, request, head;
+        };
+        int round = 0;
+        const auto advance = [&](Next& next) {
+            for (;; ++round) {
+                const uint32_t base = static_cast<uint32_t>(round) * gridDim.x;
+                if (base >= total) return false;
+                const uint32_t id = base + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                if (id >= total) continue;
+                const uint32_t group_of = id / static_cast<uint32_t>(g.cache.kv_heads);
+                const int index = row_tiles - 1 - static_cast<int>(group_of);
+                next.head = static_cast<int>(id - group_of * g.cache.kv_heads);
+                int s = 0;
+                for (int left = g.step.requests; left > 1;) {
+                    const int step = (left + 31) / 32, at = s + lane * step;
+                    const bool below = lane * step < left && ((int64_t)g.step.token_offsets[at] * g.group >> 7) + at <= index;
+                    const int hit = max(__popc(__ballot_sync(~0u, below)) - 1, 0);
+                    s += hit * step;
+                    left = min(step, left - hit * step);
+                }
+                const int64_t row0 = max64(0, g.step.token_offsets[s]);
+                const int64_t new_rows =
+                    max64(0, min64(min64(g.step.token_offsets[s + 1], g.step.tokens) - row0, g.most_tokens)) * g.group;
+                const int64_t tile_index = index - ((row0 * g.group >> 7) + s);
+                if (tile_index < 0 || tile_index * C::kRows >= new_rows) continue;
+                next.row0 = static_cast<int>(row0);
+                next.first_row = static_cast<int>(tile_index) * C::kRows;
+                next.rows = static_cast<int>(min64(C::kRows, new_rows - next.first_row));
+                next.context = g.step.context[s];
+                next.request = s;
+                const int64_t held = min64(g.step.page_offsets[s + 1] - g.step.page_offsets[s], g.step.max_pages);
+                next.keys = static_cast<int>(max64(
+                    0, min64(min64(held << g.shift, g.step.lengths[s]), (int64_t)next.context + token_of(next.first_row + next.rows - 1) + 1)));
+                ++round;
+                return true;
+            }
+        };
+        // Lanes of a row: D / 8, eight values each (a rotation pair's quarters).
+        constexpr int kLanes = D / 8;  // 4, 8, 12, 16
+        constexpr int kAtOnce = 32 / kLanes, kPass = C::kConvWarps * kAtOnce;
+        constexpr int kTurns = (C::kRows + kPass - 1) / kPass;
+        const int sub = lane / kLanes, part = lane - sub * kLanes;
+        const int half = g.rotary >> 1;
+        const bool turned = 4 * part < half;
+        const int at = turned ? 4 * part : 2 * half + 4 * (part - half / 4);
+        const int to = turned ? at + half : at + ((D - 2 * half) >> 1);
+        // Loads run a turn ahead; rotated, scaled by the row's power of two, split,
+        // stored swizzled.
+        const auto put_rows = [&](const Next& next, uint8_t* power) {
+            float4 a, b, cs, sn;
+            const auto ask = [&](int turn_index) {
+                const int r = turn_index * kPass + cw * kAtOnce + sub;
+                a = b = sn = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                cs = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+                if (sub < kAtOnce && r < next.rows) {
+                    const int t = token_of(next.first_row + r), hq = (next.first_row + r) - t * g.group;
+                    const float* src = g.q + ((int64_t)next.row0 + t) * g.q_stride + (int64_t)(next.head * g.group + hq) * D;
+                    a = load_now(reinterpret_cast<const float4*>(src + at));
+                    b = load_now(reinterpret_cast<const float4*>(src + to));
+                    if (turned) {
+                        int64_t pos = (int64_t)next.context + t;
+                        if (pos < 0 || pos >= g.table_rows) {
+                            if (part == 0) report(watch, kSiteKv8Range);
+                            pos = 0;
+                        }
+                        cs = load_now(reinterpret_cast<const float4*>(g.cos_table + pos * half + at));
+                        sn = load_now(reinterpret_cast<const float4*>(g.sin_table + pos * half + at));
+                    }
+                }
+            };
+            ask(0);
+#pragma unroll 1
+            for (int i = 0; i < kTurns; ++i) {
+                const int r = i * kPass + cw * kAtOnce + sub;
+                if (turned) turn(a, b, cs, sn);
+                const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                if (i + 1 < kTurns) ask(i + 1);
+                // A NaN is no maximum, but it stays one in its row's products.
+                float largest = fabsf(v[0]);
+#pragma unroll
+                for (int e = 1; e < 8; ++e) largest = fmaxf(largest, fabsf(v[e]));
+                if constexpr (kLanes == 12) {
+                    float all = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < kLanes; ++e) all = fmaxf(all, __shfl_sync(~0u, largest, min(sub * kLanes + e, 31)));
+                    largest = all;
+                } else {
+#pragma unroll
+                    for (int d = kLanes / 2; d > 0; d >>= 1) largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, d));
+                }
+                float up, down;
+                row_power(__float_as_uint(largest), up, down);
+                if (sub < kAtOnce && r < C::kRows) {
+                    if (part == 0) power[r] = static_cast<uint8_t>(__float_as_uint(down) >> 23);
+#pragma unroll
+                    for (int quarter = 0; quarter < 2; ++quarter) {
+                        const int d = quarter == 0 ? at : to;
+                        const float x0 = v[4 * quarter] * up, x1 = v[4 * quarter + 1] * up, x2 = v[4 * quarter + 2] * up,
+                                    x3 = v[4 * quarter + 3] * up;
+                        uint2 hi, lo;
+                        hi.x = half2_bits(x0, x1);
+                        hi.y = half2_bits(x2, x3);
+                        const __half2 h01 = *reinterpret_cast<const __half2*>(&hi.x), h23 = *reinterpret_cast<const __half2*>(&hi.y);
+                        lo.x = half2_bits(x0 - __low2float(h01), x1 - __high2float(h01));
+                        lo.y = half2_bits(x2 - __low2float(h23), x3 - __high2float(h23));
+                        const int offset = (d >> 6) * (C::kRows * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2;
+                        *reinterpret_cast<uint2*>(q_hi + offset) = hi;
+                        *reinterpret_cast<uint2*>(q_lo + offset) = lo;
                     }
                 }
             }
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (tiles > 0 && l != 0.0f)
-                    y = make_float4(__uint_as_float(x[e]) * inverse, __uint_as_float(x[e + 1]) * inverse,
-                                    __uint_as_float(x[e + 2]) * inverse, __uint_as_float(x[e + 3]) * inverse);
-                const int piece = 8 * c + e / 4;  // of the row's D / 4
-                *reinterpret_cast<float4*>(stage + lane * (D * 4) + ((piece ^ (lane & 7)) << 4)) = y;
-            }
-        }
-        __syncwarp();
-        for (int i = lane; i < 32 * (D / 4); i += 32) {
-            const int rr = i / (D / 4), piece = i - rr * (D / 4);
-            const int row = warp * 32 + rr;
-            if (row >= rows) break;
-            const float4 y = *reinterpret_cast<const float4*>(stage + rr * (D * 4) + ((piece ^ (rr & 7)) << 4));
-            const int t = (first_row + row) / g.group, hq = (first_row + row) - t * g.group;
-            *reinterpret_cast<float4*>(g.out + (row0 + t) * (int64_t)g.heads * D + (int64_t)(h * g.group + hq) * D + 4 * piece) = y;
-        }
-    } else if (warp < 7) {
-        // ---------------------------------------------- codes to fp16
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
-        const int ct = tid - 128;
-        constexpr int kRowPieces = D / 16;
-        const int32_t* table = g.step.table + (int64_t)s * g.step.max_pages;
-        const int page = 1 << g.shift;
-        const int64_t page_bytes = ((int64_t)g.cache.kv_heads << g.shift) * D, head_bytes = ((int64_t)h << g.shift) * D;
-        // Loads are asked for where they stand: the page numbers of a tile two
-        // tiles ahead, its codes and scales one.
-        const auto page_of = [&](int j, int row) {  // of key row `row` of tile j; past the keys: some page
-            const int key = min(j * C::kKeys + row, keys - 1);
-            return load_now(table + (key >> g.shift));
         };
         // Four pieces a row and 64-element block at a time: eight lanes then store
         // to eight different bank groups.
-        const auto row_of = [&](int n) {
-            const int q = n * C::kConverters + ct;
+        const auto row_of = [&](int i) {
+            const int q = i * C::kConverters + ct;
             return kRowPieces % 4 == 0 ? (q >> 2) % C::kKeys : q / kRowPieces;
         };
-        const auto piece_of = [&](int n) {
-            const int q = n * C::kConverters + ct;
+        const auto piece_of = [&](int i) {
+            const int q = i * C::kConverters + ct;
             return kRowPieces % 4 == 0 ? (q & 3) + 4 * (q / (4 * C::kKeys)) : q % kRowPieces;
         };
-        const auto mine = [&](int n) { return C::kAllPieces % C::kConverters == 0 || n * C::kConverters + ct < C::kAllPieces; };
-        // The pieces of tile j, whose pages are ids; zeros where there is no key.
-        const auto fetch = [&](const int8_t* codes, int j, const int32_t (&ids)[C::kPieces], uint4 (&w)[C::kPieces]) {
-#pragma unroll
-            for (int n = 0; n < C::kPieces; ++n) {
-                const int key = j * C::kKeys + row_of(n);
-                const int inside = (key & (page - 1)) * D + piece_of(n) * 16;
-                w[n] = make_uint4(0u, 0u, 0u, 0u);
-                if (mine(n) && key < keys && static_cast<uint32_t>(ids[n]) < static_cast<uint32_t>(g.cache.pages))
-                    w[n] = load_now(reinterpret_cast<const uint4*>(codes + (ids[n] * page_bytes + (head_bytes + inside))));
-            }
-        };
+        const auto mine = [&](int i) { return C::kAllPieces % C::kConverters == 0 || i * C::kConverters + ct < C::kAllPieces; };
         const auto convert = [&](const uint4 (&w)[C::kPieces], uint8_t* tile) {
 #pragma unroll
-            for (int n = 0; n < C::kPieces; ++n) {
-                if (!mine(n)) continue;
-                const int row = row_of(n), cc = piece_of(n);
-                const uint32_t b[4] = {w[n].x ^ 0x80808080u, w[n].y ^ 0x80808080u, w[n].z ^ 0x80808080u, w[n].w ^ 0x80808080u};
+            for (int i = 0; i < C::kPieces; ++i) {
+                if (!mine(i)) continue;
+                const int row = row_of(i), cc = piece_of(i);
+                const uint32_t b[4] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u, w[i].z ^ 0x80808080u, w[i].w ^ 0x80808080u};
                 uint8_t* line = tile + (cc >> 2) * (C::kKeys * 128) + row * 128;
                 const int chunk = (cc & 3) * 2;
                 *reinterpret_cast<uint4*>(line + ((chunk ^ (row & 7)) << 4)) =
@@ -562,123 +580,196 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2) kv8_attend_tile_ker
                     make_uint4(codes_half2(b[2], 0x4140u), codes_half2(b[2], 0x4342u), codes_half2(b[3], 0x4140u), codes_half2(b[3], 0x4342u));
             }
         };
-        int32_t ids[C::kPieces], later[C::kPieces], group_id = 0;  // pages of the pieces of two tiles; of 16-key group ct in the first lanes
-        uint4 k[C::kPieces], v[C::kPieces];
-        float ks = 0.0f, vs = -1.0f;  // the group's scales; -1: not there
-        const auto ask_pages = [&](int j, int32_t (&into)[C::kPieces]) {
+
+        Next now = {}, next;
+        bool more = false, ok = true;
+        int n = 0;  // tiles of the items before
+        // (Every piece of work stands once: the roles' code shares the instruction
+        // cache.  Turn -1 only finds the first item.)
+        for (int it = -1;; ++it) {
+            if (it > 0) ok = __all_sync(~0u, tile_wait(watch, q_empty, (it - 1) & 1));
+            if (!ok) break;
+            const int keys = more ? now.keys : 0;
+            const int tiles = more ? max(1, (keys + C::kKeys - 1) / C::kKeys) : -1;  // without keys, a tile that is all hidden
+            if (it >= 0 && ct == 0) {
+                item->row0 = now.row0;
+                item->first_row = now.first_row;
+                item->rows = now.rows;
+                item->context = now.context;
+                item->keys = keys;
+                item->tiles = tiles;
+                item->head = now.head;
+            }
+            if (it >= 0 && !more) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
+                break;
+            }
+            const int32_t* table = g.step.table + (int64_t)now.request * g.step.max_pages;
+            const int64_t head_bytes = ((int64_t)now.head << g.shift) * D;
+            // Loads are asked for where they stand: the page numbers of a tile two
+            // tiles ahead, its codes and scales one.
+            const auto page_of = [&](int j, int row) {  // of key row `row` of tile j; past the keys: some page
+                const int key = min(j * C::kKeys + row, keys - 1);
+                return keys > 0 ? load_now(table + (key >> g.shift)) : -1;
+            };
+            // The pieces of tile j, whose pages are ids; zeros where there is no key.
+            const auto fetch = [&](const int8_t* codes, int j, const int32_t (&ids)[C::kPieces], uint4 (&w)[C::kPieces]) {
 #pragma unroll
-            for (int n = 0; n < C::kPieces; ++n) into[n] = page_of(j, min(row_of(n), C::kKeys - 1));
-            if (ct < C::kGroups) group_id = page_of(j, 16 * ct);
-        };
-        const auto ask_scales = [&](int j) {
-            ks = 0.0f;
-            vs = -1.0f;
-            if (ct < C::kGroups && j * C::kKeys + 16 * ct < keys) {
-                if (static_cast<uint32_t>(group_id) < static_cast<uint32_t>(g.cache.pages)) {
-                    const int64_t at = (int64_t)group_id * g.cache.kv_heads + h;
-                    ks = load_now(g.cache.k_scales + at);
-                    vs = load_now(g.cache.v_scales + at);
-                } else {
-                    report(watch, kSiteKv8Range);
+                for (int i = 0; i < C::kPieces; ++i) {
+                    const int key = j * C::kKeys + row_of(i);
+                    const int inside = (key & (page - 1)) * D + piece_of(i) * 16;
+                    w[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (mine(i) && key < keys && static_cast<uint32_t>(ids[i]) < static_cast<uint32_t>(g.cache.pages))
+                        w[i] = load_now(reinterpret_cast<const uint4*>(codes + (ids[i] * page_bytes + (head_bytes + inside))));
+                }
+            };
+            int32_t ids[C::kPieces], later[C::kPieces], group_id = 0;  // pages of the pieces of two tiles; of 16-key group ct in the first lanes
+            uint4 k[C::kPieces], v[C::kPieces];
+            float ks = 0.0f, vs = -1.0f;  // the group's scales; -1: not there
+            const auto ask_pages = [&](int j, int32_t (&into)[C::kPieces]) {
+#pragma unroll
+                for (int i = 0; i < C::kPieces; ++i) into[i] = page_of(j, min(row_of(i), C::kKeys - 1));
+                if (ct < C::kGroups) group_id = page_of(j, 16 * ct);
+            };
+            const auto ask_scales = [&](int j) {
+                ks = 0.0f;
+                vs = -1.0f;
+                if (ct < C::kGroups && j * C::kKeys + 16 * ct < keys) {
+                    if (static_cast<uint32_t>(group_id) < static_cast<uint32_t>(g.cache.pages)) {
+                        const int64_t from = (int64_t)group_id * g.cache.kv_heads + now.head;
+                        ks = load_now(g.cache.k_scales + from);
+                        vs = load_now(g.cache.v_scales + from);
+                    } else {
+                        report(watch, kSiteKv8Range);
+                    }
+                }
+            };
+            const auto put_k = [&](int j) {  // k and the scales, into K of tile j
+                const int tile = n + j;
+                if (tile >= C::kKStages)
+                    ok = __all_sync(~0u, tile_wait(watch, &k_empty[tile % C::kKStages], (tile / C::kKStages - 1) & 1));
+                if (!ok) return;
+                convert(k, k_tiles + (tile % C::kKStages) * C::kKvBytes);
+                if (ct < C::kGroups) {
+                    float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);  // hides the group
+                    // A page of zeros counts in the sum as any other.
+                    if (!(vs < 0.0f)) f = vs == 0.0f ? make_float4(ks, -126.0f, 0x1p126f, 0.0f) : make_float4(ks, log2f(vs), __frcp_rn(vs), 0.0f);
+                    info[(tile % C::kInfo) * C::kGroups + ct] = f;
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&k_full[tile % C::kKStages]);
+            };
+            if (it >= 0) ask_pages(0, later);
+            // The next item meanwhile, and its rows into L2.
+            more = advance(next);
+            if (more) {
+                for (int i = ct; i < next.rows * (D / 32); i += C::kConverters) {
+                    const int r = i / (D / 32), t = token_of(next.first_row + r), hq = (next.first_row + r) - t * g.group;
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(g.q + ((int64_t)next.row0 + t) * g.q_stride +
+                                                                  (int64_t)(next.head * g.group + hq) * D + 32 * (i % (D / 32))));
                 }
             }
-        };
-        const auto put_k = [&](int j) {  // k and the scales, into K of tile j
-            convert(k, k_tiles + (j % C::kKStages) * C::kKvBytes);
-            if (ct < C::kGroups) {
-                float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);  // hides the group
-                // A page of zeros counts in the sum as any other.
-                if (!(vs < 0.0f)) f = vs == 0.0f ? make_float4(ks, -126.0f, 0x1p126f, 0.0f) : make_float4(ks, log2f(vs), 1.0f / vs, 0.0f);
-                info[(j % C::kInfo) * C::kGroups + ct] = f;
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&k_full[j % C::kKStages]);
-        };
-        if (tiles > 0) {
-            ask_pages(0, ids);
-            fetch(g.cache.k_codes, 0, ids, k);
-            ask_scales(0);
-            fetch(g.cache.v_codes, 0, ids, v);
-            ask_pages(1, ids);
-            put_k(0);
-            fetch(g.cache.k_codes, 1, ids, k);
-            ask_scales(1);
-            ask_pages(2, later);
-        }
-        bool ok = true;
-        // K of tile j + 1 before V of tile j: its scores are computed first.
-        for (int j = 0; j < tiles; ++j) {
-            if (j + 1 < tiles) {
-                if (j + 1 >= C::kKStages) ok = __all_sync(~0u, tile_wait(watch, &k_empty[(j + 1) % C::kKStages], ((j + 1) / C::kKStages - 1) & 1));
-                if (!ok) break;
-                put_k(j + 1);
+            // Turn j: K of tile j + 1, V of tile j (its scores are computed first), and
+            // the loads of K of tile j + 2, V of tile j + 1.
+#pragma unroll 1
+            for (int j = it >= 0 ? -2 : tiles; j < tiles; ++j) {
+                if (j >= -1 && j + 1 < tiles) {
+                    put_k(j + 1);
+                    if (!ok) break;
+                }
                 fetch(g.cache.k_codes, j + 2, later, k);
                 ask_scales(j + 2);
-            }
-            const int stage = j % C::kVStages;
-            if (j >= C::kVStages) ok = __all_sync(~0u, tile_wait(watch, &v_empty[stage], (j / C::kVStages - 1) & 1));
-            if (!ok) break;
-            convert(v, v_tiles + stage * C::kKvBytes);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&v_full[stage]);
-            fetch(g.cache.v_codes, j + 1, ids, v);
+                if (j == -2) {
+                    put_rows(now, item->power);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(q_full);
+                }
+                if (j >= 0) {
+                    const int tile = n + j, stage = tile % C::kVStages;
+                    if (tile >= C::kVStages) ok = __all_sync(~0u, tile_wait(watch, &v_empty[stage], (tile / C::kVStages - 1) & 1));
+                    if (!ok) break;
+                    convert(v, v_tiles + stage * C::kKvBytes);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&v_full[stage]);
+                }
+                if (j >= -1) fetch(g.cache.v_codes, j + 1, ids, v);
 #pragma unroll
-            for (int n = 0; n < C::kPieces; ++n) ids[n] = later[n];
-            ask_pages(j + 3, later);
+                for (int i = 0; i < C::kPieces; ++i) ids[i] = later[i];
+                ask_pages(j + 3, later);
+            }
+            if (!ok) break;
+            if (it >= 0) n += tiles;
+            now = next;
         }
     } else {
         // ------------------------------------------------------ MMA issue
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
-        if (tiles > 0 && lane == 0) {
+        if constexpr (C::kOtherRegs < C::kLaunchRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+        if (lane == 0) {
             constexpr uint32_t s_desc = umma_idesc_f16(C::kRows, C::kKeys, false), o_desc = umma_idesc_f16(C::kRows, C::kOutCols, true);
             const uint32_t qh = smem_u32(q_hi), ql = smem_u32(q_lo), kt = smem_u32(k_tiles), vt = smem_u32(v_tiles);
-            // S of tile j, into the buffer that PV of tile j - 2 reads: MMAs of
-            // unlike accumulators keep no order, so that one is waited for.
-            const auto scores = [&](int j) {
-                const int stage = j % C::kKStages;
-                if (!tile_wait(watch, &k_full[stage], (j / C::kKStages) & 1)) return false;
-                if (j >= 2 && !tile_wait(watch, o_done, j & 1)) return false;
+            // S of tile n, into the buffer that PV of tile n - 2 reads: MMAs of
+            // unlike accumulators keep no order, so that one is waited for (an
+            // item's first: PV of tile n - 1, which has been issued before).
+            const auto scores = [&](int n, bool first) {
+                const int stage = n % C::kKStages;
+                if (!tile_wait(watch, &k_full[stage], (n / C::kKStages) & 1)) return false;
+                if (n >= (first ? 1 : 2) && !tile_wait(watch, o_done, (first ? n - 1 : n) & 1)) return false;
                 tcgen05_fence_after();
 #pragma unroll
                 for (int part = 0; part < 2; ++part)
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i)
-                        umma_f16(tmem + (j & 1) * C::kKeys,
+                        umma_f16(tmem + (n & 1) * C::kKeys,
                                  umma_desc_k_sw128((part == 0 ? ql : qh) + (i >> 2) * (C::kRows * 128)) + 2 * (i & 3),
                                  umma_desc_k_sw128(kt + stage * C::kKvBytes + (i >> 2) * (C::kKeys * 128)) + 2 * (i & 3), s_desc,
                                  part > 0 || i > 0);
                 umma_commit(&k_empty[stage]);
-                umma_commit(&s_full[j & 1]);
+                umma_commit(&s_full[n & 1]);
                 return true;
             };
-            bool ok = tile_wait(watch, q_full, 0) && scores(0);
-            for (int j = 0; j < tiles && ok; ++j) {
-                if (j + 1 < tiles) ok = scores(j + 1);
-                const int stage = j % C::kVStages;
-                if (!ok || !tile_wait(watch, &v_full[stage], (j / C::kVStages) & 1) ||
-                    !tile_wait(watch, &p_full[j & 1], (j >> 1) & 1))
-                    break;
-                tcgen05_fence_after();
+            int n = 0;
+            bool ok = true;
+            for (int it = 0; ok; ++it) {
+                if (!tile_wait(watch, q_full, it & 1)) break;
+                const int tiles = item->tiles;
+                if (tiles < 0) break;
+#pragma unroll 1
+                for (int j = -1; j < tiles && ok; ++j) {
+                    if (j + 1 < tiles) {
+                        ok = scores(n + (j >= 0), j < 0);
+                        if (j + 2 == tiles) umma_commit(q_empty);
+                    }
+                    if (j < 0) continue;
+                    const int stage = n % C::kVStages;
+                    ok = ok && tile_wait(watch, &v_full[stage], (n / C::kVStages) & 1) &&
+                         tile_wait(watch, &p_full[n & 1], (n >> 1) & 1);
+                    if (!ok) break;
+                    tcgen05_fence_after();
 #pragma unroll
-                for (int i = 0; i < C::kKeys / 16; ++i)
+                    for (int i = 0; i < C::kKeys / 16; ++i)
 #pragma unroll
-                    for (int part = 0; part < 2; ++part)
-                        umma_f16_ta(o_tmem, tmem + (j & 1) * C::kKeys + (i >> 1) * 32 + part * 16 + (i & 1) * 8,
-                                    umma_desc_mn_sw128(vt + stage * C::kKvBytes + i * 2048, C::kKeys * 128), o_desc,
-                                    j % C::kSpan > 0 || i > 0 || part > 0);
-                umma_commit(&v_empty[stage]);
-                umma_commit(o_done);
+                        for (int part = 0; part < 2; ++part)
+                            umma_f16_ta(o_tmem, tmem + (n & 1) * C::kKeys + (i >> 1) * 32 + part * 16 + (i & 1) * 8,
+                                        umma_desc_mn_sw128(vt + stage * C::kKvBytes + i * 2048, C::kKeys * 128), o_desc,
+                                        j % C::kSpan > 0 || i > 0 || part > 0);
+                    umma_commit(&v_empty[stage]);
+                    umma_commit(o_done);
+                    ++n;
+                }
+                umma_commit(item_done);
             }
-            umma_commit(drained);  // all that was issued has completed: the output may be read, the block may end
+            umma_commit(drained);  // whatever was issued has completed before the block ends
             tile_wait(watch, drained, 0);
         }
     }
     __syncwarp();
     tcgen05_fence_before();
     __syncthreads();
-    if (warp == 7) {
+    if (warp == kMmaWarp) {
         tcgen05_fence_after();
         tmem_dealloc(tmem, C::kTmemCols);
     }
@@ -699,13 +790,15 @@ int run_tile(cudaStream_t s, const Kv8AttendArgs& g, bool pdl) {
         cudaFuncAttributes a;
         return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0;
     }();
-    if (registers != 128) {  // setmaxnreg would wait for registers that the launch does not have
-        set_error("leafq_kv8_attention: the tile kernel was built with " + std::to_string(registers) + " registers a thread, not 128");
+    if (TileShape<D>::kSoftmaxRegs > TileShape<D>::kLaunchRegs && registers != TileShape<D>::kLaunchRegs) {  // setmaxnreg would wait for registers that the launch does not have
+        set_error("leafq_kv8_attention: the tile kernel was built with " + std::to_string(registers) + " registers a thread, not " +
+                  std::to_string(TileShape<D>::kLaunchRegs));
         return LEAFQ_ERR_CUDA;
     }
     st = allow_smem(kernel, TileShape<D>::kSmem, "leafq_kv8_attention");
     if (st) return st;
-    return launch(kv8_attend_tile_kernel<D>, dim3(static_cast<unsigned>(row_tiles * g.cache.kv_heads)),
+    const int64_t blocks = std::min<int64_t>(row_tiles * g.cache.kv_heads, 2 * (int64_t)sm_count());
+    return launch(kv8_attend_tile_kernel<D>, dim3(static_cast<unsigned>(blocks)),
                   dim3(TileShape<D>::kThreads), TileShape<D>::kSmem, s, pdl, "leafq_kv8_attention", g, watch,
                   static_cast<int>(row_tiles));
 }
