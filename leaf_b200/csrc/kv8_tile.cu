@@ -66,7 +66,7 @@ struct TileShape {
     static constexpr int kSoftmaxRegs = D <= 64 ? 128 : 112, kOtherRegs = D <= 64 ? 128 : 80;
     static constexpr int kConverters = kConvWarps * 32;
     static constexpr int kAllPieces = kKeys * D / 16;    // 16-byte pieces of a K (or V) tile
-    static constexpr int kPieces = (kAllPieces + kConverters - 1) / kConverters;
+    static constexpr int kPieces = kAllPieces / kConverters;
     static constexpr int kOutCols = kBlocks * 64;        // O columns (those past D are not read)
     static constexpr uint32_t kTmemCols = 256;
     static constexpr bool kSumInSmem = D <= 64;          // else in local memory
@@ -165,12 +165,6 @@ __device__ __forceinline__ void store_local(uint32_t at, float4 v) {
     asm volatile("st.local.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
 template <int D>
 __global__ void __launch_bounds__(TileShape<D>::kThreads, 2)
 kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_tiles) {
@@ -265,9 +259,9 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
             if (tiles < 0) break;
             const int r = tid;
             const int t = token_of(first_row + r), hq = (first_row + r) - t * g.group;
-            const int64_t pos = (int64_t)context + t;
+            const int pos = context + t;
             const bool seen = r < rows && pos >= 0 && (g.rotary == 0 || pos < g.table_rows);
-            const int limit = seen ? static_cast<int>(min64(keys, pos + 1)) : 0;
+            const int limit = seen ? min(keys, pos + 1) : 0;
             float* out = g.out + ((int64_t)row0 + t) * g.heads * D + (int64_t)(head * g.group + hq) * D;
             float m = -INFINITY, l = 0.0f, m_sum = -INFINITY;
             for (int j = 0; j < tiles; ++j, ++n) {
@@ -300,7 +294,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                         const float* at = reinterpret_cast<const float*>(x) + 16 * half;
                         float most = fmaxf(at[0], at[1]);
 #pragma unroll
-                        for (int e = 2; e < 16; e += 2) most = max3(most, at[e], at[e + 1]);
+                        for (int e = 2; e < 16; ++e) most = fmaxf(most, at[e]);
                         const float4 scale = scales[2 * c + half];
                         top = fmaxf(top, fmaf(most, slope(scale.x), scale.y));
                     }
@@ -457,25 +451,24 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 next.head = static_cast<int>(id - group_of * g.cache.kv_heads);
                 int s = 0;
                 for (int left = g.step.requests; left > 1;) {
-                    const int step = (left + 31) / 32, at = s + lane * step;
-                    const bool below = lane * step < left && ((int64_t)g.step.token_offsets[at] * g.group >> 7) + at <= index;
+                    const int step = (left + 31) >> 5, at = s + lane * step;
+                    const bool below = lane * step < left && (g.step.token_offsets[at] * g.group >> 7) + at <= index;
                     const int hit = max(__popc(__ballot_sync(~0u, below)) - 1, 0);
                     s += hit * step;
                     left = min(step, left - hit * step);
                 }
-                const int64_t row0 = max64(0, g.step.token_offsets[s]);
-                const int64_t new_rows =
-                    max64(0, min64(min64(g.step.token_offsets[s + 1], g.step.tokens) - row0, g.most_tokens)) * g.group;
-                const int64_t tile_index = index - ((row0 * g.group >> 7) + s);
+                const int begin = max(0, g.step.token_offsets[s]), end = min(g.step.token_offsets[s + 1], static_cast<int>(g.step.tokens));
+                const int new_rows = max(0, end - begin) * g.group;
+                const int tile_index = index - ((begin * g.group >> 7) + s);
                 if (tile_index < 0 || tile_index * C::kRows >= new_rows) continue;
-                next.row0 = static_cast<int>(row0);
-                next.first_row = static_cast<int>(tile_index) * C::kRows;
-                next.rows = static_cast<int>(min64(C::kRows, new_rows - next.first_row));
+                next.row0 = begin;
+                next.first_row = tile_index * C::kRows;
+                next.rows = min(C::kRows, new_rows - next.first_row);
                 next.context = g.step.context[s];
                 next.request = s;
-                const int64_t held = min64(g.step.page_offsets[s + 1] - g.step.page_offsets[s], g.step.max_pages);
-                next.keys = static_cast<int>(max64(
-                    0, min64(min64(held << g.shift, g.step.lengths[s]), (int64_t)next.context + token_of(next.first_row + next.rows - 1) + 1)));
+                const int held = min(g.step.page_offsets[s + 1] - g.step.page_offsets[s], static_cast<int>(g.step.max_pages));
+                const int seen = next.context + token_of(next.first_row + next.rows - 1) + 1;  // by the last row
+                next.keys = max(0, min(min(held << g.shift, g.step.lengths[s]), seen));
                 ++round;
                 return true;
             }
@@ -555,21 +548,25 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 }
             }
         };
-        // Four pieces a row and 64-element block at a time: eight lanes then store
-        // to eight different bank groups.
+        // This thread's piece i of a tile: its key row and its place in the row.  Four
+        // pieces a row and 64-element block at a time, where there are as many: eight
+        // lanes then store to eight different bank groups.
+        static_assert(C::kPieces * C::kConverters == C::kAllPieces, "whole pieces");
         const auto row_of = [&](int i) {
-            const int q = i * C::kConverters + ct;
-            return kRowPieces % 4 == 0 ? (q >> 2) % C::kKeys : q / kRowPieces;
+            if (D == 128) return (i & 1) * 32 + (ct >> 2);
+            if (D == 64) return i * 24 + (ct >> 2);
+            if (D == 32) return i * 48 + (ct >> 1);
+            return i < 2 ? i * 32 + (ct >> 2) : ct >> 1;
         };
         const auto piece_of = [&](int i) {
-            const int q = i * C::kConverters + ct;
-            return kRowPieces % 4 == 0 ? (q & 3) + 4 * (q / (4 * C::kKeys)) : q % kRowPieces;
+            if (D == 128) return (ct & 3) + 4 * (i >> 1);
+            if (D == 64) return ct & 3;
+            if (D == 32) return ct & 1;
+            return i < 2 ? ct & 3 : 4 + (ct & 1);
         };
-        const auto mine = [&](int i) { return C::kAllPieces % C::kConverters == 0 || i * C::kConverters + ct < C::kAllPieces; };
         const auto convert = [&](const uint4 (&w)[C::kPieces], uint8_t* tile) {
 #pragma unroll
             for (int i = 0; i < C::kPieces; ++i) {
-                if (!mine(i)) continue;
                 const int row = row_of(i), cc = piece_of(i);
                 const uint32_t b[4] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u, w[i].z ^ 0x80808080u, w[i].w ^ 0x80808080u};
                 uint8_t* line = tile + (cc >> 2) * (C::kKeys * 128) + row * 128;
@@ -620,7 +617,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                     const int key = j * C::kKeys + row_of(i);
                     const int inside = (key & (page - 1)) * D + piece_of(i) * 16;
                     w[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (mine(i) && key < keys && static_cast<uint32_t>(ids[i]) < static_cast<uint32_t>(g.cache.pages))
+                    if (key < keys && static_cast<uint32_t>(ids[i]) < static_cast<uint32_t>(g.cache.pages))
                         w[i] = load_now(reinterpret_cast<const uint4*>(codes + (ids[i] * page_bytes + (head_bytes + inside))));
                 }
             };
@@ -629,7 +626,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
             float ks = 0.0f, vs = -1.0f;  // the group's scales; -1: not there
             const auto ask_pages = [&](int j, int32_t (&into)[C::kPieces]) {
 #pragma unroll
-                for (int i = 0; i < C::kPieces; ++i) into[i] = page_of(j, min(row_of(i), C::kKeys - 1));
+                for (int i = 0; i < C::kPieces; ++i) into[i] = page_of(j, row_of(i));
                 if (ct < C::kGroups) group_id = page_of(j, 16 * ct);
             };
             const auto ask_scales = [&](int j) {
@@ -781,7 +778,7 @@ int run_tile(cudaStream_t s, const Kv8AttendArgs& g, bool pdl) {
     int st = device_watch(&watch);
     if (st) return st;
     const int64_t row_tiles = (g.step.tokens * g.group >> 7) + g.step.requests;
-    if (row_tiles * g.cache.kv_heads > INT_MAX) {
+    if (row_tiles * g.cache.kv_heads > INT_MAX || g.step.tokens * g.group > INT_MAX) {
         set_error("leafq_kv8_attention: too many rows");
         return LEAFQ_ERR_INVALID;
     }
