@@ -17,9 +17,10 @@ namespace {
 // under the other's softmax.  Roles:
 //   warps 0-3  softmax: one row per thread (its TMEM lane), a tile's scores in
 //              registers
-//   warps 4-6  codes to fp16: 16-byte global loads a tile ahead, byte
-//              permutes, 128-byte-swizzled shared memory
-//   warp 7     MMA issue (kind::f16, fp32 accumulators in TMEM)
+//   warps 4-7  the items and their query rows; codes to fp16 (two warps K, two
+//              V): 16-byte global loads a tile ahead, byte permutes,
+//              128-byte-swizzled shared memory
+//   warp 8     MMA issue (kind::f16, fp32 accumulators in TMEM)
 // The softmax warps take registers that the others leave (setmaxnreg).  S has
 // two buffers: the next tile's scores are computed under this tile's softmax.
 // The arithmetic is the split form's: codes exact in fp16, fp32 operands as
@@ -55,18 +56,13 @@ struct TileShape {
     static constexpr int kQBytes = kBlocks * kRows * 128;
     static constexpr int kKvBytes = kBlocks * kKeys * 128;
     static constexpr int kSpan = 512 / kKeys;            // tiles between O's additions to the rounded sum
-    // Converting warps and the registers of the launch, of the softmax warps, of the
-    // others.  (Nine warps put five on one of the SM's four schedulers, so the
-    // launch gives 96 registers a thread; eight give 128.)  Registers belong to a
-    // scheduler: a softmax warp can take only what the converting warp beside it,
-    // four warps on, has left.
-    static constexpr int kConvWarps = D <= 64 ? 3 : 4;
-    static constexpr int kThreads = (4 + kConvWarps + 1) * 32;
-    static constexpr int kLaunchRegs = D <= 64 ? 128 : 96;
-    static constexpr int kSoftmaxRegs = D <= 64 ? 128 : 112, kOtherRegs = D <= 64 ? 128 : 80;
-    static constexpr int kConverters = kConvWarps * 32;
-    static constexpr int kAllPieces = kKeys * D / 16;    // 16-byte pieces of a K (or V) tile
-    static constexpr int kPieces = kAllPieces / kConverters;
+    // Two warps convert K, two V.  Registers of the launch, of the softmax warps, of
+    // the others: nine warps put five on one of the SM's four schedulers, so the
+    // launch gives 96 a thread.  They belong to a scheduler: a softmax warp can take
+    // only what the converting warp beside it, four warps on, has left.
+    static constexpr int kThreads = 9 * 32;
+    static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 104, kOtherRegs = 88;
+    static constexpr int kPieces = kKeys * D / 16 / 64;  // 16-byte pieces of a K (or V) tile per converting thread
     static constexpr int kOutCols = kBlocks * 64;        // O columns (those past D are not read)
     static constexpr uint32_t kTmemCols = 256;
     static constexpr bool kSumInSmem = D <= 64;          // else in local memory
@@ -75,8 +71,7 @@ struct TileShape {
                                     sizeof(TileItem) + (2 * kKStages + 2 * kVStages + 9) * 8 + 8;
     static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two blocks share the SM's shared memory");
     static_assert(2 * kKeys + kOutCols <= 256, "two blocks share the SM's 512 TMEM columns");
-    static_assert(kSoftmaxRegs + kOtherRegs <= 2 * kLaunchRegs && kOtherRegs <= kLaunchRegs && kConvWarps >= 3,
-                  "the split of what the launch gives each scheduler");
+    static_assert(kSoftmaxRegs + kOtherRegs <= 2 * kLaunchRegs, "the split of what the launch gives each scheduler");
 };
 
 // The library's device error word and wait limit (leafq_device.cuh), which this
@@ -190,7 +185,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
     uint64_t* drained = item_done + 1;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int kMmaWarp = 4 + C::kConvWarps;
+    constexpr int kMmaWarp = 8;
     const auto token_of = [&](int row) { return static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(g.group)); };
 
     if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled tiles need it; dynamic shared memory starts there
@@ -200,11 +195,11 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
     if (warp == kMmaWarp) {
         if (lane == 0) {
             for (int i = 0; i < C::kKStages; ++i) {
-                mbar_init(&k_full[i], C::kConvWarps);
+                mbar_init(&k_full[i], 2);
                 mbar_init(&k_empty[i], 1);
             }
             for (int i = 0; i < C::kVStages; ++i) {
-                mbar_init(&v_full[i], C::kConvWarps);
+                mbar_init(&v_full[i], 2);
                 mbar_init(&v_empty[i], 1);
             }
             for (int i = 0; i < 2; ++i) {
@@ -212,7 +207,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 mbar_init(&p_full[i], 4);
             }
             mbar_init(o_done, 1);
-            mbar_init(q_full, C::kConvWarps);
+            mbar_init(q_full, 4);
             mbar_init(q_empty, 1 + 4);
             mbar_init(item_done, 1);
             mbar_init(drained, 1);
@@ -234,7 +229,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
     // phases are waited for in order by every role.
     if (warp < 4) {
         // ------------------------------------------------------- softmax
-        if constexpr (C::kSoftmaxRegs > C::kLaunchRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
         float4* my_sum = sum_s + warp * (D / 4) * 32;
         __align__(16) float o_sum[C::kSumInSmem ? 4 : D];  // the rounded sum
@@ -272,9 +267,11 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 const float4* scales = info + (n % C::kInfo) * C::kGroups;
                 const int visible = limit - j * C::kKeys;  // columns of this tile that the row sees
                 const bool whole = __all_sync(~0u, visible >= C::kKeys);
-                // 32 scores at a time, read twice: the loops' code has to stay in the
-                // instruction cache beside the other roles'.  What is not seen is -inf.
-                const auto read = [&](int c, uint32_t (&x)[32]) {
+                // 32 scores at a time, read twice, by rolled loops: the roles' loops have to
+                // stay in the instruction cache side by side (unrolled, with all scores in
+                // registers, the kernel took 1.5 times as long).  What is not seen is -inf.
+                uint32_t x[32];
+                const auto read = [&](int c) {
                     tmem_ld_32x32b_x32(s_tmem + lanes + 32 * c, x);
                     tmem_wait_ld();
                     if (!whole) {
@@ -287,8 +284,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 float top = -INFINITY;
 #pragma unroll 1
                 for (int c = 0; c < C::kKeys / 32; ++c) {
-                    uint32_t x[32];
-                    read(c, x);
+                    read(c);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const float* at = reinterpret_cast<const float*>(x) + 16 * half;
@@ -329,8 +325,8 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 const float shift = m == -INFINITY ? 0.0f : m - kTileLift;
 #pragma unroll 1
                 for (int c = 0; c < C::kKeys / 32; ++c) {
-                    uint32_t x[32], p[32];
-                    read(c, x);
+                    uint32_t p[32];
+                    read(c);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const float4 scale = scales[2 * c + half];
@@ -426,11 +422,10 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
         }
     } else if (warp < kMmaWarp) {
         // ------------------------------- the items, their rows, codes to fp16
-        if constexpr (C::kOtherRegs < C::kLaunchRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
-        const int ct = tid - 128, cw = warp - 4;
-        constexpr int kRowPieces = D / 16;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+        const int cw = warp - 4;
         const int page = 1 << g.shift;
-        const int64_t page_bytes = ((int64_t)g.cache.kv_heads << g.shift) * D;
+        const uint32_t page_pieces = (static_cast<uint32_t>(g.cache.kv_heads) << g.shift) * (D / 16);  // 16-byte pieces of a page
 
         // Items: row tiles x kv heads, those that see most keys first, dealt to the
         // blocks back and forth.  Request s may have row tiles
@@ -441,6 +436,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
         };
         int round = 0;
         const auto advance = [&](Next& next) {
+#pragma unroll 1
             for (;; ++round) {
                 const uint32_t base = static_cast<uint32_t>(round) * gridDim.x;
                 if (base >= total) return false;
@@ -450,6 +446,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 const int index = row_tiles - 1 - static_cast<int>(group_of);
                 next.head = static_cast<int>(id - group_of * g.cache.kv_heads);
                 int s = 0;
+#pragma unroll 1
                 for (int left = g.step.requests; left > 1;) {
                     const int step = (left + 31) >> 5, at = s + lane * step;
                     const bool below = lane * step < left && (g.step.token_offsets[at] * g.group >> 7) + at <= index;
@@ -475,44 +472,46 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
         };
         // Lanes of a row: D / 8, eight values each (a rotation pair's quarters).
         constexpr int kLanes = D / 8;  // 4, 8, 12, 16
-        constexpr int kAtOnce = 32 / kLanes, kPass = C::kConvWarps * kAtOnce;
+        constexpr int kAtOnce = 32 / kLanes, kPass = 4 * kAtOnce;
         constexpr int kTurns = (C::kRows + kPass - 1) / kPass;
         const int sub = lane / kLanes, part = lane - sub * kLanes;
         const int half = g.rotary >> 1;
         const bool turned = 4 * part < half;
         const int at = turned ? 4 * part : 2 * half + 4 * (part - half / 4);
         const int to = turned ? at + half : at + ((D - 2 * half) >> 1);
-        // Loads run a turn ahead; rotated, scaled by the row's power of two, split,
+        // Loads run two turns ahead; rotated, scaled by the row's power of two, split,
         // stored swizzled.
         const auto put_rows = [&](const Next& next, uint8_t* power) {
-            float4 a, b, cs, sn;
-            const auto ask = [&](int turn_index) {
-                const int r = turn_index * kPass + cw * kAtOnce + sub;
-                a = b = sn = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                cs = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-                if (sub < kAtOnce && r < next.rows) {
-                    const int t = token_of(next.first_row + r), hq = (next.first_row + r) - t * g.group;
+            float4 a, b, cs, sn, a1, b1, cs1, sn1;  // this turn's, the next one's
+            a = b = cs = sn = a1 = b1 = cs1 = sn1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+            for (int i = -2; i < kTurns; ++i) {
+                float v[8];
+                {
+                    float4 x = a, y = b;
+                    if (turned) turn(x, y, cs, sn);
+                    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+                }
+                a = a1, b = b1, cs = cs1, sn = sn1;
+                const int ahead = (i + 2) * kPass + cw * kAtOnce + sub;
+                a1 = b1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (sub < kAtOnce && ahead < next.rows) {
+                    const int t = token_of(next.first_row + ahead), hq = (next.first_row + ahead) - t * g.group;
                     const float* src = g.q + ((int64_t)next.row0 + t) * g.q_stride + (int64_t)(next.head * g.group + hq) * D;
-                    a = load_now(reinterpret_cast<const float4*>(src + at));
-                    b = load_now(reinterpret_cast<const float4*>(src + to));
+                    a1 = load_now(reinterpret_cast<const float4*>(src + at));
+                    b1 = load_now(reinterpret_cast<const float4*>(src + to));
                     if (turned) {
                         int64_t pos = (int64_t)next.context + t;
                         if (pos < 0 || pos >= g.table_rows) {
                             if (part == 0) report(watch, kSiteKv8Range);
                             pos = 0;
                         }
-                        cs = load_now(reinterpret_cast<const float4*>(g.cos_table + pos * half + at));
-                        sn = load_now(reinterpret_cast<const float4*>(g.sin_table + pos * half + at));
+                        cs1 = load_now(reinterpret_cast<const float4*>(g.cos_table + pos * half + at));
+                        sn1 = load_now(reinterpret_cast<const float4*>(g.sin_table + pos * half + at));
                     }
                 }
-            };
-            ask(0);
-#pragma unroll 1
-            for (int i = 0; i < kTurns; ++i) {
+                if (i < 0) continue;
                 const int r = i * kPass + cw * kAtOnce + sub;
-                if (turned) turn(a, b, cs, sn);
-                const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                if (i + 1 < kTurns) ask(i + 1);
                 // A NaN is no maximum, but it stays one in its row's products.
                 float largest = fabsf(v[0]);
 #pragma unroll
@@ -548,36 +547,27 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 }
             }
         };
+        // Warps 4 and 5 convert K, 6 and 7 V, by the same code.
+        const bool is_k = cw < 2;
+        const int ct = tid & 63, stages = is_k ? C::kKStages : C::kVStages;
+        const uint4* codes = reinterpret_cast<const uint4*>(is_k ? g.cache.k_codes : g.cache.v_codes);
+        uint8_t* tiles_s = is_k ? k_tiles : v_tiles;
+        uint64_t *full = is_k ? k_full : v_full, *empty = is_k ? k_empty : v_empty;
         // This thread's piece i of a tile: its key row and its place in the row.  Four
         // pieces a row and 64-element block at a time, where there are as many: eight
         // lanes then store to eight different bank groups.
-        static_assert(C::kPieces * C::kConverters == C::kAllPieces, "whole pieces");
         const auto row_of = [&](int i) {
-            if (D == 128) return (i & 1) * 32 + (ct >> 2);
-            if (D == 64) return i * 24 + (ct >> 2);
-            if (D == 32) return i * 48 + (ct >> 1);
-            return i < 2 ? i * 32 + (ct >> 2) : ct >> 1;
+            if (D == 128) return (i & 3) * 16 + (ct >> 2);
+            if (D == 64) return i * 16 + (ct >> 2);
+            if (D == 32) return i * 32 + (ct >> 1);
+            return i < 4 ? i * 16 + (ct >> 2) : (i - 4) * 32 + (ct >> 1);
         };
         const auto piece_of = [&](int i) {
-            if (D == 128) return (ct & 3) + 4 * (i >> 1);
+            if (D == 128) return (ct & 3) + 4 * (i >> 2);
             if (D == 64) return ct & 3;
             if (D == 32) return ct & 1;
-            return i < 2 ? ct & 3 : 4 + (ct & 1);
+            return i < 4 ? ct & 3 : 4 + (ct & 1);
         };
-        const auto convert = [&](const uint4 (&w)[C::kPieces], uint8_t* tile) {
-#pragma unroll
-            for (int i = 0; i < C::kPieces; ++i) {
-                const int row = row_of(i), cc = piece_of(i);
-                const uint32_t b[4] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u, w[i].z ^ 0x80808080u, w[i].w ^ 0x80808080u};
-                uint8_t* line = tile + (cc >> 2) * (C::kKeys * 128) + row * 128;
-                const int chunk = (cc & 3) * 2;
-                *reinterpret_cast<uint4*>(line + ((chunk ^ (row & 7)) << 4)) =
-                    make_uint4(codes_half2(b[0], 0x4140u), codes_half2(b[0], 0x4342u), codes_half2(b[1], 0x4140u), codes_half2(b[1], 0x4342u));
-                *reinterpret_cast<uint4*>(line + (((chunk + 1) ^ (row & 7)) << 4)) =
-                    make_uint4(codes_half2(b[2], 0x4140u), codes_half2(b[2], 0x4342u), codes_half2(b[3], 0x4140u), codes_half2(b[3], 0x4342u));
-            }
-        };
-
         Next now = {}, next;
         bool more = false, ok = true;
         int n = 0;  // tiles of the items before
@@ -588,7 +578,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
             if (!ok) break;
             const int keys = more ? now.keys : 0;
             const int tiles = more ? max(1, (keys + C::kKeys - 1) / C::kKeys) : -1;  // without keys, a tile that is all hidden
-            if (it >= 0 && ct == 0) {
+            if (it >= 0 && tid == 128) {
                 item->row0 = now.row0;
                 item->first_row = now.first_row;
                 item->rows = now.rows;
@@ -603,36 +593,32 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 break;
             }
             const int32_t* table = g.step.table + (int64_t)now.request * g.step.max_pages;
-            const int64_t head_bytes = ((int64_t)now.head << g.shift) * D;
+            const uint32_t head_pieces = (static_cast<uint32_t>(now.head) << g.shift) * (D / 16);
             // Loads are asked for where they stand: the page numbers of a tile two
             // tiles ahead, its codes and scales one.
+            int32_t ids[C::kPieces], group_id = 0;  // pages of the pieces; of 16-key group ct in the first lanes
+            uint4 w[C::kPieces];
+            float ks = 0.0f, vs = -1.0f;            // the group's scales; -1: not there
             const auto page_of = [&](int j, int row) {  // of key row `row` of tile j; past the keys: some page
                 const int key = min(j * C::kKeys + row, keys - 1);
                 return keys > 0 ? load_now(table + (key >> g.shift)) : -1;
             };
-            // The pieces of tile j, whose pages are ids; zeros where there is no key.
-            const auto fetch = [&](const int8_t* codes, int j, const int32_t (&ids)[C::kPieces], uint4 (&w)[C::kPieces]) {
+            const auto ask_pages = [&](int j) {
+#pragma unroll
+                for (int i = 0; i < C::kPieces; ++i) ids[i] = page_of(j, row_of(i));
+                if (is_k && ct < C::kGroups) group_id = page_of(j, 16 * ct);
+            };
+            const auto fetch = [&](int j) {  // tile j, whose pages are there; zeros where there is no key
 #pragma unroll
                 for (int i = 0; i < C::kPieces; ++i) {
                     const int key = j * C::kKeys + row_of(i);
-                    const int inside = (key & (page - 1)) * D + piece_of(i) * 16;
                     w[i] = make_uint4(0u, 0u, 0u, 0u);
                     if (key < keys && static_cast<uint32_t>(ids[i]) < static_cast<uint32_t>(g.cache.pages))
-                        w[i] = load_now(reinterpret_cast<const uint4*>(codes + (ids[i] * page_bytes + (head_bytes + inside))));
+                        w[i] = load_now(codes + (ids[i] * page_pieces + (head_pieces + (key & (page - 1)) * (D / 16) + piece_of(i))));
                 }
-            };
-            int32_t ids[C::kPieces], later[C::kPieces], group_id = 0;  // pages of the pieces of two tiles; of 16-key group ct in the first lanes
-            uint4 k[C::kPieces], v[C::kPieces];
-            float ks = 0.0f, vs = -1.0f;  // the group's scales; -1: not there
-            const auto ask_pages = [&](int j, int32_t (&into)[C::kPieces]) {
-#pragma unroll
-                for (int i = 0; i < C::kPieces; ++i) into[i] = page_of(j, row_of(i));
-                if (ct < C::kGroups) group_id = page_of(j, 16 * ct);
-            };
-            const auto ask_scales = [&](int j) {
                 ks = 0.0f;
                 vs = -1.0f;
-                if (ct < C::kGroups && j * C::kKeys + 16 * ct < keys) {
+                if (is_k && ct < C::kGroups && j * C::kKeys + 16 * ct < keys) {
                     if (static_cast<uint32_t>(group_id) < static_cast<uint32_t>(g.cache.pages)) {
                         const int64_t from = (int64_t)group_id * g.cache.kv_heads + now.head;
                         ks = load_now(g.cache.k_scales + from);
@@ -642,61 +628,57 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                     }
                 }
             };
-            const auto put_k = [&](int j) {  // k and the scales, into K of tile j
-                const int tile = n + j;
-                if (tile >= C::kKStages)
-                    ok = __all_sync(~0u, tile_wait(watch, &k_empty[tile % C::kKStages], (tile / C::kKStages - 1) & 1));
-                if (!ok) return;
-                convert(k, k_tiles + (tile % C::kKStages) * C::kKvBytes);
-                if (ct < C::kGroups) {
-                    float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);  // hides the group
-                    // A page of zeros counts in the sum as any other.
-                    if (!(vs < 0.0f)) f = vs == 0.0f ? make_float4(ks, -126.0f, 0x1p126f, 0.0f) : make_float4(ks, log2f(vs), __frcp_rn(vs), 0.0f);
-                    info[(tile % C::kInfo) * C::kGroups + ct] = f;
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&k_full[tile % C::kKStages]);
-            };
-            if (it >= 0) ask_pages(0, later);
+            if (it >= 0) ask_pages(0);
             // The next item meanwhile, and its rows into L2.
             more = advance(next);
             if (more) {
-                for (int i = ct; i < next.rows * (D / 32); i += C::kConverters) {
+#pragma unroll 1
+                for (int i = tid - 128; i < next.rows * (D / 32); i += 128) {
                     const int r = i / (D / 32), t = token_of(next.first_row + r), hq = (next.first_row + r) - t * g.group;
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(g.q + ((int64_t)next.row0 + t) * g.q_stride +
                                                                   (int64_t)(next.head * g.group + hq) * D + 32 * (i % (D / 32))));
                 }
             }
-            // Turn j: K of tile j + 1, V of tile j (its scores are computed first), and
-            // the loads of K of tile j + 2, V of tile j + 1.
+            if (it >= 0) {
+                put_rows(now, item->power);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
+                fetch(0);
+                ask_pages(1);
+            }
 #pragma unroll 1
-            for (int j = it >= 0 ? -2 : tiles; j < tiles; ++j) {
-                if (j >= -1 && j + 1 < tiles) {
-                    put_k(j + 1);
-                    if (!ok) break;
-                }
-                fetch(g.cache.k_codes, j + 2, later, k);
-                ask_scales(j + 2);
-                if (j == -2) {
-                    put_rows(now, item->power);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(q_full);
-                }
-                if (j >= 0) {
-                    const int tile = n + j, stage = tile % C::kVStages;
-                    if (tile >= C::kVStages) ok = __all_sync(~0u, tile_wait(watch, &v_empty[stage], (tile / C::kVStages - 1) & 1));
-                    if (!ok) break;
-                    convert(v, v_tiles + stage * C::kKvBytes);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&v_full[stage]);
-                }
-                if (j >= -1) fetch(g.cache.v_codes, j + 1, ids, v);
+            for (int j = 0; j < (it >= 0 ? tiles : 0); ++j) {
+                const int tile = n + j, stage = tile % stages;
+                if (tile >= stages) ok = __all_sync(~0u, tile_wait(watch, &empty[stage], (tile / stages - 1) & 1));
+                if (!ok) break;
+                uint8_t* to_tile = tiles_s + stage * C::kKvBytes;
 #pragma unroll
-                for (int i = 0; i < C::kPieces; ++i) ids[i] = later[i];
-                ask_pages(j + 3, later);
+                for (int i = 0; i < C::kPieces; ++i) {
+                    const int row = row_of(i), cc = piece_of(i), chunk = (cc & 3) * 2;
+                    const uint32_t b[4] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u, w[i].z ^ 0x80808080u, w[i].w ^ 0x80808080u};
+                    uint8_t* line = to_tile + (cc >> 2) * (C::kKeys * 128) + row * 128;
+                    *reinterpret_cast<uint4*>(line + ((chunk ^ (row & 7)) << 4)) =
+                        make_uint4(codes_half2(b[0], 0x4140u), codes_half2(b[0], 0x4342u), codes_half2(b[1], 0x4140u), codes_half2(b[1], 0x4342u));
+                    *reinterpret_cast<uint4*>(line + (((chunk + 1) ^ (row & 7)) << 4)) =
+                        make_uint4(codes_half2(b[2], 0x4140u), codes_half2(b[2], 0x4342u), codes_half2(b[3], 0x4140u), codes_half2(b[3], 0x4342u));
+                }
+                if (is_k && ct < C::kGroups) {
+                    float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);  // hides the group
+                    if (!(vs < 0.0f)) {
+                        // log2 vs and 1 / vs from an approximate logarithm a: with
+                        // vs 2^-a = 1 + d, log2 vs = a + d log2 e and 1 / vs = 2^-a (1 - d),
+                        // to d^2, about 2^-44.  A page of zeros counts in the sum as any other.
+                        const float a = vs == 0.0f ? -126.0f : lg2(vs), back = ex2(-a), d = vs == 0.0f ? 0.0f : fmaf(vs, back, -1.0f);
+                        f = make_float4(ks, fmaf(d, kLog2e, a), fmaf(-d, back, back), 0.0f);
+                    }
+                    info[(tile % C::kInfo) * C::kGroups + ct] = f;
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[stage]);
+                fetch(j + 1);
+                ask_pages(j + 2);
             }
             if (!ok) break;
             if (it >= 0) n += tiles;
@@ -704,7 +686,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
         }
     } else {
         // ------------------------------------------------------ MMA issue
-        if constexpr (C::kOtherRegs < C::kLaunchRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
         if (lane == 0) {
             constexpr uint32_t s_desc = umma_idesc_f16(C::kRows, C::kKeys, false), o_desc = umma_idesc_f16(C::kRows, C::kOutCols, true);
             const uint32_t qh = smem_u32(q_hi), ql = smem_u32(q_lo), kt = smem_u32(k_tiles), vt = smem_u32(v_tiles);
@@ -716,9 +698,9 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 if (!tile_wait(watch, &k_full[stage], (n / C::kKStages) & 1)) return false;
                 if (n >= (first ? 1 : 2) && !tile_wait(watch, o_done, (first ? n - 1 : n) & 1)) return false;
                 tcgen05_fence_after();
-#pragma unroll
+#pragma unroll 1
                 for (int part = 0; part < 2; ++part)
-#pragma unroll
+#pragma unroll 2
                     for (int i = 0; i < D / 16; ++i)
                         umma_f16(tmem + (n & 1) * C::kKeys,
                                  umma_desc_k_sw128((part == 0 ? ql : qh) + (i >> 2) * (C::kRows * 128)) + 2 * (i & 3),
@@ -746,7 +728,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                          tile_wait(watch, &p_full[n & 1], (n >> 1) & 1);
                     if (!ok) break;
                     tcgen05_fence_after();
-#pragma unroll
+#pragma unroll 1
                     for (int i = 0; i < C::kKeys / 16; ++i)
 #pragma unroll
                         for (int part = 0; part < 2; ++part)
@@ -778,6 +760,10 @@ int run_tile(cudaStream_t s, const Kv8AttendArgs& g, bool pdl) {
     int st = device_watch(&watch);
     if (st) return st;
     const int64_t row_tiles = (g.step.tokens * g.group >> 7) + g.step.requests;
+    if (g.cache.pages > UINT32_MAX / (((int64_t)g.cache.kv_heads << g.shift) * (D / 16))) {
+        set_error("leafq_kv8_attention: code pools of 64 GiB and more are not supported for prompts");
+        return LEAFQ_ERR_UNSUPPORTED;
+    }
     if (row_tiles * g.cache.kv_heads > INT_MAX || g.step.tokens * g.group > INT_MAX) {
         set_error("leafq_kv8_attention: too many rows");
         return LEAFQ_ERR_INVALID;
@@ -787,7 +773,7 @@ int run_tile(cudaStream_t s, const Kv8AttendArgs& g, bool pdl) {
         cudaFuncAttributes a;
         return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0;
     }();
-    if (TileShape<D>::kSoftmaxRegs > TileShape<D>::kLaunchRegs && registers != TileShape<D>::kLaunchRegs) {  // setmaxnreg would wait for registers that the launch does not have
+    if (registers != TileShape<D>::kLaunchRegs) {  // setmaxnreg would wait for registers that the launch does not have
         set_error("leafq_kv8_attention: the tile kernel was built with " + std::to_string(registers) + " registers a thread, not " +
                   std::to_string(TileShape<D>::kLaunchRegs));
         return LEAFQ_ERR_CUDA;
