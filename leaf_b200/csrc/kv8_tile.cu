@@ -28,13 +28,14 @@ namespace {
 //   S [128][keys] = Qhi K^T + Qlo K^T   Q and K K-major in shared memory
 //   O [128][D]   += Phi V + Plo V       P from TMEM, V as stored (MN-major)
 // Each 32 columns of S are replaced in place by 16 columns of P's hi pairs and
-// 16 of its lo pairs.  O is rescaled only when a row's maximum grows by more
-// than 2^kSlack since its reference was taken: weights then stay below
-// 2^(kTileLift + kSlack) < 65504, fp16's largest.  The MMA's additions truncate,
+// 16 of its lo pairs.  Weights are 2^kTileLift times their value relative to a
+// power of two that follows the row's maximum from below: 16 of them may sum up
+// to kHighest, so that none passes 65504, fp16's largest, before the reference
+// is raised and O rescaled.  The MMA's additions truncate,
 // which adds up over long sums (8192 keys: 5.5e-6 of the result), so every
 // kSpan keys O is added to a rounded sum (in local memory) and starts anew
 // -- and the lo halves of Q go first, while S is small.
-constexpr float kTileLift = 6.0f, kSlack = 8.0f;
+constexpr float kTileLift = 6.0f, kHighest = 49152.0f;
 
 // What the roles of a block need to know of an item: 128 query rows of one kv
 // head of a request.  tiles < 0: there are no more.
@@ -267,9 +268,9 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 const float4* scales = info + (n % C::kInfo) * C::kGroups;
                 const int visible = limit - j * C::kKeys;  // columns of this tile that the row sees
                 const bool whole = __all_sync(~0u, visible >= C::kKeys);
-                // 32 scores at a time, read twice, by rolled loops: the roles' loops have to
-                // stay in the instruction cache side by side (unrolled, with all scores in
-                // registers, the kernel took 1.5 times as long).  What is not seen is -inf.
+                // 32 scores at a time, by rolled loops: the roles' loops have to stay in the
+                // instruction cache side by side (unrolled, with all scores in registers,
+                // the kernel took 1.5 times as long).  What is not seen is -inf.
                 uint32_t x[32];
                 const auto read = [&](int c) {
                     tmem_ld_32x32b_x32(s_tmem + lanes + 32 * c, x);
@@ -281,75 +282,111 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 };
                 // From an MMA sum to x_j: above zero, so that -inf stays.
                 const auto slope = [&](float ks) { return ks * factor == 0.0f ? 1e-37f : ks * factor; };
-                float top = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < C::kKeys / 32; ++c) {
-                    read(c);
+                const auto largest = [&](int c) {  // x_j of the 32
+                    float top = -INFINITY;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const float* at = reinterpret_cast<const float*>(x) + 16 * half;
-                        float most = fmaxf(at[0], at[1]);
+                        float most = at[0];
 #pragma unroll
-                        for (int e = 2; e < 16; ++e) most = fmaxf(most, at[e]);
+                        for (int e = 1; e < 16; ++e) most = fmaxf(most, at[e]);
                         const float4 scale = scales[2 * c + half];
                         top = fmaxf(top, fmaf(most, slope(scale.x), scale.y));
                     }
-                }
-                // This tile's S means that PV of tile n - 2 is done: o_done is waited
-                // for one phase on at most, here and below.
+                    return top;
+                };
+                // The weights count relative to a whole power of two m.  It is taken from
+                // the first tile with a key for the row; later tiles are weighed with it as it stands, and
+                // only where weights come out above kHighest is it raised, with what has
+                // been weighed so far scaled down, exactly but for what is lost below
+                // 2^-30 of the largest.
                 const bool anew = j % C::kSpan == 0;
                 const float m_before = m;
-                if (anew) {
-                    // O starts anew with this tile: only L has a reference to keep.
-                    const float grown = fmaxf(m, top);
-                    l *= m == -INFINITY ? 0.0f : ex2(m - grown);
-                    m = grown;
-                } else if (__any_sync(~0u, top > m + kSlack)) {
-                    ok = __all_sync(~0u, tile_wait(watch, o_done, (n - 1) & 1));
-                    if (!ok) break;
-                    tcgen05_fence_after();
-                    const float grown = top > m + kSlack ? top : m;
-                    const float old = m == -INFINITY ? 0.0f : ex2(m - grown);
-                    m = grown;
-                    l *= old;
+                if (j == 0 || __any_sync(~0u, m == -INFINITY && visible > 0)) {
+                    float top = -INFINITY;
 #pragma unroll 1
-                    for (int c = 0; c < C::kOutCols / 32; ++c) {
-                        uint32_t y[32];
-                        tmem_ld_32x32b_x32(o_tmem + lanes + 32 * c, y);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * old);
-                        tmem_st_32x32b_x32(o_tmem + lanes + 32 * c, y);
+                    for (int c = 0; c < C::kKeys / 32; ++c) {
+                        read(c);
+                        top = fmaxf(top, largest(c));
                     }
+                    if (m == -INFINITY) m = ceilf(top);
                 }
-                const float shift = m == -INFINITY ? 0.0f : m - kTileLift;
 #pragma unroll 1
                 for (int c = 0; c < C::kKeys / 32; ++c) {
-                    uint32_t p[32];
                     read(c);
+                    uint32_t p[32];
+                    float weight;  // L of the 32
+#pragma unroll 1
+                    for (;;) {
+                        const float shift = m == -INFINITY ? 0.0f : m - kTileLift;
+                        bool high = false;
+                        weight = 0.0f;
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float4 scale = scales[2 * c + half];
-                        const float a1 = slope(scale.x), b1 = scale.y - shift;
-                        const unsigned long long a = pack2(a1, a1), b = pack2(b1, b1);
-                        unsigned long long sum = 0;
+                        for (int half = 0; half < 2; ++half) {
+                            const float4 scale = scales[2 * c + half];
+                            const float a1 = slope(scale.x), b1 = scale.y - shift;
+                            const unsigned long long a = pack2(a1, a1), b = pack2(b1, b1);
+                            unsigned long long sum = 0;
 #pragma unroll
-                        for (int e = 16 * half; e < 16 * half + 16; e += 2) {
-                            const float2 y = unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), a, b));
-                            const float w0 = ex2(y.x), w1 = ex2(y.y);
-                            const unsigned long long w = pack2(w0, w1);
-                            sum = add2(sum, w);
-                            const float h0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u);
-                            const float h1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
-                            const float2 low = unpack2(sub2(w, pack2(h0, h1)));
-                            p[e / 2] = half2_bits(h0, h1);
-                            p[16 + e / 2] = half2_bits(low.x, low.y);
+                            for (int e = 16 * half; e < 16 * half + 16; e += 2) {
+                                const float2 y = unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), a, b));
+                                const float w0 = ex2(y.x), w1 = ex2(y.y);
+                                const unsigned long long w = pack2(w0, w1);
+                                sum = add2(sum, w);
+                                const float h0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u);
+                                const float h1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
+                                const float2 low = unpack2(sub2(w, pack2(h0, h1)));
+                                p[e / 2] = half2_bits(h0, h1);
+                                p[16 + e / 2] = half2_bits(low.x, low.y);
+                            }
+                            const float2 both = unpack2(sum);
+                            high |= both.x + both.y > kHighest;
+                            weight = fmaf(both.x + both.y, scale.z, weight);
                         }
-                        const float2 both = unpack2(sum);
-                        l = fmaf(both.x + both.y, scale.z, l);
+                        if (!__any_sync(~0u, high)) break;
+                        // Raise m: the weights of this tile so far, O and L come down.
+                        const float raised = high ? fmaxf(m, ceilf(largest(c))) : m;
+                        const float down = m == -INFINITY ? 0.0f : ex2(m - raised);  // of a whole number: exact
+                        float left = m == -INFINITY ? 42.0f : fminf(raised - m, 42.0f);
+                        if (!(raised > m)) left = 0.0f;
+                        m = raised;
+                        l *= down;
+                        if (!anew) {
+                            // This tile's S means that PV of tile n - 2 is done, so o_done is
+                            // waited for one phase on at most, here and below.
+                            ok = __all_sync(~0u, tile_wait(watch, o_done, (n - 1) & 1));
+                            tcgen05_fence_after();
+                        }
+                        uint32_t y[32];
+                        tmem_wait_st();
+#pragma unroll 1
+                        for (int cc = 0; cc < c; ++cc) {
+                            tmem_ld_32x32b_x32(s_tmem + lanes + 32 * cc, y);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int third = 0; third < 3; ++third) {
+                                const float part = ex2(-fminf(fmaxf(left - 14.0f * third, 0.0f), 14.0f));
+                                const uint32_t f = half2_bits(part, part);
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(y[e]) : "r"(f));
+                            }
+                            tmem_st_32x32b_x32(s_tmem + lanes + 32 * cc, y);
+                        }
+#pragma unroll 1
+                        for (int cc = 0; cc < (anew ? 0 : C::kOutCols / 32); ++cc) {
+                            tmem_ld_32x32b_x32(o_tmem + lanes + 32 * cc, y);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * down);
+                            tmem_st_32x32b_x32(o_tmem + lanes + 32 * cc, y);
+                        }
+                        if (!ok) break;
                     }
+                    if (!ok) break;
+                    l += weight;
                     tmem_st_32x32b_x32(s_tmem + lanes + 32 * c, p);
                 }
+                if (!ok) break;
                 if (anew && j > 0) {
                     // Adds O, complete up to the tile before, to the rounded sum.
                     ok = __all_sync(~0u, tile_wait(watch, o_done, (n - 1) & 1));
