@@ -724,63 +724,75 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
     } else {
         // ------------------------------------------------------ MMA issue
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
-        if (lane == 0) {
-            constexpr uint32_t s_desc = umma_idesc_f16(C::kRows, C::kKeys, false), o_desc = umma_idesc_f16(C::kRows, C::kOutCols, true);
-            const uint32_t qh = smem_u32(q_hi), ql = smem_u32(q_lo), kt = smem_u32(k_tiles), vt = smem_u32(v_tiles);
-            // S of tile n, into the buffer that PV of tile n - 2 reads: MMAs of
-            // unlike accumulators keep no order, so that one is waited for (an
-            // item's first: PV of tile n - 1, which has been issued before).
-            const auto scores = [&](int n, bool first) {
-                const int stage = n % C::kKStages;
-                if (!tile_wait(watch, &k_full[stage], (n / C::kKStages) & 1)) return false;
-                if (n >= (first ? 1 : 2) && !tile_wait(watch, o_done, (first ? n - 1 : n) & 1)) return false;
-                tcgen05_fence_after();
-#pragma unroll 1
+        // The whole warp keeps the loop, so that addresses stay in uniform registers;
+        // one lane issues.
+        const bool leader = elect_one_sync();
+        constexpr uint32_t s_desc = umma_idesc_f16(C::kRows, C::kKeys, false), o_desc = umma_idesc_f16(C::kRows, C::kOutCols, true);
+        const uint64_t qh = umma_desc_k_sw128(smem_u32(q_hi)), ql = umma_desc_k_sw128(smem_u32(q_lo)),
+                       kt = umma_desc_k_sw128(smem_u32(k_tiles)), vt = umma_desc_mn_sw128(smem_u32(v_tiles), C::kKeys * 128);
+        const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, tile_wait(watch, bar, parity)); };
+        const auto commit = [&](uint64_t* bar) {
+            if (leader) umma_commit(bar);
+        };
+        // S of tile n, into the buffer that PV of tile n - 2 reads: MMAs of
+        // unlike accumulators keep no order, so that one is waited for (an
+        // item's first: PV of tile n - 1, which has been issued before).
+        const auto scores = [&](int n, bool first) {
+            const int stage = n % C::kKStages;
+            if (!wait(&k_full[stage], (n / C::kKStages) & 1)) return false;
+            if (n >= (first ? 1 : 2) && !wait(o_done, (first ? n - 1 : n) & 1)) return false;
+            tcgen05_fence_after();
+            const uint64_t k = kt + stage * (C::kKvBytes >> 4);
+            const uint32_t s_tmem = tmem + (n & 1) * C::kKeys;
+            if (leader) {
+#pragma unroll
                 for (int part = 0; part < 2; ++part)
-#pragma unroll 2
+#pragma unroll
                     for (int i = 0; i < D / 16; ++i)
-                        umma_f16(tmem + (n & 1) * C::kKeys,
-                                 umma_desc_k_sw128((part == 0 ? ql : qh) + (i >> 2) * (C::kRows * 128)) + 2 * (i & 3),
-                                 umma_desc_k_sw128(kt + stage * C::kKvBytes + (i >> 2) * (C::kKeys * 128)) + 2 * (i & 3), s_desc,
-                                 part > 0 || i > 0);
-                umma_commit(&k_empty[stage]);
-                umma_commit(&s_full[n & 1]);
-                return true;
-            };
-            int n = 0;
-            bool ok = true;
-            for (int it = 0; ok; ++it) {
-                if (!tile_wait(watch, q_full, it & 1)) break;
-                const int tiles = item->tiles;
-                if (tiles < 0) break;
+                        umma_f16(s_tmem, (part == 0 ? ql : qh) + ((i >> 2) * (C::kRows * 128 >> 4) + 2 * (i & 3)),
+                                 k + ((i >> 2) * (C::kKeys * 128 >> 4) + 2 * (i & 3)), s_desc, part > 0 || i > 0);
+            }
+            __syncwarp();
+            commit(&k_empty[stage]);
+            commit(&s_full[n & 1]);
+            return true;
+        };
+        int n = 0;
+        bool ok = true;
+        for (int it = 0; ok; ++it) {
+            if (!wait(q_full, it & 1)) break;
+            const int tiles = item->tiles;
+            if (tiles < 0) break;
 #pragma unroll 1
-                for (int j = -1; j < tiles && ok; ++j) {
-                    if (j + 1 < tiles) {
-                        ok = scores(n + (j >= 0), j < 0);
-                        if (j + 2 == tiles) umma_commit(q_empty);
-                    }
-                    if (j < 0) continue;
-                    const int stage = n % C::kVStages;
-                    ok = ok && tile_wait(watch, &v_full[stage], (n / C::kVStages) & 1) &&
-                         tile_wait(watch, &p_full[n & 1], (n >> 1) & 1);
-                    if (!ok) break;
-                    tcgen05_fence_after();
-#pragma unroll 1
+            for (int j = -1; j < tiles && ok; ++j) {
+                if (j + 1 < tiles) {
+                    ok = scores(n + (j >= 0), j < 0);
+                    if (j + 2 == tiles) commit(q_empty);
+                }
+                if (j < 0) continue;
+                const int stage = n % C::kVStages;
+                ok = ok && wait(&v_full[stage], (n / C::kVStages) & 1) && wait(&p_full[n & 1], (n >> 1) & 1);
+                if (!ok) break;
+                tcgen05_fence_after();
+                const uint64_t v = vt + stage * (C::kKvBytes >> 4);
+                const uint32_t p_tmem = tmem + (n & 1) * C::kKeys, more = j % C::kSpan > 0;
+                if (leader) {
+#pragma unroll
                     for (int i = 0; i < C::kKeys / 16; ++i)
 #pragma unroll
                         for (int part = 0; part < 2; ++part)
-                            umma_f16_ta(o_tmem, tmem + (n & 1) * C::kKeys + (i >> 1) * 32 + part * 16 + (i & 1) * 8,
-                                        umma_desc_mn_sw128(vt + stage * C::kKvBytes + i * 2048, C::kKeys * 128), o_desc,
-                                        j % C::kSpan > 0 || i > 0 || part > 0);
-                    umma_commit(&v_empty[stage]);
-                    umma_commit(o_done);
-                    ++n;
+                            umma_f16_ta(o_tmem, p_tmem + (i >> 1) * 32 + part * 16 + (i & 1) * 8, v + i * (2048 >> 4), o_desc,
+                                        i > 0 || part > 0 ? 1u : more);
                 }
-                umma_commit(item_done);
+                __syncwarp();
+                commit(&v_empty[stage]);
+                commit(o_done);
+                ++n;
             }
-            umma_commit(drained);  // whatever was issued has completed before the block ends
-            tile_wait(watch, drained, 0);
+            commit(item_done);
         }
+        commit(drained);  // whatever was issued has completed before the block ends
+        wait(drained, 0);
     }
     __syncwarp();
     tcgen05_fence_before();
