@@ -518,22 +518,27 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
         const int to = turned ? at + half : at + ((D - 2 * half) >> 1);
         // Loads run two turns ahead; rotated, scaled by the row's power of two, split,
         // stored swizzled.
+        const int step_t = kPass / g.group, step_h = kPass - step_t * g.group;
         const auto put_rows = [&](const Next& next, uint8_t* power) {
             float4 a, b, cs, sn, a1, b1, cs1, sn1;  // this turn's, the next one's
             a = b = cs = sn = a1 = b1 = cs1 = sn1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const int r0 = next.first_row + cw * kAtOnce + sub;
+            int t = token_of(r0), hq = r0 - t * g.group;  // of the row two turns ahead
 #pragma unroll 1
             for (int i = -2; i < kTurns; ++i) {
-                float v[8];
-                {
-                    float4 x = a, y = b;
-                    if (turned) turn(x, y, cs, sn);
-                    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+                unsigned long long v[4] = {pack2(a.x, a.y), pack2(a.z, a.w), pack2(b.x, b.y), pack2(b.z, b.w)};
+                if (turned) {  // each product and sum rounded, as leafq_rotary_append does
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const unsigned long long x = v[e], y = v[2 + e];
+                        const unsigned long long c2 = e == 0 ? pack2(cs.x, cs.y) : pack2(cs.z, cs.w), s2 = e == 0 ? pack2(sn.x, sn.y) : pack2(sn.z, sn.w);
+                        v[e] = sub2(mul2(x, c2), mul2(y, s2));
+                        v[2 + e] = add2(mul2(y, c2), mul2(x, s2));
+                    }
                 }
                 a = a1, b = b1, cs = cs1, sn = sn1;
-                const int ahead = (i + 2) * kPass + cw * kAtOnce + sub;
                 a1 = b1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (sub < kAtOnce && ahead < next.rows) {
-                    const int t = token_of(next.first_row + ahead), hq = (next.first_row + ahead) - t * g.group;
+                if (sub < kAtOnce && (i + 2) * kPass + cw * kAtOnce + sub < next.rows) {
                     const float* src = g.q + ((int64_t)next.row0 + t) * g.q_stride + (int64_t)(next.head * g.group + hq) * D;
                     a1 = load_now(reinterpret_cast<const float4*>(src + at));
                     b1 = load_now(reinterpret_cast<const float4*>(src + to));
@@ -547,12 +552,21 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                         sn1 = load_now(reinterpret_cast<const float4*>(g.sin_table + pos * half + at));
                     }
                 }
+                t += step_t;
+                hq += step_h;
+                if (hq >= g.group) {
+                    hq -= g.group;
+                    ++t;
+                }
                 if (i < 0) continue;
                 const int r = i * kPass + cw * kAtOnce + sub;
                 // A NaN is no maximum, but it stays one in its row's products.
-                float largest = fabsf(v[0]);
+                float largest = 0.0f;
 #pragma unroll
-                for (int e = 1; e < 8; ++e) largest = fmaxf(largest, fabsf(v[e]));
+                for (int e = 0; e < 4; ++e) {
+                    const float2 x = unpack2(v[e]);
+                    largest = fmaxf(largest, fmaxf(fabsf(x.x), fabsf(x.y)));
+                }
                 if constexpr (kLanes == 12) {
                     float all = 0.0f;
 #pragma unroll
@@ -566,20 +580,25 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 row_power(__float_as_uint(largest), up, down);
                 if (sub < kAtOnce && r < C::kRows) {
                     if (part == 0) power[r] = static_cast<uint8_t>(__float_as_uint(down) >> 23);
+                    const unsigned long long up2 = pack2(up, up);
 #pragma unroll
                     for (int quarter = 0; quarter < 2; ++quarter) {
                         const int d = quarter == 0 ? at : to;
-                        const float x0 = v[4 * quarter] * up, x1 = v[4 * quarter + 1] * up, x2 = v[4 * quarter + 2] * up,
-                                    x3 = v[4 * quarter + 3] * up;
-                        uint2 hi, lo;
-                        hi.x = half2_bits(x0, x1);
-                        hi.y = half2_bits(x2, x3);
-                        const __half2 h01 = *reinterpret_cast<const __half2*>(&hi.x), h23 = *reinterpret_cast<const __half2*>(&hi.y);
-                        lo.x = half2_bits(x0 - __low2float(h01), x1 - __high2float(h01));
-                        lo.y = half2_bits(x2 - __low2float(h23), x3 - __high2float(h23));
+                        uint32_t hi[2], lo[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            // 11 bits (exact in fp16), and what is left.
+                            const unsigned long long x = mul2(v[2 * quarter + e], up2);
+                            const float2 whole = unpack2(x);
+                            const float h0 = __uint_as_float(__float_as_uint(whole.x) & 0xffffe000u);
+                            const float h1 = __uint_as_float(__float_as_uint(whole.y) & 0xffffe000u);
+                            const float2 rest = unpack2(sub2(x, pack2(h0, h1)));
+                            hi[e] = half2_bits(h0, h1);
+                            lo[e] = half2_bits(rest.x, rest.y);
+                        }
                         const int offset = (d >> 6) * (C::kRows * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2;
-                        *reinterpret_cast<uint2*>(q_hi + offset) = hi;
-                        *reinterpret_cast<uint2*>(q_lo + offset) = lo;
+                        *reinterpret_cast<uint2*>(q_hi + offset) = make_uint2(hi[0], hi[1]);
+                        *reinterpret_cast<uint2*>(q_lo + offset) = make_uint2(lo[0], lo[1]);
                     }
                 }
             }
