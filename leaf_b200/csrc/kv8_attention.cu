@@ -554,9 +554,15 @@ int run_split(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl)
                   static_cast<int>(f.row_blocks));
 }
 
-// The tile form pads a request's rows to 128: it is the faster one from about
-// 32 rows of one request on.
-bool takes_tiles(int64_t max_tokens, int group) { return max_tokens * group >= 32; }
+// The tile form gives each 128 rows of a request's kv head to one block: it
+// wants a quarter of them at least, and enough of them that walking a long
+// cache in few blocks is made up for.  Per key and SM clock the split form
+// takes about 0.02 cycles a row over the whole GPU, the tile form 36 (heads of
+// up to 64) or 62 whatever the rows of its 296 blocks: even at 1,800 and 3,100
+// rows in all.
+bool takes_tiles(int64_t tokens, int64_t max_tokens, int heads, int group, int dim) {
+    return max_tokens * group >= 32 && tokens * heads >= (dim <= 64 ? 2048 : 3584);
+}
 
 // Calls f(integral constant D) for a supported head size.
 template <typename F>
@@ -578,7 +584,7 @@ extern "C" {
 
 size_t leafq_kv8_attention_workspace_bytes(int64_t max_tokens, int heads, int kv_heads, int dim) {
     if (max_tokens <= 0 || max_tokens > INT_MAX || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
-        !kv8_dim_supported(dim) || takes_tiles(max_tokens, heads / kv_heads))
+        !kv8_dim_supported(dim))
         return 0;
     return with_dim(dim, [&](auto d) {
         const SplitShape f = split_shape<d()>(max_tokens, heads / kv_heads);
@@ -627,7 +633,7 @@ int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int head
     while ((1 << g.shift) < cache->page) ++g.shift;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool pdl = (flags & LEAFQ_FLAG_PDL) != 0;
-    if (takes_tiles(step->max_tokens, g.group)) return launch_kv8_tiles(s, g, pdl);
+    if (takes_tiles(step->tokens, step->max_tokens, heads, g.group, cache->dim)) return launch_kv8_tiles(s, g, pdl);
     return with_dim(cache->dim, [&](auto d) { return run_split<d()>(s, g, workspace, pdl); });
 }
 

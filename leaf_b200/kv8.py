@@ -24,28 +24,42 @@ PAGE_SIZES = (16, 32, 64, 128)
 HEAD_SIZES = (32, 64, 96, 128)
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+_F32, _I32 = torch.float32, torch.int32
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without an object around it
+
+
+def _fail(message: str) -> None:
+    raise LeafError(_lib.LEAFQ_ERR_INVALID, message)
 
 
 def _need(ok: bool, message: str) -> None:
     if not ok:
-        raise LeafError(_lib.LEAFQ_ERR_INVALID, message)
+        _fail(message)
 
 
+# The calls sit in a decode loop, a few microseconds each: the checks below ask
+# each tensor as little as they can and build their messages only to fail.
 def _check_i32(t: torch.Tensor, name: str, numel: Optional[int] = None, device=None) -> None:
-    _need(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous(), f"{name} must be a contiguous int32 CUDA tensor")
-    _need(numel is None or t.numel() == numel, f"{name} must hold {numel} values")
-    _need(device is None or t.device == device, f"{name} is on another device")
+    if not (t.is_cuda and t.dtype is _I32 and t.is_contiguous()):
+        _fail(f"{name} must be a contiguous int32 CUDA tensor")
+    if numel is not None and t.numel() != numel:
+        _fail(f"{name} must hold {numel} values")
+    if device is not None and t.device != device:
+        _fail(f"{name} is on another device")
 
 
-def _check_rows(t: torch.Tensor, name: str, width: int, device) -> None:
-    """fp32 [tokens, width] rows, contiguous in themselves (columns of a wider matrix are)."""
-    _need(t.is_cuda and t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == width,
-          f"{name} must be float32 [tokens, {width}] on a CUDA device")
-    _need(t.device == device, f"{name} is on another device")
-    _need(t.shape[0] == 0 or (t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= width)),
-          f"the rows of {name} must be contiguous and must not overlap")
+def _check_rows(t: torch.Tensor, name: str, width: int, device) -> int:
+    """fp32 [tokens, width] rows, contiguous in themselves (columns of a wider
+    matrix are).  Returns their stride."""
+    shape = t.shape
+    if not (t.is_cuda and t.dtype is _F32 and len(shape) == 2 and shape[1] == width):
+        _fail(f"{name} must be float32 [tokens, {width}] on a CUDA device")
+    if t.device != device:
+        _fail(f"{name} is on another device")
+    stride, inner = t.stride()
+    if shape[0] != 0 and (inner != 1 or (stride < width and shape[0] != 1)):
+        _fail(f"the rows of {name} must be contiguous and must not overlap")
+    return stride
 
 
 def _rope_args(rope, dim: int, device):
@@ -53,12 +67,13 @@ def _rope_args(rope, dim: int, device):
     if rope is None:
         return 0, None, None, 0
     cos, sin = rope
-    _need(cos.is_cuda and cos.dtype == torch.float32 and cos.dim() == 2 and cos.is_contiguous() and
-          sin.dtype == torch.float32 and sin.shape == cos.shape and sin.is_contiguous() and
-          cos.device == device and sin.device == device,
-          "rope tables must be two contiguous float32 [positions, rotary_dim / 2] CUDA tensors")
-    _need(2 * cos.shape[1] <= dim, "rope tables are wider than the head")
-    return 2 * cos.shape[1], cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+    shape = cos.shape
+    if not (cos.is_cuda and cos.dtype is _F32 and sin.dtype is _F32 and len(shape) == 2 and sin.shape == shape and
+            cos.is_contiguous() and sin.is_contiguous() and cos.device == device and sin.device == device):
+        _fail("rope tables must be two contiguous float32 [positions, rotary_dim / 2] CUDA tensors")
+    if 2 * shape[1] > dim:
+        _fail("rope tables are wider than the head")
+    return 2 * shape[1], cos.data_ptr(), sin.data_ptr(), shape[0]
 
 
 class Kv8Cache:
@@ -77,7 +92,7 @@ class Kv8Cache:
         _need(self.page in PAGE_SIZES, f"pages hold {PAGE_SIZES} tokens")
         _need(self.dim in HEAD_SIZES, f"head sizes are {HEAD_SIZES}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device = k.device
+        self.device, self.index, self.width = k.device, k.device.index, self.kv_heads * self.dim
         self.desc = _lib.Kv8CacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.pages,
                                       self.page, self.kv_heads, self.dim)
         self.ref = ctypes.byref(self.desc)
@@ -112,6 +127,8 @@ class Kv8Plan:
         self.token_offsets, self.page_offsets = token_offsets, page_offsets
         self.positions, self.slots, self.taken = positions, slots, taken
         self.requests, self.tokens, self.max_tokens, self.device = requests, int(tokens), int(max_tokens), device
+        self.index = device.index
+        self.inputs = self.outputs = None  # addresses, of a plan that kv8_plan made
         self.desc = _lib.Kv8StepDesc(context.data_ptr(), lengths.data_ptr(), token_offsets.data_ptr(),
                                      page_offsets.data_ptr(), table.data_ptr(), table.shape[1], self.tokens,
                                      self.max_tokens, requests)
@@ -125,11 +142,20 @@ class Kv8Workspace:
     def __init__(self, device="cuda"):
         self.device = torch.device(device)
         self.buffer = torch.empty(0, dtype=torch.uint8, device=self.device)
+        self.sizes: dict = {}
 
     def get(self, nbytes: int) -> torch.Tensor:
         if nbytes > self.buffer.numel():
             self.buffer = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
         return self.buffer
+
+    def of(self, max_tokens: int, heads: int, kv_heads: int, dim: int):
+        """(address, bytes) for a geometry."""
+        key = (max_tokens, heads, kv_heads, dim)
+        need = self.sizes.get(key)
+        if need is None:
+            need = self.sizes[key] = load().leafq_kv8_attention_workspace_bytes(*key)
+        return self.get(need).data_ptr(), need
 
 
 def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
@@ -145,7 +171,7 @@ def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tenso
     plan's ``taken``.  ``out``: a plan of the same sizes whose buffers are
     reused."""
     requests = context.numel()
-    if out is not None and out.context is context and out.table is table and out.tokens == tokens and out.slots is not None:
+    if out is not None and out.context is context and out.table is table and out.tokens == tokens and out.inputs is not None:
         plan = out
     else:
         device = context.device
@@ -158,14 +184,15 @@ def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tenso
         lengths, token_offsets, page_offsets, after, positions, slots = (p[:n] for p, n in zip(pieces, sizes))
         plan = Kv8Plan(context, lengths, token_offsets, page_offsets, table, tokens,
                        tokens if max_tokens is None else max_tokens, positions, slots, after)
-    _check_i32(new_tokens, "new_tokens", requests, plan.device)
-    _check_i32(free_pages, "free_pages", None, plan.device)
-    _check_i32(taken, "taken", 1, plan.device)
-    check(load().leafq_kv8_plan(_stream(plan.device), context.data_ptr(), new_tokens.data_ptr(), requests,
-                                table.data_ptr(), table.shape[1], free_pages.data_ptr(), free_pages.numel(),
-                                taken.data_ptr(), page, tokens, plan.lengths.data_ptr(), plan.token_offsets.data_ptr(),
-                                plan.page_offsets.data_ptr(), plan.positions.data_ptr(), plan.slots.data_ptr(),
-                                plan.taken.data_ptr(), flags))
+        plan.inputs = (context.data_ptr(), table.data_ptr(), table.shape[1])
+        plan.outputs = tuple(p.data_ptr() for p in (lengths, token_offsets, page_offsets, positions, slots, after))
+    device = plan.device
+    _check_i32(new_tokens, "new_tokens", requests, device)
+    _check_i32(free_pages, "free_pages", None, device)
+    _check_i32(taken, "taken", 1, device)
+    check(load().leafq_kv8_plan(_raw_stream(plan.index), plan.inputs[0], new_tokens.data_ptr(), requests, plan.inputs[1],
+                                plan.inputs[2], free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(), page, tokens,
+                                *plan.outputs, flags))
     return plan
 
 
@@ -176,19 +203,22 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: Kv8Cache, slots: torch.T
     With rope = (cos, sin) tables [positions, rotary_dim / 2] the keys are
     rotated by ``positions`` first.  A page's scale grows when a new row needs
     it, and its older codes are rounded to the new scale."""
-    width = cache.kv_heads * cache.dim
-    _check_rows(k, "k", width, cache.device)
-    _check_rows(v, "v", width, cache.device)
+    device = cache.device
+    k_stride = _check_rows(k, "k", cache.width, device)
+    v_stride = _check_rows(v, "v", cache.width, device)
     tokens = k.shape[0]
-    _need(v.shape[0] == tokens, "k and v must have the same rows")
-    _check_i32(slots, "slots", tokens, cache.device)
-    rotary, cos, sin, rows = _rope_args(rope, cache.dim, cache.device)
+    if v.shape[0] != tokens:
+        _fail("k and v must have the same rows")
+    _check_i32(slots, "slots", tokens, device)
+    rotary, cos, sin, rows = _rope_args(rope, cache.dim, device)
+    where = None
     if rope is not None:
-        _need(positions is not None, "rotation needs positions")
-        _check_i32(positions, "positions", tokens, cache.device)
-    check(load().leafq_kv8_append(_stream(cache.device), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), tokens,
-                                  None if positions is None else positions.data_ptr(), slots.data_ptr(), rotary, cos,
-                                  sin, rows, cache.ref, flags))
+        if positions is None:
+            _fail("rotation needs positions")
+        _check_i32(positions, "positions", tokens, device)
+        where = positions.data_ptr()
+    check(load().leafq_kv8_append(_raw_stream(cache.index), k.data_ptr(), k_stride, v.data_ptr(), v_stride, tokens, where,
+                                  slots.data_ptr(), rotary, cos, sin, rows, cache.ref, flags))
 
 
 def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float, rope=None,
@@ -199,22 +229,22 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float,
     rotated by position when rope tables are given.  Returns fp32
     [tokens, heads * dim]; a row that sees no key is zero, rows past the step's
     last new token are not written."""
-    _need(q.dim() == 2 and q.shape[1] % cache.dim == 0, "q must be [tokens, heads * dim]")
-    _check_rows(q, "q", q.shape[1], cache.device)
-    tokens, heads = q.shape[0], q.shape[1] // cache.dim
-    _need(tokens == plan.tokens, "q has other rows than the plan")
-    _need(plan.device == cache.device, "the plan is on another device")
+    device, dim, shape = cache.device, cache.dim, q.shape
+    if len(shape) != 2 or shape[1] % dim != 0:
+        _fail("q must be [tokens, heads * dim]")
+    tokens, width = shape
+    stride = _check_rows(q, "q", width, device)
+    if tokens != plan.tokens:
+        _fail("q has other rows than the plan")
+    if plan.device != device:
+        _fail("the plan is on another device")
     if out is None:
-        out = torch.empty((tokens, q.shape[1]), dtype=torch.float32, device=cache.device)
-    else:
-        _need(out.is_cuda and out.dtype == torch.float32 and out.is_contiguous() and out.shape == q.shape and
-              out.device == cache.device, "out must be contiguous float32 of q's shape")
-    rotary, cos, sin, rows = _rope_args(rope, cache.dim, cache.device)
-    lib = load()
-    need = lib.leafq_kv8_attention_workspace_bytes(plan.max_tokens, heads, cache.kv_heads, cache.dim)
-    pointer = None
-    if need:
-        pointer = (workspace or Kv8Workspace(cache.device)).get(need).data_ptr()
-    check(lib.leafq_kv8_attention(_stream(cache.device), q.data_ptr(), q.stride(0), heads, rotary, cos, sin, rows,
-                                  cache.ref, plan.ref, scale, out.data_ptr(), pointer, need, flags))
+        out = torch.empty((tokens, width), dtype=_F32, device=device)
+    elif not (out.is_cuda and out.dtype is _F32 and out.is_contiguous() and out.shape == shape and out.device == device):
+        _fail("out must be contiguous float32 of q's shape")
+    rotary, cos, sin, rows = _rope_args(rope, dim, device)
+    heads = width // dim
+    address, need = (Kv8Workspace(device) if workspace is None else workspace).of(plan.max_tokens, heads, cache.kv_heads, dim)
+    check(load().leafq_kv8_attention(_raw_stream(cache.index), q.data_ptr(), stride, heads, rotary, cos, sin, rows, cache.ref,
+                                     plan.ref, scale, out.data_ptr(), address, need, flags))
     return out

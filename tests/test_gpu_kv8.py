@@ -335,6 +335,52 @@ def test_attention_prompts(cuda_device, dim, group, page):
     _Batch(rng, [0, 0, 100, 37, 513], [130, 1, 65, 200, 33], page, 2, group, dim, rotary=dim).check()
 
 
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("kv,group,page", [(32, 1, 64), (12, 3, 16), (8, 8, 64), (4, 16, 128), (13, 5, 32)])
+def test_attention_prompts_of_many_heads(cuda_device, dim, kv, group, page):
+    # Enough query rows for the kernel that tiles them by 128, whatever the requests' lengths.
+    rng = np.random.default_rng(dim + kv + page)
+    _Batch(rng, [0, 300, 95, 0, 17], [97, 1, 33, 0, 64], page, kv, group, dim, rotary=dim // 2).check()
+
+
+@pytest.mark.parametrize("new", [40, 47, 48, 49, 95, 96, 97, 193])
+def test_attention_tile_edges(cuda_device, new):
+    rng = np.random.default_rng(new)
+    _Batch(rng, [0, 96 - new % 96], [new, new], 16, 16, 4, 64, rotary=64).check()
+    _Batch(rng, [64, 500], [new, 1], 128, 16, 6, 128).check()
+
+
+@pytest.mark.parametrize("spread", [0.0, 1e-6, 12.0, 40.0])
+def test_attention_tile_score_ranges(cuda_device, spread):
+    # Later keys outweigh earlier ones by orders of magnitude, tile after tile: the running reference has to follow.
+    rng = np.random.default_rng(33)
+    b = _Batch(rng, [400, 0], [50, 50], 16, 8, 8, 64, spread=spread)
+    rise = np.linspace(-3, 0, b.pool)[np.argsort(np.argsort(rng.random(b.pool)))]
+    b.scales[0] *= 10.0 ** rise[:, None].astype(np.float32)
+    b.scales[1] *= 10.0 ** (2 * rise[::-1, None]).astype(np.float32)
+    b.cache.k_scale.copy_(torch.from_numpy(b.scales[0]))
+    b.cache.v_scale.copy_(torch.from_numpy(b.scales[1]))
+    b.check()
+
+
+def test_attention_tiles_where_nothing_is_seen(cuda_device):
+    rng = np.random.default_rng(34)
+    b = _Batch(rng, [0, 20, 64, 0], [60] * 4, 16, 8, 8, 64, lengths=[0, 20, 124, 0], spare=20, pad=2)
+    b.q[-2:] = np.nan
+    out = b.run(out=torch.full(b.q.shape, 7.0, device="cuda"))
+    assert torch.all(out[:60] == 0) and torch.all(out[180:240] == 0) and torch.all(out[-2:] == 7.0)
+    b.check(out)
+    b.plan.table[1, 1] = b.pool  # out of range: hidden and reported
+    b.plan.table[2, 0] = -5
+    out = b.run()
+    assert torch.isfinite(out).all()
+    assert _lib.load().leafq_device_status() == _lib.LEAFQ_ERR_INVALID
+    b.cache.k_scale[int(b.table[2, 3]), 0] = float("nan")
+    out = b.run().reshape(-1, 8, 8 * 64)
+    assert torch.isnan(out[120 + 48:180, 0]).all() and torch.isfinite(out[:-2, 1:]).all()
+    assert _lib.load().leafq_device_status() == _lib.LEAFQ_ERR_INVALID
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("new", [16, 127, 128, 129, 255, 257, 600])
 def test_attention_prompt_lengths(cuda_device, dim, new):
