@@ -57,19 +57,21 @@ __device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t& tot
         part[warp][1] = b;
     }
     __syncthreads();
-    int64_t before_a = 0, before_b = 0;
-    total_a = total_b = 0;
-    for (int w = 0; w < warps; ++w) {
-        const int64_t pa = part[w][0], pb = part[w][1];
-        if (w < warp) {
-            before_a += pa;
-            before_b += pb;
+    // Every warp scans the warps' totals for itself.
+    int64_t pa = lane < warps ? part[lane][0] : 0, pb = lane < warps ? part[lane][1] : 0;
+    const int64_t own_a = pa, own_b = pb;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int64_t oa = __shfl_up_sync(~0u, pa, d), ob = __shfl_up_sync(~0u, pb, d);
+        if (lane >= d) {
+            pa += oa;
+            pb += ob;
         }
-        total_a += pa;
-        total_b += pb;
     }
-    a += before_a;
-    b += before_b;
+    total_a = __shfl_sync(~0u, pa, 31);
+    total_b = __shfl_sync(~0u, pb, 31);
+    a += __shfl_sync(~0u, pa - own_a, warp);
+    b += __shfl_sync(~0u, pb - own_b, warp);
 }
 
 __global__ void __launch_bounds__(kPlanMaxThreads) kv8_plan_kernel(const PlanArgs g) {
@@ -86,10 +88,13 @@ __global__ void __launch_bounds__(kPlanMaxThreads) kv8_plan_kernel(const PlanArg
     const bool writer = blockIdx.x == 0;
     if (tid == 0) reached_s = 0;
     int64_t token_base = 0, need_base = 0, page_base = 0;
+    int32_t next_c = tid < g.requests ? g.context[tid] : 0, next_n = tid < g.requests ? g.fresh[tid] : 0;
     for (int base = 0; base < g.requests; base += threads) {
         const int r = base + tid;
         const bool live = r < g.requests;
-        int64_t c = live ? g.context[r] : 0, n = live ? g.fresh[r] : 0;
+        int64_t c = next_c, n = next_n;
+        next_c = r + threads < g.requests ? g.context[r + threads] : 0;
+        next_n = r + threads < g.requests ? g.fresh[r + threads] : 0;
         if (c < 0 || n < 0) {
             if (writer) record_device_error(kSiteKv8Range);
             c = max64(c, 0);
@@ -208,7 +213,7 @@ struct AppendArgs {
     const float* cos_table;
     const float* sin_table;
     int64_t table_rows, tokens, pages;
-    int shift, kv_heads, dim, rotary, span;
+    int shift, kv_heads, rotary, span;
 };
 
 __device__ __forceinline__ uint32_t pack_codes(float4 x, float multiplier) {
@@ -230,7 +235,9 @@ __device__ __forceinline__ uint32_t largest_bits(uint32_t m, float4 x) {
     return max(m, __float_as_uint(x.w) & 0x7fffffffu);
 }
 
-__global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs g) {
+template <int D>
+__global__ void __launch_bounds__(512, 2) kv8_append_kernel(const AppendArgs g) {
+    __shared__ int32_t slots_s[256], positions_s[256];  // of the span's rows and a page's worth behind them
     __shared__ uint32_t starts_s[4];   // rows of the span that start a run
     __shared__ uint32_t follow_s[16];  // rows behind a start that belong to its run
     __shared__ uint32_t largest_s[16];
@@ -241,12 +248,19 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs g) {
     const int page = 1 << g.shift;
     const int64_t row0 = (int64_t)blockIdx.x * g.span;
     const int64_t pool = g.pages << g.shift;
+    const int32_t before_row0 = row0 > 0 ? g.slots[row0 - 1] : -2;
+    for (int i = tid; i < g.span + page; i += blockDim.x) {
+        const bool there = row0 + i < g.tokens;
+        slots_s[i] = there ? g.slots[row0 + i] : -1;
+        positions_s[i] = there && g.rotary > 0 && which == 0 ? g.positions[row0 + i] : 0;
+    }
+    __syncthreads();
     // span <= page <= blockDim.x: one row per thread.
     bool start = false;
     if (tid < g.span && row0 + tid < g.tokens) {
-        const int64_t slot = g.slots[row0 + tid];
+        const int32_t slot = slots_s[tid];
         if (slot >= 0 && slot < pool) {
-            start = (slot & (page - 1)) == 0 || row0 + tid == 0 || g.slots[row0 + tid - 1] != slot - 1;
+            start = (slot & (page - 1)) == 0 || (tid == 0 ? before_row0 : slots_s[tid - 1]) != slot - 1;
         } else if (slot != -1 && head == 0 && which == 0) {
             record_device_error(kSiteKv8Range);
         }
@@ -254,16 +268,16 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs g) {
     const uint32_t ballot = __ballot_sync(~0u, start);
     if (lane == 0 && warp < 4) starts_s[warp] = ballot;
     __syncthreads();
-    const int per_row = g.dim >> 3;
+    constexpr int per_row = D / 8;  // items
     const bool rotate = which == 0 && g.rotary > 0;
     const int half = rotate ? g.rotary >> 1 : 0;
     for (int word = 0; word < 4 && word * 32 < g.span; ++word) {
         for (uint32_t left = starts_s[word]; left != 0; left &= left - 1) {
-            const int64_t row = row0 + word * 32 + __ffs(left) - 1;
-            const int64_t slot = g.slots[row];
+            const int at_row = word * 32 + __ffs(left) - 1;
+            const int64_t row = row0 + at_row, slot = slots_s[at_row];
             const int first = static_cast<int>(slot & (page - 1));
             // Rows of the run: until the page ends or the slots stop following.
-            const bool follows = tid < page - first && row + tid < g.tokens && g.slots[row + tid] == slot + tid;
+            const bool follows = tid < page - first && slots_s[at_row + tid] == slot + tid;
             const uint32_t mask = __ballot_sync(~0u, follows);
             if (lane == 0) follow_s[warp] = mask;
             __syncthreads();
@@ -286,14 +300,14 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs g) {
                 const int item = tid + i * blockDim.x, r = item / per_row, j = item - r * per_row;
                 a[i] = b[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (r >= n) continue;
-                const float* src = g.rows[which] + (row + r) * g.stride[which] + (int64_t)head * g.dim;
+                const float* src = g.rows[which] + (row + r) * g.stride[which] + (int64_t)head * D;
                 const bool turned = 4 * j < half;
                 const int at = turned ? 4 * j : 2 * half + 4 * (j - half / 4);
-                const int to = turned ? at + half : at + ((g.dim - 2 * half) >> 1);
+                const int to = turned ? at + half : at + ((D - 2 * half) >> 1);
                 a[i] = *reinterpret_cast<const float4*>(src + at);
                 b[i] = *reinterpret_cast<const float4*>(src + to);
                 if (turned) {
-                    int64_t pos = g.positions[row + r];
+                    int64_t pos = positions_s[at_row + r];
                     if (pos < 0 || pos >= g.table_rows) {
                         if (j == 0 && head == 0) record_device_error(kSiteKv8Range);
                         pos = 0;
@@ -319,11 +333,11 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs g) {
             float need = __fdiv_rn(__uint_as_float(largest), 127.0f);
             if (need < 1e-12f) need = 1e-12f;  // keeps a NaN
             const float scale = first > 0 && !(need > before) && !isnan(need) ? before : need;
-            int8_t* codes = g.codes[which] + ((tile << g.shift) * g.dim);
+            int8_t* codes = g.codes[which] + ((tile << g.shift) * D);
             if (first > 0 && scale != before) {
                 // The page's older codes, rounded to the grown scale.
                 const float ratio = __fdiv_rn(before, scale);
-                for (int i = tid; i < first * g.dim / 4; i += blockDim.x) {
+                for (int i = tid; i < first * D / 4; i += blockDim.x) {
                     uint32_t* at = reinterpret_cast<uint32_t*>(codes) + i;
                     const uint32_t old = *at;
                     *at = pack_codes(make_float4(static_cast<int8_t>(old), static_cast<int8_t>(old >> 8),
@@ -338,8 +352,8 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const AppendArgs g) {
                 if (r >= n) continue;
                 const bool turned = 4 * j < half;
                 const int at = turned ? 4 * j : 2 * half + 4 * (j - half / 4);
-                const int to = turned ? at + half : at + ((g.dim - 2 * half) >> 1);
-                int8_t* dst = codes + (int64_t)(first + r) * g.dim;
+                const int to = turned ? at + half : at + ((D - 2 * half) >> 1);
+                int8_t* dst = codes + (int64_t)(first + r) * D;
                 *reinterpret_cast<uint32_t*>(dst + at) = pack_codes(a[i], multiplier);
                 *reinterpret_cast<uint32_t*>(dst + to) = pack_codes(b[i], multiplier);
             }
@@ -447,7 +461,7 @@ int leafq_kv8_append(void* stream, const float* k, int64_t k_stride, const float
     }
     AppendArgs g{{k, v}, {k_stride, v_stride}, {cache->k_codes, cache->v_codes}, {cache->k_scales, cache->v_scales},
                  positions, slots, cos_table, sin_table, table_rows, tokens, cache->pages, page_shift(cache->page),
-                 cache->kv_heads, cache->dim, rotary_dim, 1};
+                 cache->kv_heads, rotary_dim, 1};
     // 32 .. 512 threads in whole warps, at least the page.
     const int threads = (cache->page * cache->dim / 8 / kAppendItems + 31) / 32 * 32;
     // Few rows: one per block, so that a decode step's rows run side by side;
@@ -455,9 +469,10 @@ int leafq_kv8_append(void* stream, const float* k, int64_t k_stride, const float
     int span = 1;
     while (span < cache->page && tokens / (2 * span) * cache->kv_heads * 2 >= 4 * (int64_t)sm_count()) span *= 2;
     g.span = span;
-    return launch(kv8_append_kernel, dim3(static_cast<unsigned>((tokens + span - 1) / span), cache->kv_heads, 2),
-                  dim3(threads), 0, static_cast<cudaStream_t>(stream),
-                  (flags & LEAFQ_FLAG_PDL) != 0, "leafq_kv8_append", g);
+    const auto kernel = cache->dim == 32 ? kv8_append_kernel<32> : cache->dim == 64 ? kv8_append_kernel<64>
+                        : cache->dim == 96 ? kv8_append_kernel<96> : kv8_append_kernel<128>;
+    return launch(kernel, dim3(static_cast<unsigned>((tokens + span - 1) / span), cache->kv_heads, 2), dim3(threads), 0,
+                  static_cast<cudaStream_t>(stream), (flags & LEAFQ_FLAG_PDL) != 0, "leafq_kv8_append", g);
 }
 
 }  // extern "C"
