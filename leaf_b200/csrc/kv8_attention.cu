@@ -121,6 +121,13 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
     const int64_t segments = (int64_t)requests * kv_heads;
     bool whole = false;
     if (segments <= ranges) {
+        // What the block will read first, should it come to that.
+        const int likely = range < segments ? range / kv_heads : 0;
+        if (tid < 32 && tid * 8 < g.step.max_pages)
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(g.step.table + (int64_t)likely * g.step.max_pages + tid * 8));
+        if (tid == 32) asm volatile("prefetch.global.L1 [%0];" ::"l"(g.step.context + likely));
+        if (tid == 64) asm volatile("prefetch.global.L1 [%0];" ::"l"(g.step.lengths + likely));
+        if (tid == 96) asm volatile("prefetch.global.L1 [%0];" ::"l"(g.step.token_offsets + likely));
         int longest = 0;
         for (int s = lane; s < requests; s += 32) longest = max(longest, g.step.page_offsets[s + 1] - g.step.page_offsets[s]);
         longest = __reduce_max_sync(~0u, longest);
@@ -300,7 +307,7 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
             }
 
             // Scores of keys key + 8 n + {tq, 4 + tq} (n-tile n), in x + e.
-            float x[4][2], top = -INFINITY;
+            float x[4][2];
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -332,32 +339,50 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
                     for (int e = 0; e < 2; ++e)
                         if (key + 8 * n + tq + 4 * e >= limit) x[n][e] = -INFINITY;
             }
-#pragma unroll
-            for (int n = 0; n < 4; ++n) top = fmaxf(top, fmaxf(x[n][0], x[n][1]));
-            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-            // O and L so far count relative to the maximum so far.
-            const float grown = fmaxf(m, top);
-            const float old = m == -INFINITY ? 0.0f : ex2(m - grown);
-            m = grown;
-            l *= old;
-            const float shift = m == -INFINITY ? 0.0f : m - kLift;
+            // The weights count relative to m, a whole power of two that is the same for
+            // the row's four lanes.  It comes from the row's first keys; later ones are
+            // weighed with it as it stands, and only where weights come out above
+            // kHighest is it raised, with O and L scaled down (exactly) to the new one.
             uint32_t p[2][4];
+            float sum;
+#pragma unroll 1
+            for (;;) {
+                const float shift = m == -INFINITY ? INFINITY : m - kLift;
+                sum = 0.0f;
+                float most = 0.0f;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                float hi[2], lo[2];
+                for (int n = 0; n < 4; ++n) {
+                    float hi[2], lo[2];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float u = ex2(x[n][e] - shift), w = u * frac[n >> 1];
-                    l = fmaf(u, back[n >> 1], l);
-                    hi[e] = __uint_as_float(__float_as_uint(w) & 0xffffe000u);  // 11 bits: exact in fp16
-                    lo[e] = w - hi[e];
+                    for (int e = 0; e < 2; ++e) {
+                        const float u = ex2(x[n][e] - shift), w = u * frac[n >> 1];
+                        most = fmaxf(most, u);
+                        sum = fmaf(u, back[n >> 1], sum);
+                        hi[e] = __uint_as_float(__float_as_uint(w) & 0xffffe000u);  // 11 bits: exact in fp16
+                        lo[e] = w - hi[e];
+                    }
+                    p[n >> 1][2 * (n & 1)] = half2_bits(hi[0], hi[1]);
+                    p[n >> 1][2 * (n & 1) + 1] = half2_bits(lo[0], lo[1]);
                 }
-                p[n >> 1][2 * (n & 1)] = half2_bits(hi[0], hi[1]);
-                p[n >> 1][2 * (n & 1) + 1] = half2_bits(lo[0], lo[1]);
+                if (!__any_sync(~0u, most > kHighest || (m == -INFINITY && key < limit))) break;
+                float top = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) top = fmaxf(top, fmaxf(x[n][0], x[n][1]));
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+                // A row that sees none of them takes any reference: its weights are zero.
+                const float raised = m == -INFINITY && !(top > -INFINITY) ? 0.0f : fmaxf(m, ceilf(top));
+                const float down = m == -INFINITY ? 0.0f : ex2(m - raised);
+                m = raised;
+                l *= down;
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][e] *= down;
             }
+            l += sum;
             // A chunk's products sum up in the MMA, whose additions truncate; the
-            // chunks are added (and rescaled) in rounded fp32.
+            // chunks are added in rounded fp32.
             constexpr int kWords = D / 32;
 #pragma unroll
             for (int c = 0; c < kWords; ++c) {
@@ -387,7 +412,7 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[4 * c + n][e] = fmaf(o[4 * c + n][e], old, part[n][e]);
+                    for (int e = 0; e < 4; ++e) o[4 * c + n][e] += part[n][e];
             }
             __syncwarp();  // the stage is read before it is copied into again
         }

@@ -27,10 +27,10 @@ struct Kv8AttendArgs {
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
-// Weights are held as 2^kLift times their value relative to the largest, so
-// that the second half of a weight's fp16 split stays a normal number down to
-// 2^-28 of the largest; 2^14 times 127 codes is far from fp32's range.
-constexpr float kLift = 14.0f;
+// Weights are held as 2^kLift times their value relative to a row's reference,
+// so that the second half of a weight's fp16 split stays a normal number far
+// below it; twice kHighest is below 65504, fp16's largest.
+constexpr float kLift = 6.0f, kHighest = 24576.0f;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

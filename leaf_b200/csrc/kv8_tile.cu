@@ -30,12 +30,12 @@ namespace {
 // Each 32 columns of S are replaced in place by 16 columns of P's hi pairs and
 // 16 of its lo pairs.  Weights are 2^kTileLift times their value relative to a
 // power of two that follows the row's maximum from below: 16 of them may sum up
-// to kHighest, so that none passes 65504, fp16's largest, before the reference
+// to kTileHighest, so that none passes 65504, fp16's largest, before the reference
 // is raised and O rescaled.  The MMA's additions truncate,
 // which adds up over long sums (8192 keys: 5.5e-6 of the result), so every
 // kSpan keys O is added to a rounded sum (in local memory) and starts anew
 // -- and the lo halves of Q go first, while S is small.
-constexpr float kTileLift = 6.0f, kHighest = 49152.0f;
+constexpr float kTileLift = 6.0f, kTileHighest = 49152.0f;
 
 // What the roles of a block need to know of an item: 128 query rows of one kv
 // head of a request.  tiles < 0: there are no more.
@@ -297,7 +297,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 };
                 // The weights count relative to a whole power of two m.  It is taken from
                 // the first tile with a key for the row; later tiles are weighed with it as it stands, and
-                // only where weights come out above kHighest is it raised, with what has
+                // only where weights come out above kTileHighest is it raised, with what has
                 // been weighed so far scaled down, exactly but for what is lost below
                 // 2^-30 of the largest.
                 const bool anew = j % C::kSpan == 0;
@@ -340,7 +340,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                                 p[16 + e / 2] = half2_bits(low.x, low.y);
                             }
                             const float2 both = unpack2(sum);
-                            high |= both.x + both.y > kHighest;
+                            high |= both.x + both.y > kTileHighest;
                             weight = fmaf(both.x + both.y, scale.z, weight);
                         }
                         if (!__any_sync(~0u, high)) break;
