@@ -112,35 +112,59 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
     const int page = 1 << g.shift;
     const int requests = g.step.requests, kv_heads = g.cache.kv_heads;
     const int64_t units = (int64_t)kv_heads * g.step.page_offsets[requests];
-    // Work: units (page, head, request) in a row, an even share per block --
-    // a request's head may then be split over blocks, which costs a partial
-    // result each -- or one block for each request's head where that is no
-    // longer than an even share and the joining (about 12 chunks' time).
+    // Work.  With no more requests' heads than blocks, each head's pages are cut
+    // into equal pieces of at most `piece` pages and every block takes one: the
+    // smallest piece, from a warp's chunk each on, that makes no more pieces than
+    // blocks.  Otherwise the units (page, head, request) in a row are dealt out in
+    // even shares, each block walking the heads in its own.  A head over several
+    // blocks costs a partial result each, which the last of them joins.
+    const int64_t segments = (int64_t)requests * kv_heads;
+    const bool pieces = segments <= ranges;
     int64_t shares = min64(ranges, (units << g.shift) / (C::kWarps * C::kChunk));
     if (shares < 1) shares = 1;
-    const int64_t segments = (int64_t)requests * kv_heads;
-    bool whole = false;
-    if (segments <= ranges) {
-        // What the block will read first, should it come to that.
-        const int likely = range < segments ? range / kv_heads : 0;
-        if (tid < 32 && tid * 8 < g.step.max_pages)
-            asm volatile("prefetch.global.L1 [%0];" ::"l"(g.step.table + (int64_t)likely * g.step.max_pages + tid * 8));
-        if (tid == 32) asm volatile("prefetch.global.L1 [%0];" ::"l"(g.step.context + likely));
-        if (tid == 64) asm volatile("prefetch.global.L1 [%0];" ::"l"(g.step.lengths + likely));
-        if (tid == 96) asm volatile("prefetch.global.L1 [%0];" ::"l"(g.step.token_offsets + likely));
-        int longest = 0;
-        for (int s = lane; s < requests; s += 32) longest = max(longest, g.step.page_offsets[s + 1] - g.step.page_offsets[s]);
-        longest = __reduce_max_sync(~0u, longest);
-        whole = (int64_t)longest << g.shift <= (units << g.shift) / shares + 12 * C::kChunk;
-    }
     int64_t begin = 0, end = 0;
-    int s = 0;
-    if (whole) {
-        if (range < segments) {
-            s = range / kv_heads;
-            const int64_t first = g.step.page_offsets[s], held = g.step.page_offsets[s + 1] - first;
-            begin = first * kv_heads + (range - (int64_t)s * kv_heads) * held;
-            end = begin + held;
+    int s = 0, first_block = 0, last_block = 0;  // pieces: the blocks of this block's head
+    if (pieces) {
+        const auto pieces_of = [](int held, int piece) {
+            return static_cast<int>(static_cast<uint32_t>(held + piece - 1) / static_cast<uint32_t>(piece));
+        };
+        const auto held_by = [&](int r) { return r < requests ? g.step.page_offsets[r + 1] - g.step.page_offsets[r] : 0; };
+        int longest = 0;
+        for (int r = lane; r < requests; r += 32) longest = max(longest, held_by(r));
+        longest = max(__reduce_max_sync(~0u, longest), 1);
+        int piece = max(1, static_cast<int>(__fdividef(static_cast<float>(units), static_cast<float>(shares))));
+        for (;;) {
+            piece = min(piece, longest);
+            int count = 0;
+            for (int r = lane; r < requests; r += 32) count += pieces_of(held_by(r), piece);
+            count = __reduce_add_sync(~0u, count) * kv_heads;
+            if (count <= ranges || piece == longest) break;
+            piece = max(piece + 1, static_cast<int>(__fdividef(static_cast<float>(piece) * count, static_cast<float>(ranges))));
+        }
+        // The request that piece `range` belongs to, by a scan of the requests' pieces.
+        int before = 0;
+        for (int base = 0; base < requests; base += 32) {
+            const int own = pieces_of(held_by(base + lane), piece) * kv_heads;
+            int upto = own;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int other = __shfl_up_sync(~0u, upto, d);
+                if (lane >= d) upto += other;
+            }
+            const uint32_t beyond = __ballot_sync(~0u, before + upto > range);
+            if (beyond != 0) {
+                const int hit = __ffs(beyond) - 1;
+                s = base + hit;
+                const int index = range - before - __shfl_sync(~0u, upto - own, hit);  // of the request's pieces
+                const int held = held_by(s), each = pieces_of(held, piece), h = index / each, i = index - h * each;
+                const int even = held / each, rest = held - even * each;  // the first `rest` pieces have one page more
+                begin = (int64_t)kv_heads * g.step.page_offsets[s] + (int64_t)h * held + (i * even + min(i, rest));
+                end = begin + even + (i < rest);
+                first_block = range - i;
+                last_block = first_block + each - 1;
+                break;
+            }
+            before += __shfl_sync(~0u, upto, 31);
         }
     } else if (range < shares) {
         begin = units * range / shares;
@@ -462,7 +486,8 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
         }
         if (split) {
             // The last block to arrive joins the segment's parts, in block order.
-            const int64_t i0 = ((start + 1) * shares - 1) / units, i1 = ((start + held) * shares - 1) / units;
+            const int64_t i0 = pieces ? first_block : ((start + 1) * shares - 1) / units,
+                          i1 = pieces ? last_block : ((start + held) * shares - 1) / units;
             __threadfence();
             __syncthreads();
             if (tid == 0) {
