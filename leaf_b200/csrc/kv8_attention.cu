@@ -133,7 +133,17 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
         for (int r = lane; r < requests; r += 32) longest = max(longest, held_by(r));
         longest = max(__reduce_max_sync(~0u, longest), 1);
         int piece = max(1, static_cast<int>(__fdividef(static_cast<float>(units), static_cast<float>(shares))));
-        for (;;) {
+        // Heads that are not much longer than that (by about the time of a join) stay whole.
+        if (longest <= piece + ((12 * C::kChunk) >> g.shift)) {
+            if (range < segments) {
+                s = range / kv_heads;
+                const int held = held_by(s);
+                begin = (int64_t)kv_heads * g.step.page_offsets[s] + (int64_t)(range - s * kv_heads) * held;
+                end = begin + held;
+            }
+            piece = 0;
+        }
+        while (piece > 0) {
             piece = min(piece, longest);
             int count = 0;
             for (int r = lane; r < requests; r += 32) count += pieces_of(held_by(r), piece);
@@ -143,7 +153,7 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
         }
         // The request that piece `range` belongs to, by a scan of the requests' pieces.
         int before = 0;
-        for (int base = 0; base < requests; base += 32) {
+        for (int base = 0; piece > 0 && base < requests; base += 32) {
             const int own = pieces_of(held_by(base + lane), piece) * kv_heads;
             int upto = own;
 #pragma unroll
