@@ -1,5 +1,5 @@
-// Shared by the two forms of the paged INT8 cache's attention (kv8_attention.cu
-// for few query rows, kv8_tile.cu for many).
+// Shared by the paged INT8 cache's append (kv8_cache.cu) and the two forms of its
+// attention (kv8_attention.cu for few query rows, kv8_tile.cu for many).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -64,7 +64,7 @@ __device__ __forceinline__ uint32_t codes_half2(uint32_t biased, uint32_t select
 }
 
 // Rotates the pairs of a and b, in the rounding steps of leafq_rotary_append.
-__device__ __forceinline__ void turn(float4& a, float4& b, float4 c, float4 s) {
+__device__ __forceinline__ void kv8_turn(float4& a, float4& b, float4 c, float4 s) {
     const float4 x = a, y = b;
     a = make_float4(__fsub_rn(__fmul_rn(x.x, c.x), __fmul_rn(y.x, s.x)), __fsub_rn(__fmul_rn(x.y, c.y), __fmul_rn(y.y, s.y)),
                     __fsub_rn(__fmul_rn(x.z, c.z), __fmul_rn(y.z, s.z)), __fsub_rn(__fmul_rn(x.w, c.w), __fmul_rn(y.w, s.w)));
@@ -84,8 +84,8 @@ __device__ __forceinline__ void query_item(const Kv8AttendArgs& g, const float* 
     a = *reinterpret_cast<const float4*>(row + at);
     b = *reinterpret_cast<const float4*>(row + to);
     if (turned)
-        turn(a, b, *reinterpret_cast<const float4*>(g.cos_table + pos * half + at),
-             *reinterpret_cast<const float4*>(g.sin_table + pos * half + at));
+        kv8_turn(a, b, *reinterpret_cast<const float4*>(g.cos_table + pos * half + at),
+                 *reinterpret_cast<const float4*>(g.sin_table + pos * half + at));
 }
 
 // The power of two that brings a row's largest magnitude into [256, 512), as

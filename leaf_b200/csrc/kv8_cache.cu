@@ -5,8 +5,7 @@
 //                      their pages, the pages' scales grown where they must
 #include <climits>
 
-#include "leafq_device.cuh"
-#include "leafq_internal.h"
+#include "kv8_attention.cuh"
 
 namespace leafq {
 namespace {
@@ -218,19 +217,21 @@ struct AppendArgs {
 
 // Four codes: the products, rounded, plus 1.5 * 2^23, which rounds them to whole
 // numbers (half to even) in the low bits, two's complement.  |x| is at most the
-// absmax that the multiplier comes from, so no product passes 127.5.
-__device__ __forceinline__ uint32_t pack_codes(unsigned long long x01, unsigned long long x23, float multiplier) {
-    const unsigned long long m = pack2(multiplier, multiplier), whole = pack2(12582912.0f, 12582912.0f);
-    const float2 a = unpack2(add2(mul2(x01, m), whole)), b = unpack2(add2(mul2(x23, m), whole));
-    return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040),
-                       __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
+// absmax that the multiplier comes from, so no product passes 127.5.  (Scalar
+// operations: the paired mul.rn and add.rn came out as one fused rounding.)
+__device__ __forceinline__ uint32_t pack_codes(float4 x, float multiplier) {
+    const float a = __fadd_rn(__fmul_rn(x.x, multiplier), 12582912.0f), b = __fadd_rn(__fmul_rn(x.y, multiplier), 12582912.0f);
+    const float c = __fadd_rn(__fmul_rn(x.z, multiplier), 12582912.0f), d = __fadd_rn(__fmul_rn(x.w, multiplier), 12582912.0f);
+    return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
+                       __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
 }
 
 // max |x| that keeps a NaN.
-__device__ __forceinline__ float largest_of(float m, unsigned long long x) {
-    const float2 v = unpack2(x);
+__device__ __forceinline__ float largest_of(float m, float4 v) {
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v.x)));
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v.y)));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v.z)));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v.w)));
     return m;
 }
 
@@ -292,38 +293,29 @@ __global__ void __launch_bounds__(512, 2) kv8_append_kernel(const AppendArgs g) 
             const int64_t tile = (slot >> g.shift) * g.kv_heads + head;
             float* scale_at = g.scales[which] + tile;
             const float before = *scale_at;
-            unsigned long long x[kAppendItems][4];  // a's four values, b's four
+            float4 a[kAppendItems], b[kAppendItems];
             float most = 0.0f;
 #pragma unroll
             for (int i = 0; i < kAppendItems; ++i) {
                 const int item = tid + i * blockDim.x, r = item / per_row, j = item - r * per_row;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[i][e] = 0;
+                a[i] = b[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (r >= n) continue;
                 const float* src = g.rows[which] + (row + r) * g.stride[which] + (int64_t)head * D;
                 const bool turned = 4 * j < half;
                 const int at = turned ? 4 * j : 2 * half + 4 * (j - half / 4);
                 const int to = turned ? at + half : at + ((D - 2 * half) >> 1);
-                const float4 a = *reinterpret_cast<const float4*>(src + at), b = *reinterpret_cast<const float4*>(src + to);
-                x[i][0] = pack2(a.x, a.y), x[i][1] = pack2(a.z, a.w), x[i][2] = pack2(b.x, b.y), x[i][3] = pack2(b.z, b.w);
-                if (turned) {  // each product and sum rounded, as leafq_rotary_append does
+                a[i] = *reinterpret_cast<const float4*>(src + at);
+                b[i] = *reinterpret_cast<const float4*>(src + to);
+                if (turned) {
                     int64_t pos = positions_s[at_row + r];
                     if (pos < 0 || pos >= g.table_rows) {
                         if (j == 0 && head == 0) record_device_error(kSiteKv8Range);
                         pos = 0;
                     }
-                    const float4 c = *reinterpret_cast<const float4*>(g.cos_table + pos * half + at);
-                    const float4 s = *reinterpret_cast<const float4*>(g.sin_table + pos * half + at);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const unsigned long long u = x[i][e], v = x[i][2 + e];
-                        const unsigned long long c2 = e == 0 ? pack2(c.x, c.y) : pack2(c.z, c.w), s2 = e == 0 ? pack2(s.x, s.y) : pack2(s.z, s.w);
-                        x[i][e] = sub2(mul2(u, c2), mul2(v, s2));
-                        x[i][2 + e] = add2(mul2(v, c2), mul2(u, s2));
-                    }
+                    kv8_turn(a[i], b[i], *reinterpret_cast<const float4*>(g.cos_table + pos * half + at),
+                             *reinterpret_cast<const float4*>(g.sin_table + pos * half + at));
                 }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) most = largest_of(most, x[i][e]);
+                most = largest_of(largest_of(most, a[i]), b[i]);
             }
             uint32_t largest = __reduce_max_sync(~0u, __float_as_uint(most));
             if (lane == 0) largest_s[warp] = largest;
@@ -339,8 +331,8 @@ __global__ void __launch_bounds__(512, 2) kv8_append_kernel(const AppendArgs g) 
                 for (int i = tid; i < first * D / 4; i += blockDim.x) {
                     uint32_t* at = reinterpret_cast<uint32_t*>(codes) + i;
                     const uint32_t old = *at;
-                    *at = pack_codes(pack2(static_cast<int8_t>(old), static_cast<int8_t>(old >> 8)),
-                                     pack2(static_cast<int8_t>(old >> 16), static_cast<int8_t>(old >> 24)), ratio);
+                    *at = pack_codes(make_float4(static_cast<int8_t>(old), static_cast<int8_t>(old >> 8),
+                                                 static_cast<int8_t>(old >> 16), static_cast<int8_t>(old >> 24)), ratio);
                 }
             }
             const float multiplier = __fdiv_rn(1.0f, scale);
@@ -352,8 +344,8 @@ __global__ void __launch_bounds__(512, 2) kv8_append_kernel(const AppendArgs g) 
                 const int at = turned ? 4 * j : 2 * half + 4 * (j - half / 4);
                 const int to = turned ? at + half : at + ((D - 2 * half) >> 1);
                 int8_t* dst = codes + (int64_t)(first + r) * D;
-                *reinterpret_cast<uint32_t*>(dst + at) = pack_codes(x[i][0], x[i][1], multiplier);
-                *reinterpret_cast<uint32_t*>(dst + to) = pack_codes(x[i][2], x[i][3], multiplier);
+                *reinterpret_cast<uint32_t*>(dst + at) = pack_codes(a[i], multiplier);
+                *reinterpret_cast<uint32_t*>(dst + to) = pack_codes(b[i], multiplier);
             }
             if (tid == 0) *scale_at = scale;
             __syncthreads();  // follow_s and largest_s are free

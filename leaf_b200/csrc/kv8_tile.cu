@@ -527,7 +527,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
 #pragma unroll 1
             for (int i = -2; i < kTurns; ++i) {
                 unsigned long long v[4] = {pack2(a.x, a.y), pack2(a.z, a.w), pack2(b.x, b.y), pack2(b.z, b.w)};
-                if (turned) {  // each product and sum rounded, as leafq_rotary_append does
+                if (turned) {  // (a product and a sum may be rounded as one)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const unsigned long long x = v[e], y = v[2 + e];

@@ -18,7 +18,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import LeafError, check, load
+from ._lib import LEAFQ_FLAG_PDL, LeafError, check, load
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_SIZES = (32, 64, 96, 128)
@@ -160,7 +160,7 @@ class Kv8Workspace:
 
 def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
              taken: torch.Tensor, page: int, tokens: int, max_tokens: Optional[int] = None,
-             out: Optional[Kv8Plan] = None, flags: int = 0) -> Kv8Plan:
+             out: Optional[Kv8Plan] = None, flags: int = LEAFQ_FLAG_PDL) -> Kv8Plan:
     """Pages and slots of a step.  Request s holds context[s] tokens and brings
     new_tokens[s]; the pages they need are taken from free_pages[taken:] in
     request order and written into its row of ``table`` (in place).  A request
@@ -197,7 +197,7 @@ def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tenso
 
 
 def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: Kv8Cache, slots: torch.Tensor,
-               positions: Optional[torch.Tensor] = None, rope=None, flags: int = 0) -> None:
+               positions: Optional[torch.Tensor] = None, rope=None, flags: int = LEAFQ_FLAG_PDL) -> None:
     """Writes the rows of k and v (fp32 [tokens, kv_heads * dim]; columns of a
     wider matrix will do) into the cache at their slots, -1 skipping a row.
     With rope = (cos, sin) tables [positions, rotary_dim / 2] the keys are
@@ -223,7 +223,7 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: Kv8Cache, slots: torch.T
 
 def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float, rope=None,
                   out: Optional[torch.Tensor] = None, workspace: Optional[Kv8Workspace] = None,
-                  flags: int = 0) -> torch.Tensor:
+                  flags: int = LEAFQ_FLAG_PDL) -> torch.Tensor:
     """Causal grouped-query attention of the step's rows q (fp32
     [tokens, heads * dim]; columns of a wider matrix will do) over the cache,
     rotated by position when rope tables are given.  Returns fp32

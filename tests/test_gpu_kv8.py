@@ -240,6 +240,27 @@ def test_append_zero_and_not_a_number(cuda_device):
     assert np.isnan(s[1]) and np.isinf(s[2])  # the page shows what went in
 
 
+def test_append_rounds_each_step_to_float(cuda_device):
+    # code = rint(x * (1 / scale)) with every step rounded to float: bit for bit, products that round to a half included.
+    rng = np.random.default_rng(12)
+    tokens, kv, dim, page = 4096, 4, 64, 64
+    x = rng.standard_normal((2, tokens, kv * dim)).astype(np.float32)
+    cos, sin = _rope(tokens, dim)
+    cache = lq.Kv8Cache.empty(tokens // page, kv, page, dim)
+    k, v = (torch.from_numpy(a).cuda() for a in x)
+    lq.kv8_append(k, v, cache, _i32(np.arange(tokens)), _i32(np.arange(tokens)), rope=_rope_cuda((cos, sin)))
+    turned = x[0].reshape(tokens, kv, dim).copy()
+    a, b = turned[..., :dim // 2].copy(), turned[..., dim // 2:].copy()
+    turned[..., :dim // 2] = a * cos[:, None] - b * sin[:, None]
+    turned[..., dim // 2:] = b * cos[:, None] + a * sin[:, None]
+    for rows, codes, scales in ((turned, cache.k, cache.k_scale), (x[1].reshape(tokens, kv, dim), cache.v, cache.v_scale)):
+        rows = rows.reshape(-1, page, kv, dim).transpose(0, 2, 1, 3)  # [pages, kv, page, dim]
+        scale = np.maximum(np.abs(rows).max(axis=(2, 3)) / np.float32(127), np.float32(1e-12))
+        expect = np.rint(rows * (np.float32(1) / scale)[:, :, None, None])
+        assert np.array_equal(scales.cpu().numpy(), scale)
+        assert np.array_equal(codes.cpu().numpy(), expect)
+
+
 def test_append_twice_is_append_once(cuda_device):
     rng = np.random.default_rng(3)
     cache = _check_append(rng, _runs(rng, 16, 6, [30, 9], [5, 11]), 16, 2, 64, 6, 0)
