@@ -35,6 +35,7 @@ import torch
 from . import _lib
 from ._lib import LEAFQ_FLAG_PDL, LeafError, check, load
 from .artifact import Artifact, HostTensor
+from .kv8 import HEAD_SIZES, PAGE_SIZES, Kv8Cache, Kv8Workspace, kv8_append, kv8_attention, kv8_plan
 from .linear import QuantWeight, Workspace
 
 
@@ -85,7 +86,7 @@ def _concat_rows(parts: list[HostTensor], device: torch.device, interleave: bool
 class Decoder:
     def __init__(self, artifact, activation_bits: int = 8, device="cuda",
                  capacity: Optional[int] = None, sequences: int = 1, group=None,
-                 gather: str = "nccl"):
+                 gather: str = "nccl", cache: str = "fp32", page: int = 64):
         """artifact: a path, an ``Artifact``, or any object with the same
         ``config`` / ``get(name)`` interface whose payloads are tensors
         (``leaf_b200.stack.RandomDecoderModel``).
@@ -106,7 +107,14 @@ class Decoder:
         make the same calls.  gather="peer" gathers the decode steps' outputs
         with the library's own peer-memory all-gather over NVLink
         (``leafq_allgather_*``), which lets the step be one CUDA graph; the
-        prompt's gathers stay NCCL."""
+        prompt's gathers stay NCCL.
+
+        cache="int8" holds keys and values as INT8 codes in pages of `page`
+        tokens (``leaf_b200.kv8``): a quarter of the fp32 cache's bytes, and
+        ``forward_batch`` / ``generate_batch`` take prompts of unlike lengths.
+        Its results carry the rounding of 8 bits, so they are not the
+        reference's bit for bit, and the one-launch step needs the fp32
+        cache."""
         art = artifact if hasattr(artifact, "get") else Artifact(artifact)
         cfg = art.config
         if not (cfg.norm_kind == 0 and cfg.position_kind == 0 and cfg.gated == 1 and
@@ -119,6 +127,13 @@ class Decoder:
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "activation bits must be 8 or 32")
         if sequences < 1:
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "sequences must be positive")
+        if cache not in ("fp32", "int8"):
+            raise LeafError(_lib.LEAFQ_ERR_INVALID, "cache must be 'fp32' or 'int8'")
+        if cache == "int8" and page not in PAGE_SIZES:
+            raise LeafError(_lib.LEAFQ_ERR_INVALID, f"cache pages hold {PAGE_SIZES} tokens")
+        if cache == "int8" and (cfg.head_dim not in HEAD_SIZES or cfg.rotary_dim % 8 != 0):
+            raise LeafError(_lib.LEAFQ_ERR_UNSUPPORTED,
+                            f"the INT8 cache needs heads of {HEAD_SIZES} and a rotary part of whole eights")
         self.cfg = cfg
         self.sequences = int(sequences)
         self.group = group
@@ -185,9 +200,21 @@ class Decoder:
         self.has_bias |= self.lm_head.bias is not None
         d, kv = cfg.head_dim, cfg.kv_heads
         S = self.sequences
-        self.k_cache = [torch.zeros((S, kv, self.capacity, d), dtype=torch.float32, device=dev)
-                        for _ in range(cfg.layers)]
-        self.v_cache = [torch.zeros_like(k) for k in self.k_cache]
+        self.kv8 = None
+        self.k_cache = self.v_cache = []
+        if cache == "int8":
+            # One table for all layers: page i of a request is page table[s][i] of every
+            # layer's pool, which holds every request at full capacity.
+            row = -(-self.capacity // page)
+            self.page = page
+            self.kv8 = [Kv8Cache.empty(S * row, kv, page, d, dev) for _ in range(cfg.layers)]
+            self.table = torch.full((S, row), -1, dtype=torch.int32, device=dev)
+            self.free_pages = torch.arange(S * row, dtype=torch.int32, device=dev)
+            self.taken = torch.zeros(1, dtype=torch.int32, device=dev)
+        else:
+            self.k_cache = [torch.zeros((S, kv, self.capacity, d), dtype=torch.float32, device=dev)
+                            for _ in range(cfg.layers)]
+            self.v_cache = [torch.zeros_like(k) for k in self.k_cache]
         half = cfg.rotary_dim // 2
         cos = np.empty((self.capacity, half), dtype=np.float32)
         sin = np.empty_like(cos)
@@ -238,9 +265,19 @@ class Decoder:
                     need = self._workspace_bytes(w, r)
                     if need:
                         b["workspace"].get(need)
-            need = self.lib.leafq_attention_workspace_bytes(S, tokens, c.heads, c.kv_heads, c.head_dim,
-                                                            self.capacity)
-            b["attention_ws"] = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+            if self.kv8 is None:
+                need = self.lib.leafq_attention_workspace_bytes(S, tokens, c.heads, c.kv_heads, c.head_dim,
+                                                                self.capacity)
+                b["attention_ws"] = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+            else:
+                kd = c.kv_heads * c.head_dim
+                b["columns"] = b["qkv"].split([q, kd, kd], dim=1)
+                b["new"] = torch.full((S,), tokens, dtype=torch.int32, device=dev)
+                b["attn"].zero_()  # rows past a step's last token are never written
+                # A workspace of its own, sized once: a captured graph keeps its address.
+                need = self.lib.leafq_kv8_attention_workspace_bytes(tokens, c.heads, c.kv_heads, c.head_dim)
+                b["kv8_ws"] = Kv8Workspace(dev)
+                b["kv8_ws"].get(need)
             self._buffers[tokens] = b
         return b
 
@@ -371,7 +408,14 @@ class Decoder:
                 self._linear(b["normalized"], w, out, rows, b["workspace"])
 
         norm(None, 0, self.layers[0]["input_norm"], fuse)
-        ws = b["attention_ws"]
+        if self.kv8 is not None:
+            # The step's pages and slots, once for all layers.
+            b["plan"] = plan = kv8_plan(self.position, b["new"], self.table, self.free_pages, self.taken, self.page,
+                                        rows, tokens, out=b.get("plan"))
+            q_cols, k_cols, v_cols = b["columns"]
+            rope = (self.cos, self.sin)
+        else:
+            ws = b["attention_ws"]
         for i, layer in enumerate(self.layers):
             if self.smooth:
                 # Each projection on its own input scale, then q | k | v
@@ -381,16 +425,21 @@ class Decoder:
                 torch.cat((b["q"], b["k"], b["v"]), dim=1, out=b["qkv"])
             else:
                 normed_linear(layer["qkv"], b["qkv"])
-            check(lib.leafq_rotary_append_batch(s, b["qkv"].data_ptr(), S, tokens, c.heads, c.kv_heads,
-                                                c.head_dim, c.rotary_dim, self.cos.data_ptr(),
-                                                self.sin.data_ptr(), self.position.data_ptr(),
-                                                b["q_heads"].data_ptr(), self.k_cache[i].data_ptr(),
-                                                self.v_cache[i].data_ptr(), self.capacity))
-            check(lib.leafq_attention_batch(s, b["q_heads"].data_ptr(), self.k_cache[i].data_ptr(),
-                                            self.v_cache[i].data_ptr(), S, tokens, c.heads, c.kv_heads,
-                                            c.head_dim, self.position.data_ptr(), self.capacity,
-                                            self.capacity, ctypes.c_float(self.scale), b["attn"].data_ptr(),
-                                            ws.data_ptr(), ws.numel()))
+            if self.kv8 is not None:
+                kv8_append(k_cols, v_cols, self.kv8[i], plan.slots, plan.positions, rope=rope)
+                kv8_attention(q_cols, self.kv8[i], plan, c.head_dim ** -0.5, rope=rope, out=b["attn"],
+                              workspace=b["kv8_ws"])
+            else:
+                check(lib.leafq_rotary_append_batch(s, b["qkv"].data_ptr(), S, tokens, c.heads, c.kv_heads,
+                                                    c.head_dim, c.rotary_dim, self.cos.data_ptr(),
+                                                    self.sin.data_ptr(), self.position.data_ptr(),
+                                                    b["q_heads"].data_ptr(), self.k_cache[i].data_ptr(),
+                                                    self.v_cache[i].data_ptr(), self.capacity))
+                check(lib.leafq_attention_batch(s, b["q_heads"].data_ptr(), self.k_cache[i].data_ptr(),
+                                                self.v_cache[i].data_ptr(), S, tokens, c.heads, c.kv_heads,
+                                                c.head_dim, self.position.data_ptr(), self.capacity,
+                                                self.capacity, ctypes.c_float(self.scale), b["attn"].data_ptr(),
+                                                ws.data_ptr(), ws.numel()))
             self._linear(b["attn"], layer["o"], b["o"], rows, b["workspace"])
             norm(b["o"], 0, layer["post_norm"], fuse)
             if self.smooth:
@@ -424,19 +473,29 @@ class Decoder:
             norm(b["down"], 1, self.final_norm if last else self.layers[i + 1]["input_norm"], fuse and not last)
         if tokens == 1:
             last_rows = b["normalized"]
+        elif self.kv8 is not None:  # requests may bring fewer tokens than `tokens`: their rows follow one another
+            last = (plan.token_offsets[1:] - 1).clamp(min=0)
+            torch.index_select(b["normalized"], 0, last, out=b["last"])
+            last_rows = b["last"]
         elif S == 1:
             last_rows = b["normalized"][tokens - 1:tokens]
         else:  # each sequence's last row, gathered into consecutive rows
             b["last"].copy_(b["normalized"].view(S, tokens, c.hidden)[:, tokens - 1])
             last_rows = b["last"]
         self._linear(last_rows, self.lm_head, b["logits"], S, b["workspace"])
-        check(lib.leafq_advance_positions(s, self.position.data_ptr(), S, tokens))
+        if self.kv8 is not None:
+            self.position.copy_(plan.lengths)
+            self.taken.copy_(plan.taken)
+        else:
+            check(lib.leafq_advance_positions(s, self.position.data_ptr(), S, tokens))
 
     # ----------------------------------------------------------- public API
     def reset(self) -> None:
         """Decoder::reset: empty every KV cache."""
         self.length = 0
         self.position.zero_()
+        if self.kv8 is not None:
+            self.taken.zero_()
 
     def forward(self, ids) -> torch.Tensor:
         """Decoder::forward_into(ids, logits) with all_logits = false: the
@@ -482,6 +541,8 @@ class Decoder:
             widest = max(self._full_rows.values())
             self._peer = PeerAllGather(self.sequences * widest, group=self.group)
         b = self._bufs(1)
+        if self.kv8 is not None:
+            b["new"].zero_()  # the warm-up brings no tokens: it must leave the pages alone
         stream = torch.cuda.Stream(self.device)
         stream.wait_stream(torch.cuda.current_stream(self.device))
         saved = self.position.clone()
@@ -492,6 +553,8 @@ class Decoder:
         torch.cuda.current_stream(self.device).wait_stream(stream)
         torch.cuda.synchronize(self.device)
         self.position.copy_(saved)
+        if self.kv8 is not None:
+            b["new"].fill_(1)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             self._forward_device(b, 1)
@@ -526,23 +589,27 @@ class Decoder:
 
     def forward_batch(self, prompts) -> torch.Tensor:
         """forward() for every sequence of the batch at once: prompts is one
-        list of ids per sequence, all of the same length; returns each
-        sequence's last-position logits [sequences, vocab] (a device tensor
-        reused by later calls)."""
+        list of ids per sequence, all of the same length (of any lengths with
+        the INT8 cache); returns each sequence's last-position logits
+        [sequences, vocab] (a device tensor reused by later calls)."""
         prompts = [[int(i) for i in p] for p in prompts]
         if len(prompts) != self.sequences:
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "one prompt per sequence")
-        tokens = len(prompts[0])
-        if tokens == 0 or any(len(p) != tokens for p in prompts):
+        tokens = max(len(p) for p in prompts)
+        if any(len(p) == 0 for p in prompts) or (self.kv8 is None and any(len(p) != tokens for p in prompts)):
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "batched prompts must be non-empty and of equal length")
         if self.length + tokens > min(self.cfg.max_positions, self.capacity):
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "context length exceeds artifact limit")
         if any(i < 0 or i >= self.cfg.vocab for p in prompts for i in p):
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "token id exceeds vocabulary")
         b = self._bufs(tokens)
-        b["ids"].copy_(torch.tensor(prompts, dtype=torch.int32).reshape(-1))
+        ids = [i for p in prompts for i in p]
+        b["ids"][:len(ids)].copy_(torch.tensor(ids, dtype=torch.int32))
+        if self.kv8 is not None:
+            b["ids"][len(ids):].zero_()
+            b["new"].copy_(torch.tensor([len(p) for p in prompts], dtype=torch.int32))
         self._forward_device(b, tokens)
-        self.length += tokens
+        self.length += tokens  # the longest sequence at most
         return b["logits"]
 
     def generate_batch(self, prompts, max_new: int) -> list[list[int]]:
@@ -554,7 +621,7 @@ class Decoder:
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "max_new must be positive")
         if not self._step_ready:
             self.capture_decode()
-        tokens = len(prompts[0]) if prompts else 0
+        tokens = max((len(p) for p in prompts), default=0)
         if self.length + tokens + max_new - 1 > min(self.cfg.max_positions, self.capacity):
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "context length exceeds artifact limit")
         logits = self.forward_batch(prompts)
@@ -583,7 +650,7 @@ class Decoder:
         embedding, W8A8, and a cache of at most 4096 rows."""
         per_row = all(w.bits == 8 and w.group == w.cols for w in self._weights())
         return (per_row and not self.smooth and not self.has_bias and "qkv" in self.layers[0] and
-                self.sequences == 1 and self.world == 1 and self.activation_bits == 8 and
+                self.sequences == 1 and self.world == 1 and self.activation_bits == 8 and self.kv8 is None and
                 self.embed_bits == 8 and
                 self.embed_group == self.cfg.hidden and self.capacity <= 4096 and
                 self.final_norm is not None)
@@ -593,7 +660,7 @@ class Decoder:
         launch per generated token)."""
         if not self.fused_supported():
             raise LeafError(_lib.LEAFQ_ERR_UNSUPPORTED,
-                            "one-launch decode needs per-row INT8 weights, W8A8 and capacity <= 4096")
+                            "one-launch decode needs per-row INT8 weights, W8A8, an fp32 cache and capacity <= 4096")
         c, ptr = self.cfg, (lambda t: t.data_ptr())
         layers = (_lib.ModelLayer * c.layers)()
         for i, L in enumerate(self.layers):
