@@ -67,10 +67,15 @@ struct Split {
     static constexpr int kPart = 8 * (D + 2);            // floats of one partial result: m [8], l [8], O [8][D]
     static constexpr size_t kSmem = (size_t)kWarps * kRing + 8 * D * sizeof(float);
     static_assert(kRing >= kPart * 4, "a warp's partial result goes through its ring");
-    static_assert(kWarps * kRing >= (kBlocks + 1) * 8 * 4 + (kThreads * 4 + 8 * D) * 4, "joining goes through the rings");
+    static_assert(kWarps * kRing >= 4 * (kBlocks + 1) * 4, "the step's arrays go through the rings");
+    static_assert(kWarps * kRing >= (kBlocks + 1) * 16 * 4 + (kThreads * 4 + 8 * D) * 4, "joining goes through the rings");
 };
 
-// Where 16-byte piece c of row r of a chunk lies within the row.
+// Layout of a chunk.  K's rows lie in the order of the score tiles' columns:
+// row c of eight is key (c >> 1) + 4 (c & 1).  Both functions give where 16-byte
+// piece c of row r lies within the row: with them each fragment read (16, 8 or 4
+// bytes a lane) touches every bank once.
+__device__ __forceinline__ int k_key(int r) { return (r & ~7) + ((r & 7) >> 1) + 4 * (r & 1); }
 template <int D>
 __device__ __forceinline__ int k_piece(int r, int c) {
     return D == 128 ? c ^ ((r & 1) << 2) : c;
@@ -94,16 +99,88 @@ __device__ __forceinline__ int find_request(const int32_t* page_offsets, int req
     return lo;
 }
 
+// The last block of a head to arrive joins its n parts, in their order: part i at
+// parts + i stride, the first one `first` floats further.
+template <int D>
+__device__ __forceinline__ void join_parts(uint8_t* smem, const float* parts, int64_t stride, int64_t first, int n, int rows,
+                                        int group, int first_row, float* out, int64_t out_stride) {
+    using C = Split<D>;
+    // The parts' m and l and each thread's first part are asked for at once: four
+    // elements and every sets-th part per thread, then the threads' sums.
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const auto other = [&](int i) { return parts + i * stride + (i == 0 ? first : 0); };
+    float* weight_s = reinterpret_cast<float*>(smem);  // [n][16]: m and l, then weights; the rows' sums [8]
+    const int items = rows * (D / 4), sets = max(1, C::kThreads / items), set = tid / items;
+    float4 ahead;
+    if (set < sets && set < n) ahead = __ldcg(reinterpret_cast<const float4*>(other(set) + 16) + tid % items);
+    for (int i = tid; i < 16 * n; i += C::kThreads) weight_s[i] = __ldcg(other(i >> 4) + (i & 15));
+    __syncthreads();
+    for (int r = warp; r < rows; r += C::kWarps) {
+        float top = -INFINITY, total = 0.0f;
+        for (int i = lane; i < n; i += 32) top = fmaxf(top, weight_s[i * 16 + r]);
+        top = warp_max_f32(top);
+        for (int i = lane; i < n; i += 32) {
+            const float their = weight_s[i * 16 + r], part_l = weight_s[i * 16 + 8 + r];
+            const float weight = their == -INFINITY ? (part_l == 0.0f ? 0.0f : 1.0f) : ex2(their - top);
+            weight_s[i * 16 + r] = weight;
+            total = fmaf(weight, part_l, total);
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
+        if (lane == 0) weight_s[n * 16 + r] = total;
+    }
+    __syncthreads();
+    float4* set_s = reinterpret_cast<float4*>(weight_s + (n * 16 + 8));
+    for (int item = tid % items; item < items && set < sets; item += C::kThreads) {
+        const int r = item / (D / 4);
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const auto add = [&](int i, float4 v) {
+            const float weight = weight_s[i * 16 + r];
+            sum.x = fmaf(weight, v.x, sum.x);
+            sum.y = fmaf(weight, v.y, sum.y);
+            sum.z = fmaf(weight, v.z, sum.z);
+            sum.w = fmaf(weight, v.w, sum.w);
+        };
+        int i = set;
+        if (item == tid % items && i < n) {
+            add(i, ahead);
+            i += sets;
+        }
+#pragma unroll 4
+        for (; i < n; i += sets) add(i, __ldcg(reinterpret_cast<const float4*>(other(i) + 16) + item));
+        set_s[set * items + item] = sum;
+    }
+    __syncthreads();
+    for (int item = tid; item < rows * (D / 4); item += C::kThreads) {
+        const int r = item / (D / 4), d = 4 * (item - r * (D / 4));
+        float4 sum = set_s[item];
+        for (int other_set = 1; other_set < sets; ++other_set) {
+            const float4 v = set_s[other_set * items + item];
+            sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+        }
+        const float total = weight_s[n * 16 + r];
+        const float4 y = total == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                       : make_float4(sum.x / total, sum.y / total, sum.z / total, sum.w / total);
+        const int t = (first_row + r) / group, hq = (first_row + r) - t * group;
+        *reinterpret_cast<float4*>(out + t * out_stride + hq * D + d) = y;
+    }
+}
+
 template <int D>
 __global__ void __launch_bounds__(Split<D>::kThreads, Split<D>::kBlocksPerSm)
 kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals, int ranges, int row_blocks) {
     using C = Split<D>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int last_s;
+    __shared__ struct {  // what the end of a segment needs: kept out of the key loop's registers
+        int64_t row0;
+        int h, rows, own, parts, first_part;
+    } segment_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gq = lane >> 2, tq = lane & 3;
     uint8_t* ring = smem + warp * C::kRing;
-    float* q_s = reinterpret_cast<float*>(smem + C::kWarps * C::kRing);
+    uint4* q_s = reinterpret_cast<uint4*>(smem + C::kWarps * C::kRing);  // the query rows' fragments [D / 16][32]
+    __shared__ float factor_s[8];
     grid_dependency_wait();
     grid_launch_dependents();
 
@@ -120,15 +197,22 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
     // blocks costs a partial result each, which the last of them joins.
     const int64_t segments = (int64_t)requests * kv_heads;
     const bool pieces = segments <= ranges;
-    int64_t shares = min64(ranges, (units << g.shift) / (C::kWarps * C::kChunk));
-    if (shares < 1) shares = 1;
+    const int shares = pieces ? static_cast<int>(max64(1, min64(ranges, (units << g.shift) / (C::kWarps * C::kChunk)))) : ranges;
     int64_t begin = 0, end = 0;
-    int s = 0, first_block = 0, last_block = 0;  // pieces: the blocks of this block's head
+    int s = 0, h = 0, p0 = 0, p1 = 0;             // the segment: pages [p0, p1) of head h of request s
+    int first_block = 0, last_block = 0;          // pieces: the blocks of this block's head
+    const int32_t* page_offsets = g.step.page_offsets;
     if (pieces) {
-        const auto pieces_of = [](int held, int piece) {
-            return static_cast<int>(static_cast<uint32_t>(held + piece - 1) / static_cast<uint32_t>(piece));
+        // The pages of each request (at most one per block), in the rings.
+        int32_t* held_pages = reinterpret_cast<int32_t*>(smem);
+        for (int r = tid; r < requests; r += C::kThreads)
+            held_pages[r] = min(max(page_offsets[r + 1] - page_offsets[r], 0), static_cast<int>(g.step.max_pages));
+        __syncthreads();
+        // About held / piece rounded up, the same in every block; none of no pages, no more than pages.
+        const auto pieces_of = [](int held, float inverse) {
+            return min(held, max(1, __float2int_ru(static_cast<float>(held) * inverse)));
         };
-        const auto held_by = [&](int r) { return r < requests ? g.step.page_offsets[r + 1] - g.step.page_offsets[r] : 0; };
+        const auto held_by = [&](int r) { return r < requests ? held_pages[r] : 0; };
         int longest = 0;
         for (int r = lane; r < requests; r += 32) longest = max(longest, held_by(r));
         longest = max(__reduce_max_sync(~0u, longest), 1);
@@ -137,16 +221,17 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
         if (longest <= piece + ((12 * C::kChunk) >> g.shift)) {
             if (range < segments) {
                 s = range / kv_heads;
-                const int held = held_by(s);
-                begin = (int64_t)kv_heads * g.step.page_offsets[s] + (int64_t)(range - s * kv_heads) * held;
-                end = begin + held;
+                h = range - s * kv_heads;
+                p1 = held_by(s);
             }
             piece = 0;
         }
+        float inverse = 0.0f;
         while (piece > 0) {
             piece = min(piece, longest);
             int count = 0;
-            for (int r = lane; r < requests; r += 32) count += pieces_of(held_by(r), piece);
+            inverse = __fdividef(1.0f, static_cast<float>(piece));
+            for (int r = lane; r < requests; r += 32) count += pieces_of(held_by(r), inverse);
             count = __reduce_add_sync(~0u, count) * kv_heads;
             if (count <= ranges || piece == longest) break;
             piece = max(piece + 1, static_cast<int>(__fdividef(static_cast<float>(piece) * count, static_cast<float>(ranges))));
@@ -154,7 +239,7 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
         // The request that piece `range` belongs to, by a scan of the requests' pieces.
         int before = 0;
         for (int base = 0; piece > 0 && base < requests; base += 32) {
-            const int own = pieces_of(held_by(base + lane), piece) * kv_heads;
+            const int own = pieces_of(held_by(base + lane), inverse) * kv_heads;
             int upto = own;
 #pragma unroll
             for (int d = 1; d < 32; d *= 2) {
@@ -166,96 +251,105 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
                 const int hit = __ffs(beyond) - 1;
                 s = base + hit;
                 const int index = range - before - __shfl_sync(~0u, upto - own, hit);  // of the request's pieces
-                const int held = held_by(s), each = pieces_of(held, piece), h = index / each, i = index - h * each;
+                const int held = held_by(s), each = pieces_of(held, inverse), i = index % each;
                 const int even = held / each, rest = held - even * each;  // the first `rest` pieces have one page more
-                begin = (int64_t)kv_heads * g.step.page_offsets[s] + (int64_t)h * held + (i * even + min(i, rest));
-                end = begin + even + (i < rest);
+                h = index / each;
+                p0 = i * even + min(i, rest);
+                p1 = p0 + even + (i < rest);
                 first_block = range - i;
                 last_block = first_block + each - 1;
                 break;
             }
             before += __shfl_sync(~0u, upto, 31);
         }
+        end = p1 > p0;  // one segment at most
     } else if (range < shares) {
         begin = units * range / shares;
         end = units * (range + 1) / shares;
-        s = find_request(g.step.page_offsets, requests, kv_heads, begin, lane);
+        s = find_request(page_offsets, requests, kv_heads, begin, lane);
     }
 
     for (int64_t u = begin; u < end;) {
-        // Segment: pages [p0, p1) of head h of request s.
-        int64_t base = (int64_t)kv_heads * g.step.page_offsets[s];
-        int held = g.step.page_offsets[s + 1] - g.step.page_offsets[s];
-        while (u >= base + (int64_t)kv_heads * held && s + 1 < requests) {
-            ++s;
-            base = (int64_t)kv_heads * g.step.page_offsets[s];
-            held = g.step.page_offsets[s + 1] - g.step.page_offsets[s];
+        int64_t start = 0;  // shares: the head's first unit
+        int held;
+        if (pieces) {
+            held = reinterpret_cast<const int32_t*>(smem)[s];
+            u = end;
+        } else {
+            int64_t base = (int64_t)kv_heads * page_offsets[s];
+            held = page_offsets[s + 1] - page_offsets[s];
+            while (u >= base + (int64_t)kv_heads * held && s + 1 < requests) {
+                ++s;
+                base = (int64_t)kv_heads * page_offsets[s];
+                held = page_offsets[s + 1] - page_offsets[s];
+            }
+            if (held <= 0 || u < base || u >= base + (int64_t)kv_heads * held) break;  // offsets that are no prefix sum
+            h = static_cast<int>((u - base) / held);
+            start = base + (int64_t)h * held;
+            p0 = static_cast<int>(u - start);
+            p1 = static_cast<int>(min64(held, end - start));
+            u = start + p1;
         }
-        if (held <= 0 || u < base || u >= base + (int64_t)kv_heads * held) break;  // offsets that are no prefix sum
-        const int h = static_cast<int>((u - base) / held);
-        const int64_t start = base + (int64_t)h * held;  // the segment's first unit
-        const int p0 = static_cast<int>(u - start), p1 = static_cast<int>(min64(held, end - start));
-        u = start + p1;
-        const int context = g.step.context[s];
+        // This warp's chunks: keys ka + 32 (warp + kWarps i) and on.  The first page
+        // numbers are asked for together with the request's lengths.
+        const bool within = p0 < g.step.max_pages;
+        const int ka = within ? p0 << g.shift : 0;
+        const int32_t* table = g.step.table + (int64_t)s * g.step.max_pages;
+        const int pages_end = static_cast<int>(min64(p1, g.step.max_pages));
+        const auto page_of = [&](int i) {  // lanes 0-15: the page of the chunk's first group; 16-31: of the second
+            const int at = (ka + C::kChunk * (warp + C::kWarps * i) + (lane & 16)) >> g.shift;
+            return at < pages_end ? table[at] : INT_MIN;
+        };
+        int ids[C::kStages];
+#pragma unroll
+        for (int i = 0; i < C::kStages; ++i) ids[i] = page_of(i);
+        const int context = g.step.context[s], length = g.step.lengths[s];
         const int64_t row0 = max64(0, g.step.token_offsets[s]);
         const int new_rows = static_cast<int>(
             max64(0, min64(min64(g.step.token_offsets[s + 1], g.step.tokens) - row0, g.most_tokens)) * g.group);
+        if (pieces) __syncthreads();  // the requests' pages are read: the rings are free
         const int first_row = row_block * 8;
         if (first_row >= new_rows) continue;
         const int rows = min(8, new_rows - first_row);
         // Keys [ka, kb) for the block; the last row sees the most.
-        const int ka = p0 << g.shift;
-        const int kb = static_cast<int>(min64(min64((int64_t)p1 << g.shift, g.step.lengths[s]),
-                                              (int64_t)context + (first_row + rows - 1) / g.group + 1));
+        const int kb = within ? static_cast<int>(min64(min64((int64_t)p1 << g.shift, length),
+                                                       (int64_t)context + (first_row + rows - 1) / g.group + 1))
+                              : 0;
 
-        // The rows, rotated, in shared memory.
-        for (int item = tid; item < 8 * (D / 8); item += C::kThreads) {
-            const int r = item / (D / 8), j = item - r * (D / 8);
-            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
-            int at = 4 * j, to = at + D / 2;
-            if (r < rows) {
-                const int t = (first_row + r) / g.group, hq = (first_row + r) - t * g.group;
-                int64_t pos = (int64_t)context + t;
-                if (g.rotary > 0 && (pos < 0 || pos >= g.table_rows)) {
-                    if (j == 0) record_device_error(kSiteKv8Range);
-                    pos = 0;
-                }
-                query_item<D>(g, g.q + (row0 + t) * g.q_stride + (int64_t)(h * g.group + hq) * D, j, pos, at, to, a, b);
-            }
-            *reinterpret_cast<float4*>(q_s + r * D + at) = a;
-            *reinterpret_cast<float4*>(q_s + r * D + to) = b;
-        }
-
-        // This warp's chunks: keys ka + 32 (warp + kWarps i) and on.  Loads run
-        // kStages - 1 turns ahead, the page numbers they need one turn further.
+        // Loads run kStages - 1 turns ahead, the page numbers they need one turn further.
         // A chunk is two groups of 16 keys, each 16 D consecutive bytes of a page.
-        const int32_t* table = g.step.table + (int64_t)s * g.step.max_pages;
         const int chunks = kb > ka ? (kb - ka + C::kChunk - 1) / C::kChunk : 0;
         const int mine = chunks > warp ? (chunks - warp + C::kWarps - 1) / C::kWarps : 0;
-        const auto page_of = [&](int i) {  // lanes 0-15: the page of the chunk's first group; 16-31: of the second
-            const int key = ka + C::kChunk * (warp + C::kWarps * i) + (lane & 16);
-            return i < mine && key < kb && (key >> g.shift) < g.step.max_pages ? table[key >> g.shift] : INT_MIN;
-        };
-        constexpr int kPieces = D / 16;  // 16-byte pieces of a row
+        // A lane's 16-byte pieces of a group: n-th from the first, in the ring and (V) in the page.
+        constexpr int kPieces = D / 16;  // of a row
+        const int lane_row = lane / kPieces, lane_piece = lane % kPieces;
+        const int k_to = lane_row * D + 16 * k_piece<D>(lane_row, lane_piece);
+        const int v_to = lane_row * D + 16 * v_piece<D>(lane_row, lane_piece);
+        const int32_t page_bytes = (kv_heads << g.shift) * D;
+        const int8_t* k_from = g.cache.k_codes + ((int64_t)h << g.shift) * D;
+        const int8_t* v_from = g.cache.v_codes + ((int64_t)h << g.shift) * D + 16 * lane;
+        const float* scale_from = (lane == 0 ? g.cache.k_scales : g.cache.v_scales) + h;
+        int k_at[kPieces / 2];
+#pragma unroll
+        for (int n = 0; n < kPieces / 2; ++n) k_at[n] = D == 96 ? k_key((32 * n + lane) / 6) * D + 16 * ((32 * n + lane) % 6)
+                                                      : k_key(lane_row) * D + 16 * lane_piece +
+                                                            (D == 128 ? (2 * (n & 1) + 8 * (n >> 1)) * D : n * 512);
         const auto load = [&](int i, int slot, int id) {
             uint8_t* stage = ring + slot * C::kStage;
             if (i < mine) {
                 const int key = ka + C::kChunk * (warp + C::kWarps * i);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const int page_id = __shfl_sync(~0u, id, 16 * half);
-                    const int64_t tile = (int64_t)page_id * kv_heads + h;
+                    const int page_id = key + 16 * half < kb ? __shfl_sync(~0u, id, 16 * half) : INT_MIN;
                     float* scales = reinterpret_cast<float*>(stage + 2 * C::kTile) + 2 * half;
                     if (page_id >= 0 && page_id < g.cache.pages) {
-                        const int64_t src = ((tile << g.shift) + ((key + 16 * half) & (page - 1))) * D + lane * 16;
+                        const int64_t src = (int64_t)page_id * page_bytes + ((key + 16 * half) & (page - 1)) * D;
 #pragma unroll
                         for (int n = 0; n < kPieces / 2; ++n) {
-                            const int c = n * 32 + lane, r = 16 * half + c / kPieces, cc = c % kPieces;
-                            async_copy16(stage + r * D + 16 * k_piece<D>(r, cc), g.cache.k_codes + src + n * 512);
-                            async_copy16(stage + C::kTile + r * D + 16 * v_piece<D>(r, cc), g.cache.v_codes + src + n * 512);
+                            async_copy16(stage + 16 * half * D + k_to + 512 * n, k_from + src + k_at[n]);
+                            async_copy16(stage + C::kTile + 16 * half * D + v_to + 512 * n, v_from + src + 512 * n);
                         }
-                        if (lane == 0) async_copy4(scales, g.cache.k_scales + tile);
-                        if (lane == 1) async_copy4(scales + 1, g.cache.v_scales + tile);
+                        if (lane < 2) async_copy4(scales + lane, scale_from + (int64_t)page_id * kv_heads);
                     } else if (lane == 0) {
                         scales[0] = 0.0f;
                         scales[1] = -1.0f;  // the group is not there
@@ -265,56 +359,73 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
             }
             commit_async_copies();
         };
-        int next_id = page_of(0);
-#pragma unroll
-        for (int i = 0; i < C::kStages - 1; ++i) {
-            const int id = next_id;
-            next_id = page_of(i + 1);
-            load(i, i, id);
+        if (tid == 0) {
+            // Its parts' blocks i0 .. i1; a block's parts lie side by side: the head that it
+            // ends, then the one that it begins.
+            const int i0 = pieces ? first_block : static_cast<int>(((start + 1) * shares - 1) / units);
+            const int i1 = pieces ? last_block : static_cast<int>(((start + held) * shares - 1) / units);
+            segment_s.row0 = row0;
+            segment_s.h = h;
+            segment_s.rows = rows;
+            segment_s.own = p0 > 0 ? 0 : 1;
+            segment_s.parts = p0 > 0 || p1 < held ? i1 - i0 + 1 : 0;
+            segment_s.first_part = i0;
         }
-
-        __syncthreads();
-        // Query fragments: lane (gq, tq) holds row gq's elements that meet its
-        // bytes of a key: 16 of each 64 (D = 64, 128), else D / 4 in a row.
-        uint32_t q[D / 16][4];
-        float factor;  // from an MMA sum to x_j / ks
-        {
-            const float* row = q_s + gq * D;
-            uint32_t largest = 0;
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j) {
-                const int at = D % 64 == 0 ? (j / 4) * 64 + tq * 16 + (j % 4) * 4 : tq * (D / 4) + j * 4;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) largest = max(largest, __float_as_uint(row[at + e]) & 0x7fffffffu);
+        // The query rows and the first chunks are under way together.
+        constexpr int kRowThreads = D == 32 ? 4 : D == 64 ? 8 : 16;
+        static_assert(C::kThreads >= 8 * kRowThreads && kRowThreads >= D / 8, "one item of the query rows a thread");
+        const int row = tid / kRowThreads, item = tid % kRowThreads;
+        QueryItem<D> rows_item;
+        if (row < 8 && item < D / 8) {
+            const int t = (first_row + row) / g.group, hq = (first_row + row) - t * g.group;
+            int64_t pos = (int64_t)context + t;
+            if (row < rows && g.rotary > 0 && (pos < 0 || pos >= g.table_rows)) {
+                if (item == 0) record_device_error(kSiteKv8Range);
+                pos = 0;
             }
-            largest = max(largest, __shfl_xor_sync(~0u, largest, 1));
-            largest = max(largest, __shfl_xor_sync(~0u, largest, 2));
+            rows_item.load(g, row < rows ? g.q + (row0 + t) * g.q_stride + (int64_t)(h * g.group + hq) * D : nullptr, item, pos);
+        }
+#pragma unroll
+        for (int i = 0; i < C::kStages - 1; ++i) load(i, i, ids[i]);
+        int next_id = ids[C::kStages - 1];
+        if (row < 8) {
+            // Four elements in a row are one lane's part of one MMA: lane (gq, tq) holds
+            // row gq's elements that meet its bytes of a key, 16 of each 64 (D = 64, 128)
+            // or D / 4 in a row.
+            if (item < D / 8) rows_item.turn();
+            uint32_t largest = item < D / 8 ? rows_item.largest() : 0;
+#pragma unroll
+            for (int d = 1; d < kRowThreads; d *= 2) largest = max(largest, __shfl_xor_sync(~0u, largest, d));
             float up, down;
             row_power(largest, up, down);
-            factor = down * g.scale * kLog2e;
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j) {
-                const int at = D % 64 == 0 ? (j / 4) * 64 + tq * 16 + (j % 4) * 4 : tq * (D / 4) + j * 4;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float x = row[at + 2 * e] * up, y = row[at + 2 * e + 1] * up;
-                    const uint32_t hi = half2_bits(x, y);
-                    const __half2 h2 = *reinterpret_cast<const __half2*>(&hi);
-                    q[j][2 * e] = hi;
-                    q[j][2 * e + 1] = half2_bits(x - __low2float(h2), y - __high2float(h2));
-                }
+            if (item == 0) factor_s[row] = down * g.scale * kLog2e;
+            const auto put = [&](int at, float4 x) {
+                const int j = D % 64 == 0 ? at / 64 * 4 + at % 16 / 4 : at % (D / 4) / 4;
+                const int t = D % 64 == 0 ? at % 64 / 16 : at / (D / 4);
+                const float a = x.x * up, b = x.y * up, c = x.z * up, d = x.w * up;
+                const uint32_t ab = half2_bits(a, b), cd = half2_bits(c, d);
+                const __half2 ab2 = *reinterpret_cast<const __half2*>(&ab), cd2 = *reinterpret_cast<const __half2*>(&cd);
+                q_s[j * 32 + row * 4 + t] = make_uint4(ab, half2_bits(a - __low2float(ab2), b - __high2float(ab2)), cd,
+                                                       half2_bits(c - __low2float(cd2), d - __high2float(cd2)));
+            };
+            if (item < D / 8) {
+                put(rows_item.at, rows_item.a);
+                put(rows_item.to, rows_item.b);
             }
         }
+        __syncthreads();
+        uint32_t q[D / 16][4];
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) *reinterpret_cast<uint4*>(q[j]) = q_s[j * 32 + lane];
+        const float factor = factor_s[gq];  // from an MMA sum to x_j / ks
         // Keys that row gq sees; none for a row past the request's.
         const int64_t row_pos = (int64_t)context + (first_row + gq) / g.group;
         const bool seen = gq < rows && row_pos >= 0 && (g.rotary == 0 || row_pos < g.table_rows);
         const int limit = seen ? static_cast<int>(min64(kb, row_pos + 1)) : 0;
 
-        float o[D / 8][4], m = -INFINITY, l = 0.0f;
+        float o[D / 8][2], m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+        for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = 0.0f;
 
         int slot = 0;
         for (int i = 0; i < mine; ++i) {
@@ -345,8 +456,7 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                // Column c of the tile is key (c >> 1) + 4 (c & 1): lane gq's key.
-                const int r = 8 * n + (gq >> 1) + 4 * (gq & 1);
+                const int r = 8 * n + gq;
                 uint32_t w[D / 16];
                 if constexpr (D % 64 == 0) {
 #pragma unroll
@@ -410,43 +520,54 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
                 m = raised;
                 l *= down;
 #pragma unroll
-                for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][e] *= down;
+                for (int j = 0; j < D / 8; ++j) {
+                    o[j][0] *= down;
+                    o[j][1] *= down;
+                }
             }
             l += sum;
             // A chunk's products sum up in the MMA, whose additions truncate; the
             // chunks are added in rounded fp32.
             constexpr int kWords = D / 32;
+            // Keys 16 step + 4 k + tq, elements gq (D / 8) ..: byte n of word c is n-tile 4 c + n's column gq.
+            uint32_t w[2][4][kWords];
+#pragma unroll
+            for (int step = 0; step < 2; ++step)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int r = 16 * step + 4 * k + tq;
+                    const uint8_t* row = stage + C::kTile + r * D;
+                    if constexpr (D == 128) {
+                        *reinterpret_cast<uint4*>(w[step][k]) = *reinterpret_cast<const uint4*>(row + 16 * v_piece<D>(r, gq));
+                    } else if constexpr (D == 64) {
+                        *reinterpret_cast<uint2*>(w[step][k]) =
+                            *reinterpret_cast<const uint2*>(row + 16 * v_piece<D>(r, gq >> 1) + 8 * (gq & 1));
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < kWords; ++c)
+                            w[step][k][c] = *reinterpret_cast<const uint32_t*>(row + gq * (D / 8) + 4 * c);
+                    }
+                }
 #pragma unroll
             for (int c = 0; c < kWords; ++c) {
                 float part[4][4] = {};
 #pragma unroll
                 for (int step = 0; step < 2; ++step) {
-                    // Keys 16 step + 4 k + tq, elements gq (D / 8) ..: byte n of them is n-tile n's column gq.
-                    uint32_t w[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int r = 16 * step + 4 * k + tq;
-                        const uint8_t* row = stage + C::kTile + r * D;
-                        w[k] = *reinterpret_cast<const uint32_t*>(
-                                   D == 128 ? row + 16 * v_piece<D>(r, gq) + 4 * c
-                                            : (D == 64 ? row + 16 * v_piece<D>(r, gq >> 1) + 8 * (gq & 1) + 4 * c
-                                                       : row + gq * (D / 8) + 4 * c)) ^
-                               0x80808080u;
-                    }
                     // Bytes of keys (2t, 2t+1) and (2t+8, 2t+9) side by side.
-                    const uint32_t a01 = __byte_perm(w[0], w[1], 0x5140), a23 = __byte_perm(w[0], w[1], 0x7362);
-                    const uint32_t b01 = __byte_perm(w[2], w[3], 0x5140), b23 = __byte_perm(w[2], w[3], 0x7362);
+                    const uint32_t x0 = w[step][0][c] ^ 0x80808080u, x1 = w[step][1][c] ^ 0x80808080u,
+                                   x2 = w[step][2][c] ^ 0x80808080u, x3 = w[step][3][c] ^ 0x80808080u;
+                    const uint32_t a01 = __byte_perm(x0, x1, 0x5140), a23 = __byte_perm(x0, x1, 0x7362);
+                    const uint32_t b01 = __byte_perm(x2, x3, 0x5140), b23 = __byte_perm(x2, x3, 0x7362);
                     mma_f16(part[0], p[step], codes_half2(a01, 0x4140u), codes_half2(b01, 0x4140u));
                     mma_f16(part[1], p[step], codes_half2(a01, 0x4342u), codes_half2(b01, 0x4342u));
                     mma_f16(part[2], p[step], codes_half2(a23, 0x4140u), codes_half2(b23, 0x4140u));
                     mma_f16(part[3], p[step], codes_half2(a23, 0x4342u), codes_half2(b23, 0x4342u));
                 }
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[4 * c + n][e] += part[n][e];
+                for (int n = 0; n < 4; ++n) {
+                    o[4 * c + n][0] += part[n][0] + part[n][2];
+                    o[4 * c + n][1] += part[n][1] + part[n][3];
+                }
             }
             __syncwarp();  // the stage is read before it is copied into again
         }
@@ -464,12 +585,13 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
 #pragma unroll
         for (int j = 0; j < D / 8; ++j) {
             // n-tile j's columns 2t, 2t+1 are elements (2t) (D/8) + j and (2t+1) (D/8) + j.
-            part[16 + gq * D + 2 * tq * (D / 8) + j] = o[j][0] + o[j][2];
-            part[16 + gq * D + (2 * tq + 1) * (D / 8) + j] = o[j][1] + o[j][3];
+            part[16 + gq * D + 2 * tq * (D / 8) + j] = o[j][0];
+            part[16 + gq * D + (2 * tq + 1) * (D / 8) + j] = o[j][1];
         }
         __syncthreads();
-        const bool split = p0 > 0 || p1 < held;
-        const int64_t mine_part = ((2 * (int64_t)range + (p0 > 0 ? 0 : 1)) * row_blocks + row_block) * C::kPart;
+        const int count = segment_s.parts, rows_here = segment_s.rows;
+        float* out = g.out + segment_s.row0 * g.heads * D + (int64_t)segment_s.h * g.group * D;
+        float* own = parts + ((2 * (int64_t)range + segment_s.own) * row_blocks + row_block) * C::kPart;
         for (int item = tid; item < 8 * D; item += C::kThreads) {
             const int r = item / D, d = item - r * D;
             float top = -INFINITY, sum = 0.0f, total = 0.0f;
@@ -482,86 +604,32 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
                 total = fmaf(weight, other[8 + r], total);
                 sum = fmaf(weight, other[16 + item], sum);
             }
-            if (split) {
-                float* to = parts + mine_part;
+            if (count > 0) {
                 if (d == 0) {
-                    to[r] = top;
-                    to[8 + r] = total;
+                    own[r] = top;
+                    own[8 + r] = total;
                 }
-                to[16 + item] = sum;
-            } else if (r < rows) {
+                own[16 + item] = sum;
+            } else if (r < rows_here) {
                 const int t = (first_row + r) / g.group, hq = (first_row + r) - t * g.group;
-                g.out[(row0 + t) * (int64_t)g.heads * D + (int64_t)(h * g.group + hq) * D + d] = total == 0.0f ? 0.0f : sum / total;
+                out[t * (int64_t)g.heads * D + hq * D + d] = total == 0.0f ? 0.0f : sum / total;
             }
         }
-        if (split) {
-            // The last block to arrive joins the segment's parts, in block order.
-            const int64_t i0 = pieces ? first_block : ((start + 1) * shares - 1) / units,
-                          i1 = pieces ? last_block : ((start + held) * shares - 1) / units;
-            __threadfence();
+        if (count > 0) {
+            // The last block to arrive joins the segment's parts.
+            const int64_t first = (2 * (int64_t)segment_s.first_part * row_blocks + row_block) * C::kPart;
             __syncthreads();
             if (tid == 0) {
-                uint32_t* arrived = arrivals + i0 * row_blocks + row_block;
-                last_s = atomicAdd(arrived, 1u) == static_cast<uint32_t>(i1 - i0);
+                __threadfence();
+                uint32_t* arrived = arrivals + (int64_t)segment_s.first_part * row_blocks + row_block;
+                last_s = atomicAdd(arrived, 1u) == static_cast<uint32_t>(count - 1);
                 if (last_s) *arrived = 0;
+                __threadfence();
             }
             __syncthreads();
-            if (last_s) {
-                __threadfence();
-                // Weights of the parts' rows, then their weighted sums, four elements and
-                // every kSets-th part per thread.
-                const int n = static_cast<int>(i1 - i0) + 1;
-                const auto other = [&](int i) {
-                    return parts + ((2 * (i0 + i) + (i == 0 ? 1 : 0)) * row_blocks + row_block) * C::kPart;
-                };
-                float* weight_s = reinterpret_cast<float*>(smem);  // [n][8], then the rows' sums [8]
-                for (int r = warp; r < 8; r += C::kWarps) {
-                    float top = -INFINITY, total = 0.0f;
-                    for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(other(i) + r));
-                    top = warp_max_f32(top);
-                    for (int i = lane; i < n; i += 32) {
-                        const float their = __ldcg(other(i) + r), part_l = __ldcg(other(i) + 8 + r);
-                        const float weight = their == -INFINITY ? (part_l == 0.0f ? 0.0f : 1.0f) : ex2(their - top);
-                        weight_s[i * 8 + r] = weight;
-                        total = fmaf(weight, part_l, total);
-                    }
-#pragma unroll
-                    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
-                    if (lane == 0) weight_s[n * 8 + r] = total;
-                }
-                __syncthreads();
-                constexpr int kItems = 8 * D / 4, kSets = C::kThreads > kItems ? C::kThreads / kItems : 1;
-                float4* set_s = reinterpret_cast<float4*>(weight_s + (n * 8 + 8));
-                for (int item = tid % kItems, set = tid / kItems; item < kItems && set < kSets; item += C::kThreads) {
-                    const int r = item / (D / 4);
-                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-                    for (int i = set; i < n; i += kSets) {
-                        const float weight = weight_s[i * 8 + r];
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(other(i) + 16) + item);
-                        sum.x = fmaf(weight, v.x, sum.x);
-                        sum.y = fmaf(weight, v.y, sum.y);
-                        sum.z = fmaf(weight, v.z, sum.z);
-                        sum.w = fmaf(weight, v.w, sum.w);
-                    }
-                    set_s[set * kItems + item] = sum;
-                }
-                __syncthreads();
-                for (int item = tid; item < rows * (D / 4); item += C::kThreads) {
-                    const int r = item / (D / 4), d = 4 * (item - r * (D / 4));
-                    float4 sum = set_s[item];
-#pragma unroll
-                    for (int set = 1; set < kSets; ++set) {
-                        const float4 v = set_s[set * kItems + item];
-                        sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
-                    }
-                    const float total = weight_s[n * 8 + r];
-                    const float4 y = total == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                                                   : make_float4(sum.x / total, sum.y / total, sum.z / total, sum.w / total);
-                    const int t = (first_row + r) / g.group, hq = (first_row + r) - t * g.group;
-                    *reinterpret_cast<float4*>(g.out + (row0 + t) * (int64_t)g.heads * D + (int64_t)(h * g.group + hq) * D + d) = y;
-                }
-            }
+            if (last_s)
+                join_parts<D>(smem, parts + first, 2 * (int64_t)row_blocks * C::kPart, (int64_t)row_blocks * C::kPart, count,
+                              rows_here, g.group, first_row, out, (int64_t)g.heads * D);
         }
         __syncthreads();  // the rings and q_s are free for the next segment
     }

@@ -72,21 +72,41 @@ __device__ __forceinline__ void kv8_turn(float4& a, float4& b, float4 c, float4 
                     __fadd_rn(__fmul_rn(y.z, c.z), __fmul_rn(x.z, s.z)), __fadd_rn(__fmul_rn(y.w, c.w), __fmul_rn(x.w, s.w)));
 }
 
-// Eight values of a query row, its item j of D / 8 (a rotation pair's quarters
-// as in the append): a at `at`, b at `to`.
+// Eight values of a query row, its item j of D / 8: four at `at` and four at
+// `to`, a rotation pair's quarters where they are turned (as in the append).
 template <int D>
-__device__ __forceinline__ void query_item(const Kv8AttendArgs& g, const float* row, int j, int64_t pos, int& at, int& to,
-                                           float4& a, float4& b) {
-    const int half = g.rotary >> 1;
-    const bool turned = 4 * j < half;
-    at = turned ? 4 * j : 2 * half + 4 * (j - half / 4);
-    to = turned ? at + half : at + ((D - 2 * half) >> 1);
-    a = *reinterpret_cast<const float4*>(row + at);
-    b = *reinterpret_cast<const float4*>(row + to);
-    if (turned)
-        kv8_turn(a, b, *reinterpret_cast<const float4*>(g.cos_table + pos * half + at),
-                 *reinterpret_cast<const float4*>(g.sin_table + pos * half + at));
-}
+struct QueryItem {
+    int at, to;
+    bool turned;
+    float4 a, b, cos, sin;
+
+    // row: null for a row of zeros.
+    __device__ __forceinline__ void load(const Kv8AttendArgs& g, const float* row, int j, int64_t pos) {
+        const int half = g.rotary >> 1;
+        turned = 4 * j < half;
+        at = turned ? 4 * j : 2 * half + 4 * (j - half / 4);
+        to = turned ? at + half : at + ((D - 2 * half) >> 1);
+        a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (row == nullptr) {
+            turned = false;
+            return;
+        }
+        a = *reinterpret_cast<const float4*>(row + at);
+        b = *reinterpret_cast<const float4*>(row + to);
+        if (turned) {
+            cos = *reinterpret_cast<const float4*>(g.cos_table + pos * half + at);
+            sin = *reinterpret_cast<const float4*>(g.sin_table + pos * half + at);
+        }
+    }
+    __device__ __forceinline__ void turn() {
+        if (turned) kv8_turn(a, b, cos, sin);
+    }
+    __device__ __forceinline__ uint32_t largest() const {  // the magnitude's bits
+        uint32_t most = 0;
+        for (const float x : {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}) most = max(most, __float_as_uint(x) & 0x7fffffffu);
+        return most;
+    }
+};
 
 // The power of two that brings a row's largest magnitude into [256, 512), as
 // a float and its inverse (1 for a row of zeros): exact, and fp16's range
