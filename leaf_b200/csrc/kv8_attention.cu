@@ -761,7 +761,7 @@ int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int head
     while ((1 << g.shift) < cache->page) ++g.shift;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool pdl = (flags & LEAFQ_FLAG_PDL) != 0;
-    if (takes_tiles(step->tokens, step->max_tokens, heads, g.group, cache->dim)) return launch_kv8_tiles(s, g, pdl);
+    if (takes_tiles(step->tokens, step->max_tokens, heads, g.group, cache->dim)) return launch_kv8_tiles(s, g, workspace, pdl);
     return with_dim(cache->dim, [&](auto d) { return run_split<d()>(s, g, workspace, pdl); });
 }
 

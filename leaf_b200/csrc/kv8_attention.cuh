@@ -121,6 +121,6 @@ __device__ __forceinline__ void row_power(uint32_t largest_bits, float& up, floa
 }
 
 // Many query rows of a request (kv8_tile.cu).
-int launch_kv8_tiles(cudaStream_t s, const Kv8AttendArgs& g, bool pdl);
+int launch_kv8_tiles(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl);
 
 }  // namespace leafq

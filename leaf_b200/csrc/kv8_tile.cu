@@ -44,6 +44,11 @@ struct TileItem {
     uint8_t power[128];  // of two, that each row was scaled down by (its exponent bits)
 };
 
+// An item as the converting warps take it; rows < 0: there are no more.
+struct NextItem {
+    int row0, first_row, rows, context, keys, request, head, unused;
+};
+
 template <int D>
 struct TileShape {
     static constexpr int kRows = 128;
@@ -69,7 +74,7 @@ struct TileShape {
     static constexpr bool kSumInSmem = D <= 64;          // else in local memory
     static constexpr int kSumBytes = kSumInSmem ? kRows * D * 4 : 0;
     static constexpr size_t kSmem = 2 * kQBytes + (kKStages + kVStages) * kKvBytes + kSumBytes + kInfo * kGroups * 16 +
-                                    sizeof(TileItem) + (2 * kKStages + 2 * kVStages + 9) * 8 + 8;
+                                    sizeof(TileItem) + 2 * sizeof(NextItem) + (2 * kKStages + 2 * kVStages + 11) * 8 + 8;
     static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two blocks share the SM's shared memory");
     static_assert(2 * kKeys + kOutCols <= 256, "two blocks share the SM's 512 TMEM columns");
     static_assert(kSoftmaxRegs + kOtherRegs <= 2 * kLaunchRegs, "the split of what the launch gives each scheduler");
@@ -163,7 +168,7 @@ __device__ __forceinline__ void store_local(uint32_t at, float4 v) {
 
 template <int D>
 __global__ void __launch_bounds__(TileShape<D>::kThreads, 2)
-kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_tiles) {
+kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t* taken, int row_tiles) {
     using C = TileShape<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* q_hi = smem;
@@ -173,7 +178,8 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
     float4* sum_s = reinterpret_cast<float4*>(v_tiles + C::kVStages * C::kKvBytes);  // kSumInSmem: [4 warps][D / 4][32]
     float4* info = sum_s + C::kSumBytes / 16;                                        // [kInfo][kGroups]: ks, log2 vs, 1 / vs
     TileItem* item = reinterpret_cast<TileItem*>(info + C::kInfo * C::kGroups);
-    uint64_t* k_full = reinterpret_cast<uint64_t*>(item + 1);
+    NextItem* found = reinterpret_cast<NextItem*>(item + 1);  // by the item's parity
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(found + 2);
     uint64_t* k_empty = k_full + C::kKStages;
     uint64_t* v_full = k_empty + C::kKStages;
     uint64_t* v_empty = v_full + C::kVStages;
@@ -184,7 +190,8 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
     uint64_t* q_empty = q_full + 1;            // its last scores are computed, its description is read
     uint64_t* item_done = q_empty + 1;         // all its MMAs have completed
     uint64_t* drained = item_done + 1;
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
+    uint64_t* found_full = drained + 1;        // by the item's parity
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(found_full + 2);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kMmaWarp = 8;
     const auto token_of = [&](int row) { return static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(g.group)); };
@@ -212,6 +219,8 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
             mbar_init(q_empty, 1 + 4);
             mbar_init(item_done, 1);
             mbar_init(drained, 1);
+            mbar_init(&found_full[0], 1);
+            mbar_init(&found_full[1], 1);
             fence_barrier_init();
         }
         __syncwarp();
@@ -464,21 +473,25 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
         const int page = 1 << g.shift;
         const uint32_t page_pieces = (static_cast<uint32_t>(g.cache.kv_heads) << g.shift) * (D / 16);  // 16-byte pieces of a page
 
-        // Items: row tiles x kv heads, those that see most keys first, dealt to the
-        // blocks back and forth.  Request s may have row tiles
-        // floor(token_offsets[s] * group / 128) + s and on: enough of them.
+        // Items: row tiles x kv heads, those of a request that see most keys first.
+        // Request s may have row tiles floor(token_offsets[s] * group / 128) + s and
+        // on: enough of them.  A block's first item is its own number; warp 4 takes
+        // the next ones from a counter that all blocks share, while the last tile of
+        // the item before is on its way, and tells the other three.
         const uint32_t total = static_cast<uint32_t>(row_tiles) * g.cache.kv_heads;
-        struct Next {
-            int row0, first_row, rows, context, keys, request, head;
-        };
-        int round = 0;
-        const auto advance = [&](Next& next) {
+        bool first_take = true;
+        const auto advance = [&](int it) {
+            NextItem next = {};
+            next.rows = -1;
 #pragma unroll 1
-            for (;; ++round) {
-                const uint32_t base = static_cast<uint32_t>(round) * gridDim.x;
-                if (base >= total) return false;
-                const uint32_t id = base + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-                if (id >= total) continue;
+            while (true) {
+                uint32_t id = blockIdx.x;
+                if (!first_take) {
+                    if (lane == 0) id = gridDim.x + atomicAdd(taken, 1u);
+                    id = __shfl_sync(~0u, id, 0);
+                }
+                first_take = false;
+                if (id >= total) break;
                 const uint32_t group_of = id / static_cast<uint32_t>(g.cache.kv_heads);
                 const int index = row_tiles - 1 - static_cast<int>(group_of);
                 next.head = static_cast<int>(id - group_of * g.cache.kv_heads);
@@ -503,9 +516,13 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 const int held = min(g.step.page_offsets[s + 1] - g.step.page_offsets[s], static_cast<int>(g.step.max_pages));
                 const int seen = next.context + token_of(next.first_row + next.rows - 1) + 1;  // by the last row
                 next.keys = max(0, min(min(held << g.shift, g.step.lengths[s]), seen));
-                ++round;
-                return true;
+                break;
             }
+            if (lane == 0) {
+                found[it & 1] = next;
+                mbar_arrive(&found_full[it & 1]);
+            }
+            __syncwarp();
         };
         // Lanes of a row: D / 8, eight values each (a rotation pair's quarters).
         constexpr int kLanes = D / 8;  // 4, 8, 12, 16
@@ -519,7 +536,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
         // Loads run two turns ahead; rotated, scaled by the row's power of two, split,
         // stored swizzled.
         const int step_t = kPass / g.group, step_h = kPass - step_t * g.group;
-        const auto put_rows = [&](const Next& next, uint8_t* power) {
+        const auto put_rows = [&](const NextItem& next, uint8_t* power) {
             float4 a, b, cs, sn, a1, b1, cs1, sn1;  // this turn's, the next one's
             a = b = cs = sn = a1 = b1 = cs1 = sn1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             const int r0 = next.first_row + cw * kAtOnce + sub;
@@ -624,16 +641,22 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
             if (D == 32) return ct & 1;
             return i < 4 ? ct & 3 : 4 + (ct & 1);
         };
-        Next now = {}, next;
-        bool more = false, ok = true;
+        bool ok = true;
         int n = 0;  // tiles of the items before
         // (Every piece of work stands once: the roles' code shares the instruction
         // cache.  Turn -1 only finds the first item.)
         for (int it = -1;; ++it) {
-            if (it > 0) ok = __all_sync(~0u, tile_wait(watch, q_empty, (it - 1) & 1));
-            if (!ok) break;
-            const int keys = more ? now.keys : 0;
-            const int tiles = more ? max(1, (keys + C::kKeys - 1) / C::kKeys) : -1;  // without keys, a tile that is all hidden
+            NextItem now = {};
+            if (it >= 0) {
+                ok = __all_sync(~0u, tile_wait(watch, &found_full[it & 1], (it >> 1) & 1));
+                if (!ok) break;
+                now = found[it & 1];
+                if (it > 0) ok = __all_sync(~0u, tile_wait(watch, q_empty, (it - 1) & 1));
+                if (!ok) break;
+            }
+            const bool more = it >= 0 && now.rows >= 0;
+            const int keys = now.keys;
+            const int tiles = more ? max(1, (keys + C::kKeys - 1) / C::kKeys) : it < 0 ? 0 : -1;  // without keys, a tile that is all hidden
             if (it >= 0 && tid == 128) {
                 item->row0 = now.row0;
                 item->first_row = now.first_row;
@@ -685,16 +708,6 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 }
             };
             if (it >= 0) ask_pages(0);
-            // The next item meanwhile, and its rows into L2.
-            more = advance(next);
-            if (more) {
-#pragma unroll 1
-                for (int i = tid - 128; i < next.rows * (D / 32); i += 128) {
-                    const int r = i / (D / 32), t = token_of(next.first_row + r), hq = (next.first_row + r) - t * g.group;
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(g.q + ((int64_t)next.row0 + t) * g.q_stride +
-                                                                  (int64_t)(next.head * g.group + hq) * D + 32 * (i % (D / 32))));
-                }
-            }
             if (it >= 0) {
                 put_rows(now, item->power);
                 fence_proxy_async_smem();
@@ -704,7 +717,9 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 ask_pages(1);
             }
 #pragma unroll 1
-            for (int j = 0; j < (it >= 0 ? tiles : 0); ++j) {
+            for (int j = it >= 0 ? 0 : -1; j < tiles || j < 0; ++j) {
+                if (cw == 0 && j == tiles - 1) advance(it + 1);
+                if (j < 0) break;
                 const int tile = n + j, stage = tile % stages;
                 if (tile >= stages) ok = __all_sync(~0u, tile_wait(watch, &empty[stage], (tile / stages - 1) & 1));
                 if (!ok) break;
@@ -737,8 +752,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
                 ask_pages(j + 2);
             }
             if (!ok) break;
-            if (it >= 0) n += tiles;
-            now = next;
+            n += tiles;
         }
     } else {
         // ------------------------------------------------------ MMA issue
@@ -820,10 +834,15 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, int row_t
         tcgen05_fence_after();
         tmem_dealloc(tmem, C::kTmemCols);
     }
+    // The last block leaves the counters as it found them.
+    if (tid == 0) {
+        __threadfence();
+        if (atomicAdd(taken + 1, 1u) == gridDim.x - 1) taken[0] = taken[1] = 0;
+    }
 }
 
 template <int D>
-int run_tile(cudaStream_t s, const Kv8AttendArgs& g, bool pdl) {
+int run_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) {
     DeviceWatch watch;
     int st = device_watch(&watch);
     if (st) return st;
@@ -851,17 +870,17 @@ int run_tile(cudaStream_t s, const Kv8AttendArgs& g, bool pdl) {
     const int64_t blocks = std::min<int64_t>(row_tiles * g.cache.kv_heads, 2 * (int64_t)sm_count());
     return launch(kv8_attend_tile_kernel<D>, dim3(static_cast<unsigned>(blocks)),
                   dim3(TileShape<D>::kThreads), TileShape<D>::kSmem, s, pdl, "leafq_kv8_attention", g, watch,
-                  static_cast<int>(row_tiles));
+                  static_cast<uint32_t*>(workspace), static_cast<int>(row_tiles));
 }
 
 }  // namespace
 
-int launch_kv8_tiles(cudaStream_t s, const Kv8AttendArgs& g, bool pdl) {
+int launch_kv8_tiles(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) {
     switch (g.cache.dim) {
-        case 32: return run_tile<32>(s, g, pdl);
-        case 64: return run_tile<64>(s, g, pdl);
-        case 96: return run_tile<96>(s, g, pdl);
-        default: return run_tile<128>(s, g, pdl);
+        case 32: return run_tile<32>(s, g, workspace, pdl);
+        case 64: return run_tile<64>(s, g, workspace, pdl);
+        case 96: return run_tile<96>(s, g, workspace, pdl);
+        default: return run_tile<128>(s, g, workspace, pdl);
     }
 }
 
