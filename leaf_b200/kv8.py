@@ -39,38 +39,35 @@ def _need(ok: bool, message: str) -> None:
 
 # The calls sit in a decode loop, a few microseconds each: the checks below ask
 # each tensor as little as they can and build their messages only to fail.
-def _check_i32(t: torch.Tensor, name: str, numel: Optional[int] = None, device=None) -> None:
-    if not (t.is_cuda and t.dtype is _I32 and t.is_contiguous()):
-        _fail(f"{name} must be a contiguous int32 CUDA tensor")
+# index: of the CUDA device they have to be on (a tensor elsewhere has -1).
+def _check_i32(t: torch.Tensor, name: str, numel: Optional[int] = None, index: Optional[int] = None) -> None:
+    if not (t.dtype is _I32 and t.is_contiguous() and (t.is_cuda if index is None else t.get_device() == index)):
+        _fail(f"{name} must be a contiguous int32 CUDA tensor, on the others' device")
     if numel is not None and t.numel() != numel:
         _fail(f"{name} must hold {numel} values")
-    if device is not None and t.device != device:
-        _fail(f"{name} is on another device")
 
 
-def _check_rows(t: torch.Tensor, name: str, width: int, device) -> int:
+def _check_rows(t: torch.Tensor, name: str, width: int, index: int) -> int:
     """fp32 [tokens, width] rows, contiguous in themselves (columns of a wider
     matrix are).  Returns their stride."""
     shape = t.shape
-    if not (t.is_cuda and t.dtype is _F32 and len(shape) == 2 and shape[1] == width):
-        _fail(f"{name} must be float32 [tokens, {width}] on a CUDA device")
-    if t.device != device:
-        _fail(f"{name} is on another device")
+    if not (t.get_device() == index and t.dtype is _F32 and len(shape) == 2 and shape[1] == width):
+        _fail(f"{name} must be float32 [tokens, {width}] on the cache's CUDA device")
     stride, inner = t.stride()
     if shape[0] != 0 and (inner != 1 or (stride < width and shape[0] != 1)):
         _fail(f"the rows of {name} must be contiguous and must not overlap")
     return stride
 
 
-def _rope_args(rope, dim: int, device):
+def _rope_args(rope, dim: int, index: int):
     """(rotary_dim, cos, sin, rows) for the C call."""
     if rope is None:
         return 0, None, None, 0
     cos, sin = rope
     shape = cos.shape
-    if not (cos.is_cuda and cos.dtype is _F32 and sin.dtype is _F32 and len(shape) == 2 and sin.shape == shape and
-            cos.is_contiguous() and sin.is_contiguous() and cos.device == device and sin.device == device):
-        _fail("rope tables must be two contiguous float32 [positions, rotary_dim / 2] CUDA tensors")
+    if not (cos.get_device() == index and sin.get_device() == index and cos.dtype is _F32 and sin.dtype is _F32 and
+            len(shape) == 2 and sin.shape == shape and cos.is_contiguous() and sin.is_contiguous()):
+        _fail("rope tables must be two contiguous float32 [positions, rotary_dim / 2] tensors on the cache's CUDA device")
     if 2 * shape[1] > dim:
         _fail("rope tables are wider than the head")
     return 2 * shape[1], cos.data_ptr(), sin.data_ptr(), shape[0]
@@ -118,10 +115,10 @@ class Kv8Plan:
         _need(table.dim() == 2, "the block table must be [requests, max_pages]")
         requests, device = table.shape[0], table.device
         _check_i32(table, "the block table")
-        _check_i32(context, "context", requests, device)
-        _check_i32(lengths, "lengths", requests, device)
-        _check_i32(token_offsets, "token_offsets", requests + 1, device)
-        _check_i32(page_offsets, "page_offsets", requests + 1, device)
+        _check_i32(context, "context", requests, device.index)
+        _check_i32(lengths, "lengths", requests, device.index)
+        _check_i32(token_offsets, "token_offsets", requests + 1, device.index)
+        _check_i32(page_offsets, "page_offsets", requests + 1, device.index)
         _need(tokens >= 0 and max_tokens >= 0, "token counts must not be negative")
         self.context, self.lengths, self.table = context, lengths, table
         self.token_offsets, self.page_offsets = token_offsets, page_offsets
@@ -186,10 +183,9 @@ def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tenso
                        tokens if max_tokens is None else max_tokens, positions, slots, after)
         plan.inputs = (context.data_ptr(), table.data_ptr(), table.shape[1])
         plan.outputs = tuple(p.data_ptr() for p in (lengths, token_offsets, page_offsets, positions, slots, after))
-    device = plan.device
-    _check_i32(new_tokens, "new_tokens", requests, device)
-    _check_i32(free_pages, "free_pages", None, device)
-    _check_i32(taken, "taken", 1, device)
+    _check_i32(new_tokens, "new_tokens", requests, plan.index)
+    _check_i32(free_pages, "free_pages", None, plan.index)
+    _check_i32(taken, "taken", 1, plan.index)
     check(load().leafq_kv8_plan(_raw_stream(plan.index), plan.inputs[0], new_tokens.data_ptr(), requests, plan.inputs[1],
                                 plan.inputs[2], free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(), page, tokens,
                                 *plan.outputs, flags))
@@ -203,21 +199,21 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: Kv8Cache, slots: torch.T
     With rope = (cos, sin) tables [positions, rotary_dim / 2] the keys are
     rotated by ``positions`` first.  A page's scale grows when a new row needs
     it, and its older codes are rounded to the new scale."""
-    device = cache.device
-    k_stride = _check_rows(k, "k", cache.width, device)
-    v_stride = _check_rows(v, "v", cache.width, device)
+    index = cache.index
+    k_stride = _check_rows(k, "k", cache.width, index)
+    v_stride = _check_rows(v, "v", cache.width, index)
     tokens = k.shape[0]
     if v.shape[0] != tokens:
         _fail("k and v must have the same rows")
-    _check_i32(slots, "slots", tokens, device)
-    rotary, cos, sin, rows = _rope_args(rope, cache.dim, device)
+    _check_i32(slots, "slots", tokens, index)
+    rotary, cos, sin, rows = _rope_args(rope, cache.dim, index)
     where = None
     if rope is not None:
         if positions is None:
             _fail("rotation needs positions")
-        _check_i32(positions, "positions", tokens, device)
+        _check_i32(positions, "positions", tokens, index)
         where = positions.data_ptr()
-    check(load().leafq_kv8_append(_raw_stream(cache.index), k.data_ptr(), k_stride, v.data_ptr(), v_stride, tokens, where,
+    check(load().leafq_kv8_append(_raw_stream(index), k.data_ptr(), k_stride, v.data_ptr(), v_stride, tokens, where,
                                   slots.data_ptr(), rotary, cos, sin, rows, cache.ref, flags))
 
 
@@ -229,22 +225,22 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float,
     rotated by position when rope tables are given.  Returns fp32
     [tokens, heads * dim]; a row that sees no key is zero, rows past the step's
     last new token are not written."""
-    device, dim, shape = cache.device, cache.dim, q.shape
+    index, dim, shape = cache.index, cache.dim, q.shape
     if len(shape) != 2 or shape[1] % dim != 0:
         _fail("q must be [tokens, heads * dim]")
     tokens, width = shape
-    stride = _check_rows(q, "q", width, device)
+    stride = _check_rows(q, "q", width, index)
     if tokens != plan.tokens:
         _fail("q has other rows than the plan")
-    if plan.device != device:
+    if plan.index != index:
         _fail("the plan is on another device")
     if out is None:
-        out = torch.empty((tokens, width), dtype=_F32, device=device)
-    elif not (out.is_cuda and out.dtype is _F32 and out.is_contiguous() and out.shape == shape and out.device == device):
-        _fail("out must be contiguous float32 of q's shape")
-    rotary, cos, sin, rows = _rope_args(rope, dim, device)
+        out = torch.empty_like(q)  # contiguous, as q's rows do not overlap
+    elif not (out.get_device() == index and out.dtype is _F32 and out.is_contiguous() and out.shape == shape):
+        _fail("out must be contiguous float32 of q's shape, on its device")
+    rotary, cos, sin, rows = _rope_args(rope, dim, index)
     heads = width // dim
-    address, need = (Kv8Workspace(device) if workspace is None else workspace).of(plan.max_tokens, heads, cache.kv_heads, dim)
-    check(load().leafq_kv8_attention(_raw_stream(cache.index), q.data_ptr(), stride, heads, rotary, cos, sin, rows, cache.ref,
+    address, need = (Kv8Workspace(cache.device) if workspace is None else workspace).of(plan.max_tokens, heads, cache.kv_heads, dim)
+    check(load().leafq_kv8_attention(_raw_stream(index), q.data_ptr(), stride, heads, rotary, cos, sin, rows, cache.ref,
                                      plan.ref, scale, out.data_ptr(), address, need, flags))
     return out
