@@ -7,6 +7,7 @@
 //   out = sum_j exp(x_j - m) vs cv_j / sum_j exp(x_j - m),  m = max x
 // in one pass over the keys: when the maximum grows from m to m', the sums so
 // far are multiplied by exp(m - m').
+#include <algorithm>
 #include <type_traits>
 
 #include "kv8_attention.cuh"
@@ -646,11 +647,11 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
     }
 }
 
-// Row blocks of 8, key ranges per row block, and the workspace: the arrival
-// counters of every (range, row block), then two partial results for each.
+// Row blocks of 8, key ranges per row block, and what the workspace holds behind
+// the counters (one for every range and row block): two partial results for each.
 struct SplitShape {
     int64_t row_blocks, ranges;
-    size_t counter_bytes, part_bytes;
+    size_t part_bytes;
 };
 
 template <int D>
@@ -661,7 +662,7 @@ SplitShape split_shape(int64_t max_tokens, int group) {
     // About one wave of blocks in all; from there on one block per row block,
     // whose requests it walks alone.
     f.ranges = (Split<D>::kBlocks + f.row_blocks - 1) / f.row_blocks;
-    f.counter_bytes = (static_cast<size_t>(f.ranges * f.row_blocks) * sizeof(uint32_t) + 255) / 256 * 256;
+    static_assert(2 * Split<D>::kBlocks <= kSplitCounters, "ranges * row_blocks, where there is more than one range");
     f.part_bytes = f.ranges > 1 ? 2 * static_cast<size_t>(f.ranges * f.row_blocks) * Split<D>::kPart * sizeof(float) : 0;
     return f;
 }
@@ -676,20 +677,22 @@ int run_split(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl)
     const int st = allow_smem(reinterpret_cast<const void*>(kv8_attend_split_kernel<D>), Split<D>::kSmem, "leafq_kv8_attention");
     if (st) return st;
     uint32_t* arrivals = static_cast<uint32_t*>(workspace);
-    float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + f.counter_bytes);
+    float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
     return launch(kv8_attend_split_kernel<D>, dim3(static_cast<unsigned>(f.ranges * f.row_blocks)), dim3(Split<D>::kThreads),
                   Split<D>::kSmem, s, pdl, "leafq_kv8_attention", g, parts, arrivals, static_cast<int>(f.ranges),
                   static_cast<int>(f.row_blocks));
 }
 
-// The tile form gives each 128 rows of a request's kv head to one block: it
-// wants a quarter of them at least, and enough of them that walking a long
-// cache in few blocks is made up for.  Per key and SM clock the split form
-// takes about 0.02 cycles a row over the whole GPU, the tile form 36 (heads of
-// up to 64) or 62 whatever the rows of its 296 blocks: even at 1,800 and 3,100
-// rows in all.
-bool takes_tiles(int64_t tokens, int64_t max_tokens, int heads, int group, int dim) {
-    return max_tokens * group >= 32 && tokens * heads >= (dim <= 64 ? 2048 : 3584);
+// The tile form gives 128 rows of a request's kv head to a block, the split form
+// 8: the tile form wants a quarter of them at least, and enough rows in all.
+// Measured with 8 kv heads of 64 (128) and 8,000 cached tokens, split form and
+// tile form, us: 2,048 rows of 8 requests 74 and 84 (172 and 122), 4,096 rows 134
+// and 85 (294 and 122), 8,192 rows 384 and 99 (569 and 157); with 1,000 cached
+// tokens 2,048 rows 16 and 31 (33 and 42), 4,096 rows 35 and 31 (65 and 44).  Over
+// 520 shapes of 256 to 64,000 rows this rule is 1 to 3 % above the better form.
+constexpr int kTileRows = 32;
+bool takes_tiles(int64_t tokens, int64_t max_tokens, int heads, int group) {
+    return max_tokens * group >= kTileRows && tokens * heads >= 3584;
 }
 
 // Calls f(integral constant D) for a supported head size.
@@ -716,7 +719,8 @@ size_t leafq_kv8_attention_workspace_bytes(int64_t max_tokens, int heads, int kv
         return 0;
     return with_dim(dim, [&](auto d) {
         const SplitShape f = split_shape<d()>(max_tokens, heads / kv_heads);
-        return f.counter_bytes + f.part_bytes;
+        const bool tiles = max_tokens * (heads / kv_heads) >= kTileRows;
+        return kCounterBytes + std::max(f.part_bytes, tiles ? kv8_tile_part_bytes(d()) : 0);
     });
 }
 
@@ -761,7 +765,7 @@ int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int head
     while ((1 << g.shift) < cache->page) ++g.shift;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool pdl = (flags & LEAFQ_FLAG_PDL) != 0;
-    if (takes_tiles(step->tokens, step->max_tokens, heads, g.group, cache->dim)) return launch_kv8_tiles(s, g, workspace, pdl);
+    if (takes_tiles(step->tokens, step->max_tokens, heads, g.group)) return launch_kv8_tiles(s, g, workspace, pdl);
     return with_dim(cache->dim, [&](auto d) { return run_split<d()>(s, g, workspace, pdl); });
 }
 

@@ -120,7 +120,15 @@ __device__ __forceinline__ void row_power(uint32_t largest_bits, float& up, floa
     down = __uint_as_float(static_cast<uint32_t>(254 - k) << 23);
 }
 
-// Many query rows of a request (kv8_tile.cu).
+// The workspace: counters that are zero between calls, in places that do not
+// depend on the call's shape, so that calls of all shapes may share it; then the
+// parts' results.
+constexpr int kSplitCounters = 1024, kTileCounters = kSplitCounters, kTileBlocks = 296;
+constexpr size_t kCounterBytes = 8192;
+static_assert((kTileCounters + 4 + 4 * (kTileBlocks / 2)) * 4 <= kCounterBytes, "the items that have parts, four counters each");
+
+// Many query rows of a request (kv8_tile.cu), and what its parts take.
+size_t kv8_tile_part_bytes(int dim);
 int launch_kv8_tiles(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl);
 
 }  // namespace leafq

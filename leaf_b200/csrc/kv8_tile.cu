@@ -37,16 +37,22 @@ namespace {
 // -- and the lo halves of Q go first, while S is small.
 constexpr float kTileLift = 6.0f, kTileHighest = 49152.0f;
 
+// Where there are fewer items than half the blocks, each is cut into parts along
+// the keys, of kPartTiles tiles or more; the last part to end joins them.
+constexpr int kPartTiles = 4, kMostParts = 16;
+
 // What the roles of a block need to know of an item: 128 query rows of one kv
 // head of a request.  tiles < 0: there are no more.
 struct TileItem {
-    int row0, first_row, rows, context, keys, tiles, head, unused;
+    int row0, first_row, rows, context, keys, tiles, head;
+    int tile0, parts, part, place, unused;  // its first key tile; of `parts` parts, whose place in the workspace starts at `place`
     uint8_t power[128];  // of two, that each row was scaled down by (its exponent bits)
 };
 
 // An item as the converting warps take it; rows < 0: there are no more.
 struct NextItem {
-    int row0, first_row, rows, context, keys, request, head, unused;
+    int row0, first_row, rows, context, keys, tiles, head;
+    int tile0, parts, part, place, request;
 };
 
 template <int D>
@@ -75,6 +81,7 @@ struct TileShape {
     static constexpr int kSumBytes = kSumInSmem ? kRows * D * 4 : 0;
     static constexpr size_t kSmem = 2 * kQBytes + (kKStages + kVStages) * kKvBytes + kSumBytes + kInfo * kGroups * 16 +
                                     sizeof(TileItem) + 2 * sizeof(NextItem) + (2 * kKStages + 2 * kVStages + 11) * 8 + 8;
+    static constexpr int kPart = kRows * (D + 2);        // floats of a part's result: O [D / 4][128][4], m [128], l [128]
     static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two blocks share the SM's shared memory");
     static_assert(2 * kKeys + kOutCols <= 256, "two blocks share the SM's 512 TMEM columns");
     static_assert(kSoftmaxRegs + kOtherRegs <= 2 * kLaunchRegs, "the split of what the launch gives each scheduler");
@@ -166,9 +173,13 @@ __device__ __forceinline__ void store_local(uint32_t at, float4 v) {
     asm volatile("st.local.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
-template <int D>
+// kParts: some items are cut into parts (the code that joins them is left out of
+// the other kernel, whose loops it would push out of the instruction cache:
+// 64 prompts of 512 tokens 368 us without it, 379 us with it).
+template <int D, bool kParts>
 __global__ void __launch_bounds__(TileShape<D>::kThreads, 2)
-kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t* taken, int row_tiles) {
+kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t* taken, uint32_t* arrivals, float* parts,
+                       int row_tiles, int splits) {
     using C = TileShape<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* q_hi = smem;
@@ -257,7 +268,8 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             ok = ok && __all_sync(~0u, tile_wait(watch, q_full, it & 1));
             if (!ok) break;
             const int tiles = item->tiles, first_row = item->first_row, rows = item->rows, row0 = item->row0, context = item->context,
-                      keys = item->keys, head = item->head;
+                      keys = item->keys, head = item->head, tile0 = kParts ? item->tile0 : 0;
+            const int count = kParts ? item->parts : 1, part_index = kParts ? item->part : 0, place = kParts ? item->place : 0;
             const float factor = __uint_as_float(static_cast<uint32_t>(item->power[tid]) << 23) * g.scale * kLog2e;
             __syncwarp();
             if (lane == 0) mbar_arrive(q_empty);
@@ -275,7 +287,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 if (!ok) break;
                 tcgen05_fence_after();
                 const float4* scales = info + (n % C::kInfo) * C::kGroups;
-                const int visible = limit - j * C::kKeys;  // columns of this tile that the row sees
+                const int visible = limit - (tile0 + j) * C::kKeys;  // columns of this tile that the row sees
                 const bool whole = __all_sync(~0u, visible >= C::kKeys);
                 // 32 scores at a time, by rolled loops: the roles' loops have to stay in the
                 // instruction cache side by side (unrolled, with all scores in registers,
@@ -428,10 +440,11 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             if (!ok) break;
             tcgen05_fence_after();
             // The rows' output: O (and the rounded sum) over L, zeros for a row that
-            // sees no key.
-            const bool summed = tiles > C::kSpan;
+            // sees no key.  A part of an item leaves O, m and l instead.
+            const bool summed = tiles > C::kSpan, whole_item = !kParts || count == 1;
             const float old = !summed || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m);
-            const float inverse = l == 0.0f ? 0.0f : __frcp_rn(l);
+            const float inverse = !whole_item ? 1.0f : l == 0.0f ? 0.0f : __frcp_rn(l);
+            float* own = parts + (int64_t)(place + part_index) * C::kPart;
 #pragma unroll 1
             for (int c = 0; c < D / 4; c += 8) {
                 uint32_t x[32];
@@ -447,11 +460,56 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     }
                     y = l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
                                   : make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
-                    if (C::kSumInSmem) put_sum(c + e, y);
+                    if (kParts && !whole_item) reinterpret_cast<float4*>(own)[(c + e) * C::kRows + tid] = y;
+                    else if (C::kSumInSmem) put_sum(c + e, y);
                     else if (r < rows) *reinterpret_cast<float4*>(out + 4 * (c + e)) = y;
                 }
             }
-            if constexpr (C::kSumInSmem) {
+            bool there = whole_item;
+            if (kParts && !whole_item) {
+                // The last of the parts' warps to arrive joins its rows' parts, in order.
+                own[C::kRows * D + tid] = m;
+                own[C::kRows * (D + 1) + tid] = l;
+                __syncwarp();
+                uint32_t before = 0;
+                if (lane == 0) {
+                    __threadfence();
+                    uint32_t* arrived = arrivals + 4 * (place / splits) + warp;
+                    before = atomicAdd(arrived, 1u);
+                    if (before == static_cast<uint32_t>(count - 1)) *arrived = 0;
+                    __threadfence();
+                }
+                there = __shfl_sync(~0u, before, 0) == static_cast<uint32_t>(count - 1);
+                if (there) {
+                    const float* first = parts + (int64_t)place * C::kPart;
+                    float top = -INFINITY, total = 0.0f;
+#pragma unroll 1
+                    for (int i = 0; i < count; ++i) top = fmaxf(top, __ldcg(first + i * C::kPart + C::kRows * D + tid));
+#pragma unroll 1
+                    for (int i = 0; i < count; ++i) {
+                        const float* from = first + i * C::kPart;
+                        const float their = __ldcg(from + C::kRows * D + tid), part_l = __ldcg(from + C::kRows * (D + 1) + tid);
+                        // (An l that is no number comes through, whatever its m.)
+                        const float weight = their == -INFINITY ? (part_l == 0.0f ? 0.0f : 1.0f) : ex2(their - top);
+                        total = fmaf(weight, part_l, total);
+#pragma unroll 4
+                        for (int c = 0; c < D / 4; ++c) {
+                            const float4 v = __ldcg(reinterpret_cast<const float4*>(from) + c * C::kRows + tid);
+                            const float4 z = i == 0 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : get_sum(c);
+                            put_sum(c, make_float4(fmaf(weight, v.x, z.x), fmaf(weight, v.y, z.y), fmaf(weight, v.z, z.z), fmaf(weight, v.w, z.w)));
+                        }
+                    }
+                    const float over = total == 0.0f ? 0.0f : __frcp_rn(total);
+#pragma unroll 4
+                    for (int c = 0; c < D / 4; ++c) {
+                        float4 y = get_sum(c);
+                        y = total == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(y.x * over, y.y * over, y.z * over, y.w * over);
+                        if (C::kSumInSmem) put_sum(c, y);
+                        else if (r < rows) *reinterpret_cast<float4*>(out + 4 * c) = y;
+                    }
+                }
+            }
+            if (C::kSumInSmem && there) {
                 // Through the warp's sums: whole rows per store.
                 __syncwarp();
                 constexpr int kRowLanes = D / 4;  // 8 or 16 lanes a row
@@ -478,11 +536,10 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         // on: enough of them.  A block's first item is its own number; warp 4 takes
         // the next ones from a counter that all blocks share, while the last tile of
         // the item before is on its way, and tells the other three.
-        const uint32_t total = static_cast<uint32_t>(row_tiles) * g.cache.kv_heads;
+        const uint32_t total = static_cast<uint32_t>(row_tiles) * g.cache.kv_heads * splits;
         bool first_take = true;
         const auto advance = [&](int it) {
             NextItem next = {};
-            next.rows = -1;
 #pragma unroll 1
             while (true) {
                 uint32_t id = blockIdx.x;
@@ -491,10 +548,15 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     id = __shfl_sync(~0u, id, 0);
                 }
                 first_take = false;
+                next.rows = -1;
                 if (id >= total) break;
-                const uint32_t group_of = id / static_cast<uint32_t>(g.cache.kv_heads);
+                const uint32_t whole = kParts ? id / static_cast<uint32_t>(splits) : id, group_of = whole / static_cast<uint32_t>(g.cache.kv_heads);
+                if (kParts) {
+                    next.part = static_cast<int>(id - whole * splits);
+                    next.place = static_cast<int>(whole * splits);
+                }
                 const int index = row_tiles - 1 - static_cast<int>(group_of);
-                next.head = static_cast<int>(id - group_of * g.cache.kv_heads);
+                next.head = static_cast<int>(whole - group_of * g.cache.kv_heads);
                 int s = 0;
 #pragma unroll 1
                 for (int left = g.step.requests; left > 1;) {
@@ -516,6 +578,15 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 const int held = min(g.step.page_offsets[s + 1] - g.step.page_offsets[s], static_cast<int>(g.step.max_pages));
                 const int seen = next.context + token_of(next.first_row + next.rows - 1) + 1;  // by the last row
                 next.keys = max(0, min(min(held << g.shift, g.step.lengths[s]), seen));
+                // (Without keys, a tile that is all hidden.)
+                const int tiles = max(1, (next.keys + C::kKeys - 1) / C::kKeys);
+                next.tiles = tiles;
+                if (kParts) {
+                    next.parts = min(splits, max(1, tiles / kPartTiles));
+                    if (next.part >= next.parts) continue;
+                    next.tile0 = tiles * next.part / next.parts;
+                    next.tiles = tiles * (next.part + 1) / next.parts - next.tile0;
+                }
                 break;
             }
             if (lane == 0) {
@@ -656,7 +727,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             }
             const bool more = it >= 0 && now.rows >= 0;
             const int keys = now.keys;
-            const int tiles = more ? max(1, (keys + C::kKeys - 1) / C::kKeys) : it < 0 ? 0 : -1;  // without keys, a tile that is all hidden
+            const int tiles = more ? now.tiles : it < 0 ? 0 : -1;
             if (it >= 0 && tid == 128) {
                 item->row0 = now.row0;
                 item->first_row = now.first_row;
@@ -665,6 +736,12 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 item->keys = keys;
                 item->tiles = tiles;
                 item->head = now.head;
+                if (kParts) {
+                    item->tile0 = now.tile0;
+                    item->parts = now.parts;
+                    item->part = now.part;
+                    item->place = now.place;
+                }
             }
             if (it >= 0 && !more) {
                 __syncwarp();
@@ -679,7 +756,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             uint4 w[C::kPieces];
             float ks = 0.0f, vs = -1.0f;            // the group's scales; -1: not there
             const auto page_of = [&](int j, int row) {  // of key row `row` of tile j; past the keys: some page
-                const int key = min(j * C::kKeys + row, keys - 1);
+                const int key = min(((kParts ? now.tile0 : 0) + j) * C::kKeys + row, keys - 1);
                 return keys > 0 ? load_now(table + (key >> g.shift)) : -1;
             };
             const auto ask_pages = [&](int j) {
@@ -690,14 +767,14 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             const auto fetch = [&](int j) {  // tile j, whose pages are there; zeros where there is no key
 #pragma unroll
                 for (int i = 0; i < C::kPieces; ++i) {
-                    const int key = j * C::kKeys + row_of(i);
+                    const int key = ((kParts ? now.tile0 : 0) + j) * C::kKeys + row_of(i);
                     w[i] = make_uint4(0u, 0u, 0u, 0u);
                     if (key < keys && static_cast<uint32_t>(ids[i]) < static_cast<uint32_t>(g.cache.pages))
                         w[i] = load_now(codes + (ids[i] * page_pieces + (head_pieces + (key & (page - 1)) * (D / 16) + piece_of(i))));
                 }
                 ks = 0.0f;
                 vs = -1.0f;
-                if (is_k && ct < C::kGroups && j * C::kKeys + 16 * ct < keys) {
+                if (is_k && ct < C::kGroups && ((kParts ? now.tile0 : 0) + j) * C::kKeys + 16 * ct < keys) {
                     if (static_cast<uint32_t>(group_id) < static_cast<uint32_t>(g.cache.pages)) {
                         const int64_t from = (int64_t)group_id * g.cache.kv_heads + now.head;
                         ks = load_now(g.cache.k_scales + from);
@@ -841,11 +918,11 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
     }
 }
 
+template <int D, bool kParts>
+int start_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, int64_t row_tiles, int splits, bool pdl);
+
 template <int D>
 int run_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) {
-    DeviceWatch watch;
-    int st = device_watch(&watch);
-    if (st) return st;
     const int64_t row_tiles = (g.step.tokens * g.group >> 7) + g.step.requests;
     if (g.cache.pages > UINT32_MAX / (((int64_t)g.cache.kv_heads << g.shift) * (D / 16))) {
         set_error("leafq_kv8_attention: code pools of 64 GiB and more are not supported for prompts");
@@ -855,7 +932,17 @@ int run_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) 
         set_error("leafq_kv8_attention: too many rows");
         return LEAFQ_ERR_INVALID;
     }
-    const void* kernel = reinterpret_cast<const void*>(kv8_attend_tile_kernel<D>);
+    const int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostParts, kTileBlocks / (row_tiles * g.cache.kv_heads))));
+    return splits > 1 ? start_tile<D, true>(s, g, workspace, row_tiles, splits, pdl)
+                      : start_tile<D, false>(s, g, workspace, row_tiles, 1, pdl);
+}
+
+template <int D, bool kParts>
+int start_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, int64_t row_tiles, int splits, bool pdl) {
+    DeviceWatch watch;
+    int st = device_watch(&watch);
+    if (st) return st;
+    const void* kernel = reinterpret_cast<const void*>(kv8_attend_tile_kernel<D, kParts>);
     static const int registers = [kernel] {
         cudaFuncAttributes a;
         return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0;
@@ -867,13 +954,17 @@ int run_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) 
     }
     st = allow_smem(kernel, TileShape<D>::kSmem, "leafq_kv8_attention");
     if (st) return st;
-    const int64_t blocks = std::min<int64_t>(row_tiles * g.cache.kv_heads, 2 * (int64_t)sm_count());
-    return launch(kv8_attend_tile_kernel<D>, dim3(static_cast<unsigned>(blocks)),
+    const int64_t blocks = std::min<int64_t>(row_tiles * g.cache.kv_heads * splits, 2 * (int64_t)sm_count());
+    uint32_t* counters = static_cast<uint32_t*>(workspace) + kTileCounters;
+    return launch(kv8_attend_tile_kernel<D, kParts>, dim3(static_cast<unsigned>(blocks)),
                   dim3(TileShape<D>::kThreads), TileShape<D>::kSmem, s, pdl, "leafq_kv8_attention", g, watch,
-                  static_cast<uint32_t*>(workspace), static_cast<int>(row_tiles));
+                  counters, counters + 4, reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes),
+                  static_cast<int>(row_tiles), splits);
 }
 
 }  // namespace
+
+size_t kv8_tile_part_bytes(int dim) { return sizeof(float) * kTileBlocks * 128 * (dim + 2); }
 
 int launch_kv8_tiles(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) {
     switch (g.cache.dim) {

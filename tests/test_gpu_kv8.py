@@ -600,3 +600,45 @@ def test_step_in_a_graph(cuda_device):
             got = out[s].reshape(kv, group, dim)[h].cpu().numpy()
             assert np.linalg.norm(got - expect[0]) <= 1e-5 * np.linalg.norm(expect[0])
     assert _status_ok()
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("context,new", [([3000], [256]), ([0, 2500, 90, 700], [3, 150, 64, 40]), ([1200, 5000], [31, 225])])
+def test_attention_few_row_tiles_over_long_caches(cuda_device, dim, context, new):
+    # Fewer row tiles than blocks: each is cut along its keys and its parts are joined.
+    rng = np.random.default_rng(dim + len(new))
+    batch = _Batch(rng, context, new, 16, 2, 8, dim, rotary=dim)
+    first = batch.run()
+    batch.check(first)
+    for _ in range(3):
+        assert torch.equal(batch.run(), first)
+    assert _status_ok()
+
+
+def test_attention_parts_with_hidden_rows_and_values_that_are_no_numbers(cuda_device):
+    rng = np.random.default_rng(77)
+    batch = _Batch(rng, [4000, 900], [130, 126], 64, 2, 8, 64, lengths=[2100, 0])
+    batch.check()
+    batch.q[:] *= 40.0  # one key has nearly all the weight, in some part
+    batch.check()
+    q = batch.q.copy()
+    q[5, 3] = np.nan
+    got = batch.run(torch.from_numpy(q).cuda())
+    assert torch.isnan(got[5, :64]).all() and not torch.isnan(got[6]).any() and not torch.isnan(got[5, 64:]).any()
+    assert _status_ok()
+
+
+def test_attention_shapes_share_a_workspace(cuda_device):
+    # Decode, draft, prompt and few-head shapes in turn: none may find another's leavings.
+    rng = np.random.default_rng(78)
+    batches = [_Batch(rng, [9000], [1], 64, 1, 8, 64), _Batch(rng, [3000], [200], 64, 1, 8, 64),
+               _Batch(rng, [5000, 20], [1, 1], 32, 4, 2, 128), _Batch(rng, [3000], [256], 64, 2, 8, 128),
+               _Batch(rng, [2000, 700], [40, 290], 16, 1, 8, 32), _Batch(rng, [6000], [4], 16, 3, 1, 96)]
+    alone = [b.run() for b in batches]
+    for b, y in zip(batches, alone):
+        b.check(y)
+    workspace = lq.Kv8Workspace("cuda")
+    for order in ((0, 1, 2, 3, 4, 5), (5, 3, 1, 4, 0, 2), (1, 1, 0, 4, 4, 3)):
+        for i in order:
+            assert torch.equal(batches[i].run(workspace=workspace), alone[i])
+    assert _status_ok()
