@@ -424,7 +424,9 @@ int leafq_advance_positions(void* stream, int32_t* positions, int sequences, int
  * tokens need and every new token its slot, then per layer leafq_kv8_append
  * writes the new keys and values and leafq_kv8_attention attends.  All three
  * read the lengths on the device, so one CUDA graph serves every step whose
- * bounds (requests, tokens, max_tokens) are the same.  The reference keeps
+ * bounds (requests, tokens, max_tokens) are the same.  LEAFQ_FLAG_PDL is
+ * valid with all three whatever ran before: they read nothing until it has
+ * finished.  The reference keeps
  * an fp32 cache per sequence instead (kv_cache.cpp); these results are not
  * bit-identical to it. */
 typedef struct leafq_kv8_cache {
@@ -481,8 +483,9 @@ int leafq_kv8_plan(void* stream, const int32_t* context, const int32_t* new_toke
  *   new codes = rint(x * (1 / scale))
  * (a NaN row makes the scale NaN).  The tokens of one page must be
  * consecutive rows with consecutive slots, as leafq_kv8_plan lays them out.
- * A slot outside the pool or a position outside the tables is skipped and
- * reported by leafq_device_status.  positions may be NULL without tables. */
+ * A slot outside the pool is skipped and a position outside the tables turns
+ * by position 0; leafq_device_status reports both.  positions may be NULL
+ * without tables. */
 int leafq_kv8_append(void* stream, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
                      int64_t tokens, const int32_t* positions, const int32_t* slots, int rotary_dim,
                      const float* cos_table, const float* sin_table, int64_t table_rows,
@@ -490,8 +493,9 @@ int leafq_kv8_append(void* stream, const float* k, int64_t k_stride, const float
 
 /* Bytes of workspace leafq_kv8_attention needs for this geometry, 0 when it
  * needs none.  The workspace must be zeroed once before its first use; every
- * call leaves the words that need it zero again.  Calls that overlap on the
- * GPU need workspaces of their own. */
+ * call leaves the words that need it zero again, in the same places for every
+ * geometry, so that calls of all geometries may share one of the largest's
+ * size.  Calls that overlap on the GPU need workspaces of their own. */
 size_t leafq_kv8_attention_workspace_bytes(int64_t max_tokens, int heads, int kv_heads, int dim);
 
 /* Causal grouped-query attention of the step's new tokens over the cache.
@@ -501,9 +505,12 @@ size_t leafq_kv8_attention_workspace_bytes(int64_t max_tokens, int heads, int kv
  *   out = sum_j softmax_j(scale * q . key_j) value_j,
  * fp32 throughout (sums, softmax statistics, output), a row that sees no key
  * gives zeros.  heads is a multiple of the cache's kv_heads; out [tokens]
- * [heads * dim]; rows past the last new token are not written.  A table entry
- * outside the pool or a position outside the tables hides the key or empties
- * the row, and leafq_device_status reports it. */
+ * [heads * dim]; rows past the last new token are not written, a request's
+ * rows past max_tokens may be left out.  The cache's scales must not be negative.  A table
+ * entry outside the pool hides its keys and a position outside the tables
+ * empties its row; leafq_device_status reports both.  Equal calls give equal
+ * bits.  With many rows (prompts) a pool's codes have to stay below 64 GiB
+ * each and tokens * heads / kv_heads within int32. */
 int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int heads, int rotary_dim,
                         const float* cos_table, const float* sin_table, int64_t table_rows,
                         const leafq_kv8_cache* cache, const leafq_kv8_step* step, float scale, float* out,

@@ -33,8 +33,9 @@ __device__ __forceinline__ void wait_async_copies_but() {
 
 // ---------------------------------------------------------- split form
 // Few query rows, many keys (decode).  A block owns 8 query rows of one kv
-// head (rows r = token * group + head-in-group of a request) and a range of the keys; its warps take chunks of 32 keys in
-// turn, each warp with its own running maximum, sum and output.
+// head (rows r = token * group + head-in-group of a request) and a range of the
+// keys; its warps take chunks of 32 keys in turn, each warp with its own
+// reference, sum and output.
 //
 // Tensor cores: m16n8k16, fp16 in, fp32 sums.  The codes are exact in fp16.
 // An fp32 operand is split into hi + lo, 11 significand bits each, so a
@@ -47,13 +48,25 @@ __device__ __forceinline__ void wait_async_copies_but() {
 //   the bytes of two keys by byte permutes.  A step's columns 2t, 2t+1, 2t+8,
 //   2t+9 are keys t, 4+t, 8+t, 12+t, which makes the V reads conflict-free.
 // A V scale vs = f 2^e goes half into the exponent, half into the weight:
-// u_j = 2^(x_j + e - M) with M the running maximum of x_j + e; O sums f u_j cv_j
-// and L sums u_j 2^-e, so O / L is the softmax average whatever the scales'
-// range, and neither half rounds.
+// u_j = 2^(x_j + e - M) with M a reference near the maximum of x_j + e; O sums
+// f u_j cv_j and L sums u_j 2^-e, so O / L is the softmax average whatever the
+// scales' range, and neither half rounds.
 //
-// Bound: HBM (the codes are read once: cp.async into a ring per warp, 16-byte
-// pieces, rows swizzled so that both fragment reads touch every bank once);
-// behind it the conversions, 5 and 7 issue slots per four codes of K and V.
+// The codes are read once, by 16-byte asynchronous copies into a ring per warp,
+// laid out so that both fragment reads touch every bank once (with two- and
+// four-way conflicts long caches took 115 us instead of 108).  A call's first
+// microseconds are round trips, so what does not depend on one another is asked
+// for at once: the requests' pages; then a request's lengths and page numbers;
+// then its rows and its first chunks (one request 6.0 -> 5.4 us).
+//
+// Bound: for long caches HBM and the conversions (5 and 7 issue slots per four
+// codes of K and V) about alike.  6 requests of 15,000 to 91,000 tokens, 8 heads
+// of 128, 468 MB: 104 us (4.5 TB/s); the copies alone take 98 us, the arithmetic
+// alone 90 us.  For short ones the round trips: 64 requests of 521 to 765 tokens,
+// 4 heads of 64, 21.6 MB, take 13.6 us, of which 6 us pass before the first
+// chunk is there, 4 us in the key loop and 1 us in joining the warps; one request
+// of 200 tokens takes 5.5 us.  Four warps a block at 64-wide heads took 19.2 us
+// instead of 13.5, three blocks of eight warps (80 registers, spilling) 21.8.
 template <int D>
 struct Split {
     static constexpr int kWarps = D <= 64 ? 8 : 4;

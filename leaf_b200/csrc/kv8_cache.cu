@@ -19,6 +19,10 @@ namespace {
 // chunk's tokens.  Four consecutive tokens per thread: one search of the
 // chunk's prefix, one page lookup per page, 16-byte stores.  A new page's
 // table entry is written by the thread that has the page's first token.
+//
+// Bound: latency, of the launch, the lengths' load, two barriers per chunk and
+// the page lookup behind them.  64 requests of one token each take 4.8 us,
+// 2,000 requests with 288,042 new tokens 14.7 us (2.5 MB, 170 GB/s).
 struct PlanArgs {
     const int32_t* context;
     const int32_t* fresh;
@@ -200,6 +204,13 @@ __global__ void __launch_bounds__(kPlanMaxThreads) kv8_plan_kernel(const PlanArg
 // values a .. a+3 and b .. b+3 with b = a + rotary / 2 (behind the rotated
 // part, pairs of the remaining half).  The absmax is a maximum over bit
 // patterns, which is exact, order-free and lets a NaN through.
+//
+// Bound: HBM, 5 bytes a value (4 read, 1 written), once the calls are large; the
+// chain slots -> rows -> absmax -> codes is one round trip after another and is
+// hidden only by the other blocks of the SM.  4 heads of 64: a decode step of 64
+// rows 2.7 us; 64 prompts of 512 tokens, 84 MB, 25.9 us (3.2 TB/s, half of the
+// copy rate).  8 heads of 128, 37 requests with 4,737 new tokens in pages of 16,
+// 48.5 MB, 17.7 us.
 constexpr int kAppendItems = 4;
 
 struct AppendArgs {

@@ -11,16 +11,14 @@
 namespace leafq {
 namespace {
 
-// A block owns 128 query
-// rows of one kv head of a request (rows r = token * group + head-in-group),
-// walks the keys in tiles, and two blocks share an SM, so that one's MMAs run
-// under the other's softmax.  Roles:
-//   warps 0-3  softmax: one row per thread (its TMEM lane), a tile's scores in
-//              registers
+// An item is 128 query rows of one kv head of a request (rows r = token * group +
+// head-in-group) over its keys in tiles.  Two persistent blocks share an SM, so
+// that one's MMAs run under the other's softmax.  Roles:
+//   warps 0-3  softmax: one row per thread (its TMEM lane), 32 scores at a time
 //   warps 4-7  the items and their query rows; codes to fp16 (two warps K, two
 //              V): 16-byte global loads a tile ahead, byte permutes,
 //              128-byte-swizzled shared memory
-//   warp 8     MMA issue (kind::f16, fp32 accumulators in TMEM)
+//   warp 8     MMA issue (tcgen05.mma kind::f16, fp32 accumulators in TMEM)
 // The softmax warps take registers that the others leave (setmaxnreg).  S has
 // two buffers: the next tile's scores are computed under this tile's softmax.
 // The arithmetic is the split form's: codes exact in fp16, fp32 operands as
@@ -33,8 +31,17 @@ namespace {
 // to kTileHighest, so that none passes 65504, fp16's largest, before the reference
 // is raised and O rescaled.  The MMA's additions truncate,
 // which adds up over long sums (8192 keys: 5.5e-6 of the result), so every
-// kSpan keys O is added to a rounded sum (in local memory) and starts anew
-// -- and the lo halves of Q go first, while S is small.
+// kSpan tiles O is added to a rounded sum (in shared memory, for heads of 96 and
+// 128 in local memory) and starts anew -- and the lo halves of Q go first, while
+// S is small.
+//
+// Bound: issue slots, of which 58 % are used (the tensor pipe is busy 21 % of the
+// time): about a third go to the softmax (5 to 6 instructions a score), a fifth
+// to rotating and splitting query rows, a sixth to the codes' conversion; the
+// rest waits on hand-offs between the roles.  4 heads of 64, 8 queries a key: 64
+// prompts of 512 tokens 368 us (187 TFLOP/s, twice that in the MMAs, since fp32
+// operands are two halves); one of 8,192 tokens 614 us (447 TFLOP/s).  5 chunks
+// of 51 to 1,500 tokens, 8 heads of 128, 3 queries a key, 85 us (247 TFLOP/s).
 constexpr float kTileLift = 6.0f, kTileHighest = 49152.0f;
 
 // Where there are fewer items than half the blocks, each is cut into parts along
