@@ -13,8 +13,8 @@ namespace {
 // ------------------------------------------------------------------- plan
 // Two prefix sums over the requests (new tokens, new pages) decide everything:
 // a request's first row, the free pages it takes, whether the pool reaches.
-// Every block scans all requests itself, a chunk of blockDim.x at a time with
-// a running carry (8 bytes per request from L2), so that no block waits for
+// Every block scans all requests itself, a chunk of blockDim.x (two a thread,
+// where there are more requests) at a time with a running carry (8 bytes per request from L2), so that no block waits for
 // another; block 0 writes the per-request outputs and the blocks share the
 // chunk's tokens.  Four consecutive tokens per thread: one search of the
 // chunk's prefix, one page lookup per page, 16-byte stores.  A new page's
@@ -22,7 +22,8 @@ namespace {
 //
 // Bound: latency, of the launch, the lengths' load, two barriers per chunk and
 // the page lookup behind them.  64 requests of one token each take 4.8 us,
-// 2,000 requests with 288,042 new tokens 14.7 us (2.5 MB, 170 GB/s).
+// 2,000 requests with 288,042 new tokens 8.7 us (2.5 MB, 287 GB/s; one request a
+// thread, in two chunks, 14.7).
 struct PlanArgs {
     const int32_t* context;
     const int32_t* fresh;
@@ -77,60 +78,100 @@ __device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t& tot
     b += __shfl_sync(~0u, pb - own_b, warp);
 }
 
+// kPer: consecutive requests of a chunk per thread.
+template <int kPer>
 __global__ void __launch_bounds__(kPlanMaxThreads) kv8_plan_kernel(const PlanArgs g) {
     __shared__ int64_t part[32][2];
-    __shared__ int64_t first_s[kPlanMaxThreads + 1];  // first token of each request of the chunk
-    __shared__ int64_t source_s[kPlanMaxThreads];     // free_pages index of table column 0 (if it were new); LLONG_MIN: refused
-    __shared__ int32_t context_s[kPlanMaxThreads];
-    __shared__ long long reached_s;                   // pages granted so far
+    __shared__ int64_t first_s[kPlanMaxThreads * kPer + 1];  // first token of each request of the chunk
+    __shared__ int64_t source_s[kPlanMaxThreads * kPer];     // free_pages index of table column 0 (if it were new); LLONG_MIN: refused
+    __shared__ int32_t context_s[kPlanMaxThreads * kPer];
+    __shared__ long long reached_s;                          // pages granted so far
     grid_dependency_wait();
     grid_launch_dependents();
-    const int tid = threadIdx.x, threads = blockDim.x;
+    const int tid = threadIdx.x, threads = blockDim.x, chunk = threads * kPer;
     const int64_t page = int64_t{1} << g.shift;
     const int64_t taken = *g.taken;
     const bool writer = blockIdx.x == 0;
     if (tid == 0) reached_s = 0;
     int64_t token_base = 0, need_base = 0, page_base = 0;
-    int32_t next_c = tid < g.requests ? g.context[tid] : 0, next_n = tid < g.requests ? g.fresh[tid] : 0;
-    for (int base = 0; base < g.requests; base += threads) {
-        const int r = base + tid;
-        const bool live = r < g.requests;
-        int64_t c = next_c, n = next_n;
-        next_c = r + threads < g.requests ? g.context[r + threads] : 0;
-        next_n = r + threads < g.requests ? g.fresh[r + threads] : 0;
-        if (c < 0 || n < 0) {
-            if (writer) record_device_error(kSiteKv8Range);
-            c = max64(c, 0);
-            n = 0;
+    int32_t next_c[kPer], next_n[kPer];
+    const auto ask = [&](int base) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int r = base + tid * kPer + i;
+            next_c[i] = r < g.requests ? g.context[r] : 0;
+            next_n[i] = r < g.requests ? g.fresh[r] : 0;
         }
-        const int64_t before = (c + page - 1) >> g.shift, after = (c + n + page - 1) >> g.shift;
-        const bool fits = after <= g.max_pages;
-        const int64_t need = fits ? after - before : 0;
-        int64_t tn = n, tp = need, chunk_tokens, chunk_pages;
+    };
+    ask(0);
+    for (int base = 0; base < g.requests; base += chunk) {
+        int64_t c[kPer], n[kPer], before[kPer], need[kPer];
+        bool fits[kPer];
+        int64_t tn = 0, tp = 0, chunk_tokens, chunk_pages;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            c[i] = next_c[i];
+            n[i] = next_n[i];
+            if (c[i] < 0 || n[i] < 0) {
+                if (writer) record_device_error(kSiteKv8Range);
+                c[i] = max64(c[i], 0);
+                n[i] = 0;
+            }
+            before[i] = (c[i] + page - 1) >> g.shift;
+            const int64_t after = (c[i] + n[i] + page - 1) >> g.shift;
+            fits[i] = after <= g.max_pages;
+            need[i] = fits[i] ? after - before[i] : 0;
+            tn += n[i];
+            tp += need[i];
+        }
+        ask(base + chunk);
+        const int64_t own_tn = tn, own_tp = tp;
         block_scan2(tn, tp, chunk_tokens, chunk_pages, part);
-        const int64_t upto = need_base + tp;  // pages wanted by requests 0 .. r
-        const bool granted = fits && (need == 0 || (taken >= 0 && taken + upto <= g.free_count));
-        const int64_t length = granted ? c + n : c;
-        first_s[tid] = token_base + tn - n;
-        if (tid == threads - 1) first_s[threads] = token_base + tn;
-        source_s[tid] = granted ? taken + upto - need - before : LLONG_MIN;
-        context_s[tid] = static_cast<int32_t>(c);
+        int64_t first = token_base + tn - own_tn, upto = need_base + tp - own_tp;  // pages wanted by the requests before
+        int64_t length[kPer], held = 0, reached = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            upto += need[i];
+            const bool granted = fits[i] && (need[i] == 0 || (taken >= 0 && taken + upto <= g.free_count));
+            length[i] = granted ? c[i] + n[i] : c[i];
+            const int at = tid * kPer + i;
+            first_s[at] = first;
+            source_s[at] = granted ? taken + upto - need[i] - before[i] : LLONG_MIN;
+            context_s[at] = static_cast<int32_t>(c[i]);
+            first += n[i];
+            if (granted && need[i] > 0) reached = upto;
+        }
+        if (tid == threads - 1) first_s[chunk] = first;
         if (writer) {
             // Pages held are bounded by the table's row (a context past it is the caller's error).
-            int64_t held = live ? min64((length + page - 1) >> g.shift, g.max_pages) : 0, none = 0, chunk_held, unused;
-            block_scan2(held, none, chunk_held, unused, part);
-            if (live) {
-                g.lengths[r] = static_cast<int32_t>(length);
-                g.token_offsets[r + 1] = static_cast<int32_t>(min64(token_base + tn, g.tokens));
-                g.page_offsets[r + 1] = static_cast<int32_t>(min64(page_base + held, INT_MAX));
-                if (granted && need > 0) atomicMax(&reached_s, static_cast<long long>(upto));
+            int64_t pages[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                pages[i] = base + tid * kPer + i < g.requests ? min64((length[i] + page - 1) >> g.shift, g.max_pages) : 0;
+                held += pages[i];
             }
+            const int64_t own_held = held;
+            int64_t none = 0, chunk_held, unused, end = token_base + tn - own_tn;
+            block_scan2(held, none, chunk_held, unused, part);
+            held += page_base - own_held;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int r = base + tid * kPer + i;
+                end += n[i];
+                held += pages[i];
+                if (r < g.requests) {
+                    g.lengths[r] = static_cast<int32_t>(length[i]);
+                    g.token_offsets[r + 1] = static_cast<int32_t>(min64(end, g.tokens));
+                    g.page_offsets[r + 1] = static_cast<int32_t>(min64(held, INT_MAX));
+                }
+            }
+            if (reached > 0) atomicMax(&reached_s, static_cast<long long>(reached));
             page_base += chunk_held;
         }
         __syncthreads();
         // Tokens [t0, t1) of the chunk, in aligned groups of four.
         const int64_t t0 = token_base, t1 = min64(token_base + chunk_tokens, g.tokens);
-        const int count = min(threads, g.requests - base);
+        const int count = min(chunk, g.requests - base);
         for (int64_t u = t0 / 4 + (int64_t)blockIdx.x * threads + tid; u * 4 < t1; u += (int64_t)gridDim.x * threads) {
             const int64_t begin = max64(u * 4, t0), end = min64(u * 4 + 4, t1);
             int lo = 0, hi = count - 1;  // the last request whose first token is at most begin
@@ -429,7 +470,7 @@ int leafq_kv8_plan(void* stream, const int32_t* context, const int32_t* new_toke
     const int threads = requests <= 256 && tokens <= 1024 ? 256 : kPlanMaxThreads;
     int64_t blocks = (tokens + 4 * threads - 1) / (4 * threads);
     blocks = blocks < 1 ? 1 : blocks > sm_count() ? sm_count() : blocks;
-    return launch(kv8_plan_kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads), 0,
+    return launch(requests > threads ? kv8_plan_kernel<2> : kv8_plan_kernel<1>, dim3(static_cast<unsigned>(blocks)), dim3(threads), 0,
                   static_cast<cudaStream_t>(stream), (flags & LEAFQ_FLAG_PDL) != 0, "leafq_kv8_plan", g);
 }
 
