@@ -31,9 +31,8 @@ namespace {
 // to kTileHighest, so that none passes 65504, fp16's largest, before the reference
 // is raised and O rescaled.  The MMA's additions truncate,
 // which adds up over long sums (8192 keys: 5.5e-6 of the result), so every
-// kSpan tiles O is added to a rounded sum (in shared memory, for heads of 96 and
-// 128 in local memory) and starts anew -- and the lo halves of Q go first, while
-// S is small.
+// kSpan tiles O is added to a rounded sum (in local memory) and starts anew -- and
+// the lo halves of Q go first, while S is small.
 //
 // Bound: issue slots, of which 58 % are used (the tensor pipe is busy 21 % of the
 // time): about a third go to the softmax (5 to 6 instructions a score), a fifth
@@ -49,17 +48,11 @@ constexpr float kTileLift = 6.0f, kTileHighest = 49152.0f;
 constexpr int kPartTiles = 4, kMostParts = 16;
 
 // What the roles of a block need to know of an item: 128 query rows of one kv
-// head of a request.  tiles < 0: there are no more.
+// head of a request, and, where it is cut into parts, which one.  tiles < 0:
+// there are no more.
 struct TileItem {
-    int row0, first_row, rows, context, keys, tiles, head;
-    int tile0, parts, part, place, unused;  // its first key tile; of `parts` parts, whose place in the workspace starts at `place`
-    uint8_t power[128];  // of two, that each row was scaled down by (its exponent bits)
-};
-
-// An item as the converting warps take it; rows < 0: there are no more.
-struct NextItem {
-    int row0, first_row, rows, context, keys, tiles, head;
-    int tile0, parts, part, place, request;
+    int row0, first_row, rows, context, keys, tiles, head, request;
+    int tile0, parts, part, place;  // its first key tile; the parts' place in the workspace
 };
 
 template <int D>
@@ -73,6 +66,8 @@ struct TileShape {
     static constexpr int kInfo = 4;                      // ring of the groups' scales: a tile's are read while those of
                                                          // up to kKStages + 1 later tiles are written
     static constexpr int kQBytes = kBlocks * kRows * 128;
+    static constexpr int kQSlots = D <= 64 ? 2 : 1;      // of query rows: the next item's beside this one's
+    static constexpr int kItems = 3;                     // ring of their descriptions
     static constexpr int kKvBytes = kBlocks * kKeys * 128;
     static constexpr int kSpan = 512 / kKeys;            // tiles between O's additions to the rounded sum
     // Two warps convert K, two V.  Registers of the launch, of the softmax warps, of
@@ -84,10 +79,9 @@ struct TileShape {
     static constexpr int kPieces = kKeys * D / 16 / 64;  // 16-byte pieces of a K (or V) tile per converting thread
     static constexpr int kOutCols = kBlocks * 64;        // O columns (those past D are not read)
     static constexpr uint32_t kTmemCols = 256;
-    static constexpr bool kSumInSmem = D <= 64;          // else in local memory
-    static constexpr int kSumBytes = kSumInSmem ? kRows * D * 4 : 0;
-    static constexpr size_t kSmem = 2 * kQBytes + (kKStages + kVStages) * kKvBytes + kSumBytes + kInfo * kGroups * 16 +
-                                    sizeof(TileItem) + 2 * sizeof(NextItem) + (2 * kKStages + 2 * kVStages + 11) * 8 + 8;
+    static constexpr size_t kSmem = kQSlots * 2 * kQBytes + (kKStages + kVStages) * kKvBytes + kInfo * kGroups * 16 +
+                                    kItems * sizeof(TileItem) + kQSlots * kRows + (2 * kKStages + 2 * kVStages + 2 * kQSlots + kItems + 7) * 8 + 8;
+    static_assert(kQSlots == 1 || kRows * D * 4 <= 2 * kQBytes, "the output goes through the place of the item's rows");
     static constexpr int kPart = kRows * (D + 2);        // floats of a part's result: O [D / 4][128][4], m [128], l [128]
     static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two blocks share the SM's shared memory");
     static_assert(2 * kKeys + kOutCols <= 256, "two blocks share the SM's 512 TMEM columns");
@@ -189,27 +183,25 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                        int row_tiles, int splits) {
     using C = TileShape<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t* q_hi = smem;
-    uint8_t* q_lo = q_hi + C::kQBytes;
-    uint8_t* k_tiles = q_lo + C::kQBytes;
+    uint8_t* q_rows = smem;  // [kQSlots]: hi, lo
+    uint8_t* k_tiles = q_rows + C::kQSlots * 2 * C::kQBytes;
     uint8_t* v_tiles = k_tiles + C::kKStages * C::kKvBytes;
-    float4* sum_s = reinterpret_cast<float4*>(v_tiles + C::kVStages * C::kKvBytes);  // kSumInSmem: [4 warps][D / 4][32]
-    float4* info = sum_s + C::kSumBytes / 16;                                        // [kInfo][kGroups]: ks, log2 vs, 1 / vs
-    TileItem* item = reinterpret_cast<TileItem*>(info + C::kInfo * C::kGroups);
-    NextItem* found = reinterpret_cast<NextItem*>(item + 1);  // by the item's parity
-    uint64_t* k_full = reinterpret_cast<uint64_t*>(found + 2);
+    float4* info = reinterpret_cast<float4*>(v_tiles + C::kVStages * C::kKvBytes);  // [kInfo][kGroups]: ks, log2 vs, 1 / vs
+    TileItem* items = reinterpret_cast<TileItem*>(info + C::kInfo * C::kGroups);
+    uint8_t* power = reinterpret_cast<uint8_t*>(items + C::kItems);  // [kQSlots][128]: of two, that a row was scaled down by (exponent bits)
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(power + C::kQSlots * C::kRows);
     uint64_t* k_empty = k_full + C::kKStages;
     uint64_t* v_full = k_empty + C::kKStages;
     uint64_t* v_empty = v_full + C::kVStages;
-    uint64_t* s_full = v_empty + C::kVStages;  // by S buffer, as p_full
+    uint64_t* s_full = v_empty + C::kVStages;    // by S buffer, as p_full
     uint64_t* p_full = s_full + 2;
-    uint64_t* o_done = p_full + 2;             // PV of a tile has completed
-    uint64_t* q_full = o_done + 1;             // an item's rows and description are there
-    uint64_t* q_empty = q_full + 1;            // its last scores are computed, its description is read
-    uint64_t* item_done = q_empty + 1;         // all its MMAs have completed
+    uint64_t* q_full = p_full + 2;               // by slot: an item's rows are there
+    uint64_t* q_empty = q_full + C::kQSlots;     // its last scores are computed, its description read (its output written)
+    uint64_t* found_full = q_empty + C::kQSlots; // by description: it is there
+    uint64_t* o_done = found_full + C::kItems;   // PV of a tile has completed
+    uint64_t* item_done = o_done + 1;            // all its MMAs have completed
     uint64_t* drained = item_done + 1;
-    uint64_t* found_full = drained + 1;        // by the item's parity
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(found_full + 2);
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kMmaWarp = 8;
     const auto token_of = [&](int row) { return static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(g.group)); };
@@ -232,13 +224,14 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 mbar_init(&s_full[i], 1);
                 mbar_init(&p_full[i], 4);
             }
+            for (int i = 0; i < C::kQSlots; ++i) {
+                mbar_init(&q_full[i], 4);
+                mbar_init(&q_empty[i], 1 + 4);
+            }
+            for (int i = 0; i < C::kItems; ++i) mbar_init(&found_full[i], 1);
             mbar_init(o_done, 1);
-            mbar_init(q_full, 4);
-            mbar_init(q_empty, 1 + 4);
             mbar_init(item_done, 1);
             mbar_init(drained, 1);
-            mbar_init(&found_full[0], 1);
-            mbar_init(&found_full[1], 1);
             fence_barrier_init();
         }
         __syncwarp();
@@ -259,28 +252,26 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         // ------------------------------------------------------- softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-        float4* my_sum = sum_s + warp * (D / 4) * 32;
-        __align__(16) float o_sum[C::kSumInSmem ? 4 : D];  // the rounded sum
+        __align__(16) float o_sum[D];  // the rounded sum
         const uint32_t o_local = local_address(o_sum);
-        // Elements 4 c .. 4 c + 3 of a row; in shared memory the rows are permuted so
-        // that a row's pieces lie in different banks, as a column's do.
-        const auto get_sum = [&](int c) { return C::kSumInSmem ? my_sum[c * 32 + (lane ^ (c & 7))] : load_local(o_local + 16 * c); };
-        const auto put_sum = [&](int c, float4 v) {
-            if (C::kSumInSmem) my_sum[c * 32 + (lane ^ (c & 7))] = v;
-            else store_local(o_local + 16 * c, v);
-        };
+        const auto get_sum = [&](int c) { return load_local(o_local + 16 * c); };  // elements 4 c .. 4 c + 3 of a row
+        const auto put_sum = [&](int c, float4 v) { store_local(o_local + 16 * c, v); };
         int n = 0;
         bool ok = true;
         for (int it = 0;; ++it) {
-            ok = ok && __all_sync(~0u, tile_wait(watch, q_full, it & 1));
+            const int q_slot = it % C::kQSlots;
+            const TileItem* item = items + it % C::kItems;
+            ok = ok && __all_sync(~0u, tile_wait(watch, &q_full[q_slot], it / C::kQSlots & 1));
             if (!ok) break;
             const int tiles = item->tiles, first_row = item->first_row, rows = item->rows, row0 = item->row0, context = item->context,
                       keys = item->keys, head = item->head, tile0 = kParts ? item->tile0 : 0;
             const int count = kParts ? item->parts : 1, part_index = kParts ? item->part : 0, place = kParts ? item->place : 0;
-            const float factor = __uint_as_float(static_cast<uint32_t>(item->power[tid]) << 23) * g.scale * kLog2e;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_empty);
+            const float factor = __uint_as_float(static_cast<uint32_t>(power[q_slot * C::kRows + tid]) << 23) * g.scale * kLog2e;
             if (tiles < 0) break;
+            if (C::kQSlots == 1) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_empty);
+            }
             const int r = tid;
             const int t = token_of(first_row + r), hq = (first_row + r) - t * g.group;
             const int pos = context + t;
@@ -452,6 +443,15 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             const float old = !summed || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m);
             const float inverse = !whole_item ? 1.0f : l == 0.0f ? 0.0f : __frcp_rn(l);
             float* own = parts + (int64_t)(place + part_index) * C::kPart;
+            // Where there is room beside the next item's rows, whole rows are stored, by
+            // way of the place of this item's; permuted so that a row's pieces lie in
+            // different banks, as a column's do.
+            constexpr bool kStaged = C::kQSlots > 1;
+            float4* staged = reinterpret_cast<float4*>(q_rows + q_slot * 2 * C::kQBytes) + warp * (D / 4) * 32;
+            const auto put_out = [&](int c, float4 y) {
+                if (kStaged) staged[c * 32 + (lane ^ (c & 7))] = y;
+                else if (r < rows) *reinterpret_cast<float4*>(out + 4 * c) = y;
+            };
 #pragma unroll 1
             for (int c = 0; c < D / 4; c += 8) {
                 uint32_t x[32];
@@ -468,8 +468,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     y = l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
                                   : make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
                     if (kParts && !whole_item) reinterpret_cast<float4*>(own)[(c + e) * C::kRows + tid] = y;
-                    else if (C::kSumInSmem) put_sum(c + e, y);
-                    else if (r < rows) *reinterpret_cast<float4*>(out + 4 * (c + e)) = y;
+                    else put_out(c + e, y);
                 }
             }
             bool there = whole_item;
@@ -511,25 +510,26 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     for (int c = 0; c < D / 4; ++c) {
                         float4 y = get_sum(c);
                         y = total == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(y.x * over, y.y * over, y.z * over, y.w * over);
-                        if (C::kSumInSmem) put_sum(c, y);
-                        else if (r < rows) *reinterpret_cast<float4*>(out + 4 * c) = y;
+                        put_out(c, y);
                     }
                 }
             }
-            if (C::kSumInSmem && there) {
-                // Through the warp's sums: whole rows per store.
+            if (kStaged && there) {
                 __syncwarp();
                 constexpr int kRowLanes = D / 4;  // 8 or 16 lanes a row
 #pragma unroll 4
                 for (int i = 0; i < 32; i += 32 / kRowLanes) {
                     const int row = i + lane / kRowLanes, c = lane % kRowLanes;
                     float* to = reinterpret_cast<float*>(__shfl_sync(~0u, reinterpret_cast<uintptr_t>(out), row));
-                    const float4 v = my_sum[c * 32 + (row ^ (c & 7))];
+                    const float4 v = staged[c * 32 + (row ^ (c & 7))];
                     if (warp * 32 + row < rows) *reinterpret_cast<float4*>(to + 4 * c) = v;
                 }
-                __syncwarp();
             }
             tcgen05_fence_before();
+            if (kStaged) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_empty[q_slot]);
+            }
         }
     } else if (warp < kMmaWarp) {
         // ------------------------------- the items, their rows, codes to fp16
@@ -546,7 +546,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         const uint32_t total = static_cast<uint32_t>(row_tiles) * g.cache.kv_heads * splits;
         bool first_take = true;
         const auto advance = [&](int it) {
-            NextItem next = {};
+            TileItem next = {};
 #pragma unroll 1
             while (true) {
                 uint32_t id = blockIdx.x;
@@ -555,7 +555,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     id = __shfl_sync(~0u, id, 0);
                 }
                 first_take = false;
-                next.rows = -1;
+                next.tiles = -1;
                 if (id >= total) break;
                 const uint32_t whole = kParts ? id / static_cast<uint32_t>(splits) : id, group_of = whole / static_cast<uint32_t>(g.cache.kv_heads);
                 if (kParts) {
@@ -597,8 +597,8 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 break;
             }
             if (lane == 0) {
-                found[it & 1] = next;
-                mbar_arrive(&found_full[it & 1]);
+                items[it % C::kItems] = next;
+                mbar_arrive(&found_full[it % C::kItems]);
             }
             __syncwarp();
         };
@@ -614,7 +614,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         // Loads run two turns ahead; rotated, scaled by the row's power of two, split,
         // stored swizzled.
         const int step_t = kPass / g.group, step_h = kPass - step_t * g.group;
-        const auto put_rows = [&](const NextItem& next, uint8_t* power) {
+        const auto put_rows = [&](const TileItem& next, uint8_t* q_hi, uint8_t* powers) {
             float4 a, b, cs, sn, a1, b1, cs1, sn1;  // this turn's, the next one's
             a = b = cs = sn = a1 = b1 = cs1 = sn1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             const int r0 = next.first_row + cw * kAtOnce + sub;
@@ -674,7 +674,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 float up, down;
                 row_power(__float_as_uint(largest), up, down);
                 if (sub < kAtOnce && r < C::kRows) {
-                    if (part == 0) power[r] = static_cast<uint8_t>(__float_as_uint(down) >> 23);
+                    if (part == 0) powers[r] = static_cast<uint8_t>(__float_as_uint(down) >> 23);
                     const unsigned long long up2 = pack2(up, up);
 #pragma unroll
                     for (int quarter = 0; quarter < 2; ++quarter) {
@@ -693,7 +693,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                         }
                         const int offset = (d >> 6) * (C::kRows * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2;
                         *reinterpret_cast<uint2*>(q_hi + offset) = make_uint2(hi[0], hi[1]);
-                        *reinterpret_cast<uint2*>(q_lo + offset) = make_uint2(lo[0], lo[1]);
+                        *reinterpret_cast<uint2*>(q_hi + C::kQBytes + offset) = make_uint2(lo[0], lo[1]);
                     }
                 }
             }
@@ -724,35 +724,18 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         // (Every piece of work stands once: the roles' code shares the instruction
         // cache.  Turn -1 only finds the first item.)
         for (int it = -1;; ++it) {
-            NextItem now = {};
+            TileItem now = {};
+            const int q_slot = it % C::kQSlots;
             if (it >= 0) {
-                ok = __all_sync(~0u, tile_wait(watch, &found_full[it & 1], (it >> 1) & 1));
+                ok = __all_sync(~0u, tile_wait(watch, &found_full[it % C::kItems], it / C::kItems & 1));
                 if (!ok) break;
-                now = found[it & 1];
-                if (it > 0) ok = __all_sync(~0u, tile_wait(watch, q_empty, (it - 1) & 1));
+                now = items[it % C::kItems];
+                if (it >= C::kQSlots) ok = __all_sync(~0u, tile_wait(watch, &q_empty[q_slot], (it / C::kQSlots - 1) & 1));
                 if (!ok) break;
             }
-            const bool more = it >= 0 && now.rows >= 0;
-            const int keys = now.keys;
-            const int tiles = more ? now.tiles : it < 0 ? 0 : -1;
-            if (it >= 0 && tid == 128) {
-                item->row0 = now.row0;
-                item->first_row = now.first_row;
-                item->rows = now.rows;
-                item->context = now.context;
-                item->keys = keys;
-                item->tiles = tiles;
-                item->head = now.head;
-                if (kParts) {
-                    item->tile0 = now.tile0;
-                    item->parts = now.parts;
-                    item->part = now.part;
-                    item->place = now.place;
-                }
-            }
-            if (it >= 0 && !more) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_full);
+            const int keys = now.keys, tiles = now.tiles;
+            if (tiles < 0) {
+                if (lane == 0) mbar_arrive(&q_full[q_slot]);
                 break;
             }
             const int32_t* table = g.step.table + (int64_t)now.request * g.step.max_pages;
@@ -793,10 +776,10 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             };
             if (it >= 0) ask_pages(0);
             if (it >= 0) {
-                put_rows(now, item->power);
+                put_rows(now, q_rows + q_slot * 2 * C::kQBytes, power + q_slot * C::kRows);
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(q_full);
+                if (lane == 0) mbar_arrive(&q_full[q_slot]);
                 fetch(0);
                 ask_pages(1);
             }
@@ -845,7 +828,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         // one lane issues.
         const bool leader = elect_one_sync();
         constexpr uint32_t s_desc = umma_idesc_f16(C::kRows, C::kKeys, false), o_desc = umma_idesc_f16(C::kRows, C::kOutCols, true);
-        const uint64_t qh = umma_desc_k_sw128(smem_u32(q_hi)), ql = umma_desc_k_sw128(smem_u32(q_lo)),
+        const uint64_t qh = umma_desc_k_sw128(smem_u32(q_rows)), ql = qh + (C::kQBytes >> 4),
                        kt = umma_desc_k_sw128(smem_u32(k_tiles)), vt = umma_desc_mn_sw128(smem_u32(v_tiles), C::kKeys * 128);
         const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, tile_wait(watch, bar, parity)); };
         const auto commit = [&](uint64_t* bar) {
@@ -854,7 +837,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         // S of tile n, into the buffer that PV of tile n - 2 reads: MMAs of
         // unlike accumulators keep no order, so that one is waited for (an
         // item's first: PV of tile n - 1, which has been issued before).
-        const auto scores = [&](int n, bool first) {
+        const auto scores = [&](int n, bool first, int q_at) {
             const int stage = n % C::kKStages;
             if (!wait(&k_full[stage], (n / C::kKStages) & 1)) return false;
             if (n >= (first ? 1 : 2) && !wait(o_done, (first ? n - 1 : n) & 1)) return false;
@@ -866,7 +849,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 for (int part = 0; part < 2; ++part)
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i)
-                        umma_f16(s_tmem, (part == 0 ? ql : qh) + ((i >> 2) * (C::kRows * 128 >> 4) + 2 * (i & 3)),
+                        umma_f16(s_tmem, (part == 0 ? ql : qh) + q_at + ((i >> 2) * (C::kRows * 128 >> 4) + 2 * (i & 3)),
                                  k + ((i >> 2) * (C::kKeys * 128 >> 4) + 2 * (i & 3)), s_desc, part > 0 || i > 0);
             }
             __syncwarp();
@@ -877,14 +860,15 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         int n = 0;
         bool ok = true;
         for (int it = 0; ok; ++it) {
-            if (!wait(q_full, it & 1)) break;
-            const int tiles = item->tiles;
+            const int q_slot = it % C::kQSlots, q_at = q_slot * (2 * C::kQBytes >> 4);
+            if (!wait(&q_full[q_slot], it / C::kQSlots & 1)) break;
+            const int tiles = items[it % C::kItems].tiles;
             if (tiles < 0) break;
 #pragma unroll 1
             for (int j = -1; j < tiles && ok; ++j) {
                 if (j + 1 < tiles) {
-                    ok = scores(n + (j >= 0), j < 0);
-                    if (j + 2 == tiles) commit(q_empty);
+                    ok = scores(n + (j >= 0), j < 0, q_at);
+                    if (j + 2 == tiles) commit(&q_empty[q_slot]);
                 }
                 if (j < 0) continue;
                 const int stage = n % C::kVStages;
