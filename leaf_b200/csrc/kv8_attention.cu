@@ -67,10 +67,14 @@ __device__ __forceinline__ void wait_async_copies_but() {
 // chunk is there, 4 us in the key loop and 1 us in joining the warps; one request
 // of 200 tokens takes 5.5 us.  Four warps a block at 64-wide heads took 19.2 us
 // instead of 13.5, three blocks of eight warps (80 registers, spilling) 21.8.
-template <int D>
+//
+// kNarrow: blocks of two warps, four or three times as many, for more heads than
+// wide blocks: a block that walks several short heads is idle in each one's round
+// trips, which the other blocks of the SM then fill.
+template <int D, bool kNarrow>
 struct Split {
-    static constexpr int kWarps = D <= 64 ? 8 : 4;
-    static constexpr int kBlocksPerSm = D <= 64 ? 2 : 3;
+    static constexpr int kWarps = kNarrow ? 2 : D <= 64 ? 8 : 4;
+    static constexpr int kBlocksPerSm = (D <= 64 ? 16 : 12) / kWarps;
     static constexpr int kStages = D <= 64 ? 3 : 2;
     static constexpr int kThreads = kWarps * 32;
     static constexpr int kBlocks = 148 * kBlocksPerSm;   // key ranges of one row block
@@ -80,9 +84,10 @@ struct Split {
     static constexpr int kRing = kStages * kStage;
     static constexpr int kPart = 8 * (D + 2);            // floats of one partial result: m [8], l [8], O [8][D]
     static constexpr size_t kSmem = (size_t)kWarps * kRing + 8 * D * sizeof(float);
+    static_assert(kBlocksPerSm * (kSmem + 1152) <= 228 * 1024, "the blocks share the SM's shared memory");
     static_assert(kRing >= kPart * 4, "a warp's partial result goes through its ring");
-    static_assert(kWarps * kRing >= 4 * (kBlocks + 1) * 4, "the step's arrays go through the rings");
-    static_assert(kWarps * kRing >= (kBlocks + 1) * 16 * 4 + (kThreads * 4 + 8 * D) * 4, "joining goes through the rings");
+    static_assert(kWarps * kRing >= kBlocks * 4, "the requests' pages go through the rings");
+    static_assert(kWarps * kRing >= (16 + kThreads * 4 + 8 * D) * 4, "joining goes through the rings");
 };
 
 // Layout of a chunk.  K's rows lie in the order of the score tiles' columns:
@@ -115,64 +120,63 @@ __device__ __forceinline__ int find_request(const int32_t* page_offsets, int req
 
 // The last block of a head to arrive joins its n parts, in their order: part i at
 // parts + i stride, the first one `first` floats further.
-template <int D>
+template <int D, bool kNarrow>
 __device__ __forceinline__ void join_parts(uint8_t* smem, const float* parts, int64_t stride, int64_t first, int n, int rows,
-                                        int group, int first_row, float* out, int64_t out_stride) {
-    using C = Split<D>;
-    // The parts' m and l and each thread's first part are asked for at once: four
-    // elements and every sets-th part per thread, then the threads' sums.
+                                           int group, int first_row, float* out, int64_t out_stride) {
+    using C = Split<D, kNarrow>;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const auto other = [&](int i) { return parts + i * stride + (i == 0 ? first : 0); };
-    float* weight_s = reinterpret_cast<float*>(smem);  // [n][16]: m and l, then weights; the rows' sums [8]
-    const int items = rows * (D / 4), sets = max(1, C::kThreads / items), set = tid / items;
-    float4 ahead;
-    if (set < sets && set < n) ahead = __ldcg(reinterpret_cast<const float4*>(other(set) + 16) + tid % items);
-    for (int i = tid; i < 16 * n; i += C::kThreads) weight_s[i] = __ldcg(other(i >> 4) + (i & 15));
-    __syncthreads();
+    float *top_s = reinterpret_cast<float*>(smem), *total_s = top_s + 8;  // of the rows
+    float4* set_s = reinterpret_cast<float4*>(total_s + 8);
+    // A part's weight, from its m (one that saw no key counts nothing, but shows an l that is no number).
+    const auto weigh = [&](float their, float part_l, float top) {
+        return their == -INFINITY ? (part_l == 0.0f ? 0.0f : 1.0f) : ex2(their - top);
+    };
     for (int r = warp; r < rows; r += C::kWarps) {
         float top = -INFINITY, total = 0.0f;
-        for (int i = lane; i < n; i += 32) top = fmaxf(top, weight_s[i * 16 + r]);
-        top = warp_max_f32(top);
-        for (int i = lane; i < n; i += 32) {
-            const float their = weight_s[i * 16 + r], part_l = weight_s[i * 16 + 8 + r];
-            const float weight = their == -INFINITY ? (part_l == 0.0f ? 0.0f : 1.0f) : ex2(their - top);
-            weight_s[i * 16 + r] = weight;
-            total = fmaf(weight, part_l, total);
+        const float m0 = lane < n ? __ldcg(other(lane) + r) : -INFINITY, l0 = lane < n ? __ldcg(other(lane) + 8 + r) : 0.0f;
+        for (int i = lane + 32; i < n; i += 32) top = fmaxf(top, __ldcg(other(i) + r));
+        top = warp_max_f32(fmaxf(top, m0));
+        total = weigh(m0, l0, top) * l0;
+        for (int i = lane + 32; i < n; i += 32) {
+            const float part_l = __ldcg(other(i) + 8 + r);
+            total = fmaf(weigh(__ldcg(other(i) + r), part_l, top), part_l, total);
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
-        if (lane == 0) weight_s[n * 16 + r] = total;
+        if (lane == 0) {
+            top_s[r] = top;
+            total_s[r] = total;
+        }
     }
     __syncthreads();
-    float4* set_s = reinterpret_cast<float4*>(weight_s + (n * 16 + 8));
+    // Four elements and every sets-th part per thread, then the threads' sums.
+    constexpr int kAhead = D <= 64 ? 2 : 4;  // (four would have the key loop of 64-wide heads spill)
+    const int items = rows * (D / 4), sets = max(1, C::kThreads / items), set = tid / items;
     for (int item = tid % items; item < items && set < sets; item += C::kThreads) {
         const int r = item / (D / 4);
+        const float top = top_s[r];
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const auto add = [&](int i, float4 v) {
-            const float weight = weight_s[i * 16 + r];
+#pragma unroll kAhead
+        for (int i = set; i < n; i += sets) {
+            const float weight = weigh(__ldcg(other(i) + r), __ldcg(other(i) + 8 + r), top);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(other(i) + 16) + item);
             sum.x = fmaf(weight, v.x, sum.x);
             sum.y = fmaf(weight, v.y, sum.y);
             sum.z = fmaf(weight, v.z, sum.z);
             sum.w = fmaf(weight, v.w, sum.w);
-        };
-        int i = set;
-        if (item == tid % items && i < n) {
-            add(i, ahead);
-            i += sets;
         }
-#pragma unroll 4
-        for (; i < n; i += sets) add(i, __ldcg(reinterpret_cast<const float4*>(other(i) + 16) + item));
         set_s[set * items + item] = sum;
     }
     __syncthreads();
-    for (int item = tid; item < rows * (D / 4); item += C::kThreads) {
+    for (int item = tid; item < items; item += C::kThreads) {
         const int r = item / (D / 4), d = 4 * (item - r * (D / 4));
         float4 sum = set_s[item];
         for (int other_set = 1; other_set < sets; ++other_set) {
             const float4 v = set_s[other_set * items + item];
             sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
         }
-        const float total = weight_s[n * 16 + r];
+        const float total = total_s[r];
         const float4 y = total == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
                                        : make_float4(sum.x / total, sum.y / total, sum.z / total, sum.w / total);
         const int t = (first_row + r) / group, hq = (first_row + r) - t * group;
@@ -180,10 +184,10 @@ __device__ __forceinline__ void join_parts(uint8_t* smem, const float* parts, in
     }
 }
 
-template <int D>
-__global__ void __launch_bounds__(Split<D>::kThreads, Split<D>::kBlocksPerSm)
+template <int D, bool kNarrow>
+__global__ void __launch_bounds__(Split<D, kNarrow>::kThreads, Split<D, kNarrow>::kBlocksPerSm)
 kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals, int ranges, int row_blocks) {
-    using C = Split<D>;
+    using C = Split<D, kNarrow>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int last_s;
     __shared__ struct {  // what the end of a segment needs: kept out of the key loop's registers
@@ -387,27 +391,36 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
         }
         // The query rows and the first chunks are under way together.
         constexpr int kRowThreads = D == 32 ? 4 : D == 64 ? 8 : 16;
-        static_assert(C::kThreads >= 8 * kRowThreads && kRowThreads >= D / 8, "one item of the query rows a thread");
-        const int row = tid / kRowThreads, item = tid % kRowThreads;
-        QueryItem<D> rows_item;
-        if (row < 8 && item < D / 8) {
-            const int t = (first_row + row) / g.group, hq = (first_row + row) - t * g.group;
-            int64_t pos = (int64_t)context + t;
-            if (row < rows && g.rotary > 0 && (pos < 0 || pos >= g.table_rows)) {
-                if (item == 0) record_device_error(kSiteKv8Range);
-                pos = 0;
+        constexpr int kRowPasses = 8 * kRowThreads <= C::kThreads ? 1 : 8 * kRowThreads / C::kThreads;
+        static_assert(kRowThreads >= D / 8 && kRowPasses * C::kThreads >= 8 * kRowThreads, "eight values a thread and pass");
+        const int item = tid % kRowThreads;
+        QueryItem<D> rows_item[kRowPasses];
+#pragma unroll
+        for (int pass = 0; pass < kRowPasses; ++pass) {
+            const int row = tid / kRowThreads + pass * (C::kThreads / kRowThreads);
+            if (row < 8 && item < D / 8) {
+                const int t = (first_row + row) / g.group, hq = (first_row + row) - t * g.group;
+                int64_t pos = (int64_t)context + t;
+                if (row < rows && g.rotary > 0 && (pos < 0 || pos >= g.table_rows)) {
+                    if (item == 0) record_device_error(kSiteKv8Range);
+                    pos = 0;
+                }
+                rows_item[pass].load(g, row < rows ? g.q + (row0 + t) * g.q_stride + (int64_t)(h * g.group + hq) * D : nullptr, item, pos);
             }
-            rows_item.load(g, row < rows ? g.q + (row0 + t) * g.q_stride + (int64_t)(h * g.group + hq) * D : nullptr, item, pos);
         }
 #pragma unroll
         for (int i = 0; i < C::kStages - 1; ++i) load(i, i, ids[i]);
         int next_id = ids[C::kStages - 1];
-        if (row < 8) {
+#pragma unroll
+        for (int pass = 0; pass < kRowPasses; ++pass) {
+            const int row = tid / kRowThreads + pass * (C::kThreads / kRowThreads);
+            if (row >= 8) break;
             // Four elements in a row are one lane's part of one MMA: lane (gq, tq) holds
             // row gq's elements that meet its bytes of a key, 16 of each 64 (D = 64, 128)
             // or D / 4 in a row.
-            if (item < D / 8) rows_item.turn();
-            uint32_t largest = item < D / 8 ? rows_item.largest() : 0;
+            QueryItem<D>& mine_item = rows_item[pass];
+            if (item < D / 8) mine_item.turn();
+            uint32_t largest = item < D / 8 ? mine_item.largest() : 0;
 #pragma unroll
             for (int d = 1; d < kRowThreads; d *= 2) largest = max(largest, __shfl_xor_sync(~0u, largest, d));
             float up, down;
@@ -423,8 +436,8 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
                                                        half2_bits(c - __low2float(cd2), d - __high2float(cd2)));
             };
             if (item < D / 8) {
-                put(rows_item.at, rows_item.a);
-                put(rows_item.to, rows_item.b);
+                put(mine_item.at, mine_item.a);
+                put(mine_item.to, mine_item.b);
             }
         }
         __syncthreads();
@@ -642,7 +655,7 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
             }
             __syncthreads();
             if (last_s)
-                join_parts<D>(smem, parts + first, 2 * (int64_t)row_blocks * C::kPart, (int64_t)row_blocks * C::kPart, count,
+                join_parts<D, kNarrow>(smem, parts + first, 2 * (int64_t)row_blocks * C::kPart, (int64_t)row_blocks * C::kPart, count,
                               rows_here, g.group, first_row, out, (int64_t)g.heads * D);
         }
         __syncthreads();  // the rings and q_s are free for the next segment
@@ -667,33 +680,41 @@ struct SplitShape {
     size_t part_bytes;
 };
 
-template <int D>
+template <int D, bool kNarrow>
 SplitShape split_shape(int64_t max_tokens, int group) {
+    using C = Split<D, kNarrow>;
     SplitShape f;
     f.row_blocks = (max_tokens * group + 7) / 8;
     if (f.row_blocks < 1) f.row_blocks = 1;
     // About one wave of blocks in all; from there on one block per row block,
     // whose requests it walks alone.
-    f.ranges = (Split<D>::kBlocks + f.row_blocks - 1) / f.row_blocks;
-    static_assert(2 * Split<D>::kBlocks <= kSplitCounters, "ranges * row_blocks, where there is more than one range");
-    f.part_bytes = f.ranges > 1 ? 2 * static_cast<size_t>(f.ranges * f.row_blocks) * Split<D>::kPart * sizeof(float) : 0;
+    f.ranges = (C::kBlocks + f.row_blocks - 1) / f.row_blocks;
+    static_assert(2 * C::kBlocks <= kSplitCounters, "ranges * row_blocks, where there is more than one range");
+    f.part_bytes = f.ranges > 1 ? 2 * static_cast<size_t>(f.ranges * f.row_blocks) * C::kPart * sizeof(float) : 0;
     return f;
 }
 
-template <int D>
+template <int D, bool kNarrow>
 int run_split(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) {
-    const SplitShape f = split_shape<D>(g.step.max_tokens, g.group);
+    using C = Split<D, kNarrow>;
+    const SplitShape f = split_shape<D, kNarrow>(g.step.max_tokens, g.group);
+    // More heads than wide blocks go to narrow ones.  Wide and narrow, us, 64-wide
+    // heads: 256 heads of 521 to 765 tokens 13.5 and 20.3, 1,024 heads of 500 to
+    // 1,000 tokens 54.6 and 39.7, 2,048 of 100 to 400 72 and 47; 128-wide: 48 of
+    // 15,000 to 91,000 tokens 103 and 124, 512 of 1,000 to 4,000 88 and 90, 1,024 of
+    // 500 to 1,500 85 and 78, 2,048 of 200 to 2,000 167 and 146.
+    if (!kNarrow && (int64_t)g.step.requests * g.cache.kv_heads > f.ranges) return run_split<D, true>(s, g, workspace, pdl);
     if (f.ranges * f.row_blocks > INT_MAX / 8) {
         set_error("leafq_kv8_attention: max_tokens * group is too large");
         return LEAFQ_ERR_INVALID;
     }
-    const int st = allow_smem(reinterpret_cast<const void*>(kv8_attend_split_kernel<D>), Split<D>::kSmem, "leafq_kv8_attention");
+    const auto kernel = kv8_attend_split_kernel<D, kNarrow>;
+    const int st = allow_smem(reinterpret_cast<const void*>(kernel), C::kSmem, "leafq_kv8_attention");
     if (st) return st;
     uint32_t* arrivals = static_cast<uint32_t*>(workspace);
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
-    return launch(kv8_attend_split_kernel<D>, dim3(static_cast<unsigned>(f.ranges * f.row_blocks)), dim3(Split<D>::kThreads),
-                  Split<D>::kSmem, s, pdl, "leafq_kv8_attention", g, parts, arrivals, static_cast<int>(f.ranges),
-                  static_cast<int>(f.row_blocks));
+    return launch(kernel, dim3(static_cast<unsigned>(f.ranges * f.row_blocks)), dim3(C::kThreads), C::kSmem, s, pdl,
+                  "leafq_kv8_attention", g, parts, arrivals, static_cast<int>(f.ranges), static_cast<int>(f.row_blocks));
 }
 
 // The tile form gives 128 rows of a request's kv head to a block, the split form
@@ -731,9 +752,10 @@ size_t leafq_kv8_attention_workspace_bytes(int64_t max_tokens, int heads, int kv
         !kv8_dim_supported(dim))
         return 0;
     return with_dim(dim, [&](auto d) {
-        const SplitShape f = split_shape<d()>(max_tokens, heads / kv_heads);
+        const size_t parts = std::max(split_shape<d(), false>(max_tokens, heads / kv_heads).part_bytes,
+                                      split_shape<d(), true>(max_tokens, heads / kv_heads).part_bytes);
         const bool tiles = max_tokens * (heads / kv_heads) >= kTileRows;
-        return kCounterBytes + std::max(f.part_bytes, tiles ? kv8_tile_part_bytes(d()) : 0);
+        return kCounterBytes + std::max(parts, tiles ? kv8_tile_part_bytes(d()) : 0);
     });
 }
 
@@ -779,7 +801,7 @@ int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int head
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool pdl = (flags & LEAFQ_FLAG_PDL) != 0;
     if (takes_tiles(step->tokens, step->max_tokens, heads, g.group)) return launch_kv8_tiles(s, g, workspace, pdl);
-    return with_dim(cache->dim, [&](auto d) { return run_split<d()>(s, g, workspace, pdl); });
+    return with_dim(cache->dim, [&](auto d) { return run_split<d(), false>(s, g, workspace, pdl); });
 }
 
 }  // extern "C"

@@ -123,8 +123,8 @@ __device__ __forceinline__ void row_power(uint32_t largest_bits, float& up, floa
 // The workspace: counters that are zero between calls, in places that do not
 // depend on the call's shape, so that calls of all shapes may share it; then the
 // parts' results.
-constexpr int kSplitCounters = 1024, kTileCounters = kSplitCounters, kTileBlocks = 296;
-constexpr size_t kCounterBytes = 8192;
+constexpr int kSplitCounters = 2560, kTileCounters = kSplitCounters, kTileBlocks = 296;
+constexpr size_t kCounterBytes = 16384;
 static_assert((kTileCounters + 4 + 4 * (kTileBlocks / 2)) * 4 <= kCounterBytes, "the items that have parts, four counters each");
 
 // Many query rows of a request (kv8_tile.cu), and what its parts take.

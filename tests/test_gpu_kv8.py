@@ -642,3 +642,20 @@ def test_attention_shapes_share_a_workspace(cuda_device):
         for i in order:
             assert torch.equal(batches[i].run(workspace=workspace), alone[i])
     assert _status_ok()
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("requests,new,page", [(70, 1, 16), (160, 2, 64), (400, 1, 32)])
+def test_attention_more_heads_than_blocks(cuda_device, dim, requests, new, page):
+    # Short caches, empty ones and a long one; requests that bring nothing among them.
+    rng = np.random.default_rng(dim + requests)
+    context = rng.integers(0, 60, requests)
+    context[rng.random(requests) < 0.1] = 0
+    context[requests // 3] = 4000
+    fresh = np.where(rng.random(requests) < 0.1, 0, rng.integers(1, new + 1, requests))
+    batch = _Batch(rng, [int(c) for c in context], [int(n) for n in fresh], page, 8, 5, dim, rotary=dim // 2)
+    first = batch.run()
+    batch.check(first)
+    assert torch.equal(batch.run(), first)
+    assert _status_ok()
+
