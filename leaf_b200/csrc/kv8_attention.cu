@@ -282,9 +282,20 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
         }
         end = p1 > p0;  // one segment at most
     } else if (range < shares) {
-        begin = units * range / shares;
-        end = units * (range + 1) / shares;
-        s = find_request(page_offsets, requests, kv_heads, begin, lane);
+        // A bound that falls into a short head moves to the nearer end of it: a join
+        // would take longer than the head (2,048 heads of 100 to 400 tokens 47 -> 37 us).
+        // A long head's shares stay the same ones.
+        const auto bound = [&](int64_t u, int& at) {
+            at = find_request(page_offsets, requests, kv_heads, u, lane);
+            const int64_t base = (int64_t)kv_heads * page_offsets[at];
+            const int held = page_offsets[at + 1] - page_offsets[at];
+            if (held <= 0 || held > ((8 * C::kWarps * C::kChunk) >> g.shift) || u < base || u >= base + (int64_t)kv_heads * held) return u;
+            const int into = static_cast<int>(u - base), rest = into % held;
+            return u - rest + (2 * rest < held ? 0 : held);
+        };
+        int unused;
+        end = bound(units * (range + 1) / shares, unused);
+        begin = bound(units * range / shares, s);
     }
 
     for (int64_t u = begin; u < end;) {
@@ -700,9 +711,9 @@ int run_split(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl)
     const SplitShape f = split_shape<D, kNarrow>(g.step.max_tokens, g.group);
     // More heads than wide blocks go to narrow ones.  Wide and narrow, us, 64-wide
     // heads: 256 heads of 521 to 765 tokens 13.5 and 20.3, 1,024 heads of 500 to
-    // 1,000 tokens 54.6 and 39.7, 2,048 of 100 to 400 72 and 47; 128-wide: 48 of
+    // 1,000 tokens 54.6 and 39.7, 2,048 of 100 to 400 72 and 37; 128-wide: 48 of
     // 15,000 to 91,000 tokens 103 and 124, 512 of 1,000 to 4,000 88 and 90, 1,024 of
-    // 500 to 1,500 85 and 78, 2,048 of 200 to 2,000 167 and 146.
+    // 500 to 1,500 85 and 76, 2,048 of 200 to 2,000 167 and 138.
     if (!kNarrow && (int64_t)g.step.requests * g.cache.kv_heads > f.ranges) return run_split<D, true>(s, g, workspace, pdl);
     if (f.ranges * f.row_blocks > INT_MAX / 8) {
         set_error("leafq_kv8_attention: max_tokens * group is too large");
