@@ -38,9 +38,9 @@ namespace {
 // time): about a third go to the softmax (5 to 6 instructions a score), a fifth
 // to rotating and splitting query rows, a sixth to the codes' conversion; the
 // rest waits on hand-offs between the roles.  4 heads of 64, 8 queries a key: 64
-// prompts of 512 tokens 368 us (187 TFLOP/s, twice that in the MMAs, since fp32
-// operands are two halves); one of 8,192 tokens 614 us (447 TFLOP/s).  5 chunks
-// of 51 to 1,500 tokens, 8 heads of 128, 3 queries a key, 85 us (247 TFLOP/s).
+// prompts of 512 tokens 362 us (190 TFLOP/s, twice that in the MMAs, since fp32
+// operands are two halves); one of 8,192 tokens 619 us (444 TFLOP/s).  5 chunks
+// of 100 to 1,500 tokens, 8 heads of 128, 3 queries a key, 83 us (250 TFLOP/s).
 constexpr float kTileLift = 6.0f, kTileHighest = 49152.0f;
 
 // Where there are fewer items than half the blocks, each is cut into parts along
