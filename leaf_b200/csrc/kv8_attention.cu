@@ -211,11 +211,12 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
     // into equal pieces of at most `piece` pages and every block takes one: the
     // smallest piece, from a warp's chunk each on, that makes no more pieces than
     // blocks.  Otherwise the units (page, head, request) in a row are dealt out in
-    // even shares, each block walking the heads in its own.  A head over several
-    // blocks costs a partial result each, which the last of them joins.
+    // even shares of one unit at least, each block walking the heads in its own.  A
+    // head over several blocks costs a partial result each, which the last of them
+    // joins: it counts every share between the head's ends, so none may be empty.
     const int64_t segments = (int64_t)requests * kv_heads;
     const bool pieces = segments <= ranges;
-    const int shares = pieces ? static_cast<int>(max64(1, min64(ranges, (units << g.shift) / (C::kWarps * C::kChunk)))) : ranges;
+    const int shares = static_cast<int>(max64(1, min64(ranges, pieces ? (units << g.shift) / (C::kWarps * C::kChunk) : units)));
     int64_t begin = 0, end = 0;
     int s = 0, h = 0, p0 = 0, p1 = 0;             // the segment: pages [p0, p1) of head h of request s
     int first_block = 0, last_block = 0;          // pieces: the blocks of this block's head

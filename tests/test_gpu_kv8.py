@@ -659,3 +659,24 @@ def test_attention_more_heads_than_blocks(cuda_device, dim, requests, new, page)
     assert torch.equal(batch.run(), first)
     assert _status_ok()
 
+
+
+def _no_counter_left(workspace):
+    torch.cuda.synchronize()
+    return not bool(workspace.buffer[:16384].any())  # the counters, in front of the partial results
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("requests,live,kv,group,new", [
+    (256, {97: 1000}, 8, 2, 1), (112, {0: 1000}, 8, 1, 1), (320, {3: 1500, 150: 1500, 319: 1500}, 4, 8, 1),
+    (24, {11: 1000}, 8, 8, 8), (200, {7: 700, 8: 40, 199: 2000}, 12, 3, 2)])
+def test_attention_few_live_requests_among_idle_ones(cuda_device, dim, requests, live, kv, group, new):
+    # More heads than blocks, but fewer pages of heads: no block that has none may be waited for.
+    rng = np.random.default_rng(dim + requests)
+    idle = _Batch(rng, [live.get(s, 0) for s in range(requests)], [new if s in live else 0 for s in range(requests)], 64, kv,
+                  group, dim, rotary=dim)
+    other = _Batch(rng, [3000, 50], [1, 1], 64, 2, 8, dim)
+    workspace = lq.Kv8Workspace()
+    for b in (idle, idle, other, idle):
+        b.check(b.run(out=torch.full(b.q.shape, float("nan"), device="cuda"), workspace=workspace))
+        assert _no_counter_left(workspace)
