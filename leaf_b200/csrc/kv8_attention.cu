@@ -526,8 +526,11 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
             // the row's four lanes.  It comes from the row's first keys; later ones are
             // weighed with it as it stands, and only where weights come out above
             // kHighest is it raised, with O and L scaled down (exactly) to the new one.
+            // A row that sees none of them keeps having none: any other would stand above
+            // its own keys' where the warps and the parts are joined.
             uint32_t p[2][4];
             float sum;
+            bool first = true;
 #pragma unroll 1
             for (;;) {
                 const float shift = m == -INFINITY ? INFINITY : m - kLift;
@@ -547,14 +550,14 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
                     p[n >> 1][2 * (n & 1)] = half2_bits(hi[0], hi[1]);
                     p[n >> 1][2 * (n & 1) + 1] = half2_bits(lo[0], lo[1]);
                 }
-                if (!__any_sync(~0u, most > kHighest || (m == -INFINITY && key < limit))) break;
+                if (!__any_sync(~0u, most > kHighest || (first && m == -INFINITY && key < limit))) break;
+                first = false;
                 float top = -INFINITY;
 #pragma unroll
                 for (int n = 0; n < 4; ++n) top = fmaxf(top, fmaxf(x[n][0], x[n][1]));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                // A row that sees none of them takes any reference: its weights are zero.
-                const float raised = m == -INFINITY && !(top > -INFINITY) ? 0.0f : fmaxf(m, ceilf(top));
+                const float raised = fmaxf(m, ceilf(top));
                 const float down = m == -INFINITY ? 0.0f : ex2(m - raised);
                 m = raised;
                 l *= down;

@@ -680,3 +680,39 @@ def test_attention_few_live_requests_among_idle_ones(cuda_device, dim, requests,
     for b in (idle, idle, other, idle):
         b.check(b.run(out=torch.full(b.q.shape, float("nan"), device="cuda"), workspace=workspace))
         assert _no_counter_left(workspace)
+
+
+def _with_scores_near(b, level):
+    """Keys whose scores are all about -level: large codes of one sign, queries of the other."""
+    b.codes[0] = b.rng.integers(64, 128, b.codes[0].shape)
+    b.q = -np.abs(b.q)
+    b.scales[0] = np.where(np.isnan(b.scales[0]), np.nan, level / (b.scale * 0.8 * 95.5 * b.dim))
+    b.cache.k.copy_(torch.from_numpy(b.codes[0]))
+    b.cache.k_scale.copy_(torch.from_numpy(b.scales[0]))
+    return b
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("context,new,group", [([27, 5], [9, 3], 1), ([61, 2045], [6, 7], 1), ([30, 4090, 94], [4, 9, 2], 3)])
+def test_attention_low_scores_beside_chunks_that_a_row_does_not_see(cuda_device, dim, context, new, group):
+    # Keys that only the later rows of a block see are no reference for the earlier ones.
+    rng = np.random.default_rng(dim + group)
+    for heads in (1, 2):
+        _with_scores_near(_Batch(rng, context, new, 16, heads, group, dim), 140.0).check()
+
+
+@pytest.mark.parametrize("new,kv,group", [(1, 2, 4), (60, 8, 8)])
+def test_attention_low_scores_behind_hidden_pages(cuda_device, new, kv, group):
+    # Pages outside the pool hide their keys: what is seen behind them is weighed as if they were not there.
+    rng = np.random.default_rng(35)
+    b = _with_scores_near(_Batch(rng, [300], [new], 16, kv, group, 64), 140.0)
+    b.plan.table[0, :8] = -1
+    got = b.run().reshape(new, kv, group, 64).cpu().numpy()
+    assert _lib.load().leafq_device_status() == _lib.LEAFQ_ERR_INVALID
+    held = b.table[0, 8:ok.pages_of(300 + new, 16)]
+    for h in range(kv):
+        k, v = (b.codes[i][held, h].reshape(-1, 64) * np.repeat(b.scales[i][held, h].astype(np.float64), 16)[:, None]
+                for i in range(2))
+        q = b.q.reshape(new, kv, group, 64)[:, h].astype(np.float64)
+        expect, reach = ok.attention(q, np.arange(300, 300 + new) + 1 - 128, k, v, b.scale)
+        assert np.all(np.abs(got[:, h] - expect) <= np.abs(v).max() * (2 * (64 + 16) * reach[..., None] + 64) * U)
