@@ -227,15 +227,17 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
         for (int r = tid; r < requests; r += C::kThreads)
             held_pages[r] = min(max(page_offsets[r + 1] - page_offsets[r], 0), static_cast<int>(g.step.max_pages));
         __syncthreads();
-        // About held / piece rounded up, the same in every block; none of no pages, no more than pages.
-        const auto pieces_of = [](int held, float inverse) {
-            return min(held, max(1, __float2int_ru(static_cast<float>(held) * inverse)));
+        int piece = max(1, static_cast<int>(__fdividef(static_cast<float>(units), static_cast<float>(shares))));
+        // About held / piece rounded up, the same in every block; none of no pages, no more than
+        // pages.  One of up to `piece` pages, whatever the inverse's last bit: at the longest
+        // head's length there are no more pieces than heads, which have a block each.
+        const auto pieces_of = [&piece](int held, float inverse) {
+            return min(held, held <= piece ? 1 : max(1, __float2int_ru(static_cast<float>(held) * inverse)));
         };
         const auto held_by = [&](int r) { return r < requests ? held_pages[r] : 0; };
         int longest = 0;
         for (int r = lane; r < requests; r += 32) longest = max(longest, held_by(r));
         longest = max(__reduce_max_sync(~0u, longest), 1);
-        int piece = max(1, static_cast<int>(__fdividef(static_cast<float>(units), static_cast<float>(shares))));
         // Heads that are not much longer than that (by about the time of a join) stay whole.
         if (longest <= piece + ((12 * C::kChunk) >> g.shift)) {
             if (range < segments) {

@@ -716,3 +716,30 @@ def test_attention_low_scores_behind_hidden_pages(cuda_device, new, kv, group):
         q = b.q.reshape(new, kv, group, 64)[:, h].astype(np.float64)
         expect, reach = ok.attention(q, np.arange(300, 300 + new) + 1 - 128, k, v, b.scale)
         assert np.all(np.abs(got[:, h] - expect) <= np.abs(v).max() * (2 * (64 + 16) * reach[..., None] + 64) * U)
+
+
+@pytest.mark.parametrize("requests,kv,dim", [(74, 4, 64), (37, 8, 64), (111, 4, 128), (37, 12, 96), (296, 1, 32)])
+def test_attention_as_many_heads_as_blocks(cuda_device, requests, kv, dim):
+    # One piece a head is all that the blocks can take, whatever the longest heads' length.
+    page, most = 16, 700
+    cache = lq.Kv8Cache.empty(most, kv, page, dim)
+    for codes, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        codes.copy_(torch.randint(-127, 128, codes.shape, device="cuda", dtype=torch.int8))
+        scale.fill_(0.02)
+    table = torch.arange(most, dtype=torch.int32, device="cuda").repeat(requests, 1)
+    q = torch.randn((requests, kv * dim), device="cuda")
+    workspace = lq.Kv8Workspace()
+    offsets = _i32(np.arange(requests + 1))
+    alone = {}
+    for held in list(range(26, 400)) + [511, 513, 699, 700]:
+        pages = np.where(np.arange(requests) % 2 == 0, held, 1 + np.arange(requests) % 5)
+        lengths = pages * page
+        plan = lq.Kv8Plan(_i32(lengths - 1), _i32(lengths), offsets, _i32(np.concatenate([[0], np.cumsum(pages)])), table,
+                          requests, 1)
+        out = torch.full(q.shape, float("nan"), device="cuda")
+        lq.kv8_attention(q, cache, plan, dim ** -0.5, out=out, workspace=workspace)
+        assert torch.isfinite(out).all(), f"{held} pages"
+        assert _no_counter_left(workspace), f"{held} pages"
+        alone.setdefault("short", out[1::2])
+        assert torch.equal(alone["short"], out[1::2])
+    assert _status_ok()
