@@ -131,6 +131,11 @@ class Kv8Plan:
                                      self.max_tokens, requests)
         self.ref = ctypes.byref(self.desc)
 
+    def bound(self, max_tokens: int) -> None:
+        """Another bound on any one request's new tokens, for the calls to come."""
+        _need(max_tokens >= 0, "token counts must not be negative")
+        self.max_tokens = self.desc.max_tokens = int(max_tokens)
+
 
 class Kv8Workspace:
     """Device scratch of ``kv8_attention``, zeroed when it grows.  Reuse it
@@ -165,11 +170,14 @@ def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tenso
     lengths[s] == context[s].  tokens: the step's rows, at least the sum of
     new_tokens (the rest get slot -1); max_tokens: a bound on any request's new
     tokens (default: tokens).  ``taken`` is only read, the new count is the
-    plan's ``taken``.  ``out``: a plan of the same sizes whose buffers are
-    reused."""
+    plan's ``taken``.  ``out``: a plan of the same buffers and rows, which is
+    filled again; max_tokens may be another."""
     requests = context.numel()
+    most = tokens if max_tokens is None else max_tokens
     if out is not None and out.context is context and out.table is table and out.tokens == tokens and out.inputs is not None:
         plan = out
+        if plan.max_tokens != most:
+            plan.bound(most)
     else:
         device = context.device
         _need(out is None, "the plan to reuse is of other buffers or sizes")
@@ -179,8 +187,7 @@ def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tenso
         room = [-(-n // 4) * 4 for n in sizes]  # 16-byte aligned pieces
         pieces = torch.empty(sum(room), dtype=torch.int32, device=device).split(room)
         lengths, token_offsets, page_offsets, after, positions, slots = (p[:n] for p, n in zip(pieces, sizes))
-        plan = Kv8Plan(context, lengths, token_offsets, page_offsets, table, tokens,
-                       tokens if max_tokens is None else max_tokens, positions, slots, after)
+        plan = Kv8Plan(context, lengths, token_offsets, page_offsets, table, tokens, most, positions, slots, after)
         plan.inputs = (context.data_ptr(), table.data_ptr(), table.shape[1])
         plan.outputs = tuple(p.data_ptr() for p in (lengths, token_offsets, page_offsets, positions, slots, after))
     _check_i32(new_tokens, "new_tokens", requests, plan.index)

@@ -743,3 +743,42 @@ def test_attention_as_many_heads_as_blocks(cuda_device, requests, kv, dim):
         alone.setdefault("short", out[1::2])
         assert torch.equal(alone["short"], out[1::2])
     assert _status_ok()
+
+
+def test_plan_that_is_reused_takes_the_new_bound(cuda_device):
+    # The rows stay the same, one request's share of them does not: 64 requests of one token, then one of 60.
+    rng = np.random.default_rng(36)
+    requests, page, kv, group, dim = 64, 16, 2, 4, 64
+    context, table = _i32([0] * requests), torch.full((requests, 8), -1, dtype=torch.int32, device="cuda")
+    free, taken = _i32(rng.permutation(requests * 8)), _i32([0])
+    cache = lq.Kv8Cache.empty(requests * 8, kv, page, dim)
+    rows = torch.randn((requests, kv * dim), device="cuda")
+    q = torch.randn((requests, kv * group * dim), device="cuda")
+    plan = lq.kv8_plan(context, _i32([1] * requests), table, free, taken, page, requests, max_tokens=1)
+    lq.kv8_append(rows, rows, cache, plan.slots)
+    lq.kv8_attention(q, cache, plan, dim ** -0.5)
+    context.copy_(plan.lengths)
+    taken.copy_(plan.taken)
+    new = [0] * requests
+    new[5] = 60
+    again = lq.kv8_plan(context, _i32(new), table, free, taken, page, requests, max_tokens=60, out=plan)
+    assert again is plan and plan.max_tokens == 60
+    lq.kv8_append(rows, rows, cache, plan.slots)
+    out = lq.kv8_attention(q, cache, plan, dim ** -0.5, out=torch.full(q.shape, float("nan"), device="cuda"))
+    fresh = lq.kv8_plan(context, _i32(new), table.clone(), free, taken, page, requests, max_tokens=60)
+    expect = lq.kv8_attention(q, cache, fresh, dim ** -0.5)
+    assert torch.isfinite(out[:60]).all() and torch.equal(out[:60], expect[:60])
+    held = table[5, :4].long()
+    k, v = ((c[held].float() * s[held][:, :, None, None]).permute(1, 0, 2, 3).reshape(kv, -1, dim).double().cpu().numpy()
+            for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    for h in range(kv):
+        x = q[:60].reshape(60, kv, group, dim)[:, h].double().cpu().numpy()
+        exact, reach = ok.attention(x, np.arange(60) + 2, k[h], v[h], dim ** -0.5)
+        got = out[:60].reshape(60, kv, group, dim)[:, h].cpu().numpy()
+        assert np.all(np.abs(got - exact) <= np.abs(v[h]).max() * (2 * (dim + 16) * reach[..., None] + 64) * U)
+    # Without a bound it is the step's rows again.
+    assert lq.kv8_plan(context, _i32(new), table, free, taken, page, requests, out=plan).max_tokens == requests
+    assert plan.desc.max_tokens == requests
+    with pytest.raises(lq.LeafError, match="negative"):
+        lq.kv8_plan(context, _i32(new), table, free, taken, page, requests, max_tokens=-1, out=plan)
+    assert _status_ok()
