@@ -139,15 +139,19 @@ class Kv8Plan:
 
 class Kv8Workspace:
     """Device scratch of ``kv8_attention``, zeroed when it grows.  Reuse it
-    across calls on one stream."""
+    across calls on one stream.  A buffer that was outgrown lives as long as the
+    handle: a graph captured with it holds its address, and so do calls that
+    have not run yet.  Keep the handle as long as the graph."""
 
     def __init__(self, device="cuda"):
         self.device = torch.device(device)
         self.buffer = torch.empty(0, dtype=torch.uint8, device=self.device)
+        self.outgrown: list = []
         self.sizes: dict = {}
 
     def get(self, nbytes: int) -> torch.Tensor:
         if nbytes > self.buffer.numel():
+            self.outgrown.append(self.buffer)
             self.buffer = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
         return self.buffer
 

@@ -782,3 +782,28 @@ def test_plan_that_is_reused_takes_the_new_bound(cuda_device):
     with pytest.raises(lq.LeafError, match="negative"):
         lq.kv8_plan(context, _i32(new), table, free, taken, page, requests, max_tokens=-1, out=plan)
     assert _status_ok()
+
+
+def test_graph_replays_after_its_workspace_has_grown(cuda_device):
+    rng = np.random.default_rng(38)
+    decode, prompt = _Batch(rng, [9000, 300], [1, 1], 64, 2, 8, 64), _Batch(rng, [40], [700], 64, 4, 8, 64)
+    workspace = lq.Kv8Workspace()
+    q, out = torch.from_numpy(decode.q).cuda(), torch.zeros(decode.q.shape, device="cuda")
+    decode.run(q, out=out, workspace=workspace)
+    expect = out.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        decode.run(q, out=out, workspace=workspace)
+    first = workspace.buffer.data_ptr()
+    size = workspace.buffer.numel()
+    prompt.check(prompt.run(workspace=workspace))
+    assert workspace.buffer.data_ptr() != first
+    others = [torch.full((size,), 77, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    for _ in range(3):
+        out.fill_(7.0)
+        graph.replay()
+        assert torch.equal(out, expect)
+    assert all(bool((t == 77).all()) for t in others)
+    prompt.check(prompt.run(workspace=workspace))
+    assert _no_counter_left(workspace)

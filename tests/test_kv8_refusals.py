@@ -1,6 +1,7 @@
 """The paged INT8 cache's entry points reject invalid arguments on the host,
 before touching a device."""
 import ctypes
+import weakref
 
 import pytest
 import torch
@@ -102,3 +103,13 @@ def test_python_refuses_what_it_cannot_pass_on():
         lq.Kv8Plan(i(2), i(2), i(3), i(3), i(2), 2, 1)
     with pytest.raises(lq.LeafError, match="int32 CUDA"):
         lq.kv8_plan(i(2), i(2), i(2, 3), i(4), i(1), 16, 2)
+
+
+def test_workspace_that_grows_keeps_what_a_graph_may_hold():
+    workspace = lq.Kv8Workspace("cpu")
+    small = workspace.get(64)
+    kept, address = weakref.ref(small), small.data_ptr()
+    del small
+    assert workspace.get(4096).numel() == 4096
+    assert kept() is not None and kept().data_ptr() == address and kept().numel() == 64
+    assert workspace.get(64).numel() == 4096
