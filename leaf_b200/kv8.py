@@ -251,7 +251,9 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float,
         _fail("out must be contiguous float32 of q's shape, on its device")
     rotary, cos, sin, rows = _rope_args(rope, dim, index)
     heads = width // dim
-    address, need = (Kv8Workspace(cache.device) if workspace is None else workspace).of(plan.max_tokens, heads, cache.kv_heads, dim)
+    if workspace is None:
+        workspace = Kv8Workspace(cache.device)  # in a name of its own, until the launch is enqueued
+    address, need = workspace.of(plan.max_tokens, heads, cache.kv_heads, dim)
     check(load().leafq_kv8_attention(_raw_stream(index), q.data_ptr(), stride, heads, rotary, cos, sin, rows, cache.ref,
                                      plan.ref, scale, out.data_ptr(), address, need, flags))
     return out

@@ -1,13 +1,14 @@
 """The paged INT8 cache's entry points reject invalid arguments on the host,
 before touching a device."""
 import ctypes
+import types
 import weakref
 
 import pytest
 import torch
 
 import leaf_b200 as lq
-from leaf_b200 import _lib
+from leaf_b200 import _lib, kv8
 
 P = ctypes.c_void_p(256)
 ODD = ctypes.c_void_p(264)
@@ -113,3 +114,36 @@ def test_workspace_that_grows_keeps_what_a_graph_may_hold():
     assert workspace.get(4096).numel() == 4096
     assert kept() is not None and kept().data_ptr() == address and kept().numel() == 64
     assert workspace.get(64).numel() == 4096
+
+
+class _Host:
+    """Stand-ins for a cache and a plan in host memory: what the Python layer does before and around a C call, without one."""
+
+    def __init__(self, monkeypatch, dim=32, requests=2, tokens=3):
+        self.cache = types.SimpleNamespace(index=-1, device=torch.device("cpu"), dim=dim, kv_heads=1, width=dim, page=16,
+                                           ref=None)
+        self.plan = types.SimpleNamespace(index=-1, tokens=tokens, max_tokens=tokens, page=16, ref=None)
+        self.rows = torch.zeros((tokens, dim))
+        self.calls = []
+        monkeypatch.setattr(kv8, "_raw_stream", lambda index: 1000 + index)
+        for name in ("leafq_kv8_plan", "leafq_kv8_append", "leafq_kv8_attention"):
+            monkeypatch.setattr(_lib.load(), name, lambda *args, name=name: self.called(name, args))
+
+    def called(self, name, args):
+        self.calls.append((name, args))
+        return 0
+
+
+def test_attention_holds_its_own_workspace_until_the_call_has_returned(monkeypatch):
+    host, made, alive = _Host(monkeypatch), [], []
+
+    class Watched(lq.Kv8Workspace):
+        def get(self, nbytes):
+            buffer = super().get(nbytes)
+            made.append(weakref.ref(buffer))
+            return buffer
+
+    monkeypatch.setattr(kv8, "Kv8Workspace", Watched)
+    monkeypatch.setattr(_lib.load(), "leafq_kv8_attention", lambda *args: alive.append(made[-1]() is not None) or 0)
+    lq.kv8_attention(host.rows, host.cache, host.plan, 1.0)
+    assert alive == [True]
