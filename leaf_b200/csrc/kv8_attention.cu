@@ -485,11 +485,12 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const float vs = n == 0 ? scales.y : scales.w;
-                const int e = (__float_as_int(vs) >> 23) & 255;
+                const bool zero = vs < kLeastScale;
+                const int e = zero ? kZeroExponent + 127 : min(__float_as_int(vs) >> 23, 253);  // (no number: 253)
                 ks[n] = (n == 0 ? scales.x : scales.z) * factor;
                 bias[n] = vs < 0.0f ? -INFINITY : static_cast<float>(e - 127);
-                back[n] = __int_as_float(max(0, 254 - e) << 23);
-                frac[n] = vs * back[n];
+                back[n] = __int_as_float((254 - e) << 23);
+                frac[n] = zero ? 0.0f : vs * back[n];
             }
 
             // Scores of keys key + 8 n + {tq, 4 + tq} (n-tile n), in x + e.

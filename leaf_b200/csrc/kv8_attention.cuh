@@ -31,6 +31,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 // so that the second half of a weight's fp16 split stays a normal number far
 // below it; twice kHighest is below 65504, fp16's largest.
 constexpr float kLift = 6.0f, kHighest = 24576.0f;
+// A page's weights carry its V scale's exponent, which their sum takes out again: as
+// a factor of up to 2^90, so that the sum of 2^17 keys' weights stays below 2^127.
+// Smaller scales count as zero.  The weights of such a page count in the sum as at a
+// scale of 2^-63, which stands in reach (2^126) of the others of a cache, and below
+// those that an append gives.
+constexpr float kLeastScale = 0x1p-90f;
+constexpr int kZeroExponent = -63;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

@@ -807,3 +807,39 @@ def test_graph_replays_after_its_workspace_has_grown(cuda_device):
     assert all(bool((t == 77).all()) for t in others)
     prompt.check(prompt.run(workspace=workspace))
     assert _no_counter_left(workspace)
+
+
+@pytest.mark.parametrize("new,kv,group,dim", [(1, 2, 4, 64), (3, 4, 2, 128), (40, 8, 8, 64), (60, 8, 6, 128), (260, 1, 8, 96)])
+@pytest.mark.parametrize("kind", ["first", "all", "last", "small", "beside large", "steps"])
+def test_attention_value_scales_of_zero_and_small_ones(cuda_device, new, kv, group, dim, kind):
+    # A page whose values are all zero counts in the sum of the weights as any other.
+    rng = np.random.default_rng(new + dim)
+    b = _Batch(rng, [1500, 200], [new, new], 16, kv, group, dim, spread=0.5)
+    for held in ([int(p) for p in row if p >= 0] for row in b.table):
+        pages = np.arange(len(held))
+        if kind == "first":
+            b.scales[1, held[:5]] = 0.0
+        elif kind == "all":
+            b.scales[1, held] = 0.0
+        elif kind == "last":
+            b.scales[1, held[-3:]] = 0.0
+        elif kind == "small":
+            b.scales[1, held] *= 2.0 ** -80
+        elif kind == "beside large":
+            b.scales[1, held] *= np.where(pages % 3 == 0, 0.0, 1e14)[:, None].astype(np.float32)
+        else:
+            b.scales[1, held] = (10.0 ** (-7.0 * (4 - pages % 5)))[:, None]
+    b.cache.v_scale.copy_(torch.from_numpy(b.scales[1]))
+    b.check()
+
+
+@pytest.mark.parametrize("new,kv,group", [(1, 2, 4), (70, 8, 8)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_attention_values_that_are_all_no_numbers(cuda_device, new, kv, group, value):
+    rng = np.random.default_rng(37)
+    b = _Batch(rng, [20, 6], [new, new], 16, kv, group, 64)
+    b.cache.v_scale[[int(p) for p in b.table[0] if p >= 0], 1] = value
+    got = b.run().reshape(2, new, kv, -1)
+    assert not torch.isfinite(got[0, :, 1]).any()
+    assert torch.isfinite(got[0, :, 0]).all() and torch.isfinite(got[1]).all()
+    assert _status_ok()
