@@ -485,12 +485,13 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const float vs = n == 0 ? scales.y : scales.w;
-                const bool zero = vs < kLeastScale;
-                const int e = zero ? kZeroExponent + 127 : min(__float_as_int(vs) >> 23, 253);  // (no number: 253)
-                ks[n] = (n == 0 ? scales.x : scales.z) * factor;
+                const bool number = vs >= kLeastScale && vs < INFINITY;
+                const int e = number ? __float_as_int(vs) >> 23 : static_cast<int>(kZeroExponent) + 127;
+                // A V scale that is no number shows in the scores: where they are hidden it does not.
+                ks[n] = fmaf(vs, 0.0f, (n == 0 ? scales.x : scales.z) * factor);
                 bias[n] = vs < 0.0f ? -INFINITY : static_cast<float>(e - 127);
                 back[n] = __int_as_float((254 - e) << 23);
-                frac[n] = zero ? 0.0f : vs * back[n];
+                frac[n] = number ? vs * back[n] : 0.0f;
             }
 
             // Scores of keys key + 8 n + {tq, 4 + tq} (n-tile n), in x + e.

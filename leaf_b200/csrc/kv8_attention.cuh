@@ -37,7 +37,7 @@ constexpr float kLift = 6.0f, kHighest = 24576.0f;
 // scale of 2^-63, which stands in reach (2^126) of the others of a cache, and below
 // those that an append gives.
 constexpr float kLeastScale = 0x1p-90f;
-constexpr int kZeroExponent = -63;
+constexpr float kZeroExponent = -63.0f, kZeroInverse = 0x1p63f;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

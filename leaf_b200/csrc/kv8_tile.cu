@@ -80,7 +80,7 @@ struct TileShape {
     static constexpr int kOutCols = kBlocks * 64;        // O columns (those past D are not read)
     static constexpr uint32_t kTmemCols = 256;
     static constexpr size_t kSmem = kQSlots * 2 * kQBytes + (kKStages + kVStages) * kKvBytes + kInfo * kGroups * 16 +
-                                    kItems * sizeof(TileItem) + kQSlots * kRows + (2 * kKStages + 2 * kVStages + 2 * kQSlots + kItems + 7) * 8 + 8 + kInfo * 4;
+                                    kItems * sizeof(TileItem) + kQSlots * kRows + (2 * kKStages + 2 * kVStages + 2 * kQSlots + kItems + 7) * 8 + 16;
     static_assert(kQSlots == 1 || kRows * D * 4 <= 2 * kQBytes, "the output goes through the place of the item's rows");
     static constexpr int kPart = kRows * (D + 2);        // floats of a part's result: O [D / 4][128][4], m [128], l [128]
     static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two blocks share the SM's shared memory");
@@ -189,7 +189,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
     uint8_t* q_rows = smem;  // [kQSlots]: hi, lo
     uint8_t* k_tiles = q_rows + C::kQSlots * 2 * C::kQBytes;
     uint8_t* v_tiles = k_tiles + C::kKStages * C::kKvBytes;
-    float4* info = reinterpret_cast<float4*>(v_tiles + C::kVStages * C::kKvBytes);  // [kInfo][kGroups]: ks, log2 vs, 1 / vs, 1 where vs counts as zero
+    float4* info = reinterpret_cast<float4*>(v_tiles + C::kVStages * C::kKvBytes);  // [kInfo][kGroups]: ks, log2 vs, 1 / vs, 1: vs counts as zero, 2: they are no numbers
     TileItem* items = reinterpret_cast<TileItem*>(info + C::kInfo * C::kGroups);
     uint8_t* power = reinterpret_cast<uint8_t*>(items + C::kItems);  // [kQSlots][128]: of two, that a row was scaled down by (exponent bits)
     uint64_t* k_full = reinterpret_cast<uint64_t*>(power + C::kQSlots * C::kRows);
@@ -205,7 +205,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
     uint64_t* item_done = o_done + 1;            // all its MMAs have completed
     uint64_t* drained = item_done + 1;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
-    int* marked = reinterpret_cast<int*>(tmem_holder + 2);  // by info: the last tile there that has a group of zeros
+    int* marked = reinterpret_cast<int*>(tmem_holder + 2);  // the last tile so far that has such a group
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kMmaWarp = 8;
     const auto token_of = [&](int row) { return static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(g.group)); };
@@ -236,7 +236,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             mbar_init(o_done, 1);
             mbar_init(item_done, 1);
             mbar_init(drained, 1);
-            for (int i = 0; i < C::kInfo; ++i) marked[i] = -1;
+            *marked = -1;
             fence_barrier_init();
         }
         __syncwarp();
@@ -411,13 +411,16 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     tmem_st_32x32b_x32(s_tmem + lanes + 32 * c, p);
                 }
                 if (!ok) break;
-                if (marked[n % C::kInfo] == n) {
-                    // Values of zero: their weights count in L alone.  (Apart from the loop above,
-                    // which it would slow by 7 %, as a vote over the groups would the conversion.)
+                if (*marked >= n) {  // this tile, or one soon
+                    // Values of zero: their weights count in L alone.  Scales that are no numbers: nor is
+                    // the output of a row that sees them.  (Apart from the loop above, which it would
+                    // slow by 7 %, as a vote over the groups would the conversion.)
                     tmem_wait_st();
 #pragma unroll 1
                     for (int i = 0; i < C::kGroups; ++i) {
-                        if (scales[i].w == 0.0f) continue;
+                        const float kind = scales[i].w;
+                        if (kind == 2.0f && visible > 16 * i) l = NAN;
+                        if (kind != 1.0f) continue;
                         const uint32_t at = s_tmem + lanes + 32 * (i >> 1) + 8 * (i & 1);  // the hi pairs
                         tmem_zero_x8(at);
                         tmem_zero_x8(at + 16);
@@ -820,15 +823,18 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 }
                 if (is_k && ct < C::kGroups) {
                     float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);  // hides the group
-                    if (!(vs < 0.0f)) {
+                    if (vs >= kLeastScale && !isnan(fmaf(vs, 0.0f, ks))) {
                         // log2 vs and 1 / vs from an approximate logarithm a: with
                         // vs 2^-a = 1 + d, log2 vs = a + d log2 e and 1 / vs = 2^-a (1 - d),
-                        // to d^2, about 2^-44.  A page of zeros counts in the sum as any other.
-                        const bool zero = vs < kLeastScale;
-                        const float a = zero ? static_cast<float>(kZeroExponent) : lg2(vs), back = ex2(-a);
-                        const float d = zero ? 0.0f : fmaf(vs, back, -1.0f);
-                        f = make_float4(ks, fmaf(d, kLog2e, a), fmaf(-d, back, back), zero ? 1.0f : 0.0f);
-                        if (zero) marked[tile % C::kInfo] = tile;
+                        // to d^2, about 2^-44.
+                        const float a = lg2(vs), back = ex2(-a), d = fmaf(vs, back, -1.0f);
+                        f = make_float4(ks, fmaf(d, kLog2e, a), fmaf(-d, back, back), 0.0f);
+                    } else if (!(vs < 0.0f)) {
+                        // A page of zeros counts in the sum as any other.  Scales that are no numbers
+                        // would reach rows that do not see the group: they are shown to those that do.
+                        const bool zero = vs < kLeastScale && !isnan(ks);
+                        f = make_float4(zero ? ks : 0.0f, kZeroExponent, kZeroInverse, zero ? 1.0f : 2.0f);
+                        *marked = tile;
                     }
                     info[(tile % C::kInfo) * C::kGroups + ct] = f;
                 }

@@ -843,3 +843,23 @@ def test_attention_values_that_are_all_no_numbers(cuda_device, new, kv, group, v
     assert not torch.isfinite(got[0, :, 1]).any()
     assert torch.isfinite(got[0, :, 0]).all() and torch.isfinite(got[1]).all()
     assert _status_ok()
+
+
+@pytest.mark.parametrize("new,kv,group,dim", [(9, 2, 1, 64), (9, 2, 1, 96), (6, 3, 4, 128), (70, 8, 8, 64), (70, 8, 6, 128), (70, 8, 8, 32)])
+@pytest.mark.parametrize("which,value", [("k", float("nan")), ("v", float("nan")), ("k", float("inf")), ("v", float("inf"))])
+def test_attention_rows_are_clear_of_pages_that_they_do_not_see(cuda_device, new, kv, group, dim, which, value):
+    # A page of scale NaN or infinity shows in the rows that see it, not in those before it.
+    rng = np.random.default_rng(new + dim)
+    b = _Batch(rng, [43, 11], [new, new], 16, kv, group, dim)
+    clean = b.run()
+    first = 3  # request 0's page of positions 48 .., which its first five rows do not see
+    scales = b.cache.k_scale if which == "k" else b.cache.v_scale
+    scales[int(b.table[0, first]), 0] = value
+    got = b.run()
+    rows = torch.arange(b.tokens, device="cuda")
+    columns = torch.arange(b.q.shape[1], device="cuda")
+    sees = ((rows >= 16 * first - 43) & (rows < new))[:, None] & (columns < group * dim)
+    assert torch.isfinite(got[~sees]).all()
+    if not (which == "k" and value == float("inf")):  # (a score of minus infinity weighs nothing)
+        assert not torch.isfinite(got[sees]).any()
+    b.check(torch.where(sees, clean, got))
