@@ -26,6 +26,7 @@ HEAD_SIZES = (32, 64, 96, 128)
 
 _F32, _I32 = torch.float32, torch.int32
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without an object around it
+_current_device = torch._C._cuda_getDevice
 
 
 def _fail(message: str) -> None:
@@ -35,6 +36,17 @@ def _fail(message: str) -> None:
 def _need(ok: bool, message: str) -> None:
     if not ok:
         _fail(message)
+
+
+def _enqueue(index: int, function, *args) -> None:
+    """A C call on the current stream of the tensors' device `index`.  The
+    library launches on the current device, so the call is made with that one
+    current."""
+    if _current_device() == index:
+        check(function(_raw_stream(index), *args))
+    else:
+        with torch.cuda.device(index):
+            check(function(_raw_stream(index), *args))
 
 
 # The calls sit in a decode loop, a few microseconds each: the checks below ask
@@ -197,9 +209,8 @@ def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tenso
     _check_i32(new_tokens, "new_tokens", requests, plan.index)
     _check_i32(free_pages, "free_pages", None, plan.index)
     _check_i32(taken, "taken", 1, plan.index)
-    check(load().leafq_kv8_plan(_raw_stream(plan.index), plan.inputs[0], new_tokens.data_ptr(), requests, plan.inputs[1],
-                                plan.inputs[2], free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(), page, tokens,
-                                *plan.outputs, flags))
+    _enqueue(plan.index, load().leafq_kv8_plan, plan.inputs[0], new_tokens.data_ptr(), requests, plan.inputs[1],
+             plan.inputs[2], free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(), page, tokens, *plan.outputs, flags)
     return plan
 
 
@@ -224,8 +235,8 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: Kv8Cache, slots: torch.T
             _fail("rotation needs positions")
         _check_i32(positions, "positions", tokens, index)
         where = positions.data_ptr()
-    check(load().leafq_kv8_append(_raw_stream(index), k.data_ptr(), k_stride, v.data_ptr(), v_stride, tokens, where,
-                                  slots.data_ptr(), rotary, cos, sin, rows, cache.ref, flags))
+    _enqueue(index, load().leafq_kv8_append, k.data_ptr(), k_stride, v.data_ptr(), v_stride, tokens, where,
+             slots.data_ptr(), rotary, cos, sin, rows, cache.ref, flags)
 
 
 def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float, rope=None,
@@ -254,6 +265,6 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float,
     if workspace is None:
         workspace = Kv8Workspace(cache.device)  # in a name of its own, until the launch is enqueued
     address, need = workspace.of(plan.max_tokens, heads, cache.kv_heads, dim)
-    check(load().leafq_kv8_attention(_raw_stream(index), q.data_ptr(), stride, heads, rotary, cos, sin, rows, cache.ref,
-                                     plan.ref, scale, out.data_ptr(), address, need, flags))
+    _enqueue(index, load().leafq_kv8_attention, q.data_ptr(), stride, heads, rotary, cos, sin, rows, cache.ref, plan.ref,
+             scale, out.data_ptr(), address, need, flags)
     return out

@@ -126,6 +126,7 @@ class _Host:
         self.rows = torch.zeros((tokens, dim))
         self.calls = []
         monkeypatch.setattr(kv8, "_raw_stream", lambda index: 1000 + index)
+        monkeypatch.setattr(kv8, "_current_device", lambda: -1, raising=False)
         for name in ("leafq_kv8_plan", "leafq_kv8_append", "leafq_kv8_attention"):
             monkeypatch.setattr(_lib.load(), name, lambda *args, name=name: self.called(name, args))
 
@@ -147,3 +148,43 @@ def test_attention_holds_its_own_workspace_until_the_call_has_returned(monkeypat
     monkeypatch.setattr(_lib.load(), "leafq_kv8_attention", lambda *args: alive.append(made[-1]() is not None) or 0)
     lq.kv8_attention(host.rows, host.cache, host.plan, 1.0)
     assert alive == [True]
+
+
+def _plan_tensors(requests=2, pages=3):
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    return dict(context=i(requests), new_tokens=i(requests), table=i(requests, pages), free_pages=i(4), taken=i(1))
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_calls_are_made_on_their_tensors_device(monkeypatch, current):
+    # Tensors of device 1, with 0 or 1 current: the launch is 1's either way, and what was current is so again.
+    host, devices = _Host(monkeypatch), [current]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            devices.append(self.index)
+
+        def __exit__(self, *error):
+            devices.pop()
+
+    monkeypatch.setattr(kv8, "_current_device", lambda: devices[-1], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    seen = []
+    monkeypatch.setattr(host, "called", lambda name, args: seen.append((name, devices[-1], args[0])) or 0)
+    for name in ("_check_i32", "_check_rows"):
+        monkeypatch.setattr(kv8, name, lambda *a, **k: 0)
+    host.cache.index = host.plan.index = 1
+    workspace = types.SimpleNamespace(index=1, of=lambda *a: (0, 0))
+    tensors = _plan_tensors()
+    plan = types.SimpleNamespace(context=tensors["context"], table=tensors["table"], tokens=3, max_tokens=3, page=16,
+                                 inputs=(0, 0, 3), outputs=(0,) * 6, index=1)
+    lq.kv8_plan(**tensors, page=16, tokens=3, out=plan)
+    lq.kv8_append(host.rows, host.rows, host.cache, torch.zeros(3, dtype=torch.int32))
+    out = types.SimpleNamespace(get_device=lambda: 1, dtype=torch.float32, is_contiguous=lambda: True, shape=host.rows.shape,
+                                data_ptr=lambda: 0)
+    lq.kv8_attention(host.rows, host.cache, host.plan, 1.0, out=out, workspace=workspace)
+    assert seen == [("leafq_kv8_plan", 1, 1001), ("leafq_kv8_append", 1, 1001), ("leafq_kv8_attention", 1, 1001)]
+    assert devices == [current]
