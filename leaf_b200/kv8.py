@@ -156,8 +156,8 @@ class Kv8Workspace:
     have not run yet.  Keep the handle as long as the graph."""
 
     def __init__(self, device="cuda"):
-        self.device = torch.device(device)
-        self.buffer = torch.empty(0, dtype=torch.uint8, device=self.device)
+        self.buffer = torch.empty(0, dtype=torch.uint8, device=device)
+        self.device, self.index = self.buffer.device, self.buffer.get_device()
         self.outgrown: list = []
         self.sizes: dict = {}
 
@@ -264,6 +264,8 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float,
     heads = width // dim
     if workspace is None:
         workspace = Kv8Workspace(cache.device)  # in a name of its own, until the launch is enqueued
+    elif workspace.index != index:
+        _fail("the workspace is on another device")
     address, need = workspace.of(plan.max_tokens, heads, cache.kv_heads, dim)
     _enqueue(index, load().leafq_kv8_attention, q.data_ptr(), stride, heads, rotary, cos, sin, rows, cache.ref, plan.ref,
              scale, out.data_ptr(), address, need, flags)

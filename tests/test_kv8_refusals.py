@@ -188,3 +188,20 @@ def test_calls_are_made_on_their_tensors_device(monkeypatch, current):
     lq.kv8_attention(host.rows, host.cache, host.plan, 1.0, out=out, workspace=workspace)
     assert seen == [("leafq_kv8_plan", 1, 1001), ("leafq_kv8_append", 1, 1001), ("leafq_kv8_attention", 1, 1001)]
     assert devices == [current]
+
+
+def test_attention_refuses_a_workspace_of_another_device(monkeypatch):
+    host = _Host(monkeypatch)
+    away = types.SimpleNamespace(index=0, of=lambda *a: (256, 256))
+    with pytest.raises(lq.LeafError, match="workspace is on another device"):
+        lq.kv8_attention(host.rows, host.cache, host.plan, 1.0, workspace=away)
+    assert not host.calls
+    here = lq.Kv8Workspace("cpu")
+    lq.kv8_attention(host.rows, host.cache, host.plan, 1.0, workspace=here)
+    assert here.index == -1 and here.device == here.buffer.device and len(host.calls) == 1
+
+
+@pytest.mark.gpu
+def test_workspace_keeps_the_device_that_it_was_made_on(cuda_device):
+    workspace = lq.Kv8Workspace()
+    assert workspace.device == torch.device("cuda", workspace.index) == workspace.get(64).device
