@@ -405,6 +405,16 @@ __global__ void __launch_bounds__(512, 2) kv8_append_kernel(const AppendArgs g) 
     }
 }
 
+// `count` values of a call's argument.
+struct Span {
+    const int32_t* begin;
+    int64_t count;
+    bool overlaps(const Span& other) const {
+        const auto at = reinterpret_cast<uintptr_t>(begin), other_at = reinterpret_cast<uintptr_t>(other.begin);
+        return count > 0 && other.count > 0 && at < other_at + 4 * other.count && other_at < at + 4 * count;
+    }
+};
+
 int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1; }
 
 }  // namespace
@@ -464,6 +474,16 @@ int leafq_kv8_plan(void* stream, const int32_t* context, const int32_t* new_toke
         set_error("leafq_kv8_plan: positions and slots must be 16-byte aligned");
         return LEAFQ_ERR_INVALID;
     }
+    // Every block reads the inputs while block 0 writes the requests' outputs.
+    const Span inputs[] = {{context, requests}, {new_tokens, requests}, {table, requests * max_pages}, {free_pages, free_count}, {taken, 1}};
+    const Span outputs[] = {{lengths, requests}, {token_offsets, requests + 1}, {page_offsets, requests + 1}, {positions, tokens},
+                            {slots, tokens}, {taken_after, 1}};
+    for (const Span& out : outputs)
+        for (const Span& in : inputs)
+            if (out.overlaps(in)) {
+                set_error("leafq_kv8_plan: outputs must not overlap the inputs (taken_after and taken, lengths and context, ...)");
+                return LEAFQ_ERR_INVALID;
+            }
     PlanArgs g{context, new_tokens, table, free_pages, taken, lengths, token_offsets, page_offsets, positions, slots,
                taken_after, max_pages, free_count, tokens, requests, shift};
     // One block for a decode step; with many tokens one block per 4096 of them.

@@ -186,7 +186,8 @@ def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tenso
     lengths[s] == context[s].  tokens: the step's rows, at least the sum of
     new_tokens (the rest get slot -1); max_tokens: a bound on any request's new
     tokens (default: tokens).  ``taken`` is only read, the new count is the
-    plan's ``taken``.  ``out``: a plan of the same buffers and rows, which is
+    plan's ``taken`` (copy it back for the next step: a plan's own outputs are no
+    inputs of its next filling).  ``out``: a plan of the same buffers and rows, which is
     filled again; max_tokens may be another."""
     requests = context.numel()
     most = tokens if max_tokens is None else max_tokens

@@ -205,3 +205,19 @@ def test_attention_refuses_a_workspace_of_another_device(monkeypatch):
 def test_workspace_keeps_the_device_that_it_was_made_on(cuda_device):
     workspace = lq.Kv8Workspace()
     assert workspace.device == torch.device("cuda", workspace.index) == workspace.get(64).device
+
+
+@pytest.mark.parametrize("output,given", [("after", "taken"), ("lengths", "context"), ("lengths", "new"), ("slots", "table"),
+                                          ("positions", "free"), ("token_offsets", "taken"), ("page_offsets", "context")])
+def test_plan_rejects_outputs_that_overlap_its_inputs(output, given):
+    # 3 requests, 3 tokens, 4 pages a row, 8 free pages, each array 256 bytes from the next.
+    names = ("context", "new", "table", "free", "taken", "lengths", "token_offsets", "page_offsets", "positions", "slots", "after")
+    place = {name: 4096 + 256 * i for i, name in enumerate(names)}
+    place[output] = place[given]
+    assert _plan(**{name: ctypes.c_void_p(at) for name, at in place.items()}) == _lib.LEAFQ_ERR_INVALID
+    assert b"overlap" in _lib.load().leafq_last_error()
+    # The last value of the input is as bad as the first.
+    place[output] = place[given] + 4 * ({"context": 3, "new": 3, "table": 12, "free": 8, "taken": 1}[given] - 1)
+    place[output] -= place[output] % 16 if output in ("positions", "slots") else 0
+    assert _plan(**{name: ctypes.c_void_p(at) for name, at in place.items()}) == _lib.LEAFQ_ERR_INVALID
+    assert b"overlap" in _lib.load().leafq_last_error()
