@@ -120,10 +120,11 @@ class Kv8Plan:
     [requests + 1], ``table`` [requests, max_pages], and, from ``kv8_plan``,
     ``positions`` and ``slots`` [tokens] and ``taken``.  ``tokens`` and
     ``max_tokens`` are the host's bounds: the rows of the step, and any one
-    request's new tokens."""
+    request's new tokens; ``page``, where it is given, the tokens of a page,
+    which the cache's have to be."""
 
     def __init__(self, context, lengths, token_offsets, page_offsets, table, tokens: int, max_tokens: int,
-                 positions=None, slots=None, taken=None):
+                 positions=None, slots=None, taken=None, page: Optional[int] = None):
         _need(table.dim() == 2, "the block table must be [requests, max_pages]")
         requests, device = table.shape[0], table.device
         _check_i32(table, "the block table")
@@ -136,7 +137,7 @@ class Kv8Plan:
         self.token_offsets, self.page_offsets = token_offsets, page_offsets
         self.positions, self.slots, self.taken = positions, slots, taken
         self.requests, self.tokens, self.max_tokens, self.device = requests, int(tokens), int(max_tokens), device
-        self.index = device.index
+        self.index, self.page = device.index, page
         self.inputs = self.outputs = None  # addresses, of a plan that kv8_plan made
         self.desc = _lib.Kv8StepDesc(context.data_ptr(), lengths.data_ptr(), token_offsets.data_ptr(),
                                      page_offsets.data_ptr(), table.data_ptr(), table.shape[1], self.tokens,
@@ -212,6 +213,7 @@ def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tenso
     _check_i32(taken, "taken", 1, plan.index)
     _enqueue(plan.index, load().leafq_kv8_plan, plan.inputs[0], new_tokens.data_ptr(), requests, plan.inputs[1],
              plan.inputs[2], free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(), page, tokens, *plan.outputs, flags)
+    plan.page = page
     return plan
 
 
@@ -257,6 +259,8 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float,
         _fail("q has other rows than the plan")
     if plan.index != index:
         _fail("the plan is on another device")
+    if plan.page is not None and plan.page != cache.page:
+        _fail(f"the plan has pages of {plan.page} tokens, the cache of {cache.page}")
     if out is None:
         out = torch.empty_like(q)  # contiguous, as q's rows do not overlap
     elif not (out.get_device() == index and out.dtype is _F32 and out.is_contiguous() and out.shape == shape):

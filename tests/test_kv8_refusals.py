@@ -221,3 +221,31 @@ def test_plan_rejects_outputs_that_overlap_its_inputs(output, given):
     place[output] -= place[output] % 16 if output in ("positions", "slots") else 0
     assert _plan(**{name: ctypes.c_void_p(at) for name, at in place.items()}) == _lib.LEAFQ_ERR_INVALID
     assert b"overlap" in _lib.load().leafq_last_error()
+
+
+def test_attention_refuses_a_plan_of_other_pages(monkeypatch):
+    host = _Host(monkeypatch)
+    host.plan.page = 64
+    with pytest.raises(lq.LeafError, match="pages of 64 tokens, the cache of 16"):
+        lq.kv8_attention(host.rows, host.cache, host.plan, 1.0)
+    assert not host.calls
+    for page in (16, None):  # None: a plan that its caller made and did not say
+        host.plan.page = page
+        lq.kv8_attention(host.rows, host.cache, host.plan, 1.0)
+    assert len(host.calls) == 2
+
+
+@pytest.mark.gpu
+def test_plan_remembers_its_pages(cuda_device):
+    i = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    context, table, free = i(2), i(2, 8), torch.arange(16, dtype=torch.int32, device="cuda")
+    plan = lq.kv8_plan(context, i(2) + 20, table, free, i(1), 16, 40, max_tokens=20)
+    assert plan.page == 16
+    cache, q = lq.Kv8Cache.empty(16, 1, 64, 32), torch.zeros((40, 32), device="cuda")
+    with pytest.raises(lq.LeafError, match="pages of 16 tokens"):
+        lq.kv8_attention(q, cache, plan, 1.0)
+    assert lq.kv8_plan(context, i(2) + 20, table, free, i(1), 64, 40, max_tokens=20, out=plan).page == 64
+    rows = torch.ones((40, 32), device="cuda")
+    lq.kv8_append(rows, rows, cache, plan.slots)
+    assert torch.equal(lq.kv8_attention(q, cache, plan, 1.0), torch.ones_like(q))
+    assert lq.Kv8Plan(context, plan.lengths, plan.token_offsets, plan.page_offsets, table, 40, 20).page is None
