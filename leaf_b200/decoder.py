@@ -226,7 +226,7 @@ class Decoder:
         self.scale = float(np.float32(1.0) / np.sqrt(np.sqrt(np.float32(d))))
         self.position = torch.zeros(S, dtype=torch.int32, device=dev)
         self.error_flag = torch.zeros(1, dtype=torch.int32, device=dev)
-        self.length = 0
+        self.lengths = [0] * self.sequences
         self._buffers: dict[int, dict] = {}
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.token = torch.zeros(S, dtype=torch.int32, device=dev)
@@ -489,10 +489,18 @@ class Decoder:
         else:
             check(lib.leafq_advance_positions(s, self.position.data_ptr(), S, tokens))
 
+    @property
+    def length(self) -> int:
+        """Cached tokens of the longest sequence."""
+        return max(self.lengths)
+
+    def _grow(self, tokens: int) -> None:
+        self.lengths = [held + tokens for held in self.lengths]
+
     # ----------------------------------------------------------- public API
     def reset(self) -> None:
         """Decoder::reset: empty every KV cache."""
-        self.length = 0
+        self.lengths = [0] * self.sequences
         self.position.zero_()
         if self.kv8 is not None:
             self.taken.zero_()
@@ -513,7 +521,7 @@ class Decoder:
         b = self._bufs(len(ids))
         b["ids"].copy_(torch.tensor(ids, dtype=torch.int32))
         self._forward_device(b, len(ids))
-        self.length += len(ids)
+        self._grow(len(ids))
         return b["logits"]
 
     def _decode_step(self) -> None:
@@ -583,7 +591,7 @@ class Decoder:
                 produced = i
                 break
             self._decode_step()
-            self.length += 1
+            self._grow(1)
             out[i:i + 1].copy_(step["ids"])
         return [int(t) for t in out[:produced].tolist()]
 
@@ -598,7 +606,8 @@ class Decoder:
         tokens = max(len(p) for p in prompts)
         if any(len(p) == 0 for p in prompts) or (self.kv8 is None and any(len(p) != tokens for p in prompts)):
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "batched prompts must be non-empty and of equal length")
-        if self.length + tokens > min(self.cfg.max_positions, self.capacity):
+        lengths = [held + len(p) for held, p in zip(self.lengths, prompts)]
+        if max(lengths) > min(self.cfg.max_positions, self.capacity):
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "context length exceeds artifact limit")
         if any(i < 0 or i >= self.cfg.vocab for p in prompts for i in p):
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "token id exceeds vocabulary")
@@ -609,7 +618,7 @@ class Decoder:
             b["ids"][len(ids):].zero_()
             b["new"].copy_(torch.tensor([len(p) for p in prompts], dtype=torch.int32))
         self._forward_device(b, tokens)
-        self.length += tokens  # the longest sequence at most
+        self.lengths = lengths
         return b["logits"]
 
     def generate_batch(self, prompts, max_new: int) -> list[list[int]]:
@@ -621,8 +630,8 @@ class Decoder:
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "max_new must be positive")
         if not self._step_ready:
             self.capture_decode()
-        tokens = max((len(p) for p in prompts), default=0)
-        if self.length + tokens + max_new - 1 > min(self.cfg.max_positions, self.capacity):
+        longest = max((held + len(p) for held, p in zip(self.lengths, prompts)), default=0)
+        if longest + max_new - 1 > min(self.cfg.max_positions, self.capacity):
             raise LeafError(_lib.LEAFQ_ERR_INVALID, "context length exceeds artifact limit")
         logits = self.forward_batch(prompts)
         step = self._bufs(1)
@@ -633,7 +642,7 @@ class Decoder:
         for i in range(1, max_new):
             self._decode_step()
             out[i].copy_(step["ids"])
-        self.length += max_new - 1
+        self._grow(max_new - 1)
         eos = set(self.cfg.eos_tokens)
         result = []
         for seq in out.t().tolist():
@@ -719,7 +728,7 @@ class Decoder:
         self.history[n:n + 1].copy_(self.token)
         for _ in range(max_new - 1):
             self.step_fused()
-        self.length += max_new - 1
+        self._grow(max_new - 1)
         out = [int(t) for t in self.history[n:n + max_new].tolist()]
         eos = set(self.cfg.eos_tokens)
         for i, t in enumerate(out):

@@ -227,3 +227,26 @@ def test_refusals(cuda_device, tmp_path):
     assert not one.fused_supported()
     with pytest.raises(LeafError):
         one.generate_fused([1, 2, 3], 2)
+
+
+@pytest.mark.gpu
+def test_unlike_steps_fill_the_capacity(cuda_device, tmp_path):
+    # Two steps of 1 and 100 tokens the other way round hold 101 each, and leave room for the rest.
+    rng = np.random.default_rng(9)
+    dec = Decoder(_artifact(tmp_path), sequences=2, capacity=128, cache="int8", page=16)
+    for lengths in ((1, 100), (100, 1)):
+        dec.forward_batch([_prompt(rng, fx.TINY, n) for n in lengths])
+    assert dec.position.tolist() == [101, 101] and dec.length == 101
+    dec.forward_batch([_prompt(rng, fx.TINY, n) for n in (7, 2)])
+    with pytest.raises(LeafError):
+        dec.forward_batch([_prompt(rng, fx.TINY, n) for n in (21, 1)])  # the longer one is at 108
+    with pytest.raises(LeafError):
+        dec.generate_batch([_prompt(rng, fx.TINY, n) for n in (1, 18)], 21)
+    tokens = dec.generate_batch([_prompt(rng, fx.TINY, n) for n in (1, 18)], 8)
+    assert [len(t) for t in tokens] == [8, 8] and dec.position.tolist() == [116, 128] and dec.length == 128
+    with pytest.raises(LeafError):
+        dec.forward_batch([[1], [1]])
+    assert dec.device_status() == 0
+    dec.reset()
+    dec.forward_batch([_prompt(rng, fx.TINY, n) for n in (128, 1)])
+    assert dec.length == 128
