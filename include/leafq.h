@@ -493,8 +493,8 @@ int leafq_kv8_append(void* stream, const float* k, int64_t k_stride, const float
 
 /* Bytes of workspace leafq_kv8_attention needs for this geometry, 0 when it
  * needs none.  The workspace must be zeroed once before its first use; every
- * call leaves the words that need it zero again, in the same places for every
- * geometry, so that calls of all geometries may share one of the largest's
+ * call leaves the words that need it zero again (one whose wait ran out too), in the
+ * same places for every geometry, so that calls of all geometries may share one of the largest's
  * size.  Calls that overlap on the GPU need workspaces of their own. */
 size_t leafq_kv8_attention_workspace_bytes(int64_t max_tokens, int heads, int kv_heads, int dim);
 

@@ -500,9 +500,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 uint32_t before = 0;
                 if (lane == 0) {
                     __threadfence();
-                    uint32_t* arrived = arrivals + 4 * (place / splits) + warp;
-                    before = atomicAdd(arrived, 1u);
-                    if (before == static_cast<uint32_t>(count - 1)) *arrived = 0;
+                    before = atomicAdd(arrivals + 4 * (place / splits) + warp, 1u);
                     __threadfence();
                 }
                 there = __shfl_sync(~0u, before, 0) == static_cast<uint32_t>(count - 1);
@@ -928,10 +926,17 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         tcgen05_fence_after();
         tmem_dealloc(tmem, C::kTmemCols);
     }
-    // The last block leaves the counters as it found them.
-    if (tid == 0) {
-        __threadfence();
-        if (atomicAdd(taken + 1, 1u) == gridDim.x - 1) taken[0] = taken[1] = 0;
+    // The last block leaves the counters at zero, also where a wait has run out and parts
+    // have not arrived.
+    if (warp == 0) {
+        bool last = false;
+        if (lane == 0) {
+            __threadfence();
+            last = atomicAdd(taken + 1, 1u) == gridDim.x - 1;
+            if (last) taken[0] = taken[1] = 0;
+        }
+        if (kParts && __any_sync(~0u, last))
+            for (int i = lane; i < 4 * row_tiles * g.cache.kv_heads; i += 32) arrivals[i] = 0;
     }
 }
 

@@ -863,3 +863,18 @@ def test_attention_rows_are_clear_of_pages_that_they_do_not_see(cuda_device, new
     if not (which == "k" and value == float("inf")):  # (a score of minus infinity weighs nothing)
         assert not torch.isfinite(got[sees]).any()
     b.check(torch.where(sees, clean, got))
+
+
+def test_attention_leaves_its_counters_zero_whatever_it_finds(cuda_device):
+    # A call that gave up a wait leaves parts that never arrived: the next one's result is its own again.
+    rng = np.random.default_rng(39)
+    b = _Batch(rng, [3000], [256], 64, 2, 8, 64, rotary=64)  # 17 row tiles of 2 heads, cut along their keys
+    workspace = lq.Kv8Workspace()
+    b.check(b.run(workspace=workspace))
+    assert _no_counter_left(workspace)
+    arrivals = workspace.buffer.view(torch.int32)[2560 + 4:][:4 * 17 * 2]
+    for words in (arrivals[:8], arrivals):  # of heads past the last row; of all
+        words.fill_(1)
+        b.run(workspace=workspace)
+        assert _no_counter_left(workspace)
+        b.check(b.run(workspace=workspace))
