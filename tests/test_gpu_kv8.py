@@ -878,3 +878,28 @@ def test_attention_leaves_its_counters_zero_whatever_it_finds(cuda_device):
         b.run(workspace=workspace)
         assert _no_counter_left(workspace)
         b.check(b.run(workspace=workspace))
+
+
+@pytest.mark.parametrize("context,new", [([700, 12, 3000], [1, 1, 1]), ([100, 0, 2000], [90, 140, 300])])
+def test_step_without_early_launch_gives_the_same_bits(cuda_device, context, new):
+    # Plan, append and attention with and without LEAFQ_FLAG_PDL, over the same cache.
+    rng = np.random.default_rng(40)
+    results = []
+    for flags in (_lib.LEAFQ_FLAG_PDL, 0):
+        rng = np.random.default_rng(40)
+        b = _Batch(rng, context, new, 16, 4, 8, 64, rotary=64)
+        free = _i32(np.concatenate([b.unused, np.arange(b.pool, b.pool + 4)]))
+        table = _i32(np.where(np.arange(b.table.shape[1]) < np.array([[ok.pages_of(c, 16)] for c in context]), b.table, -1))
+        # Pages of the new tokens: what the batch holds for them, in request order.
+        fresh = np.concatenate([b.table[s, ok.pages_of(c, 16):ok.pages_of(c + n, 16)] for s, (c, n) in enumerate(zip(context, new))])
+        plan = lq.kv8_plan(_i32(context), _i32(new), table, torch.cat((_i32(fresh), free)), _i32([0]), 16, b.tokens,
+                           max_tokens=max(new), flags=flags)
+        rows = [torch.from_numpy(rng.standard_normal((b.tokens, 4 * 64)).astype(np.float32)).cuda() for _ in range(2)]
+        rope = _rope_cuda(b.rope)
+        lq.kv8_append(*rows, b.cache, plan.slots, plan.positions, rope=rope, flags=flags)
+        out = lq.kv8_attention(torch.from_numpy(b.q).cuda(), b.cache, plan, b.scale, rope=rope, flags=flags)
+        held = _i32(np.unique(b.table[b.table >= 0])).long()
+        results.append([plan.slots, plan.lengths, b.cache.k[held], b.cache.v_scale[held], out])
+        assert torch.equal(table, _i32(b.table)) and torch.isfinite(out).all()
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+    assert _status_ok()
