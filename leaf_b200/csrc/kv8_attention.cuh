@@ -33,11 +33,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLift = 6.0f, kHighest = 24576.0f;
 // A page's weights carry its V scale's exponent, which their sum takes out again: as
 // a factor of up to 2^90, so that the sum of 2^17 keys' weights stays below 2^127.
-// Smaller scales count as zero.  The weights of such a page count in the sum as at a
-// scale of 2^-63, which stands in reach (2^126) of the others of a cache, and below
-// those that an append gives.
+// Smaller scales count as zero.
 constexpr float kLeastScale = 0x1p-90f;
-constexpr float kZeroExponent = -63.0f, kZeroInverse = 0x1p63f;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

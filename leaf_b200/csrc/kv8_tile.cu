@@ -4,6 +4,7 @@
 // device code.
 #define LEAFQ_WHOLE_PROGRAM
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "kv8_attention.cuh"
@@ -42,6 +43,18 @@ namespace {
 // operands are two halves); one of 8,192 tokens 619 us (444 TFLOP/s).  5 chunks
 // of 100 to 1,500 tokens, 8 heads of 128, 3 queries a key, 83 us (250 TFLOP/s).
 constexpr float kTileLift = 6.0f, kTileHighest = 49152.0f;
+// Two kinds of pages are told apart without a test in the softmax (one a tile took 2 %
+// of the time), by their V scale's logarithm.  Values of zero count in L as any other:
+// as of scale 2^kZeroLog2, with a reference that stands kZeroAbove over their scores (below
+// those of the scales that an append gives), which leaves their weights at 2^-37, zeros
+// in fp16.  (Where later scores are 2^12 times as heavy, and no other page's raise the
+// reference, they come through as values below 2^-76.)  Scales that are no numbers:
+// every key that a row sees weighs one, the reference is out of all others' reach, and L
+// passes kNoNumber; a row that sees none of them keeps its own.
+constexpr float kZeroLog2 = -83.0f, kZeroInverse = 0x1p83f, kZeroAbove = 43.0f;
+constexpr float kNoNumberLog2 = 1e30f, kNoNumber = 3e38f;
+// 1 / L: none for a row that sees no key, and for one that sees a scale that is no number.
+__device__ __forceinline__ float inverse_of(float l) { return l == 0.0f ? 0.0f : l > kNoNumber ? NAN : __frcp_rn(l); }
 
 // Where there are fewer items than half the blocks, each is cut into parts along
 // the keys, of kPartTiles tiles or more; the last part to end joins them.
@@ -80,7 +93,7 @@ struct TileShape {
     static constexpr int kOutCols = kBlocks * 64;        // O columns (those past D are not read)
     static constexpr uint32_t kTmemCols = 256;
     static constexpr size_t kSmem = kQSlots * 2 * kQBytes + (kKStages + kVStages) * kKvBytes + kInfo * kGroups * 16 +
-                                    kItems * sizeof(TileItem) + kQSlots * kRows + (2 * kKStages + 2 * kVStages + 2 * kQSlots + kItems + 7) * 8 + 16;
+                                    kItems * sizeof(TileItem) + kQSlots * kRows + (2 * kKStages + 2 * kVStages + 2 * kQSlots + kItems + 7) * 8 + 8;
     static_assert(kQSlots == 1 || kRows * D * 4 <= 2 * kQBytes, "the output goes through the place of the item's rows");
     static constexpr int kPart = kRows * (D + 2);        // floats of a part's result: O [D / 4][128][4], m [128], l [128]
     static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two blocks share the SM's shared memory");
@@ -139,9 +152,6 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
-__device__ __forceinline__ void tmem_zero_x8(uint32_t taddr) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1};" ::"r"(taddr), "r"(0) : "memory");
-}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Loads of read-only data that stay where they are written, ahead of their use.
@@ -189,7 +199,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
     uint8_t* q_rows = smem;  // [kQSlots]: hi, lo
     uint8_t* k_tiles = q_rows + C::kQSlots * 2 * C::kQBytes;
     uint8_t* v_tiles = k_tiles + C::kKStages * C::kKvBytes;
-    float4* info = reinterpret_cast<float4*>(v_tiles + C::kVStages * C::kKvBytes);  // [kInfo][kGroups]: ks, log2 vs, 1 / vs, 1: vs counts as zero, 2: they are no numbers
+    float4* info = reinterpret_cast<float4*>(v_tiles + C::kVStages * C::kKvBytes);  // [kInfo][kGroups]: ks, log2 vs, 1 / vs, what the reference stands higher
     TileItem* items = reinterpret_cast<TileItem*>(info + C::kInfo * C::kGroups);
     uint8_t* power = reinterpret_cast<uint8_t*>(items + C::kItems);  // [kQSlots][128]: of two, that a row was scaled down by (exponent bits)
     uint64_t* k_full = reinterpret_cast<uint64_t*>(power + C::kQSlots * C::kRows);
@@ -205,7 +215,6 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
     uint64_t* item_done = o_done + 1;            // all its MMAs have completed
     uint64_t* drained = item_done + 1;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
-    int* marked = reinterpret_cast<int*>(tmem_holder + 2);  // the last tile so far that has such a group
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kMmaWarp = 8;
     const auto token_of = [&](int row) { return static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(g.group)); };
@@ -236,7 +245,6 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             mbar_init(o_done, 1);
             mbar_init(item_done, 1);
             mbar_init(drained, 1);
-            *marked = -1;
             fence_barrier_init();
         }
         __syncwarp();
@@ -315,7 +323,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
 #pragma unroll
                         for (int e = 1; e < 16; ++e) most = fmaxf(most, at[e]);
                         const float4 scale = scales[2 * c + half];
-                        top = fmaxf(top, fmaf(most, slope(scale.x), scale.y));
+                        top = fmaxf(top, fmaf(most, slope(scale.x), scale.y + scale.w));
                     }
                     return top;
                 };
@@ -411,21 +419,6 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     tmem_st_32x32b_x32(s_tmem + lanes + 32 * c, p);
                 }
                 if (!ok) break;
-                if (*marked >= n) {  // this tile, or one soon
-                    // Values of zero: their weights count in L alone.  Scales that are no numbers: nor is
-                    // the output of a row that sees them.  (Apart from the loop above, which it would
-                    // slow by 7 %, as a vote over the groups would the conversion.)
-                    tmem_wait_st();
-#pragma unroll 1
-                    for (int i = 0; i < C::kGroups; ++i) {
-                        const float kind = scales[i].w;
-                        if (kind == 2.0f && visible > 16 * i) l = NAN;
-                        if (kind != 1.0f) continue;
-                        const uint32_t at = s_tmem + lanes + 32 * (i >> 1) + 8 * (i & 1);  // the hi pairs
-                        tmem_zero_x8(at);
-                        tmem_zero_x8(at + 16);
-                    }
-                }
                 if (anew && j > 0) {
                     // Adds O, complete up to the tile before, to the rounded sum.
                     ok = __all_sync(~0u, tile_wait(watch, o_done, (n - 1) & 1));
@@ -461,7 +454,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             // sees no key.  A part of an item leaves O, m and l instead.
             const bool summed = tiles > C::kSpan, whole_item = !kParts || count == 1;
             const float old = !summed || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m);
-            const float inverse = !whole_item ? 1.0f : l == 0.0f ? 0.0f : __frcp_rn(l);
+            const float inverse = !whole_item ? 1.0f : inverse_of(l);
             float* own = parts + (int64_t)(place + part_index) * C::kPart;
             // Where there is room beside the next item's rows, whole rows are stored, by
             // way of the place of this item's; permuted so that a row's pieces lie in
@@ -523,7 +516,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                             put_sum(c, make_float4(fmaf(weight, v.x, z.x), fmaf(weight, v.y, z.y), fmaf(weight, v.z, z.z), fmaf(weight, v.w, z.w)));
                         }
                     }
-                    const float over = total == 0.0f ? 0.0f : __frcp_rn(total);
+                    const float over = inverse_of(total);
 #pragma unroll 4
                     for (int c = 0; c < D / 4; ++c) {
                         float4 y = get_sum(c);
@@ -828,11 +821,8 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                         const float a = lg2(vs), back = ex2(-a), d = fmaf(vs, back, -1.0f);
                         f = make_float4(ks, fmaf(d, kLog2e, a), fmaf(-d, back, back), 0.0f);
                     } else if (!(vs < 0.0f)) {
-                        // A page of zeros counts in the sum as any other.  Scales that are no numbers
-                        // would reach rows that do not see the group: they are shown to those that do.
-                        const bool zero = vs < kLeastScale && !isnan(ks);
-                        f = make_float4(zero ? ks : 0.0f, kZeroExponent, kZeroInverse, zero ? 1.0f : 2.0f);
-                        *marked = tile;
+                        f = vs < kLeastScale && !isnan(ks) ? make_float4(ks, kZeroLog2, kZeroInverse, kZeroAbove)
+                                                           : make_float4(0.0f, kNoNumberLog2, FLT_MAX, 0.0f);
                     }
                     info[(tile % C::kInfo) * C::kGroups + ct] = f;
                 }
@@ -926,17 +916,13 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         tcgen05_fence_after();
         tmem_dealloc(tmem, C::kTmemCols);
     }
-    // The last block leaves the counters at zero, also where a wait has run out and parts
-    // have not arrived.
-    if (warp == 0) {
-        bool last = false;
-        if (lane == 0) {
-            __threadfence();
-            last = atomicAdd(taken + 1, 1u) == gridDim.x - 1;
-            if (last) taken[0] = taken[1] = 0;
+    if (tid == 0) {
+        __threadfence();
+        if (atomicAdd(taken + 1, 1u) == gridDim.x - 1) {
+            taken[0] = taken[1] = 0;
+            if (kParts)
+                for (int i = 0; i < row_tiles * g.cache.kv_heads; ++i) reinterpret_cast<uint4*>(arrivals)[i] = make_uint4(0, 0, 0, 0);
         }
-        if (kParts && __any_sync(~0u, last))
-            for (int i = lane; i < 4 * row_tiles * g.cache.kv_heads; i += 32) arrivals[i] = 0;
     }
 }
 
