@@ -507,9 +507,9 @@ size_t leafq_kv8_attention_workspace_bytes(int64_t max_tokens, int heads, int kv
  * gives zeros.  heads is a multiple of the cache's kv_heads; out [tokens]
  * [heads * dim]; rows past the last new token are not written, a request's
  * rows past max_tokens may be left out.  The cache's scales must not be negative;
- * a V scale below 2^-90 (8e-28) counts as zero (values below 1e-22 may come
- * through), and V scales that a row sees are to be below 2^126 and to lie within a
- * factor of 2^110 of one another (a zero counting as 2^-83).  Scales that are no numbers show in the rows that see their
+ * a V scale below 2^-82 (2e-25) may count as zero, one of zero may let values of
+ * up to 1e-22 through, and V scales that a row sees are to be below 2^126 and to lie
+ * within a factor of 2^110 of one another (a zero counting as 2^-83).  Scales that are no numbers show in the rows that see their
  * page only.  A table entry outside the pool hides its keys and a position outside the tables
  * empties its row; leafq_device_status reports both.  Equal calls give equal
  * bits.  With many rows (prompts) a pool's codes have to stay below 64 GiB

@@ -43,14 +43,14 @@ namespace {
 // operands are two halves); one of 8,192 tokens 619 us (444 TFLOP/s).  5 chunks
 // of 100 to 1,500 tokens, 8 heads of 128, 3 queries a key, 83 us (250 TFLOP/s).
 constexpr float kTileLift = 6.0f, kTileHighest = 49152.0f;
-// Two kinds of pages are told apart without a test in the softmax (one a tile took 2 %
-// of the time), by their V scale's logarithm.  Values of zero count in L as any other:
-// as of scale 2^kZeroLog2, with a reference that stands kZeroAbove over their scores (below
-// those of the scales that an append gives), which leaves their weights at 2^-37, zeros
-// in fp16.  (Where later scores are 2^12 times as heavy, and no other page's raise the
-// reference, they come through as values below 2^-76.)  Scales that are no numbers:
-// every key that a row sees weighs one, the reference is out of all others' reach, and L
-// passes kNoNumber; a row that sees none of them keeps its own.
+// Two kinds of pages need no test in the softmax (one a tile took 2 % of the time): what
+// stands for their V scale does it.  Values of zero count in L as any other, as of scale
+// 2^kZeroLog2, with a reference that stands kZeroAbove over their scores (below those of
+// the scales that an append gives), which leaves their weights at 2^-37, zeros in fp16.
+// (Where later scores are 2^12 times as heavy, and no other page's raise the reference,
+// they come through as values below 2^-76.)  Scales that are no numbers: every key that
+// a row sees weighs one, the reference is out of all others' reach, and L passes
+// kNoNumber; a row that sees none of them keeps its own.
 constexpr float kZeroLog2 = -83.0f, kZeroInverse = 0x1p83f, kZeroAbove = 43.0f;
 constexpr float kNoNumberLog2 = 1e30f, kNoNumber = 3e38f;
 // 1 / L: none for a row that sees no key, and for one that sees a scale that is no number.
@@ -199,7 +199,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
     uint8_t* q_rows = smem;  // [kQSlots]: hi, lo
     uint8_t* k_tiles = q_rows + C::kQSlots * 2 * C::kQBytes;
     uint8_t* v_tiles = k_tiles + C::kKStages * C::kKvBytes;
-    float4* info = reinterpret_cast<float4*>(v_tiles + C::kVStages * C::kKvBytes);  // [kInfo][kGroups]: ks, log2 vs, 1 / vs, what the reference stands higher
+    float4* info = reinterpret_cast<float4*>(v_tiles + C::kVStages * C::kKvBytes);  // [kInfo][kGroups]: ks, log2 vs, 1 / vs
     TileItem* items = reinterpret_cast<TileItem*>(info + C::kInfo * C::kGroups);
     uint8_t* power = reinterpret_cast<uint8_t*>(items + C::kItems);  // [kQSlots][128]: of two, that a row was scaled down by (exponent bits)
     uint64_t* k_full = reinterpret_cast<uint64_t*>(power + C::kQSlots * C::kRows);
@@ -323,7 +323,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
 #pragma unroll
                         for (int e = 1; e < 16; ++e) most = fmaxf(most, at[e]);
                         const float4 scale = scales[2 * c + half];
-                        top = fmaxf(top, fmaf(most, slope(scale.x), scale.y + scale.w));
+                        top = fmaxf(top, fmaf(most, slope(scale.x), scale.z == kZeroInverse ? kZeroLog2 + kZeroAbove : scale.y));
                     }
                     return top;
                 };
@@ -821,7 +821,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                         const float a = lg2(vs), back = ex2(-a), d = fmaf(vs, back, -1.0f);
                         f = make_float4(ks, fmaf(d, kLog2e, a), fmaf(-d, back, back), 0.0f);
                     } else if (!(vs < 0.0f)) {
-                        f = vs < kLeastScale && !isnan(ks) ? make_float4(ks, kZeroLog2, kZeroInverse, kZeroAbove)
+                        f = vs < kLeastScale && !isnan(ks) ? make_float4(ks, kZeroLog2, kZeroInverse, 0.0f)
                                                            : make_float4(0.0f, kNoNumberLog2, FLT_MAX, 0.0f);
                     }
                     info[(tile % C::kInfo) * C::kGroups + ct] = f;
