@@ -38,19 +38,10 @@ def _need(ok: bool, message: str) -> None:
         _fail(message)
 
 
-def _enqueue(index: int, function, *args) -> None:
-    """A C call on the current stream of the tensors' device `index`.  The
-    library launches on the current device, so the call is made with that one
-    current."""
-    if _current_device() == index:
-        check(function(_raw_stream(index), *args))
-    else:
-        with torch.cuda.device(index):
-            check(function(_raw_stream(index), *args))
-
-
 # The calls sit in a decode loop, a few microseconds each: the checks below ask
-# each tensor as little as they can and build their messages only to fail.
+# each tensor as little as they can and build their messages only to fail.  The
+# library launches on the current device: a call whose tensors are on another
+# is made again with that one current.
 # index: of the CUDA device they have to be on (a tensor elsewhere has -1).
 def _check_i32(t: torch.Tensor, name: str, numel: Optional[int] = None, index: Optional[int] = None) -> None:
     if not (t.dtype is _I32 and t.is_contiguous() and (t.is_cuda if index is None else t.get_device() == index)):
@@ -187,9 +178,13 @@ def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tenso
     lengths[s] == context[s].  tokens: the step's rows, at least the sum of
     new_tokens (the rest get slot -1); max_tokens: a bound on any request's new
     tokens (default: tokens).  ``taken`` is only read, the new count is the
-    plan's ``taken`` (copy it back for the next step: a plan's own outputs are no
-    inputs of its next filling).  ``out``: a plan of the same buffers and rows, which is
+    plan's ``taken`` (copy it back for the next step: outputs that overlap the
+    inputs are refused).  ``out``: a plan of the same buffers and rows, which is
     filled again; max_tokens may be another."""
+    index = context.get_device() if out is None else out.index
+    if index >= 0 and _current_device() != index:
+        with torch.cuda.device(index):
+            return kv8_plan(context, new_tokens, table, free_pages, taken, page, tokens, max_tokens, out, flags)
     requests = context.numel()
     most = tokens if max_tokens is None else max_tokens
     if out is not None and out.context is context and out.table is table and out.tokens == tokens and out.inputs is not None:
@@ -211,8 +206,9 @@ def kv8_plan(context: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tenso
     _check_i32(new_tokens, "new_tokens", requests, plan.index)
     _check_i32(free_pages, "free_pages", None, plan.index)
     _check_i32(taken, "taken", 1, plan.index)
-    _enqueue(plan.index, load().leafq_kv8_plan, plan.inputs[0], new_tokens.data_ptr(), requests, plan.inputs[1],
-             plan.inputs[2], free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(), page, tokens, *plan.outputs, flags)
+    check(load().leafq_kv8_plan(_raw_stream(plan.index), plan.inputs[0], new_tokens.data_ptr(), requests, plan.inputs[1],
+                                plan.inputs[2], free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(), page, tokens,
+                                *plan.outputs, flags))
     plan.page = page
     return plan
 
@@ -225,6 +221,9 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: Kv8Cache, slots: torch.T
     rotated by ``positions`` first.  A page's scale grows when a new row needs
     it, and its older codes are rounded to the new scale."""
     index = cache.index
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return kv8_append(k, v, cache, slots, positions, rope, flags)
     k_stride = _check_rows(k, "k", cache.width, index)
     v_stride = _check_rows(v, "v", cache.width, index)
     tokens = k.shape[0]
@@ -238,8 +237,8 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: Kv8Cache, slots: torch.T
             _fail("rotation needs positions")
         _check_i32(positions, "positions", tokens, index)
         where = positions.data_ptr()
-    _enqueue(index, load().leafq_kv8_append, k.data_ptr(), k_stride, v.data_ptr(), v_stride, tokens, where,
-             slots.data_ptr(), rotary, cos, sin, rows, cache.ref, flags)
+    check(load().leafq_kv8_append(_raw_stream(index), k.data_ptr(), k_stride, v.data_ptr(), v_stride, tokens, where,
+                                  slots.data_ptr(), rotary, cos, sin, rows, cache.ref, flags))
 
 
 def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float, rope=None,
@@ -251,6 +250,9 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float,
     [tokens, heads * dim]; a row that sees no key is zero, rows past the step's
     last new token are not written."""
     index, dim, shape = cache.index, cache.dim, q.shape
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return kv8_attention(q, cache, plan, scale, rope, out, workspace, flags)
     if len(shape) != 2 or shape[1] % dim != 0:
         _fail("q must be [tokens, heads * dim]")
     tokens, width = shape
@@ -272,6 +274,6 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float,
     elif workspace.index != index:
         _fail("the workspace is on another device")
     address, need = workspace.of(plan.max_tokens, heads, cache.kv_heads, dim)
-    _enqueue(index, load().leafq_kv8_attention, q.data_ptr(), stride, heads, rotary, cos, sin, rows, cache.ref, plan.ref,
-             scale, out.data_ptr(), address, need, flags)
+    check(load().leafq_kv8_attention(_raw_stream(index), q.data_ptr(), stride, heads, rotary, cos, sin, rows, cache.ref,
+                                     plan.ref, scale, out.data_ptr(), address, need, flags))
     return out
