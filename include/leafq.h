@@ -465,7 +465,7 @@ typedef struct leafq_kv8_step {
  * pages, its tokens get slot -1 and lengths[s] = context[s].  Rows of
  * positions / slots past the last new token get 0 / -1; more new tokens than
  * `tokens`, or a negative length, is reported by leafq_device_status.
- * Outputs other than table must not overlap the inputs. */
+ * Outputs that overlap the inputs (table excepted) are refused. */
 int leafq_kv8_plan(void* stream, const int32_t* context, const int32_t* new_tokens, int requests, int32_t* table,
                    int64_t max_pages, const int32_t* free_pages, int64_t free_count, const int32_t* taken, int page,
                    int64_t tokens, int32_t* lengths, int32_t* token_offsets, int32_t* page_offsets,
@@ -503,17 +503,24 @@ size_t leafq_kv8_attention_workspace_bytes(int64_t max_tokens, int heads, int kv
  * when tables are given; the query of new token t of request s is at position
  * context[s] + t and sees the keys j < min(position + 1, lengths[s]):
  *   out = sum_j softmax_j(scale * q . key_j) value_j,
- * fp32 throughout (sums, softmax statistics, output), a row that sees no key
- * gives zeros.  heads is a multiple of the cache's kv_heads; out [tokens]
- * [heads * dim]; rows past the last new token are not written, a request's
- * rows past max_tokens may be left out.  The cache's scales must not be negative;
- * a V scale below 2^-82 (2e-25) may count as zero, one of zero may let values of
- * up to 1e-22 through, and V scales that a row sees are to be below 2^126 and to lie
- * within a factor of 2^110 of one another (a zero counting as 2^-83).  Scales that are no numbers show in the rows that see their
- * page only.  A table entry outside the pool hides its keys and a position outside the tables
- * empties its row; leafq_device_status reports both.  Equal calls give equal
- * bits.  With many rows (prompts) a pool's codes have to stay below 64 GiB
- * each and tokens * heads / kv_heads within int32. */
+ * with sums, softmax statistics and output in fp32; a row that sees no key gives
+ * zeros.  heads is a multiple of the cache's kv_heads; out [tokens][heads * dim];
+ * rows past the last new token are not written, a request's rows past max_tokens
+ * may be left out.  A table entry outside the pool hides its keys and a position
+ * outside the tables empties its row; leafq_device_status reports both.  Equal
+ * calls give equal bits.  With many rows (prompts) a pool's codes have to stay
+ * below 64 GiB each and tokens * heads / kv_heads within int32.
+ *
+ * The products take queries and weights to 22 significand bits (two fp16 halves;
+ * fewer for elements below 2^-11 of their row's largest) and sum up to 512 keys
+ * with truncation: the result is within about 1e-6 of its size.  Steps of few and
+ * of many rows run different kernels, whose results differ by as much.
+ *
+ * Scales must not be negative.  A V scale below 2^-82 (2e-25) may count as zero,
+ * one of zero may let values of up to 1e-22 through, and V scales that a row sees
+ * are to be below 2^126 and within a factor of 2^110 of one another (a zero
+ * counting as 2^-83).  Scales that are no numbers show in the rows that see their
+ * page, and in no others. */
 int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int heads, int rotary_dim,
                         const float* cos_table, const float* sin_table, int64_t table_rows,
                         const leafq_kv8_cache* cache, const leafq_kv8_step* step, float scale, float* out,

@@ -49,7 +49,7 @@ __device__ __forceinline__ void wait_async_copies_but() {
 //   2t+9 are keys t, 4+t, 8+t, 12+t, which makes the V reads conflict-free.
 // A V scale vs = f 2^e goes half into the exponent, half into the weight:
 // u_j = 2^(x_j + e - M) with M a reference near the maximum of x_j + e; O sums
-// f u_j cv_j and L sums u_j 2^-e, so O / L is the softmax average whatever the
+// f u_j cv_j and L sums u_j 2^-e, so O / L is the softmax average over 2^110 of the
 // scales' range, and neither half rounds.
 //
 // The codes are read once, by 16-byte asynchronous copies into a ring per warp,
@@ -63,9 +63,9 @@ __device__ __forceinline__ void wait_async_copies_but() {
 // codes of K and V) about alike.  6 requests of 15,000 to 91,000 tokens, 8 heads
 // of 128, 468 MB: 104 us (4.5 TB/s); the copies alone take 98 us, the arithmetic
 // alone 90 us.  For short ones the round trips: 64 requests of 521 to 765 tokens,
-// 4 heads of 64, 21.6 MB, take 13.6 us, of which 6 us pass before the first
+// 4 heads of 64, 21.6 MB, take 13.4 us, of which 6 us pass before the first
 // chunk is there, 4 us in the key loop and 1 us in joining the warps; one request
-// of 200 tokens takes 5.5 us.  Four warps a block at 64-wide heads took 19.2 us
+// of 200 tokens takes 5.6 us.  Four warps a block at 64-wide heads took 19.2 us
 // instead of 13.5, three blocks of eight warps (80 registers, spilling) 21.8.
 //
 // kNarrow: blocks of two warps, four or three times as many, for more heads than
@@ -752,7 +752,10 @@ int run_split(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl)
 // tile form, us: 2,048 rows of 8 requests 74 and 84 (172 and 122), 4,096 rows 134
 // and 85 (294 and 122), 8,192 rows 384 and 99 (569 and 157); with 1,000 cached
 // tokens 2,048 rows 16 and 31 (33 and 42), 4,096 rows 35 and 31 (65 and 44).  Over
-// 520 shapes of 256 to 64,000 rows this rule is 1 to 3 % above the better form.
+// 520 shapes of 256 to 64,000 rows this rule is 1 to 3 % above the better form; in
+// all of them the requests bring equally many tokens to equally long caches.  A batch
+// takes one form: one-token requests beside a prompt's chunk go to the tiles with it,
+// which is right but was not measured.
 constexpr int kTileRows = 32;
 bool takes_tiles(int64_t tokens, int64_t max_tokens, int heads, int group) {
     return max_tokens * group >= kTileRows && tokens * heads >= 3584;

@@ -39,9 +39,9 @@ namespace {
 // time): about a third go to the softmax (5 to 6 instructions a score), a fifth
 // to rotating and splitting query rows, a sixth to the codes' conversion; the
 // rest waits on hand-offs between the roles.  4 heads of 64, 8 queries a key: 64
-// prompts of 512 tokens 362 us (190 TFLOP/s, twice that in the MMAs, since fp32
-// operands are two halves); one of 8,192 tokens 619 us (444 TFLOP/s).  5 chunks
-// of 100 to 1,500 tokens, 8 heads of 128, 3 queries a key, 83 us (250 TFLOP/s).
+// prompts of 512 tokens 360 us (191 TFLOP/s, twice that in the MMAs, since fp32
+// operands are two halves); one of 8,192 tokens 612 us (449 TFLOP/s).  5 chunks
+// of 100 to 1,500 tokens, 8 heads of 128, 3 queries a key, 83 us (252 TFLOP/s).
 constexpr float kTileLift = 6.0f, kTileHighest = 49152.0f;
 // Two kinds of pages need no test in the softmax (one a tile took 2 % of the time): what
 // stands for their V scale does it.  Values of zero count in L as any other, as of scale
