@@ -35,7 +35,7 @@ namespace {
 // kSpan tiles O is added to a rounded sum (in local memory) and starts anew -- and
 // the lo halves of Q go first, while S is small.
 //
-// Bound: issue slots, of which 58 % are used (the tensor pipe is busy 21 % of the
+// Bound: issue slots, of which 57 % are used (the tensor pipe is busy 21 % of the
 // time): about a third go to the softmax (5 to 6 instructions a score), a fifth
 // to rotating and splitting query rows, a sixth to the codes' conversion; the
 // rest waits on hand-offs between the roles.  4 heads of 64, 8 queries a key: 64
