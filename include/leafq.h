@@ -519,7 +519,8 @@ size_t leafq_kv8_attention_workspace_bytes(int64_t max_tokens, int heads, int kv
  * Scales must not be negative.  A V scale below 2^-82 (2e-25) may count as zero,
  * one of zero may let values of up to 1e-22 through, and V scales that a row sees
  * are to be below 2^126 and within a factor of 2^110 of one another (a zero
- * counting as 2^-83).  Scales that are no numbers show in the rows that see their
+ * counting as 2^-83); beside pages of zeros, those below an append's least (1e-12)
+ * keep fewer bits.  Scales that are no numbers show in the rows that see their
  * page, and in no others. */
 int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int heads, int rotary_dim,
                         const float* cos_table, const float* sin_table, int64_t table_rows,

@@ -916,6 +916,9 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         tcgen05_fence_after();
         tmem_dealloc(tmem, C::kTmemCols);
     }
+    // The last block leaves the counters at zero, those of the parts also where a wait has
+    // run out and some have not arrived.  (By one thread: with all of them, behind a
+    // barrier, 256 rows over 8,000 keys took 110 us instead of 104.)
     if (tid == 0) {
         __threadfence();
         if (atomicAdd(taken + 1, 1u) == gridDim.x - 1) {

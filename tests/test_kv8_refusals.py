@@ -8,7 +8,8 @@ import pytest
 import torch
 
 import leaf_b200 as lq
-from leaf_b200 import _lib, kv8
+from leaf_b200 import _lib
+from leaf_b200 import kv8
 
 P = ctypes.c_void_p(256)
 ODD = ctypes.c_void_p(264)
