@@ -482,11 +482,10 @@ def _plain_keep(s):
     column = torch.arange(s["dropped"], device=DEVICE)
     drops = column < freed[:, None]
     source = table.gather(1, (after[:, None] + column).clamp(max=table.shape[1] - 1))
-    taken = s["taken"].long() - upto[-1]
-    place = taken + (upto - freed)[:, None] + column
+    place = (s["taken"].long() - upto)[:, None] + column  # each request's pages below those of the one before
     free = s["free"]
     free[place[drops]] = source[drops].to(torch.int32)
-    return dict(_read(s), free=free, lengths=left.to(torch.int32), taken=taken.to(torch.int32))
+    return dict(_read(s), free=free, lengths=left.to(torch.int32), taken=(s["taken"].long() - upto[-1]).to(torch.int32))
 
 
 def _read(s):
