@@ -527,6 +527,106 @@ int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int head
                         const leafq_kv8_cache* cache, const leafq_kv8_step* step, float scale, float* out,
                         void* workspace, size_t workspace_bytes, uint32_t flags);
 
+/* ------------------------------------------------------------------------
+ * Drafted tokens.  A request's new tokens of a step may be a tree: row 0 the
+ * token that is certain, the others drafts, each behind its parent row.  The
+ * step is leafq_kv8_plan, leafq_kv8_tree, per layer leafq_kv8_append (with the
+ * tree's positions) and leafq_kv8_tree_attention, then leafq_verify_drafts on
+ * the logits of all rows, leafq_kv8_compact, which moves the accepted rows
+ * together, and leafq_kv8_release, which gives back the pages behind them.
+ * All of them read lengths and trees on the device, and LEAFQ_FLAG_PDL is valid
+ * with all of them whatever ran before.  A tree has at most
+ * LEAFQ_KV8_TREE_MOST rows. */
+#define LEAFQ_KV8_TREE_MOST 1024
+
+/* Ancestors and positions of every row.  parents [tokens]: the parent of a
+ * request's row t, one of its rows 0 .. t - 1, or -1 for a row that follows the
+ * request's cached tokens.  masks [tokens][words]: bit j (of word j / 32) is set
+ * for j = t and every ancestor j of row t; words is at least max_tokens / 32,
+ * rounded up.  positions [tokens]: context + the number of t's ancestors.  A row
+ * whose parent is none of these, and every row below it, gets position -1 and an
+ * empty mask, as do a request's rows past max_tokens (leafq_device_status reports
+ * both), and rows past the last new token.  Of the step: context, token_offsets,
+ * tokens, max_tokens and requests.  Outputs must not overlap one another or the
+ * inputs. */
+int leafq_kv8_tree(void* stream, const int32_t* parents, const leafq_kv8_step* step, int32_t* positions, int32_t* masks,
+                   int words, uint32_t flags);
+
+/* leafq_kv8_attention for trees: row t of request s is at position
+ * positions[row] (which the tables turn it by) and sees the keys j < context[s]
+ * and those new ones, j = context[s] + i < lengths[s], whose bit i its mask has;
+ * a mask's bits past its own row count as unset.  A row with a negative position
+ * gives zeros.  Everything else (rotation, workspace, precision, limits,
+ * what is reported) is leafq_kv8_attention's. */
+int leafq_kv8_tree_attention(void* stream, const float* q, int64_t q_stride, int heads, int rotary_dim,
+                             const float* cos_table, const float* sin_table, int64_t table_rows,
+                             const leafq_kv8_cache* cache, const leafq_kv8_step* step, const int32_t* positions,
+                             const int32_t* masks, int words, float scale, float* out, void* workspace,
+                             size_t workspace_bytes, uint32_t flags);
+
+/* Which drafts the target takes, and the token behind them.  Request s has the
+ * rows token_offsets[s] .. token_offsets[s + 1] (at most max_tokens) of logits
+ * [tokens][vocab] (rows logits_stride floats apart), ids and parents (as
+ * leafq_kv8_tree has them).  A walk starts at its row 0.  At row u, with
+ *   p = softmax(logits[u] / temperature[s]), or one at the first of the largest
+ *       logits where temperature[s] is not above zero,
+ *   q = draft_probs[u] (rows probs_stride floats apart), from which the children
+ *       of u were drawn, or one at the child's token where draft_probs is NULL,
+ * the children c of u are looked at in row order: c is taken, and the walk goes on
+ * from it, if accept[c] q(ids[c]) < p(ids[c]); otherwise p becomes max(p - q, 0) over
+ * its sum (over the target's own p again where that is zero).  Where no child is
+ * taken the walk ends with the first token whose sum of p over itself and those
+ * before it is above sample[s] times p's whole sum.  accept [tokens] and sample
+ * [requests] are uniform numbers from [0, 1); greedy requests use neither.
+ * Outputs: path [requests][max_tokens], the rows of the walk; tokens_out
+ * [requests][max_tokens], the token taken behind each of them; both end with -1s;
+ * kept [requests], how many there are (0 for a request without rows); next
+ * [requests], the last of the tokens.
+ *
+ * -inf and NaN logits have no probability, +inf ones share all of it; a row that
+ * has none gives the token -1 and ends the walk.  Negative and NaN draft
+ * probabilities count as zero.  A child whose id is outside the vocabulary is
+ * passed over (leafq_device_status reports it).  Comparisons of children hold p to
+ * about 1e-6 of itself, the sums of a draw 64 bits.  vocab is at most
+ * LEAFQ_VERIFY_MOST_VOCAB. */
+#define LEAFQ_VERIFY_MOST_VOCAB (1 << 20)
+int leafq_verify_drafts(void* stream, const float* logits, int64_t logits_stride, int64_t vocab, const int32_t* ids,
+                        const int32_t* parents, const int32_t* token_offsets, int requests, int64_t tokens,
+                        int64_t max_tokens, const float* accept, const float* sample, const float* temperature,
+                        const float* draft_probs, int64_t probs_stride, int32_t* path, int32_t* tokens_out,
+                        int32_t* kept, int32_t* next, uint32_t flags);
+
+/* Moves accepted rows together, in the caches of all layers (`caches`, a host
+ * array; all of one geometry): for i < min(kept[s], path_width, lengths[s] -
+ * context[s]) the codes of the token at context[s] + path[s][i] go to
+ * context[s] + i.  path [requests][path_width] has to ascend.  Rows of a page keep
+ * their codes; rows from another page may make its scale grow, per kv head:
+ *   need  = max(|code| * its page's scale) / 127 over the rows from other pages
+ *   scale = max(old scale, need)
+ *   the request's older rows of the page become rint(code * (old scale / scale))
+ *   moved rows become rint(code * (their page's old scale / scale))
+ * with the quotients and products in 64 bits.  What lies behind the kept rows is left
+ * undefined.  A request whose path does not ascend, or leads outside its new rows or
+ * the pool, is left as it is, and leafq_device_status reports it.  Of the step:
+ * context, lengths, table, max_pages and requests. */
+int leafq_kv8_compact(void* stream, const leafq_kv8_cache* caches, int layers, const leafq_kv8_step* step, const int32_t* path,
+                      int64_t path_width, const int32_t* kept, uint32_t flags);
+
+/* Lengths after a step of which only `kept` new tokens stay, and the pages that
+ * this gives back: lengths[s] = context[s] + kept[s], at least 0 and at most the
+ * step's lengths[s] (a negative kept drops cached tokens too, down to none when a
+ * request ends).  The pages between ceil(new length / page) and ceil(old length /
+ * page) of its row of the table go back to the free list, in request order, each
+ * request's (in the table's order) below those of the one before: the first
+ * request's end at free_pages[*taken - 1].  *taken_after is what *taken becomes.
+ * The table's entries stay, as leafq_kv8_plan overwrites them.  A request whose pages would
+ * go below the list's start keeps its length and pages, and leafq_device_status
+ * reports it, as it does a length that does not fit the table's row (which is kept).
+ * A page must be held by one request only.  Outputs must not overlap one another
+ * or the inputs. */
+int leafq_kv8_release(void* stream, const leafq_kv8_step* step, const int32_t* kept, int page, int32_t* free_pages,
+                      int64_t free_count, const int32_t* taken, int32_t* lengths, int32_t* taken_after, uint32_t flags);
+
 #ifdef __cplusplus
 }
 #endif

@@ -24,6 +24,8 @@ LEAFQ_FLAG_VNNI_ROUNDING = 0x1
 LEAFQ_FLAG_PDL = 0x2
 
 LEAFQ_IPC_HANDLE_BYTES = 64
+LEAFQ_KV8_TREE_MOST = 1024
+LEAFQ_VERIFY_MOST_VOCAB = 1 << 20
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -91,6 +93,13 @@ _SIGNATURES = {
     "leafq_kv8_attention_workspace_bytes": ([_i64, _int, _int, _int], _size),
     "leafq_kv8_attention": ([_vp, _vp, _i64, _int, _int, _vp, _vp, _i64, _vp, _vp, _f32, _vp, _vp, _size, _u32],
                             _int),
+    "leafq_kv8_tree": ([_vp, _vp, _vp, _vp, _vp, _int, _u32], _int),
+    "leafq_kv8_tree_attention": ([_vp, _vp, _i64, _int, _int, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _int, _f32, _vp, _vp,
+                                  _size, _u32], _int),
+    "leafq_verify_drafts": ([_vp, _vp, _i64, _i64, _vp, _vp, _vp, _int, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp,
+                             _vp, _vp, _u32], _int),
+    "leafq_kv8_compact": ([_vp, _vp, _int, _vp, _vp, _i64, _vp, _u32], _int),
+    "leafq_kv8_release": ([_vp, _vp, _vp, _int, _vp, _i64, _vp, _vp, _vp, _u32], _int),
 }
 
 

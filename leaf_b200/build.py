@@ -20,7 +20,8 @@ CSRC = PACKAGE / "csrc"
 LIBRARY = PACKAGE / "libleafq.so"
 SOURCES = ["act_quant.cu", "gemv_w8a8.cu", "gemv_w4a32.cu", "linear_generic.cu", "gemm_tc.cu",
            "gemm_grouped_tc.cu", "graph_gemm.cu", "api.cu", "static_scratch.cu", "decode_persistent.cu",
-           "peer_allgather.cu", "decoder_ops.cu", "decode_model.cu", "kv8_cache.cu", "kv8_attention.cu"]
+           "peer_allgather.cu", "decoder_ops.cu", "decode_model.cu", "kv8_cache.cu", "kv8_attention.cu", "kv8_tree.cu",
+           "verify_drafts.cu"]
 # Compiled as whole programs: setmaxnreg is ignored in relocatable device code.
 WHOLE_SOURCES = ["kv8_tile.cu"]
 GENCODE = "arch=compute_100a,code=sm_100a"

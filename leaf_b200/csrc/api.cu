@@ -181,6 +181,11 @@ int leafq_device_status(void) {
                   std::to_string(word & 0xffffu) + "); the kernel skipped it");
         return LEAFQ_ERR_INVALID;
     }
+    if ((word >> 16) == kSiteDraftRange) {
+        set_error("a drafted token was outside the vocabulary (block " + std::to_string(word & 0xffffu) +
+                  "); it was not taken");
+        return LEAFQ_ERR_INVALID;
+    }
     set_error("a device wait timed out (site " + std::to_string(word >> 16) + ", block " +
               std::to_string(word & 0xffffu) + ")");
     return LEAFQ_ERR_TIMEOUT;

@@ -1,10 +1,11 @@
-// Causal grouped-query attention over the paged INT8 KV cache
-// (include/leafq.h, leafq_kv8_attention).
+// Grouped-query attention over the paged INT8 KV cache, causal and of trees
+// (include/leafq.h, leafq_kv8_attention and leafq_kv8_tree_attention).
 //
 // For the query row (request s, new token t, head h) at position
 // p = context[s] + t, over keys j < min(p + 1, lengths[s]):
 //   x_j = scale * ks * (q . ck_j)      ks, vs: the scales of key j's page
 //   out = sum_j exp(x_j - m) vs cv_j / sum_j exp(x_j - m),  m = max x
+// (a tree's row: over all j < context[s], and the new keys that its mask names),
 // in one pass over the keys: when the maximum grows from m to m', the sums so
 // far are multiplied by exp(m - m').
 #include <algorithm>
@@ -188,7 +189,8 @@ __device__ __forceinline__ void join_parts(uint8_t* smem, const float* parts, in
     }
 }
 
-template <int D, bool kNarrow>
+// kTree: the request's new rows see those of the new keys that their masks name.
+template <int D, bool kNarrow, bool kTree>
 __global__ void __launch_bounds__(Split<D, kNarrow>::kThreads, Split<D, kNarrow>::kBlocksPerSm)
 kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals, int ranges, int row_blocks) {
     using C = Split<D, kNarrow>;
@@ -424,9 +426,9 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
             const int row = tid / kRowThreads + pass * (C::kThreads / kRowThreads);
             if (row < 8 && item < D / 8) {
                 const int t = (first_row + row) / g.group, hq = (first_row + row) - t * g.group;
-                int64_t pos = (int64_t)context + t;
+                int64_t pos = kTree ? (row < rows ? g.positions[row0 + t] : 0) : (int64_t)context + t;
                 if (row < rows && g.rotary > 0 && (pos < 0 || pos >= g.table_rows)) {
-                    if (item == 0) record_device_error(kSiteKv8Range);
+                    if (item == 0 && !(kTree && pos < 0)) record_device_error(kSiteKv8Range);
                     pos = 0;
                 }
                 rows_item[pass].load(g, row < rows ? g.q + (row0 + t) * g.q_stride + (int64_t)(h * g.group + hq) * D : nullptr, item, pos);
@@ -470,9 +472,11 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
         for (int j = 0; j < D / 16; ++j) *reinterpret_cast<uint4*>(q[j]) = q_s[j * 32 + lane];
         const float factor = factor_s[gq];  // from an MMA sum to x_j / ks
         // Keys that row gq sees; none for a row past the request's.
-        const int64_t row_pos = (int64_t)context + (first_row + gq) / g.group;
+        const int64_t row_end = (int64_t)context + (first_row + gq) / g.group;
+        const int64_t row_pos = !kTree ? row_end : gq < rows ? g.positions[row0 + (first_row + gq) / g.group] : -1;
         const bool seen = gq < rows && row_pos >= 0 && (g.rotary == 0 || row_pos < g.table_rows);
-        const int limit = seen ? static_cast<int>(min64(kb, row_pos + 1)) : 0;
+        const int limit = seen ? static_cast<int>(min64(kb, row_end + 1)) : 0;
+        const uint32_t* row_mask = kTree ? g.masks + (row0 + (first_row + min(gq, rows - 1)) / g.group) * g.mask_words : nullptr;
 
         float o[D / 8][2], m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -529,12 +533,14 @@ kv8_attend_split_kernel(const Kv8AttendArgs g, float* parts, uint32_t* arrivals,
 #pragma unroll
                 for (int e = 0; e < 2; ++e) x[n][e] = fmaf(acc[e] + acc[e + 2], ks[n >> 1], bias[n >> 1]);
             }
-            if (__any_sync(~0u, key + C::kChunk > limit)) {
+            if (__any_sync(~0u, key + C::kChunk > limit || (kTree && key + C::kChunk > context))) {
+                const uint32_t window = kTree ? tree_window(row_mask, g.mask_words, key - context) : ~0u;
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        if (key + 8 * n + tq + 4 * e >= limit) x[n][e] = -INFINITY;
+                        if (key + 8 * n + tq + 4 * e >= limit || (kTree && !(window >> (8 * n + tq + 4 * e) & 1u)))
+                            x[n][e] = -INFINITY;
             }
             // The weights count relative to m, a whole power of two that is the same for
             // the row's four lanes.  It comes from the row's first keys; later ones are
@@ -723,7 +729,7 @@ SplitShape split_shape(int64_t max_tokens, int group) {
     return f;
 }
 
-template <int D, bool kNarrow>
+template <int D, bool kNarrow, bool kTree>
 int run_split(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) {
     using C = Split<D, kNarrow>;
     const SplitShape f = split_shape<D, kNarrow>(g.step.max_tokens, g.group);
@@ -732,12 +738,12 @@ int run_split(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl)
     // 1,000 tokens 54.6 and 39.7, 2,048 of 100 to 400 72 and 37; 128-wide: 48 of
     // 15,000 to 91,000 tokens 103 and 124, 512 of 1,000 to 4,000 88 and 90, 1,024 of
     // 500 to 1,500 85 and 76, 2,048 of 200 to 2,000 167 and 138.
-    if (!kNarrow && (int64_t)g.step.requests * g.cache.kv_heads > f.ranges) return run_split<D, true>(s, g, workspace, pdl);
+    if (!kNarrow && (int64_t)g.step.requests * g.cache.kv_heads > f.ranges) return run_split<D, true, kTree>(s, g, workspace, pdl);
     if (f.ranges * f.row_blocks > INT_MAX / 8) {
         set_error("leafq_kv8_attention: max_tokens * group is too large");
         return LEAFQ_ERR_INVALID;
     }
-    const auto kernel = kv8_attend_split_kernel<D, kNarrow>;
+    const auto kernel = kv8_attend_split_kernel<D, kNarrow, kTree>;
     const int st = allow_smem(reinterpret_cast<const void*>(kernel), C::kSmem, "leafq_kv8_attention");
     if (st) return st;
     uint32_t* arrivals = static_cast<uint32_t*>(workspace);
@@ -772,6 +778,54 @@ auto with_dim(int dim, F&& f) {
     }
 }
 
+// Both entry points: of trees where there are masks.
+int attend(const char* what, void* stream, const float* q, int64_t q_stride, int heads, int rotary_dim, const float* cos_table,
+           const float* sin_table, int64_t table_rows, const leafq_kv8_cache* cache, const leafq_kv8_step* step,
+           const int32_t* positions, const uint32_t* masks, int words, float scale, float* out, void* workspace,
+           size_t workspace_bytes, uint32_t flags) {
+    clear_error();
+    if (!kv8_cache_valid(cache, what)) return LEAFQ_ERR_INVALID;
+    if (!kv8_dim_supported(cache->dim)) {
+        set_error(std::string(what) + ": head sizes are 32, 64, 96 and 128");
+        return LEAFQ_ERR_UNSUPPORTED;
+    }
+    if (!kv8_rope_valid(cache->dim, rotary_dim, cos_table, sin_table, table_rows, what))
+        return LEAFQ_ERR_INVALID;
+    if (!step || step->tokens < 0 || step->tokens > INT_MAX || step->max_tokens < 0 || step->requests < 0 ||
+        step->max_pages < 0 || step->max_pages > INT_MAX / cache->page || heads <= 0 || heads > 65535 ||
+        heads % cache->kv_heads != 0 || !(scale > 0.0f) || scale > 3.0e38f) {
+        set_error(std::string(what) + ": invalid step, heads (a multiple of the cache's) or scale (positive)");
+        return LEAFQ_ERR_INVALID;
+    }
+    if (step->tokens == 0 || step->requests == 0) return LEAFQ_OK;
+    if (!q || !out || !step->context || !step->lengths || !step->token_offsets || !step->page_offsets ||
+        (step->max_pages > 0 && !step->table)) {
+        set_error(std::string(what) + ": null pointer");
+        return LEAFQ_ERR_INVALID;
+    }
+    if ((step->tokens > 1 && q_stride < (int64_t)heads * cache->dim) || q_stride % 4 != 0 || !aligned16(q) ||
+        !aligned16(out)) {
+        set_error(std::string(what) + ": q and out rows must be 16-byte aligned and must not overlap");
+        return LEAFQ_ERR_INVALID;
+    }
+    if (step->max_tokens == 0) return LEAFQ_OK;
+    const size_t need = leafq_kv8_attention_workspace_bytes(step->max_tokens, heads, cache->kv_heads, cache->dim);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
+        set_error(std::string(what) + ": this shape needs " + std::to_string(need) +
+                  " bytes of 16-byte aligned workspace");
+        return LEAFQ_ERR_INVALID;
+    }
+    Kv8AttendArgs g{q, q_stride, cos_table, sin_table, table_rows, *cache, *step, out, scale, heads,
+                 heads / cache->kv_heads, rotary_dim, 0, INT_MAX / (heads / cache->kv_heads), positions, masks, words};
+    while ((1 << g.shift) < cache->page) ++g.shift;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool pdl = (flags & LEAFQ_FLAG_PDL) != 0;
+    if (takes_tiles(step->tokens, step->max_tokens, heads, g.group)) return launch_kv8_tiles(s, g, workspace, pdl);
+    return with_dim(cache->dim, [&](auto d) {
+        return masks ? run_split<d(), false, true>(s, g, workspace, pdl) : run_split<d(), false, false>(s, g, workspace, pdl);
+    });
+}
+
 }  // namespace
 }  // namespace leafq
 
@@ -795,45 +849,24 @@ int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int head
                         const float* cos_table, const float* sin_table, int64_t table_rows,
                         const leafq_kv8_cache* cache, const leafq_kv8_step* step, float scale, float* out,
                         void* workspace, size_t workspace_bytes, uint32_t flags) {
-    clear_error();
-    if (!kv8_cache_valid(cache, "leafq_kv8_attention")) return LEAFQ_ERR_INVALID;
-    if (!kv8_dim_supported(cache->dim)) {
-        set_error("leafq_kv8_attention: head sizes are 32, 64, 96 and 128");
-        return LEAFQ_ERR_UNSUPPORTED;
-    }
-    if (!kv8_rope_valid(cache->dim, rotary_dim, cos_table, sin_table, table_rows, "leafq_kv8_attention"))
-        return LEAFQ_ERR_INVALID;
-    if (!step || step->tokens < 0 || step->tokens > INT_MAX || step->max_tokens < 0 || step->requests < 0 ||
-        step->max_pages < 0 || step->max_pages > INT_MAX / cache->page || heads <= 0 || heads > 65535 ||
-        heads % cache->kv_heads != 0 || !(scale > 0.0f) || scale > 3.0e38f) {
-        set_error("leafq_kv8_attention: invalid step, heads (a multiple of the cache's) or scale (positive)");
-        return LEAFQ_ERR_INVALID;
-    }
-    if (step->tokens == 0 || step->requests == 0) return LEAFQ_OK;
-    if (!q || !out || !step->context || !step->lengths || !step->token_offsets || !step->page_offsets ||
-        (step->max_pages > 0 && !step->table)) {
-        set_error("leafq_kv8_attention: null pointer");
+    return attend("leafq_kv8_attention", stream, q, q_stride, heads, rotary_dim, cos_table, sin_table, table_rows, cache, step,
+                  nullptr, nullptr, 0, scale, out, workspace, workspace_bytes, flags);
+}
+
+int leafq_kv8_tree_attention(void* stream, const float* q, int64_t q_stride, int heads, int rotary_dim,
+                             const float* cos_table, const float* sin_table, int64_t table_rows,
+                             const leafq_kv8_cache* cache, const leafq_kv8_step* step, const int32_t* positions,
+                             const int32_t* masks, int words, float scale, float* out, void* workspace,
+                             size_t workspace_bytes, uint32_t flags) {
+    const char* what = "leafq_kv8_tree_attention";
+    if (step && step->tokens > 0 && step->requests > 0 &&
+        (!positions || !masks || words <= 0 || words > LEAFQ_KV8_TREE_MOST / 32 || step->max_tokens > 32 * (int64_t)words)) {
+        clear_error();
+        set_error(std::string(what) + ": positions and masks are needed, of max_tokens / 32 words a row, rounded up (32 at most)");
         return LEAFQ_ERR_INVALID;
     }
-    if ((step->tokens > 1 && q_stride < (int64_t)heads * cache->dim) || q_stride % 4 != 0 || !aligned16(q) ||
-        !aligned16(out)) {
-        set_error("leafq_kv8_attention: q and out rows must be 16-byte aligned and must not overlap");
-        return LEAFQ_ERR_INVALID;
-    }
-    if (step->max_tokens == 0) return LEAFQ_OK;
-    const size_t need = leafq_kv8_attention_workspace_bytes(step->max_tokens, heads, cache->kv_heads, cache->dim);
-    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
-        set_error("leafq_kv8_attention: this shape needs " + std::to_string(need) +
-                  " bytes of 16-byte aligned workspace");
-        return LEAFQ_ERR_INVALID;
-    }
-    Kv8AttendArgs g{q, q_stride, cos_table, sin_table, table_rows, *cache, *step, out, scale, heads,
-                 heads / cache->kv_heads, rotary_dim, 0, INT_MAX / (heads / cache->kv_heads)};
-    while ((1 << g.shift) < cache->page) ++g.shift;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool pdl = (flags & LEAFQ_FLAG_PDL) != 0;
-    if (takes_tiles(step->tokens, step->max_tokens, heads, g.group)) return launch_kv8_tiles(s, g, workspace, pdl);
-    return with_dim(cache->dim, [&](auto d) { return run_split<d(), false>(s, g, workspace, pdl); });
+    return attend(what, stream, q, q_stride, heads, rotary_dim, cos_table, sin_table, table_rows, cache, step, positions,
+                  reinterpret_cast<const uint32_t*>(masks), words, scale, out, workspace, workspace_bytes, flags);
 }
 
 }  // extern "C"

@@ -1,5 +1,6 @@
-// Shared by the paged INT8 cache's append (kv8_cache.cu) and the two forms of its
-// attention (kv8_attention.cu for few query rows, kv8_tile.cu for many).
+// Shared by the paged INT8 cache's plan and append (kv8_cache.cu), the two forms of its
+// attention (kv8_attention.cu for few query rows, kv8_tile.cu for many) and its trees of
+// drafts (kv8_tree.cu).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -11,6 +12,18 @@
 #include "leafq_internal.h"
 
 namespace leafq {
+
+// `count` values of a call's argument.
+struct Span {
+    const int32_t* begin;
+    int64_t count;
+    bool overlaps(const Span& other) const {
+        const auto at = reinterpret_cast<uintptr_t>(begin), other_at = reinterpret_cast<uintptr_t>(other.begin);
+        return count > 0 && other.count > 0 && at < other_at + 4 * other.count && other_at < at + 4 * count;
+    }
+};
+
+inline int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1; }
 
 struct Kv8AttendArgs {
     const float* q;
@@ -24,6 +37,11 @@ struct Kv8AttendArgs {
     float scale;
     int heads, group, rotary, shift;
     int most_tokens;  // of a request: its rows (tokens * group) fit int32
+    // Trees of drafts (leafq_kv8_tree_attention): each row's position, and which of the
+    // request's new rows it sees, as bits.  Null for causal attention.
+    const int32_t* positions;
+    const uint32_t* masks;
+    int mask_words;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -74,6 +92,16 @@ __device__ __forceinline__ void kv8_turn(float4& a, float4& b, float4 c, float4 
                     __fsub_rn(__fmul_rn(x.z, c.z), __fmul_rn(y.z, s.z)), __fsub_rn(__fmul_rn(x.w, c.w), __fmul_rn(y.w, s.w)));
     b = make_float4(__fadd_rn(__fmul_rn(y.x, c.x), __fmul_rn(x.x, s.x)), __fadd_rn(__fmul_rn(y.y, c.y), __fmul_rn(x.y, s.y)),
                     __fadd_rn(__fmul_rn(y.z, c.z), __fmul_rn(x.z, s.z)), __fadd_rn(__fmul_rn(y.w, c.w), __fmul_rn(x.w, s.w)));
+}
+
+// Bit i: whether a tree's row with these mask words sees key `at` + i, the request's new
+// keys being numbered from 0 (those before them are cached ones, which every row sees;
+// the mask's words end with those of the tree).
+__device__ __forceinline__ uint32_t tree_window(const uint32_t* row_mask, int words, int at) {
+    if (at <= -32) return ~0u;
+    const int w = at >> 5;
+    const auto word = [&](int i) { return i < 0 ? ~0u : i < words ? row_mask[i] : 0u; };
+    return __funnelshift_r(word(w), word(w + 1), at & 31);
 }
 
 // Eight values of a query row, its item j of D / 8: four at `at` and four at

@@ -190,7 +190,8 @@ __device__ __forceinline__ void store_local(uint32_t at, float4 v) {
 // kParts: some items are cut into parts (the code that joins them is left out of
 // the other kernel, whose loops it would push out of the instruction cache:
 // 64 prompts of 512 tokens 368 us without it, 379 us with it).
-template <int D, bool kParts>
+// kTree: the request's new rows see those of the new keys that their masks name.
+template <int D, bool kParts, bool kTree>
 __global__ void __launch_bounds__(TileShape<D>::kThreads, 2)
 kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t* taken, uint32_t* arrivals, float* parts,
                        int row_tiles, int splits) {
@@ -287,9 +288,10 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             }
             const int r = tid;
             const int t = token_of(first_row + r), hq = (first_row + r) - t * g.group;
-            const int pos = context + t;
+            const int pos = !kTree ? context + t : r < rows ? g.positions[row0 + t] : -1;
             const bool seen = r < rows && pos >= 0 && (g.rotary == 0 || pos < g.table_rows);
-            const int limit = seen ? min(keys, pos + 1) : 0;
+            const int limit = seen ? min(keys, context + t + 1) : 0;
+            const uint32_t* row_mask = kTree ? g.masks + (int64_t)(row0 + token_of(first_row + min(r, rows - 1))) * g.mask_words : nullptr;
             float* out = g.out + ((int64_t)row0 + t) * g.heads * D + (int64_t)(head * g.group + hq) * D;
             float m = -INFINITY, l = 0.0f, m_sum = -INFINITY;
             for (int j = 0; j < tiles; ++j, ++n) {
@@ -299,7 +301,8 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 tcgen05_fence_after();
                 const float4* scales = info + (n % C::kInfo) * C::kGroups;
                 const int visible = limit - (tile0 + j) * C::kKeys;  // columns of this tile that the row sees
-                const bool whole = __all_sync(~0u, visible >= C::kKeys);
+                const int drafted = (tile0 + j) * C::kKeys - context;  // the tile's first key among the request's new ones
+                const bool whole = __all_sync(~0u, visible >= C::kKeys) && !(kTree && drafted + C::kKeys > 0);
                 // 32 scores at a time, by rolled loops: the roles' loops have to stay in the
                 // instruction cache side by side (unrolled, with all scores in registers,
                 // the kernel took 1.5 times as long).  What is not seen is -inf.
@@ -308,8 +311,10 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     tmem_ld_32x32b_x32(s_tmem + lanes + 32 * c, x);
                     tmem_wait_ld();
                     if (!whole) {
+                        const uint32_t window = kTree ? tree_window(row_mask, g.mask_words, drafted + 32 * c) : ~0u;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x[e] = 32 * c + e >= visible ? 0xff800000u : x[e];
+                        for (int e = 0; e < 32; ++e)
+                            x[e] = 32 * c + e >= visible || (kTree && !(window >> e & 1u)) ? 0xff800000u : x[e];
                     }
                 };
                 // From an MMA sum to x_j: above zero, so that -inf stays.
@@ -649,9 +654,9 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     a1 = load_now(reinterpret_cast<const float4*>(src + at));
                     b1 = load_now(reinterpret_cast<const float4*>(src + to));
                     if (turned) {
-                        int64_t pos = (int64_t)next.context + t;
+                        int64_t pos = kTree ? load_now(g.positions + (next.row0 + t)) : (int64_t)next.context + t;
                         if (pos < 0 || pos >= g.table_rows) {
-                            if (part == 0) report(watch, kSiteKv8Range);
+                            if (part == 0 && !(kTree && pos < 0)) report(watch, kSiteKv8Range);
                             pos = 0;
                         }
                         cs1 = load_now(reinterpret_cast<const float4*>(g.cos_table + pos * half + at));
@@ -929,7 +934,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
     }
 }
 
-template <int D, bool kParts>
+template <int D, bool kParts, bool kTree>
 int start_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, int64_t row_tiles, int splits, bool pdl);
 
 template <int D>
@@ -944,16 +949,19 @@ int run_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) 
         return LEAFQ_ERR_INVALID;
     }
     const int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostParts, kTileBlocks / (row_tiles * g.cache.kv_heads))));
-    return splits > 1 ? start_tile<D, true>(s, g, workspace, row_tiles, splits, pdl)
-                      : start_tile<D, false>(s, g, workspace, row_tiles, 1, pdl);
+    if (g.masks)
+        return splits > 1 ? start_tile<D, true, true>(s, g, workspace, row_tiles, splits, pdl)
+                          : start_tile<D, false, true>(s, g, workspace, row_tiles, 1, pdl);
+    return splits > 1 ? start_tile<D, true, false>(s, g, workspace, row_tiles, splits, pdl)
+                      : start_tile<D, false, false>(s, g, workspace, row_tiles, 1, pdl);
 }
 
-template <int D, bool kParts>
+template <int D, bool kParts, bool kTree>
 int start_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, int64_t row_tiles, int splits, bool pdl) {
     DeviceWatch watch;
     int st = device_watch(&watch);
     if (st) return st;
-    const void* kernel = reinterpret_cast<const void*>(kv8_attend_tile_kernel<D, kParts>);
+    const void* kernel = reinterpret_cast<const void*>(kv8_attend_tile_kernel<D, kParts, kTree>);
     static const int registers = [kernel] {
         cudaFuncAttributes a;
         return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0;
@@ -967,7 +975,7 @@ int start_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, int64_t 
     if (st) return st;
     const int64_t blocks = std::min<int64_t>(row_tiles * g.cache.kv_heads * splits, 2 * (int64_t)sm_count());
     uint32_t* counters = static_cast<uint32_t*>(workspace) + kTileCounters;
-    return launch(kv8_attend_tile_kernel<D, kParts>, dim3(static_cast<unsigned>(blocks)),
+    return launch(kv8_attend_tile_kernel<D, kParts, kTree>, dim3(static_cast<unsigned>(blocks)),
                   dim3(TileShape<D>::kThreads), TileShape<D>::kSmem, s, pdl, "leafq_kv8_attention", g, watch,
                   counters, counters + 4, reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes),
                   static_cast<int>(row_tiles), splits);

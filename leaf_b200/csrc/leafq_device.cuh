@@ -57,6 +57,7 @@ enum WaitSite : unsigned {
     kSiteCacheRange = 14,  // not a wait: a position outside the KV cache
     kSiteKv8Range = 15,    // not a wait: a paged-cache index or length out of range
     kSiteKv8Tile = 16,
+    kSiteDraftRange = 17,  // not a wait: a drafted token outside the vocabulary
 };
 
 __device__ __forceinline__ unsigned long long global_timer_ns() {

@@ -7,8 +7,14 @@ slots from the request lengths, on the device), then per layer ``kv8_append``
 cache per sequence (kv_cache.cpp:21-59); this one holds a quarter of its bytes
 and lets requests of different lengths share memory, at the rounding of 8 bits.
 
-``Kv8Cache``, ``Kv8Plan`` and ``Kv8Workspace`` are handles a serving loop makes
-once and keeps; the calls only enqueue work on the current stream.
+With drafted tokens a request's rows of a step are a tree: ``kv8_tree`` once a
+step, ``kv8_tree_attention`` in the place of ``kv8_attention``, and, once
+``verify_drafts`` (drafts.py) has said which rows stay, ``kv8_compact`` for all
+layers and ``kv8_release`` for the pages behind them.
+
+``Kv8Cache``, ``Kv8Layers``, ``Kv8Plan``, ``Kv8Tree`` and ``Kv8Workspace`` are
+handles a serving loop makes once and keeps; the calls only enqueue work on the
+current stream.
 """
 from __future__ import annotations
 
@@ -22,6 +28,7 @@ from ._lib import LEAFQ_FLAG_PDL, LeafError, check, load
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_SIZES = (32, 64, 96, 128)
+TREE_MOST = _lib.LEAFQ_KV8_TREE_MOST  # rows of a request's tree
 
 
 _F32, _I32 = torch.float32, torch.int32
@@ -141,6 +148,49 @@ class Kv8Plan:
         self.max_tokens = self.desc.max_tokens = int(max_tokens)
 
 
+class Kv8Layers:
+    """The caches of all layers of a model, of one geometry, for the calls that
+    do them all at once."""
+
+    def __init__(self, caches):
+        self.caches = list(caches)
+        _need(len(self.caches) > 0, "there must be a layer's cache")
+        first = self.caches[0]
+        _need(all((c.index, c.pages, c.page, c.kv_heads, c.dim) == (first.index, first.pages, first.page, first.kv_heads, first.dim)
+                  for c in self.caches), "the layers' caches must be on one device and have the same pages, kv heads and head size")
+        self.index, self.page = first.index, first.page
+        self.descs = (_lib.Kv8CacheDesc * len(self.caches))(*(c.desc for c in self.caches))
+
+
+class Kv8Tree:
+    """The trees of a step: ``positions`` [tokens], and ``masks`` [tokens, words]
+    of 32 bits, bit j of a row's being set for itself and its ancestors j."""
+
+    def __init__(self, positions: torch.Tensor, masks: torch.Tensor):
+        _check_i32(positions, "positions")
+        self.index, self.tokens = positions.get_device(), positions.numel()
+        _need(masks.dim() == 2 and masks.shape[0] == self.tokens and 1 <= masks.shape[1] <= TREE_MOST // 32,
+              f"masks must be [tokens, words], of at most {TREE_MOST // 32} words")
+        _check_i32(masks, "masks", None, self.index)
+        self.positions, self.masks, self.words = positions, masks, masks.shape[1]
+        self.address = positions.data_ptr(), masks.data_ptr()
+
+    def fits(self, plan: Kv8Plan) -> None:
+        if self.tokens != plan.tokens or self.index != plan.index or plan.max_tokens > 32 * self.words:
+            _fail("the tree is of other rows than the plan's, or on another device")
+
+
+class Kv8Released:
+    """What kv8_release gives: ``lengths`` [requests] and ``taken`` [1]."""
+
+    def __init__(self, lengths: torch.Tensor, taken: torch.Tensor):
+        _check_i32(taken, "taken", 1)
+        self.index, self.requests = taken.get_device(), lengths.numel()
+        _check_i32(lengths, "lengths", None, self.index)
+        self.lengths, self.taken = lengths, taken
+        self.address = lengths.data_ptr(), taken.data_ptr()
+
+
 class Kv8Workspace:
     """Device scratch of ``kv8_attention``, zeroed when it grows.  Reuse it
     across calls on one stream.  A buffer that was outgrown lives as long as the
@@ -243,16 +293,17 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: Kv8Cache, slots: torch.T
 
 def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float, rope=None,
                   out: Optional[torch.Tensor] = None, workspace: Optional[Kv8Workspace] = None,
-                  flags: int = LEAFQ_FLAG_PDL) -> torch.Tensor:
+                  flags: int = LEAFQ_FLAG_PDL, tree: Optional[Kv8Tree] = None) -> torch.Tensor:
     """Causal grouped-query attention of the step's rows q (fp32
     [tokens, heads * dim]; columns of a wider matrix will do) over the cache,
     rotated by position when rope tables are given.  Returns fp32
     [tokens, heads * dim]; a row that sees no key is zero, rows past the step's
-    last new token are not written."""
+    last new token are not written.  With a tree the rows are at its positions
+    and see its ancestors only (kv8_tree_attention)."""
     index, dim, shape = cache.index, cache.dim, q.shape
     if _current_device() != index:
         with torch.cuda.device(index):
-            return kv8_attention(q, cache, plan, scale, rope, out, workspace, flags)
+            return kv8_attention(q, cache, plan, scale, rope, out, workspace, flags, tree)
     if len(shape) != 2 or shape[1] % dim != 0:
         _fail("q must be [tokens, heads * dim]")
     tokens, width = shape
@@ -274,6 +325,94 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float,
     elif workspace.index != index:
         _fail("the workspace is on another device")
     address, need = workspace.of(plan.max_tokens, heads, cache.kv_heads, dim)
+    if tree is not None:
+        tree.fits(plan)
+        check(load().leafq_kv8_tree_attention(_raw_stream(index), q.data_ptr(), stride, heads, rotary, cos, sin, rows,
+                                              cache.ref, plan.ref, tree.address[0], tree.address[1], tree.words, scale,
+                                              out.data_ptr(), address, need, flags))
+        return out
     check(load().leafq_kv8_attention(_raw_stream(index), q.data_ptr(), stride, heads, rotary, cos, sin, rows, cache.ref,
                                      plan.ref, scale, out.data_ptr(), address, need, flags))
+    return out
+
+
+def kv8_tree(parents: torch.Tensor, plan: Kv8Plan, out: Optional[Kv8Tree] = None, flags: int = LEAFQ_FLAG_PDL) -> Kv8Tree:
+    """Positions and ancestors of a step's rows: parents (int32 [tokens]) holds
+    each row's parent among its request's rows, one before it, or -1 for a row
+    that follows the cached tokens.  A request brings at most TREE_MOST rows.
+    A row whose parent is none of these, and those below it, get position -1 and
+    see nothing.  ``out``: a tree of the same rows, which is filled again."""
+    index = plan.index
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return kv8_tree(parents, plan, out, flags)
+    _check_i32(parents, "parents", plan.tokens, index)
+    words = max(1, (plan.max_tokens + 31) // 32)
+    if out is None:
+        if plan.max_tokens > TREE_MOST:
+            raise LeafError(_lib.LEAFQ_ERR_UNSUPPORTED, f"a request's tree has at most {TREE_MOST} rows")
+        out = Kv8Tree(torch.empty(plan.tokens, dtype=_I32, device=plan.device),
+                      torch.empty((plan.tokens, words), dtype=_I32, device=plan.device))
+    else:
+        out.fits(plan)
+    check(load().leafq_kv8_tree(_raw_stream(index), parents.data_ptr(), plan.ref, out.address[0], out.address[1], out.words,
+                                flags))
+    return out
+
+
+def kv8_tree_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, tree: Kv8Tree, scale: float, rope=None,
+                       out: Optional[torch.Tensor] = None, workspace: Optional[Kv8Workspace] = None,
+                       flags: int = LEAFQ_FLAG_PDL) -> torch.Tensor:
+    """kv8_attention of a step whose requests bring trees: each row is at its
+    position in the tree and sees the cached tokens, its ancestors and itself."""
+    if tree is None:
+        _fail("the tree is missing (kv8_tree makes it)")
+    return kv8_attention(q, cache, plan, scale, rope, out, workspace, flags, tree)
+
+
+def kv8_compact(layers: Kv8Layers, plan: Kv8Plan, path: torch.Tensor, kept: torch.Tensor, flags: int = LEAFQ_FLAG_PDL) -> None:
+    """Moves the accepted rows of every request together, in every layer: for
+    i < kept[s] the row at context + path[s][i] goes to context + i.  path (int32
+    [requests, width]) ascends, kept is int32 [requests], as verify_drafts gives
+    them.  Codes that leave their page are rounded to the scale of the one they
+    come to, which grows where they need it.  Before kv8_release."""
+    index = layers.index
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return kv8_compact(layers, plan, path, kept, flags)
+    if plan.index != index:
+        _fail("the plan is on another device")
+    if plan.page is not None and plan.page != layers.page:
+        _fail(f"the plan has pages of {plan.page} tokens, the caches of {layers.page}")
+    if len(path.shape) != 2 or path.shape[0] != plan.requests:
+        _fail("path must be [requests, width]")
+    _check_i32(path, "path", None, index)
+    _check_i32(kept, "kept", plan.requests, index)
+    check(load().leafq_kv8_compact(_raw_stream(index), layers.descs, len(layers.caches), plan.ref, path.data_ptr(),
+                                   path.shape[1], kept.data_ptr(), flags))
+
+
+def kv8_release(plan: Kv8Plan, kept: torch.Tensor, free_pages: torch.Tensor, taken: torch.Tensor,
+                out: Optional[Kv8Released] = None, flags: int = LEAFQ_FLAG_PDL) -> Kv8Released:
+    """Lengths of the requests of which kept[s] (int32 [requests]) of the step's
+    new tokens stay: context + kept, at least 0 and at most the step's lengths (a
+    negative kept drops cached tokens too).  The pages behind them go back to
+    free_pages (in place), in front of those that kv8_plan takes next.  ``taken``
+    is only read, the new count is the result's ``taken``: copy it and
+    ``lengths`` back for the next step.  ``out``: a result that is filled again."""
+    index = plan.index
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return kv8_release(plan, kept, free_pages, taken, out, flags)
+    if plan.page is None:
+        _fail("the plan's page size is not known (Kv8Plan(page=...))")
+    _check_i32(kept, "kept", plan.requests, index)
+    _check_i32(free_pages, "free_pages", None, index)
+    _check_i32(taken, "taken", 1, index)
+    if out is None:
+        out = Kv8Released(*(torch.empty(n, dtype=_I32, device=plan.device) for n in (plan.requests, 1)))
+    elif out.index != index or out.requests != plan.requests:
+        _fail("the result to reuse is of other requests, or on another device")
+    check(load().leafq_kv8_release(_raw_stream(index), plan.ref, kept.data_ptr(), plan.page, free_pages.data_ptr(),
+                                   free_pages.numel(), taken.data_ptr(), out.address[0], out.address[1], flags))
     return out

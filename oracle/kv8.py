@@ -96,3 +96,89 @@ def attention(q, visible, keys, values, scale):
         e = np.exp(x - x.max(axis=1, keepdims=True))
         out[r] = e @ values[:n] / e.sum(axis=1, keepdims=True)
     return out, reach
+
+
+def tree(parents, context: int):
+    """Of one request: (positions, ancestors) of its rows, a row's ancestors as a
+    set that holds itself; position -1 and none where the way to the cached
+    tokens is broken."""
+    positions, above = [], []
+    for t, p in enumerate(parents):
+        p = int(p)
+        if p == -1:
+            above.append({t})
+        elif 0 <= p < t and above[p]:
+            above.append(above[p] | {t})
+        else:
+            above.append(set())
+        positions.append(context + len(above[t]) - 1 if above[t] else -1)
+    return positions, above
+
+
+def tree_attention(q, visible, keys, values, scale):
+    """attention() with visible [rows, n] saying which keys each row sees."""
+    out = np.zeros_like(q)
+    reach = np.zeros(q.shape[:2])
+    for r, seen in enumerate(visible):
+        if not seen.any():
+            continue
+        o, e = attention(q[r:r + 1], [int(seen.sum())], keys[seen], values[seen], scale)
+        out[r], reach[r] = o[0], e[0]
+    return out, reach
+
+
+def compact(codes, scales, context, lengths, table, path, kept):
+    """leafq_kv8_compact on one layer's codes [pages, heads, page, dim] and scales:
+    (codes, scales, unrounded), new arrays; what lies behind a request's kept rows is as
+    it was."""
+    codes, scales = codes.astype(np.float64), scales.astype(np.float32).copy()
+    unrounded = codes.copy()
+    page, pool = codes.shape[2], codes.shape[0]
+    for s in range(len(context)):
+        c, fresh = int(context[s]), int(lengths[s]) - int(context[s])
+        m = max(0, min(int(kept[s]), len(path[s]), fresh))
+        way = [int(p) for p in path[s][:m]]
+        if any(p < 0 or p >= fresh for p in way) or any(b <= a for a, b in zip(way, way[1:])):
+            continue
+        places = [(int(table[s][(c + i) // page]), int(table[s][(c + j) // page])) for i, j in enumerate(way) if i != j]
+        if any(not 0 <= p < pool for pair in places for p in pair):
+            continue
+        i = 0
+        while i < m:  # the rows that go to one page
+            end = min(m, i + page - (c + i) % page)
+            moves = [(k, way[k]) for k in range(i, end) if way[k] != k]
+            if moves:
+                p = int(table[s][(c + i) // page])
+                source = [(int(table[s][(c + j) // page]), (c + j) % page) for _, j in moves]
+                rows = [codes[a][:, b].copy() for a, b in source]  # [heads, dim]
+                old = scales.copy()
+                for h in range(codes.shape[1]):
+                    need = [np.abs(x[h]).max() * float(old[a, h]) / 127 for x, (a, _) in zip(rows, source) if a != p]
+                    scales[p, h] = np.float32(max([float(old[p, h])] + need))
+                    if scales[p, h] != old[p, h]:
+                        stay = (c + moves[0][0]) % page
+                        unrounded[p, h, :stay] = codes[p, h, :stay] * (float(old[p, h]) / float(scales[p, h]))
+                        codes[p, h, :stay] = np.rint(unrounded[p, h, :stay])
+                    for (k, _), x, (a, _) in zip(moves, rows, source):
+                        unrounded[p, h, (c + k) % page] = x[h] * (float(old[a, h]) / float(scales[p, h]))
+                        codes[p, h, (c + k) % page] = np.rint(unrounded[p, h, (c + k) % page])
+            i = end
+    return codes, scales, unrounded
+
+
+def release(context, lengths, kept, table, free, taken: int, page: int):
+    """leafq_kv8_release: (lengths, free list, taken)."""
+    free, after, wanted, taken_after = np.array(free), [], 0, taken
+    for s in range(len(context)):
+        length = int(lengths[s])
+        left = max(0, min(length, int(context[s]) + int(kept[s])))
+        a, b = pages_of(left, page), pages_of(length, page)
+        wanted += b - a
+        if b > a and (taken - wanted < 0 or taken > len(free)):
+            after.append(length)
+            continue
+        free[taken - wanted:taken - wanted + b - a] = table[s][a:b]
+        if b > a:
+            taken_after = taken - wanted
+        after.append(left)
+    return np.array(after), free, taken_after
