@@ -552,12 +552,16 @@ int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int head
 int leafq_kv8_tree(void* stream, const int32_t* parents, const leafq_kv8_step* step, int32_t* positions, int32_t* masks,
                    int words, uint32_t flags);
 
+/* As leafq_kv8_attention_workspace_bytes: the same words of a workspace are zero
+ * between calls, so that calls of both kinds may share one of the larger size. */
+size_t leafq_kv8_tree_attention_workspace_bytes(int64_t max_tokens, int heads, int kv_heads, int dim);
+
 /* leafq_kv8_attention for trees: row t of request s is at position
  * positions[row] (which the tables turn it by) and sees the keys j < context[s]
  * and those new ones, j = context[s] + i < lengths[s], whose bit i its mask has;
  * a mask's bits past its own row count as unset.  A row with a negative position
- * gives zeros.  Everything else (rotation, workspace, precision, limits,
- * what is reported) is leafq_kv8_attention's. */
+ * gives zeros.  Everything else (rotation, precision, limits, what is reported) is
+ * leafq_kv8_attention's. */
 int leafq_kv8_tree_attention(void* stream, const float* q, int64_t q_stride, int heads, int rotary_dim,
                              const float* cos_table, const float* sin_table, int64_t table_rows,
                              const leafq_kv8_cache* cache, const leafq_kv8_step* step, const int32_t* positions,

@@ -93,6 +93,7 @@ _SIGNATURES = {
     "leafq_kv8_attention_workspace_bytes": ([_i64, _int, _int, _int], _size),
     "leafq_kv8_attention": ([_vp, _vp, _i64, _int, _int, _vp, _vp, _i64, _vp, _vp, _f32, _vp, _vp, _size, _u32],
                             _int),
+    "leafq_kv8_tree_attention_workspace_bytes": ([_i64, _int, _int, _int], _size),
     "leafq_kv8_tree": ([_vp, _vp, _vp, _vp, _vp, _int, _u32], _int),
     "leafq_kv8_tree_attention": ([_vp, _vp, _i64, _int, _int, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _int, _f32, _vp, _vp,
                                   _size, _u32], _int),

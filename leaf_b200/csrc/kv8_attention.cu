@@ -778,11 +778,23 @@ auto with_dim(int dim, F&& f) {
     }
 }
 
+size_t workspace_bytes(int64_t max_tokens, int heads, int kv_heads, int dim, bool tree) {
+    if (max_tokens <= 0 || max_tokens > INT_MAX || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
+        !kv8_dim_supported(dim))
+        return 0;
+    return with_dim(dim, [&](auto d) {
+        const size_t parts = std::max(split_shape<d(), false>(max_tokens, heads / kv_heads).part_bytes,
+                                      split_shape<d(), true>(max_tokens, heads / kv_heads).part_bytes);
+        const bool tiles = max_tokens * (heads / kv_heads) >= kTileRows;
+        return kCounterBytes + std::max(parts, tiles ? kv8_tile_part_bytes(d(), tree) : 0);
+    });
+}
+
 // Both entry points: of trees where there are masks.
 int attend(const char* what, void* stream, const float* q, int64_t q_stride, int heads, int rotary_dim, const float* cos_table,
            const float* sin_table, int64_t table_rows, const leafq_kv8_cache* cache, const leafq_kv8_step* step,
            const int32_t* positions, const uint32_t* masks, int words, float scale, float* out, void* workspace,
-           size_t workspace_bytes, uint32_t flags) {
+           size_t given_bytes, uint32_t flags) {
     clear_error();
     if (!kv8_cache_valid(cache, what)) return LEAFQ_ERR_INVALID;
     if (!kv8_dim_supported(cache->dim)) {
@@ -809,8 +821,8 @@ int attend(const char* what, void* stream, const float* q, int64_t q_stride, int
         return LEAFQ_ERR_INVALID;
     }
     if (step->max_tokens == 0) return LEAFQ_OK;
-    const size_t need = leafq_kv8_attention_workspace_bytes(step->max_tokens, heads, cache->kv_heads, cache->dim);
-    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
+    const size_t need = workspace_bytes(step->max_tokens, heads, cache->kv_heads, cache->dim, masks != nullptr);
+    if (need > 0 && (!workspace || given_bytes < need || !aligned16(workspace))) {
         set_error(std::string(what) + ": this shape needs " + std::to_string(need) +
                   " bytes of 16-byte aligned workspace");
         return LEAFQ_ERR_INVALID;
@@ -834,15 +846,11 @@ using namespace leafq;
 extern "C" {
 
 size_t leafq_kv8_attention_workspace_bytes(int64_t max_tokens, int heads, int kv_heads, int dim) {
-    if (max_tokens <= 0 || max_tokens > INT_MAX || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
-        !kv8_dim_supported(dim))
-        return 0;
-    return with_dim(dim, [&](auto d) {
-        const size_t parts = std::max(split_shape<d(), false>(max_tokens, heads / kv_heads).part_bytes,
-                                      split_shape<d(), true>(max_tokens, heads / kv_heads).part_bytes);
-        const bool tiles = max_tokens * (heads / kv_heads) >= kTileRows;
-        return kCounterBytes + std::max(parts, tiles ? kv8_tile_part_bytes(d()) : 0);
-    });
+    return workspace_bytes(max_tokens, heads, kv_heads, dim, false);
+}
+
+size_t leafq_kv8_tree_attention_workspace_bytes(int64_t max_tokens, int heads, int kv_heads, int dim) {
+    return workspace_bytes(max_tokens, heads, kv_heads, dim, true);
 }
 
 int leafq_kv8_attention(void* stream, const float* q, int64_t q_stride, int heads, int rotary_dim,

@@ -60,6 +60,12 @@ __device__ __forceinline__ float inverse_of(float l) { return l == 0.0f ? 0.0f :
 // the keys, of kPartTiles tiles or more; the last part to end joins them.
 constexpr int kPartTiles = 4, kMostParts = 16;
 
+// Trees: every item longer than the piece that gives each of kTreePieces one, kTreeTiles at
+// least, is cut into equal parts no longer than it.  Those are no more than 2 kTreePieces:
+// an item of T tiles has T / piece + 1 at most, and is longer than a piece.
+constexpr int kTreeTiles = 16, kTreePieces = kTileBlocks, kTreePlaces = 2 * kTreePieces, kMostTreeParts = 32;
+static_assert(kTreePlaces <= 4 * (kTileBlocks / 2), "a counter for each place");
+
 // What the roles of a block need to know of an item: 128 query rows of one kv
 // head of a request, and, where it is cut into parts, which one.  tiles < 0:
 // there are no more.
@@ -196,6 +202,7 @@ __global__ void __launch_bounds__(TileShape<D>::kThreads, 2)
 kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t* taken, uint32_t* arrivals, float* parts,
                        int row_tiles, int splits) {
     using C = TileShape<D>;
+    constexpr int kSpan = C::kSpan;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* q_rows = smem;  // [kQSlots]: hi, lo
     uint8_t* k_tiles = q_rows + C::kQSlots * 2 * C::kQBytes;
@@ -337,7 +344,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 // only where weights come out above kTileHighest is it raised, with what has
                 // been weighed so far scaled down, exactly but for what is lost below
                 // 2^-30 of the largest.
-                const bool anew = j % C::kSpan == 0;
+                const bool anew = j % kSpan == 0;
                 const float m_before = m;
                 if (j == 0 || __any_sync(~0u, m == -INFINITY && visible > 0)) {
                     float top = -INFINITY;
@@ -429,7 +436,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     ok = __all_sync(~0u, tile_wait(watch, o_done, (n - 1) & 1));
                     if (!ok) break;
                     tcgen05_fence_after();
-                    const bool first = j == C::kSpan;
+                    const bool first = j == kSpan;
                     const float old = first || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m_before);
                     m_sum = m_before;
 #pragma unroll 1
@@ -457,7 +464,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             tcgen05_fence_after();
             // The rows' output: O (and the rounded sum) over L, zeros for a row that
             // sees no key.  A part of an item leaves O, m and l instead.
-            const bool summed = tiles > C::kSpan, whole_item = !kParts || count == 1;
+            const bool summed = tiles > kSpan, whole_item = !kParts || count == 1;
             const float old = !summed || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m);
             const float inverse = !whole_item ? 1.0f : inverse_of(l);
             float* own = parts + (int64_t)(place + part_index) * C::kPart;
@@ -498,11 +505,53 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 uint32_t before = 0;
                 if (lane == 0) {
                     __threadfence();
-                    before = atomicAdd(arrivals + 4 * (place / splits) + warp, 1u);
+                    // (A tree's item has one word, with eight bits a warp.)
+                    if (kTree) before = atomicAdd(arrivals + place, 1u << (8 * warp)) >> (8 * warp) & 0xffu;
+                    else before = atomicAdd(arrivals + 4 * (place / splits) + warp, 1u);
                     __threadfence();
                 }
                 there = __shfl_sync(~0u, before, 0) == static_cast<uint32_t>(count - 1);
-                if (there) {
+                if (kTree && there) {
+                    // Eight float4 of the row at a time, two parts' under way.
+                    const float* first = parts + (int64_t)place * C::kPart;
+                    float top = -INFINITY, total = 0.0f;
+                    float weights[kMostTreeParts];
+#pragma unroll 4
+                    for (int i = 0; i < count; ++i) {
+                        weights[i] = __ldcg(first + i * C::kPart + C::kRows * D + tid);
+                        top = fmaxf(top, weights[i]);
+                    }
+#pragma unroll 4
+                    for (int i = 0; i < count; ++i) {
+                        const float part_l = __ldcg(first + i * C::kPart + C::kRows * (D + 1) + tid);
+                        // (An l that is no number comes through, whatever its m.)
+                        weights[i] = weights[i] == -INFINITY ? (part_l == 0.0f ? 0.0f : 1.0f) : ex2(weights[i] - top);
+                        total = fmaf(weights[i], part_l, total);
+                    }
+                    const float over = total == 0.0f ? 0.0f : inverse_of(total);
+#pragma unroll 1
+                    for (int c = 0; c < D / 4; c += 8) {
+                        float4 y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+                        for (int i = 0; i < count; ++i) {
+                            const float4* from = reinterpret_cast<const float4*>(first + i * C::kPart) + c * C::kRows + tid;
+                            const float weight = weights[i];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float4 v = __ldcg(from + e * C::kRows);
+                                y[e] = make_float4(fmaf(weight, v.x, y[e].x), fmaf(weight, v.y, y[e].y), fmaf(weight, v.z, y[e].z),
+                                                   fmaf(weight, v.w, y[e].w));
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            put_out(c + e, total == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                                         : make_float4(y[e].x * over, y[e].y * over, y[e].z * over, y[e].w * over));
+                    }
+                }
+                if (!kTree && there) {
                     const float* first = parts + (int64_t)place * C::kPart;
                     float top = -INFINITY, total = 0.0f;
 #pragma unroll 1
@@ -561,7 +610,96 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         // the item before is on its way, and tells the other three.
         const uint32_t total = static_cast<uint32_t>(row_tiles) * g.cache.kv_heads * splits;
         bool first_take = true;
-        const auto advance = [&](int it) {
+        // Trees: the requests are gone through once, 32 at a time, as the numbers of the parts
+        // rise; `piece` is the longest part.
+        int window = 0, piece = 0;
+        uint32_t before = 0, places = 0;  // parts, and places of parts, of the requests before the window
+        const auto tiles_of = [&](int s, int& row_tiles_of) {
+            const int begin = max(0, g.step.token_offsets[s]), end = min(g.step.token_offsets[s + 1], static_cast<int>(g.step.tokens));
+            row_tiles_of = (max(0, end - begin) * g.group + C::kRows - 1) / C::kRows;
+            const int held = min(g.step.page_offsets[s + 1] - g.step.page_offsets[s], static_cast<int>(g.step.max_pages));
+            const int seen = max(0, min(min(held << g.shift, g.step.lengths[s]), g.step.context[s] + max(0, end - begin)));
+            return max(1, (seen + C::kKeys - 1) / C::kKeys);
+        };
+        if (kTree && cw == 0) {
+            int64_t all = 0;
+            for (int s = lane; s < g.step.requests; s += 32) {
+                int row_tiles_of;
+                const int64_t tiles = tiles_of(s, row_tiles_of);
+                all += tiles * row_tiles_of;
+            }
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
+            all = (all * g.cache.kv_heads + kTreePieces - 1) / kTreePieces;
+            piece = static_cast<int>(max64(kTreeTiles, all));
+        }
+        const auto advance_tree = [&](int it) {
+            TileItem next = {};
+#pragma unroll 1
+            while (true) {
+                uint32_t id = blockIdx.x;
+                if (!first_take) {
+                    if (lane == 0) id = gridDim.x + atomicAdd(taken, 1u);
+                    id = __shfl_sync(~0u, id, 0);
+                }
+                first_take = false;
+                next.tiles = -1;
+                uint32_t cuts = 1, own = 0, upto = 0, places_upto = 0;
+                int request_tiles = 1, row_tiles_of = 0, hit = -1;
+#pragma unroll 1
+                for (; window < g.step.requests; window += 32) {
+                    request_tiles = 1;
+                    row_tiles_of = 0;
+                    if (window + lane < g.step.requests) request_tiles = tiles_of(window + lane, row_tiles_of);
+                    cuts = request_tiles > piece ? min((request_tiles + piece - 1) / piece, kMostTreeParts) : 1;
+                    upto = own = static_cast<uint32_t>(row_tiles_of) * g.cache.kv_heads * cuts;
+                    places_upto = cuts > 1 ? own : 0;
+#pragma unroll
+                    for (int d = 1; d < 32; d *= 2) {
+                        const uint32_t other = __shfl_up_sync(~0u, upto, d), other_places = __shfl_up_sync(~0u, places_upto, d);
+                        if (lane >= d) {
+                            upto += other;
+                            places_upto += other_places;
+                        }
+                    }
+                    const uint32_t beyond = __ballot_sync(~0u, before + upto > id);
+                    if (beyond != 0) {
+                        hit = __ffs(beyond) - 1;
+                        break;
+                    }
+                    before += __shfl_sync(~0u, upto, 31);
+                    places += __shfl_sync(~0u, places_upto, 31);
+                }
+                if (hit < 0) break;
+                const int s = window + hit;
+                const uint32_t index = id - before - __shfl_sync(~0u, upto - own, hit), first_place = places + __shfl_sync(~0u, places_upto - (cuts > 1 ? own : 0), hit);
+                cuts = __shfl_sync(~0u, cuts, hit);
+                request_tiles = __shfl_sync(~0u, request_tiles, hit);
+                const uint32_t whole = index / cuts, part = index - whole * cuts, row_tile = whole / static_cast<uint32_t>(g.cache.kv_heads);
+                const int begin = max(0, g.step.token_offsets[s]), end = min(g.step.token_offsets[s + 1], static_cast<int>(g.step.tokens));
+                next.head = static_cast<int>(whole - row_tile * g.cache.kv_heads);
+                next.row0 = begin;
+                next.first_row = static_cast<int>(row_tile) * C::kRows;
+                next.rows = min(C::kRows, (end - begin) * g.group - next.first_row);
+                next.context = g.step.context[s];
+                next.request = s;
+                const int held = min(g.step.page_offsets[s + 1] - g.step.page_offsets[s], static_cast<int>(g.step.max_pages));
+                const int seen = next.context + token_of(next.first_row + next.rows - 1) + 1;  // by the last row
+                next.keys = max(0, min(min(held << g.shift, g.step.lengths[s]), seen));
+                const int tiles = max(1, (next.keys + C::kKeys - 1) / C::kKeys);
+                // The request's tiles are cut; the parts behind this item's last tile have none.
+                const auto bound = [&](uint32_t i) { return static_cast<int>((int64_t)request_tiles * i / cuts); };
+                next.parts = __popc(__ballot_sync(~0u, lane < cuts && bound(lane) < tiles));
+                if (static_cast<int>(part) >= next.parts) continue;
+                next.part = static_cast<int>(part);
+                next.place = static_cast<int>(first_place + whole * cuts);
+                next.tile0 = bound(part);
+                next.tiles = (static_cast<int>(part) + 1 == next.parts ? tiles : bound(part + 1)) - next.tile0;
+                break;
+            }
+            return next;
+        };
+        const auto advance_causal = [&](int it) {
             TileItem next = {};
 #pragma unroll 1
             while (true) {
@@ -612,6 +750,10 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 }
                 break;
             }
+            return next;
+        };
+        const auto advance = [&](int it) {
+            const TileItem next = kTree ? advance_tree(it) : advance_causal(it);
             if (lane == 0) {
                 items[it % C::kItems] = next;
                 mbar_arrive(&found_full[it % C::kItems]);
@@ -895,7 +1037,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 if (!ok) break;
                 tcgen05_fence_after();
                 const uint64_t v = vt + stage * (C::kKvBytes >> 4);
-                const uint32_t p_tmem = tmem + (n & 1) * C::kKeys, more = j % C::kSpan > 0;
+                const uint32_t p_tmem = tmem + (n & 1) * C::kKeys, more = j % kSpan > 0;
                 if (leader) {
 #pragma unroll
                     for (int i = 0; i < C::kKeys / 16; ++i)
@@ -929,7 +1071,8 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         if (atomicAdd(taken + 1, 1u) == gridDim.x - 1) {
             taken[0] = taken[1] = 0;
             if (kParts)
-                for (int i = 0; i < row_tiles * g.cache.kv_heads; ++i) reinterpret_cast<uint4*>(arrivals)[i] = make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < (kTree ? kTreePlaces / 4 : row_tiles * g.cache.kv_heads); ++i)
+                    reinterpret_cast<uint4*>(arrivals)[i] = make_uint4(0, 0, 0, 0);
         }
     }
 }
@@ -949,9 +1092,7 @@ int run_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) 
         return LEAFQ_ERR_INVALID;
     }
     const int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostParts, kTileBlocks / (row_tiles * g.cache.kv_heads))));
-    if (g.masks)
-        return splits > 1 ? start_tile<D, true, true>(s, g, workspace, row_tiles, splits, pdl)
-                          : start_tile<D, false, true>(s, g, workspace, row_tiles, 1, pdl);
+    if (g.masks) return start_tile<D, true, true>(s, g, workspace, row_tiles, kMostTreeParts, pdl);
     return splits > 1 ? start_tile<D, true, false>(s, g, workspace, row_tiles, splits, pdl)
                       : start_tile<D, false, false>(s, g, workspace, row_tiles, 1, pdl);
 }
@@ -983,7 +1124,7 @@ int start_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, int64_t 
 
 }  // namespace
 
-size_t kv8_tile_part_bytes(int dim) { return sizeof(float) * kTileBlocks * 128 * (dim + 2); }
+size_t kv8_tile_part_bytes(int dim, bool tree) { return sizeof(float) * (tree ? kTreePlaces : kTileBlocks) * 128 * (dim + 2); }
 
 int launch_kv8_tiles(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) {
     switch (g.cache.dim) {

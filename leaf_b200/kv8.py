@@ -209,12 +209,13 @@ class Kv8Workspace:
             self.buffer = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
         return self.buffer
 
-    def of(self, max_tokens: int, heads: int, kv_heads: int, dim: int):
+    def of(self, max_tokens: int, heads: int, kv_heads: int, dim: int, tree: bool = False):
         """(address, bytes) for a geometry."""
-        key = (max_tokens, heads, kv_heads, dim)
+        key = (max_tokens, heads, kv_heads, dim, tree)
         need = self.sizes.get(key)
         if need is None:
-            need = self.sizes[key] = load().leafq_kv8_attention_workspace_bytes(*key)
+            size = load().leafq_kv8_tree_attention_workspace_bytes if tree else load().leafq_kv8_attention_workspace_bytes
+            need = self.sizes[key] = size(*key[:4])
         return self.get(need).data_ptr(), need
 
 
@@ -324,13 +325,14 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, plan: Kv8Plan, scale: float,
         workspace = Kv8Workspace(cache.device)  # in a name of its own, until the launch is enqueued
     elif workspace.index != index:
         _fail("the workspace is on another device")
-    address, need = workspace.of(plan.max_tokens, heads, cache.kv_heads, dim)
     if tree is not None:
         tree.fits(plan)
+        address, need = workspace.of(plan.max_tokens, heads, cache.kv_heads, dim, True)
         check(load().leafq_kv8_tree_attention(_raw_stream(index), q.data_ptr(), stride, heads, rotary, cos, sin, rows,
                                               cache.ref, plan.ref, tree.address[0], tree.address[1], tree.words, scale,
                                               out.data_ptr(), address, need, flags))
         return out
+    address, need = workspace.of(plan.max_tokens, heads, cache.kv_heads, dim)
     check(load().leafq_kv8_attention(_raw_stream(index), q.data_ptr(), stride, heads, rotary, cos, sin, rows, cache.ref,
                                      plan.ref, scale, out.data_ptr(), address, need, flags))
     return out

@@ -45,6 +45,7 @@ def test_tree_rejects(change):
 def test_trees_of_too_many_rows():
     assert _tree(step=_step(max_tokens=1025), words=32) == _lib.LEAFQ_ERR_UNSUPPORTED
     assert _verify(most=1025) == _lib.LEAFQ_ERR_UNSUPPORTED
+    assert _verify(vocab=2**20 + 1, stride=2**21, probs_stride=2**21) == _lib.LEAFQ_ERR_UNSUPPORTED
 
 
 def _attend(cache=None, step=None, q=P, stride=256, heads=4, rotary=0, cos=None, sin=None, rows=0, positions=P, masks=P, words=1,
@@ -106,8 +107,7 @@ def _verify(logits=P, stride=100, vocab=100, ids=P, parents=P, offsets=P, reques
                                            heat, probs, probs_stride, path, out, kept, nxt, 0)
 
 
-@pytest.mark.parametrize("change", [dict(vocab=0), dict(vocab=-5), dict(vocab=2**20 + 1, stride=2**21, probs_stride=2**21),
-                                    dict(requests=-1), dict(requests=2**31 // 8), dict(tokens=-1), dict(tokens=2**31), dict(most=-1),
+@pytest.mark.parametrize("change", [dict(vocab=0), dict(vocab=-5), dict(requests=-1), dict(requests=2**31 // 8), dict(tokens=-1), dict(tokens=2**31), dict(most=-1),
                                     dict(stride=99), dict(probs_stride=99), dict(logits=None), dict(ids=None), dict(parents=None),
                                     dict(offsets=None), dict(accept=None), dict(sample=None), dict(heat=None), dict(path=None),
                                     dict(out=None), dict(kept=None), dict(nxt=None)])

@@ -13,7 +13,7 @@ Tolerances, with u = 2^-24:
   turning out the other way than the operator's own error: for a child 2^-17 of p (the
   exponentials' 32 bits: 2 ulp each and an exponent of up to 2^5 rounded to 2^-24 of itself,
   2^-18.5 at most), for a draw 2^-40 of the sum (64-bit sums of up to 2^20 terms, each of them
-  within 2^-50).  Where a request is nearer than that it is left out, and at most 2 % may be.
+  within 2^-46).  Where a request is nearer than that it is left out, and at most 2 % may be.
 """
 import numpy as np
 import pytest
