@@ -23,7 +23,7 @@ SOURCES = ["act_quant.cu", "gemv_w8a8.cu", "gemv_w4a32.cu", "linear_generic.cu",
            "peer_allgather.cu", "decoder_ops.cu", "decode_model.cu", "kv8_cache.cu", "kv8_attention.cu", "kv8_tree.cu",
            "verify_drafts.cu"]
 # Compiled as whole programs: setmaxnreg is ignored in relocatable device code.
-WHOLE_SOURCES = ["kv8_tile.cu"]
+WHOLE_SOURCES = ["kv8_tile.cu", "kv8_tree_tile.cu"]
 GENCODE = "arch=compute_100a,code=sm_100a"
 
 

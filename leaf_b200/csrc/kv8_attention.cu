@@ -786,7 +786,7 @@ size_t workspace_bytes(int64_t max_tokens, int heads, int kv_heads, int dim, boo
         const size_t parts = std::max(split_shape<d(), false>(max_tokens, heads / kv_heads).part_bytes,
                                       split_shape<d(), true>(max_tokens, heads / kv_heads).part_bytes);
         const bool tiles = max_tokens * (heads / kv_heads) >= kTileRows;
-        return kCounterBytes + std::max(parts, tiles ? kv8_tile_part_bytes(d(), tree) : 0);
+        return kCounterBytes + std::max(parts, !tiles ? 0 : tree ? kv8_tree_part_bytes(d()) : kv8_tile_part_bytes(d()));
     });
 }
 
@@ -832,7 +832,8 @@ int attend(const char* what, void* stream, const float* q, int64_t q_stride, int
     while ((1 << g.shift) < cache->page) ++g.shift;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool pdl = (flags & LEAFQ_FLAG_PDL) != 0;
-    if (takes_tiles(step->tokens, step->max_tokens, heads, g.group)) return launch_kv8_tiles(s, g, workspace, pdl);
+    if (takes_tiles(step->tokens, step->max_tokens, heads, g.group))
+        return masks ? launch_kv8_tree_tiles(s, g, workspace, pdl) : launch_kv8_tiles(s, g, workspace, pdl);
     return with_dim(cache->dim, [&](auto d) {
         return masks ? run_split<d(), false, true>(s, g, workspace, pdl) : run_split<d(), false, false>(s, g, workspace, pdl);
     });

@@ -160,7 +160,10 @@ constexpr size_t kCounterBytes = 16384;
 static_assert((kTileCounters + 4 + 4 * (kTileBlocks / 2)) * 4 <= kCounterBytes, "the items that have parts, four counters each");
 
 // Many query rows of a request (kv8_tile.cu), and what its parts take.
-size_t kv8_tile_part_bytes(int dim, bool tree);
+size_t kv8_tile_part_bytes(int dim);
 int launch_kv8_tiles(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl);
+// The same for trees (kv8_tree_tile.cu).
+size_t kv8_tree_part_bytes(int dim);
+int launch_kv8_tree_tiles(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl);
 
 }  // namespace leafq

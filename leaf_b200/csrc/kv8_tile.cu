@@ -2,12 +2,10 @@
 //
 // Compiled as a whole program (build.py): setmaxnreg is ignored in relocatable
 // device code.
-#define LEAFQ_WHOLE_PROGRAM
 #include <algorithm>
-#include <cfloat>
 #include <type_traits>
 
-#include "kv8_attention.cuh"
+#include "kv8_tile.cuh"
 
 namespace leafq {
 namespace {
@@ -42,29 +40,10 @@ namespace {
 // prompts of 512 tokens 360 us (191 TFLOP/s, twice that in the MMAs, since fp32
 // operands are two halves); one of 8,192 tokens 612 us (449 TFLOP/s).  5 chunks
 // of 100 to 1,500 tokens, 8 heads of 128, 3 queries a key, 83 us (252 TFLOP/s).
-constexpr float kTileLift = 6.0f, kTileHighest = 49152.0f;
-// Two kinds of pages need no test in the softmax (one a tile took 2 % of the time): what
-// stands for their V scale does it.  Values of zero count in L as any other, as of scale
-// 2^kZeroLog2, with a reference that stands kZeroAbove over their scores (below those of
-// the scales that an append gives), which leaves their weights at 2^-37, zeros in fp16.
-// (Where later scores are 2^12 times as heavy, and no other page's raise the reference,
-// they come through as values below 2^-76.)  Scales that are no numbers: every key that
-// a row sees weighs one, the reference is out of all others' reach, and L passes
-// kNoNumber; a row that sees none of them keeps its own.
-constexpr float kZeroLog2 = -83.0f, kZeroInverse = 0x1p83f, kZeroAbove = 43.0f;
-constexpr float kNoNumberLog2 = 1e30f, kNoNumber = 3e38f;
-// 1 / L: none for a row that sees no key, and for one that sees a scale that is no number.
-__device__ __forceinline__ float inverse_of(float l) { return l == 0.0f ? 0.0f : l > kNoNumber ? NAN : __frcp_rn(l); }
 
 // Where there are fewer items than half the blocks, each is cut into parts along
 // the keys, of kPartTiles tiles or more; the last part to end joins them.
 constexpr int kPartTiles = 4, kMostParts = 16;
-
-// Trees: every item longer than the piece that gives each of kTreePieces one, kTreeTiles at
-// least, is cut into equal parts no longer than it.  Those are no more than 2 kTreePieces:
-// an item of T tiles has T / piece + 1 at most, and is longer than a piece.
-constexpr int kTreeTiles = 16, kTreePieces = kTileBlocks, kTreePlaces = 2 * kTreePieces, kMostTreeParts = 32;
-static_assert(kTreePlaces <= 4 * (kTileBlocks / 2), "a counter for each place");
 
 // What the roles of a block need to know of an item: 128 query rows of one kv
 // head of a request, and, where it is cut into parts, which one.  tiles < 0:
@@ -107,102 +86,14 @@ struct TileShape {
     static_assert(kSoftmaxRegs + kOtherRegs <= 2 * kLaunchRegs, "the split of what the launch gives each scheduler");
 };
 
-// The library's device error word and wait limit (leafq_device.cuh), which this
-// file, compiled as a whole program, cannot name.
-__device__ __forceinline__ void report(const DeviceWatch& w, unsigned site) {
-    atomicCAS(w.error, 0u, (site << 16) | (blockIdx.x & 0xffffu));
-}
-
-// Bounded wait that other requests' range errors do not end.
-__device__ __forceinline__ bool tile_wait(const DeviceWatch& w, uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const unsigned long long start = global_timer_ns();
-    do {
-        if (mbar_try_wait(bar, parity)) return true;
-    } while (global_timer_ns() - start <= *static_cast<volatile const unsigned long long*>(w.limit_ns));
-    report(w, kSiteKv8Tile);
-    return false;
-}
-
-__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// The A operand from tensor memory: two fp16 per 32-bit column.
-__device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// Instruction descriptor for kind::f16: fp32 accumulator (1) in [4,6), fp16 A
-// and B (0), B MN-major (bit 16) or K-major, N >> 3 in [17,23), M >> 4 in [24,29).
-__host__ __device__ constexpr uint32_t umma_idesc_f16(uint32_t m, uint32_t n, bool b_mn) {
-    return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((m >> 4) << 24);
-}
-
-__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// Loads of read-only data that stay where they are written, ahead of their use.
-__device__ __forceinline__ uint4 load_now(const uint4* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ float4 load_now(const float4* p) {
-    float4 v;
-    asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ int32_t load_now(const int32_t* p) {
-    int32_t v;
-    asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ float load_now(const float* p) {
-    float v;
-    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
-    return v;
-}
-
-// An array that stays in local memory: its address, and 16 bytes of it.
-__device__ __forceinline__ uint32_t local_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_local(p)); }
-__device__ __forceinline__ float4 load_local(uint32_t at) {
-    float4 v;
-    asm volatile("ld.local.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-    return v;
-}
-__device__ __forceinline__ void store_local(uint32_t at, float4 v) {
-    asm volatile("st.local.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
-}
-
 // kParts: some items are cut into parts (the code that joins them is left out of
 // the other kernel, whose loops it would push out of the instruction cache:
 // 64 prompts of 512 tokens 368 us without it, 379 us with it).
-// kTree: the request's new rows see those of the new keys that their masks name.
-template <int D, bool kParts, bool kTree>
+template <int D, bool kParts>
 __global__ void __launch_bounds__(TileShape<D>::kThreads, 2)
 kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t* taken, uint32_t* arrivals, float* parts,
                        int row_tiles, int splits) {
     using C = TileShape<D>;
-    constexpr int kSpan = C::kSpan;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* q_rows = smem;  // [kQSlots]: hi, lo
     uint8_t* k_tiles = q_rows + C::kQSlots * 2 * C::kQBytes;
@@ -295,10 +186,9 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             }
             const int r = tid;
             const int t = token_of(first_row + r), hq = (first_row + r) - t * g.group;
-            const int pos = !kTree ? context + t : r < rows ? g.positions[row0 + t] : -1;
+            const int pos = context + t;
             const bool seen = r < rows && pos >= 0 && (g.rotary == 0 || pos < g.table_rows);
-            const int limit = seen ? min(keys, context + t + 1) : 0;
-            const uint32_t* row_mask = kTree ? g.masks + (int64_t)(row0 + token_of(first_row + min(r, rows - 1))) * g.mask_words : nullptr;
+            const int limit = seen ? min(keys, pos + 1) : 0;
             float* out = g.out + ((int64_t)row0 + t) * g.heads * D + (int64_t)(head * g.group + hq) * D;
             float m = -INFINITY, l = 0.0f, m_sum = -INFINITY;
             for (int j = 0; j < tiles; ++j, ++n) {
@@ -308,8 +198,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 tcgen05_fence_after();
                 const float4* scales = info + (n % C::kInfo) * C::kGroups;
                 const int visible = limit - (tile0 + j) * C::kKeys;  // columns of this tile that the row sees
-                const int drafted = (tile0 + j) * C::kKeys - context;  // the tile's first key among the request's new ones
-                const bool whole = __all_sync(~0u, visible >= C::kKeys) && !(kTree && drafted + C::kKeys > 0);
+                const bool whole = __all_sync(~0u, visible >= C::kKeys);
                 // 32 scores at a time, by rolled loops: the roles' loops have to stay in the
                 // instruction cache side by side (unrolled, with all scores in registers,
                 // the kernel took 1.5 times as long).  What is not seen is -inf.
@@ -318,10 +207,8 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     tmem_ld_32x32b_x32(s_tmem + lanes + 32 * c, x);
                     tmem_wait_ld();
                     if (!whole) {
-                        const uint32_t window = kTree ? tree_window(row_mask, g.mask_words, drafted + 32 * c) : ~0u;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            x[e] = 32 * c + e >= visible || (kTree && !(window >> e & 1u)) ? 0xff800000u : x[e];
+                        for (int e = 0; e < 32; ++e) x[e] = 32 * c + e >= visible ? 0xff800000u : x[e];
                     }
                 };
                 // From an MMA sum to x_j: above zero, so that -inf stays.
@@ -344,7 +231,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 // only where weights come out above kTileHighest is it raised, with what has
                 // been weighed so far scaled down, exactly but for what is lost below
                 // 2^-30 of the largest.
-                const bool anew = j % kSpan == 0;
+                const bool anew = j % C::kSpan == 0;
                 const float m_before = m;
                 if (j == 0 || __any_sync(~0u, m == -INFINITY && visible > 0)) {
                     float top = -INFINITY;
@@ -436,7 +323,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     ok = __all_sync(~0u, tile_wait(watch, o_done, (n - 1) & 1));
                     if (!ok) break;
                     tcgen05_fence_after();
-                    const bool first = j == kSpan;
+                    const bool first = j == C::kSpan;
                     const float old = first || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m_before);
                     m_sum = m_before;
 #pragma unroll 1
@@ -464,7 +351,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             tcgen05_fence_after();
             // The rows' output: O (and the rounded sum) over L, zeros for a row that
             // sees no key.  A part of an item leaves O, m and l instead.
-            const bool summed = tiles > kSpan, whole_item = !kParts || count == 1;
+            const bool summed = tiles > C::kSpan, whole_item = !kParts || count == 1;
             const float old = !summed || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m);
             const float inverse = !whole_item ? 1.0f : inverse_of(l);
             float* own = parts + (int64_t)(place + part_index) * C::kPart;
@@ -505,53 +392,11 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 uint32_t before = 0;
                 if (lane == 0) {
                     __threadfence();
-                    // (A tree's item has one word, with eight bits a warp.)
-                    if (kTree) before = atomicAdd(arrivals + place, 1u << (8 * warp)) >> (8 * warp) & 0xffu;
-                    else before = atomicAdd(arrivals + 4 * (place / splits) + warp, 1u);
+                    before = atomicAdd(arrivals + 4 * (place / splits) + warp, 1u);
                     __threadfence();
                 }
                 there = __shfl_sync(~0u, before, 0) == static_cast<uint32_t>(count - 1);
-                if (kTree && there) {
-                    // Eight float4 of the row at a time, two parts' under way.
-                    const float* first = parts + (int64_t)place * C::kPart;
-                    float top = -INFINITY, total = 0.0f;
-                    float weights[kMostTreeParts];
-#pragma unroll 4
-                    for (int i = 0; i < count; ++i) {
-                        weights[i] = __ldcg(first + i * C::kPart + C::kRows * D + tid);
-                        top = fmaxf(top, weights[i]);
-                    }
-#pragma unroll 4
-                    for (int i = 0; i < count; ++i) {
-                        const float part_l = __ldcg(first + i * C::kPart + C::kRows * (D + 1) + tid);
-                        // (An l that is no number comes through, whatever its m.)
-                        weights[i] = weights[i] == -INFINITY ? (part_l == 0.0f ? 0.0f : 1.0f) : ex2(weights[i] - top);
-                        total = fmaf(weights[i], part_l, total);
-                    }
-                    const float over = total == 0.0f ? 0.0f : inverse_of(total);
-#pragma unroll 1
-                    for (int c = 0; c < D / 4; c += 8) {
-                        float4 y[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 2
-                        for (int i = 0; i < count; ++i) {
-                            const float4* from = reinterpret_cast<const float4*>(first + i * C::kPart) + c * C::kRows + tid;
-                            const float weight = weights[i];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const float4 v = __ldcg(from + e * C::kRows);
-                                y[e] = make_float4(fmaf(weight, v.x, y[e].x), fmaf(weight, v.y, y[e].y), fmaf(weight, v.z, y[e].z),
-                                                   fmaf(weight, v.w, y[e].w));
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            put_out(c + e, total == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                                                         : make_float4(y[e].x * over, y[e].y * over, y[e].z * over, y[e].w * over));
-                    }
-                }
-                if (!kTree && there) {
+                if (there) {
                     const float* first = parts + (int64_t)place * C::kPart;
                     float top = -INFINITY, total = 0.0f;
 #pragma unroll 1
@@ -610,96 +455,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         // the item before is on its way, and tells the other three.
         const uint32_t total = static_cast<uint32_t>(row_tiles) * g.cache.kv_heads * splits;
         bool first_take = true;
-        // Trees: the requests are gone through once, 32 at a time, as the numbers of the parts
-        // rise; `piece` is the longest part.
-        int window = 0, piece = 0;
-        uint32_t before = 0, places = 0;  // parts, and places of parts, of the requests before the window
-        const auto tiles_of = [&](int s, int& row_tiles_of) {
-            const int begin = max(0, g.step.token_offsets[s]), end = min(g.step.token_offsets[s + 1], static_cast<int>(g.step.tokens));
-            row_tiles_of = (max(0, end - begin) * g.group + C::kRows - 1) / C::kRows;
-            const int held = min(g.step.page_offsets[s + 1] - g.step.page_offsets[s], static_cast<int>(g.step.max_pages));
-            const int seen = max(0, min(min(held << g.shift, g.step.lengths[s]), g.step.context[s] + max(0, end - begin)));
-            return max(1, (seen + C::kKeys - 1) / C::kKeys);
-        };
-        if (kTree && cw == 0) {
-            int64_t all = 0;
-            for (int s = lane; s < g.step.requests; s += 32) {
-                int row_tiles_of;
-                const int64_t tiles = tiles_of(s, row_tiles_of);
-                all += tiles * row_tiles_of;
-            }
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
-            all = (all * g.cache.kv_heads + kTreePieces - 1) / kTreePieces;
-            piece = static_cast<int>(max64(kTreeTiles, all));
-        }
-        const auto advance_tree = [&](int it) {
-            TileItem next = {};
-#pragma unroll 1
-            while (true) {
-                uint32_t id = blockIdx.x;
-                if (!first_take) {
-                    if (lane == 0) id = gridDim.x + atomicAdd(taken, 1u);
-                    id = __shfl_sync(~0u, id, 0);
-                }
-                first_take = false;
-                next.tiles = -1;
-                uint32_t cuts = 1, own = 0, upto = 0, places_upto = 0;
-                int request_tiles = 1, row_tiles_of = 0, hit = -1;
-#pragma unroll 1
-                for (; window < g.step.requests; window += 32) {
-                    request_tiles = 1;
-                    row_tiles_of = 0;
-                    if (window + lane < g.step.requests) request_tiles = tiles_of(window + lane, row_tiles_of);
-                    cuts = request_tiles > piece ? min((request_tiles + piece - 1) / piece, kMostTreeParts) : 1;
-                    upto = own = static_cast<uint32_t>(row_tiles_of) * g.cache.kv_heads * cuts;
-                    places_upto = cuts > 1 ? own : 0;
-#pragma unroll
-                    for (int d = 1; d < 32; d *= 2) {
-                        const uint32_t other = __shfl_up_sync(~0u, upto, d), other_places = __shfl_up_sync(~0u, places_upto, d);
-                        if (lane >= d) {
-                            upto += other;
-                            places_upto += other_places;
-                        }
-                    }
-                    const uint32_t beyond = __ballot_sync(~0u, before + upto > id);
-                    if (beyond != 0) {
-                        hit = __ffs(beyond) - 1;
-                        break;
-                    }
-                    before += __shfl_sync(~0u, upto, 31);
-                    places += __shfl_sync(~0u, places_upto, 31);
-                }
-                if (hit < 0) break;
-                const int s = window + hit;
-                const uint32_t index = id - before - __shfl_sync(~0u, upto - own, hit), first_place = places + __shfl_sync(~0u, places_upto - (cuts > 1 ? own : 0), hit);
-                cuts = __shfl_sync(~0u, cuts, hit);
-                request_tiles = __shfl_sync(~0u, request_tiles, hit);
-                const uint32_t whole = index / cuts, part = index - whole * cuts, row_tile = whole / static_cast<uint32_t>(g.cache.kv_heads);
-                const int begin = max(0, g.step.token_offsets[s]), end = min(g.step.token_offsets[s + 1], static_cast<int>(g.step.tokens));
-                next.head = static_cast<int>(whole - row_tile * g.cache.kv_heads);
-                next.row0 = begin;
-                next.first_row = static_cast<int>(row_tile) * C::kRows;
-                next.rows = min(C::kRows, (end - begin) * g.group - next.first_row);
-                next.context = g.step.context[s];
-                next.request = s;
-                const int held = min(g.step.page_offsets[s + 1] - g.step.page_offsets[s], static_cast<int>(g.step.max_pages));
-                const int seen = next.context + token_of(next.first_row + next.rows - 1) + 1;  // by the last row
-                next.keys = max(0, min(min(held << g.shift, g.step.lengths[s]), seen));
-                const int tiles = max(1, (next.keys + C::kKeys - 1) / C::kKeys);
-                // The request's tiles are cut; the parts behind this item's last tile have none.
-                const auto bound = [&](uint32_t i) { return static_cast<int>((int64_t)request_tiles * i / cuts); };
-                next.parts = __popc(__ballot_sync(~0u, lane < cuts && bound(lane) < tiles));
-                if (static_cast<int>(part) >= next.parts) continue;
-                next.part = static_cast<int>(part);
-                next.place = static_cast<int>(first_place + whole * cuts);
-                next.tile0 = bound(part);
-                next.tiles = (static_cast<int>(part) + 1 == next.parts ? tiles : bound(part + 1)) - next.tile0;
-                break;
-            }
-            return next;
-        };
-        const auto advance_causal = [&](int it) {
+        const auto advance = [&](int it) {
             TileItem next = {};
 #pragma unroll 1
             while (true) {
@@ -750,10 +506,6 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 }
                 break;
             }
-            return next;
-        };
-        const auto advance = [&](int it) {
-            const TileItem next = kTree ? advance_tree(it) : advance_causal(it);
             if (lane == 0) {
                 items[it % C::kItems] = next;
                 mbar_arrive(&found_full[it % C::kItems]);
@@ -796,9 +548,9 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                     a1 = load_now(reinterpret_cast<const float4*>(src + at));
                     b1 = load_now(reinterpret_cast<const float4*>(src + to));
                     if (turned) {
-                        int64_t pos = kTree ? load_now(g.positions + (next.row0 + t)) : (int64_t)next.context + t;
+                        int64_t pos = (int64_t)next.context + t;
                         if (pos < 0 || pos >= g.table_rows) {
-                            if (part == 0 && !(kTree && pos < 0)) report(watch, kSiteKv8Range);
+                            if (part == 0) report(watch, kSiteKv8Range);
                             pos = 0;
                         }
                         cs1 = load_now(reinterpret_cast<const float4*>(g.cos_table + pos * half + at));
@@ -1037,7 +789,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 if (!ok) break;
                 tcgen05_fence_after();
                 const uint64_t v = vt + stage * (C::kKvBytes >> 4);
-                const uint32_t p_tmem = tmem + (n & 1) * C::kKeys, more = j % kSpan > 0;
+                const uint32_t p_tmem = tmem + (n & 1) * C::kKeys, more = j % C::kSpan > 0;
                 if (leader) {
 #pragma unroll
                     for (int i = 0; i < C::kKeys / 16; ++i)
@@ -1071,13 +823,12 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         if (atomicAdd(taken + 1, 1u) == gridDim.x - 1) {
             taken[0] = taken[1] = 0;
             if (kParts)
-                for (int i = 0; i < (kTree ? kTreePlaces / 4 : row_tiles * g.cache.kv_heads); ++i)
-                    reinterpret_cast<uint4*>(arrivals)[i] = make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < row_tiles * g.cache.kv_heads; ++i) reinterpret_cast<uint4*>(arrivals)[i] = make_uint4(0, 0, 0, 0);
         }
     }
 }
 
-template <int D, bool kParts, bool kTree>
+template <int D, bool kParts>
 int start_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, int64_t row_tiles, int splits, bool pdl);
 
 template <int D>
@@ -1092,17 +843,16 @@ int run_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) 
         return LEAFQ_ERR_INVALID;
     }
     const int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostParts, kTileBlocks / (row_tiles * g.cache.kv_heads))));
-    if (g.masks) return start_tile<D, true, true>(s, g, workspace, row_tiles, kMostTreeParts, pdl);
-    return splits > 1 ? start_tile<D, true, false>(s, g, workspace, row_tiles, splits, pdl)
-                      : start_tile<D, false, false>(s, g, workspace, row_tiles, 1, pdl);
+    return splits > 1 ? start_tile<D, true>(s, g, workspace, row_tiles, splits, pdl)
+                      : start_tile<D, false>(s, g, workspace, row_tiles, 1, pdl);
 }
 
-template <int D, bool kParts, bool kTree>
+template <int D, bool kParts>
 int start_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, int64_t row_tiles, int splits, bool pdl) {
     DeviceWatch watch;
     int st = device_watch(&watch);
     if (st) return st;
-    const void* kernel = reinterpret_cast<const void*>(kv8_attend_tile_kernel<D, kParts, kTree>);
+    const void* kernel = reinterpret_cast<const void*>(kv8_attend_tile_kernel<D, kParts>);
     static const int registers = [kernel] {
         cudaFuncAttributes a;
         return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0;
@@ -1116,7 +866,7 @@ int start_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, int64_t 
     if (st) return st;
     const int64_t blocks = std::min<int64_t>(row_tiles * g.cache.kv_heads * splits, 2 * (int64_t)sm_count());
     uint32_t* counters = static_cast<uint32_t*>(workspace) + kTileCounters;
-    return launch(kv8_attend_tile_kernel<D, kParts, kTree>, dim3(static_cast<unsigned>(blocks)),
+    return launch(kv8_attend_tile_kernel<D, kParts>, dim3(static_cast<unsigned>(blocks)),
                   dim3(TileShape<D>::kThreads), TileShape<D>::kSmem, s, pdl, "leafq_kv8_attention", g, watch,
                   counters, counters + 4, reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes),
                   static_cast<int>(row_tiles), splits);
@@ -1124,7 +874,7 @@ int start_tile(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, int64_t 
 
 }  // namespace
 
-size_t kv8_tile_part_bytes(int dim, bool tree) { return sizeof(float) * (tree ? kTreePlaces : kTileBlocks) * 128 * (dim + 2); }
+size_t kv8_tile_part_bytes(int dim) { return sizeof(float) * kTileBlocks * 128 * (dim + 2); }
 
 int launch_kv8_tiles(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) {
     switch (g.cache.dim) {
