@@ -19,8 +19,7 @@ namespace {
 //   warps 0-3, 4-7  softmax of a half: one row per thread (its TMEM lane)
 //   warps 8-11      codes to fp16: two warps K, two V
 //   warps 12, 13    MMA issue, a half each
-//   warp 14         the items
-//   warps 16-19     their query rows (warp 15 has nothing to do)
+//   warps 14, 15    the items and their query rows, the first half's first
 // A unit is a tile of keys for one half.  The tensor pipe has one half's units while the other
 // is in its softmax; one warp that issued for both halves was itself what they waited for (some
 // 250 instructions a unit, one after another).
@@ -38,7 +37,7 @@ struct TreeItem {
 // the blocks in even shares.  An item of more than kShortTiles tiles is cut where a share
 // ends, a shorter one goes to the block that has its middle: a join would take longer.  A
 // share is kLeastShare units at least, so that every part of an item has a tile.
-constexpr int kTreeBlocks = 148, kTreePlaces = 2 * kTreeBlocks, kShortTiles = 32, kLeastShare = 32, kItemCost = 3;
+constexpr int kTreeBlocks = 148, kTreePlaces = 2 * kTreeBlocks, kShortTiles = 32, kLeastShare = 32;
 static_assert((kTileCounters + 4 + 2 * kTreeBlocks) * 4 <= kCounterBytes, "two counters for each block");
 static_assert(kTreePlaces % 4 == 0, "the counters are zeroed four at a time");
 
@@ -54,22 +53,23 @@ struct TreeShape {
     static constexpr int kQSlots = D <= 64 ? 2 : 1;      // of query rows: the next item's beside this one's
     static constexpr int kItems = 3;                     // ring of their descriptions
     static constexpr int kKvBytes = kBlocks * kKeys * 128;
-    static constexpr int kSpan = 384 / kKeys;            // a half's tiles between O's additions to the rounded sum
-    static constexpr int kThreads = 640;
-    // A scheduler has two softmax warps, a converting one, one of warps 12 to 15 and one for rows.
-    static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 136, kConvertRegs = 88, kIssueRegs = 56, kRowsRegs = 64;
+    static constexpr int kSpan = (D <= 64 ? 384 : 512) / kKeys;           // a half's tiles between O's additions to the rounded sum
+    static constexpr int kItemCost = D <= 64 ? 4 : 6;    // of an item for its own sake, in units
+    static constexpr int kThreads = 512;
+    // A scheduler has two softmax warps, a converting one and one of the last four.
+    static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 152, kConvertRegs = 104, kOtherRegs = 104;
     static constexpr int kPieces = kKeys * D / 16 / 64;  // 16-byte pieces of a K (or V) tile per converting thread
     static constexpr int kOutCols = kBlocks * 64;        // O columns (those past D are not read)
     static constexpr int kHalfCols = 256;
     static constexpr int kPart = kHalves * kRows * (D + 2);  // floats of a part's result: O [D / 4][256][4], m [256], l [256]
-    static constexpr size_t kBarriers = 4 * kStages + 6 * kHalves + 2 * kQSlots + kItems + 3 + kHalves;
+    static constexpr size_t kBarriers = 4 * kStages + 6 * kHalves + 3 * kQSlots + kItems + 2 + kHalves;
     static constexpr size_t kSmem = kQSlots * kHalves * 2 * kQBytes + 2 * kStages * kKvBytes + kInfo * kGroups * 16 + kRows * 8 +
                                     kItems * sizeof(TreeItem) + 4 + kQSlots * kHalves * kRows + kBarriers * 8 + 8;
     static_assert(sizeof(TreeItem) * kItems % 8 == 4, "the barriers' alignment");
     static_assert(kRows * D * 4 <= 2 * kQBytes, "a half's output goes through the place of its rows");
     static_assert(kSmem <= 227 * 1024, "a block a SM");
     static_assert(2 * kKeys + kOutCols <= kHalfCols, "the halves share the SM's 512 TMEM columns");
-    static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs + kRowsRegs <= 5 * kLaunchRegs, "the split of what the launch gives each scheduler");
+    static_assert(2 * kSoftmaxRegs + kConvertRegs + kOtherRegs <= 4 * kLaunchRegs, "the split of what the launch gives each scheduler");
 };
 
 template <int D>
@@ -93,13 +93,12 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
     uint64_t* p_full = s_full + 2 * kHalves;
     uint64_t* o_done = p_full + 2 * kHalves;     // [half]: PV of a unit has completed
     uint64_t* item_done = o_done + kHalves;      // [half]: all the item's MMAs have completed
-    uint64_t* q_full = item_done + kHalves;      // by slot: an item's rows are there
-    uint64_t* q_empty = q_full + C::kQSlots;     // its last scores are computed, its description read (its output written)
+    uint64_t* q_full = item_done + kHalves;      // [slot][half]: an item's rows are there
+    uint64_t* q_empty = q_full + C::kQSlots * kHalves;  // its last scores are computed, its description read (its output written)
     uint64_t* found_full = q_empty + C::kQSlots; // by description: it is there
     uint64_t* joined = found_full + C::kItems;   // the second half has left its results to the first
     uint64_t* taken_over = joined + 1;           // and the first has read m and l
-    uint64_t* wanted = taken_over + 1;           // the next item may be found
-    uint64_t* drained = wanted + 1;              // [half]
+    uint64_t* drained = taken_over + 1;          // [half]
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + kHalves);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kMmaWarp = 12;
@@ -127,13 +126,12 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 mbar_init(&drained[i], 1);
             }
             for (int i = 0; i < C::kQSlots; ++i) {
-                mbar_init(&q_full[i], 4);
+                for (int half = 0; half < kHalves; ++half) mbar_init(&q_full[i * kHalves + half], 4);
                 mbar_init(&q_empty[i], 5 * kHalves);
             }
             for (int i = 0; i < C::kItems; ++i) mbar_init(&found_full[i], 1);
             mbar_init(joined, 4);
             mbar_init(taken_over, 4);
-            mbar_init(wanted, 4);
             fence_barrier_init();
         }
         __syncwarp();
@@ -146,6 +144,112 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
     const uint32_t tmem = *tmem_holder;
     grid_dependency_wait();
     grid_launch_dependents();
+
+    // Lanes of a row: D / 8, eight values each (a rotation pair's quarters).
+    constexpr int kLanes = D / 8;  // 4, 8, 12, 16
+    constexpr int kAtOnce = 32 / kLanes;
+    const int sub = lane / kLanes, part = lane - sub * kLanes;
+    const int pairs = g.rotary >> 1;
+    const bool turned = 4 * part < pairs;
+    const int at = turned ? 4 * part : 2 * pairs + 4 * (part - pairs / 4);
+    const int to = turned ? at + pairs : at + ((D - 2 * pairs) >> 1);
+    // Query rows of an item's half, by `warps` warps of which this is the pw-th.  Loads run two turns
+    // ahead; rotated, scaled by the row's power of two, split, stored swizzled.  (What lies behind the
+    // item's rows is left as it is: every row of S and O is its own.)
+    const auto put_rows = [&](const TreeItem& next, int half_of, uint8_t* q_hi, uint8_t* powers, int pw, int warps) {
+        const int pass = warps * kAtOnce, first = half_of * kRows, turns = (min(kRows, next.rows - first) + pass - 1) / pass;
+        const int step_t = pass / g.group, step_h = pass - step_t * g.group;
+        float4 a, b, cs, sn, a1, b1, cs1, sn1;  // this turn's, the next one's
+        a = b = cs = sn = a1 = b1 = cs1 = sn1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const int r0 = next.first_row + first + pw * kAtOnce + sub;
+        int t = token_of(r0), hq = r0 - t * g.group;  // of the row two turns ahead
+        // Its position is asked for a turn earlier still: the tables' rows depend on it.
+        const auto row_there = [&](int i) { return sub < kAtOnce && i < turns && first + i * pass + pw * kAtOnce + sub < next.rows; };
+        int pos_next = turned && row_there(0) ? load_now(g.positions + (next.row0 + t)) : 0;
+#pragma unroll 2
+        for (int i = -2; i < turns; ++i) {
+            unsigned long long v[4] = {pack2(a.x, a.y), pack2(a.z, a.w), pack2(b.x, b.y), pack2(b.z, b.w)};
+            if (turned) {  // (a product and a sum may be rounded as one)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const unsigned long long x = v[e], y = v[2 + e];
+                    const unsigned long long c2 = e == 0 ? pack2(cs.x, cs.y) : pack2(cs.z, cs.w), s2 = e == 0 ? pack2(sn.x, sn.y) : pack2(sn.z, sn.w);
+                    v[e] = sub2(mul2(x, c2), mul2(y, s2));
+                    v[2 + e] = add2(mul2(y, c2), mul2(x, s2));
+                }
+            }
+            a = a1, b = b1, cs = cs1, sn = sn1;
+            a1 = b1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const int64_t pos_asked = pos_next;
+            const int t_asked = t, hq_asked = hq;
+            t += step_t;
+            hq += step_h;
+            if (hq >= g.group) {
+                hq -= g.group;
+                ++t;
+            }
+            if (turned && row_there(i + 3)) pos_next = load_now(g.positions + (next.row0 + t));
+            if (row_there(i + 2)) {
+                const float* src = g.q + ((int64_t)next.row0 + t_asked) * g.q_stride + (int64_t)(next.head * g.group + hq_asked) * D;
+                a1 = load_now(reinterpret_cast<const float4*>(src + at));
+                b1 = load_now(reinterpret_cast<const float4*>(src + to));
+                if (turned) {
+                    int64_t pos = pos_asked;
+                    if (pos < 0 || pos >= g.table_rows) {
+                        if (part == 0 && pos >= 0) report(watch, kSiteKv8Range);
+                        pos = 0;
+                    }
+                    cs1 = load_now(reinterpret_cast<const float4*>(g.cos_table + pos * pairs + at));
+                    sn1 = load_now(reinterpret_cast<const float4*>(g.sin_table + pos * pairs + at));
+                }
+            }
+            if (i < 0) continue;
+            const int r = i * pass + pw * kAtOnce + sub;
+            // A NaN is no maximum, but it stays one in its row's products.
+            float largest = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 x = unpack2(v[e]);
+                largest = fmaxf(largest, fmaxf(fabsf(x.x), fabsf(x.y)));
+            }
+            if constexpr (kLanes == 12) {
+                float all = 0.0f;
+#pragma unroll
+                for (int e = 0; e < kLanes; ++e) all = fmaxf(all, __shfl_sync(~0u, largest, min(sub * kLanes + e, 31)));
+                largest = all;
+            } else {
+#pragma unroll
+                for (int d = kLanes / 2; d > 0; d >>= 1) largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, d));
+            }
+            float up, down;
+            row_power(__float_as_uint(largest), up, down);
+            if (sub < kAtOnce && r < kRows) {
+                if (part == 0) powers[r] = static_cast<uint8_t>(__float_as_uint(down) >> 23);
+                const unsigned long long up2 = pack2(up, up);
+#pragma unroll
+                for (int quarter = 0; quarter < 2; ++quarter) {
+                    const int d = quarter == 0 ? at : to;
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        // 11 bits (exact in fp16), and what is left.
+                        const unsigned long long x = mul2(v[2 * quarter + e], up2);
+                        const float2 whole = unpack2(x);
+                        const float h0 = __uint_as_float(__float_as_uint(whole.x) & 0xffffe000u);
+                        const float h1 = __uint_as_float(__float_as_uint(whole.y) & 0xffffe000u);
+                        const float2 rest = unpack2(sub2(x, pack2(h0, h1)));
+                        hi[e] = half2_bits(h0, h1);
+                        lo[e] = half2_bits(rest.x, rest.y);
+                    }
+                    const int offset = (d >> 6) * (kRows * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2;
+                    *reinterpret_cast<uint2*>(q_hi + offset) = make_uint2(hi[0], hi[1]);
+                    *reinterpret_cast<uint2*>(q_hi + C::kQBytes + offset) = make_uint2(lo[0], lo[1]);
+                }
+            }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+    };
 
     // Units are counted on over the items, by half (n); barriers of per-unit and per-item
     // phases are waited for in order by every role.
@@ -164,15 +268,25 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         for (int it = 0;; ++it) {
             const int q_slot = it % C::kQSlots;
             const TreeItem* item = items + it % C::kItems;
-            ok = ok && __all_sync(~0u, tile_wait(watch, &q_full[q_slot], it / C::kQSlots & 1));
+            ok = ok && __all_sync(~0u, tile_wait(watch, &found_full[it % C::kItems], it / C::kItems & 1));
             if (!ok) break;
             const bool both = item->both != 0;
+            const int rows_at = q_slot * kHalves + (both ? side : 0);
+            if (item->tiles < 0) break;
+            // The first item's rows, or all where there is no room beside them, are its softmax warps' own work.
+            if (it == 0 || C::kQSlots == 1) {
+                if (it > 0) ok = __all_sync(~0u, tile_wait(watch, q_empty, (it - 1) & 1));
+                if (!ok) break;
+                if (both || side == 0) put_rows(*item, side, q_rows + side * 2 * C::kQBytes, power + side * kRows, warp & 3, 4);
+                if (lane == 0) mbar_arrive(&q_full[side]);
+            }
+            ok = __all_sync(~0u, tile_wait(watch, &q_full[rows_at], it / C::kQSlots & 1));
+            if (!ok) break;
             const int tiles = item->tiles, first_row = item->first_row + (both ? side * kRows : 0);
             const int rows = both ? max(0, min(kRows, item->rows - side * kRows)) : item->rows;
             const int row0 = item->row0, context = item->context, keys = item->keys, head = item->head, tile0 = item->tile0;
             const int count = item->parts, part_index = item->part, place = item->place;
-            const float factor = __uint_as_float(static_cast<uint32_t>(power[(q_slot * kHalves + (both ? side : 0)) * kRows + r]) << 23) * g.scale * kLog2e;
-            if (tiles < 0) break;
+            const float factor = __uint_as_float(static_cast<uint32_t>(power[rows_at * kRows + r]) << 23) * g.scale * kLog2e;
             if (C::kQSlots == 1 && (both || side == 1)) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_empty);
@@ -186,11 +300,16 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             const uint32_t* row_mask = g.masks + (int64_t)(row0 + (r < rows ? t : 0)) * g.mask_words;
             float* out = g.out + ((int64_t)row0 + t) * g.heads * D + (int64_t)(head * g.group + hq) * D;
             float m = -INFINITY, l = 0.0f, m_sum = -INFINITY;
+            const bool idle = (warp & 3) * 32 >= rows;  // none of the warp's rows is the item's
             for (int j = 0; j < units; ++j, ++n) {
                 const int tile = first + step * j;
                 const uint32_t s_tmem = half_tmem + (n & 1) * C::kKeys;
                 ok = __all_sync(~0u, tile_wait(watch, &s_full[2 * side + (n & 1)], (n >> 1) & 1));
                 if (!ok) break;
+                if (idle) {
+                    if (lane == 0) mbar_arrive(&p_full[2 * side + (n & 1)]);
+                    continue;
+                }
                 tcgen05_fence_after();
                 const float4* scales = info + ((first_tile + tile) % C::kInfo) * C::kGroups;
                 const int drafted = (tile0 + tile) * C::kKeys - context;  // the tile's first key among the request's new ones
@@ -314,26 +433,34 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 }
                 if (!ok) break;
                 if (anew && j > 0) {
-                    // Adds O, complete up to the tile before, to the rounded sum.
+                    // Adds O, complete up to the tile before, to the rounded sum, which is asked
+                    // for ahead: local memory of 256 rows is more than L1 holds.
+                    const bool first = j == kSpan;
+                    const auto ask_sum = [&](float4 (&to)[8], int c) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) to[e] = first ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : get_sum(c + e);
+                    };
+                    float4 z[8];
+                    ask_sum(z, 0);
                     ok = __all_sync(~0u, tile_wait(watch, &o_done[side], (n - 1) & 1));
                     if (!ok) break;
                     tcgen05_fence_after();
-                    const bool first = j == kSpan;
                     const float old = first || m_sum == -INFINITY ? 0.0f : ex2(m_sum - m_before);
                     m_sum = m_before;
 #pragma unroll 1
                     for (int c = 0; c < D / 4; c += 8) {
-                        float4 z[8];
+                        float4 ahead[8];
                         uint32_t y[32];
                         tmem_ld_32x32b_x32(o_tmem + lanes + 4 * c, y);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) z[e] = first ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : get_sum(c + e);
+                        if (c + 8 < D / 4) ask_sum(ahead, c + 8);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
+                        for (int e = 0; e < 8; ++e) {
                             put_sum(c + e, make_float4(fmaf(z[e].x, old, __uint_as_float(y[4 * e])), fmaf(z[e].y, old, __uint_as_float(y[4 * e + 1])),
                                                        fmaf(z[e].z, old, __uint_as_float(y[4 * e + 2])),
                                                        fmaf(z[e].w, old, __uint_as_float(y[4 * e + 3]))));
+                            z[e] = ahead[e];
+                        }
                     }
                 }
                 tmem_wait_st();
@@ -353,6 +480,14 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             uint8_t* slot_rows = q_rows + q_slot * kHalves * 2 * C::kQBytes;
             float4* other = reinterpret_cast<float4*>(slot_rows + 2 * C::kQBytes);  // [D / 4][128]: the second side's O, in the place of its rows
             float own_weight = 1.0f, other_weight = 0.0f;
+            if (idle) {  // it has nothing to leave to anyone, but keeps to the others' turns
+                if (!both && side == 1 && shared_items > 0) ok = __all_sync(~0u, tile_wait(watch, taken_over, (shared_items - 1) & 1));
+                if (!ok) break;
+                if (!both && lane == 0) mbar_arrive(side == 1 ? joined : taken_over);
+                if ((C::kQSlots > 1 || (!both && side == 0)) && lane == 0) mbar_arrive(&q_empty[q_slot]);
+                shared_items += !both;
+                continue;
+            }
             if (!both && side == 1) {
                 // (The halves' units do not wait for one another: the first may be an item behind.)
                 if (shared_items > 0) ok = __all_sync(~0u, tile_wait(watch, taken_over, (shared_items - 1) & 1));
@@ -619,8 +754,8 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             if (!ok) break;
             n += tiles;
         }
-    } else if (warp < kMmaWarp + 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kIssueRegs));  // (a warpgroup's four warps, by one instruction)
+    } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));  // (a warpgroup's four warps, by one instruction)
     if (warp < kMmaWarp + kHalves) {
         // ------------------------------------------------------ MMA issue
         // The whole warp keeps the loop, so that addresses stay in uniform registers (REDUX
@@ -639,11 +774,11 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         bool ok = true;
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t q_slot = it % C::kQSlots;
-            if (!wait(&q_full[q_slot], it / C::kQSlots & 1)) break;
+            if (!wait(&found_full[it % C::kItems], it / C::kItems & 1)) break;
             const TreeItem* item = items + it % C::kItems;
             const int tiles = item->tiles;
             const bool both = item->both != 0;
-            if (tiles < 0) break;
+            if (tiles < 0 || !wait(&q_full[q_slot * kHalves + (both ? half : 0)], it / C::kQSlots & 1)) break;
             const int units = both ? tiles : (tiles + 1 - static_cast<int>(half)) / 2;
             const uint32_t q_at = uniform((q_slot * kHalves + (both ? half : 0)) * (2 * C::kQBytes >> 4));
             // The tiles that are the other half's are let go of, in their turn.
@@ -715,14 +850,15 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         }
         commit(&drained[half]);  // whatever was issued has completed before the block ends
         wait(&drained[half], 0);
-    } else if (warp == kMmaWarp + kHalves) {
-        // ------------------------------------------------------- the items
+    } else {
+        // ------------------------------------------ the items and their rows
+        const int pw = warp - kMmaWarp - kHalves;
         const int requests = g.step.requests, heads = g.cache.kv_heads;
         // A request's groups of 256 rows and what is left, its tiles, and its items' units in all.
         struct Cost {
             int full, rest, tiles;
-            __device__ __forceinline__ int64_t of_full() const { return 2 * static_cast<int64_t>(tiles) + kItemCost; }
-            __device__ __forceinline__ int64_t of_rest() const { return rest == 0 ? 0 : (rest > kRows ? 2 : 1) * static_cast<int64_t>(tiles) + kItemCost; }
+            __device__ __forceinline__ int64_t of_full() const { return 2 * static_cast<int64_t>(tiles) + C::kItemCost; }
+            __device__ __forceinline__ int64_t of_rest() const { return rest == 0 ? 0 : (rest > kRows ? 2 : 1) * static_cast<int64_t>(tiles) + C::kItemCost; }
         };
         const auto held_keys = [&](int s) {
             const int held = min(g.step.page_offsets[s + 1] - g.step.page_offsets[s], static_cast<int>(g.step.max_pages));
@@ -813,10 +949,10 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 next.tile0 = 0;
                 next.tiles = tiles;
                 if (tiles <= kShortTiles) {
-                    const int64_t middle = unit + (static_cast<int64_t>(each) * tiles + kItemCost) / 2;
+                    const int64_t middle = unit + (static_cast<int64_t>(each) * tiles + C::kItemCost) / 2;
                     if (middle >= begin && middle < end) break;
                 } else {
-                    const int64_t first = unit + kItemCost;
+                    const int64_t first = unit + C::kItemCost;
                     const auto cut = [&](int64_t at) { return static_cast<int>(max64(0, min64(tiles, (at - first) / each))); };  // (towards zero: of those before, none)
                     const int from = cut(begin), to = cut(end);
                     if (from < to) {
@@ -836,134 +972,31 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 mbar_arrive(&found_full[it % C::kItems]);
             }
             __syncwarp();
-            return next.tiles >= 0;
-        };
-        bool more = advance(0);
-        for (int it = 0; more; ++it) {
-            if (!__all_sync(~0u, tile_wait(watch, wanted, it & 1))) break;
-            more = advance(it + 1);
-        }
-    }
-    } else {
-        // ------------------------------------------------- their query rows
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRowsRegs));
-        const int pw = warp - kMmaWarp - 4;
-        // Lanes of a row: D / 8, eight values each (a rotation pair's quarters).
-        constexpr int kLanes = D / 8;  // 4, 8, 12, 16
-        constexpr int kAtOnce = 32 / kLanes, kPass = 4 * kAtOnce;
-        const int sub = lane / kLanes, part = lane - sub * kLanes;
-        const int half = g.rotary >> 1;
-        const bool turned = 4 * part < half;
-        const int at = turned ? 4 * part : 2 * half + 4 * (part - half / 4);
-        const int to = turned ? at + half : at + ((D - 2 * half) >> 1);
-        // Loads run two turns ahead; rotated, scaled by the row's power of two, split,
-        // stored swizzled.
-        const int step_t = kPass / g.group, step_h = kPass - step_t * g.group;
-        const auto put_rows = [&](const TreeItem& next, uint8_t* q_hi, uint8_t* powers) {
-            const int all_rows = next.both ? kHalves * kRows : kRows, turns = (all_rows + kPass - 1) / kPass;
-            float4 a, b, cs, sn, a1, b1, cs1, sn1;  // this turn's, the next one's
-            a = b = cs = sn = a1 = b1 = cs1 = sn1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const int r0 = next.first_row + pw * kAtOnce + sub;
-            int t = token_of(r0), hq = r0 - t * g.group;  // of the row two turns ahead
-#pragma unroll 1
-            for (int i = -2; i < turns; ++i) {
-                unsigned long long v[4] = {pack2(a.x, a.y), pack2(a.z, a.w), pack2(b.x, b.y), pack2(b.z, b.w)};
-                if (turned) {  // (a product and a sum may be rounded as one)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const unsigned long long x = v[e], y = v[2 + e];
-                        const unsigned long long c2 = e == 0 ? pack2(cs.x, cs.y) : pack2(cs.z, cs.w), s2 = e == 0 ? pack2(sn.x, sn.y) : pack2(sn.z, sn.w);
-                        v[e] = sub2(mul2(x, c2), mul2(y, s2));
-                        v[2 + e] = add2(mul2(y, c2), mul2(x, s2));
-                    }
-                }
-                a = a1, b = b1, cs = cs1, sn = sn1;
-                a1 = b1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (sub < kAtOnce && (i + 2) * kPass + pw * kAtOnce + sub < next.rows) {
-                    const float* src = g.q + ((int64_t)next.row0 + t) * g.q_stride + (int64_t)(next.head * g.group + hq) * D;
-                    a1 = load_now(reinterpret_cast<const float4*>(src + at));
-                    b1 = load_now(reinterpret_cast<const float4*>(src + to));
-                    if (turned) {
-                        int64_t pos = load_now(g.positions + (next.row0 + t));
-                        if (pos < 0 || pos >= g.table_rows) {
-                            if (part == 0 && pos >= 0) report(watch, kSiteKv8Range);
-                            pos = 0;
-                        }
-                        cs1 = load_now(reinterpret_cast<const float4*>(g.cos_table + pos * half + at));
-                        sn1 = load_now(reinterpret_cast<const float4*>(g.sin_table + pos * half + at));
-                    }
-                }
-                t += step_t;
-                hq += step_h;
-                if (hq >= g.group) {
-                    hq -= g.group;
-                    ++t;
-                }
-                if (i < 0) continue;
-                const int r = i * kPass + pw * kAtOnce + sub;
-                // A NaN is no maximum, but it stays one in its row's products.
-                float largest = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 x = unpack2(v[e]);
-                    largest = fmaxf(largest, fmaxf(fabsf(x.x), fabsf(x.y)));
-                }
-                if constexpr (kLanes == 12) {
-                    float all = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < kLanes; ++e) all = fmaxf(all, __shfl_sync(~0u, largest, min(sub * kLanes + e, 31)));
-                    largest = all;
-                } else {
-#pragma unroll
-                    for (int d = kLanes / 2; d > 0; d >>= 1) largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, d));
-                }
-                float up, down;
-                row_power(__float_as_uint(largest), up, down);
-                if (sub < kAtOnce && r < all_rows) {
-                    if (part == 0) powers[r] = static_cast<uint8_t>(__float_as_uint(down) >> 23);
-                    const unsigned long long up2 = pack2(up, up);
-#pragma unroll
-                    for (int quarter = 0; quarter < 2; ++quarter) {
-                        const int d = quarter == 0 ? at : to;
-                        uint32_t hi[2], lo[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            // 11 bits (exact in fp16), and what is left.
-                            const unsigned long long x = mul2(v[2 * quarter + e], up2);
-                            const float2 whole = unpack2(x);
-                            const float h0 = __uint_as_float(__float_as_uint(whole.x) & 0xffffe000u);
-                            const float h1 = __uint_as_float(__float_as_uint(whole.y) & 0xffffe000u);
-                            const float2 rest = unpack2(sub2(x, pack2(h0, h1)));
-                            hi[e] = half2_bits(h0, h1);
-                            lo[e] = half2_bits(rest.x, rest.y);
-                        }
-                        const int offset = (r / kRows) * (2 * C::kQBytes) + (d >> 6) * (kRows * 128) + (r % kRows) * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2;
-                        *reinterpret_cast<uint2*>(q_hi + offset) = make_uint2(hi[0], hi[1]);
-                        *reinterpret_cast<uint2*>(q_hi + C::kQBytes + offset) = make_uint2(lo[0], lo[1]);
-                    }
-                }
-            }
         };
         bool ok = true;
+        if (pw == 0) advance(0);
 #pragma unroll 1
         for (int it = 0;; ++it) {
             const int q_slot = it % C::kQSlots;
             ok = __all_sync(~0u, tile_wait(watch, &found_full[it % C::kItems], it / C::kItems & 1));
             if (!ok) break;
             const TreeItem now = items[it % C::kItems];
+            if (now.tiles < 0) break;
             if (it >= C::kQSlots) ok = __all_sync(~0u, tile_wait(watch, &q_empty[q_slot], (it / C::kQSlots - 1) & 1));
             if (!ok) break;
-            // Who is done with an item's rows is done with its description, kQSlots items on; those
-            // before are read by now.
-            if (now.tiles >= 0) {
-                if (lane == 0) mbar_arrive(wanted);
-                put_rows(now, q_rows + q_slot * kHalves * 2 * C::kQBytes, power + q_slot * kHalves * kRows);
+            // Who is done with the slot's item before is done with its description, and those before it are
+            // read by now.
+            if (pw == 0) advance(it + 1);
+            if (it > 0 && C::kQSlots > 1) {
+#pragma unroll 1
+                for (int half = 0; half < kHalves; ++half) {
+                    const int at_half = q_slot * kHalves + half;
+                    if (now.both || half == 0) put_rows(now, half, q_rows + at_half * 2 * C::kQBytes, power + at_half * kRows, pw, kHalves);
+                    if (lane < 2) mbar_arrive(&q_full[at_half]);
+                }
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full[q_slot]);
-            if (now.tiles < 0) break;
         }
+    }
     }
     __syncwarp();
     tcgen05_fence_before();
