@@ -37,7 +37,7 @@ struct TreeItem {
 // the blocks in even shares.  An item of more than kShortTiles tiles is cut where a share
 // ends, a shorter one goes to the block that has its middle: a join would take longer.  A
 // share is kLeastShare units at least, so that every part of an item has a tile.
-constexpr int kTreeBlocks = 148, kTreePlaces = 2 * kTreeBlocks, kShortTiles = 32, kLeastShare = 32;
+constexpr int kTreeBlocks = 148, kTreePlaces = 2 * kTreeBlocks, kShortTiles = 32, kLeastShare = 8;
 static_assert((kTileCounters + 4 + 2 * kTreeBlocks) * 4 <= kCounterBytes, "two counters for each block");
 static_assert(kTreePlaces % 4 == 0, "the counters are zeroed four at a time");
 
