@@ -763,14 +763,22 @@ int run_split(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl)
 // takes one form: one-token requests beside a prompt's chunk go to the tiles with it,
 // which is right but was not measured.
 //
-// Trees go by the same rule, to a tile form of their own.  Split form and tile form there,
-// us, requests x nodes: 8 heads of 64 with 4 queries each, 700 cached tokens, 4 x 16 14 and
-// 21, 4 x 32 26 and 23, 16 x 16 35 and 23, 16 x 64 122 and 34; with 8,000 tokens 4 x 8 47 and
-// 43, 4 x 32 146 and 48; 64 x 8 69 and 67 (480 and 381), 64 x 4, 16 rows each, 34 and 80.
-// Over 189 such shapes of 64- and 128-wide heads the rule is 5 % above the better form.
+// Trees have a tile form of their own, which cuts long caches into parts: it pays from fewer
+// rows on where the tables have room for kTreeTileKeys keys.  Split form and tile form, us, 8
+// heads of 64 (128) and 32 to 256 rows a head: 2,048 rows in all over 700 tokens 14 and 21 to
+// 27 (26 and 31 to 40), over 1,500 22 and 27 to 38 (45 and 34 to 47), over 3,000 35 and 28 to
+// 33 (75 and 47 to 58), over 5,000 53 and 36 to 47 (116 and 58 to 71); 4,096 rows over 700
+// tokens 26 and 22 (45 and 28 to 36); 32,768 rows over 700 tokens 123 and 34 to 73.  With
+// fewer than 32 rows a head the split form is ahead: 64 requests of 8 rows over 700 tokens 27
+// and 80.
 constexpr int kTileRows = 32;
 bool takes_tiles(int64_t tokens, int64_t max_tokens, int heads, int group) {
     return max_tokens * group >= kTileRows && tokens * heads >= 3584;
+}
+constexpr int64_t kTreeTileKeys = 2048;
+bool tree_takes_tiles(const leafq_kv8_step& step, int page, int heads, int group) {
+    return takes_tiles(step.tokens, step.max_tokens, heads, group) ||
+           (step.max_tokens * group >= kTileRows && step.tokens * heads >= 2048 && step.max_pages * page >= kTreeTileKeys);
 }
 
 // Calls f(integral constant D) for a supported head size.
@@ -838,7 +846,8 @@ int attend(const char* what, void* stream, const float* q, int64_t q_stride, int
     while ((1 << g.shift) < cache->page) ++g.shift;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool pdl = (flags & LEAFQ_FLAG_PDL) != 0;
-    if (takes_tiles(step->tokens, step->max_tokens, heads, g.group))
+    if (masks ? tree_takes_tiles(*step, cache->page, heads, g.group)
+              : takes_tiles(step->tokens, step->max_tokens, heads, g.group))
         return masks ? launch_kv8_tree_tiles(s, g, workspace, pdl) : launch_kv8_tiles(s, g, workspace, pdl);
     return with_dim(cache->dim, [&](auto d) {
         return masks ? run_split<d(), false, true>(s, g, workspace, pdl) : run_split<d(), false, false>(s, g, workspace, pdl);
