@@ -19,6 +19,8 @@ namespace {
 // most 32 more).  A row whose way meets a parent that is none of the rows before it
 // sees nothing.
 constexpr int kNoRow = -2;  // the way ends at a row that is none; -1: at the request's cached tokens
+constexpr int kTreeWords = 8;
+static_assert(kTreeWords == 8, "a sector of 32 bytes, and the swizzle");
 
 struct TreeArgs {
     const int32_t* parents;
@@ -32,7 +34,7 @@ struct TreeArgs {
 
 __global__ void __launch_bounds__(LEAFQ_KV8_TREE_MOST) kv8_tree_kernel(const TreeArgs g) {
     __shared__ int32_t parent_s[LEAFQ_KV8_TREE_MOST], exit_s[LEAFQ_KV8_TREE_MOST];
-    __shared__ uint32_t within_s[LEAFQ_KV8_TREE_MOST];
+    __shared__ uint32_t within_s[LEAFQ_KV8_TREE_MOST], tile_s[LEAFQ_KV8_TREE_MOST * kTreeWords];
     grid_dependency_wait();
     grid_launch_dependents();
     const int s = blockIdx.x, t = threadIdx.x;
@@ -55,24 +57,44 @@ __global__ void __launch_bounds__(LEAFQ_KV8_TREE_MOST) kv8_tree_kernel(const Tre
         exit_s[t] = at;
     }
     __syncthreads();
+    bool rooted = false;
     if (t < n) {
         int depth = __popc(within), up = at;
         while (up >= 0) {
             depth += __popc(within_s[up]);
             up = exit_s[up];
         }
-        const bool rooted = up != kNoRow;
+        rooted = up != kNoRow;
         g.positions[begin + t] = rooted ? g.context[s] + depth - 1 : -1;
-        int32_t* row = g.masks + (begin + t) * g.words;
-        for (int w = g.words - 1; w >= 0; --w) {
-            uint32_t bits = 0;
-            if (w == t >> 5) {
-                bits = within;
-            } else if (at >= 0 && at >> 5 == w) {
-                bits = within_s[at];
-                at = exit_s[at];
+    }
+    if (!rooted) at = -1;
+    if (g.words == 1) {
+        if (t < n) g.masks[begin + t] = static_cast<int32_t>(rooted ? within : 0u);
+    }
+    const int lane = t & 31, row0 = t - lane, rows = min(32, n - row0);
+    uint32_t* tile = tile_s + row0 * kTreeWords;  // word j of lane l at l * 8 + (j ^ (l / 4)): no two lanes in a bank
+    if (rows > 0 && g.words > 1) {
+        for (int w0 = (g.words - 1) / kTreeWords * kTreeWords; w0 >= 0; w0 -= kTreeWords) {
+#pragma unroll
+            for (int j = kTreeWords - 1; j >= 0; --j) {
+                uint32_t bits = 0;
+                if (w0 + j == t >> 5) {
+                    bits = rooted ? within : 0;
+                } else if (at >= 0 && at >> 5 == w0 + j) {
+                    bits = within_s[at];
+                    at = exit_s[at];
+                }
+                tile[lane * kTreeWords + (j ^ lane >> 2)] = bits;
             }
-            row[w] = static_cast<int32_t>(rooted ? bits : 0u);
+            __syncwarp();
+            const int word = w0 + (lane & 7);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int row = 4 * i + (lane >> 3);
+                if (row < rows && word < g.words)
+                    g.masks[(begin + row0 + row) * g.words + word] = static_cast<int32_t>(tile[row * kTreeWords + ((lane & 7) ^ i)]);
+            }
+            __syncwarp();
         }
     }
     // Rows past the bound, or past the last request's.

@@ -201,6 +201,15 @@ def test_tree_attention_long_caches_and_large_trees(cuda_device):
     _Trees(rng, [50], [1024], 64, 1, 1, 32, kind="binary").check()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("context,requests,new", [(2900, 1, 64), (2900, 1, 33), (2100, 4, 16), (1500, 2, 64), (700, 1, 128)])
+def test_tree_attention_few_items(cuda_device, dim, context, requests, new):
+    # 2,048 rows and more, fewer items than blocks: short ones are cut and joined, at 2,048 keys' room too.
+    rng = np.random.default_rng(context + new + dim)
+    _Trees(rng, [context] * requests, [new] * requests, 64, 8, 4, dim, rotary=dim).check()
+    _Trees(rng, [context, 0, 40][:requests + 2], [new, 1, 7], 16, 8, 8, dim, kind="binary").check()
+
+
 @pytest.mark.parametrize("requests", [200, 500])
 def test_tree_attention_many_requests(cuda_device, requests):
     rng = np.random.default_rng(requests)
