@@ -591,7 +591,9 @@ int leafq_kv8_tree_attention(void* stream, const float* q, int64_t q_stride, int
  * has none gives the token -1 and ends the walk.  Negative and NaN draft
  * probabilities count as zero.  A child whose id is outside the vocabulary is
  * passed over (leafq_device_status reports it).  Comparisons of children hold p to
- * about 1e-6 of itself, the sums of a draw 64 bits.  vocab is at most
+ * about 1e-6 of itself, the sums of a draw 64 bits; what rejections leave of p has the
+ * rounding of the whole (about 2^-45 of it), so a p of which they left little has fewer
+ * bits.  vocab is at most
  * LEAFQ_VERIFY_MOST_VOCAB. */
 #define LEAFQ_VERIFY_MOST_VOCAB (1 << 20)
 int leafq_verify_drafts(void* stream, const float* logits, int64_t logits_stride, int64_t vocab, const int32_t* ids,
@@ -601,7 +603,7 @@ int leafq_verify_drafts(void* stream, const float* logits, int64_t logits_stride
                         int32_t* kept, int32_t* next, uint32_t flags);
 
 /* Moves accepted rows together, in the caches of all layers (`caches`, a host
- * array; all of one geometry): for i < min(kept[s], path_width, lengths[s] -
+ * array; all of one geometry, none there twice): for i < min(kept[s], path_width, lengths[s] -
  * context[s]) the codes of the token at context[s] + path[s][i] go to
  * context[s] + i.  path [requests][path_width] has to ascend.  Rows of a page keep
  * their codes; rows from another page may make its scale grow, per kv head:
@@ -611,7 +613,8 @@ int leafq_verify_drafts(void* stream, const float* logits, int64_t logits_stride
  *   moved rows become rint(code * (their page's old scale / scale))
  * with the quotients and products in 64 bits.  What lies behind the kept rows is left
  * undefined.  A request whose path does not ascend, or leads outside its new rows or
- * the pool, is left as it is, and leafq_device_status reports it.  Of the step:
+ * the pool, is left as it is, and leafq_device_status reports it.  The pages from
+ * context on must be held by one request only, as for leafq_kv8_append.  Of the step:
  * context, lengths, table, max_pages and requests. */
 int leafq_kv8_compact(void* stream, const leafq_kv8_cache* caches, int layers, const leafq_kv8_step* step, const int32_t* path,
                       int64_t path_width, const int32_t* kept, uint32_t flags);

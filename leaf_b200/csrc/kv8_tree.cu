@@ -110,7 +110,9 @@ __global__ void __launch_bounds__(LEAFQ_KV8_TREE_MOST) kv8_tree_kernel(const Tre
 // a row never moves to a place that a later one comes from, and whole pages can be
 // done in order: the page's new scale (the largest that its rows from other pages
 // need), the rows that stay rounded to it where it grew, then the moved rows.  A warp
-// does one request and kv head, of the keys or the values of one layer.
+// does one request and kv head, of the keys or the values of one layer; a launch does up
+// to 32 layers.  Bound by the chain path - table - rows - scales, a few round trips: 64 requests, 22
+// layers of 4 heads of 64, 9.0 us; 37 requests, 4 layers of 8 heads of 128, pages of 16, 7.5.
 constexpr int kLayersAtOnce = 32;
 
 struct CompactArgs {
@@ -235,7 +237,7 @@ __global__ void __launch_bounds__(128) kv8_compact_kernel(const CompactArgs g) {
 // to free_pages[taken - upto ... taken - upto + own), below those of the requests
 // before it.  Every block scans all requests, a thread each and a chunk at a time, and
 // the blocks share the chunk's pages (found by a search of the prefix); block 0 writes
-// the requests' outputs.
+// the requests' outputs.  Launch bound: 64 requests 2.9 us, 2,000 (two chunks) 7.3.
 constexpr int kReleaseThreads = 1024;
 
 struct ReleaseArgs {

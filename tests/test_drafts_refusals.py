@@ -138,6 +138,17 @@ def test_python_refuses_what_it_cannot_pass_on():
         lq.Kv8Tree(i(4), i(4, 1))
     with pytest.raises(lq.LeafError, match="there must be a layer"):
         lq.Kv8Layers([])
+    def cache(pools):
+        c = lq.Kv8Cache.__new__(lq.Kv8Cache)
+        c.k, c.v, c.k_scale, c.v_scale = pools
+        c.index, c.pages, c.page, c.kv_heads, c.dim = 0, 2, 16, 1, 32
+        c.desc = lq._lib.Kv8CacheDesc(*(t.data_ptr() for t in pools), 2, 16, 1, 32)
+        return c
+    apart = [[torch.zeros(4) for _ in range(4)] for _ in range(2)]
+    assert len(lq.Kv8Layers([cache(p) for p in apart]).caches) == 2
+    for twice in ([apart[0], apart[0]], [apart[0], [*apart[1][:3], apart[0][0]]]):  # both would be moved at once
+        with pytest.raises(lq.LeafError, match="a cache is there twice"):
+            lq.Kv8Layers([cache(p) for p in twice])
     with pytest.raises(lq.LeafError, match="tree is missing"):
         lq.kv8_tree_attention(torch.zeros(1, 64), None, None, None, 0.125)
     with pytest.raises(lq.LeafError, match="int32 CUDA"):
