@@ -104,9 +104,9 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
     uint64_t* s_full = v_empty + C::kStages;     // [half][S buffer], as p_full
     uint64_t* p_full = s_full + 2 * kHalves;
     uint64_t* o_done = p_full + 2 * kHalves;     // [half]: PV of a unit has completed
-    uint64_t* item_done = o_done + kHalves;      // [half]: all the item's MMAs have completed
+    uint64_t* item_done = o_done + kHalves;      // [half]: all MMAs of an item that gave it units have completed
     uint64_t* q_full = item_done + kHalves;      // [slot][half]: an item's rows are there
-    uint64_t* q_empty = q_full + C::kQSlots * kHalves;  // its last scores are computed, its description read (its output written)
+    uint64_t* q_empty = q_full + C::kQSlots * kHalves;  // its last scores are computed, its description read (its output written), the end before it seen
     uint64_t* found_full = q_empty + C::kQSlots; // by description: it is there
     uint64_t* joined = found_full + C::kItems;   // the second half has left its results to the first
     uint64_t* taken_over = joined + 1;           // and the first has read m and l
@@ -139,7 +139,7 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             }
             for (int i = 0; i < C::kQSlots; ++i) {
                 for (int half = 0; half < kHalves; ++half) mbar_init(&q_full[i * kHalves + half], 4);
-                mbar_init(&q_empty[i], 5 * kHalves);
+                mbar_init(&q_empty[i], 5 * kHalves + 2);
             }
             for (int i = 0; i < C::kItems; ++i) mbar_init(&found_full[i], 1);
             mbar_init(joined, 4);
@@ -276,6 +276,7 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         const auto get_sum = [&](int c) { return load_local(o_local + 16 * c); };  // elements 4 c .. 4 c + 3 of a row
         const auto put_sum = [&](int c, float4 v) { store_local(o_local + 16 * c, v); };
         int n = 0, first_tile = 0, shared_items = 0;  // the half's units, the block's tiles, and the items that shared keys, before
+        int worked = 0;                               // items before of which the half had units
         bool ok = true;
         for (int it = 0;; ++it) {
             const int q_slot = it % C::kQSlots;
@@ -292,7 +293,10 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 if (both || side == 0) put_rows(*item, side, q_rows + side * 2 * C::kQBytes, power + side * kRows, warp & 3, 4);
                 if (lane == 0) mbar_arrive(&q_full[side]);
             }
-            ok = __all_sync(~0u, tile_wait(watch, &q_full[rows_at], it / C::kQSlots & 1));
+            // (A phase is waited for by whoever waits for a later one: the end of the one before would pass for
+            // it.  The second half needs the first's rows in some items only.)
+            ok = __all_sync(~0u, tile_wait(watch, &q_full[q_slot * kHalves], it / C::kQSlots & 1));
+            if (side == 1) ok = ok && __all_sync(~0u, tile_wait(watch, &q_full[q_slot * kHalves + 1], it / C::kQSlots & 1));
             if (!ok) break;
             const int tiles = item->tiles, first_row = item->first_row + (both ? side * kRows : 0);
             const int rows = both ? max(0, min(kRows, item->rows - side * kRows)) : item->rows;
@@ -481,7 +485,9 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 if (lane == 0) mbar_arrive(&p_full[2 * side + (n & 1)]);
             }
             first_tile += tiles;
-            ok = ok && __all_sync(~0u, tile_wait(watch, &item_done[side], it & 1));
+            // (An item of one tile may have none for the second half: a phase for it would end with the
+            // one before, whose end this warp could then miss.)
+            if (units > 0) ok = ok && __all_sync(~0u, tile_wait(watch, &item_done[side], worked++ & 1));
             if (!ok) break;
             tcgen05_fence_after();
             // The rows' output: O (and the rounded sum) over L, zeros for a row that
@@ -790,7 +796,8 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             const TreeItem* item = items + it % C::kItems;
             const int tiles = item->tiles;
             const bool both = item->both != 0;
-            if (tiles < 0 || !wait(&q_full[q_slot * kHalves + (both ? half : 0)], it / C::kQSlots & 1)) break;
+            if (tiles < 0 || !wait(&q_full[q_slot * kHalves], it / C::kQSlots & 1)) break;
+            if (half && !wait(&q_full[q_slot * kHalves + 1], it / C::kQSlots & 1)) break;  // (as the softmax warps)
             const int units = both ? tiles : (tiles + 1 - static_cast<int>(half)) / 2;
             const uint32_t q_at = uniform((q_slot * kHalves + (both ? half : 0)) * (2 * C::kQBytes >> 4));
             // The tiles that are the other half's are let go of, in their turn.
@@ -837,6 +844,8 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 if (ok && !both && half) ok = pass(v_full, v_empty, 2 * i);
                 const uint32_t tile = n + (both ? i : 2 * i + half), stage = uniform(tile % C::kStages), buffer = uniform(count & 1);
                 ok = ok && wait(&v_full[stage], (tile / C::kStages) & 1) && wait(&p_full[2 * half + buffer], (count >> 1) & 1);
+                // (No scores have waited for the unit before an item's last; the next item's wait for the last.)
+                if (ok && i > 0 && i + 1 == units) ok = wait(&o_done[half], (count - 1) & 1);
                 if (!ok) break;
                 tcgen05_fence_after();
                 const uint64_t v = vt + stage * (C::kKvBytes >> 4);
@@ -858,7 +867,7 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             }
             if (units == 0) commit(&q_empty[q_slot]);
             n += tiles;
-            commit(&item_done[half]);
+            if (units > 0) commit(&item_done[half]);
         }
         commit(&drained[half]);  // whatever was issued has completed before the block ends
         wait(&drained[half], 0);
@@ -996,6 +1005,8 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             if (now.tiles < 0) break;
             if (it >= C::kQSlots) ok = __all_sync(~0u, tile_wait(watch, &q_empty[q_slot], (it / C::kQSlots - 1) & 1));
             if (!ok) break;
+            // (Its phases wait for those who wait for them.)
+            if (lane == 0) mbar_arrive(&q_empty[q_slot]);
             // Who is done with the slot's item before is done with its description, and those before it are
             // read by now.
             if (pw == 0) advance(it + 1);

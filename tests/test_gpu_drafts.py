@@ -210,6 +210,23 @@ def test_tree_attention_few_items(cuda_device, dim, context, requests, new):
     _Trees(rng, [context, 0, 40][:requests + 2], [new, 1, 7], 16, 8, 8, dim, kind="binary").check()
 
 
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+def test_tree_attention_items_that_leave_a_half_without_keys(cuda_device, dim):
+    # 264 rows a head: an item of both halves, then one of 8 rows whose only tile the first half has.
+    rng = np.random.default_rng(dim)
+    _Trees(rng, rng.integers(0, 25, 200), [33] * 200, 64, 2, 8, dim, rotary=dim).check()
+    # The same of parts: items of several tiles, cut into shares.
+    _Trees(rng, rng.integers(0, 800, 60), [*rng.integers(1, 34, 59), 33], 16, 1, 16, dim).check()
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("wide", [9, 12, 16])
+def test_tree_attention_items_of_one_half_behind_those_of_both(cuda_device, dim, wide):
+    # Of 144 to 256 rows and one tile, the second half's fewer; then of 96 rows and two, whose keys the halves share.
+    rng = np.random.default_rng(dim + wide)
+    _Trees(rng, [30, 97] * 90, [wide, 6] * 90, 16, 2, 16, dim, rotary=dim).check()
+
+
 @pytest.mark.parametrize("requests", [200, 500])
 def test_tree_attention_many_requests(cuda_device, requests):
     rng = np.random.default_rng(requests)
