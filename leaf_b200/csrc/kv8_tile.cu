@@ -749,11 +749,13 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         };
         // S of tile n, into the buffer that PV of tile n - 2 reads: MMAs of
         // unlike accumulators keep no order, so that one is waited for (an
-        // item's first: PV of tile n - 1, which has been issued before).
-        const auto scores = [&](int n, bool first, int q_at) {
+        // item's first: all of the item before; of o_done, an item's last phase but one may
+        // not have been seen, and would pass for the last).
+        const auto scores = [&](int n, bool first, int q_at, int it) {
             const int stage = n % C::kKStages;
             if (!wait(&k_full[stage], (n / C::kKStages) & 1)) return false;
-            if (n >= (first ? 1 : 2) && !wait(o_done, (first ? n - 1 : n) & 1)) return false;
+            if (first ? it > 0 : n >= 2)
+                if (!wait(first ? item_done : o_done, (first ? it - 1 : n) & 1)) return false;
             tcgen05_fence_after();
             const uint64_t k = kt + stage * (C::kKvBytes >> 4);
             const uint32_t s_tmem = tmem + (n & 1) * C::kKeys;
@@ -780,7 +782,7 @@ kv8_attend_tile_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
 #pragma unroll 1
             for (int j = -1; j < tiles && ok; ++j) {
                 if (j + 1 < tiles) {
-                    ok = scores(n + (j >= 0), j < 0, q_at);
+                    ok = scores(n + (j >= 0), j < 0, q_at, it);
                     if (j + 2 == tiles) commit(&q_empty[q_slot]);
                 }
                 if (j < 0) continue;
