@@ -788,7 +788,7 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
         const auto commit = [&](uint64_t* bar) {
             if (leader) umma_commit(bar);
         };
-        uint32_t n = 0, count = 0;  // tiles of the items before; the half's units whose PV is issued
+        uint32_t n = 0, count = 0, worked = 0;  // tiles of the items before; the half's units whose PV is issued; its items that had some
         bool ok = true;
         for (uint32_t it = 0; ok; ++it) {
             const uint32_t q_slot = it % C::kQSlots;
@@ -810,12 +810,14 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             };
             // S of unit i, into the buffer that PV of the unit before the last one reads: MMAs of
             // unlike accumulators keep no order, so that one is waited for (an item's first:
-            // the last one's, which has been issued before).
+            // all of the item before; of o_done, an item's last phase but one may not have been seen,
+            // and would pass for the last).
             const auto scores = [&](int i) {
                 if (!both && half && !pass(k_full, k_empty, 2 * i)) return false;
                 const uint32_t tile = n + (both ? i : 2 * i + half), stage = uniform(tile % C::kStages), unit = count + (i > 0);
                 if (!wait(&k_full[stage], (tile / C::kStages) & 1)) return false;
-                if (unit >= (i == 0 ? 1 : 2) && !wait(&o_done[half], (i == 0 ? unit - 1 : unit) & 1)) return false;
+                if (i == 0 ? worked > 0 : unit >= 2)
+                    if (!wait(i == 0 ? &item_done[half] : &o_done[half], (i == 0 ? worked - 1 : unit) & 1)) return false;
                 tcgen05_fence_after();
                 const uint64_t q = qh + q_at, k = kt + stage * (C::kKvBytes >> 4);
                 const uint32_t s_tmem = half_tmem + uniform(unit & 1) * C::kKeys;
@@ -844,8 +846,6 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
                 if (ok && !both && half) ok = pass(v_full, v_empty, 2 * i);
                 const uint32_t tile = n + (both ? i : 2 * i + half), stage = uniform(tile % C::kStages), buffer = uniform(count & 1);
                 ok = ok && wait(&v_full[stage], (tile / C::kStages) & 1) && wait(&p_full[2 * half + buffer], (count >> 1) & 1);
-                // (No scores have waited for the unit before an item's last; the next item's wait for the last.)
-                if (ok && i > 0 && i + 1 == units) ok = wait(&o_done[half], (count - 1) & 1);
                 if (!ok) break;
                 tcgen05_fence_after();
                 const uint64_t v = vt + stage * (C::kKvBytes >> 4);
@@ -867,7 +867,10 @@ kv8_attend_tree_kernel(const Kv8AttendArgs g, const DeviceWatch watch, uint32_t*
             }
             if (units == 0) commit(&q_empty[q_slot]);
             n += tiles;
-            if (units > 0) commit(&item_done[half]);
+            if (units > 0) {
+                commit(&item_done[half]);
+                ++worked;
+            }
         }
         commit(&drained[half]);  // whatever was issued has completed before the block ends
         wait(&drained[half], 0);
