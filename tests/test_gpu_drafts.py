@@ -821,6 +821,34 @@ def test_verify_streams_graphs_and_reuse(cuda_device):
     assert _status_ok()
 
 
+def test_calls_of_several_streams_at_once(cuda_device):
+    # Each with its own workspace and outputs: both forms of the attention, causal tiles, and verification.
+    rng = np.random.default_rng(61)
+    batches = [_Trees(rng, [3000, 40], [70, 60], 16, 8, 8, 64, rotary=64), _Trees(rng, [900], [90], 64, 8, 8, 128),
+               _Trees(rng, [100, 40], [5, 9], 16, 2, 4, 64, rotary=64)]
+    trees = [_random_tree(rng, int(n), "near") for n in rng.integers(1, 9, 70)]
+    logits, ids, accept, sample, heat, q = _verify_case(rng, trees, 4099, True)
+    plan, parents = _plan([0] * 70, trees), _i32([p for t in trees for p in t])
+    inputs = [_f32(logits), _i32(ids), parents, plan, _f32(accept), _f32(sample), _f32(heat), _f32(q)]
+    rows = [torch.from_numpy(b.q).cuda() for b in batches]
+    ropes = [_rope_cuda(b.rope) for b in batches]
+    calls = [lambda w, b=b, x=x, r=r: lq.kv8_tree_attention(x, b.cache, b.plan, b.tree, b.scale, rope=r, workspace=w)
+             for b, x, r in zip(batches, rows, ropes)]
+    calls.append(lambda w: lq.kv8_attention(rows[0], batches[0].cache, batches[0].plan, batches[0].scale, rope=ropes[0], workspace=w))
+    calls.append(lambda w: lq.verify_drafts(*inputs).path)
+    expect = [call(lq.Kv8Workspace()) for call in calls]
+    streams, workspaces = [torch.cuda.Stream() for _ in calls], [lq.Kv8Workspace() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[] for _ in calls]
+    for _ in range(12):
+        for out, call, stream, w in zip(got, calls, streams, workspaces):
+            with torch.cuda.stream(stream):
+                out.append(call(w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, e) for out, e in zip(got, expect) for o in out)
+    assert _status_ok()
+
+
 # ------------------------------------------------------------- a run of them
 @pytest.mark.parametrize("page", [16, 64])
 def test_a_step_of_drafts_end_to_end(cuda_device, page):
