@@ -594,7 +594,8 @@ int leafq_kv8_tree_attention(void* stream, const float* q, int64_t q_stride, int
  * about 1e-6 of itself, the sums of a draw 64 bits; what rejections leave of p has the
  * rounding of the whole (about 2^-45 of it), so a p of which they left little has fewer
  * bits.  vocab is at most
- * LEAFQ_VERIFY_MOST_VOCAB. */
+ * LEAFQ_VERIFY_MOST_VOCAB.  Outputs must not overlap one another or the inputs (of
+ * logits and draft_probs, from the first row's begin to the last one's end). */
 #define LEAFQ_VERIFY_MOST_VOCAB (1 << 20)
 int leafq_verify_drafts(void* stream, const float* logits, int64_t logits_stride, int64_t vocab, const int32_t* ids,
                         const int32_t* parents, const int32_t* token_offsets, int requests, int64_t tokens,

@@ -13,16 +13,6 @@
 
 namespace leafq {
 
-// `count` values of a call's argument.
-struct Span {
-    const int32_t* begin;
-    int64_t count;
-    bool overlaps(const Span& other) const {
-        const auto at = reinterpret_cast<uintptr_t>(begin), other_at = reinterpret_cast<uintptr_t>(other.begin);
-        return count > 0 && other.count > 0 && at < other_at + 4 * other.count && other_at < at + 4 * count;
-    }
-};
-
 inline int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1; }
 
 struct Kv8AttendArgs {

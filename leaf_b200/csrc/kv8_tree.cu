@@ -324,17 +324,6 @@ __global__ void __launch_bounds__(kReleaseThreads) kv8_release_kernel(const Rele
     if (writer && tid == 0) *g.taken_after = static_cast<int32_t>(taken - reached_s);
 }
 
-template <size_t kOut, size_t kIn>
-bool apart(const Span (&outputs)[kOut], const Span (&inputs)[kIn]) {
-    for (size_t i = 0; i < kOut; ++i) {
-        for (const Span& in : inputs)
-            if (outputs[i].overlaps(in)) return false;
-        for (size_t j = 0; j < i; ++j)
-            if (outputs[i].overlaps(outputs[j])) return false;
-    }
-    return true;
-}
-
 // The sizes that the step's arrays have.
 bool step_valid(const leafq_kv8_step* step, const char* what) {
     if (!step || step->tokens < 0 || step->tokens > INT_MAX || step->max_tokens < 0 || step->requests < 0 || step->max_pages < 0 ||

@@ -55,6 +55,28 @@ int allow_smem(const void* kernel, size_t bytes, const char* what);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// `count` values of four bytes of a call's argument.
+struct Span {
+    const void* begin;
+    int64_t count;
+    bool overlaps(const Span& other) const {
+        const auto at = reinterpret_cast<uintptr_t>(begin), other_at = reinterpret_cast<uintptr_t>(other.begin);
+        return count > 0 && other.count > 0 && at < other_at + 4 * other.count && other_at < at + 4 * count;
+    }
+};
+
+// Whether no output shares memory with another one or with an input.
+template <size_t kOut, size_t kIn>
+bool apart(const Span (&outputs)[kOut], const Span (&inputs)[kIn]) {
+    for (size_t i = 0; i < kOut; ++i) {
+        for (const Span& in : inputs)
+            if (outputs[i].overlaps(in)) return false;
+        for (size_t j = 0; j < i; ++j)
+            if (outputs[i].overlaps(outputs[j])) return false;
+    }
+    return true;
+}
+
 // ------------------------------------------------ peer-memory all-gather
 // A kernel that ends an N-sharded linear can store its output rows straight
 // into every rank's receive buffer (CUDA IPC mappings over NVLink) as

@@ -659,6 +659,15 @@ extern "C" int leafq_verify_drafts(void* stream, const float* logits, int64_t lo
         set_error("leafq_verify_drafts: null pointer");
         return LEAFQ_ERR_INVALID;
     }
+    // A request's blocks read the inputs while other requests' write.
+    const auto rows_span = [&](const float* rows, int64_t stride) { return Span{rows, tokens > 0 && rows ? (tokens - 1) * stride + vocab : 0}; };
+    const Span inputs[] = {rows_span(logits, logits_stride), rows_span(draft_probs, probs_stride), {ids, tokens}, {parents, tokens},
+                           {token_offsets, int64_t{requests} + 1}, {accept, tokens}, {sample, requests}, {temperature, requests}};
+    const Span outputs[] = {{path, requests * max_tokens}, {tokens_out, requests * max_tokens}, {kept, requests}, {next, requests}};
+    if (!apart(outputs, inputs)) {
+        set_error("leafq_verify_drafts: outputs must not overlap one another or the inputs");
+        return LEAFQ_ERR_INVALID;
+    }
     // Blocks a request: as many as leave a warp 512 values of a row, which it reads at once.  (A
     // batch's longest walk is what it waits for, so many short ones do not call for fewer.)
     int blocks = kMostBlocks;

@@ -57,7 +57,7 @@ def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor
     for drafts that were not drawn.  The token behind the last row is drawn by
     sample from what p then is.  accept [tokens] and sample [requests] are uniform
     in [0, 1); temperature [requests] of 0 is greedy.  ``out``: a verdict of the same
-    sizes, which is filled again."""
+    sizes, which is filled again (its tensors may not be inputs of the call)."""
     index = plan.index
     if _current_device() != index:
         with torch.cuda.device(index):
