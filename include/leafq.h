@@ -604,7 +604,7 @@ int leafq_verify_drafts(void* stream, const float* logits, int64_t logits_stride
                         int32_t* kept, int32_t* next, uint32_t flags);
 
 /* Moves accepted rows together, in the caches of all layers (`caches`, a host
- * array; all of one geometry, none there twice): for i < min(kept[s], path_width, lengths[s] -
+ * array; all of one geometry, no two pools sharing memory): for i < min(kept[s], path_width, lengths[s] -
  * context[s]) the codes of the token at context[s] + path[s][i] go to
  * context[s] + i.  path [requests][path_width] has to ascend.  Rows of a page keep
  * their codes; rows from another page may make its scale grow, per kv head:

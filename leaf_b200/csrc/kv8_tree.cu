@@ -5,6 +5,8 @@
 //   kv8_release_kernel  pages behind a request's new length given back
 #include <algorithm>
 #include <climits>
+#include <memory>
+#include <new>
 
 #include "kv8_attention.cuh"
 
@@ -324,6 +326,35 @@ __global__ void __launch_bounds__(kReleaseThreads) kv8_release_kernel(const Rele
     if (writer && tid == 0) *g.taken_after = static_cast<int32_t>(taken - reached_s);
 }
 
+// Whether no two pools of the layers share memory.
+bool pools_apart(const leafq_kv8_cache* caches, int layers, const char* what) {
+    struct Pool {
+        uintptr_t begin, end;
+    };
+    const size_t count = 4 * static_cast<size_t>(layers);
+    const std::unique_ptr<Pool[]> pools(new (std::nothrow) Pool[count]);
+    if (!pools) {
+        set_error(std::string(what) + ": out of host memory");
+        return false;
+    }
+    for (int i = 0; i < layers; ++i) {
+        const leafq_kv8_cache& c = caches[i];
+        const uintptr_t scales = 4 * static_cast<uintptr_t>(c.pages) * c.kv_heads, codes = scales / 4 * c.page * c.dim;
+        const void* begins[4] = {c.k_codes, c.v_codes, c.k_scales, c.v_scales};
+        for (int j = 0; j < 4; ++j) {
+            const uintptr_t begin = reinterpret_cast<uintptr_t>(begins[j]);
+            pools[4 * i + j] = Pool{begin, begin + (j < 2 ? codes : scales)};
+        }
+    }
+    std::sort(pools.get(), pools.get() + count, [](const Pool& a, const Pool& b) { return a.begin < b.begin; });
+    for (size_t i = 1; i < count; ++i)
+        if (pools[i].begin < pools[i - 1].end) {
+            set_error(std::string(what) + ": a cache is there twice, or has memory of another");
+            return false;
+        }
+    return true;
+}
+
 // The sizes that the step's arrays have.
 bool step_valid(const leafq_kv8_step* step, const char* what) {
     if (!step || step->tokens < 0 || step->tokens > INT_MAX || step->max_tokens < 0 || step->requests < 0 || step->max_pages < 0 ||
@@ -395,6 +426,7 @@ int leafq_kv8_compact(void* stream, const leafq_kv8_cache* caches, int layers, c
         set_error("leafq_kv8_compact: null pointer");
         return LEAFQ_ERR_INVALID;
     }
+    if (!pools_apart(caches, layers, what)) return LEAFQ_ERR_INVALID;
     const leafq_kv8_cache& c = caches[0];
     const int64_t blocks = ((int64_t)step->requests * 2 * c.kv_heads + 3) / 4;
     if (blocks > INT_MAX) {

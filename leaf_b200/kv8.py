@@ -158,8 +158,9 @@ class Kv8Layers:
         first = self.caches[0]
         _need(all((c.index, c.pages, c.page, c.kv_heads, c.dim) == (first.index, first.pages, first.page, first.kv_heads, first.dim)
                   for c in self.caches), "the layers' caches must be on one device and have the same pages, kv heads and head size")
-        pools = [t.data_ptr() for c in self.caches for t in (c.k, c.v, c.k_scale, c.v_scale) if t.numel()]
-        _need(len(set(pools)) == len(pools), "a cache is there twice")
+        pools = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                       for c in self.caches for t in (c.k, c.v, c.k_scale, c.v_scale) if t.numel())
+        _need(all(end <= begin for (_, end), (begin, _) in zip(pools, pools[1:])), "a cache is there twice, or has memory of another")
         self.index, self.page = first.index, first.page
         self.descs = (_lib.Kv8CacheDesc * len(self.caches))(*(c.desc for c in self.caches))
 
