@@ -612,7 +612,8 @@ int leafq_verify_drafts(void* stream, const float* logits, int64_t logits_stride
  *   scale = max(old scale, need)
  *   the request's older rows of the page become rint(code * (old scale / scale))
  *   moved rows become rint(code * (their page's old scale / scale))
- * with the quotients and products in 64 bits.  What lies behind the kept rows is left
+ * with the quotients and products in 64 bits and codes kept within -128 .. 127 (which matters
+ * only for scales below 2^-126, whose rounding is coarse).  What lies behind the kept rows is left
  * undefined.  A request whose path does not ascend, or leads outside its new rows or
  * the pool, is left as it is, and leafq_device_status reports it.  The pages from
  * context on must be held by one request only, as for leafq_kv8_append.  Of the step:

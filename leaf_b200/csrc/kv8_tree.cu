@@ -129,12 +129,20 @@ struct CompactArgs {
     int requests, width, shift, kv_heads;
 };
 
-// Four codes times a ratio that has 64 bits, rounded.
+// What takes codes of one scale to another; zeros where the other is zero or no number.
+__device__ __forceinline__ double ratio_of(float from, float to) {
+    return to > 0.0f ? static_cast<double>(from) / static_cast<double>(to) : 0.0;
+}
+
+// Four codes times a ratio that has 64 bits, rounded.  (They fit eight bits, but for scales below
+// 2^-126: their own rounding is coarse, and may leave them too small.)
 __device__ __forceinline__ uint32_t scale_codes(uint32_t codes, double ratio) {
     uint32_t out = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        out |= (static_cast<uint32_t>(__double2int_rn(static_cast<int8_t>(codes >> (8 * i)) * ratio)) & 0xffu) << (8 * i);
+    for (int i = 0; i < 4; ++i) {
+        const int code = __double2int_rn(static_cast<int8_t>(codes >> (8 * i)) * ratio);
+        out |= (static_cast<uint32_t>(min(max(code, -128), 127)) & 0xffu) << (8 * i);
+    }
     return out;
 }
 
@@ -204,7 +212,7 @@ __global__ void __launch_bounds__(128) kv8_compact_kernel(const CompactArgs g) {
         const float scale = isnan(before) || (!(need > before) && !isnan(need)) ? before : need;
         const bool grown = !same(scale, before);
         if (grown) {
-            const double ratio = static_cast<double>(before) / static_cast<double>(scale);
+            const double ratio = ratio_of(before, scale);
             for (int i = lane; i < row0 * (D / 4); i += 32) {
                 uint32_t* at = reinterpret_cast<uint32_t*>(to) + i;
                 *at = scale_codes(*at, ratio);
@@ -220,7 +228,7 @@ __global__ void __launch_bounds__(128) kv8_compact_kernel(const CompactArgs g) {
                 v = *reinterpret_cast<const uint4*>(codes + ((tile_of(from_id) << g.shift) + (from & (page - 1))) * D + 16 * piece);
                 const float own = from_id == id ? before : scales[tile_of(from_id)];
                 if (!same(own, scale)) {
-                    const double ratio = static_cast<double>(own) / static_cast<double>(scale);
+                    const double ratio = ratio_of(own, scale);
                     v = make_uint4(scale_codes(v.x, ratio), scale_codes(v.y, ratio), scale_codes(v.z, ratio), scale_codes(v.w, ratio));
                 }
             }
