@@ -732,6 +732,7 @@ SplitShape split_shape(int64_t max_tokens, int group) {
 template <int D, bool kNarrow, bool kTree>
 int run_split(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl) {
     using C = Split<D, kNarrow>;
+    const char* what = kTree ? "leafq_kv8_tree_attention" : "leafq_kv8_attention";
     const SplitShape f = split_shape<D, kNarrow>(g.step.max_tokens, g.group);
     // More heads than wide blocks go to narrow ones.  Wide and narrow, us, 64-wide
     // heads: 256 heads of 521 to 765 tokens 13.5 and 20.3, 1,024 heads of 500 to
@@ -740,16 +741,16 @@ int run_split(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl)
     // 500 to 1,500 85 and 76, 2,048 of 200 to 2,000 167 and 138.
     if (!kNarrow && (int64_t)g.step.requests * g.cache.kv_heads > f.ranges) return run_split<D, true, kTree>(s, g, workspace, pdl);
     if (f.ranges * f.row_blocks > INT_MAX / 8) {
-        set_error("leafq_kv8_attention: max_tokens * group is too large");
+        set_error(std::string(what) + ": max_tokens * group is too large");
         return LEAFQ_ERR_INVALID;
     }
     const auto kernel = kv8_attend_split_kernel<D, kNarrow, kTree>;
-    const int st = allow_smem(reinterpret_cast<const void*>(kernel), C::kSmem, "leafq_kv8_attention");
+    const int st = allow_smem(reinterpret_cast<const void*>(kernel), C::kSmem, what);
     if (st) return st;
     uint32_t* arrivals = static_cast<uint32_t*>(workspace);
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
     return launch(kernel, dim3(static_cast<unsigned>(f.ranges * f.row_blocks)), dim3(C::kThreads), C::kSmem, s, pdl,
-                  "leafq_kv8_attention", g, parts, arrivals, static_cast<int>(f.ranges), static_cast<int>(f.row_blocks));
+                  what, g, parts, arrivals, static_cast<int>(f.ranges), static_cast<int>(f.row_blocks));
 }
 
 // The tile form gives 128 rows of a request's kv head to a block, the split form
