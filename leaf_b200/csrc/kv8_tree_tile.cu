@@ -60,7 +60,9 @@ struct TreeShape {
     static constexpr int kStages = D <= 64 ? 4 : 3;      // of K, and of V
     static constexpr int kGroups = kKeys / 16;           // of keys that share a page for certain
     static constexpr int kInfo = 8;                      // ring of the groups' scales: a tile's are read while those of
-                                                         // up to kStages + 2 later tiles are written
+                                                         // up to kStages + 3 later tiles are written (where halves
+                                                         // share the keys: of tile t + 2 the scores are issued then and
+                                                         // t + 3 is passed, so that its stage may be filled again)
     static constexpr int kQBytes = kBlocks * kRows * 128;
     static constexpr int kQSlots = D <= 64 ? 2 : 1;      // of query rows: the next item's beside this one's
     static constexpr int kItems = 3;                     // ring of their descriptions
@@ -80,6 +82,7 @@ struct TreeShape {
     static_assert(sizeof(TreeItem) * kItems % 8 == 4, "the barriers' alignment");
     static_assert(kRows * D * 4 <= 2 * kQBytes, "a half's output goes through the place of its rows");
     static_assert(kSmem <= 227 * 1024, "a block a SM");
+    static_assert(kInfo >= kStages + 4, "no scales are written over that are still read");
     static_assert(2 * kKeys + kOutCols <= kHalfCols, "the halves share the SM's 512 TMEM columns");
     static_assert(2 * kSoftmaxRegs + kConvertRegs + kOtherRegs <= 4 * kLaunchRegs, "the split of what the launch gives each scheduler");
 };
