@@ -590,10 +590,12 @@ int leafq_kv8_tree_attention(void* stream, const float* q, int64_t q_stride, int
  * -inf and NaN logits have no probability, +inf ones share all of it; a row that
  * has none gives the token -1 and ends the walk.  Negative and NaN draft
  * probabilities count as zero.  A child whose id is outside the vocabulary is
- * passed over (leafq_device_status reports it).  Comparisons of children hold p to
- * about 1e-6 of itself, the sums of a draw 64 bits; what rejections leave of p has the
- * rounding of the whole (about 2^-45 of it), so a p of which they left little has fewer
- * bits.  vocab is at most
+ * passed over (leafq_device_status reports it).  A comparison of a row's first child
+ * holds p to within 2^-17 of itself for vocabularies up to 2^17 and 2^-15.9 for 2^20, all
+ * roundings of its 32-bit sum added up (temperatures of 1e-30 and more, logits less than
+ * 3.4e38 apart); further children's, of draft_probs, and the draw have sums of 64 bits.  What
+ * rejections leave of p has the rounding of the whole (about 2^-45 of it), so a p of which
+ * they left little has fewer bits.  vocab is at most
  * LEAFQ_VERIFY_MOST_VOCAB.  Outputs must not overlap one another or the inputs (of
  * logits and draft_probs, from the first row's begin to the last one's end). */
 #define LEAFQ_VERIFY_MOST_VOCAB (1 << 20)

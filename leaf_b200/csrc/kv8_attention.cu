@@ -771,7 +771,9 @@ int run_split(cudaStream_t s, const Kv8AttendArgs& g, void* workspace, bool pdl)
 // 33 (75 and 47 to 58), over 5,000 53 and 36 to 47 (116 and 58 to 71); 4,096 rows over 700
 // tokens 26 and 22 (45 and 28 to 36); 32,768 rows over 700 tokens 123 and 34 to 73.  With
 // fewer than 32 rows a head the split form is ahead: 64 requests of 8 rows over 700 tokens 27
-// and 80.
+// and 80.  The lengths are on the device: the tables' room stands for them, which in the shapes
+// measured was no more than the requests held.  Steps of 2,048 to 3,583 rows over short caches take
+// tiles where the tables are wide: 21 to 27 us of 14, 31 to 40 of 26, by the figures above.
 constexpr int kTileRows = 32;
 bool takes_tiles(int64_t tokens, int64_t max_tokens, int heads, int group) {
     return max_tokens * group >= kTileRows && tokens * heads >= 3584;

@@ -113,8 +113,11 @@ __global__ void __launch_bounds__(LEAFQ_KV8_TREE_MOST) kv8_tree_kernel(const Tre
 // done in order: the page's new scale (the largest that its rows from other pages
 // need), the rows that stay rounded to it where it grew, then the moved rows.  A warp
 // does one request and kv head, of the keys or the values of one layer; a launch does up
-// to 32 layers.  Bound by the chain path - table - rows - scales, a few round trips: 64 requests, 22
-// layers of 4 heads of 64, 9.0 us; 37 requests, 4 layers of 8 heads of 128, pages of 16, 7.5.
+// to 32 layers.  Bound by the chain path - table - rows - scales, a few round trips, and where a scale
+// grows by the page's older rows, which a warp rounds 128 codes at a time, one after another: 64
+// requests, 22 layers of 4 heads of 64, pages of 64, 30 us (12 to 14 of a layer's 344 key scales grow)
+// and 9 to 10 where none does, as in caches that were compacted so before; 37 requests, 4 layers of 8
+// heads of 128, pages of 16, 18 us and 7.5.
 constexpr int kLayersAtOnce = 32;
 
 struct CompactArgs {

@@ -27,11 +27,13 @@ namespace {
 // Bound, 128-wide heads: the hand-offs S - softmax - P - PV of a half, of which the other half's
 // fill a part (5 requests of 12 to 18 thousand cached tokens: tensor pipe busy 45 %, issue slots
 // 38 %).  6 requests of 9 to 100 thousand cached tokens, trees of 40, 64 / 8 heads: 1,202 us,
-// 0.99 PFLOP of MMAs (fp32 operands are two halves) at 825 TFLOP/s; 128 rows a block and two
-// blocks a SM took 1,771.  64-wide heads: the softmax's issue slots, 1.5 to 2.5 us a tile of 96
+// 0.99 PFLOP of MMAs (fp32 operands are two halves) at 825 TFLOP/s, calls back to back in a graph for
+// some milliseconds; for two seconds without a rest 1,327 us, in a graph or not, the power limit
+// holding the clock at 1.7 GHz.  128 rows a block and two blocks a SM took 1,771.  64-wide heads: the softmax's issue slots, 1.5 to 2.5 us a tile of 96
 // keys for 256 rows, and for short caches 6 us for a block's first rows and 2 to 3 for an item's
 // output: 64 trees of 26 over 512 to 767 tokens, 32 / 4 heads, 74 us, in 256 items on 148 blocks
-// (all cut into even shares 90; two blocks a SM of 128 rows 60, the price of the long caches).
+// (all cut into even shares 90; kv8_tile.cu's shape, two blocks a SM of 128 rows, 60: that form of
+// trees was given up for this one, which is the better one for long caches).
 constexpr int kRows = 128, kHalves = 2;
 
 // What the roles need to know of an item: up to 256 query rows of one kv head of a request,

@@ -16,18 +16,23 @@
 // A cluster of blocks walks one request, each warp on its part of the vocabulary, and
 // reads only the rows that the walk comes to.  The decisions are made by every warp for
 // itself, from the same numbers in the same order: the warps exchange sums through the
-// blocks' shared memory, one barrier of the cluster each.  A comparison of one child needs the
-// softmax's sum to about 2^-21 (32-bit exponentials and sums of them); a draw compares with a sum
-// over the vocabulary, where each of its tokens has a border, and takes one pass over its row with
-// 64 bits.  (All rows' sums in 64 bits, which saves that pass, took 113 us instead of 105 for 200
+// blocks' shared memory, one barrier of the cluster each.  A comparison of a row's first child
+// takes the softmax's sum from 32-bit exponentials: with u = 2^-24, of the exponent 3.25 u times its
+// mean under p (at most the logarithm of the vocabulary), of ex2 4 u, 5 u for every rescaling, u for
+// every addition, at most 92 u = 2^-17.5 up to 2^17 tokens and 267 u = 2^-15.9 for 2^20 (temperatures
+// from 1e-30 on, differences of logits below 3.4e38).  What follows a rejection, and a draw, which has
+// a border at each token, compare with a sum over the vocabulary in 64 bits, one more pass over the row.  (All rows' sums in 64 bits, which saves that pass, took 113 us instead of 105 for 200
 // requests over 100,003 tokens: some 45 instructions a value against 8.)
 //
 // Bound: the walk, whose rows and rejections depend on one another.  One chain of 5 rows of
-// 32,000: 18 us, latency of one pass over all rows and one of the last in 64 bits.  64 trees of 26
-// rows with probabilities: 75 us, every rejected child that another follows being a pass over its
+// 32,000: 18 us, in a trace of clocks of some 30 thousand: 4 until the cluster is there, 6.9 the
+// first pass over all rows, 4.1 their sums' exchange, 5.3 two rows' children, 8.2 the 64-bit sum
+// for the draw, 1.2 the draw.  64 trees of 26 rows with probabilities: 75 us, every rejected child that another follows being a pass over its
 // row and q (of 426 MB 39 are read from memory; issue slots 40 % used, the most frequent stalls
 // are loads, 3.6 warps an issue, and the cluster's barrier, 3.3).  200 ragged requests over
-// 100,003 tokens: 110 us, 1.0 TB/s of the 114 MB that the walks need.
+// 100,003 tokens: 110 us, 1.0 TB/s of the 114 MB that the walks need: latency, of blocks that ask
+// for 256 or 512 of a warp's 1,560 values of a row at a time and work on these before they ask again
+// (a draw's 45 instructions a value are about 24 us at the issue rate).
 #include <algorithm>
 #include <cfloat>
 #include <climits>
